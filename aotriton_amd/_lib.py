@@ -92,7 +92,16 @@ class fa_kernel_config(ctypes.Structure):
                 ('backend_index', ctypes.c_int32), ('head_dim', ctypes.c_int32), ('flags', ctypes.c_int32)]
 
 
-# every symbol include/aotriton_amd/flash.h declares: name -> (restype, argtypes)
+class fa_cache(ctypes.Structure):
+    _fields_ = [('K', fa_tensor4), ('V', fa_tensor4), ('table', fa_tensor2), ('lengths', fa_tensor1)]
+
+
+class fa_tree_params(ctypes.Structure):
+    _fields_ = [('Q', fa_tensor4), ('Out', fa_tensor4), ('L', fa_tensor2), ('cache', fa_cache), ('parents', fa_tensor2),
+                ('Sm_scale', ctypes.c_float), ('max_length', ctypes.c_int32), ('window', ctypes.c_int32), ('sinks', ctypes.c_int32)]
+
+
+# every symbol that include/aotriton_amd/*.h declare: name -> (restype, argtypes)
 P = ctypes.POINTER
 SYMBOLS = {
     'fa_check_gpu': (ctypes.c_int, [ctypes.c_void_p]),
@@ -102,6 +111,16 @@ SYMBOLS = {
     'fa_attn_fwd_key_mask': (ctypes.c_int, [P(fa_fwd_params), ctypes.c_int32, ctypes.c_void_p, P(fa_options),
                                             ctypes.c_void_p]),
     'fa_attn_bwd': (ctypes.c_int, [P(fa_bwd_params), ctypes.c_int32, ctypes.c_void_p, P(fa_options)]),
+    'fa_attn_fwd_sinks': (ctypes.c_int, [P(fa_fwd_params), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                         P(fa_options)]),
+    'fa_attn_bwd_sinks': (ctypes.c_int, [P(fa_bwd_params), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                         P(fa_options), ctypes.c_void_p]),
+    'fa_tree_attn': (ctypes.c_int, [P(fa_tree_params), ctypes.c_void_p, ctypes.c_void_p]),
+    'fa_cache_append': (ctypes.c_int, [P(fa_tensor4), P(fa_tensor4), P(fa_cache), P(fa_tensor1), ctypes.c_void_p]),
+    'fa_cache_copy_pages': (ctypes.c_int, [P(fa_tensor4)] * 2 + [P(fa_tensor1)] * 2 + [ctypes.c_void_p]),
+    'fa_cache_fork': (ctypes.c_int, [P(fa_cache)] + [P(fa_tensor1)] * 4 + [ctypes.c_void_p]),
+    'fa_cache_keep_path': (ctypes.c_int, [P(fa_cache), P(fa_tensor2), P(fa_tensor1), P(fa_tensor1), ctypes.c_void_p]),
+    'fa_cache_free': (ctypes.c_int, [P(fa_tensor2)] + [P(fa_tensor1)] * 4 + [ctypes.c_void_p]),
     'fa_v2_attn_fwd': (ctypes.c_int, [P(fa_tensor4)] * 4 + [ctypes.c_float, P(fa_tensor2), P(fa_tensor4), ctypes.c_float,
                                       P(fa_tensor0), P(fa_tensor0), ctypes.c_int64, P(fa_tensor0), P(fa_tensor0),
                                       P(fa_tensor4), ctypes.c_int32, P(fa_tensor0), ctypes.c_void_p]),

@@ -18,7 +18,8 @@ CSRC = os.path.join(HERE, 'csrc')
 ROOT = os.path.dirname(HERE)
 OBJ = os.path.join(CSRC, 'obj')
 LIB = os.path.join(HERE, 'libaotriton_amd.so')
-HOST_SRC = os.path.join(CSRC, 'torch', 'host.cpp')
+HOST_SRC = [os.path.join(CSRC, 'torch', f) for f in ('host.cpp', 'cache.cpp')]
+HOST_HEADERS = [os.path.join(CSRC, 'torch', 'views.h')] + [os.path.join(ROOT, 'include', 'aotriton_amd', f) for f in ('flash.h', 'cache.h')]
 HOST_LIB = os.path.join(HERE, '_torch_host.so')
 HOST_STAMP = os.path.join(OBJ, '_torch_host.torch')      # the torch version it was built for
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
@@ -49,13 +50,16 @@ EXTRA = {
     'fa_bwd_dqs.hip': ['-Wno-inline-asm'],
     'fa_fwd_d256.hip': ['-Wno-inline-asm'],
     'fa_bwd_dq_d128.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form'],
+    # (the same kernels with sinks)
+    'fa_sinks_dkdv_d128.hip': ['-mllvm', '-amdgpu-sched-strategy=max-ilp'],
+    'fa_sinks_dq_d128.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form'],
 }
 
 # The per-head-dim kernel files are compiled a second time with FA_PADDED = the head dim: the copies that
 # serve head dims rounded up to the compiled one.
-PADDED_RE = re.compile(r'fa_(fwd|fwd_rows|fwd_wide|bwd_dkdv|bwd_dkdv_parts|bwd_dq|bwd_dq_bias|bwd_wide|bwd_pair|bwd_fused)_d(\d+)\.hip$')
+PADDED_RE = re.compile(r'fa_(fwd|fwd_rows|fwd_wide|bwd_dkdv|bwd_dkdv_parts|bwd_dq|bwd_dq_bias|bwd_wide|bwd_pair|bwd_fused|sinks_fwd|sinks_dkdv|sinks_dq|tree)_d(\d+)\.hip$')
 # ... and these a third time with 96 columns, for head dims above 64 and up to 96
-COLS96_RE = re.compile(r'fa_(fwd|fwd_wide|bwd_dkdv|bwd_dq|bwd_wide)_d128\.hip$')
+COLS96_RE = re.compile(r'fa_(fwd|fwd_wide|bwd_dkdv|bwd_dq|bwd_wide|sinks_fwd|sinks_dkdv|sinks_dq)_d128\.hip$')
 
 
 def sources():
@@ -112,7 +116,7 @@ def _host_is_current(torch_version):
     is another with every version)."""
     try:
         built_for = open(HOST_STAMP).read()
-        newest = max(os.path.getmtime(p) for p in [HOST_SRC, os.path.join(ROOT, 'include', 'aotriton_amd', 'flash.h')])
+        newest = max(os.path.getmtime(p) for p in HOST_SRC + HOST_HEADERS)
         return built_for == torch_version and os.path.getmtime(HOST_LIB) >= newest
     except OSError:
         return False
@@ -129,13 +133,13 @@ def build_host(force=False):
     torch_lib = os.path.join(os.path.dirname(torch.__file__), 'lib')
     cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}', f'-DFA_TORCH_VERSION="{torch.__version__}"', '-Wno-deprecated-declarations',
-           *[x for i in includes for x in ('-isystem', i)], HOST_SRC, '-o', HOST_LIB,
+           *[x for i in includes for x in ('-isystem', i)], *HOST_SRC, '-o', HOST_LIB,
            '-L' + HERE, '-laotriton_amd', '-Wl,-rpath,$ORIGIN', '-L' + torch_lib, '-ltorch_python', '-ltorch', '-ltorch_cpu',
            '-ltorch_hip', '-lc10_hip', '-lc10']
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stderr)
-        raise RuntimeError('g++ failed on ' + HOST_SRC)
+        raise RuntimeError('g++ failed on ' + ' '.join(HOST_SRC))
     os.makedirs(OBJ, exist_ok=True)
     with open(HOST_STAMP, 'w') as f:
         f.write(torch.__version__)

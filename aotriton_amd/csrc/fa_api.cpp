@@ -1357,6 +1357,122 @@ int fa_attn_fwd_key_mask(const fa_fwd_params* p, int32_t params_version, void* h
   return attn_fwd_impl(&q, params_version, hip_stream, options, alloc, true);
 }
 
+// ---- a sliding window and first keys that stay visible ------------------------------------------------------------
+namespace {
+
+// what the kernels with sinks take, beyond the checks that every call goes through
+int check_sinks(const Shape& s, int dtype, int causal_type, int32_t window, int32_t sinks) {
+  if (window < 1 || sinks < 0 || causal_type != FA_CAUSAL_NONE) return FA_ERROR_INVALID_VALUE;
+  if (sinks > FA_MAX_SINKS || s.bias || s.dropout || s.elementwise || !is_16bit(dtype) || s.d > 128) return FA_ERROR_NOT_SUPPORTED;
+  return FA_SUCCESS;
+}
+
+// (the kernels add the window to positions)
+int32_t window_of(int32_t window) { return window < (1 << 30) ? window : 1 << 30; }
+
+// Tiles of 128 rows, two workgroups per CU, instead of 256 and one?  The costs are those of fwd_small_tiles (us per item, and per
+// 64 keys); a tile of 256 rows meets 128 keys more.
+int sinks_half_tiles(const Shape& s, int64_t tokens, int32_t window, int32_t sinks, int num_cu) {
+  const int64_t cus = num_cu >= fa::kNumXcd ? num_cu / fa::kNumXcd : 1, seqs = s.num_seqlens != 0 ? std::abs(s.num_seqlens) : s.batch;
+  const int64_t rows = s.num_seqlens > 0 ? std::max<int64_t>(1, tokens / std::max<int64_t>(1, seqs)) : s.max_sq;
+  auto time = [&](int bm, int per_cu, double a, double b) {
+    const double keys = std::min<int64_t>(s.max_sk, (int64_t)window + bm) + std::min<int64_t>(sinks, 64);
+    const int64_t items = (seqs * s.hq + fa::kNumXcd - 1) / fa::kNumXcd * ((rows + bm - 1) / bm);
+    return (double)((items + per_cu * cus - 1) / (per_cu * cus)) * (a + b * keys / 64);
+  };
+  return s.d > 64 ? (time(128, 2, 7.3, 1.99) < 0.97 * time(256, 1, 6.3, 1.74) ? 2 : 0)
+                  : (time(128, 2, 4.54, 1.27) < 0.97 * time(256, 1, 4.35, 1.12) ? 2 : 0);
+}
+
+}  // namespace
+
+int fa_attn_fwd_sinks(const fa_fwd_params* p, int32_t params_version, int32_t window, int32_t sinks, void* hip_stream,
+                      const fa_options* options) {
+  Shape s{};
+  int e = validate_fwd(p, params_version, options, &s);
+  if (e != FA_SUCCESS) return e;
+  if ((e = check_sinks(s, p->Q.dtype, p->causal_type, window, sinks)) != FA_SUCCESS) return e;
+  if (p->encoded_softmax.ptr != nullptr) return FA_ERROR_NOT_SUPPORTED;
+  hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+  const DeviceInfo* dev = device_of_stream(stream);
+  if (dev == nullptr || !dev->is_gfx950) return FA_ERROR_NO_BINARY_FOR_GPU;
+  fa::FwdArgs a{};
+  a.q = p->Q.ptr; a.k = p->K.ptr; a.v = p->V.ptr;
+  a.out = p->Out.ptr;
+  a.lse = static_cast<float*>(p->L.ptr);
+  a.sq = strides3(p->Q); a.sk = strides3(p->K); a.sv = strides3(p->V); a.so = strides3(p->Out);
+  a.batch = s.batch; a.hq = s.hq; a.hk = s.hk; a.head_dim = s.d_qk; a.head_dim_v = s.d_v;
+  a.sm_scale = p->Sm_scale;
+  a.seq = seq_args(s, p->cu_seqlens_q, p->cu_seqlens_k, p->seq_strides_q, p->seq_strides_k, p->varlen_type);
+  a.num_cu = dev->num_cu;
+  a.window = window_of(window);
+  a.sinks = sinks;
+  if (s.max_sq > 0 && s.batch > 0) a.half_tiles = sinks_half_tiles(s, (int64_t)p->Q.sizes[2], a.window, sinks, dev->num_cu);
+  FA_LOG(4, "attn_fwd_sinks: D=%d window=%d sinks=%d nseq=%d half_tiles=%d", s.d, a.window, sinks, s.num_seqlens, a.half_tiles);
+  return (int)fa::run_sinks_fwd(p->Q.dtype, s.d, a, stream);
+}
+
+int fa_attn_bwd_sinks(const fa_bwd_params* p, int32_t params_version, int32_t window, int32_t sinks, void* hip_stream,
+                      const fa_options* options, fa_allocator* alloc) {
+  Shape s{};
+  int e = validate_bwd(p, params_version, options, &s, nullptr);
+  if (e != FA_SUCCESS) return e;
+  if ((e = check_sinks(s, p->Q.dtype, p->causal_type, window, sinks)) != FA_SUCCESS) return e;
+  if (bwd_backend(p, options) != 0) return FA_ERROR_PEER_ACCESS_UNSUPPORTED;      // (no single-launch kernel)
+  hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+  const DeviceInfo* dev = device_of_stream(stream);
+  if (dev == nullptr || !dev->is_gfx950) return FA_ERROR_NO_BINARY_FOR_GPU;
+  fa::BwdArgs a{};
+  a.q = p->Q.ptr; a.k = p->K.ptr; a.v = p->V.ptr;
+  a.out = p->Out.ptr; a.dout = p->DO.ptr;
+  a.dq = p->DQ.ptr; a.dk = p->DK.ptr; a.dv = p->DV.ptr;
+  a.lse = static_cast<const float*>(p->L.ptr);
+  a.sq = strides3(p->Q); a.sk = strides3(p->K); a.sv = strides3(p->V); a.so = strides3(p->Out);
+  a.sdo = strides3(p->DO); a.sdq = strides3(p->DQ); a.sdk = strides3(p->DK); a.sdv = strides3(p->DV);
+  a.batch = s.batch; a.hq = s.hq; a.hk = s.hk; a.head_dim = s.d_qk; a.head_dim_v = s.d_v;
+  a.sm_scale = p->Sm_scale;
+  a.seq = seq_args(s, p->cu_seqlens_q, p->cu_seqlens_k, p->seq_strides_q, p->seq_strides_k, p->varlen_type);
+  a.num_cu = dev->num_cu;
+  a.window = window_of(window);
+  a.sinks = std::min(sinks, s.max_sk);
+
+  // The parts of the sinks' sums: workgroups for the chip twice over, of eight steps at least.
+  const int64_t seqs = s.num_seqlens != 0 ? std::abs(s.num_seqlens) : s.batch, blocks = (a.sinks + 31) / 32;
+  const int64_t items = seqs * s.hk * blocks, steps = (int64_t)(s.hq / s.hk) * ((s.max_sq + 31) / 32);
+  a.sink_parts = (int32_t)std::max<int64_t>(1, items > 0 ? std::min<int64_t>(2 * dev->num_cu / items, steps / 8) : 1);
+  const size_t bytes = (size_t)items * a.sink_parts * 2 * 32 * s.d * sizeof(float);
+  bool held = false;
+  if (bytes > 0) {
+    void* sums = nullptr;
+    if (alloc != nullptr) {
+      sums = alloc->alloc(alloc, (uint64_t)bytes);
+    } else if (!stream_is_capturing(stream) && (int64_t)bytes <= ws_limit_bytes(device_index(dev))) {
+      held = ws_acquire(device_index(dev), bytes, stream, &sums) == hipSuccess;
+      if (!held) sums = nullptr;
+    }
+    if (sums == nullptr) return FA_ERROR_OUT_OF_MEMORY;
+    a.sink_ws = static_cast<float*>(sums);
+  }
+  fa_lazy_tensor2* lazy = const_cast<fa_lazy_tensor2*>(&p->D);
+  fa_tensor2 delta = p->D.eager;
+  bool acquired = false;
+  int rc = FA_SUCCESS;
+  if (delta.ptr == nullptr) {
+    const bool no_query = p->Q.sizes[0] == 0 || p->Q.sizes[2] == 0;
+    acquired = lazy->acquire(lazy, &delta) == 0;
+    if (!acquired || (delta.ptr == nullptr && !no_query) ||
+        (delta.ptr != nullptr && check_row_stats(delta, s.row_stats) != FA_SUCCESS))
+      rc = FA_ERROR_INVALID_VALUE;
+  }
+  a.delta = static_cast<float*>(delta.ptr);
+  FA_LOG(4, "attn_bwd_sinks: D=%d window=%d sinks=%d nseq=%d parts=%d", s.d, a.window, a.sinks, s.num_seqlens, a.sink_parts);
+  if (rc == FA_SUCCESS) rc = (int)fa::run_sinks_dq(p->Q.dtype, s.d, a, stream);      // (and delta, which the others read)
+  if (rc == FA_SUCCESS) rc = (int)fa::run_sinks_dkdv(p->Q.dtype, s.d, a, stream);
+  if (held) ws_release(device_index(dev), stream);
+  if (acquired && lazy->dispose != nullptr) lazy->dispose(lazy);
+  return rc;
+}
+
 // kernel_slot < 0: the whole backward of the chosen backend; otherwise only that
 // kernel (0 delta, 1 dK/dV, 2 dQ, 3 fused; 4-6 the three kernels of the backward that keeps dS).
 // own_delta: the split backend with delta in the library's own per-device array (params->D is

@@ -163,6 +163,8 @@ struct FwdArgs {
   float* part_o;         // columns: the compiled head dim
   float* part_ml;        // reference maximum (units of the scores) and row sum
   int32_t key_mask;      // the bias is one byte per key, the same for all rows (sb_m = 0): 0 hides the key
+  // kernels with kSinks: a query sees `window` keys up to its own position (aligned_window), and of those before them the first `sinks`
+  int32_t window, sinks;
 };
 
 struct BwdArgs {
@@ -200,6 +202,9 @@ struct BwdArgs {
   // (sequence and kv-head, key tile, part, dK then dV, key, column), where a second kernel adds them up
   int32_t part_heads, part_tiles;
   float* part_ws;            // null: not cut
+  // kernels with kSinks: as in FwdArgs; dK and dV of the first keys come from fp32 sums over sink_parts parts of the queries (fa_sinks.h)
+  int32_t window, sinks, sink_parts;
+  float* sink_ws;
 };
 
 // Copy between a rank-4 tensor of any strides and head dim (unit last stride) and its packed

@@ -172,7 +172,7 @@ __device__ __forceinline__ uint32_t dropout_append4(const DropoutState& s, int m
 // 15 of which are the forward's).  Keep bits in one word: 78 of 1031 instructions a tile less at D = 96, cross attention 1000 x 1531
 // D80 315 -> 303 us.
 template <typename T, int D, int NW, int BM, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kStoreDs = false,
-          bool kParts = false, int kForm = kBiasAny>
+          bool kParts = false, int kForm = kBiasAny, bool kSinks = false>
 __device__ __forceinline__ void dkdv_item(const BwdArgs& a, const int hk, const int nt, const int z, const int part,
                                           char* smem_raw) {
   using Tr = Traits<T>;
@@ -198,7 +198,8 @@ __device__ __forceinline__ void dkdv_item(const BwdArgs& a, const int hk, const 
   if (n0 >= si.seqlen_k) return;
 
   Window w{0, 0};
-  if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right,
+  if (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);      // (dK and dV of the first keys: fa_sinks.h)
+  else if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right,
                                   si.seqlen_q, si.seqlen_k);
   w.left = w.left > (1 << 30) ? (1 << 30) : (w.left < -(1 << 30) ? -(1 << 30) : w.left);
   w.right = w.right > (1 << 30) ? (1 << 30) : (w.right < -(1 << 30) ? -(1 << 30) : w.right);
@@ -897,7 +898,7 @@ __device__ __forceinline__ void dkdv_item(const BwdArgs& a, const int hk, const 
 // load anyway (dO) and their O rows, instead of being read.  kStoreDelta: it is also written out:
 // the split backward has no preprocess launch, the dK/dV kernel runs after this one and reads it.
 template <typename T, int D, int NW, int BN, bool kWindowed, bool kBias, bool kDropout, bool kInlineDelta, int kPad,
-          bool kStoreDelta = false>
+          bool kStoreDelta = false, bool kSinks = false>
 __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int mt, const int z,
                                         char* smem_raw) {
   using Tr = Traits<T>;
@@ -921,7 +922,8 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
   if (q0 >= si.seqlen_q) return;
 
   Window w{0, 0};
-  if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right,
+  if (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);
+  else if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right,
                                   si.seqlen_q, si.seqlen_k);
   w.left = w.left > (1 << 30) ? (1 << 30) : (w.left < -(1 << 30) ? -(1 << 30) : w.left);
   w.right = w.right > (1 << 30) ? (1 << 30) : (w.right < -(1 << 30) ? -(1 << 30) : w.right);
@@ -940,6 +942,10 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
   }
   const bool m_none = m_hi < m_lo;
   const unsigned m_rng = m_none ? 0u : (unsigned)(m_hi - m_lo);
+  // kSinks, as in fwd_item: tiles before the window's first, in which only sinks are visible; where the row's sinks end
+  static_assert(!kSinks || (kWindowed && !kBias && !kDropout), "a window with sinks and nothing else");
+  const int front = kSinks ? (a.sinks < br.lo * BN ? (a.sinks + BN - 1) / BN : br.lo) : 0;
+  const int m_sink = a.sinks < m_hi + 1 ? a.sinks : m_hi + 1;
 
   T* dqptr = reinterpret_cast<T*>(a.dq) + (int64_t)si.batch_index * a.sdq.z + (int64_t)h * a.sdq.h +
              (int64_t)(si.q_start + row_c) * a.sdq.s;
@@ -1143,10 +1149,11 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
   // lane constants of the two LDS access patterns
   const int row_a = Swz<D>::row_base(lane), tr_a0 = Swz<D>::tr_base(lane, 0), tr_a1 = Swz<D>::tr_base(lane, 1);
 
-  const T* kt = kbase + (int64_t)br.lo * BN * a.sk.s;
-  const T* vt = vbase + (int64_t)br.lo * BN * a.sv.s;
+  const T* kt = kbase + (front > 0 ? 0 : (int64_t)br.lo * BN * a.sk.s);
+  const T* vt = vbase + (front > 0 ? 0 : (int64_t)br.lo * BN * a.sv.s);
   const int64_t k_step = (int64_t)BN * a.sk.s, v_step = (int64_t)BN * a.sv.s;
-  int rows_left = si.seqlen_k - br.lo * BN;      // > 0
+  int rows_left = si.seqlen_k - (front > 0 ? 0 : br.lo * BN);      // > 0
+  int front_left = front;
   __amdgpu_buffer_rsrc_t k_rs, v_rs;
   // tiles are fetched in ascending order; `live` false: nothing is fetched
   auto fetch_begin = [&](bool live) {
@@ -1156,6 +1163,9 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
     k_rs = wave_rsrc(kt, any ? ((rows - 1) * (int)a.sk.s + d_qk) * 2 : 0);
     v_rs = wave_rsrc(vt, any ? ((rows - 1) * (int)a.sv.s + d_v) * 2 : 0);
     if (live) { kt += k_step; vt += v_step; rows_left -= BN; }
+    if (kSinks && live && --front_left == 0) {
+      kt += (br.lo - front) * k_step; vt += (br.lo - front) * v_step; rows_left -= (br.lo - front) * BN;
+    }
   };
   constexpr int FETCH_PIECES = 2 * CH;
   auto fetch_piece = [&](int i) {        // K pieces first, then V
@@ -1289,7 +1299,7 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
       }
       if (masked) {
         // one unsigned comparison of n - m_lo against the length of the visible range
-        const bool vis = m_d + (unsigned)(32 * mb + 8 * g + r) <= m_rng;
+        const bool vis = m_d + (unsigned)(32 * mb + 8 * g + r) <= m_rng || (kSinks && n < m_sink);
         x = vis ? x : -__builtin_inff();
       }
       s[mb][i] = fast_exp2(x);
@@ -1388,12 +1398,13 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
   __syncthreads();
   // K tiles come as [masked | full | masked]; one straight-line loop per run
   {
-    int j = br.lo;
+    int j = front > 0 ? 0 : br.lo, t = 0;
     auto step = [&](auto masked_tag, auto fast_tag) __attribute__((always_inline)) {
-      const int stage = (j - br.lo) & 1;
+      const int stage = (kSinks ? t : j - br.lo) & 1;
       compute(masked_tag, fast_tag, j, stage, j < br.hi);
       __syncthreads();
-      ++j;
+      j = kSinks && j + 1 == front ? br.lo : j + 1;
+      ++t;
     };
     const int full_lo = br.fb_lo <= br.fb_hi ? br.fb_lo : br.hi + 1;
     const int full_hi = br.fb_lo <= br.fb_hi ? br.fb_hi : br.hi;
@@ -1440,7 +1451,7 @@ __host__ __device__ inline bool dkdv_level_list(const BwdArgs& a) {
 }
 
 template <typename T, int D, int NW, int BM, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kStoreDs = false,
-          bool kParts = false, int kForm = kBiasAny>
+          bool kParts = false, int kForm = kBiasAny, bool kSinks = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(NW * 64, NW * 64)))
 __attribute__((amdgpu_waves_per_eu(kTwoDkDv<D, kBias, kDropout, kStoreDs, kForm> ? 2 : 1, kTwoDkDv<D, kBias, kDropout, kStoreDs, kForm> ? 2 : 1)))
 void bwd_dkdv_kernel(const BwdArgs a) {
@@ -1482,12 +1493,12 @@ void bwd_dkdv_kernel(const BwdArgs a) {
     }
     int z, hk;
     split_zh(zh, a.num_zh / a.hk, 1, z, hk);
-    dkdv_item<T, D, NW, BM, kWindowed, kBias, kDropout, kPad, kStoreDs, kParts, kForm>(a, hk, nt, z, kParts ? lp % parts : 0, smem_raw);
+    dkdv_item<T, D, NW, BM, kWindowed, kBias, kDropout, kPad, kStoreDs, kParts, kForm, kSinks>(a, hk, nt, z, kParts ? lp % parts : 0, smem_raw);
     __syncthreads();     // the next item reuses the LDS stages
   }
 }
 
-template <typename T, int D, int NW, int BN, bool kWindowed, bool kBias, bool kDropout, int kPad>
+template <typename T, int D, int NW, int BN, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kSinks = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(NW * 64, NW * 64))) __attribute__((amdgpu_waves_per_eu(kTwoWaves<D, kBias> ? 2 : 1, kTwoWaves<D, kBias> ? 2 : 1)))
 void bwd_dq_kernel(const BwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
@@ -1506,7 +1517,7 @@ void bwd_dq_kernel(const BwdArgs a) {
     const int mt = a.num_m_tiles - 1 - gr / a.zh_group;
     int z, h;
     split_zh(zh, a.num_zh / a.hq, a.hq / a.hk, z, h);
-    dq_item<T, D, NW, BN, kWindowed, kBias, kDropout, true, kPad, true>(a, h, mt, z, smem_raw);
+    dq_item<T, D, NW, BN, kWindowed, kBias, kDropout, true, kPad, true, kSinks>(a, h, mt, z, smem_raw);
     __syncthreads();     // the next item reuses the LDS stages
   }
 }
@@ -1595,7 +1606,7 @@ hipError_t launch_combine_dkdv(const BwdArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T, int D, int kPad, bool W, bool B, bool P, bool kParts, bool kStoreDs, int kForm>
+template <typename T, int D, int kPad, bool W, bool B, bool P, bool kParts, bool kStoreDs, int kForm, bool kSinks = false>
 hipError_t launch_dkdv_form(const BwdArgs& a0, hipStream_t stream) {
   constexpr int NW = BwdTile<T, D, W>::NW, BM = kDkDvBM<T, D, W, B, P, kStoreDs>, BN = NW * 32;
   BwdArgs a = a0;
@@ -1604,7 +1615,7 @@ hipError_t launch_dkdv_form(const BwdArgs& a0, hipStream_t stream) {
   dim3 grid((unsigned)(kNumXcd * bwd_workers(D, B, a.items_per_xcd, a.num_cu, kTwoWaves<D, B> ? 2 : 1)));
   // (the level table's LDS is requested whether or not this launch uses it: the kernel's limit is set once)
   constexpr int smem = DkDvSmem<D, BM>::BYTES + (D < 256 ? kLevelBytes : 0);
-  hipError_t e = launch_with_lds<bwd_dkdv_kernel<T, D, NW, BM, W, B, P, kPad, kStoreDs, kParts, kForm>>(grid, NW * 64, smem, stream, a);
+  hipError_t e = launch_with_lds<bwd_dkdv_kernel<T, D, NW, BM, W, B, P, kPad, kStoreDs, kParts, kForm, kSinks>>(grid, NW * 64, smem, stream, a);
   if constexpr (kParts) {
     if (e == hipSuccess) e = launch_combine_dkdv<T, D>(a, stream);
   }
@@ -1644,7 +1655,7 @@ hipError_t launch_bwd_dkdv(const BwdArgs& a0, bool windowed, bool bias, bool dro
 #undef FA_CALL
 }
 
-template <typename T, int D, int kPad, bool W, bool B, bool P>
+template <typename T, int D, int kPad, bool W, bool B, bool P, bool kSinks = false>
 hipError_t launch_dq_variant(const BwdArgs& a0, hipStream_t stream) {
   using Tile = BwdTile<T, D, W>;
   constexpr int NW = Tile::NW, BN = kDqBN<T, D, W, B>, BM = NW * 32;
@@ -1652,7 +1663,7 @@ hipError_t launch_dq_variant(const BwdArgs& a0, hipStream_t stream) {
   a.num_m_tiles = (a.seq.max_seqlen_q + BM - 1) / BM;
   set_work(a, tile_work(bwd_nseq(a) * a.hq, q_head_group(a.hq, a.hk), a.num_m_tiles));
   dim3 grid((unsigned)(kNumXcd * bwd_workers(D, B, a.items_per_xcd, a.num_cu, kTwoWaves<D, B> ? 2 : 1)));
-  return launch_with_lds<bwd_dq_kernel<T, D, NW, BN, W, B, P, kPad>>(grid, NW * 64, DqSmem<D, BN>::BYTES, stream, a);
+  return launch_with_lds<bwd_dq_kernel<T, D, NW, BN, W, B, P, kPad, kSinks>>(grid, NW * 64, DqSmem<D, BN>::BYTES, stream, a);
 }
 
 template <typename T, int D, int kPad, bool W, bool B, bool P, bool kBuilt>

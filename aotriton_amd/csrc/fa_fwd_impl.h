@@ -41,8 +41,10 @@ struct FwdSmem {
 // One Q tile (BM rows of head h of sequence z) against all its visible K/V tiles, or with kSplit
 // against part `split` of a.splits of them: the fp32 sums and the row statistics of the part then go to
 // scratch memory, where combine_rows_kernel picks them up.
+// kSinks: a window of FwdArgs::window keys up to the query's position and the first FwdArgs::sinks keys.  The item's tiles are then
+// the `front` ones that only the first keys are visible in, and those of the window, as one run of tiles with a jump in it.
 template <typename T, int D, int NW, int BN, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kSplit, bool kKeyBias,
-          bool kAnyRow>
+          bool kAnyRow, bool kSinks>
 __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const int h, const int mt, const int split,
                                          char* smem_raw) {
   using Tr = Traits<T>;
@@ -74,7 +76,8 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
   if (q0 >= si.seqlen_q) return;
 
   Window w{0, 0};
-  if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right,
+  if (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);
+  else if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right,
                                   si.seqlen_q, si.seqlen_k);
   // keep row +/- window inside int32
   w.left = w.left > (1 << 30) ? (1 << 30) : (w.left < -(1 << 30) ? -(1 << 30) : w.left);
@@ -85,6 +88,9 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
     br.lo += split * per;
     if (br.lo + per - 1 < br.hi) br.hi = br.lo + per - 1;
   }
+  // (a key before the window's first tile is no later than the item's first query, so that all its rows see it if it is a sink)
+  static_assert(!kSinks || (kWindowed && !kBias && !kDropout && !kSplit && D <= 128), "a window with sinks and nothing else");
+  const int front = kSinks ? (a.sinks < br.lo * BN ? (a.sinks + BN - 1) / BN : br.lo) : 0;
 
   const int hk = h / (a.hq / a.hk);                       // fwd_kernel.py:360
   const int row = q0 + wave * 32 + c;                     // this lane's query row
@@ -192,11 +198,12 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
 
   // tiles are fetched in ascending order: the tile bases and the count of rows left
   // advance by one tile per call
-  const T* kt = kbase + (int64_t)br.lo * BN * a.sk.s;
-  const T* vt = vbase + (int64_t)br.lo * BN * a.sv.s;
+  const T* kt = kbase + (front > 0 ? 0 : (int64_t)br.lo * BN * a.sk.s);
+  const T* vt = vbase + (front > 0 ? 0 : (int64_t)br.lo * BN * a.sv.s);
   const int64_t k_step = (int64_t)BN * a.sk.s, v_step = (int64_t)BN * a.sv.s;
   const int k_row_bytes = (int)a.sk.s * 2, v_row_bytes = (int)a.sv.s * 2;
-  int rows_left = si.seqlen_k - br.lo * BN;      // > 0
+  int rows_left = si.seqlen_k - (front > 0 ? 0 : br.lo * BN);      // > 0
+  int front_left = front;
   auto load_next_tile = [&]() {
     const int rows = rows_left < BN ? rows_left : BN;
     const auto krs = wave_rsrc(kt, (rows - 1) * k_row_bytes + d_qk * 2);
@@ -213,6 +220,9 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
       kb_next += (int64_t)BN * a.sb_n * kb_size;
     }
     kt += k_step; vt += v_step; rows_left -= BN;
+    if (kSinks && --front_left == 0) {
+      kt += (br.lo - front) * k_step; vt += (br.lo - front) * v_step; rows_left -= (br.lo - front) * BN;
+    }
   };
 
   // the first K/V tile is requested before the Q rows are waited for: both fetches are in flight
@@ -289,7 +299,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
   auto wave_sees_all = [&](int j) -> bool {
     const int n_first = j * BN, n_last = j * BN + BN - 1;
     bool all = n_last < si.seqlen_k;
-    if (kWindowed) all = all && n_last <= w_rmin + w.right && n_first >= w_rmax - w.left;
+    if (kWindowed) all = all && n_last <= w_rmin + w.right && (n_first >= w_rmax - w.left || (kSinks && n_last < a.sinks));
     return all;
   };
   // visible columns of this lane's row as one range [m_lo, m_lo + m_rng] (empty: m_rng < 0)
@@ -300,6 +310,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
   }
   const bool m_none = m_hi < m_lo;
   const unsigned m_rng = m_none ? 0u : (unsigned)(m_hi - m_lo);
+  const int m_sink = a.sinks < m_hi + 1 ? a.sinks : m_hi + 1;      // the row's sinks end here
 
   f32x16 s[MB];   // S^T of the current tile
 
@@ -501,7 +512,8 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const bool vis = d + (unsigned)(mb * 32 + 8 * (i / 4) + (i % 4)) <= m_rng;
+          const bool vis = d + (unsigned)(mb * 32 + 8 * (i / 4) + (i % 4)) <= m_rng ||
+                           (kSinks && j * BN + 4 * hi + mb * 32 + 8 * (i / 4) + (i % 4) < m_sink);
           s[mb][i] = vis ? s[mb][i] : -__builtin_inff();
         }
     } else if (masked) {
@@ -650,8 +662,8 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
   request_bias(br.lo);
   store_tile(0);
   __syncthreads();
-  for (int j = br.lo; j <= br.hi; ++j) {
-    const int stage = (j - br.lo) & 1;
+  for (int j = front > 0 ? 0 : br.lo, t = 0; j <= br.hi; j = kSinks && j + 1 == front ? br.lo : j + 1, ++t) {
+    const int stage = (kSinks ? t : j - br.lo) & 1;
     store_bias(j);
     if (j < br.hi) {
       load_next_tile();
@@ -725,7 +737,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
 // fwd_item with NW waves of 32 rows, two waves per SIMD or (FwdThirdTile) three; or, kPairs, fwd_item_pair with two waves for 32 rows.
 template <int D, int NW, int BN> constexpr int kFwdWaves = D == 64 && NW == 4 && BN == 32 ? 3 : 2;
 template <typename T, int D, int NW, int BN, bool kPairs, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kSplit,
-          bool kKeyBias, bool kAnyRow = false>
+          bool kKeyBias, bool kAnyRow = false, bool kSinks = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(NW * 64, NW * 64)))
 __attribute__((amdgpu_waves_per_eu(kFwdWaves<D, NW, BN>, kFwdWaves<D, NW, BN>)))
 void fwd_kernel(const FwdArgs a) {
@@ -787,7 +799,7 @@ void fwd_kernel(const FwdArgs a) {
       split_zh(zh, nseq, ratio, z, h);
     }
     if constexpr (kPairs) fwd_item_pair<T, kWindowed, kBias, kDropout, kPad>(a, z, h, mt, smem_raw);
-    else fwd_item<T, D, NW, BN, kWindowed, kBias, kDropout, kPad, kSplit, kKeyBias, kAnyRow>(a, z, h, mt, split, smem_raw);
+    else fwd_item<T, D, NW, BN, kWindowed, kBias, kDropout, kPad, kSplit, kKeyBias, kAnyRow, kSinks>(a, z, h, mt, split, smem_raw);
   }
 }
 
@@ -824,10 +836,10 @@ template <int D> struct FwdHalfTile : FwdTileOf<D, 4, D == 64 ? 64 : 32> {};
 struct FwdThirdTile : FwdTileOf<64, 4, 32> {};
 
 template <typename T, int D, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kSplit = false,
-          bool kKeyBias = false, typename Tile = FwdTile<T, D, kWindowed>, bool kAnyRow = false>
+          bool kKeyBias = false, typename Tile = FwdTile<T, D, kWindowed>, bool kAnyRow = false, bool kSinks = false>
 hipError_t launch_fwd_variant(const FwdArgs& a, dim3 grid, hipStream_t stream) {
   constexpr int NW = Tile::NW;
-  auto kern = fwd_kernel<T, D, NW, Tile::BN, Tile::kPairs, kWindowed, kBias, kDropout, kPad, kSplit, kKeyBias, kAnyRow>;
+  auto kern = fwd_kernel<T, D, NW, Tile::BN, Tile::kPairs, kWindowed, kBias, kDropout, kPad, kSplit, kKeyBias, kAnyRow, kSinks>;
   constexpr int smem = Tile::LDS;
   if (grid.x == 0) return hipSuccess;      // no batch, no head or no query row: nothing to write
   if (smem > 64 * 1024) {

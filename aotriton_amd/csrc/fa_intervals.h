@@ -33,6 +33,12 @@ FA_HD Window parse_window(int causal_type, int32_t Wl, int32_t Wr, int32_t seqle
   return w;
 }
 
+// A window of `window` >= 1 keys up to the query's own position (the last query stands at the last key), as the two bounds above.
+FA_HD Window aligned_window(int32_t window, int32_t seqlen_q, int32_t seqlen_k) {
+  const int32_t shift = seqlen_k - seqlen_q;
+  return Window{window - 1 - shift, shift};
+}
+
 FA_HD int32_t floor_div(int32_t x, int32_t y) {  // y > 0
   int32_t d = x / y;
   return (d * y > x) ? d - 1 : d;

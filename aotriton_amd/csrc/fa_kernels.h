@@ -95,6 +95,25 @@ hipError_t run_bwd_f32_rows(int head_dim, int kernel_slot, const BwdArgs& a, boo
 TileShape f32_rows_tile_shape(int head_dim);
 TileShape f32_tile_shape(int head_dim, int kernel_slot);
 
+// A window and sinks (fa_sinks.h): 16-bit types, head dims up to 128.  run_sinks_dq also writes delta, which run_sinks_dkdv reads.
+#define FA_DECL_SINKS(name, Args)                                                             \
+  hipError_t name##_d64(int, const Args&, hipStream_t);                                       \
+  hipError_t name##_d64_padded(int, const Args&, hipStream_t);                                \
+  hipError_t name##_d128(int, const Args&, hipStream_t);                                      \
+  hipError_t name##_d128_padded(int, const Args&, hipStream_t);                               \
+  hipError_t name##_d128_cols96(int, const Args&, hipStream_t);                               \
+  inline hipError_t name(int dtype, int head_dim, const Args& a, hipStream_t s) {             \
+    const bool padded = a.head_dim != head_dim || a.head_dim_v != head_dim;                   \
+    if (head_dim == 64) return (padded ? name##_d64_padded : name##_d64)(dtype, a, s);        \
+    if (head_dim != 128) return hipErrorNotSupported;                                         \
+    if (a.head_dim <= 96 && a.head_dim_v <= 96) return name##_d128_cols96(dtype, a, s);       \
+    return (padded ? name##_d128_padded : name##_d128)(dtype, a, s);                          \
+  }
+FA_DECL_SINKS(run_sinks_fwd, FwdArgs)
+FA_DECL_SINKS(run_sinks_dkdv, BwdArgs)
+FA_DECL_SINKS(run_sinks_dq, BwdArgs)
+#undef FA_DECL_SINKS
+
 // Vector-ALU kernels (no MFMA): every type at every compiled head dim; they serve tensors whose
 // rows the MFMA kernels cannot load in 16-byte pieces, and delta of the fp32 and split-head-dim families.
 // head_dim is the compiled one (64, 128, 256, 512).  kernel_slot of the backward: 0 delta,

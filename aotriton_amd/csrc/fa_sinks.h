@@ -1,0 +1,249 @@
+// Attention with a sliding window and a few first tokens that stay visible (sinks): gfx950, MFMA 32x32x16.
+//
+// Query i of a sequence of n_q queries and n_k keys stands at p = i + n_k - n_q and sees key c iff
+//   c <= p  and  (c > p - window  or  c < sinks).
+// Forward and dQ are fwd_item and dq_item with kSinks: their tiles are the window's and, in front of those, the tiles that hold
+// sinks only.  dK and dV of the window are dkdv_item's.  What is left is here: dK and dV of the first `sinks` keys, which all
+// queries see.
+//
+// One workgroup of the window's kernel per 128 keys would make the first one loop over all queries while the others loop over
+// window + 128 of them, with 124 of its 128 keys idle for 4 sinks.  So these keys are computed on their own, 32 at a time (one MFMA
+// operand), the queries of all q-heads of the group cut into parts, and the fp32 sums of the parts are added by a second kernel,
+// which overwrites what the window's kernel wrote for these keys (dK and dV are rounded once):
+//   S  (queries x keys) = Q K^T, P = exp2(S c - L), dP = dO V^T, dS = P (dP - delta)
+//   dV^T (d x keys) += dO^T P,   dK^T (d x keys) += Q^T dS
+// Each of the four waves takes 32-query steps of its own through a private LDS area (Q and dO rows, swizzled, read by rows and
+// transposed), so that the loop has no barrier; the next step's rows are in flight meanwhile.
+// What bounds it: HBM, one read of Q and dO (4 D bytes a query against 8 D 32 MFMA operations).
+#pragma once
+#include "fa_bwd_impl.h"
+#include "fa_fwd_impl.h"
+
+namespace fa {
+
+template <int D>
+struct SinkSmem {      // per wave: Q and dO rows; L and -delta.  The waves' sums meet where the rows were
+  static constexpr int TILE_BYTES = 32 * D * 2;
+  static constexpr int STAT_OFF = 2 * TILE_BYTES;
+  static constexpr int WAVE_BYTES = STAT_OFF + 256;
+  static constexpr int SUM_BYTES = 2 * 32 * D * 4;      // dK and dV of 32 keys
+  static constexpr int BYTES = 4 * WAVE_BYTES;
+  static_assert(BYTES >= 2 * SUM_BYTES, "the sums of two waves fit");
+};
+
+template <typename T, int D, int kPad>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256))) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1)))
+void sink_dkdv_kernel(const BwdArgs a) {
+  extern __shared__ __attribute__((aligned(kSwzAlign))) char smem_raw[];
+  using Tr = Traits<T>;
+  using op_t = typename Tr::op_t;
+  using SM = SinkSmem<D>;
+  constexpr int DC = kPad ? kPad : D;
+  constexpr int KS = DC / 16, DB = DC / 32;
+  constexpr int LPR = D / 8, RPI = 64 / LPR, CH = 32 / RPI;      // lanes per row, rows per access, accesses
+
+  const int blocks = (a.sinks + 31) / 32;
+  const int part = blockIdx.x % a.sink_parts, block = blockIdx.x / a.sink_parts % blocks, pair = blockIdx.x / a.sink_parts / blocks;
+  const int z = pair / a.hk, hk = pair % a.hk, group = a.hq / a.hk;
+  const SeqInfo si = get_seq(a.seq, z);
+  const int n0 = block * 32;
+  const int keys = a.sinks < si.seqlen_k ? a.sinks : si.seqlen_k;
+  if (n0 >= keys) return;
+
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31, hi = lane >> 5;
+  const int d_qk = kPad ? a.head_dim : D, d_v = kPad ? a.head_dim_v : D;
+  char* area = smem_raw + wave * SM::WAVE_BYTES;
+  float* stat = reinterpret_cast<float*>(area + SM::STAT_OFF);
+
+  // the lane's key, and the first query that sees it
+  const int key = n0 + c, key_c = key < keys ? key : keys - 1;
+  const int shift = si.seqlen_k - si.seqlen_q;
+  const int q_lo = key < keys ? (key - shift > 0 ? key - shift : 0) : 0x7fffffff;
+  op_t kreg[KS], vreg[KS];
+  {
+    const T* kp = reinterpret_cast<const T*>(a.k) + (int64_t)si.batch_index * a.sk.z + (int64_t)hk * a.sk.h + (int64_t)(si.k_start + key_c) * a.sk.s;
+    const T* vp = reinterpret_cast<const T*>(a.v) + (int64_t)si.batch_index * a.sv.z + (int64_t)hk * a.sv.h + (int64_t)(si.k_start + key_c) * a.sv.s;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      kreg[k] = op_t{};
+      vreg[k] = op_t{};
+      if (16 * k + 8 * hi < d_qk) kreg[k] = *reinterpret_cast<const op_t*>(kp + 16 * k + 8 * hi);
+      if (16 * k + 8 * hi < d_v) vreg[k] = *reinterpret_cast<const op_t*>(vp + 16 * k + 8 * hi);
+    }
+  }
+
+  // steps: (q-head of the group, 32 queries), the part's a contiguous run of them, which the waves take in turn
+  const int first = n0 - shift > 0 ? (n0 - shift) / 32 : 0;      // (no query before it sees a key of the block)
+  const int per_head = (si.seqlen_q + 31) / 32 - first;
+  const int steps = per_head > 0 ? per_head * group : 0;
+  const int t0 = (int)((int64_t)steps * part / a.sink_parts), t1 = (int)((int64_t)steps * (part + 1) / a.sink_parts);
+
+  f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { dk[db][i] = 0.f; dv[db][i] = 0.f; }
+  const float qk_scale = a.sm_scale * kLog2e;
+  const int row_a = Swz<D>::row_base(lane), tr_a0 = Swz<D>::tr_base(lane, 0), tr_a1 = Swz<D>::tr_base(lane, 1);
+  const int r0 = lane / LPR, ch0 = lane % LPR;
+  const int q_row = (int)a.sq.s * 2, do_row = (int)a.sdo.s * 2;
+  const int qvoff = ch0 * 8 < d_qk ? r0 * q_row + ch0 * 16 : kVoffOutOfRange;
+  const int dovoff = ch0 * 8 < d_v ? r0 * do_row + ch0 * 16 : kVoffOutOfRange;
+
+  op_t qn[CH], don[CH];
+  float stat_n = 0.f;
+  int q_at = 0;
+  auto load = [&](int t) {
+    const int h = hk * group + t / per_head;
+    q_at = (first + t % per_head) * 32;
+    const int rows = si.seqlen_q - q_at < 32 ? si.seqlen_q - q_at : 32;
+    const auto qrs = wave_rsrc(reinterpret_cast<const T*>(a.q) + (int64_t)si.batch_index * a.sq.z + (int64_t)h * a.sq.h +
+                                   (int64_t)(si.q_start + q_at) * a.sq.s, (rows - 1) * q_row + d_qk * 2);
+    const auto dors = wave_rsrc(reinterpret_cast<const T*>(a.dout) + (int64_t)si.batch_index * a.sdo.z + (int64_t)h * a.sdo.h +
+                                    (int64_t)(si.q_start + q_at) * a.sdo.s, (rows - 1) * do_row + d_v * 2);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      qn[i] = __builtin_bit_cast(op_t, __builtin_amdgcn_raw_buffer_load_b128(qrs, qvoff, i * RPI * q_row, 0));
+      don[i] = __builtin_bit_cast(op_t, __builtin_amdgcn_raw_buffer_load_b128(dors, dovoff, i * RPI * do_row, 0));
+    }
+    // lanes below 32: L, above: delta.  A query past the sequence gets L = inf, so that its P is 0
+    const int64_t at = lse_offset(si, h, a.hq) + q_at;
+    const auto lrs = wave_rsrc(a.lse + at, rows * 4);
+    const auto drs = wave_rsrc(a.delta + at, rows * 4);
+    const float l = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(lrs, c * 4, 0, 0));
+    const float d = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(drs, c * 4, 0, 0));
+    stat_n = hi ? -d : c < rows ? l * kRcpLn2 : __builtin_inff();
+  };
+
+  int t = t0 + wave;
+  if (t < t1) load(t);
+  for (; t < t1; t += 4) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int at = Swz<D>::addr(r0 + i * RPI, ch0);
+      *reinterpret_cast<op_t*>(area + at) = qn[i];
+      *reinterpret_cast<op_t*>(area + SM::TILE_BYTES + at) = don[i];
+    }
+    stat[lane] = stat_n;
+    const int q0 = q_at;
+    if (t + 4 < t1) load(t + 4);
+    // (the areas are the wave's own, and its LDS operations run in order: what remains is to keep the compiler's order)
+    __builtin_amdgcn_wave_barrier();
+    f32x16 s, dp;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + 32 + 8 * g + 4 * hi);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) dp[4 * g + r] = d4[r];      // dP starts at -delta
+    }
+#pragma unroll
+    for (int k = 0; k < KS; ++k) s = Tr::mfma(swz_read_row<T, D>(area, row_a, k, 0), kreg[k], s);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) dp = Tr::mfma(swz_read_row<T, D>(area + SM::TILE_BYTES, row_a, k, 0), vreg[k], dp);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 l4 = *reinterpret_cast<const f32x4*>(stat + 8 * g + 4 * hi);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = __builtin_fmaf(s[4 * g + r], qk_scale, -l4[r]);
+        s[4 * g + r] = q0 + 8 * g + 4 * hi + r >= q_lo ? fast_exp2(x) : 0.f;
+        dp[4 * g + r] *= s[4 * g + r];
+      }
+    }
+    const op_t p0 = pack8<T>(s, 0), p1 = pack8<T>(s, 1), s0 = pack8<T>(dp, 0), s1 = pack8<T>(dp, 1);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      dv[db] = Tr::mfma(swz_read_tr<T, D>(area + SM::TILE_BYTES, tr_a0, tr_a1, 0, db), p0, dv[db]);
+      dk[db] = Tr::mfma(swz_read_tr<T, D>(area, tr_a0, tr_a1, 0, db), s0, dk[db]);
+    }
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      dv[db] = Tr::mfma(swz_read_tr<T, D>(area + SM::TILE_BYTES, tr_a0, tr_a1, 1, db), p1, dv[db]);
+      dk[db] = Tr::mfma(swz_read_tr<T, D>(area, tr_a0, tr_a1, 1, db), s1, dk[db]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // ---- the four waves' sums: two in LDS, the other two onto them, both out as one -----------------------------
+  // (as the lanes hold them: dK then dV, [32 columns][4 columns of 8][lane])
+  auto sum_at = [&](int w, int which, int db, int g) {
+    return reinterpret_cast<f32x4*>(smem_raw + w * SM::SUM_BYTES) + ((which * (D / 32) + db) * 4 + g) * 64 + lane;
+  };
+  __syncthreads();
+#pragma unroll
+  for (int round = 0; round < 2; ++round) {
+    if (wave / 2 == round) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4 x = {dk[db][4 * g], dk[db][4 * g + 1], dk[db][4 * g + 2], dk[db][4 * g + 3]};
+          f32x4 y = {dv[db][4 * g], dv[db][4 * g + 1], dv[db][4 * g + 2], dv[db][4 * g + 3]};
+          f32x4 *xp = sum_at(wave & 1, 0, db, g), *yp = sum_at(wave & 1, 1, db, g);
+          *xp = round ? *xp + x : x;
+          *yp = round ? *yp + y : y;
+        }
+    }
+    __syncthreads();
+  }
+  f32x4* out = reinterpret_cast<f32x4*>(a.sink_ws) + (int64_t)blockIdx.x * (SM::SUM_BYTES / 16);
+  const f32x4* in = reinterpret_cast<const f32x4*>(smem_raw);
+#pragma unroll
+  for (int e = tid; e < SM::SUM_BYTES / 16; e += 256)
+    if (DC == D || e / 256 % (D / 32) < DB) out[e] = in[e] + in[e + SM::SUM_BYTES / 16];
+}
+
+// Adds up the parts: four columns of a key's dK or dV per thread.
+template <typename T, int D>
+static __global__ __launch_bounds__(256) void sink_sum_kernel(const BwdArgs a) {
+  constexpr int SUMS = SinkSmem<D>::SUM_BYTES / 16, PER = SUMS / 256;      // pieces of a key block, workgroups for them
+  const int blocks = (a.sinks + 31) / 32;
+  const int e = blockIdx.x % PER * 256 + threadIdx.x, block = blockIdx.x / PER % blocks, pair = blockIdx.x / PER / blocks;
+  const int z = pair / a.hk, hk = pair % a.hk;
+  const SeqInfo si = get_seq(a.seq, z);
+  const int lane = e % 64, g = e / 64 % 4, db = e / 256 % (D / 32), which = e / (SUMS / 2);
+  const int key = block * 32 + (lane & 31), col = 32 * db + 8 * g + 4 * (lane >> 5);
+  if (key >= si.seqlen_k || key >= a.sinks || col >= (which ? a.head_dim_v : a.head_dim)) return;
+  const f32x4* p = reinterpret_cast<const f32x4*>(a.sink_ws) + ((int64_t)pair * blocks + block) * a.sink_parts * SUMS + e;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < a.sink_parts; ++i) acc += p[(int64_t)i * SUMS];
+  const Strides3& st = which ? a.sdv : a.sdk;
+  const float f = which ? 1.0f : a.sm_scale;
+  vec<T, 4> t4;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) t4[r] = Traits<T>::cvt(acc[r] * f);
+  *reinterpret_cast<vec<T, 4>*>(reinterpret_cast<T*>(which ? a.dv : a.dk) + (int64_t)si.batch_index * st.z + (int64_t)hk * st.h +
+                                (int64_t)(si.k_start + key) * st.s + col) = t4;
+}
+
+// ---- launchers ------------------------------------------------------------------------------------------------
+template <typename T, int D, int kPad>
+hipError_t launch_fwd_sinks(const FwdArgs& a, hipStream_t stream) {
+  const int half = a.half_tiles, BM = half ? 128 : FwdTile<T, D, true>::BM;
+  FwdArgs b = a;
+  b.num_m_tiles = (a.seq.max_seqlen_q + BM - 1) / BM;
+  const TileWork w = tile_work(nseq_of(a.seq, a.batch) * a.hq, q_head_group(a.hq, a.hk), b.num_m_tiles);
+  b.num_zh = w.num_zh; b.zh_per_xcd = w.zh_per_xcd; b.zh_group = w.zh_group; b.items_per_xcd = w.items_per_xcd;
+  const dim3 grid((unsigned)(kNumXcd * tile_workers(w.items_per_xcd, a.num_cu, half ? half : 1)));
+  if (half) return launch_fwd_variant<T, D, true, false, false, kPad, false, false, FwdHalfTile<D>, false, true>(b, grid, stream);
+  return launch_fwd_variant<T, D, true, false, false, kPad, false, false, FwdTile<T, D, true>, false, true>(b, grid, stream);
+}
+
+// dK and dV of the window's keys, and over them those of the sinks
+template <typename T, int D, int kPad>
+hipError_t launch_dkdv_sinks(const BwdArgs& a, hipStream_t stream) {
+  hipError_t e = launch_dkdv_form<T, D, kPad, true, false, false, false, false, kBiasAny, true>(a, stream);
+  const int pairs = bwd_nseq(a) * a.hk, blocks = (a.sinks + 31) / 32;
+  if (e != hipSuccess || blocks == 0 || pairs == 0 || a.seq.max_seqlen_k <= 0) return e;
+  e = launch_with_lds<sink_dkdv_kernel<T, D, kPad>>(dim3((unsigned)(pairs * blocks * a.sink_parts)), 256, SinkSmem<D>::BYTES, stream, a);
+  if (e == hipSuccess) {
+    hipLaunchKernelGGL((sink_sum_kernel<T, D>), dim3((unsigned)(pairs * blocks * (SinkSmem<D>::SUM_BYTES / 16 / 256))), dim3(256), 0, stream, a);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+}  // namespace fa

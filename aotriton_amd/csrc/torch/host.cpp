@@ -36,90 +36,13 @@
 #include <vector>
 
 #include "aotriton_amd/flash.h"
+#include "views.h"
 
 namespace {
 
-using at::Tensor;
+using namespace fa_host;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-// ---- views ------------------------------------------------------------------------------------
-
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return FA_DTYPE_FLOAT32;
-    case at::kHalf: return FA_DTYPE_FLOAT16;
-    case at::kBFloat16: return FA_DTYPE_BFLOAT16;
-    case at::kChar: return FA_DTYPE_INT8;
-    case at::kShort: return FA_DTYPE_INT16;
-    case at::kInt: return FA_DTYPE_INT32;
-    case at::kLong: return FA_DTYPE_INT64;
-    case at::kByte: return FA_DTYPE_UINT8;
-    case at::kUInt16: return FA_DTYPE_UINT16;
-    case at::kUInt32: return FA_DTYPE_UINT32;
-    case at::kUInt64: return FA_DTYPE_UINT64;
-    default: return FA_DTYPE_UNKNOWN;
-  }
-}
-
-// View of a tensor of rank N (fa_tensor4, fa_tensor2 or fa_tensor1), null for an undefined one.
-// False: not a view the operators take (rank, last stride, element type).
-template <typename V, int N>
-bool view_of(const Tensor& t, V* v) {
-  *v = V{};
-  if (!t.defined()) return true;
-  if (t.dim() != N || t.stride(-1) != 1) return false;
-  v->ptr = t.data_ptr();
-  for (int i = 0; i < N; ++i) {
-    v->sizes[i] = (uint64_t)t.size(i);
-    v->strides[i] = (uint64_t)t.stride(i);
-  }
-  v->dtype = dtype_code(t.scalar_type());
-  return v->dtype != FA_DTYPE_UNKNOWN;
-}
-bool view4(const Tensor& t, fa_tensor4* v) { return view_of<fa_tensor4, 4>(t, v); }
-bool view2(const Tensor& t, fa_tensor2* v) { return view_of<fa_tensor2, 2>(t, v); }
-// a rank-1 view has two elements or more: one element or none is a device scalar
-bool view1(const Tensor& t, fa_tensor1* v) {
-  return view_of<fa_tensor1, 1>(t, v) && (!t.defined() || t.numel() > 1);
-}
-bool view0(const Tensor& t, fa_tensor0* v) {
-  *v = fa_tensor0{};
-  if (!t.defined()) return true;
-  if (t.dim() != 1 || t.numel() > 1) return false;
-  v->ptr = t.data_ptr();
-  v->dtype = dtype_code(t.scalar_type());
-  return v->dtype != FA_DTYPE_UNKNOWN;
-}
-
-fa_tensor0 scalar_at(const Tensor& block, int i) {
-  fa_tensor0 v{};
-  v.ptr = static_cast<uint64_t*>(block.data_ptr()) + i;
-  v.dtype = FA_DTYPE_UINT64;
-  return v;
-}
-
-void* current_stream() { return c10::hip::getCurrentHIPStream().stream(); }
-
-const char* error_name(int rc) {
-  switch (rc) {
-    case 1: return "hipErrorInvalidValue";
-    case 2: return "hipErrorOutOfMemory";
-    case 13: return "hipErrorInvalidSymbol";
-    case 209: return "hipErrorNoBinaryForGpu";
-    case 217: return "hipErrorPeerAccessUnsupported";
-    case 700: return "hipErrorIllegalAddress";
-    case 801: return "hipErrorNotSupported";
-    default: return "hipError";
-  }
-}
-
-void check_rc(int rc, bool backend_is_not_implemented) {
-  if (rc == FA_SUCCESS) return;
-  TORCH_CHECK_NOT_IMPLEMENTED(!(backend_is_not_implemented && rc == FA_ERROR_PEER_ACCESS_UNSUPPORTED),
-                              "backend cannot take this input");
-  TORCH_CHECK(false, "flash operator failed: <hipError_t.", error_name(rc), ": ", rc, ">");
-}
 
 // delta of the split backward, allocated when the library asks for it
 struct LazyDelta {
@@ -142,28 +65,6 @@ struct LazyDelta {
     }
   }
   static void dispose(fa_lazy_tensor2* self) { static_cast<LazyDelta*>(self->cookie)->held.reset(); }
-};
-
-// Scratch memory of a forward, from torch's allocator: ordered with the stream, and a graph's own under capture.
-// It is taken on the current device, whose current stream the call runs on: on another device (where the
-// caller's tensors lie, say) the allocator could hand it on before the kernels are done with it.
-struct Scratch {
-  fa_allocator c{};
-  Tensor held;
-  Scratch() {
-    c.cookie = this;
-    c.alloc = &alloc;
-  }
-  static void* alloc(fa_allocator* self, uint64_t bytes) {
-    auto* me = static_cast<Scratch*>(self->cookie);
-    try {
-      const at::Device device(at::kCUDA, c10::hip::current_device());
-      me->held = at::empty({(int64_t)bytes}, at::TensorOptions(at::kByte).device(device));
-      return me->held.data_ptr();
-    } catch (...) {
-      return nullptr;
-    }
-  }
 };
 
 // ---- what `attention`, the custom ops and their backwards share -----------------------------------
@@ -311,15 +212,6 @@ struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
     return {dq, dk, dv, db, Tensor()};
   }
 };
-
-// There is no forward-mode formula.  A call without a gradient goes past the Function, whose own error would
-// come after the launch: without this check such a call would answer without the tangent.
-void refuse_tangents(std::initializer_list<const Tensor*> inputs) {
-  if (torch::autograd::ForwardADLevel::try_get_by_idx(0) == nullptr) return;      // (the tensors' own look takes locks)
-  for (const Tensor* t : inputs)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
-                                "forward-mode AD of the attention operators (jvp) is not implemented");
-}
 
 // (Out, encoded softmax, logsumexp); the last two undefined unless asked for
 variable_list attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& b, const AttentionOptions& x) {
@@ -560,6 +452,168 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> backward_autograd(
   return {r[0], r[1], r[2], r[3]};
 }
 
+// ---- a sliding window and first tokens that stay visible ------------------------------------------------------------
+// sink_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks, sm_scale) -> out, logsumexp
+// sink_attention_backward(dout, q, k, v, out, logsumexp, the same from cu_seqlens_q on) -> dQ, dK, dV
+
+using SinkFwdSig = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
+                                              const std::optional<Tensor>&, c10::SymInt, c10::SymInt, c10::SymInt, c10::SymInt, double);
+using SinkBwdSig = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                      const std::optional<Tensor>&, const std::optional<Tensor>&, c10::SymInt, c10::SymInt,
+                                                      c10::SymInt, c10::SymInt, double);
+const c10::TypedOperatorHandle<SinkFwdSig>& sink_forward_op() {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("aotriton_amd::sink_attention_forward", "").typed<SinkFwdSig>();
+  return op;
+}
+const c10::TypedOperatorHandle<SinkBwdSig>& sink_backward_op() {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("aotriton_amd::sink_attention_backward", "").typed<SinkBwdSig>();
+  return op;
+}
+
+// The kernels move rows in aligned 16-byte pieces; a tensor whose rows are not made of them is copied.
+Tensor pieces(const Tensor& t) {
+  bool ok = t.stride(-1) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
+  for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.size(i) <= 1 || t.stride(i) % 8 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+int32_t as_int32(int64_t x, const char* what) {
+  TORCH_CHECK_VALUE(x >= 0 && x <= std::numeric_limits<int32_t>::max(), what, " must be a number of 31 bits, not ", x);
+  return (int32_t)x;
+}
+
+Varlen sink_varlen(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& cu_q, const std::optional<Tensor>& cu_k,
+                   int64_t max_q, int64_t max_k) {
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "expected (batch, heads, seq, head_dim) tensors");
+  TORCH_CHECK_VALUE(k.device() == q.device() && v.device() == q.device(), "q, k and v are on different devices");
+  const bool has = cu_q.has_value() && cu_q->defined();
+  TORCH_CHECK_VALUE(has == (cu_k.has_value() && cu_k->defined()), "cu_seqlens come for queries and keys or for neither");
+  Varlen vl;
+  if (!has) return vl;
+  for (const Tensor* t : {&*cu_q, &*cu_k})
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->numel() >= 2 && t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == q.device(),
+                      "cu_seqlens are contiguous int32 tensors of the sequences + 1 offsets, on the device of the queries");
+  TORCH_CHECK_VALUE(q.size(0) == 1, "packed sequences are (1, heads, tokens, head_dim) tensors");
+  vl.cu_q = *cu_q;
+  vl.cu_k = *cu_k;
+  vl.max_q = as_int32(max_q, "max_seqlen_q");
+  vl.max_k = as_int32(max_k, "max_seqlen_k");
+  return vl;
+}
+
+std::tuple<Tensor, Tensor> sink_forward_kernel(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const std::optional<Tensor>& cu_q,
+                                               const std::optional<Tensor>& cu_k, int64_t max_q, int64_t max_k, int64_t window,
+                                               int64_t sinks, double sm_scale) {
+  const c10::DeviceGuard guard(q_in.device());
+  const Varlen vl = sink_varlen(q_in, k_in, v_in, cu_q, cu_k, max_q, max_k);
+  const int32_t w = as_int32(window, "window"), n = as_int32(sinks, "sinks");
+  const Tensor q = pieces(q_in), k = pieces(k_in), v = pieces(v_in);
+  fa_fwd_params p{};
+  fill_common(p, q, k, v, Tensor(), sm_scale, 0.0, Mask{}, vl);
+  const bool packed = vl.cu_q.defined();
+  // in the memory order of the queries
+  Tensor o = q.size(3) == v.size(3) ? at::empty_like(q) : at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
+  if (o.stride(-1) != 1) o = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
+  Tensor lse = at::empty({packed ? q.size(1) : q.size(0) * q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  TORCH_CHECK(view2(lse, &p.L) && view4(o, &p.Out), "outputs");
+  check_rc(fa_attn_fwd_sinks(&p, FA_FWD_PARAMS_VERSION, w, n, current_stream(), nullptr), false);
+  return {std::move(o), std::move(lse)};
+}
+
+std::tuple<Tensor, Tensor, Tensor> sink_backward_kernel(const Tensor& dout_in, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
+                                                        const Tensor& out_in, const Tensor& lse_in, const std::optional<Tensor>& cu_q,
+                                                        const std::optional<Tensor>& cu_k, int64_t max_q, int64_t max_k,
+                                                        int64_t window, int64_t sinks, double sm_scale) {
+  const c10::DeviceGuard guard(q_in.device());
+  const Varlen vl = sink_varlen(q_in, k_in, v_in, cu_q, cu_k, max_q, max_k);
+  const int32_t w = as_int32(window, "window"), n = as_int32(sinks, "sinks");
+  TORCH_CHECK_VALUE(dout_in.dim() == 4 && out_in.dim() == 4 && lse_in.dim() == 2 && dout_in.device() == q_in.device() &&
+                        out_in.device() == q_in.device() && lse_in.device() == q_in.device(),
+                    "expected the outputs of sink_attention_forward and a gradient like the first, on the device of the queries");
+  const Tensor q = pieces(q_in), k = pieces(k_in), v = pieces(v_in), out = pieces(out_in), dout = pieces(dout_in), lse = lse_in.contiguous();
+  fa_bwd_params p{};
+  fill_common(p, q, k, v, Tensor(), sm_scale, 0.0, Mask{}, vl);
+  const auto like = [](const Tensor& t) { Tensor g = at::empty_like(t); return g.stride(-1) == 1 ? g : at::empty(t.sizes(), t.options()); };
+  Tensor dq = like(q), dk = like(k), dv = like(v);
+  TORCH_CHECK(view4(out, &p.Out) && view4(dout, &p.DO) && view2(lse, &p.L) && view4(dq, &p.DQ) && view4(dk, &p.DK) && view4(dv, &p.DV),
+              "the last stride of tensors must be 1");
+  LazyDelta delta(lse.sizes(), lse.device());
+  p.D = delta.c;
+  Scratch scratch;
+  check_rc(fa_attn_bwd_sinks(&p, FA_BWD_PARAMS_VERSION, w, n, current_stream(), nullptr, &scratch.c), false);
+  return {std::move(dq), std::move(dk), std::move(dv)};
+}
+
+struct SinkFunction : torch::autograd::Function<SinkFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& cu_q,
+                               const std::optional<Tensor>& cu_k, const c10::SymInt& max_q, const c10::SymInt& max_k,
+                               const c10::SymInt& window, const c10::SymInt& sinks, double sm_scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [o, lse] = sink_forward_op().call(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale);
+    ctx->save_for_backward({q, k, v, o, lse, cu_q.value_or(Tensor()), cu_k.value_or(Tensor())});
+    ctx->mark_non_differentiable({lse});
+    ctx->set_materialize_grads(false);
+    auto& d = ctx->saved_data;
+    d["max_q"] = max_q;
+    d["max_k"] = max_k;
+    d["window"] = window;
+    d["sinks"] = sinks;
+    d["sm_scale"] = sm_scale;
+    return {o, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    auto& d = ctx->saved_data;
+    const Tensor dout = grads[0].defined() ? grads[0] : at::zeros_like(s[3]);
+    const auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+    auto [dq, dk, dv] = sink_backward_op().call(dout, s[0], s[1], s[2], s[3], s[4], maybe(s[5]), maybe(s[6]), d["max_q"].toSymInt(),
+                                                d["max_k"].toSymInt(), d["window"].toSymInt(), d["sinks"].toSymInt(), d["sm_scale"].toDouble());
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> sink_forward_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& cu_q,
+                                                 const std::optional<Tensor>& cu_k, c10::SymInt max_q, c10::SymInt max_k,
+                                                 c10::SymInt window, c10::SymInt sinks, double sm_scale) {
+  refuse_tangents({&q, &k, &v});
+  if (!(at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return sink_forward_op().call(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale);
+  }
+  variable_list r = SinkFunction::apply(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale);
+  return {r[0], r[1]};
+}
+
+// (no derivative of its own, as flash_attention_backward)
+struct SinkBackwardFunction : torch::autograd::Function<SinkBackwardFunction> {
+  static variable_list forward(AutogradContext*, const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+                               const Tensor& lse, const std::optional<Tensor>& cu_q, const std::optional<Tensor>& cu_k,
+                               const c10::SymInt& max_q, const c10::SymInt& max_k, const c10::SymInt& window, const c10::SymInt& sinks,
+                               double sm_scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [dq, dk, dv] = sink_backward_op().call(dout, q, k, v, out, lse, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale);
+    return {dq, dk, dv};
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "Trying to backward through aotriton_amd::sink_attention_backward, which has no autograd formula: "
+                       "second derivatives of the attention operators are not implemented");
+  }
+};
+std::tuple<Tensor, Tensor, Tensor> sink_backward_autograd(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v,
+                                                          const Tensor& out, const Tensor& lse, const std::optional<Tensor>& cu_q,
+                                                          const std::optional<Tensor>& cu_k, c10::SymInt max_q, c10::SymInt max_k,
+                                                          c10::SymInt window, c10::SymInt sinks, double sm_scale) {
+  refuse_tangents({&dout, &q, &k, &v, &out, &lse});
+  bool grad = false;
+  for (const Tensor* t : {&dout, &q, &k, &v, &out, &lse}) grad |= t->requires_grad();
+  if (!(at::GradMode::is_enabled() && grad)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return sink_backward_op().call(dout, q, k, v, out, lse, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale);
+  }
+  variable_list r = SinkBackwardFunction::apply(dout, q, k, v, out, lse, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale);
+  return {r[0], r[1], r[2]};
+}
+
 // (pt2_compliant_tag: fake implementations and Autograd kernels are there, so that torch.compile may keep the
 // ops in its graphs also where it is told to take compliant ops only)
 TORCH_LIBRARY(aotriton_amd, m) {
@@ -574,14 +628,23 @@ TORCH_LIBRARY(aotriton_amd, m) {
         "float dropout_p, SymInt causal_type, SymInt window_left, SymInt window_right, float sm_scale, "
         "Tensor philox_seed, Tensor philox_offset, bool need_dbias, SymInt backend) -> (Tensor, Tensor, Tensor, Tensor)",
         compliant);
+  m.def("sink_attention_forward(Tensor q, Tensor k, Tensor v, Tensor? cu_seqlens_q, Tensor? cu_seqlens_k, SymInt max_seqlen_q, "
+        "SymInt max_seqlen_k, SymInt window, SymInt sinks, float sm_scale) -> (Tensor, Tensor)", compliant);
+  m.def("sink_attention_backward(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor? cu_seqlens_q, "
+        "Tensor? cu_seqlens_k, SymInt max_seqlen_q, SymInt max_seqlen_k, SymInt window, SymInt sinks, float sm_scale) "
+        "-> (Tensor, Tensor, Tensor)", compliant);
 }
 TORCH_LIBRARY_IMPL(aotriton_amd, CUDA, m) {
+  m.impl("sink_attention_forward", &sink_forward_kernel);
+  m.impl("sink_attention_backward", &sink_backward_kernel);
   m.impl("philox_state", &philox_kernel);
   m.impl("flash_attention_forward", &forward_kernel);
   m.impl("flash_attention_forward_key_mask", &key_mask_kernel);
   m.impl("flash_attention_backward", &backward_kernel);
 }
 TORCH_LIBRARY_IMPL(aotriton_amd, Autograd, m) {
+  m.impl("sink_attention_forward", &sink_forward_autograd);
+  m.impl("sink_attention_backward", &sink_backward_autograd);
   m.impl("flash_attention_forward", &forward_autograd);
   m.impl("flash_attention_forward_key_mask", &key_mask_autograd);
   m.impl("flash_attention_backward", &backward_autograd);

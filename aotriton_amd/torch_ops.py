@@ -11,6 +11,12 @@ so that code using them can be traced by torch.compile / AOTAutograd.
     flash_attention_backward(dout, q, k, v, bias, out, lse, dropout_p, causal_type, window_left, window_right,
                              sm_scale, seed, offset, need_dbias, backend)
         -> dQ, dK, dV, dB (empty unless need_dbias); backend: -1 the library's choice, 0 split, 1 fused
+    sink_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks, sm_scale)
+        -> Out, logsumexp; a sliding window and first tokens that stay visible (sink_attention below)
+    sink_attention_backward(dout, q, k, v, out, lse, cu_seqlens_q, ..., sm_scale)
+        -> dQ, dK, dV
+    tree_attention, cache_append, cache_copy_pages, cache_fork, cache_keep_path, cache_free
+        the cache of pages (cache.py)
     philox_state(like, increment)
         -> seed and offset (uint64[1] tensors on like's device) of the device's default generator, whose
            offset moves on by `increment` counters (rounded up to a multiple of 4)
@@ -29,6 +35,8 @@ device between replays.
 `scaled_dot_product_attention` here has the signature of
 torch.nn.functional.scaled_dot_product_attention and runs on those ops.
 """
+import math
+
 import torch
 from torch import Tensor
 
@@ -38,7 +46,8 @@ from .sdpa import prepare
 
 _torch_host = _host.load()      # registers the ops
 
-__all__ = ['flash_attention_forward', 'flash_attention_backward', 'philox_state', 'scaled_dot_product_attention']
+__all__ = ['flash_attention_forward', 'flash_attention_backward', 'philox_state', 'scaled_dot_product_attention',
+           'sink_attention']
 
 
 philox_state = torch.ops.aotriton_amd.philox_state
@@ -72,6 +81,50 @@ def _(dout, q, k, v, bias, out, lse, dropout_p, causal_type, window_left, window
     mk = lambda t: torch.empty(t.shape, device=q.device, dtype=q.dtype)
     want_db = need_dbias and bias is not None
     return mk(q), mk(k), mk(v), (mk(bias) if want_db else torch.empty([0], device=q.device, dtype=q.dtype))
+
+
+@torch.library.register_fake('aotriton_amd::sink_attention_forward')
+def _(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks, sm_scale):
+    shape = (q.shape[0], q.shape[1], q.shape[2], v.shape[3])
+    o = torch.empty_like(q) if q.shape[3] == v.shape[3] else torch.empty(shape, device=q.device, dtype=q.dtype)
+    if o.stride(-1) != 1:
+        o = torch.empty(shape, device=q.device, dtype=q.dtype)
+    heads = q.shape[1] if cu_seqlens_q is not None else q.shape[0] * q.shape[1]
+    return o, torch.empty((heads, q.shape[2]), device=q.device, dtype=torch.float32)
+
+
+@torch.library.register_fake('aotriton_amd::sink_attention_backward')
+def _(dout, q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks, sm_scale):
+    def like(t):
+        g = torch.empty_like(t)
+        return g if g.stride(-1) == 1 else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+    return like(q), like(k), like(v)
+
+
+def sink_attention(query, key, value, window, sinks=0, scale=None, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=None,
+                   max_seqlen_k=None):
+    """Causal attention with a sliding window and a few first tokens that stay visible, forward and backward.
+
+    query (B, Hq, Sq, E), key (B, Hk, Sk, E), value (B, Hk, Sk, Ev), fp16 or bf16 CUDA tensors of any storage, head dims multiples
+    of 8 up to 128, Hq a multiple of Hk.  The queries stand at the last keys: query i is at position p = i + Sk - Sq and sees
+    the ``window`` keys up to its own (p - window < c <= p) and, before those, keys c < ``sinks`` (at most 1024).  A query
+    before the first key yields zeros and no gradient.
+
+    Packed sequences: (1, H, tokens, E) tensors with the sequences' offsets in cu_seqlens_q / cu_seqlens_k (int32 tensors on the device,
+    sequences + 1 values) and their greatest lengths in max_seqlen_q / max_seqlen_k; positions and sinks count from each
+    sequence's start, and tokens behind the last offset are left alone: their rows of the result are not written.
+
+    Works under HIP graph capture and torch.compile; results do not change from call to call.  There is no dropout and no bias.
+    Single tokens over a cache: aotriton_amd.cache.tree_attention with a window.
+    """
+    sm_scale = 1.0 / math.sqrt(query.shape[-1]) if scale is None else float(scale)
+    if (cu_seqlens_q is None) != (cu_seqlens_k is None):
+        raise ValueError('cu_seqlens come for queries and keys or for neither')
+    if cu_seqlens_q is not None and (max_seqlen_q is None or max_seqlen_k is None):
+        raise ValueError('packed sequences need max_seqlen_q and max_seqlen_k')
+    o, _ = torch.ops.aotriton_amd.sink_attention_forward(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q or 0,
+                                                         max_seqlen_k or 0, window, sinks, sm_scale)
+    return o
 
 
 def scaled_dot_product_attention(query, key, value, attn_mask=None, dropout_p=0.0, is_causal=False,

@@ -274,6 +274,24 @@ FA_API int fa_attn_fwd_key_mask(const fa_fwd_params* params, int32_t params_vers
 FA_API int fa_attn_bwd(const fa_bwd_params* params, int32_t params_version,
                        void* hip_stream, const fa_options* options);
 
+/* Attention with a sliding window and a few first tokens that stay visible ("sinks").  The queries of a sequence stand at its
+ * last keys: query i of n_q queries and n_k keys is at position p = i + n_k - n_q and sees key c iff
+ *   c <= p  and  (c > p - window  or  c < sinks),
+ * so `window` counts the query's own key.  Dense, packed, padded and strided sequences as in fa_attn_fwd / fa_attn_bwd, grouped heads,
+ * fp16 and bf16, head dims up to 128 (q/k's and v's may differ) of tensors whose rows are aligned 16-byte pieces; a row that sees no key
+ * (more queries than keys) gives 0 and a logsumexp of +inf, and no gradient.  params->causal_type is FA_CAUSAL_NONE: the two
+ * numbers are the mask.  FA_ERROR_INVALID_VALUE: window < 1, sinks < 0, another causal_type; FA_ERROR_NOT_SUPPORTED: a bias, dropout,
+ * encoded_softmax, other element types, head dims or alignment, sinks > FA_MAX_SINKS; all before anything is launched.
+ * The backward takes scratch memory for fp32 sums of the sinks' gradients (all queries add to them): from `alloc`, as
+ * fa_attn_fwd_alloc describes it, or without one from the library's workspace; FA_ERROR_OUT_OF_MEMORY where there is none (stream
+ * capture without an allocator, the limit), with nothing launched.  It needs params->D, has no single-launch backend and no
+ * atomics: results do not change from call to call.  No counterpart in the reference. */
+#define FA_MAX_SINKS 1024
+FA_API int fa_attn_fwd_sinks(const fa_fwd_params* params, int32_t params_version, int32_t window, int32_t sinks,
+                             void* hip_stream, const fa_options* options);
+FA_API int fa_attn_bwd_sinks(const fa_bwd_params* params, int32_t params_version, int32_t window, int32_t sinks,
+                             void* hip_stream, const fa_options* options, fa_allocator* alloc);
+
 /* The positional v2 API: v2::flash::attn_fwd, attn_fwd_compact_varlen, attn_bwd, attn_bwd_fused,
  * attn_bwd_compact_varlen.  These are not in the reference tree (0.14 keeps only the v3 params
  * entry points); their signatures are those of AOTriton 0.11's include/aotriton/v2/flash.h:31-141

@@ -1,0 +1,404 @@
+"""The cache of pages and the attention of drafted tokens over it, against the 64-bit oracle: lengths around blocks, pages and parts, trees
+with tokens that are not there, windows with sinks, holes in the page table, slots that hold anything.  Bounds: tests/_longctx.py."""
+import math
+import random
+
+import pytest
+import torch
+
+from _longctx import assert_within, lse_bound, out_bound, score_error
+from oracle import longctx
+
+pytestmark = pytest.mark.gpu
+
+DEV = 'cuda'
+
+
+def _pool(lens, tokens, Hk, D, page, dtype, seed, Dv=None, extra=5, slot_major=True, columns=None):
+    """caches with pages in any order, the table, and the lengths; slots that belong to nobody hold NaN and inf"""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-(max(n, 0) + tokens) // page) for n in lens]
+    columns = max(need) + 1 if columns is None else columns
+    pages = sum(need) + extra
+    order = torch.randperm(pages, generator=g).tolist()
+    table = torch.full((len(lens), columns), -1, dtype=torch.int32)
+    rubbish = torch.tensor([float('nan'), float('inf')], dtype=dtype)
+
+    def cache(d):
+        c = rubbish[torch.randint(0, 2, (pages, page, Hk, d), generator=g)]
+        return c.transpose(1, 2) if slot_major else c.transpose(1, 2).contiguous()
+    k, v = cache(D), cache(D if Dv is None else Dv)
+    at = 0
+    for z, n in enumerate(lens):
+        table[z, :need[z]] = torch.tensor(order[at:at + need[z]], dtype=torch.int32)
+        at += need[z]
+        for s in range(max(n, 0) + tokens):
+            for c in (k, v):
+                c[table[z, s // page], :, s % page] = torch.randn(Hk, c.shape[3], generator=g).to(dtype)
+    return k, v, table, torch.tensor(lens, dtype=torch.int32)
+
+
+def _tree(rng, t, holes=0.0):
+    return [-2 if rng.random() < holes else -1 if i == 0 or rng.random() < 0.15 else rng.randint(max(0, i - 4), i - 1) for i in range(t)]
+
+
+def _run(q, k, v, table, lens, parents, window, sinks, scale, max_length=None):
+    from aotriton_amd import cache
+    dev = lambda t: None if t is None else t.to(DEV)
+    return cache.tree_attention(dev(q), dev(k), dev(v), dev(table), dev(lens), dev(parents), max_length, window, sinks, scale, return_lse=True)
+
+
+def _check(q, k, v, table, lens, parents, window, sinks, scale, out, lse):
+    want, want_lse, size = longctx.tree_attention(q, k, v, table, lens, parents, window, sinks, scale)
+    clean = lambda c: torch.where(torch.isfinite(c.double()), c.double(), 0.0)
+    e = score_error(q, clean(k), scale)
+    values = clean(v).abs().amax() * (int(lens.max()) + q.shape[2] + 1)
+    assert_within('out', out, want, out_bound(q.dtype, want, size, values, e))
+    assert_within('lse', lse, want_lse, lse_bound(torch.where(want_lse.isinf(), 0.0, want_lse), e))
+
+
+CASES = [
+    # lens, Hq, Hk, tokens, D, page, window, sinks, dtype, tree
+    ([0], 1, 1, 1, 64, 16, 0, 0, torch.bfloat16, False),
+    ([1], 4, 4, 1, 128, 16, 0, 0, torch.float16, False),
+    ([31, 32, 33], 8, 2, 1, 128, 16, 0, 0, torch.bfloat16, False),
+    ([15, 16, 17, 0], 4, 1, 2, 64, 16, 0, 0, torch.float16, True),
+    ([4095], 32, 8, 1, 128, 64, 0, 0, torch.bfloat16, False),
+    ([700, 3, 129], 8, 8, 1, 64, 32, 0, 0, torch.float16, False),
+    ([500, 77], 8, 2, 9, 128, 16, 0, 0, torch.bfloat16, True),           # 36 packed rows
+    ([100, 0, 64], 7, 1, 33, 64, 64, 0, 0, torch.bfloat16, True),
+    ([1000, 40], 16, 2, 64, 128, 256, 0, 0, torch.float16, True),        # 512 rows
+    ([300], 4, 4, 64, 64, 16, 0, 0, torch.float16, False),               # a chain
+    ([900, 20, 333], 8, 2, 1, 128, 16, 100, 4, torch.bfloat16, False),
+    ([900, 64, 5], 4, 2, 12, 64, 32, 64, 40, torch.float16, True),
+    ([640, 700], 4, 1, 30, 128, 64, 5, 2, torch.bfloat16, False),        # a chain longer than the window
+    ([640, 3], 4, 1, 40, 64, 16, 3, 5, torch.float16, True),
+    ([200], 2, 2, 3, 64, 16, 1, 0, torch.bfloat16, False),               # nothing but itself
+    ([50, 200], 2, 2, 3, 64, 16, 2000, 1000, torch.bfloat16, True),      # a window beyond everything
+    ([333, 5], 6, 2, 5, 256, 32, 0, 0, torch.bfloat16, True),
+    ([333, 5], 6, 2, 5, 200, 32, 77, 3, torch.float16, True),
+    ([97], 3, 1, 4, 72, 16, 0, 0, torch.bfloat16, True),
+    ([97, 1], 2, 1, 4, 40, 16, 0, 0, torch.float16, True),
+]
+
+
+@pytest.mark.parametrize('lens,Hq,Hk,tokens,D,page,window,sinks,dtype,tree', CASES)
+def test_tree_attention(lens, Hq, Hk, tokens, D, page, window, sinks, dtype, tree):
+    k, v, table, n = _pool(lens, tokens, Hk, D, page, dtype, seed=sum(lens) + D + tokens)
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(len(lens), tokens, Hq, D, generator=g).to(dtype).transpose(1, 2)
+    rng = random.Random(tokens)
+    parents = torch.tensor([_tree(rng, tokens) for _ in lens], dtype=torch.int32) if tree else None
+    scale = 1 / math.sqrt(D)
+    for top in (max(lens), 0, None):      # split for the lengths, hardly, and for the table's
+        out, lse = _run(q, k, v, table, n, parents, window, sinks, scale, top)
+        _check(q, k, v, table, n, parents, window, sinks, scale, out, lse)
+
+
+def test_many_parts_of_a_long_cache():
+    lens = [9000]
+    k, v, table, n = _pool(lens, 1, 1, 64, 64, torch.bfloat16, seed=3)
+    q = torch.randn(1, 4, 1, 64, generator=torch.Generator().manual_seed(2)).bfloat16()
+    out, lse = _run(q, k, v, table, n, None, 0, 0, 0.125)
+    _check(q, k, v, table, n, None, 0, 0, 0.125, out, lse)
+
+
+@pytest.mark.parametrize('window', [0, 20])
+def test_tokens_that_are_not_there(window):
+    lens, tokens = [70, 33, 0], 21
+    k, v, table, n = _pool(lens, tokens, 2, 64, 16, torch.float16, seed=4)
+    rng = random.Random(5)
+    rows = [_tree(rng, tokens, holes=0.25) for _ in lens]
+    rows[0][3], rows[0][7], rows[1][0] = 3, 9, 5            # itself, a later one, a later one
+    rows[2] = [-2] * tokens                                 # nothing at all
+    parents = torch.tensor(rows, dtype=torch.int32)
+    # what is not there may hold anything
+    for z in range(3):
+        for t in range(tokens):
+            if longctx.chain(rows[z], t) is None:
+                s = lens[z] + t
+                k[table[z, s // 16], :, s % 16] = float('inf')
+                v[table[z, s // 16], :, s % 16] = float('nan')
+    q = torch.randn(3, 4, tokens, 64, generator=torch.Generator().manual_seed(6)).half()
+    out, lse = _run(q, k, v, table, n, parents, window, 2 if window else 0, 0.125)
+    _check(q, k, v, table, n, parents, window, 2 if window else 0, 0.125, out, lse)
+    assert (out[2] == 0).all() and torch.isinf(lse[2]).all()
+
+
+def test_bad_lengths_and_pages():
+    """a negative length, lengths past the table, entries that are no pages: what they stand for is not there"""
+    lens, tokens, page = [100, 200, 60, 150], 3, 16
+    k, v, table, n = _pool(lens, tokens, 2, 64, page, torch.bfloat16, seed=7)
+    k, v = (torch.where(torch.isfinite(c.float()), c, torch.zeros_like(c)) for c in (k, v))
+    n[0] = -5
+    n[1] = table.shape[1] * page - 1                         # the drafted tokens lie behind the table's end, all but one
+    table[2, 1] = k.shape[0]
+    table[2, 2] = 2 ** 31 - 1
+    table[3, :3] = -(2 ** 31)
+    table[1, 5] = -1
+    q = torch.randn(4, 4, tokens, 64, generator=torch.Generator().manual_seed(8)).bfloat16()
+    parents = torch.tensor([[-1, 0, 0]] * 4, dtype=torch.int32)
+    for window, sinks in ((0, 0), (50, 20)):
+        out, lse = _run(q, k, v, table, n, parents, window, sinks, 0.125)
+        _check(q, k, v, table, n, parents, window, sinks, 0.125, out, lse)
+    assert (out[0] == 0).all()
+
+
+def test_released_pages_under_a_window():
+    """pages between the sinks and the window go back to the pool and are somebody else's"""
+    from aotriton_amd import cache
+    lens, page, window, sinks = [600, 310], 16, 64, 4
+    k, v, table, n = _pool(lens, 1, 2, 64, page, torch.float16, seed=9)
+    q = torch.randn(2, 4, 1, 64, generator=torch.Generator().manual_seed(10)).half()
+    k, v, table, n, q = (t.to(DEV) for t in (k, v, table, n, q))
+    want = cache.tree_attention(q, k, v, table, n, window=window, sinks=sinks)
+    uses = torch.zeros(k.shape[0], dtype=torch.int32, device=DEV)
+    uses[table[table >= 0].long()] = 1
+    before = table.clone()
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    cache.free(table, uses, ints(0, 1), ints(1, 1), (n - window + 1) // page)
+    gone = before[(before >= 0) & (table < 0)].long()
+    assert len(gone) == (600 - 63) // 16 - 1 + (310 - 63) // 16 - 1 and (uses[gone] == 0).all()
+    k[gone], v[gone] = float('nan'), float('nan')
+    assert torch.equal(cache.tree_attention(q, k, v, table, n, window=window, sinks=sinks), want)
+
+
+def test_value_head_dim_heads_first_and_strides():
+    lens, tokens = [130, 64], 4
+    k, v, table, n = _pool(lens, tokens, 2, 64, 32, torch.bfloat16, seed=11, Dv=128, slot_major=False)
+    q = torch.randn(2, 6, tokens, 64, generator=torch.Generator().manual_seed(12)).bfloat16()
+    wide = torch.zeros(2, 9, dtype=torch.int32)[:, 2:2 + table.shape[1]].copy_(table)      # rows of a bigger table
+    out, lse = _run(q, k, v, table, n, None, 0, 0, 0.125)
+    _check(q, k, v, table, n, None, 0, 0, 0.125, out, lse)
+    out2, _ = _run(q, k, v, wide, n, None, 0, 0, 0.125)
+    assert torch.equal(out, out2)
+    odd = torch.empty(2, 6, tokens, 67, dtype=q.dtype)[..., 1:65].copy_(q)
+    assert torch.equal(_run(odd, k, v, table, n, None, 0, 0, 0.125)[0], out)
+
+
+@pytest.mark.parametrize('scale', [0.0, -0.3, 8.0])
+def test_scales(scale):
+    k, v, table, n = _pool([90], 2, 1, 64, 16, torch.bfloat16, seed=13)
+    q = torch.randn(1, 2, 2, 64, generator=torch.Generator().manual_seed(14)).bfloat16()
+    out, lse = _run(q, k, v, table, n, None, 0, 0, scale)
+    _check(q, k, v, table, n, None, 0, 0, scale, out, lse)
+
+
+# ---- rows, pages and sequences: everything is exact ---------------------------------------------------------------
+
+def _equal(a, b):
+    as_int = lambda t: t.cpu().contiguous().view(torch.int16)
+    assert torch.equal(as_int(a), as_int(b))
+
+
+@pytest.mark.parametrize('page,Hk,D,Dv,slot_major', [(16, 1, 64, 64, True), (64, 8, 128, 128, True), (32, 3, 72, 40, False)])
+def test_append_and_keep(page, Hk, D, Dv, slot_major):
+    from aotriton_amd import cache
+    lens, tokens, steps = [0, 15, 16, 100, -3, 47], 20, 9
+    k, v, table, n = _pool(lens, tokens, Hk, D, page, torch.float16, seed=15, Dv=Dv, slot_major=slot_major)
+    table[3, (100 + 5) // page] = -1                             # a hole: what goes there is dropped
+    g = torch.Generator().manual_seed(16)
+    nk = torch.randn(6, tokens, Hk, D, generator=g).half().transpose(1, 2)
+    nv = torch.randn(6, tokens, Hk, Dv, generator=g).half().transpose(1, 2)
+    counts = torch.tensor([20, 7, 0, 20, 20, 25], dtype=torch.int32)
+    rng = random.Random(17)
+    path = torch.tensor([sorted(rng.sample(range(tokens), steps)) for _ in lens], dtype=torch.int32)
+    kept = torch.tensor([9, 4, 0, 9, 3, 30], dtype=torch.int32)
+    dk, dv, dt, dn = (t.to(DEV) for t in (k, v, table, n))
+    cache.append(nk.to(DEV), nv.to(DEV), dk, dv, dt, dn, counts.to(DEV))
+    where = lambda z, s: (int(table[z, s // page]), s % page) if s // page < table.shape[1] and table[z, s // page] >= 0 else None
+    for z in range(6):
+        for t in range(min(tokens, int(counts[z]))):
+            at = where(z, lens[z] + t) if lens[z] >= 0 else None
+            if at:
+                k[at[0], :, at[1]], v[at[0], :, at[1]] = nk[z, :, t], nv[z, :, t]
+    _equal(dk, k)
+    _equal(dv, v)
+    after = cache.keep_path(dk, dv, dt, dn, path.to(DEV), kept.to(DEV))
+    for z in range(6):
+        if lens[z] < 0:
+            continue
+        for i in range(min(int(kept[z]), steps)):
+            a, b = where(z, lens[z] + int(path[z, i])), where(z, lens[z] + i)
+            if a and b:
+                k[b[0], :, b[1]], v[b[0], :, b[1]] = k[a[0], :, a[1]].clone(), v[a[0], :, a[1]].clone()
+    _equal(dk, k)
+    _equal(dv, v)
+    assert after.tolist() == [9, 19, 16, 109, -3, 56]
+    assert dn.tolist() == lens
+
+
+@pytest.mark.parametrize('layout', ['slots first', 'heads first', 'apart'])
+def test_copy_pages(layout):
+    from aotriton_amd import cache
+    g = torch.Generator().manual_seed(18)
+    k, v = torch.randn(12, 16, 3, 72, generator=g).bfloat16(), torch.randn(12, 16, 3, 72, generator=g).bfloat16()
+    if layout == 'heads first':
+        k, v = k.view(12, 3, 16, 72), v.view(12, 3, 16, 72)
+        dk, dv = k.to(DEV), v.to(DEV)
+    else:
+        k, v = k.transpose(1, 2), v.transpose(1, 2)
+        dk, dv = (t.to(DEV) for t in (k, v))
+        if layout == 'apart':
+            dk = torch.zeros(12, 3, 20, 80, dtype=k.dtype, device=DEV)[:, :, :16, :72].copy_(k)
+    source, target = [0, 5, 5, -1, 12, 7, 2], [3, 1, 9, 4, 6, 7, 40]
+    cache.copy_pages(dk, dv, *(torch.tensor(x, dtype=torch.int32, device=DEV) for x in (source, target)))
+    for a, b in ((0, 3), (5, 1), (5, 9)):
+        k[b], v[b] = k[a].clone(), v[a].clone()
+    _equal(dk, k)
+    _equal(dv, v)
+
+
+def test_fork_and_free():
+    from aotriton_amd import cache
+    page, lens = 16, [40, 32, 7, 0, 16]
+    k, v, table, n = _pool(lens + [0] * 5, 0, 2, 64, page, torch.float16, seed=19, extra=8, columns=300)
+    pages = k.shape[0]
+    table[0, 1] = -1                                             # a released page
+    used = set(table[table >= 0].tolist())
+    unused = [p for p in range(pages) if p not in used]
+    uses = torch.zeros(pages, dtype=torch.int32)
+    uses[table[table >= 0].long()] = 1
+    table[9, :4] = torch.tensor([3, 4, 5, 6], dtype=torch.int32)    # overwritten
+    source, target = [0, 0, 1, 2, 3, 4, 99], [5, 6, 7, 8, 9, -1, 3]
+    spare = unused[:2] + [pages + 1] + unused[2:3] + [-1, 0, 0]
+    dk, dv, dt, dn, du = (t.to(DEV) for t in (k, v, table, n, uses))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    cache.fork(dk, dv, dt, dn, du, ints(source), ints(target), ints(spare))
+    for a, b, x in list(zip(source, target, spare))[:5]:
+        full, tail = divmod(lens[a], page)
+        row = table[a].clone()
+        row[full:] = -1
+        if tail:
+            k[x, :, :tail], v[x, :, :tail] = k[table[a, full], :, :tail], v[table[a, full], :, :tail]
+            row[full] = x
+        table[b] = row
+        n[b] = lens[a]
+        for p in row[row >= 0].tolist():
+            uses[p] += 1
+    _equal(dk, k)
+    _equal(dv, v)
+    assert torch.equal(dt.cpu(), table) and torch.equal(dn.cpu(), n) and torch.equal(du.cpu(), uses)
+    # the first sequence goes, twice in one call; another one's first page; nothing; a sequence that is not there
+    cache.free(dt, du, ints([0, 0, 7, 1, 50, -1]), ints([0, 0, 0, 5, 0, 0]), ints([300, 1000, 1, 2, 9, 9]))
+    for p in table[0][table[0] >= 0].tolist() + [int(table[7, 0])]:
+        uses[p] -= 1
+    table[0] = -1
+    table[7, 0] = -1
+    assert torch.equal(dt.cpu(), table) and torch.equal(du.cpu(), uses)
+
+
+@pytest.mark.parametrize('window,sinks', [(0, 0), (90, 4)])
+def test_a_prompt_then_drafted_tokens(window, sinks):
+    """The operators together: a prompt goes through attention with sinks into the cache, the sequence is forked, trees are drafted,
+    attended and kept, and what the tokens get equals attention over the whole sequence at once."""
+    from aotriton_amd import cache, torch_ops
+    B, Hq, Hk, D, page, prompt, tokens, dt = 2, 4, 2, 64, 16, 75, 6, torch.bfloat16
+    g = torch.Generator().manual_seed(21)
+    rn = lambda h, n: torch.randn(B, n, h, D, generator=g).to(dt).to(DEV).transpose(1, 2)
+    total = prompt + 2 * tokens
+    w = window or 10 ** 6
+    qs, ks, vs = rn(Hq, prompt), rn(Hk, prompt), rn(Hk, prompt)
+    columns = -(-total // page) + 1
+    k = torch.full((60, page, Hk, D), float('nan'), dtype=dt, device=DEV).transpose(1, 2)
+    v = k.clone()
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    table = ints([list(range(z * columns, (z + 1) * columns)) for z in range(B)] + [[-1] * columns] * B)
+    uses = torch.zeros(60, dtype=torch.int32, device=DEV)
+    uses[:B * columns] = 1
+    lengths = ints([0] * B)
+    for at in range(0, prompt, 50):
+        cache.append(ks[:, :, at:at + 50], vs[:, :, at:at + 50], k, v, table[:B], lengths + at)
+    lengths = ints([prompt] * B + [0] * B)
+    cache.fork(k, v, table, lengths, uses, ints([0, 1]), ints([2, 3]), ints([50, 51]))
+    table[2:, prompt // page + 1:prompt // page + 2] = ints([[52], [53]])      # room for the drafts
+    assert lengths.tolist() == [prompt] * 4
+    grow = [(ks, vs, qs)]
+    for step in range(2):
+        q, nk, nv = rn(Hq, tokens), rn(Hk, tokens), rn(Hk, tokens)
+        parents = ints([[-1, 0, 0, 1, 2, 3], [-1, 0, 1, 1, -1, 4]])
+        path, counts = ints([[0, 1, 3, 5], [0, 1, 3, 3]]), ints([4, 3])
+        both = lambda t: torch.cat([t, t])
+        cache.append(both(nk), both(nv), k, v, table, lengths)
+        out = cache.tree_attention(both(q), k, v, table, lengths, both(parents), window=window, sinks=sinks)
+        assert torch.equal(out[:B], out[B:])                               # the fork sees what its source sees
+        after = cache.keep_path(k, v, table, lengths, both(path), both(counts))
+        if step == 0:
+            # the accepted path as a sequence of its own, all at once
+            for z in range(B):
+                take = path[z, :counts[z]].long()
+                kk, vv, qq = (torch.cat([a[z], b[z][:, take]], 1)[None] for a, b in ((ks, nk), (vs, nv), (qs, q)))
+                whole = torch_ops.sink_attention(qq, kk, vv, w, sinks)[0, :, prompt:]
+                seen = longctx.sink_mask(qq.shape[2], kk.shape[2], w, sinks)
+                want, _, p = longctx.attention(qq[0].cpu(), kk[0].cpu(), vv[0].cpu(), seen, D ** -0.5)
+                size = torch.matmul(p, vv[0].cpu().double().abs().repeat_interleave(2, 0))
+                bound = out_bound(dt, want, size, vv.abs().sum().cpu().double(), score_error(qq, kk, D ** -0.5))[:, prompt:]
+                assert_within('tree', out[z][:, take], want[:, prompt:], bound)
+                assert_within('whole', whole, want[:, prompt:], bound)
+                rows, there = longctx.rows_of(k.cpu(), table[z].tolist(), int(after[z]))
+                assert there.all()
+                _equal(rows, kk[0])
+        lengths = after
+    assert lengths.tolist() == [prompt + 8, prompt + 6] * 2
+    cache.free(table, uses, ints([0, 1, 2, 3]), ints([0] * 4), ints([columns] * 4))
+    assert (table == -1).all()
+    assert (uses[:B * columns] == 0).all() and (uses[50:52] == 0).all()
+
+
+def test_captured_serving_step():
+    """append, attention and keep in a graph, replayed with eager work between the replays"""
+    from aotriton_amd import cache
+    lens, tokens = [300, 45], 8
+    k, v, table, n = (t.to(DEV) for t in _pool(lens, tokens * 4, 2, 64, 16, torch.bfloat16, seed=22))
+    g = torch.Generator().manual_seed(23)
+    q, nk, nv = (torch.zeros(2, h, tokens, 64, dtype=torch.bfloat16, device=DEV) for h in (4, 2, 2))
+    parents = torch.tensor([_tree(random.Random(z), tokens) for z in range(2)], dtype=torch.int32, device=DEV)
+    path = torch.tensor([[0, 2, 3, 6], [1, 2, 4, 7]], dtype=torch.int32, device=DEV)
+    counts = torch.tensor([4, 2], dtype=torch.int32, device=DEV)
+
+    def step(k, v, n):
+        cache.append(nk, nv, k, v, table, n)
+        out = cache.tree_attention(q, k, v, table, n, parents, max_length=320)
+        return out, cache.keep_path(k, v, table, n, path, counts)
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        step(k.clone(), v.clone(), n)
+    torch.cuda.current_stream().wait_stream(warm)
+    ek, ev, en = k.clone(), v.clone(), n.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, after = step(k, v, n)
+    for _ in range(4):
+        for t in (q, nk, nv):
+            t.copy_(torch.randn(t.shape, generator=g).bfloat16())
+        graph.replay()
+        torch.cuda.synchronize()
+        want, en2 = step(ek, ev, en)
+        assert torch.equal(out, want) and torch.equal(after, en2)
+        _equal(k, ek)
+        n.copy_(after)
+        en = en2
+
+
+def test_two_streams_and_schemas():
+    from aotriton_amd import cache
+    k, v, table, n = (t.to(DEV) for t in _pool([2000, 30], 5, 2, 128, 64, torch.bfloat16, seed=24))
+    q = torch.randn(2, 8, 5, 128, device=DEV).bfloat16()
+    want = cache.tree_attention(q, k, v, table, n)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(cache.tree_attention(q, k, v, table, n))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
+    torch.library.opcheck(torch.ops.aotriton_amd.tree_attention, (q, k, v, table, n, None, 2000, 0, 0, 0.1),
+                          test_utils=('test_schema', 'test_faketensor'))
+    one = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for op, args in (('cache_append', (q[:, :2], q[:, :2], k, v, table, n, None)), ('cache_copy_pages', (k, v, one, one + 1)),
+                     ('cache_keep_path', (k, v, table, n, torch.zeros(2, 1, dtype=torch.int32, device=DEV), n * 0))):
+        torch.library.opcheck(getattr(torch.ops.aotriton_amd, op), args, test_utils=('test_schema', 'test_faketensor'))
+    with pytest.raises(NotImplementedError, match='no gradient'):
+        cache.tree_attention(q.requires_grad_(True), k, v, table, n)
