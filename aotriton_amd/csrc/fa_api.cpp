@@ -1396,7 +1396,7 @@ int fa_attn_fwd_sinks(const fa_fwd_params* p, int32_t params_version, int32_t wi
   hipStream_t stream = static_cast<hipStream_t>(hip_stream);
   const DeviceInfo* dev = device_of_stream(stream);
   if (dev == nullptr || !dev->is_gfx950) return FA_ERROR_NO_BINARY_FOR_GPU;
-  fa::FwdArgs a{};
+  fa::SinkFwdArgs a{};
   a.q = p->Q.ptr; a.k = p->K.ptr; a.v = p->V.ptr;
   a.out = p->Out.ptr;
   a.lse = static_cast<float*>(p->L.ptr);
@@ -1422,7 +1422,7 @@ int fa_attn_bwd_sinks(const fa_bwd_params* p, int32_t params_version, int32_t wi
   hipStream_t stream = static_cast<hipStream_t>(hip_stream);
   const DeviceInfo* dev = device_of_stream(stream);
   if (dev == nullptr || !dev->is_gfx950) return FA_ERROR_NO_BINARY_FOR_GPU;
-  fa::BwdArgs a{};
+  fa::SinkBwdArgs a{};
   a.q = p->Q.ptr; a.k = p->K.ptr; a.v = p->V.ptr;
   a.out = p->Out.ptr; a.dout = p->DO.ptr;
   a.dq = p->DQ.ptr; a.dk = p->DK.ptr; a.dv = p->DV.ptr;

@@ -3,6 +3,8 @@
 #pragma once
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace fa {
 
 constexpr int kNumXcd = 8;   // MI355X: 8 XCDs x 32 CUs, one L2 each
@@ -163,8 +165,6 @@ struct FwdArgs {
   float* part_o;         // columns: the compiled head dim
   float* part_ml;        // reference maximum (units of the scores) and row sum
   int32_t key_mask;      // the bias is one byte per key, the same for all rows (sb_m = 0): 0 hides the key
-  // kernels with kSinks: a query sees `window` keys up to its own position (aligned_window), and of those before them the first `sinks`
-  int32_t window, sinks;
 };
 
 struct BwdArgs {
@@ -202,10 +202,22 @@ struct BwdArgs {
   // (sequence and kv-head, key tile, part, dK then dV, key, column), where a second kernel adds them up
   int32_t part_heads, part_tiles;
   float* part_ws;            // null: not cut
-  // kernels with kSinks: as in FwdArgs; dK and dV of the first keys come from fp32 sums over sink_parts parts of the queries (fa_sinks.h)
-  int32_t window, sinks, sink_parts;
+};
+
+// Kernels with kSinks: a query sees `window` keys up to its own position (aligned_window), and of those before them the first `sinks`.
+// (Blocks of their own, and not members of the ones above: the kernels without sinks keep their argument layout and so their code.)
+struct SinkFwdArgs : FwdArgs {
+  int32_t window, sinks;
+};
+struct SinkBwdArgs : BwdArgs {
+  int32_t window, sinks;
+  // dK and dV of the first keys come from fp32 sums over sink_parts parts of the queries (fa_sinks.h)
+  int32_t sink_parts;
   float* sink_ws;
 };
+
+template <bool kSinks> using FwdArgsOf = std::conditional_t<kSinks, SinkFwdArgs, FwdArgs>;
+template <bool kSinks> using BwdArgsOf = std::conditional_t<kSinks, SinkBwdArgs, BwdArgs>;
 
 // Copy between a rank-4 tensor of any strides and head dim (unit last stride) and its packed
 // image: contiguous (n0, n1, n2, dp) with dp the head dim rounded up to a multiple of 8, zeros in

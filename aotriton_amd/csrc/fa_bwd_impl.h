@@ -173,7 +173,7 @@ __device__ __forceinline__ uint32_t dropout_append4(const DropoutState& s, int m
 // D80 315 -> 303 us.
 template <typename T, int D, int NW, int BM, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kStoreDs = false,
           bool kParts = false, int kForm = kBiasAny, bool kSinks = false>
-__device__ __forceinline__ void dkdv_item(const BwdArgs& a, const int hk, const int nt, const int z, const int part,
+__device__ __forceinline__ void dkdv_item(const BwdArgsOf<kSinks>& a, const int hk, const int nt, const int z, const int part,
                                           char* smem_raw) {
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
@@ -198,7 +198,7 @@ __device__ __forceinline__ void dkdv_item(const BwdArgs& a, const int hk, const 
   if (n0 >= si.seqlen_k) return;
 
   Window w{0, 0};
-  if (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);      // (dK and dV of the first keys: fa_sinks.h)
+  if constexpr (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);      // (dK and dV of the first keys: fa_sinks.h)
   else if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right,
                                   si.seqlen_q, si.seqlen_k);
   w.left = w.left > (1 << 30) ? (1 << 30) : (w.left < -(1 << 30) ? -(1 << 30) : w.left);
@@ -899,7 +899,7 @@ __device__ __forceinline__ void dkdv_item(const BwdArgs& a, const int hk, const 
 // the split backward has no preprocess launch, the dK/dV kernel runs after this one and reads it.
 template <typename T, int D, int NW, int BN, bool kWindowed, bool kBias, bool kDropout, bool kInlineDelta, int kPad,
           bool kStoreDelta = false, bool kSinks = false>
-__device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int mt, const int z,
+__device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h, const int mt, const int z,
                                         char* smem_raw) {
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
@@ -922,7 +922,7 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
   if (q0 >= si.seqlen_q) return;
 
   Window w{0, 0};
-  if (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);
+  if constexpr (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);
   else if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right,
                                   si.seqlen_q, si.seqlen_k);
   w.left = w.left > (1 << 30) ? (1 << 30) : (w.left < -(1 << 30) ? -(1 << 30) : w.left);
@@ -944,8 +944,10 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
   const unsigned m_rng = m_none ? 0u : (unsigned)(m_hi - m_lo);
   // kSinks, as in fwd_item: tiles before the window's first, in which only sinks are visible; where the row's sinks end
   static_assert(!kSinks || (kWindowed && !kBias && !kDropout), "a window with sinks and nothing else");
-  const int front = kSinks ? (a.sinks < br.lo * BN ? (a.sinks + BN - 1) / BN : br.lo) : 0;
-  const int m_sink = a.sinks < m_hi + 1 ? a.sinks : m_hi + 1;
+  int sinks = 0;
+  if constexpr (kSinks) sinks = a.sinks;
+  const int front = kSinks ? (sinks < br.lo * BN ? (sinks + BN - 1) / BN : br.lo) : 0;
+  const int m_sink = sinks < m_hi + 1 ? sinks : m_hi + 1;
 
   T* dqptr = reinterpret_cast<T*>(a.dq) + (int64_t)si.batch_index * a.sdq.z + (int64_t)h * a.sdq.h +
              (int64_t)(si.q_start + row_c) * a.sdq.s;
@@ -1163,9 +1165,10 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
     k_rs = wave_rsrc(kt, any ? ((rows - 1) * (int)a.sk.s + d_qk) * 2 : 0);
     v_rs = wave_rsrc(vt, any ? ((rows - 1) * (int)a.sv.s + d_v) * 2 : 0);
     if (live) { kt += k_step; vt += v_step; rows_left -= BN; }
-    if (kSinks && live && --front_left == 0) {
-      kt += (br.lo - front) * k_step; vt += (br.lo - front) * v_step; rows_left -= (br.lo - front) * BN;
-    }
+    if constexpr (kSinks)
+      if (live && --front_left == 0) {
+        kt += (br.lo - front) * k_step; vt += (br.lo - front) * v_step; rows_left -= (br.lo - front) * BN;
+      }
   };
   constexpr int FETCH_PIECES = 2 * CH;
   auto fetch_piece = [&](int i) {        // K pieces first, then V
@@ -1299,7 +1302,8 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
       }
       if (masked) {
         // one unsigned comparison of n - m_lo against the length of the visible range
-        const bool vis = m_d + (unsigned)(32 * mb + 8 * g + r) <= m_rng || (kSinks && n < m_sink);
+        bool vis = m_d + (unsigned)(32 * mb + 8 * g + r) <= m_rng;
+        if constexpr (kSinks) vis = vis || n < m_sink;
         x = vis ? x : -__builtin_inff();
       }
       s[mb][i] = fast_exp2(x);
@@ -1398,13 +1402,18 @@ __device__ __forceinline__ void dq_item(const BwdArgs& a, const int h, const int
   __syncthreads();
   // K tiles come as [masked | full | masked]; one straight-line loop per run
   {
-    int j = front > 0 ? 0 : br.lo, t = 0;
+    int j = br.lo;
+    int at = 0;      // kSinks: tiles done
+    if constexpr (kSinks)
+      if (front > 0) j = 0;
     auto step = [&](auto masked_tag, auto fast_tag) __attribute__((always_inline)) {
-      const int stage = (kSinks ? t : j - br.lo) & 1;
+      int stage = (j - br.lo) & 1;
+      if constexpr (kSinks) stage = at++ & 1;
       compute(masked_tag, fast_tag, j, stage, j < br.hi);
       __syncthreads();
-      j = kSinks && j + 1 == front ? br.lo : j + 1;
-      ++t;
+      ++j;
+      if constexpr (kSinks)
+        if (j == front) j = br.lo;
     };
     const int full_lo = br.fb_lo <= br.fb_hi ? br.fb_lo : br.hi + 1;
     const int full_hi = br.fb_lo <= br.fb_hi ? br.fb_hi : br.hi;
@@ -1454,7 +1463,7 @@ template <typename T, int D, int NW, int BM, bool kWindowed, bool kBias, bool kD
           bool kParts = false, int kForm = kBiasAny, bool kSinks = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(NW * 64, NW * 64)))
 __attribute__((amdgpu_waves_per_eu(kTwoDkDv<D, kBias, kDropout, kStoreDs, kForm> ? 2 : 1, kTwoDkDv<D, kBias, kDropout, kStoreDs, kForm> ? 2 : 1)))
-void bwd_dkdv_kernel(const BwdArgs a) {
+void bwd_dkdv_kernel(const BwdArgsOf<kSinks> a) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   // Persistent workgroups, one per CU (a relaunch per item costs a dispatch gap of several
   // microseconds on every CU).  Each XCD owns a contiguous range of (batch, kv-head)
@@ -1500,7 +1509,7 @@ void bwd_dkdv_kernel(const BwdArgs a) {
 
 template <typename T, int D, int NW, int BN, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kSinks = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(NW * 64, NW * 64))) __attribute__((amdgpu_waves_per_eu(kTwoWaves<D, kBias> ? 2 : 1, kTwoWaves<D, kBias> ? 2 : 1)))
-void bwd_dq_kernel(const BwdArgs a) {
+void bwd_dq_kernel(const BwdArgsOf<kSinks> a) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   // persistent workgroups with the same walk as the forward kernel: (batch, q-head) pairs
   // per XCD, heaviest Q tile first, serpentine over the workgroups of the XCD
@@ -1533,8 +1542,8 @@ inline void set_work(BwdArgs& a, const TileWork& w) {
   a.num_zh = w.num_zh; a.zh_per_xcd = w.zh_per_xcd; a.zh_group = w.zh_group; a.items_per_xcd = w.items_per_xcd;
 }
 
-template <auto kern>
-hipError_t launch_with_lds(dim3 grid, int nthreads, int smem, hipStream_t stream, const BwdArgs& a) {
+template <auto kern, typename A>
+hipError_t launch_with_lds(dim3 grid, int nthreads, int smem, hipStream_t stream, const A& a) {
   if (grid.x == 0 || grid.y == 0 || grid.z == 0) return hipSuccess;   // an empty tensor: nothing to write
   if (smem > 64 * 1024) {
     static std::atomic<uint64_t> lds_set{0};
@@ -1607,9 +1616,9 @@ hipError_t launch_combine_dkdv(const BwdArgs& a, hipStream_t stream) {
 }
 
 template <typename T, int D, int kPad, bool W, bool B, bool P, bool kParts, bool kStoreDs, int kForm, bool kSinks = false>
-hipError_t launch_dkdv_form(const BwdArgs& a0, hipStream_t stream) {
+hipError_t launch_dkdv_form(const BwdArgsOf<kSinks>& a0, hipStream_t stream) {
   constexpr int NW = BwdTile<T, D, W>::NW, BM = kDkDvBM<T, D, W, B, P, kStoreDs>, BN = NW * 32;
-  BwdArgs a = a0;
+  BwdArgsOf<kSinks> a = a0;
   a.num_n_tiles = (a.seq.max_seqlen_k + BN - 1) / BN;
   set_work(a, tile_work(bwd_nseq(a) * a.hk, 2, a.num_n_tiles * (kParts ? a.part_heads * a.part_tiles : 1)));
   dim3 grid((unsigned)(kNumXcd * bwd_workers(D, B, a.items_per_xcd, a.num_cu, kTwoWaves<D, B> ? 2 : 1)));
@@ -1656,10 +1665,10 @@ hipError_t launch_bwd_dkdv(const BwdArgs& a0, bool windowed, bool bias, bool dro
 }
 
 template <typename T, int D, int kPad, bool W, bool B, bool P, bool kSinks = false>
-hipError_t launch_dq_variant(const BwdArgs& a0, hipStream_t stream) {
+hipError_t launch_dq_variant(const BwdArgsOf<kSinks>& a0, hipStream_t stream) {
   using Tile = BwdTile<T, D, W>;
   constexpr int NW = Tile::NW, BN = kDqBN<T, D, W, B>, BM = NW * 32;
-  BwdArgs a = a0;
+  BwdArgsOf<kSinks> a = a0;
   a.num_m_tiles = (a.seq.max_seqlen_q + BM - 1) / BM;
   set_work(a, tile_work(bwd_nseq(a) * a.hq, q_head_group(a.hq, a.hk), a.num_m_tiles));
   dim3 grid((unsigned)(kNumXcd * bwd_workers(D, B, a.items_per_xcd, a.num_cu, kTwoWaves<D, B> ? 2 : 1)));

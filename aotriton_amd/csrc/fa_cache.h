@@ -1,7 +1,6 @@
 // Attention of drafted tokens over a cache of pages: gfx950, MFMA 32x32x16.
 #pragma once
 #include "fa_cache_args.h"
-#include "fa_combine.h"
 #include "fa_device.h"
 
 namespace fa {
@@ -76,6 +75,54 @@ struct PageTable {
   }
 };
 
+// The blocks of 32 slots that a sequence's rows may see: those that hold sinks, then those of the window (without one: all).
+struct TreeBlocks {
+  int win_lo, all_lo;            // first slot that some row, that every row sees by its window
+  int sinks, first, front, blocks;
+  __device__ __forceinline__ TreeBlocks(const TreeArgs& a, const TreeSeq& seq) {
+    win_lo = all_lo = 0;
+    if (a.window > 0) {
+      win_lo = seq.length - a.window + 1 > 0 ? seq.length - a.window + 1 : 0;
+      all_lo = seq.length + a.tokens - a.window > 0 ? seq.length + a.tokens - a.window : 0;
+    }
+    const int last = seq.end > 0 ? (seq.end - 1) / 32 : -1;
+    first = win_lo / 32;
+    sinks = a.window > 0 ? a.sinks : 0;
+    front = sinks < first * 32 ? (sinks + 31) / 32 : first;
+    blocks = last >= first ? front + last - first + 1 : 0;
+  }
+  __device__ __forceinline__ int block_of(int i) const { return i < front ? i : first + i - front; }
+  // every row sees all of these slots, as far as their pages are there
+  __device__ __forceinline__ bool whole(const TreeSeq& seq, int n0, int n) const {
+    return n0 + n <= seq.length && (n0 >= all_lo || n0 + n <= sinks);
+  }
+  // some row sees slot n: what lies in the others may be inf or NaN
+  __device__ __forceinline__ bool seen(const TreeSeq& seq, uint64_t there, int n) const {
+    const int j = n - seq.length;
+    return j < 0 ? (n >= win_lo || n < sinks) : j < 64 && (there >> (j & 63) & 1) != 0;
+  }
+  __device__ __forceinline__ int parts(const TreeArgs& a) const { return blocks > a.part_blocks ? (blocks + a.part_blocks - 1) / a.part_blocks : 1; }
+};
+
+// What a packed row sees.
+struct TreeRow {
+  uint64_t kin;
+  int m_lo, m_sink;              // of the filled slots [m_lo, length) and those below m_sink
+  bool alive;
+  __device__ __forceinline__ TreeRow(const TreeArgs& a, const TreeSeq& seq, const TreeNode& node, uint64_t there, int token) {
+    kin = shfl64(node.kin, token);
+    const int depth = __shfl(node.depth, token);
+    alive = (there >> token & 1) != 0;
+    m_lo = !alive ? 0x7fffffff : a.window > 0 ? seq.length + depth - a.window + 1 : 0;
+    m_sink = alive && a.window > 0 ? a.sinks : 0;
+    if (!alive) kin = 0;
+  }
+  __device__ __forceinline__ bool sees(const TreeSeq& seq, int n) const {
+    const int j = n - seq.length;
+    return j < 0 ? (n >= m_lo || n < m_sink) : j < 64 && (kin >> (j & 63) & 1) != 0;
+  }
+};
+
 // ---- few rows: 32 packed (token, q-head) rows of one K/V head x one part of its keys per workgroup -----------------------
 // As fwd_rows_kernel: the waves take blocks of 32 slots in turn, each with an online softmax of its own; they meet in LDS, the parts
 // in combine_rows_kernel.  K and V are read once per 32 rows, and what bounds it is HBM.  The blocks of an item are those that hold
@@ -103,13 +150,17 @@ void tree_rows_kernel(const TreeArgs a) {
   constexpr int VSTR = SM::VSTR, OSTR = SM::OSTR;
   constexpr int LPR = D / 8, RPI = 64 / LPR, CHV = 32 / RPI;      // V: lanes per row, rows per access, accesses
 
-  // units (pair, split) go round the XCDs, the row blocks of a unit follow each other on one
+  // units (pair, part) go round the XCDs, the row blocks of a unit follow each other on one
   const CacheArgs& c = a.cache;
   const int xcd = blockIdx.x % kNumXcd, idx = blockIdx.x / kNumXcd;
   const int unit = (idx / a.row_blocks) * kNumXcd + xcd, rb = idx % a.row_blocks;
-  const int pair = unit / a.splits, split = unit % a.splits;
+  const int pair = unit / a.parts, part = unit % a.parts;
   if (pair >= c.sequences * c.heads) return;
   const int z = pair / c.heads, hk = pair % c.heads, group = a.hq / c.heads;
+  const TreeSeq seq = tree_seq(a, z);
+  const TreeBlocks range(a, seq);
+  const int parts = range.parts(a);
+  if (part >= parts) return;
   const int rows = a.tokens * group, r0 = rb * 32;
   const int nrows = rows - r0 < 32 ? rows - r0 : 32;
 
@@ -117,7 +168,6 @@ void tree_rows_kernel(const TreeArgs a) {
   const int lane = tid & 63, col = lane & 31, hi = lane >> 5;
   const int d_qk = kPad ? c.head_dim : D, d_v = kPad ? c.head_dim_v : D;
 
-  const TreeSeq seq = tree_seq(a, z);
   uint64_t there;
   const TreeNode node = tree_nodes(a, z, seq.length, lane, there);
   if (seq.end == 0) there = 0;
@@ -126,26 +176,8 @@ void tree_rows_kernel(const TreeArgs a) {
   const bool row_ok = col < nrows;
   const int pr = r0 + (row_ok ? col : nrows - 1);
   const int token = pr / group, h = hk * group + pr % group;
-  const uint64_t kin = shfl64(node.kin, token);
-  const int depth = __shfl(node.depth, token);
-  const bool alive = (there >> token & 1) != 0;
-  // of the filled slots [m_lo, length) and those below m_sink
-  const int m_lo = !alive ? 0x7fffffff : a.window > 0 ? seq.length + depth - a.window + 1 : 0;
-  const int m_sink = alive && a.window > 0 ? a.sinks : 0;
-
-  // blocks of 32 slots: the sinks' in front of the window's
-  int win_lo = 0, all_lo = 0;      // first slot that some row, that every row sees by its window
-  if (a.window > 0) {
-    win_lo = seq.length - a.window + 1 > 0 ? seq.length - a.window + 1 : 0;
-    all_lo = seq.length + a.tokens - a.window > 0 ? seq.length + a.tokens - a.window : 0;
-  }
-  const int last = seq.end > 0 ? (seq.end - 1) / 32 : -1, first = win_lo / 32;
-  const int sinks = a.window > 0 ? a.sinks : 0;
-  const int front = sinks < first * 32 ? (sinks + 31) / 32 : first;
-  const int blocks = last >= first ? front + last - first + 1 : 0;
-  const int per = (blocks + a.splits - 1) / a.splits;
-  const int b0 = split * per, b1 = b0 + per < blocks ? b0 + per : blocks;
-  auto block_of = [&](int i) { return i < front ? i : first + i - front; };
+  const TreeRow row(a, seq, node, there, token);
+  const int b0 = part * a.part_blocks, b1 = b0 + a.part_blocks < range.blocks ? b0 + a.part_blocks : range.blocks;
 
   // ---- Q rows as the B operand (column = packed row), straight from global memory ----------------
   op_t qreg[KS];
@@ -212,14 +244,13 @@ void tree_rows_kernel(const TreeArgs a) {
   int i = b0 + wave;
   Halves now{-1, -1}, next{-1, -1};
   if (i < b1) {
-    now = halves_of(block_of(i));
-    load_block(block_of(i), now);
-    if (i + 4 < b1) next = halves_of(block_of(i + 4));
+    now = halves_of(range.block_of(i));
+    load_block(range.block_of(i), now);
+    if (i + 4 < b1) next = halves_of(range.block_of(i + 4));
   }
   for (; i < b1; i += 4) {
-    const int n0 = block_of(i) * 32;
-    // a block that some row does not see whole
-    const bool edge = n0 + 32 > seq.length || (n0 < all_lo && n0 + 32 > sinks) || now.p0 < 0 || now.p1 < 0;
+    const int n0 = range.block_of(i) * 32;
+    const bool edge = !range.whole(seq, n0, 32) || now.p0 < 0 || now.p1 < 0;
     f32x16 s;
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0.f;
@@ -230,9 +261,7 @@ void tree_rows_kernel(const TreeArgs a) {
       // token that is not there) may be inf or NaN
 #pragma unroll
       for (int e = 0; e < CHV; ++e) {
-        const int n = n0 + vr0 + e * RPI, j = n - seq.length;
-        const bool seen = n < seq.length ? (n >= win_lo || n < sinks) : j < 64 && (there >> (j & 63) & 1) != 0;
-        if (!seen || (e * RPI < 16 ? now.p0 : now.p1) < 0) vreg[e] = op_t{};
+        if (!range.seen(seq, there, n0 + vr0 + e * RPI) || (e * RPI < 16 ? now.p0 : now.p1) < 0) vreg[e] = op_t{};
       }
     }
 #pragma unroll
@@ -240,8 +269,8 @@ void tree_rows_kernel(const TreeArgs a) {
     const Halves was = now;
     if (i + 4 < b1) {
       now = next;
-      load_block(block_of(i + 4), now);
-      if (i + 8 < b1) next = halves_of(block_of(i + 8));
+      load_block(range.block_of(i + 4), now);
+      if (i + 8 < b1) next = halves_of(range.block_of(i + 8));
     }
 
     if (prescale)
@@ -250,9 +279,7 @@ void tree_rows_kernel(const TreeArgs a) {
     if (edge) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int n = n0 + 8 * (e / 4) + 4 * hi + (e % 4), j = n - seq.length;
-        const bool seen = (n < seq.length ? (n >= m_lo || n < m_sink) : j < 64 && (kin >> (j & 63) & 1) != 0) && alive &&
-                          (e < 8 ? was.p0 : was.p1) >= 0;
+        const bool seen = row.sees(seq, n0 + 8 * (e / 4) + 4 * hi + (e % 4)) && (e < 8 ? was.p0 : was.p1) >= 0;
         s[e] = seen ? s[e] : -__builtin_inff();
       }
     }
@@ -289,7 +316,7 @@ void tree_rows_kernel(const TreeArgs a) {
 
   // ---- the four waves' partial results meet in LDS --------------------------------------------
   // (a token that is not there is masked in edge blocks only; it ends without a sum, and what it summed is not looked at)
-  const float l = alive ? cross_sum(l_i) : 0.f;
+  const float l = row.alive ? cross_sum(l_i) : 0.f;
   __syncthreads();      // the V areas become the O areas
   float* ml = reinterpret_cast<float*>(smem_raw + SM::ML_OFF);
   float* ow = reinterpret_cast<float*>(smem_raw + wave * SM::O_BYTES);
@@ -320,12 +347,12 @@ void tree_rows_kernel(const TreeArgs a) {
       lsum += f * ml[(v * 32 + r) * 2 + 1];
       acc += f * *reinterpret_cast<const f32x4*>(smem_raw + v * SM::O_BYTES + (r * OSTR + at) * 4);
     }
-    if (a.splits > 1) {
-      const int64_t part = ((int64_t)(pair * a.row_blocks + rb) * a.splits + split) * a.part_rows + r;
-      *reinterpret_cast<f32x4*>(a.part_o + part * D + at) = acc;
+    if (parts > 1) {
+      const int64_t to = ((int64_t)(pair * a.row_blocks + rb) * a.parts + part) * a.part_rows + r;
+      *reinterpret_cast<f32x4*>(a.part_o + to * D + at) = acc;
       if (at == 0) {
-        a.part_ml[part * 2] = m;
-        a.part_ml[part * 2 + 1] = lsum;
+        a.part_ml[to * 2] = m;
+        a.part_ml[to * 2 + 1] = lsum;
       }
     } else {
       const int pq = (r0 + r) / group, ph = hk * group + (r0 + r) % group;
@@ -341,6 +368,103 @@ void tree_rows_kernel(const TreeArgs a) {
   }
 }
 
+// ---- the parts' sums: out = sum_i 2^((m_i - m) sc) O_i / sum_i 2^((m_i - m) sc) l_i ------------------------------------------------
+// A thread takes four columns of a row, and of its parts every kSlots-th.  What bounds it is the latency of loads that miss L2 (other
+// XCDs wrote them): with many parts of few rows the threads of a workgroup hold all parts of a row between them.
+template <typename T, int D, int kSlots>
+static __global__ __launch_bounds__(256) void tree_sum_kernel(const TreeArgs a) {
+  constexpr int TPR = D / 4, ROWS = 256 / TPR / kSlots, AHEAD = 4;
+  __shared__ f32x4 s_acc[kSlots > 1 ? 256 : 1];
+  __shared__ float s_m[kSlots > 1 ? 256 / TPR : 1], s_l[kSlots > 1 ? 256 / TPR : 1];
+  const CacheArgs& c = a.cache;
+  const int chunks = (a.part_rows + ROWS - 1) / ROWS;
+  const int block = blockIdx.x / chunks, pair = block / a.row_blocks, rb = block % a.row_blocks;
+  const int z = pair / c.heads, hk = pair % c.heads, group = a.hq / c.heads;
+  const TreeSeq seq = tree_seq(a, z);
+  const int parts = TreeBlocks(a, seq).parts(a);
+  if (parts <= 1) return;                              // (the whole workgroup: its results are there already)
+  const int lane_row = threadIdx.x / TPR / kSlots, slot = threadIdx.x / TPR % kSlots, col = threadIdx.x % TPR * 4;
+  const int r = blockIdx.x % chunks * ROWS + lane_row, pr = rb * a.row_rows + r;
+  const bool ok = r < a.part_rows && pr < a.tokens * group;
+  const float sc = score_scale(a.sm_scale, false);
+  const int64_t at = (int64_t)block * a.parts * a.part_rows + (ok ? r : 0);
+  const float* po = a.part_o + at * D + col;
+  const float* pm = a.part_ml + at * 2;
+  float m = kNegBig, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = slot; i0 < parts; i0 += kSlots * AHEAD) {
+    f32x4 x[AHEAD];
+    vec<float, 2> ml[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = i0 + k * kSlots < parts ? i0 + k * kSlots : i0;
+      ml[k] = *reinterpret_cast<const vec<float, 2>*>(pm + (int64_t)i * a.part_rows * 2);
+      x[k] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(po + (int64_t)i * a.part_rows * D));
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (i0 + k * kSlots >= parts) ml[k][1] = 0.f;
+      if (ml[k][1] != 0.f) top = fmaxf(top, ml[k][0]);
+    }
+    const float f0 = fast_exp2((m - top) * sc);
+    acc *= f0;
+    l *= f0;
+    m = top;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (ml[k][1] != 0.f) {                           // (a part in which the row sees nothing has sums of nothing)
+        const float f = fast_exp2((ml[k][0] - m) * sc);
+        l += f * ml[k][1];
+        acc += f * x[k];
+      }
+  }
+  if (kSlots > 1) {
+    s_acc[threadIdx.x] = acc;
+    if (col == 0) { s_m[threadIdx.x / TPR] = m; s_l[threadIdx.x / TPR] = l; }
+    __syncthreads();
+    if (slot != 0) return;
+    float top = m;
+#pragma unroll
+    for (int k = 1; k < kSlots; ++k) top = fmaxf(top, s_m[lane_row * kSlots + k]);
+    const float f0 = fast_exp2((m - top) * sc);
+    acc *= f0;
+    l *= f0;
+#pragma unroll
+    for (int k = 1; k < kSlots; ++k) {
+      const float f = fast_exp2((s_m[lane_row * kSlots + k] - top) * sc);
+      l += f * s_l[lane_row * kSlots + k];
+      acc += f * s_acc[threadIdx.x + k * TPR];
+    }
+    m = top;
+  }
+  if (!ok) return;
+  const int token = pr / group, h = hk * group + pr % group;
+  if (col < c.head_dim_v) {
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    vec<T, 4> t;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = Traits<T>::cvt(acc[j] * inv);
+    *reinterpret_cast<vec<T, 4>*>(reinterpret_cast<T*>(a.out) + (int64_t)z * a.so.z + (int64_t)h * a.so.h + (int64_t)token * a.so.s + col) = t;
+  }
+  if (a.lse && col == 0) a.lse[((int64_t)z * a.hq + h) * a.tokens + token] = lse_of(m, sc, l);
+}
+
+template <typename T, int D, int kSlots>
+hipError_t launch_tree_sum_slots(const TreeArgs& a, hipStream_t stream) {
+  constexpr int ROWS = 256 / (D / 4) / kSlots;
+  const unsigned blocks = (unsigned)(a.cache.sequences * a.cache.heads * a.row_blocks);
+  hipLaunchKernelGGL((tree_sum_kernel<T, D, kSlots>), dim3(blocks * ((a.part_rows + ROWS - 1) / ROWS)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+// Slots of a row: as many as halve the rounds of loads while the rows alone leave the chip empty.
+template <typename T, int D>
+hipError_t launch_tree_sum(const TreeArgs& a, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.cache.sequences * a.cache.heads * a.row_blocks * a.part_rows;
+  if (a.parts <= 4 || rows > 4096) return launch_tree_sum_slots<T, D, 1>(a, stream);
+  return launch_tree_sum_slots<T, D, 256 / (D / 4)>(a, stream);
+}
+
 template <typename T, int D, bool kPad>
 hipError_t launch_tree_rows(const TreeArgs& a, hipStream_t stream) {
   auto kern = tree_rows_kernel<T, D, kPad>;
@@ -351,22 +475,11 @@ hipError_t launch_tree_rows(const TreeArgs& a, hipStream_t stream) {
     if (e != hipSuccess) return e;
   }
   const int pairs = a.cache.sequences * a.cache.heads;
-  const int units = (pairs * a.splits + kNumXcd - 1) / kNumXcd;
+  const int units = (pairs * a.parts + kNumXcd - 1) / kNumXcd;
   if (units == 0 || a.row_blocks == 0) return hipSuccess;
   hipLaunchKernelGGL(kern, dim3((unsigned)(kNumXcd * units * a.row_blocks)), dim3(256), smem, stream, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits <= 1) return e;
-  FwdArgs f{};
-  f.out = a.out; f.lse = a.lse; f.so = a.so;
-  f.batch = a.cache.sequences; f.hq = a.hq; f.hk = a.cache.heads;
-  f.head_dim = a.cache.head_dim; f.head_dim_v = a.cache.head_dim_v;
-  f.sm_scale = a.sm_scale;
-  f.seq.max_seqlen_q = a.tokens;
-  f.num_zh = a.cache.sequences * a.hq;
-  f.splits = a.splits; f.row_blocks = a.row_blocks; f.part_rows = a.part_rows;
-  f.part_group = a.hq / a.cache.heads; f.part_block = 32;
-  f.part_o = a.part_o; f.part_ml = a.part_ml;
-  return launch_combine_rows<T, D>(f, pairs, stream);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || a.parts <= 1 ? e : launch_tree_sum<T, D>(a, stream);
 }
 
 }  // namespace fa

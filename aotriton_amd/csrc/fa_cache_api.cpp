@@ -117,23 +117,36 @@ int check_cache(const fa_cache* p, fa::CacheArgs* out) {
 // a launch's workgroups have to fit 31 bits
 bool fits(double workgroups) { return workgroups < 2147483648.0; }
 
-// Parts of the keys, and the scratch for their sums.  Two workgroups run on a CU (one above 128 columns), each with four waves that take
-// blocks of 32 slots in turn: as many parts as fill the chip, of at least one round of the waves.
-struct TreePlan { int row_blocks, part_rows, splits; int64_t o_bytes, bytes; };
-TreePlan tree_plan(const fa::TreeArgs& a, int64_t max_length, int num_cu) {
+// Blocks of 32 slots per part, and the scratch for the parts' sums.  Two workgroups run on a CU (one above 128 columns), each with
+// four waves that take the blocks in turn.  `kRounds` rounds of workgroups if all sequences had max_length, so that those of different
+// lengths even out; at least two blocks per wave, and at most kMaxParts parts.
+struct TreePlan { int64_t o_bytes, bytes; };
+constexpr int kMaxParts = 256, kRounds = 4;
+constexpr int64_t kMostScratch = 256 << 20;
+TreePlan tree_plan(fa::TreeArgs* a, int64_t max_length, int num_cu) {
   TreePlan p{};
-  const int d = fa::compiled_columns(a.cache);
-  const int64_t rows = (int64_t)a.tokens * (a.hq / a.cache.heads);
-  p.row_blocks = (int)((rows + 31) / 32);
-  p.part_rows = (int)(rows < 32 ? rows : 32);
-  int64_t slots = max_length + a.tokens;
-  if (a.window > 0) slots = std::min<int64_t>(slots, (int64_t)a.window + a.tokens + std::min<int64_t>(a.sinks, max_length) + 32);
-  const int64_t blocks = (slots + 31) / 32, items = (int64_t)a.cache.sequences * a.cache.heads * p.row_blocks;
-  const int64_t slots_of_chip = (int64_t)(d > 128 ? 1 : 2) * num_cu;
-  int64_t splits = items > 0 ? slots_of_chip / items : 1;
-  splits = std::min<int64_t>(splits, std::min<int64_t>((blocks + 3) / 4, 64));
-  p.splits = (int)std::max<int64_t>(1, splits);
-  const int64_t stored = items * p.splits * p.part_rows;
+  const int d = fa::compiled_columns(a->cache);
+  const int64_t rows = (int64_t)a->tokens * (a->hq / a->cache.heads);
+  a->row_rows = 32;
+  a->row_blocks = (int)((rows + 31) / 32);
+  a->part_rows = (int)(rows < 32 ? rows : 32);
+  // (the blocks that a sequence of that length has, and the most that any may have)
+  auto blocks_of = [&](int64_t length) {
+    int64_t slots = length + a->tokens;
+    if (a->window > 0) slots = std::min<int64_t>(slots, (int64_t)a->window + a->tokens + std::min<int64_t>(a->sinks, length) + 96);
+    return (slots + 31) / 32;
+  };
+  const int64_t room = (int64_t)a->cache.columns << a->cache.page_shift;
+  const int64_t blocks = blocks_of(max_length), most = blocks_of(room), items = (int64_t)a->cache.sequences * a->cache.heads * a->row_blocks;
+  const int64_t chip = (int64_t)(d > 128 ? 1 : 2) * num_cu * kRounds;
+  int64_t per = std::max<int64_t>(8, (blocks * items + chip - 1) / chip);
+  per = std::max(per, (most + kMaxParts - 1) / kMaxParts);
+  // (a table with room for far more than max_length: parts that no sequence may come to have take scratch as well)
+  const int64_t part_bytes = items * a->part_rows * (d * 4 + 8);
+  if (part_bytes > 0) per = std::max(per, (most * part_bytes + kMostScratch - 1) / kMostScratch);
+  a->part_blocks = (int)per;
+  a->parts = (int)std::max<int64_t>(1, (most + per - 1) / per);
+  const int64_t stored = a->parts > 1 ? items * a->parts * a->part_rows : 0;
   p.o_bytes = stored * d * 4;
   p.bytes = p.o_bytes + stored * 8;
   return p;
@@ -179,16 +192,17 @@ int fa_tree_attn(const fa_tree_params* p, void* hip_stream, fa_allocator* alloc)
   a.window = std::min(p->window, 1 << 30);
   a.sinks = std::min(p->sinks, 1 << 30);
   const int64_t room = (int64_t)c.columns << c.page_shift;
-  const TreePlan plan = tree_plan(a, std::min<int64_t>(p->max_length, room), fa_get_multiprocessor_count(hip_stream));
-  a.row_blocks = plan.row_blocks; a.part_rows = plan.part_rows;
-  a.splits = 1;
-  if (!fits(((double)c.sequences * c.heads * plan.splits + 8) * plan.row_blocks)) return FA_ERROR_NOT_SUPPORTED;
-  if (plan.splits > 1 && alloc != nullptr)
-    if (void* scratch = alloc->alloc(alloc, (uint64_t)plan.bytes)) {
-      a.splits = plan.splits;
-      a.part_o = static_cast<float*>(scratch);
-      a.part_ml = reinterpret_cast<float*>(static_cast<char*>(scratch) + plan.o_bytes);
+  const TreePlan plan = tree_plan(&a, std::min<int64_t>(p->max_length, room), fa_get_multiprocessor_count(hip_stream));
+  if (a.parts > 1) {
+    void* scratch = alloc != nullptr ? alloc->alloc(alloc, (uint64_t)plan.bytes) : nullptr;
+    a.part_o = static_cast<float*>(scratch);
+    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(scratch) + plan.o_bytes);
+    if (scratch == nullptr) {
+      a.parts = 1;
+      a.part_blocks = 0x7fffffff;
     }
+  }
+  if (!fits(((double)c.sequences * c.heads * a.parts + 8) * a.row_blocks)) return FA_ERROR_NOT_SUPPORTED;
   return (int)fa::run_tree(dtype, a, static_cast<hipStream_t>(hip_stream));
 }
 

@@ -31,8 +31,11 @@ struct TreeArgs {
   int32_t hq, tokens;
   float sm_scale;
   int32_t window, sinks;         // window 0: none
-  int32_t splits, row_blocks, part_rows;
-  float* part_o; float* part_ml; // as FwdArgs has them
+  // A workgroup takes `part_blocks` blocks of 32 slots for row_rows packed rows; a sequence has as many parts as its length needs, at
+  // most `parts`.  The sums of a sequence with one part only are its results; those of the others lie in part_o as (pair,
+  // block of rows, part, row of the block, compiled columns) and, maximum and row sum, in part_ml.
+  int32_t parts, part_blocks, row_blocks, row_rows, part_rows;      // part_rows: stored per block
+  float* part_o; float* part_ml;
 };
 
 struct AppendArgs {

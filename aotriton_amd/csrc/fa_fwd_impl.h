@@ -41,11 +41,11 @@ struct FwdSmem {
 // One Q tile (BM rows of head h of sequence z) against all its visible K/V tiles, or with kSplit
 // against part `split` of a.splits of them: the fp32 sums and the row statistics of the part then go to
 // scratch memory, where combine_rows_kernel picks them up.
-// kSinks: a window of FwdArgs::window keys up to the query's position and the first FwdArgs::sinks keys.  The item's tiles are then
+// kSinks: a window up to the query's position and the first keys (SinkFwdArgs).  The item's tiles are then
 // the `front` ones that only the first keys are visible in, and those of the window, as one run of tiles with a jump in it.
 template <typename T, int D, int NW, int BN, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kSplit, bool kKeyBias,
           bool kAnyRow, bool kSinks>
-__device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const int h, const int mt, const int split,
+__device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z, const int h, const int mt, const int split,
                                          char* smem_raw) {
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
@@ -76,7 +76,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
   if (q0 >= si.seqlen_q) return;
 
   Window w{0, 0};
-  if (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);
+  if constexpr (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);
   else if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right,
                                   si.seqlen_q, si.seqlen_k);
   // keep row +/- window inside int32
@@ -90,7 +90,9 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
   }
   // (a key before the window's first tile is no later than the item's first query, so that all its rows see it if it is a sink)
   static_assert(!kSinks || (kWindowed && !kBias && !kDropout && !kSplit && D <= 128), "a window with sinks and nothing else");
-  const int front = kSinks ? (a.sinks < br.lo * BN ? (a.sinks + BN - 1) / BN : br.lo) : 0;
+  int sinks = 0;
+  if constexpr (kSinks) sinks = a.sinks;
+  const int front = kSinks ? (sinks < br.lo * BN ? (sinks + BN - 1) / BN : br.lo) : 0;
 
   const int hk = h / (a.hq / a.hk);                       // fwd_kernel.py:360
   const int row = q0 + wave * 32 + c;                     // this lane's query row
@@ -299,7 +301,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
   auto wave_sees_all = [&](int j) -> bool {
     const int n_first = j * BN, n_last = j * BN + BN - 1;
     bool all = n_last < si.seqlen_k;
-    if (kWindowed) all = all && n_last <= w_rmin + w.right && (n_first >= w_rmax - w.left || (kSinks && n_last < a.sinks));
+    if (kWindowed) all = all && n_last <= w_rmin + w.right && (n_first >= w_rmax - w.left || (kSinks && n_last < sinks));
     return all;
   };
   // visible columns of this lane's row as one range [m_lo, m_lo + m_rng] (empty: m_rng < 0)
@@ -310,7 +312,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgs& a, const int z, const in
   }
   const bool m_none = m_hi < m_lo;
   const unsigned m_rng = m_none ? 0u : (unsigned)(m_hi - m_lo);
-  const int m_sink = a.sinks < m_hi + 1 ? a.sinks : m_hi + 1;      // the row's sinks end here
+  const int m_sink = sinks < m_hi + 1 ? sinks : m_hi + 1;      // the row's sinks end here
 
   f32x16 s[MB];   // S^T of the current tile
 
@@ -740,7 +742,7 @@ template <typename T, int D, int NW, int BN, bool kPairs, bool kWindowed, bool k
           bool kKeyBias, bool kAnyRow = false, bool kSinks = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(NW * 64, NW * 64)))
 __attribute__((amdgpu_waves_per_eu(kFwdWaves<D, NW, BN>, kFwdWaves<D, NW, BN>)))
-void fwd_kernel(const FwdArgs a) {
+void fwd_kernel(const FwdArgsOf<kSinks> a) {
   extern __shared__ __attribute__((aligned(kPairs ? kSwzAlign : 16))) char smem_raw[];
   static_assert(!kPairs || __alignof__(smem_raw) >= kSwzAlign, "fwd_item_pair picks operands by exclusive or with addresses");
   if (kDropout && blockIdx.x == 0 && threadIdx.x == 0) {
@@ -837,7 +839,7 @@ struct FwdThirdTile : FwdTileOf<64, 4, 32> {};
 
 template <typename T, int D, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kSplit = false,
           bool kKeyBias = false, typename Tile = FwdTile<T, D, kWindowed>, bool kAnyRow = false, bool kSinks = false>
-hipError_t launch_fwd_variant(const FwdArgs& a, dim3 grid, hipStream_t stream) {
+hipError_t launch_fwd_variant(const FwdArgsOf<kSinks>& a, dim3 grid, hipStream_t stream) {
   constexpr int NW = Tile::NW;
   auto kern = fwd_kernel<T, D, NW, Tile::BN, Tile::kPairs, kWindowed, kBias, kDropout, kPad, kSplit, kKeyBias, kAnyRow, kSinks>;
   constexpr int smem = Tile::LDS;

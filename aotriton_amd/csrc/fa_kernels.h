@@ -109,9 +109,9 @@ TileShape f32_tile_shape(int head_dim, int kernel_slot);
     if (a.head_dim <= 96 && a.head_dim_v <= 96) return name##_d128_cols96(dtype, a, s);       \
     return (padded ? name##_d128_padded : name##_d128)(dtype, a, s);                          \
   }
-FA_DECL_SINKS(run_sinks_fwd, FwdArgs)
-FA_DECL_SINKS(run_sinks_dkdv, BwdArgs)
-FA_DECL_SINKS(run_sinks_dq, BwdArgs)
+FA_DECL_SINKS(run_sinks_fwd, SinkFwdArgs)
+FA_DECL_SINKS(run_sinks_dkdv, SinkBwdArgs)
+FA_DECL_SINKS(run_sinks_dq, SinkBwdArgs)
 #undef FA_DECL_SINKS
 
 // Vector-ALU kernels (no MFMA): every type at every compiled head dim; they serve tensors whose

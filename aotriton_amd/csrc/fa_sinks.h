@@ -33,7 +33,7 @@ struct SinkSmem {      // per wave: Q and dO rows; L and -delta.  The waves' sum
 
 template <typename T, int D, int kPad>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256))) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1)))
-void sink_dkdv_kernel(const BwdArgs a) {
+void sink_dkdv_kernel(const SinkBwdArgs a) {
   extern __shared__ __attribute__((aligned(kSwzAlign))) char smem_raw[];
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
@@ -197,7 +197,7 @@ void sink_dkdv_kernel(const BwdArgs a) {
 
 // Adds up the parts: four columns of a key's dK or dV per thread.
 template <typename T, int D>
-static __global__ __launch_bounds__(256) void sink_sum_kernel(const BwdArgs a) {
+static __global__ __launch_bounds__(256) void sink_sum_kernel(const SinkBwdArgs a) {
   constexpr int SUMS = SinkSmem<D>::SUM_BYTES / 16, PER = SUMS / 256;      // pieces of a key block, workgroups for them
   const int blocks = (a.sinks + 31) / 32;
   const int e = blockIdx.x % PER * 256 + threadIdx.x, block = blockIdx.x / PER % blocks, pair = blockIdx.x / PER / blocks;
@@ -221,9 +221,9 @@ static __global__ __launch_bounds__(256) void sink_sum_kernel(const BwdArgs a) {
 
 // ---- launchers ------------------------------------------------------------------------------------------------
 template <typename T, int D, int kPad>
-hipError_t launch_fwd_sinks(const FwdArgs& a, hipStream_t stream) {
+hipError_t launch_fwd_sinks(const SinkFwdArgs& a, hipStream_t stream) {
   const int half = a.half_tiles, BM = half ? 128 : FwdTile<T, D, true>::BM;
-  FwdArgs b = a;
+  SinkFwdArgs b = a;
   b.num_m_tiles = (a.seq.max_seqlen_q + BM - 1) / BM;
   const TileWork w = tile_work(nseq_of(a.seq, a.batch) * a.hq, q_head_group(a.hq, a.hk), b.num_m_tiles);
   b.num_zh = w.num_zh; b.zh_per_xcd = w.zh_per_xcd; b.zh_group = w.zh_group; b.items_per_xcd = w.items_per_xcd;
@@ -234,7 +234,7 @@ hipError_t launch_fwd_sinks(const FwdArgs& a, hipStream_t stream) {
 
 // dK and dV of the window's keys, and over them those of the sinks
 template <typename T, int D, int kPad>
-hipError_t launch_dkdv_sinks(const BwdArgs& a, hipStream_t stream) {
+hipError_t launch_dkdv_sinks(const SinkBwdArgs& a, hipStream_t stream) {
   hipError_t e = launch_dkdv_form<T, D, kPad, true, false, false, false, false, kBiasAny, true>(a, stream);
   const int pairs = bwd_nseq(a) * a.hk, blocks = (a.sinks + 31) / 32;
   if (e != hipSuccess || blocks == 0 || pairs == 0 || a.seq.max_seqlen_k <= 0) return e;

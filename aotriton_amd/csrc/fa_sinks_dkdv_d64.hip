@@ -12,7 +12,7 @@
 #endif
 
 namespace fa {
-hipError_t FA_RUN(int dtype, const BwdArgs& a, hipStream_t s) {
+hipError_t FA_RUN(int dtype, const SinkBwdArgs& a, hipStream_t s) {
   if (dtype == kDtypeBF16) return launch_dkdv_sinks<bf16_t, 64, FA_PADDED>(a, s);
   return launch_dkdv_sinks<f16_t, 64, FA_PADDED>(a, s);
 }

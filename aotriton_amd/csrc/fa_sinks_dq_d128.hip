@@ -14,7 +14,7 @@
 #endif
 
 namespace fa {
-hipError_t FA_RUN(int dtype, const BwdArgs& a, hipStream_t s) {
+hipError_t FA_RUN(int dtype, const SinkBwdArgs& a, hipStream_t s) {
   if (dtype == kDtypeBF16) return launch_dq_variant<bf16_t, 128, FA_PADDED, true, false, false, true>(a, s);
   return launch_dq_variant<f16_t, 128, FA_PADDED, true, false, false, true>(a, s);
 }
