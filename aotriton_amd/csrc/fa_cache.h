@@ -75,7 +75,7 @@ struct PageTable {
   }
 };
 
-// The blocks of 32 slots that a sequence's rows may see: those that hold sinks, then those of the window (without one: all).
+// The blocks of slots that a sequence's rows may see: those that hold sinks, then those of the window (without one: all).
 struct TreeBlocks {
   int win_lo, all_lo;            // first slot that some row, that every row sees by its window
   int sinks, first, front, blocks;
@@ -85,10 +85,10 @@ struct TreeBlocks {
       win_lo = seq.length - a.window + 1 > 0 ? seq.length - a.window + 1 : 0;
       all_lo = seq.length + a.tokens - a.window > 0 ? seq.length + a.tokens - a.window : 0;
     }
-    const int last = seq.end > 0 ? (seq.end - 1) / 32 : -1;
-    first = win_lo / 32;
+    const int shift = a.block_shift, last = seq.end > 0 ? (seq.end - 1) >> shift : -1;
+    first = win_lo >> shift;
     sinks = a.window > 0 ? a.sinks : 0;
-    front = sinks < first * 32 ? (sinks + 31) / 32 : first;
+    front = sinks < first << shift ? (sinks + (1 << shift) - 1) >> shift : first;
     blocks = last >= first ? front + last - first + 1 : 0;
   }
   __device__ __forceinline__ int block_of(int i) const { return i < front ? i : first + i - front; }
@@ -101,8 +101,103 @@ struct TreeBlocks {
     const int j = n - seq.length;
     return j < 0 ? (n >= win_lo || n < sinks) : j < 64 && (there >> (j & 63) & 1) != 0;
   }
-  __device__ __forceinline__ int parts(const TreeArgs& a) const { return blocks > a.part_blocks ? (blocks + a.part_blocks - 1) / a.part_blocks : 1; }
 };
+__device__ __forceinline__ int tree_blocks(const TreeArgs& a, int z) {      // in the list of all sequences' blocks: one at least
+  const int n = TreeBlocks(a, tree_seq(a, z)).blocks;
+  return n > 1 ? n : 1;
+}
+
+// The list of all sequences' blocks, and its cut into pieces.  Every lane of a wave takes part in the functions.
+struct TreeList {
+  int64_t per, total;            // blocks of a piece, of all
+  int z;                         // of seek
+  int64_t start;                 // of the sequence that cut or seek was asked for
+  int n, sum;                    // of the last 64 sequences that cut looked at: this lane's blocks, and the sum up to it
+  __device__ __forceinline__ void look(const TreeArgs& a, int base, int lane) {
+    n = base + lane < a.cache.sequences ? tree_blocks(a, base + lane) : 0;
+    sum = n;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+      const int y = __shfl_up(sum, i);
+      sum += lane >= i ? y : 0;
+    }
+  }
+  __device__ __forceinline__ void cut(const TreeArgs& a, int lane, int find) {      // find < 0: none
+    total = 0;
+    start = 0;
+    for (int base = 0; base < a.cache.sequences; base += 64) {
+      look(a, base, lane);
+      if (find >= base && find < base + 64) start = total + __builtin_amdgcn_readlane(sum - n, find - base);
+      total += __builtin_amdgcn_readlane(sum, 63);
+    }
+    const int64_t even = (total + a.workers - 1) / a.workers;
+    per = even > a.least ? even : a.least;
+  }
+  __device__ __forceinline__ void seek(const TreeArgs& a, int lane, int64_t at) {      // the sequence of block at < total
+    int64_t before = 0;
+    for (int base = 0; base < a.cache.sequences; base += 64) {
+      if (a.cache.sequences > 64) look(a, base, lane);
+      const int all = __builtin_amdgcn_readlane(sum, 63);
+      if (at < before + all) {
+        const int i = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + sum > at));
+        z = base + i;
+        start = before + __builtin_amdgcn_readlane(sum - n, i);
+        return;
+      }
+      before += all;
+    }
+  }
+};
+
+// First row of the sums of a sequence in one of its pieces.  Pieces of the list and their sequences ascend together, so that
+// piece + sequence names the pair.
+__device__ __forceinline__ int64_t tree_sums(const TreeArgs& a, int hk, int rb, int piece, int z) {
+  const int64_t block = hk * a.row_blocks + rb;
+  return (a.workers > 0 ? block * (a.workers + a.cache.sequences) + piece + z : (block * a.cache.sequences + z) * a.parts + piece) * a.part_rows;
+}
+
+// A workgroup's items: f(sequence, head, block of rows, first block, end, whether these are all of the sequence's, piece).
+template <typename F>
+__device__ __forceinline__ void tree_work(const TreeArgs& a, int lane, F f) {
+  // units go round the XCDs, the row blocks of one follow each other on one XCD
+  const int xcd = blockIdx.x % kNumXcd, idx = blockIdx.x / kNumXcd, heads = a.cache.heads;
+  const int unit = (idx / a.row_blocks) * kNumXcd + xcd, rb = idx % a.row_blocks;
+  const int hk = unit % heads;
+  int z, first, take, size, piece;
+  int64_t at = 0, end = 1;
+  TreeList list;
+  if (a.workers > 0) {
+    piece = unit / heads;
+    if (piece >= a.workers) return;
+    list.cut(a, lane, -1);
+    at = piece * list.per;
+    end = at + list.per < list.total ? at + list.per : list.total;
+    if (at >= end) return;
+    list.seek(a, lane, at);
+    z = list.z;
+  } else {
+    // (all sequences' first pieces in front: every sequence has one, the long ones have the others)
+    z = unit / heads % a.cache.sequences;
+    piece = unit / heads / a.cache.sequences;
+    if (piece >= a.parts) return;
+  }
+  for (;; ++z) {
+    size = tree_blocks(a, z);
+    if (a.workers > 0) {
+      first = (int)(at - list.start);
+      take = size - first < end - at ? size - first : (int)(end - at);
+    } else {
+      if (piece > 0 && piece >= (size + a.part_blocks - 1) / a.part_blocks) return;
+      first = piece * a.part_blocks;
+      take = size - first < a.part_blocks ? size - first : a.part_blocks;
+    }
+    f(z, hk, rb, first, first + take, take == size, piece);
+    at += take;
+    if (at >= end) return;
+    list.start += size;
+    __syncthreads();      // the next item reuses the LDS areas
+  }
+}
 
 // What a packed row sees.
 struct TreeRow {
@@ -123,44 +218,36 @@ struct TreeRow {
   }
 };
 
-// ---- few rows: 32 packed (token, q-head) rows of one K/V head x one part of its keys per workgroup -----------------------
+// ---- few rows: 32 packed (token, q-head) rows of one K/V head x one piece of the keys per workgroup -----------------------
 // As fwd_rows_kernel: the waves take blocks of 32 slots in turn, each with an online softmax of its own; they meet in LDS, the parts
 // in combine_rows_kernel.  K and V are read once per 32 rows, and what bounds it is HBM.  The blocks of an item are those that hold
 // sinks, then those of the window (without one: all).
 template <int D>
 struct TreeSmem {
-  static constexpr int VSTR = D + 32;                    // elements; transposing reads sweep all banks
-  static constexpr int V_BYTES = 32 * VSTR * 2;          // per wave
+  static constexpr int KSTR = D + 8;                     // elements; row reads sweep all banks
+  static constexpr int VSTR = D + 32;                    // the same for transposing reads
+  static constexpr int V_BYTES = 32 * VSTR * 2;          // per wave: a block's K, then its V
   static constexpr int OSTR = D + 4;                     // floats per row of a wave's partial O
   static constexpr int O_BYTES = 32 * OSTR * 4;          // per wave
   static constexpr int ML_OFF = 4 * (V_BYTES > O_BYTES ? V_BYTES : O_BYTES);
   static constexpr int BYTES = ML_OFF + 4 * 32 * 8;
 };
 
+// Blocks [from, to) of sequence z; `whole`: they are all of its blocks.
 template <typename T, int D, bool kPad>
-__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
-__attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1, D <= 128 ? 2 : 1)))
-void tree_rows_kernel(const TreeArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+__device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, const int hk, const int rb, const int from, const int to,
+                                               const bool whole, const int piece, char* smem_raw) {
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
   using q4_t = typename Tr::q4_t;
   using SM = TreeSmem<D>;
   constexpr int KS = D / 16, DB = D / 32;
-  constexpr int VSTR = SM::VSTR, OSTR = SM::OSTR;
-  constexpr int LPR = D / 8, RPI = 64 / LPR, CHV = 32 / RPI;      // V: lanes per row, rows per access, accesses
-
-  // units (pair, part) go round the XCDs, the row blocks of a unit follow each other on one
+  constexpr int KSTR = SM::KSTR, VSTR = SM::VSTR, OSTR = SM::OSTR;
+  constexpr int LPR = D / 8, RPI = 64 / LPR, CH = 32 / RPI;      // lanes per row, rows per access, accesses
   const CacheArgs& c = a.cache;
-  const int xcd = blockIdx.x % kNumXcd, idx = blockIdx.x / kNumXcd;
-  const int unit = (idx / a.row_blocks) * kNumXcd + xcd, rb = idx % a.row_blocks;
-  const int pair = unit / a.parts, part = unit % a.parts;
-  if (pair >= c.sequences * c.heads) return;
-  const int z = pair / c.heads, hk = pair % c.heads, group = a.hq / c.heads;
+  const int group = a.hq / c.heads;
   const TreeSeq seq = tree_seq(a, z);
   const TreeBlocks range(a, seq);
-  const int parts = range.parts(a);
-  if (part >= parts) return;
   const int rows = a.tokens * group, r0 = rb * 32;
   const int nrows = rows - r0 < 32 ? rows - r0 : 32;
 
@@ -177,7 +264,7 @@ void tree_rows_kernel(const TreeArgs a) {
   const int pr = r0 + (row_ok ? col : nrows - 1);
   const int token = pr / group, h = hk * group + pr % group;
   const TreeRow row(a, seq, node, there, token);
-  const int b0 = part * a.part_blocks, b1 = b0 + a.part_blocks < range.blocks ? b0 + a.part_blocks : range.blocks;
+  const int b1 = to < range.blocks ? to : range.blocks;
 
   // ---- Q rows as the B operand (column = packed row), straight from global memory ----------------
   op_t qreg[KS];
@@ -195,7 +282,7 @@ void tree_rows_kernel(const TreeArgs a) {
   const T* vbase = reinterpret_cast<const T*>(c.v) + (int64_t)hk * c.sv.h;
   const int slot_mask = (1 << c.page_shift) - 1;
   const int vr0 = lane / LPR, vc0 = lane % LPR;
-  const bool v_col = !kPad || vc0 * 8 < d_v;
+  const bool k_col = !kPad || vc0 * 8 < d_qk, v_col = !kPad || vc0 * 8 < d_v;
   // pages have 16 slots or more, so a block lies in two pages at most, 16 slots in one
   struct Halves { int p0, p1; };
   auto halves_of = [&](int b) {
@@ -204,32 +291,35 @@ void tree_rows_kernel(const TreeArgs a) {
     x.p1 = pages.page_of(b * 32 + 16);
     return x;
   };
-  op_t kreg[KS], vreg[CHV];
+  // K and V travel as whole rows, 16 bytes per lane and consecutive lanes along a row, and change to the operands' layouts in the wave's
+  // LDS area, one after the other.  (K loaded as the operand that it is, 16 bytes of 32 rows per access, takes its cache lines a quarter at
+  // a time: B64 Hq 32 Hk 8 up to 8192 slots D128 226 us instead of 193.)
+  op_t kreg[CH], vreg[CH];
+  const int64_t k_off = vr0 * c.sk.s + vc0 * 8, v_off = vr0 * c.sv.s + vc0 * 8;
   // (a page that is not there stands aside for page 0, whose values are not used)
-  auto load_block = [&](int b, Halves x) {
-    const int s0 = (b * 32) & slot_mask, s1 = (b * 32 + 16) & slot_mask;
-    const int64_t p0 = x.p0 < 0 ? 0 : x.p0, p1 = x.p1 < 0 ? 0 : x.p1;
-    const T* k0 = kbase + p0 * c.sk.z + s0 * c.sk.s;
-    const T* k1 = kbase + p1 * c.sk.z + s1 * c.sk.s;
-    const T* v0 = vbase + p0 * c.sv.z + s0 * c.sv.s;
-    const T* v1 = vbase + p1 * c.sv.z + s1 * c.sv.s;
-    const T* kp = (col < 16 ? k0 : k1) + (col & 15) * c.sk.s + 8 * hi;
+  auto load_k = [&](int b, Halves x) {
+    const T* p0 = kbase + (int64_t)(x.p0 < 0 ? 0 : x.p0) * c.sk.z + ((b * 32) & slot_mask) * c.sk.s;
+    const T* p1 = kbase + (int64_t)(x.p1 < 0 ? 0 : x.p1) * c.sk.z + ((b * 32 + 16) & slot_mask) * c.sk.s;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      kreg[ks] = op_t{};
-      if (!kPad || 16 * ks + 8 * hi < d_qk) kreg[ks] = *reinterpret_cast<const op_t*>(kp + 16 * ks);
+    for (int i = 0; i < CH; ++i) {
+      kreg[i] = op_t{};
+      if (k_col) kreg[i] = *reinterpret_cast<const op_t*>((i * RPI < 16 ? p0 : p1) + (i * RPI & 15) * c.sk.s + k_off);
     }
+  };
+  auto load_v = [&](int b, Halves x) {
+    const T* p0 = vbase + (int64_t)(x.p0 < 0 ? 0 : x.p0) * c.sv.z + ((b * 32) & slot_mask) * c.sv.s;
+    const T* p1 = vbase + (int64_t)(x.p1 < 0 ? 0 : x.p1) * c.sv.z + ((b * 32 + 16) & slot_mask) * c.sv.s;
 #pragma unroll
-    for (int i = 0; i < CHV; ++i) {
-      const int r = vr0 + i * RPI;
+    for (int i = 0; i < CH; ++i) {
       vreg[i] = op_t{};
-      if (v_col) vreg[i] = *reinterpret_cast<const op_t*>((i * RPI < 16 ? v0 : v1) + (r & 15) * c.sv.s + vc0 * 8);
+      if (v_col) vreg[i] = *reinterpret_cast<const op_t*>((i * RPI < 16 ? p0 : p1) + (i * RPI & 15) * c.sv.s + v_off);
     }
   };
 
-  T* vs = reinterpret_cast<T*>(smem_raw + wave * SM::V_BYTES);
-  const int v_st = vr0 * VSTR + vc0 * 8;
-  const T* v_ld = vs + (4 * hi + (lane & 15) / 4) * VSTR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);      // see lds_read_tr8
+  T* area = reinterpret_cast<T*>(smem_raw + wave * SM::V_BYTES);
+  const int k_st = vr0 * KSTR + vc0 * 8, v_st = vr0 * VSTR + vc0 * 8;
+  const T* k_ld = area + col * KSTR + 8 * hi;
+  const T* v_ld = area + (4 * hi + (lane & 15) / 4) * VSTR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);      // see lds_read_tr8
 
   f32x16 o[DB];
 #pragma unroll
@@ -241,35 +331,42 @@ void tree_rows_kernel(const TreeArgs a) {
   const float sc = score_scale(a.sm_scale, false);
   const bool prescale = !(qk_scale > 0.f);
 
-  int i = b0 + wave;
+  int i = from + wave;
   Halves now{-1, -1}, next{-1, -1};
   if (i < b1) {
     now = halves_of(range.block_of(i));
-    load_block(range.block_of(i), now);
+    load_k(range.block_of(i), now);
+    load_v(range.block_of(i), now);
     if (i + 4 < b1) next = halves_of(range.block_of(i + 4));
   }
   for (; i < b1; i += 4) {
     const int n0 = range.block_of(i) * 32;
     const bool edge = !range.whole(seq, n0, 32) || now.p0 < 0 || now.p1 < 0;
+    const Halves was = now;
+#pragma unroll
+    for (int e = 0; e < CH; ++e) *reinterpret_cast<op_t*>(area + k_st + e * RPI * KSTR) = kreg[e];
+    if (i + 4 < b1) load_k(range.block_of(i + 4), next);
+    op_t ka[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ka[ks] = *reinterpret_cast<const op_t*>(k_ld + 16 * ks);
     f32x16 s;
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = Tr::mfma(kreg[ks], qreg[ks], s);
+    for (int ks = 0; ks < KS; ++ks) s = Tr::mfma(ka[ks], qreg[ks], s);
     if (edge) {
       // V of slots that no row sees is 0: its probability is, and what lies there (a stale slot, a page of somebody else's, a drafted
       // token that is not there) may be inf or NaN
 #pragma unroll
-      for (int e = 0; e < CHV; ++e) {
-        if (!range.seen(seq, there, n0 + vr0 + e * RPI) || (e * RPI < 16 ? now.p0 : now.p1) < 0) vreg[e] = op_t{};
-      }
+      for (int e = 0; e < CH; ++e)
+        if (!range.seen(seq, there, n0 + vr0 + e * RPI) || (e * RPI < 16 ? was.p0 : was.p1) < 0) vreg[e] = op_t{};
     }
+    // (the area is the wave's own and its LDS operations run in order: K has been read)
 #pragma unroll
-    for (int e = 0; e < CHV; ++e) *reinterpret_cast<op_t*>(vs + v_st + e * RPI * VSTR) = vreg[e];
-    const Halves was = now;
+    for (int e = 0; e < CH; ++e) *reinterpret_cast<op_t*>(area + v_st + e * RPI * VSTR) = vreg[e];
     if (i + 4 < b1) {
       now = next;
-      load_block(range.block_of(i + 4), now);
+      load_v(range.block_of(i + 4), now);
       if (i + 8 < b1) next = halves_of(range.block_of(i + 8));
     }
 
@@ -347,12 +444,12 @@ void tree_rows_kernel(const TreeArgs a) {
       lsum += f * ml[(v * 32 + r) * 2 + 1];
       acc += f * *reinterpret_cast<const f32x4*>(smem_raw + v * SM::O_BYTES + (r * OSTR + at) * 4);
     }
-    if (parts > 1) {
-      const int64_t to = ((int64_t)(pair * a.row_blocks + rb) * a.parts + part) * a.part_rows + r;
-      *reinterpret_cast<f32x4*>(a.part_o + to * D + at) = acc;
+    if (!whole) {
+      const int64_t sums = tree_sums(a, hk, rb, piece, z) + r;
+      *reinterpret_cast<f32x4*>(a.part_o + sums * D + at) = acc;
       if (at == 0) {
-        a.part_ml[to * 2] = m;
-        a.part_ml[to * 2 + 1] = lsum;
+        a.part_ml[sums * 2] = m;
+        a.part_ml[sums * 2 + 1] = lsum;
       }
     } else {
       const int pq = (r0 + r) / group, ph = hk * group + (r0 + r) % group;
@@ -368,9 +465,324 @@ void tree_rows_kernel(const TreeArgs a) {
   }
 }
 
-// ---- the parts' sums: out = sum_i 2^((m_i - m) sc) O_i / sum_i 2^((m_i - m) sc) l_i ------------------------------------------------
-// A thread takes four columns of a row, and of its parts every kSlots-th.  What bounds it is the latency of loads that miss L2 (other
-// XCDs wrote them): with many parts of few rows the threads of a workgroup hold all parts of a row between them.
+template <typename T, int D, bool kPad>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256)))
+__attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1, D <= 128 ? 2 : 1)))
+void tree_rows_kernel(const TreeArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  tree_work(a, threadIdx.x & 63, [&](int z, int hk, int rb, int from, int to, bool whole, int piece) __attribute__((always_inline)) {
+    tree_rows_item<T, D, kPad>(a, z, hk, rb, from, to, whole, piece, smem_raw);
+  });
+}
+
+// ---- many rows: 32 * NW packed rows of one K/V head x one piece of the keys per workgroup ---------------------------------------
+// With 64 drafted tokens and grouped heads a K/V head has hundreds of packed rows.  The kernel above would read its K and V once per 32 of
+// them (from L2) and feed one MFMA operand with each piece; here a tile of 64 slots is staged in LDS once for all waves, which own
+// 32 rows each, as in fwd_item (the same layouts, double buffer and one barrier per tile).  Bound by HBM up to about
+// 128 rows, by the matrix pipe and the exponentials beyond.
+template <int D>
+struct TreeTileSmem {
+  static constexpr int KSTR = D + 8, VSTR = D + 32;
+  static constexpr int K_ELEMS = 64 * KSTR, V_ELEMS = 64 * VSTR;
+  static constexpr int BYTES = 2 * (K_ELEMS + V_ELEMS) * 2;
+};
+
+template <typename T, int D, int NW, bool kPad>
+__device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, const int hk, const int rb, const int from, const int to,
+                                               const bool whole, const int piece, char* smem_raw) {
+  using Tr = Traits<T>;
+  using op_t = typename Tr::op_t;
+  using q4_t = typename Tr::q4_t;
+  using SM = TreeTileSmem<D>;
+  constexpr int KS = D / 16, DB = D / 32, KSTR = SM::KSTR, VSTR = SM::VSTR;
+  constexpr int LPR = D / 8, RW = 64 / LPR, RPI = NW * RW, CH = 64 / RPI;      // lanes per row; rows per wave's access, per workgroup's; accesses
+  static_assert(16 % RW == 0 && (RPI % 16 == 0), "a wave's access lies in 16 slots");
+
+  const CacheArgs& c = a.cache;
+  const int group = a.hq / c.heads;
+  const TreeSeq seq = tree_seq(a, z);
+  const TreeBlocks range(a, seq);
+  const int rows = a.tokens * group;
+
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, col = lane & 31, hi = lane >> 5;
+  const int d_qk = kPad ? c.head_dim : D, d_v = kPad ? c.head_dim_v : D;
+  uint64_t there;
+  const TreeNode node = tree_nodes(a, z, seq.length, lane, there);
+  if (seq.end == 0) there = 0;
+
+  // this lane's packed row (waves past the last row only stage)
+  const int first_row = rb * a.row_rows + wave * 32;
+  const bool active = first_row < rows;
+  const bool row_ok = first_row + col < rows;
+  const int pr = row_ok ? first_row + col : rows - 1;
+  const int token = pr / group, h = hk * group + pr % group;
+  const TreeRow row(a, seq, node, there, token);
+  const int t0 = from, t1 = to < range.blocks ? to : range.blocks;
+
+  op_t qreg[KS];
+  {
+    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)z * a.sq.z + (int64_t)h * a.sq.h + (int64_t)token * a.sq.s + 8 * hi;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qreg[ks] = op_t{};
+      if (row_ok && (!kPad || 16 * ks + 8 * hi < d_qk)) qreg[ks] = *reinterpret_cast<const op_t*>(qp + 16 * ks);
+    }
+  }
+
+  const PageTable table(c, z);
+  const T* kbase = reinterpret_cast<const T*>(c.k) + (int64_t)hk * c.sk.h;
+  const T* vbase = reinterpret_cast<const T*>(c.v) + (int64_t)hk * c.sv.h;
+  const int slot_mask = (1 << c.page_shift) - 1;
+  const int rl = lane / LPR, cl = lane % LPR;      // the lane's row within a wave's access, and its piece
+  const bool k_col = !kPad || cl * 8 < d_qk, v_col = !kPad || cl * 8 < d_v;
+  const int64_t k_off = rl * c.sk.s + cl * 8, v_off = rl * c.sv.s + cl * 8;
+  struct Quarters { int p[4]; };      // pages of a tile's 16-slot quarters
+  auto pages_of = [&](int n0) {
+    Quarters x;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) x.p[g] = table.page_of(n0 + 16 * g);
+    return x;
+  };
+  // access i of this wave: rows row_of(i) .. + RW - 1 of the tile
+  auto row_of = [&](int i) { return wave * RW + i * RPI; };
+  auto page_at = [&](const Quarters& x, int i) {
+    const int g = row_of(i) / 16;
+    return g == 0 ? x.p[0] : g == 1 ? x.p[1] : g == 2 ? x.p[2] : x.p[3];
+  };
+  op_t kreg[CH], vreg[CH];
+  auto load_tile = [&](int n0, const Quarters& x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int p = page_at(x, i), slot = (n0 + row_of(i)) & slot_mask;
+      const int64_t page = p < 0 ? 0 : p;      // (not there: page 0 stands aside for it)
+      kreg[i] = op_t{};
+      vreg[i] = op_t{};
+      if (k_col) kreg[i] = *reinterpret_cast<const op_t*>(kbase + page * c.sk.z + slot * c.sk.s + k_off);
+      if (v_col) vreg[i] = *reinterpret_cast<const op_t*>(vbase + page * c.sv.z + slot * c.sv.s + v_off);
+    }
+  };
+  T* const Ks = reinterpret_cast<T*>(smem_raw);
+  T* const Vs = Ks + 2 * SM::K_ELEMS;
+  auto is_edge = [&](int n0, const Quarters& x) {
+    return !range.whole(seq, n0, 64) || (x.p[0] | x.p[1] | x.p[2] | x.p[3]) < 0;
+  };
+  auto store_tile = [&](int stage, int n0, const Quarters& x) __attribute__((always_inline)) {
+    if (is_edge(n0, x)) {
+      // (V of slots that no row sees is 0, as above)
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        if (!range.seen(seq, there, n0 + row_of(i) + rl) || page_at(x, i) < 0) vreg[i] = op_t{};
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      *reinterpret_cast<op_t*>(Ks + stage * SM::K_ELEMS + (row_of(i) + rl) * KSTR + cl * 8) = kreg[i];
+      *reinterpret_cast<op_t*>(Vs + stage * SM::V_ELEMS + (row_of(i) + rl) * VSTR + cl * 8) = vreg[i];
+    }
+  };
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
+  float m_i = kNegBig, l_i = 0.f;
+  const float qk_scale = a.sm_scale * kLog2e;
+  const float sc = score_scale(a.sm_scale, false);
+  const bool prescale = !(qk_scale > 0.f);
+  const int v_lane = (4 * hi + (lane & 15) / 4) * VSTR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);      // see lds_read_tr8
+
+  auto slot_of = [&](int t) { return range.block_of(t) * 64; };
+  // S^T = K Q^T with the operands read two k-steps ahead of their MFMAs; V's first operands are in flight while the softmax runs; the
+  // exponentials are taken against the maximum that the rows have already, and a tile whose row sums tell that it does not do
+  // goes through the full step: all as in fwd_item.
+  f32x16 s[2];
+  op_t va[2][DB];
+  auto qk = [&](int stage) __attribute__((always_inline)) {
+    const T* ks = Ks + stage * SM::K_ELEMS + col * KSTR + 8 * hi;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[mb][e] = 0.f;
+    __builtin_amdgcn_s_setprio(2);
+    constexpr int kAhead = 2;
+    op_t ka[kAhead + 1][2];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) ka[k][mb] = *reinterpret_cast<const op_t*>(ks + mb * 32 * KSTR + 16 * k);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      if (k + kAhead < KS)
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+          ka[(k + kAhead) % (kAhead + 1)][mb] = *reinterpret_cast<const op_t*>(ks + mb * 32 * KSTR + 16 * (k + kAhead));
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) s[mb] = Tr::mfma(ka[k % (kAhead + 1)][mb], qreg[k], s[mb]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto prepare = [&](int stage, int n0, const Quarters& x, bool edge) __attribute__((always_inline)) {
+    const T* vs = Vs + stage * SM::V_ELEMS + v_lane;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) va[0][db] = lds_read_tr8<T>(vs + db * 32, VSTR);
+    if (prescale) {
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[mb][e] *= qk_scale;
+    }
+    if (edge) {
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const bool seen = row.sees(seq, n0 + 32 * mb + 8 * (e / 4) + 4 * hi + (e % 4)) && x.p[2 * mb + e / 8] >= 0;
+          s[mb][e] = seen ? s[mb][e] : -__builtin_inff();
+        }
+    }
+  };
+  auto finish = [&](int stage) __attribute__((always_inline)) {
+    const T* vs = Vs + stage * SM::V_ELEMS + v_lane;
+    op_t pb[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) pb[k] = pack8<T>(s[k / 2], k % 2);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(2);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k + 1 < 4)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) va[(k + 1) & 1][db] = lds_read_tr8<T>(vs + (k + 1) * 16 * VSTR + db * 32, VSTR);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = Tr::mfma(va[k & 1][db], pb[k], o[db]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  bool have_ref = false;      // every row of the wave has a usable maximum
+  float msc = 0.f;            // m_i * sc
+  auto fast_step = [&](int stage, int n0, const Quarters& x, bool edge) __attribute__((always_inline)) {
+    prepare(stage, n0, x, edge);
+    float rs = 0.f;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[mb][e] = fast_exp2(__builtin_fmaf(s[mb][e], sc, -msc));
+        rs += s[mb][e];
+      }
+    if (__builtin_amdgcn_ballot_w64(!(rs < 4096.f)) != 0) return false;      // also inf and NaN
+    l_i += rs;
+    finish(stage);
+    return true;
+  };
+  auto full_step = [&](int stage, int n0, const Quarters& x, bool edge) __attribute__((always_inline)) {
+    prepare(stage, n0, x, edge);
+    float mx = s[0][0];
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[mb][e]);
+    mx = cross_max(mx);
+    const float m_cand = fmaxf(m_i, mx);
+    const bool upd = (m_cand - m_i) * sc > 8.0f;
+    const float m_new = upd ? m_cand : m_i;
+    const float alpha = fast_exp2((m_i - m_new) * sc);
+    m_i = m_new;
+    msc = m_new * sc;
+    // (a row that has seen nothing yet keeps the seed, and with it the wave the full step)
+    have_ref = __builtin_amdgcn_ballot_w64(!(__builtin_fabsf(msc) < 1024.f)) == 0;
+    float rs = 0.f;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[mb][e] = fast_exp2((s[mb][e] - m_new) * sc);
+        rs += s[mb][e];
+      }
+    l_i = l_i * alpha + rs;
+    if (__builtin_amdgcn_ballot_w64(upd) != 0) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+    }
+    finish(stage);
+  };
+
+  Quarters now{}, next{};      // pages of the tile that is worked on; of the next one to be asked for
+  if (t0 < t1) {
+    now = pages_of(slot_of(t0));
+    load_tile(slot_of(t0), now);
+    if (t0 + 1 < t1) next = pages_of(slot_of(t0 + 1));
+    store_tile(0, slot_of(t0), now);
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int stage = (t - t0) & 1, n0 = slot_of(t);
+    const Quarters was = now;
+    if (t + 1 < t1) {
+      now = next;
+      load_tile(slot_of(t + 1), now);
+      if (t + 2 < t1) next = pages_of(slot_of(t + 2));
+    }
+    if (active) {
+      const bool edge = is_edge(n0, was);
+      qk(stage);
+      if (!(have_ref && fast_step(stage, n0, was, edge))) {
+        if (have_ref) qk(stage);      // (the scores are spent)
+        full_step(stage, n0, was, edge);
+      }
+    }
+    if (t + 1 < t1) store_tile(stage ^ 1, slot_of(t + 1), now);
+    __syncthreads();
+  }
+
+  if (!active) return;
+  const float l = row.alive ? cross_sum(l_i) : 0.f;
+  if (!row_ok) return;
+  if (!whole) {
+    const int64_t sums = tree_sums(a, hk, rb, piece, z) + wave * 32 + col;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(a.part_o + sums * D + 32 * db + 8 * g + 4 * hi) = f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+    if (hi == 0) {
+      a.part_ml[sums * 2] = m_i;
+      a.part_ml[sums * 2 + 1] = l;
+    }
+    return;
+  }
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  T* op = reinterpret_cast<T*>(a.out) + (int64_t)z * a.so.z + (int64_t)h * a.so.h + (int64_t)token * a.so.s;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      q4_t t4;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) t4[x] = Tr::cvt(l > 0.f ? o[db][4 * g + x] * inv : 0.f);
+      const int at = 32 * db + 8 * g + 4 * hi;
+      if (!kPad || at < d_v) *reinterpret_cast<q4_t*>(op + at) = t4;
+    }
+  if (a.lse && hi == 0) a.lse[((int64_t)z * a.hq + h) * a.tokens + token] = lse_of(m_i, sc, l);
+}
+
+template <typename T, int D, int NW, bool kPad>
+__global__ __attribute__((amdgpu_flat_work_group_size(NW * 64, NW * 64))) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void tree_tile_kernel(const TreeArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  tree_work(a, threadIdx.x & 63, [&](int z, int hk, int rb, int from, int to, bool whole, int piece) __attribute__((always_inline)) {
+    tree_tile_item<T, D, NW, kPad>(a, z, hk, rb, from, to, whole, piece, smem_raw);
+  });
+}
+
+// ---- the pieces' sums: out = sum_i 2^((m_i - m) sc) O_i / sum_i 2^((m_i - m) sc) l_i -----------------------------------------------
+// A thread takes four columns of a row, and of its pieces every kSlots-th.  What bounds it is the latency of loads that miss L2 (other
+// XCDs wrote them): with many pieces of few rows the threads of a workgroup hold all of a row's between them.
 template <typename T, int D, int kSlots>
 static __global__ __launch_bounds__(256) void tree_sum_kernel(const TreeArgs a) {
   constexpr int TPR = D / 4, ROWS = 256 / TPR / kSlots, AHEAD = 4;
@@ -378,16 +790,24 @@ static __global__ __launch_bounds__(256) void tree_sum_kernel(const TreeArgs a) 
   __shared__ float s_m[kSlots > 1 ? 256 / TPR : 1], s_l[kSlots > 1 ? 256 / TPR : 1];
   const CacheArgs& c = a.cache;
   const int chunks = (a.part_rows + ROWS - 1) / ROWS;
-  const int block = blockIdx.x / chunks, pair = block / a.row_blocks, rb = block % a.row_blocks;
-  const int z = pair / c.heads, hk = pair % c.heads, group = a.hq / c.heads;
-  const TreeSeq seq = tree_seq(a, z);
-  const int parts = TreeBlocks(a, seq).parts(a);
+  const int block = blockIdx.x / chunks, rb = block % a.row_blocks, hk = block / a.row_blocks % c.heads, z = block / a.row_blocks / c.heads;
+  const int group = a.hq / c.heads;
+  const int size = tree_blocks(a, z);
+  int p0 = 0, parts;
+  if (a.workers > 0) {
+    TreeList list;
+    list.cut(a, threadIdx.x & 63, z);
+    p0 = (int)(list.start / list.per);
+    parts = (int)((list.start + size - 1) / list.per) - p0 + 1;
+  } else {
+    parts = (size + a.part_blocks - 1) / a.part_blocks;
+  }
   if (parts <= 1) return;                              // (the whole workgroup: its results are there already)
   const int lane_row = threadIdx.x / TPR / kSlots, slot = threadIdx.x / TPR % kSlots, col = threadIdx.x % TPR * 4;
   const int r = blockIdx.x % chunks * ROWS + lane_row, pr = rb * a.row_rows + r;
   const bool ok = r < a.part_rows && pr < a.tokens * group;
   const float sc = score_scale(a.sm_scale, false);
-  const int64_t at = (int64_t)block * a.parts * a.part_rows + (ok ? r : 0);
+  const int64_t at = tree_sums(a, hk, rb, p0, z) + (ok ? r : 0);
   const float* po = a.part_o + at * D + col;
   const float* pm = a.part_ml + at * 2;
   float m = kNegBig, l = 0.f;
@@ -457,29 +877,37 @@ hipError_t launch_tree_sum_slots(const TreeArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((tree_sum_kernel<T, D, kSlots>), dim3(blocks * ((a.part_rows + ROWS - 1) / ROWS)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
-// Slots of a row: as many as halve the rounds of loads while the rows alone leave the chip empty.
+// Slots of a row: where the rows alone leave the chip empty and a sequence may lie in many pieces.
 template <typename T, int D>
 hipError_t launch_tree_sum(const TreeArgs& a, hipStream_t stream) {
   const int64_t rows = (int64_t)a.cache.sequences * a.cache.heads * a.row_blocks * a.part_rows;
-  if (a.parts <= 4 || rows > 4096) return launch_tree_sum_slots<T, D, 1>(a, stream);
+  if ((a.workers > 0 ? a.workers / a.cache.sequences : a.parts) <= 8 || rows > 1024) return launch_tree_sum_slots<T, D, 1>(a, stream);
   return launch_tree_sum_slots<T, D, 256 / (D / 4)>(a, stream);
 }
 
-template <typename T, int D, bool kPad>
-hipError_t launch_tree_rows(const TreeArgs& a, hipStream_t stream) {
-  auto kern = tree_rows_kernel<T, D, kPad>;
-  constexpr int smem = TreeSmem<D>::BYTES;
+template <auto kern>
+hipError_t launch_tree_kernel(const TreeArgs& a, int threads, int smem, hipStream_t stream) {
   if (smem > 64 * 1024) {
     static std::atomic<uint64_t> lds_set{0};
     const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern), smem, lds_set);
     if (e != hipSuccess) return e;
   }
-  const int pairs = a.cache.sequences * a.cache.heads;
-  const int units = (pairs * a.parts + kNumXcd - 1) / kNumXcd;
+  const int pieces = a.workers > 0 ? a.workers : a.cache.sequences * a.parts, units = (a.cache.heads * pieces + kNumXcd - 1) / kNumXcd;
   if (units == 0 || a.row_blocks == 0) return hipSuccess;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(kNumXcd * units * a.row_blocks)), dim3(256), smem, stream, a);
-  const hipError_t e = hipGetLastError();
-  return e != hipSuccess || a.parts <= 1 ? e : launch_tree_sum<T, D>(a, stream);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(kNumXcd * units * a.row_blocks)), dim3(threads), smem, stream, a);
+  return hipGetLastError();
+}
+
+// a.row_rows names the kernel: 32 rows, or those of a tile
+template <typename T, int D, bool kPad>
+hipError_t launch_tree(const TreeArgs& a, hipStream_t stream) {
+  hipError_t e = hipErrorNotSupported;
+  if (a.row_rows == 32) e = launch_tree_kernel<tree_rows_kernel<T, D, kPad>>(a, 256, TreeSmem<D>::BYTES, stream);
+  if constexpr (D <= 128) {
+    if (a.row_rows == 128) e = launch_tree_kernel<tree_tile_kernel<T, D, 4, kPad>>(a, 256, TreeTileSmem<D>::BYTES, stream);
+    if (a.row_rows == 256) e = launch_tree_kernel<tree_tile_kernel<T, D, 8, kPad>>(a, 512, TreeTileSmem<D>::BYTES, stream);
+  }
+  return e != hipSuccess || a.part_o == nullptr ? e : launch_tree_sum<T, D>(a, stream);
 }
 
 }  // namespace fa

@@ -104,8 +104,8 @@ int check_cache(const fa_cache* p, fa::CacheArgs* out) {
   if (p->lengths.sizes[0] > kMaxCount) return FA_ERROR_INVALID_VALUE;
   if ((e = check_ints(p->lengths, p->lengths.sizes[0])) != FA_SUCCESS) return e;
   if ((e = check_int_rows(p->table, p->lengths.sizes[0])) != FA_SUCCESS) return e;
-  // slots are numbered in 32 bits, the drafted tokens behind the last one among them
-  if ((p->table.sizes[1] << c.page_shift) > 0x7ffff000ull) return FA_ERROR_NOT_SUPPORTED;
+  // slots, and the blocks of 64 sequences, are counted in 32 bits
+  if ((p->table.sizes[1] << c.page_shift) > 1ull << 29) return FA_ERROR_NOT_SUPPORTED;
   c.table = static_cast<const int32_t*>(p->table.ptr);
   c.table_row = (int64_t)p->table.strides[0];
   c.lengths = static_cast<const int32_t*>(p->lengths.ptr);
@@ -117,38 +117,46 @@ int check_cache(const fa_cache* p, fa::CacheArgs* out) {
 // a launch's workgroups have to fit 31 bits
 bool fits(double workgroups) { return workgroups < 2147483648.0; }
 
-// Blocks of 32 slots per part, and the scratch for the parts' sums.  Two workgroups run on a CU (one above 128 columns), each with
-// four waves that take the blocks in turn.  `kRounds` rounds of workgroups if all sequences had max_length, so that those of different
-// lengths even out; at least two blocks per wave, and at most kMaxParts parts.
+// Rows per workgroup, how the keys are cut, and the scratch for the sums of sequences that lie in several pieces.
 struct TreePlan { int64_t o_bytes, bytes; };
-constexpr int kMaxParts = 256, kRounds = 4;
 constexpr int64_t kMostScratch = 256 << 20;
 TreePlan tree_plan(fa::TreeArgs* a, int64_t max_length, int num_cu) {
   TreePlan p{};
   const int d = fa::compiled_columns(a->cache);
-  const int64_t rows = (int64_t)a->tokens * (a->hq / a->cache.heads);
-  a->row_rows = 32;
-  a->row_blocks = (int)((rows + 31) / 32);
-  a->part_rows = (int)(rows < 32 ? rows : 32);
-  // (the blocks that a sequence of that length has, and the most that any may have)
+  const int64_t rows = (int64_t)a->tokens * (a->hq / a->cache.heads), sequences = a->cache.sequences;
+  a->row_rows = rows <= 64 || d > 128 ? 32 : rows <= 128 ? 128 : 256;
+  a->row_blocks = (int)((rows + a->row_rows - 1) / a->row_rows);
+  a->part_rows = (int)std::min<int64_t>(rows, a->row_rows);
+  a->block_shift = a->row_rows == 32 ? 5 : 6;
+  a->least = a->row_rows == 32 ? 8 : 2;
+  // (the blocks that a sequence of that length has, at the most)
+  const int64_t size = 1 << a->block_shift;
   auto blocks_of = [&](int64_t length) {
     int64_t slots = length + a->tokens;
-    if (a->window > 0) slots = std::min<int64_t>(slots, (int64_t)a->window + a->tokens + std::min<int64_t>(a->sinks, length) + 96);
-    return (slots + 31) / 32;
+    if (a->window > 0) slots = std::min<int64_t>(slots, (int64_t)a->window + a->tokens + std::min<int64_t>(a->sinks, length) + 3 * size);
+    return std::max<int64_t>(1, (slots + size - 1) / size);
   };
-  const int64_t room = (int64_t)a->cache.columns << a->cache.page_shift;
-  const int64_t blocks = blocks_of(max_length), most = blocks_of(room), items = (int64_t)a->cache.sequences * a->cache.heads * a->row_blocks;
-  const int64_t chip = (int64_t)(d > 128 ? 1 : 2) * num_cu * kRounds;
-  int64_t per = std::max<int64_t>(8, (blocks * items + chip - 1) / chip);
-  per = std::max(per, (most + kMaxParts - 1) / kMaxParts);
-  // (a table with room for far more than max_length: parts that no sequence may come to have take scratch as well)
-  const int64_t part_bytes = items * a->part_rows * (d * 4 + 8);
-  if (part_bytes > 0) per = std::max(per, (most * part_bytes + kMostScratch - 1) / kMostScratch);
-  a->part_blocks = (int)per;
-  a->parts = (int)std::max<int64_t>(1, (most + per - 1) / per);
-  const int64_t stored = a->parts > 1 ? items * a->parts * a->part_rows : 0;
+  // One round of workgroups: two on a CU, one with tiles of 256 rows or more than 128 columns.
+  const int64_t heads = (int64_t)a->cache.heads * a->row_blocks, chip = (int64_t)(d > 128 || a->row_rows == 256 ? 1 : 2) * num_cu;
+  const int64_t blocks = blocks_of(max_length), most = blocks_of((int64_t)a->cache.columns << a->cache.page_shift);
+  const int64_t row_bytes = d * 4 + 8;
+  int64_t per = std::max<int64_t>(a->least, (blocks * sequences * heads + chip - 1) / chip), stored = 0;
+  const int64_t short_piece = a->row_rows == 32 ? 32 : 16;
+  // Short pieces: a workgroup has one, of one sequence, so that nothing waits for the lengths of the others or for an item before.
+  // Long ones: equal pieces of all keys, whatever the lengths.  (us, the one / the other, D128 unless said, Hq 32 Hk 8: B1 4096 slots 11.7 / 13.3,
+  // B8 up to 2048 14.9 / 18.2, B32 Hq 16 Hk 2 D64 7 tokens window 1024 15.4 / 22.3; B64 up to 8192 145 / 132, D64 87 / 79, B8 48 tokens up to
+  // 16384 94 / 75; level B16 8 tokens up to 8192.)
+  if (per <= short_piece) {
+    per = std::max(per, (most * sequences * heads * a->part_rows * row_bytes + kMostScratch - 1) / kMostScratch);
+    a->part_blocks = (int)per;
+    a->parts = (int)((most + per - 1) / per);
+    if (a->parts > 1) stored = heads * sequences * a->parts * a->part_rows;
+  } else if (chip / heads > 1) {
+    a->workers = (int)(chip / heads);
+    stored = heads * (a->workers + sequences) * a->part_rows;
+  }
   p.o_bytes = stored * d * 4;
-  p.bytes = p.o_bytes + stored * 8;
+  p.bytes = stored * row_bytes;
   return p;
 }
 
@@ -193,16 +201,19 @@ int fa_tree_attn(const fa_tree_params* p, void* hip_stream, fa_allocator* alloc)
   a.sinks = std::min(p->sinks, 1 << 30);
   const int64_t room = (int64_t)c.columns << c.page_shift;
   const TreePlan plan = tree_plan(&a, std::min<int64_t>(p->max_length, room), fa_get_multiprocessor_count(hip_stream));
-  if (a.parts > 1) {
+  if (plan.bytes > 0) {
     void* scratch = alloc != nullptr ? alloc->alloc(alloc, (uint64_t)plan.bytes) : nullptr;
-    a.part_o = static_cast<float*>(scratch);
-    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(scratch) + plan.o_bytes);
-    if (scratch == nullptr) {
-      a.parts = 1;
-      a.part_blocks = 0x7fffffff;
+    if (scratch != nullptr) {
+      a.part_o = static_cast<float*>(scratch);
+      a.part_ml = reinterpret_cast<float*>(static_cast<char*>(scratch) + plan.o_bytes);
     }
   }
-  if (!fits(((double)c.sequences * c.heads * a.parts + 8) * a.row_blocks)) return FA_ERROR_NOT_SUPPORTED;
+  if (a.part_o == nullptr) {      // every sequence is one piece
+    a.workers = 0;
+    a.parts = 1;
+    a.part_blocks = 1 << 29;
+  }
+  if (!fits(((double)c.heads * (a.workers > 0 ? a.workers : (double)c.sequences * a.parts) + 8) * a.row_blocks) || !fits((double)c.sequences * c.heads * a.row_blocks * 256)) return FA_ERROR_NOT_SUPPORTED;
   return (int)fa::run_tree(dtype, a, static_cast<hipStream_t>(hip_stream));
 }
 

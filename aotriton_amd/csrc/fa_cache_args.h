@@ -31,10 +31,12 @@ struct TreeArgs {
   int32_t hq, tokens;
   float sm_scale;
   int32_t window, sinks;         // window 0: none
-  // A workgroup takes `part_blocks` blocks of 32 slots for row_rows packed rows; a sequence has as many parts as its length needs, at
-  // most `parts`.  The sums of a sequence with one part only are its results; those of the others lie in part_o as (pair,
-  // block of rows, part, row of the block, compiled columns) and, maximum and row sum, in part_ml.
-  int32_t parts, part_blocks, row_blocks, row_rows, part_rows;      // part_rows: stored per block
+  // Work, in blocks of 1 << block_shift slots for row_rows packed rows of a head.  workers > 0: the blocks of all sequences, one after the
+  // other, are cut into that many equal pieces of at least `least` blocks, one for a workgroup.  Otherwise every sequence is cut into
+  // pieces of part_blocks blocks, at most `parts`.  The rows' sums over a sequence that lies in several pieces go to part_o (null: none does)
+  // as (head, block of rows, tree_sums' place, row of the block, compiled columns) and, maximum and row sum, to part_ml.
+  int32_t workers, least, parts, part_blocks, block_shift;
+  int32_t row_blocks, row_rows, part_rows;      // part_rows: stored per block of rows
   float* part_o; float* part_ml;
 };
 

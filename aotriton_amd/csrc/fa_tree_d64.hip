@@ -14,7 +14,7 @@
 
 namespace fa {
 hipError_t FA_RUN(int dtype, const TreeArgs& a, hipStream_t s) {
-  if (dtype == kDtypeBF16) return launch_tree_rows<bf16_t, 64, FA_PADDED != 0>(a, s);
-  return launch_tree_rows<f16_t, 64, FA_PADDED != 0>(a, s);
+  if (dtype == kDtypeBF16) return launch_tree<bf16_t, 64, FA_PADDED != 0>(a, s);
+  return launch_tree<f16_t, 64, FA_PADDED != 0>(a, s);
 }
 }  // namespace fa
