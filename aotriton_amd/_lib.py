@@ -112,7 +112,7 @@ SYMBOLS = {
                                             ctypes.c_void_p]),
     'fa_attn_bwd': (ctypes.c_int, [P(fa_bwd_params), ctypes.c_int32, ctypes.c_void_p, P(fa_options)]),
     'fa_attn_fwd_sinks': (ctypes.c_int, [P(fa_fwd_params), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
-                                         P(fa_options)]),
+                                         P(fa_options), ctypes.c_void_p]),
     'fa_attn_bwd_sinks': (ctypes.c_int, [P(fa_bwd_params), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
                                          P(fa_options), ctypes.c_void_p]),
     'fa_tree_attn': (ctypes.c_int, [P(fa_tree_params), ctypes.c_void_p, ctypes.c_void_p]),

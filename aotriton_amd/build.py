@@ -53,13 +53,14 @@ EXTRA = {
     # (the same kernels with sinks)
     'fa_sinks_dkdv_d128.hip': ['-mllvm', '-amdgpu-sched-strategy=max-ilp'],
     'fa_sinks_dq_d128.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form'],
+    'fa_sinks_wide_d128.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', '-Wno-inline-asm'],
 }
 
 # The per-head-dim kernel files are compiled a second time with FA_PADDED = the head dim: the copies that
 # serve head dims rounded up to the compiled one.
-PADDED_RE = re.compile(r'fa_(fwd|fwd_rows|fwd_wide|bwd_dkdv|bwd_dkdv_parts|bwd_dq|bwd_dq_bias|bwd_wide|bwd_pair|bwd_fused|sinks_fwd|sinks_dkdv|sinks_dq|tree)_d(\d+)\.hip$')
+PADDED_RE = re.compile(r'fa_(fwd|fwd_rows|fwd_wide|bwd_dkdv|bwd_dkdv_parts|bwd_dq|bwd_dq_bias|bwd_wide|bwd_pair|bwd_fused|sinks_fwd|sinks_dkdv|sinks_dq|sinks_wide|tree)_d(\d+)\.hip$')
 # ... and these a third time with 96 columns, for head dims above 64 and up to 96
-COLS96_RE = re.compile(r'fa_(fwd|fwd_wide|bwd_dkdv|bwd_dq|bwd_wide|sinks_fwd|sinks_dkdv|sinks_dq)_d128\.hip$')
+COLS96_RE = re.compile(r'fa_(fwd|fwd_wide|bwd_dkdv|bwd_dq|bwd_wide|sinks_fwd|sinks_dkdv|sinks_dq|sinks_wide)_d128\.hip$')
 
 
 def sources():

@@ -1370,24 +1370,60 @@ int check_sinks(const Shape& s, int dtype, int causal_type, int32_t window, int3
 // (the kernels add the window to positions)
 int32_t window_of(int32_t window) { return window < (1 << 30) ? window : 1 << 30; }
 
-// Tiles of 128 rows, two workgroups per CU, instead of 256 and one?  The costs are those of fwd_small_tiles (us per item, and per
-// 64 keys); a tile of 256 rows meets 128 keys more.
-int sinks_half_tiles(const Shape& s, int64_t tokens, int32_t window, int32_t sinks, int num_cu) {
-  const int64_t cus = num_cu >= fa::kNumXcd ? num_cu / fa::kNumXcd : 1, seqs = s.num_seqlens != 0 ? std::abs(s.num_seqlens) : s.batch;
-  const int64_t rows = s.num_seqlens > 0 ? std::max<int64_t>(1, tokens / std::max<int64_t>(1, seqs)) : s.max_sq;
-  auto time = [&](int bm, int per_cu, double a, double b) {
-    const double keys = std::min<int64_t>(s.max_sk, (int64_t)window + bm) + std::min<int64_t>(sinks, 64);
-    const int64_t items = (seqs * s.hq + fa::kNumXcd - 1) / fa::kNumXcd * ((rows + bm - 1) / bm);
-    return (double)((items + per_cu * cus - 1) / (per_cu * cus)) * (a + b * keys / 64);
+// Estimated times of walks of even items, in microseconds: rounds of the chip, each as long as an item.
+double rounds_time(int64_t items, int64_t slots, double item) { return (double)((items + slots - 1) / slots) * item; }
+// tiles of `rows` rows of all heads' sequences (packed ones end in the middle of a tile)
+int64_t sink_tiles(const Shape& s, int heads, bool keys, int64_t tokens, int rows) {
+  const int64_t seqs = s.num_seqlens != 0 ? std::abs(s.num_seqlens) : s.batch;
+  return heads * (s.num_seqlens > 0 ? tokens / rows + seqs / 2 + 1 : seqs * (((keys ? s.max_sk : s.max_sq) + rows - 1) / rows));
+}
+
+// Forward: tiles of 256 rows or of 128, two workgroups per CU, and the parts that a tile's keys are split into where the tiles do not fill
+// the chip.  The costs are about those of fwd_small_tiles and fwd_plan (an item, 64 keys of it; a second launch and the parts' sums at 4 TB/s).
+// (us, 256 rows / 128 rows / split in two / in four: B1 Hq 32 Hk 8 D128 S32768 window 4096 2023 / 2249, S8192 1024 197 / 194, 256 100 / 83; 256 queries
+// of 4096 keys window 1024 43 / 38 / 32 / 31, 64 of 8192 window 4096 108 / 110 / 65 / 40; B4 H16 D64 512 of 4601 window 2048 58 / 46 / 43 / 51.)
+struct SinkFwdPlan { int half_tiles, splits; int64_t o_bytes, bytes; };
+SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, int32_t window, int32_t sinks, int num_cu) {
+  SinkFwdPlan best{0, 1, 0, 0};
+  double least = 0;
+  const int64_t seqs = s.num_seqlens != 0 ? std::abs(s.num_seqlens) : s.batch;
+  for (int half = 0; half < 2; ++half) {
+    const int bm = half ? 128 : 256, per_cu = half ? 2 : 1;
+    const double item = s.d > 64 ? (half ? 6.5 : 6.3) : (half ? 4.5 : 4.35), step = s.d > 64 ? (half ? 1.8 : 1.74) : (half ? 1.2 : 1.12);
+    const int64_t keys = std::min<int64_t>(s.max_sk, (int64_t)window + bm) + std::min<int64_t>(sinks, 64), tiles = (keys + 63) / 64;
+    const int64_t items = sink_tiles(s, s.hq, false, tokens, bm), stored = seqs * s.hq * ((s.max_sq + bm - 1) / bm) * bm;
+    for (int splits = 1; splits <= 8 && (splits == 1 || (s.num_seqlens == 0 && splits * 2 <= tiles)); ++splits) {
+      const int64_t o_bytes = splits > 1 ? stored * splits * s.d * 4 : 0, bytes = splits > 1 ? o_bytes + stored * splits * 8 : 0;
+      const double t = rounds_time(items * splits, (int64_t)per_cu * num_cu, item + step * ((tiles + splits - 1) / splits)) +
+                       (splits > 1 ? 5 + 2.0 * bytes / 4e6 : 0.0);
+      if ((half == 0 && splits == 1) || t < 0.97 * least) {
+        least = t;
+        best = SinkFwdPlan{half ? 2 : 0, splits, o_bytes, bytes};
+      }
+    }
+  }
+  return best;
+}
+
+// Backward: the kernels with 64 rows per wave (head dims above 64)?  Costs as in bwd_route.  (us of the whole backward, 128 rows / 256: bf16
+// Hq 32 Hk 8 S8192 D128 window 256 297 / 299, 512 389 / 372, 1024 613 / 541, 2048 928 / 845; B4 Hq 16 Hk 4 S1024 window 256 112 / 156,
+// only dQ wide 109; B1 Hq 8 Hk 2 S4096 window 512 122 / 199.)
+struct SinkBwdRoute { bool wide_dq, wide_dkdv; };
+SinkBwdRoute sink_bwd_route(const Shape& s, int64_t tokens_q, int64_t tokens_k, int32_t window, int num_cu) {
+  if (s.d != 128) return SinkBwdRoute{false, false};
+  auto time = [&](bool keys, int tile, int step, double item, double cost) {
+    const int64_t span = std::min<int64_t>(keys ? s.max_sq : s.max_sk, (int64_t)window - 1 + tile);
+    const double steps = (keys ? s.hq / s.hk : 1) * (double)(span / step + 1) + (keys ? 0 : 1);
+    return rounds_time(sink_tiles(s, keys ? s.hk : s.hq, keys, keys ? tokens_k : tokens_q, tile), num_cu, item + cost * steps);
   };
-  return s.d > 64 ? (time(128, 2, 7.3, 1.99) < 0.97 * time(256, 1, 6.3, 1.74) ? 2 : 0)
-                  : (time(128, 2, 4.54, 1.27) < 0.97 * time(256, 1, 4.35, 1.12) ? 2 : 0);
+  return SinkBwdRoute{time(false, 256, 32, 5, 1.42) < 0.95 * time(false, 128, 64, 5, 1.7),
+                      time(true, 256, 32, 7, 1.8) < time(true, 128, 64, 9, 1.95)};
 }
 
 }  // namespace
 
 int fa_attn_fwd_sinks(const fa_fwd_params* p, int32_t params_version, int32_t window, int32_t sinks, void* hip_stream,
-                      const fa_options* options) {
+                      const fa_options* options, fa_allocator* alloc) {
   Shape s{};
   int e = validate_fwd(p, params_version, options, &s);
   if (e != FA_SUCCESS) return e;
@@ -1407,9 +1443,30 @@ int fa_attn_fwd_sinks(const fa_fwd_params* p, int32_t params_version, int32_t wi
   a.num_cu = dev->num_cu;
   a.window = window_of(window);
   a.sinks = sinks;
-  if (s.max_sq > 0 && s.batch > 0) a.half_tiles = sinks_half_tiles(s, (int64_t)p->Q.sizes[2], a.window, sinks, dev->num_cu);
-  FA_LOG(4, "attn_fwd_sinks: D=%d window=%d sinks=%d nseq=%d half_tiles=%d", s.d, a.window, sinks, s.num_seqlens, a.half_tiles);
-  return (int)fa::run_sinks_fwd(p->Q.dtype, s.d, a, stream);
+  bool held = false;
+  a.splits = 1;
+  if (s.max_sq > 0 && s.max_sk > 0 && s.batch > 0) {
+    const SinkFwdPlan plan = sink_fwd_plan(s, (int64_t)p->Q.sizes[2], a.window, sinks, dev->num_cu);
+    a.half_tiles = plan.half_tiles;
+    if (plan.splits > 1) {
+      void* scratch = nullptr;
+      if (alloc != nullptr) {
+        scratch = alloc->alloc(alloc, (uint64_t)plan.bytes);
+      } else if (!stream_is_capturing(stream) && plan.bytes <= ws_limit_bytes(device_index(dev))) {
+        held = ws_acquire(device_index(dev), (size_t)plan.bytes, stream, &scratch) == hipSuccess;
+        if (!held) scratch = nullptr;
+      }
+      if (scratch != nullptr) {
+        a.splits = plan.splits;
+        a.part_o = static_cast<float*>(scratch);
+        a.part_ml = reinterpret_cast<float*>(static_cast<char*>(scratch) + plan.o_bytes);
+      }
+    }
+  }
+  FA_LOG(4, "attn_fwd_sinks: D=%d window=%d sinks=%d nseq=%d half_tiles=%d splits=%d", s.d, a.window, sinks, s.num_seqlens, a.half_tiles, a.splits);
+  const hipError_t err = fa::run_sinks_fwd(p->Q.dtype, s.d, a, stream);
+  if (held) ws_release(device_index(dev), stream);
+  return (int)err;
 }
 
 int fa_attn_bwd_sinks(const fa_bwd_params* p, int32_t params_version, int32_t window, int32_t sinks, void* hip_stream,
@@ -1436,10 +1493,13 @@ int fa_attn_bwd_sinks(const fa_bwd_params* p, int32_t params_version, int32_t wi
   a.window = window_of(window);
   a.sinks = std::min(sinks, s.max_sk);
 
-  // The parts of the sinks' sums: workgroups for the chip twice over, of eight steps at least.
+  // Pieces of the sinks' sums: one round of workgroups (two on a CU at 64 columns, one at 128), of eight steps at least.
   const int64_t seqs = s.num_seqlens != 0 ? std::abs(s.num_seqlens) : s.batch, blocks = (a.sinks + 31) / 32;
-  const int64_t items = seqs * s.hk * blocks, steps = (int64_t)(s.hq / s.hk) * ((s.max_sq + 31) / 32);
-  a.sink_parts = (int32_t)std::max<int64_t>(1, items > 0 ? std::min<int64_t>(2 * dev->num_cu / items, steps / 8) : 1);
+  const int64_t items = seqs * s.hk * blocks, longest = (int64_t)(s.hq / s.hk) * ((s.max_sq + 31) / 32);
+  const int64_t steps = s.num_seqlens > 0 ? (int64_t)s.hq * ((int64_t)p->Q.sizes[2] / 32 + seqs) : seqs * s.hk * longest;
+  const int64_t chip = (int64_t)(s.d == 64 ? 2 : 1) * dev->num_cu;
+  a.sink_steps = (int32_t)std::max<int64_t>(8, (steps * blocks + chip - 1) / chip);
+  a.sink_parts = (int32_t)std::max<int64_t>(1, (longest + a.sink_steps - 1) / a.sink_steps);
   const size_t bytes = (size_t)items * a.sink_parts * 2 * 32 * s.d * sizeof(float);
   bool held = false;
   if (bytes > 0) {
@@ -1466,7 +1526,12 @@ int fa_attn_bwd_sinks(const fa_bwd_params* p, int32_t params_version, int32_t wi
   }
   a.delta = static_cast<float*>(delta.ptr);
   FA_LOG(4, "attn_bwd_sinks: D=%d window=%d sinks=%d nseq=%d parts=%d", s.d, a.window, a.sinks, s.num_seqlens, a.sink_parts);
-  if (rc == FA_SUCCESS) rc = (int)fa::run_sinks_dq(p->Q.dtype, s.d, a, stream);      // (and delta, which the others read)
+  const SinkBwdRoute route = sink_bwd_route(s, (int64_t)p->Q.sizes[2], (int64_t)p->K.sizes[2], a.window, dev->num_cu);
+  a.wide = route.wide_dkdv ? 1 : 0;
+  a.walk_group = 2;
+  // (dQ in front: it writes delta, which the others read)
+  if (rc == FA_SUCCESS) rc = (int)(route.wide_dq ? fa::run_sinks_dq_wide(p->Q.dtype, a, stream) : fa::run_sinks_dq(p->Q.dtype, s.d, a, stream));
+  if (rc == FA_SUCCESS && route.wide_dkdv) rc = (int)fa::run_sinks_dkdv_wide(p->Q.dtype, a, stream);
   if (rc == FA_SUCCESS) rc = (int)fa::run_sinks_dkdv(p->Q.dtype, s.d, a, stream);
   if (held) ws_release(device_index(dev), stream);
   if (acquired && lazy->dispose != nullptr) lazy->dispose(lazy);

@@ -211,8 +211,10 @@ struct SinkFwdArgs : FwdArgs {
 };
 struct SinkBwdArgs : BwdArgs {
   int32_t window, sinks;
-  // dK and dV of the first keys come from fp32 sums over sink_parts parts of the queries (fa_sinks.h)
-  int32_t sink_parts;
+  // dK and dV of the first keys come from fp32 sums over pieces of sink_steps steps, at most sink_parts of them per sequence and K/V head
+  // (fa_sinks.h)
+  int32_t sink_parts, sink_steps;
+  int32_t wide;          // the window's part of dK and dV is another launch's (64 keys per wave)
   float* sink_ws;
 };
 

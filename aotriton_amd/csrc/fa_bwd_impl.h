@@ -1472,6 +1472,16 @@ void bwd_dkdv_kernel(const BwdArgsOf<kSinks> a) {
   // workgroups of the XCD take the items in serpentine order (worker p takes p,
   // 2P-1-p, 2P+p, ...), which pairs heavy with light items.
   const int xcd = blockIdx.x % kNumXcd, p = blockIdx.x / kNumXcd, workers = gridDim.x / kNumXcd;
+  if constexpr (kSinks) {
+    EvenWalk even;
+    int pos = even.template init<NW * 64>(reinterpret_cast<int*>(smem_raw + DkDvSmem<D, BM>::BYTES), a.seq, a.num_zh / a.hk, a.num_n_tiles, a.hk, 1, NW * 32,
+                                          true, xcd, threadIdx.x) + p;
+    for (int z, hk, nt; even.at(pos, z, hk, nt); pos += workers) {
+      dkdv_item<T, D, NW, BM, kWindowed, kBias, kDropout, kPad, kStoreDs, kParts, kForm, kSinks>(a, hk, nt, z, 0, smem_raw);
+      __syncthreads();     // the next item reuses the LDS stages
+    }
+    return;
+  }
   const int per_group = a.zh_group * a.num_n_tiles;
   // Sequences of different lengths: the valid tiles only, heaviest first (LevelWalk), taken in the
   // same serpentine order.
@@ -1514,6 +1524,16 @@ void bwd_dq_kernel(const BwdArgsOf<kSinks> a) {
   // persistent workgroups with the same walk as the forward kernel: (batch, q-head) pairs
   // per XCD, heaviest Q tile first, serpentine over the workgroups of the XCD
   const int xcd = blockIdx.x % kNumXcd, p = blockIdx.x / kNumXcd, workers = gridDim.x / kNumXcd;
+  if constexpr (kSinks) {
+    EvenWalk even;
+    int pos = even.template init<NW * 64>(reinterpret_cast<int*>(smem_raw + DqSmem<D, BN>::BYTES), a.seq, a.num_zh / a.hq, a.num_m_tiles, a.hk, a.hq / a.hk,
+                                          NW * 32, false, xcd, threadIdx.x) + p;
+    for (int z, h, mt; even.at(pos, z, h, mt); pos += workers) {
+      dq_item<T, D, NW, BN, kWindowed, kBias, kDropout, true, kPad, true, kSinks>(a, h, mt, z, smem_raw);
+      __syncthreads();     // the next item reuses the LDS stages
+    }
+    return;
+  }
   const int per_group = a.zh_group * a.num_m_tiles;
   // (D = 256 is launched with one workgroup per item: the loop would cost registers there)
   for (int r = 0; D >= 256 ? r < 1 : r * workers < a.items_per_xcd; ++r) {
@@ -1672,7 +1692,7 @@ hipError_t launch_dq_variant(const BwdArgsOf<kSinks>& a0, hipStream_t stream) {
   a.num_m_tiles = (a.seq.max_seqlen_q + BM - 1) / BM;
   set_work(a, tile_work(bwd_nseq(a) * a.hq, q_head_group(a.hq, a.hk), a.num_m_tiles));
   dim3 grid((unsigned)(kNumXcd * bwd_workers(D, B, a.items_per_xcd, a.num_cu, kTwoWaves<D, B> ? 2 : 1)));
-  return launch_with_lds<bwd_dq_kernel<T, D, NW, BN, W, B, P, kPad, kSinks>>(grid, NW * 64, DqSmem<D, BN>::BYTES, stream, a);
+  return launch_with_lds<bwd_dq_kernel<T, D, NW, BN, W, B, P, kPad, kSinks>>(grid, NW * 64, DqSmem<D, BN>::BYTES + (kSinks ? kLevelBytes : 0), stream, a);
 }
 
 template <typename T, int D, int kPad, bool W, bool B, bool P, bool kBuilt>

@@ -35,8 +35,8 @@ struct WideDkDvSmem {
   static_assert(3 * STAGE_BYTES <= V_OFF, "three stages");
 };
 
-template <typename T, bool kWindowed, int kPad>
-__device__ __forceinline__ void dkdv_wide_item(const BwdArgs& a, const int hk, const int nt, const int z, char* smem_raw) {
+template <typename T, bool kWindowed, int kPad, bool kSinks = false>
+__device__ __forceinline__ void dkdv_wide_item(const BwdArgsOf<kSinks>& a, const int hk, const int nt, const int z, char* smem_raw) {
   constexpr int D = 128, BM = kWideBM, BN = kWideBN, KB = 2;
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
@@ -56,7 +56,8 @@ __device__ __forceinline__ void dkdv_wide_item(const BwdArgs& a, const int hk, c
   if (n0 >= si.seqlen_k) return;
 
   Window w{0, 0};
-  if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right, si.seqlen_q, si.seqlen_k);
+  if constexpr (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);
+  else if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right, si.seqlen_q, si.seqlen_k);
   w.left = w.left > (1 << 30) ? (1 << 30) : (w.left < -(1 << 30) ? -(1 << 30) : w.left);
   w.right = w.right > (1 << 30) ? (1 << 30) : (w.right < -(1 << 30) ? -(1 << 30) : w.right);
   const BlockRanges br = block_ranges(kWindowed, w.right, w.left, n0, si.seqlen_k, si.seqlen_q, BN, BM);
@@ -416,11 +417,21 @@ __device__ __forceinline__ void dkdv_wide_item(const BwdArgs& a, const int hk, c
   }
 }
 
-template <typename T, bool kWindowed, int kPad>
+template <typename T, bool kWindowed, int kPad, bool kSinks = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256))) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void bwd_dkdv_wide_kernel(const BwdArgs a) {
+void bwd_dkdv_wide_kernel(const BwdArgsOf<kSinks> a) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   const int xcd = blockIdx.x % kNumXcd, p = blockIdx.x / kNumXcd, workers = gridDim.x / kNumXcd;
+  if constexpr (kSinks) {
+    EvenWalk even;
+    int pos = even.template init<256>(reinterpret_cast<int*>(smem_raw + WideDkDvSmem::BYTES), a.seq, a.num_zh / a.hk, a.num_n_tiles, a.hk, 1, kWideBN, true,
+                                      xcd, threadIdx.x) + p;
+    for (int z, hk, nt; even.at(pos, z, hk, nt); pos += workers) {
+      dkdv_wide_item<T, kWindowed, kPad, kSinks>(a, hk, nt, z, smem_raw);
+      __syncthreads();
+    }
+    return;
+  }
   const int per_group = a.zh_group * a.num_n_tiles;
   const bool ragged = dkdv_level_list<128>(a);
   const int zh_lo = xcd * a.zh_per_xcd;
@@ -446,7 +457,7 @@ void bwd_dkdv_wide_kernel(const BwdArgs a) {
     }
     int z, hk;
     split_zh(zh, a.num_zh / a.hk, 1, z, hk);
-    dkdv_wide_item<T, kWindowed, kPad>(a, hk, nt, z, smem_raw);
+    dkdv_wide_item<T, kWindowed, kPad, kSinks>(a, hk, nt, z, smem_raw);
     __syncthreads();
   }
 }
@@ -460,8 +471,8 @@ struct WideDqSmem {
   static_assert(3 * STAGE_BYTES <= DO_OFF, "three stages");
 };
 
-template <typename T, bool kWindowed, int kPad>
-__device__ __forceinline__ void dq_wide_item(const BwdArgs& a, const int h, const int mt, const int z, char* smem_raw) {
+template <typename T, bool kWindowed, int kPad, bool kSinks = false>
+__device__ __forceinline__ void dq_wide_item(const BwdArgsOf<kSinks>& a, const int h, const int mt, const int z, char* smem_raw) {
   constexpr int D = 128, BM = kWideBN, BN = kWideBM, QB = 2;
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
@@ -482,12 +493,18 @@ __device__ __forceinline__ void dq_wide_item(const BwdArgs& a, const int h, cons
   if (q0 >= si.seqlen_q) return;
 
   Window w{0, 0};
-  if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right, si.seqlen_q, si.seqlen_k);
+  if constexpr (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);
+  else if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right, si.seqlen_q, si.seqlen_k);
   w.left = w.left > (1 << 30) ? (1 << 30) : (w.left < -(1 << 30) ? -(1 << 30) : w.left);
   w.right = w.right > (1 << 30) ? (1 << 30) : (w.right < -(1 << 30) ? -(1 << 30) : w.right);
   const BlockRanges br = block_ranges(kWindowed, w.left, w.right, q0, si.seqlen_q, si.seqlen_k, BM, BN);
   const int qw = q0 + 64 * wave;
   const BlockRanges wr = block_ranges(kWindowed, w.left, w.right, qw, si.seqlen_q, si.seqlen_k, 64, BN);
+  // kSinks, as in dq_item: tiles before the window's first, in which only sinks are visible
+  int sinks = 0;
+  if constexpr (kSinks) sinks = a.sinks;
+  const int front = kSinks ? (sinks < br.lo * BN ? (sinks + BN - 1) / BN : br.lo) : 0;
+  const int fetch_lo = front > 0 ? 0 : br.lo;
 
   const int hk = h / (a.hq / a.hk);
   const int row0 = qw + c;                       // this lane's queries: row0 and row0 + 32
@@ -530,9 +547,10 @@ __device__ __forceinline__ void dq_wide_item(const BwdArgs& a, const int h, cons
   const int k_voff = gch * 8 < d_qk ? r0 * (int)a.sk.s * 2 + gch * 16 : kVoffOutOfRange;
   const int v_voff = gch * 8 < d_v ? r0 * (int)a.sv.s * 2 + gch * 16 : kVoffOutOfRange;
   const int k_row = (int)a.sk.s * 2, v_row = (int)a.sv.s * 2;
-  const T* kb = reinterpret_cast<const T*>(a.k) + (int64_t)si.batch_index * a.sk.z + (int64_t)hk * a.sk.h + ((int64_t)si.k_start + (int64_t)br.lo * BN) * a.sk.s;
-  const T* vb = reinterpret_cast<const T*>(a.v) + (int64_t)si.batch_index * a.sv.z + (int64_t)hk * a.sv.h + ((int64_t)si.k_start + (int64_t)br.lo * BN) * a.sv.s;
-  int f_tiles = ntk, f_rows = si.seqlen_k - br.lo * BN;
+  const T* kb = reinterpret_cast<const T*>(a.k) + (int64_t)si.batch_index * a.sk.z + (int64_t)hk * a.sk.h + ((int64_t)si.k_start + (int64_t)fetch_lo * BN) * a.sk.s;
+  const T* vb = reinterpret_cast<const T*>(a.v) + (int64_t)si.batch_index * a.sv.z + (int64_t)hk * a.sv.h + ((int64_t)si.k_start + (int64_t)fetch_lo * BN) * a.sv.s;
+  int f_tiles = ntk + front, f_rows = si.seqlen_k - fetch_lo * BN;
+  int front_left = front;
   u32x4_t k_rs, v_rs;
   auto fetch_begin = [&]() __attribute__((always_inline)) {
     const int rows = f_tiles > 0 ? min(f_rows, BN) : 0;
@@ -540,6 +558,11 @@ __device__ __forceinline__ void dq_wide_item(const BwdArgs& a, const int h, cons
     v_rs = wave_rsrc_words(vb, rows_extent(rows, v_row, d_v * 2));
     kb += (int64_t)BN * a.sk.s; vb += (int64_t)BN * a.sv.s;
     f_rows -= BN; --f_tiles;
+    if constexpr (kSinks)
+      if (--front_left == 0) {
+        kb += (int64_t)(br.lo - front) * BN * a.sk.s; vb += (int64_t)(br.lo - front) * BN * a.sv.s;
+        f_rows -= (br.lo - front) * BN;
+      }
   };
   auto fetch_piece = [&](int stage, int i) __attribute__((always_inline)) {
     const int lds = smem0 + stage + i * SM::TILE_BYTES + wave * 4 * ROWB;
@@ -611,6 +634,7 @@ __device__ __forceinline__ void dq_wide_item(const BwdArgs& a, const int h, cons
   int m_lo[QB];
   unsigned m_rng[QB];
   bool m_none[QB];
+  int m_sink[QB];      // where the row's sinks end
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
     const int row = row0 + 32 * b;
@@ -620,6 +644,7 @@ __device__ __forceinline__ void dq_wide_item(const BwdArgs& a, const int h, cons
       hi_ = row + w.right < hi_ ? row + w.right : hi_;
     }
     m_none[b] = hi_ < lo;
+    m_sink[b] = sinks < hi_ + 1 ? sinks : hi_ + 1;
     m_rng[b] = m_none[b] ? 0u : (unsigned)(hi_ - lo);
     m_lo[b] = lo;
   }
@@ -684,7 +709,8 @@ __device__ __forceinline__ void dq_wide_item(const BwdArgs& a, const int h, cons
     auto p_el = [&](int b, int i) __attribute__((always_inline)) {
       float v = __builtin_fmaf(s[b][i], qk_scale, l_row[b]);
       if (masked) {
-        const bool vis = m_d[b] + (unsigned)(8 * (i / 4) + i % 4) <= m_rng[b];
+        bool vis = m_d[b] + (unsigned)(8 * (i / 4) + i % 4) <= m_rng[b];
+        if constexpr (kSinks) vis = vis || j * BN + 4 * hi + 8 * (i / 4) + i % 4 < m_sink[b];
         v = vis ? v : -__builtin_inff();
       }
       s[b][i] = fast_exp2(v);
@@ -761,6 +787,13 @@ __device__ __forceinline__ void dq_wide_item(const BwdArgs& a, const int h, cons
   const int j_lo = none ? br.hi + 1 : wr.lo, j_end = none ? br.hi + 1 : wr.hi + 1;
   const int f_lo = full ? wr.fb_lo : j_end, f_end = full ? wr.fb_hi + 1 : j_end;
   int j = br.lo;
+  if constexpr (kSinks) {
+    // (the wave computes what it would skip where there are sinks; a wave without a key has j_lo behind the last tile)
+    for (int f = 0; f < front; ++f)
+      if (none) skip();
+      else compute(std::true_type{}, f);
+    for (; j < j_lo && j * BN < sinks && !none; ++j) compute(std::true_type{}, j);
+  }
   for (; j < j_lo; ++j) skip();
   for (; j < f_lo; ++j) compute(std::true_type{}, j);
   for (; j < f_end; ++j) compute(std::false_type{}, j);
@@ -785,11 +818,21 @@ __device__ __forceinline__ void dq_wide_item(const BwdArgs& a, const int h, cons
   }
 }
 
-template <typename T, bool kWindowed, int kPad>
+template <typename T, bool kWindowed, int kPad, bool kSinks = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256))) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void bwd_dq_wide_kernel(const BwdArgs a) {
+void bwd_dq_wide_kernel(const BwdArgsOf<kSinks> a) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   const int xcd = blockIdx.x % kNumXcd, p = blockIdx.x / kNumXcd, workers = gridDim.x / kNumXcd;
+  if constexpr (kSinks) {
+    EvenWalk even;
+    int pos = even.template init<256>(reinterpret_cast<int*>(smem_raw + WideDqSmem::BYTES), a.seq, a.num_zh / a.hq, a.num_m_tiles, a.hk, a.hq / a.hk, kWideBN,
+                                      false, xcd, threadIdx.x) + p;
+    for (int z, h, mt; even.at(pos, z, h, mt); pos += workers) {
+      dq_wide_item<T, kWindowed, kPad, kSinks>(a, h, mt, z, smem_raw);
+      __syncthreads();
+    }
+    return;
+  }
   const int per_group = a.zh_group * a.num_m_tiles;
   // Sequences of different lengths: the valid tiles only, by their distance from the start of the sequence, which is their
   // weight under a causal mask (16 packed sequences of 256-8192 tokens, Hq 32 Hk 8: 4760 -> 4250 us against the dense list).
@@ -817,27 +860,27 @@ void bwd_dq_wide_kernel(const BwdArgs a) {
     }
     int z, h;
     split_zh(zh, a.num_zh / a.hq, a.hq / a.hk, z, h);
-    dq_wide_item<T, kWindowed, kPad>(a, h, mt, z, smem_raw);
+    dq_wide_item<T, kWindowed, kPad, kSinks>(a, h, mt, z, smem_raw);
     __syncthreads();
   }
 }
 
-template <typename T, bool W, int kPad>
-hipError_t launch_dq_wide(const BwdArgs& a0, hipStream_t stream) {
-  BwdArgs a = a0;
+template <typename T, bool W, int kPad, bool kSinks = false>
+hipError_t launch_dq_wide(const BwdArgsOf<kSinks>& a0, hipStream_t stream) {
+  BwdArgsOf<kSinks> a = a0;
   a.num_m_tiles = (a.seq.max_seqlen_q + kWideBN - 1) / kWideBN;
   set_work(a, tile_work(bwd_nseq(a) * a.hq, a.walk_group, a.num_m_tiles));
   dim3 grid((unsigned)(kNumXcd * bwd_workers(128, false, a.items_per_xcd, a.num_cu, 1)));
-  return launch_with_lds<bwd_dq_wide_kernel<T, W, kPad>>(grid, 256, WideDqSmem::BYTES + kLevelBytes, stream, a);
+  return launch_with_lds<bwd_dq_wide_kernel<T, W, kPad, kSinks>>(grid, 256, WideDqSmem::BYTES + kLevelBytes, stream, a);
 }
 
-template <typename T, bool W, int kPad>
-hipError_t launch_dkdv_wide(const BwdArgs& a0, hipStream_t stream) {
-  BwdArgs a = a0;
+template <typename T, bool W, int kPad, bool kSinks = false>
+hipError_t launch_dkdv_wide(const BwdArgsOf<kSinks>& a0, hipStream_t stream) {
+  BwdArgsOf<kSinks> a = a0;
   a.num_n_tiles = (a.seq.max_seqlen_k + kWideBN - 1) / kWideBN;
   set_work(a, tile_work(bwd_nseq(a) * a.hk, a.walk_group, a.num_n_tiles));
   dim3 grid((unsigned)(kNumXcd * bwd_workers(128, false, a.items_per_xcd, a.num_cu, 1)));
-  return launch_with_lds<bwd_dkdv_wide_kernel<T, W, kPad>>(grid, 256, WideDkDvSmem::BYTES + kLevelBytes, stream, a);
+  return launch_with_lds<bwd_dkdv_wide_kernel<T, W, kPad, kSinks>>(grid, 256, WideDkDvSmem::BYTES + kLevelBytes, stream, a);
 }
 
 }  // namespace fa

@@ -504,6 +504,79 @@ struct LevelWalk {
   }
 };
 
+// A third list, for items of about equal weight (a window bounds every tile's work): all valid tiles of all sequences, K/V head after
+// K/V head, the q-heads of a group side by side, cut into equal shares for the XCDs and taken by an XCD's workers in turn.  An XCD then
+// has as many items as any other whatever the heads and lengths are (the lists above give it whole (sequence, head) pairs: 16 packed
+// sequences of 266-6000 tokens and 4 K/V heads, window 512: forward 329 -> 269 us, dQ 524 -> 406), and the tiles that its workers have in hand
+// are neighbours, whose windows overlap.  `table`: tiles in front of each sequence, in LDS; packed sequences beyond kEvenCap, and dense
+// batches, count num_tiles for every sequence (a tile behind a sequence's end is an empty item).
+constexpr int kEvenCap = kLevelBytes / 4 - 1;
+struct EvenWalk {
+  const int* table;                // null: num_tiles per sequence
+  int nseq, num_tiles, ratio, hi;
+  int splits;                      // items per tile
+  int total;                       // tiles of a head
+  template <int NT>
+  __device__ __forceinline__ int init(int* lds, const SeqArgs& seq, int nseq_, int num_tiles_, int groups, int ratio_, int rows_per_tile,
+                                      bool keys, int xcd, int tid, int splits_ = 1) {      // first position of the XCD
+    nseq = nseq_; num_tiles = num_tiles_; ratio = ratio_; splits = splits_;
+    table = nullptr;
+    total = nseq * num_tiles;
+    if (seq.num_seqlens != 0 && nseq <= kEvenCap) {
+      table = lds;
+      if (tid < 64) {
+        int sum = 0;
+        for (int base = 0; base < nseq; base += 64) {
+          int n = 0;
+          if (base + tid < nseq) {
+            const SeqInfo si = get_seq(seq, base + tid);
+            n = ((keys ? si.seqlen_k : si.seqlen_q) + rows_per_tile - 1) / rows_per_tile;
+          }
+#pragma unroll
+          for (int i = 1; i < 64; i *= 2) {
+            const int y = __shfl_up(n, i);
+            n += tid >= i ? y : 0;
+          }
+          if (base + tid < nseq) lds[base + tid + 1] = sum + n;
+          sum += __builtin_amdgcn_readlane(n, 63);
+        }
+        if (tid == 0) lds[0] = 0;
+      }
+      __syncthreads();
+      total = __builtin_amdgcn_readfirstlane(lds[nseq]);
+    }
+    const int64_t items = (int64_t)total * groups * ratio * splits;
+    hi = (int)(items * (xcd + 1) / kNumXcd);
+    return (int)(items * xcd / kNumXcd);
+  }
+  __device__ __forceinline__ bool at(int pos, int& z, int& head, int& tile) const {
+    int split;
+    return at(pos, z, head, tile, split);
+  }
+  __device__ __forceinline__ bool at(int pos, int& z, int& head, int& tile, int& split) const {
+    if (pos >= hi) return false;
+    const int all = pos;
+    pos /= splits;
+    split = all - pos * splits;
+    const int per_group = total * ratio, group = pos / per_group, rem = pos - group * per_group, u = rem / ratio;
+    head = group * ratio + rem - u * ratio;
+    if (table == nullptr) {
+      z = u / num_tiles;
+      tile = u - z * num_tiles;
+      return true;
+    }
+    int lo = 0, n = nseq;            // the last sequence that starts at or in front of u
+    while (n > 1) {
+      const int half = n / 2;
+      if (__builtin_amdgcn_readfirstlane(table[lo + half]) <= u) lo += half;
+      n -= half;
+    }
+    z = lo;
+    tile = u - __builtin_amdgcn_readfirstlane(table[lo]);
+    return true;
+  }
+};
+
 // 1-D grids of the kernels that launch one workgroup per tile.  Consecutive workgroup ids go round
 // the 8 XCDs, so XCD x = id % 8 takes the (sequence, kv-head) pairs x, x + 8, ... one after the
 // other and the `per` tiles of a pair back to back: what every tile of a pair streams (its K/V, or

@@ -83,16 +83,27 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   w.left = w.left > (1 << 30) ? (1 << 30) : (w.left < -(1 << 30) ? -(1 << 30) : w.left);
   w.right = w.right > (1 << 30) ? (1 << 30) : (w.right < -(1 << 30) ? -(1 << 30) : w.right);
   BlockRanges br = block_ranges(kWindowed, w.left, w.right, q0, si.seqlen_q, si.seqlen_k, BM, BN);
-  if (kSplit && br.lo <= br.hi) {
+  if (kSplit && !kSinks && br.lo <= br.hi) {
     const int per = (br.hi - br.lo + a.splits) / a.splits;
     br.lo += split * per;
     if (br.lo + per - 1 < br.hi) br.hi = br.lo + per - 1;
   }
   // (a key before the window's first tile is no later than the item's first query, so that all its rows see it if it is a sink)
-  static_assert(!kSinks || (kWindowed && !kBias && !kDropout && !kSplit && D <= 128), "a window with sinks and nothing else");
+  static_assert(!kSinks || (kWindowed && !kBias && !kDropout && D <= 128), "a window with sinks and nothing else");
   int sinks = 0;
   if constexpr (kSinks) sinks = a.sinks;
-  const int front = kSinks ? (sinks < br.lo * BN ? (sinks + BN - 1) / BN : br.lo) : 0;
+  int front = kSinks ? (sinks < br.lo * BN ? (sinks + BN - 1) / BN : br.lo) : 0;
+  // (kSinks: tiles to work on and the first of them; of a split item those of the part)
+  int tiles = 0, first_tile = front > 0 ? 0 : br.lo;
+  if constexpr (kSinks) {
+    tiles = br.lo <= br.hi ? front + br.hi - br.lo + 1 : 0;
+    if constexpr (kSplit) {
+      const int per = (tiles + a.splits - 1) / a.splits, t0 = split * per;
+      tiles = t0 + per < tiles ? per : tiles - t0;
+      first_tile = t0 < front ? t0 : br.lo + t0 - front;
+      if (t0 >= front) front = 0;
+    }
+  }
 
   const int hk = h / (a.hq / a.hk);                       // fwd_kernel.py:360
   const int row = q0 + wave * 32 + c;                     // this lane's query row
@@ -104,7 +115,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   float* lse_ptr = a.lse ? a.lse + lse_offset(si, h, a.hq) : nullptr;
 
   const int64_t part_row = kSplit ? (((int64_t)z * a.hq + h) * a.num_m_tiles + mt) * (int64_t)(a.splits * BM) + split * BM + wave * 32 + c : 0;
-  if (kSplit && br.lo > br.hi) {
+  if (kSplit && (kSinks ? tiles <= 0 : br.lo > br.hi)) {
     if (row_ok && hi == 0) {
       a.part_ml[part_row * 2] = kNegBig;
       a.part_ml[part_row * 2 + 1] = 0.f;
@@ -200,12 +211,12 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
 
   // tiles are fetched in ascending order: the tile bases and the count of rows left
   // advance by one tile per call
-  const T* kt = kbase + (front > 0 ? 0 : (int64_t)br.lo * BN * a.sk.s);
-  const T* vt = vbase + (front > 0 ? 0 : (int64_t)br.lo * BN * a.sv.s);
+  const T* kt = kbase + (int64_t)first_tile * BN * a.sk.s;
+  const T* vt = vbase + (int64_t)first_tile * BN * a.sv.s;
   const int64_t k_step = (int64_t)BN * a.sk.s, v_step = (int64_t)BN * a.sv.s;
   const int k_row_bytes = (int)a.sk.s * 2, v_row_bytes = (int)a.sv.s * 2;
-  int rows_left = si.seqlen_k - (front > 0 ? 0 : br.lo * BN);      // > 0
-  int front_left = front;
+  int rows_left = si.seqlen_k - first_tile * BN;      // > 0
+  int front_left = front - first_tile;
   auto load_next_tile = [&]() {
     const int rows = rows_left < BN ? rows_left : BN;
     const auto krs = wave_rsrc(kt, (rows - 1) * k_row_bytes + d_qk * 2);
@@ -664,10 +675,10 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   request_bias(br.lo);
   store_tile(0);
   __syncthreads();
-  for (int j = front > 0 ? 0 : br.lo, t = 0; j <= br.hi; j = kSinks && j + 1 == front ? br.lo : j + 1, ++t) {
+  for (int j = first_tile, t = 0; kSinks ? t < tiles : j <= br.hi; j = kSinks && j + 1 == front ? br.lo : j + 1, ++t) {
     const int stage = (kSinks ? t : j - br.lo) & 1;
     store_bias(j);
-    if (j < br.hi) {
+    if (kSinks ? t + 1 < tiles : j < br.hi) {
       load_next_tile();
       request_bias(j + 1);
     }
@@ -680,7 +691,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
         sv(j, stage, masked);
       }
     }
-    if (j < br.hi) store_tile(stage ^ 1);
+    if (kSinks ? t + 1 < tiles : j < br.hi) store_tile(stage ^ 1);
     __syncthreads();
   }
 
@@ -769,6 +780,15 @@ void fwd_kernel(const FwdArgsOf<kSinks> a) {
   constexpr int kRows = kPairs ? NW * 16 : NW * 32;
   constexpr int kSmem = kPairs ? FwdPairSmem::BYTES : FwdSmem<D, BN, NW>::BYTES;
   const int zh_lo = xcd * a.zh_per_xcd;
+  if constexpr (kSinks) {
+    EvenWalk even;
+    int pos = even.template init<NW * 64>(reinterpret_cast<int*>(smem_raw + kSmem), a.seq, nseq, a.num_m_tiles, a.hk, ratio, kRows, false, xcd, threadIdx.x, kSplit ? a.splits : 1) + p;
+    for (int z, h, mt, split; even.at(pos, z, h, mt, split); pos += workers) {
+      fwd_item<T, D, NW, BN, kWindowed, kBias, kDropout, kPad, kSplit, kKeyBias, kAnyRow, kSinks>(a, z, h, mt, split, smem_raw);
+      __syncthreads();      // (the table's reads and the next item's areas)
+    }
+    return;
+  }
   RaggedWalk walk;
   LevelWalk lwalk;
   if (levels)

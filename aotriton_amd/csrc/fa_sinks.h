@@ -8,7 +8,7 @@
 //
 // One workgroup of the window's kernel per 128 keys would make the first one loop over all queries while the others loop over
 // window + 128 of them, with 124 of its 128 keys idle for 4 sinks.  So these keys are computed on their own, 32 at a time (one MFMA
-// operand), the queries of all q-heads of the group cut into parts, and the fp32 sums of the parts are added by a second kernel,
+// operand), the queries of all q-heads of the group cut into pieces of equal length, and the fp32 sums of the pieces are added by a second kernel,
 // which overwrites what the window's kernel wrote for these keys (dK and dV are rounded once):
 //   S  (queries x keys) = Q K^T, P = exp2(S c - L), dP = dO V^T, dS = P (dP - delta)
 //   dV^T (d x keys) += dO^T P,   dK^T (d x keys) += Q^T dS
@@ -31,6 +31,18 @@ struct SinkSmem {      // per wave: Q and dO rows; L and -delta.  The waves' sum
   static_assert(BYTES >= 2 * SUM_BYTES, "the sums of two waves fit");
 };
 
+// The steps of a block of 32 sinks: (q-head of the group, 32 queries), from the first query that sees one of its keys.
+struct SinkSteps {
+  int first, per_head, steps;
+  __device__ __forceinline__ SinkSteps(const SinkBwdArgs& a, const SeqInfo& si, int n0) {
+    const int shift = si.seqlen_k - si.seqlen_q;
+    first = n0 - shift > 0 ? (n0 - shift) / 32 : 0;
+    per_head = (si.seqlen_q + 31) / 32 - first;
+    steps = per_head > 0 ? per_head * (a.hq / a.hk) : 0;
+  }
+  __device__ __forceinline__ int pieces(const SinkBwdArgs& a) const { return steps > a.sink_steps ? (steps + a.sink_steps - 1) / a.sink_steps : 1; }
+};
+
 template <typename T, int D, int kPad>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256))) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1)))
 void sink_dkdv_kernel(const SinkBwdArgs a) {
@@ -49,6 +61,8 @@ void sink_dkdv_kernel(const SinkBwdArgs a) {
   const int n0 = block * 32;
   const int keys = a.sinks < si.seqlen_k ? a.sinks : si.seqlen_k;
   if (n0 >= keys) return;
+  const SinkSteps work(a, si, n0);
+  if (part >= work.pieces(a)) return;
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31, hi = lane >> 5;
   const int d_qk = kPad ? a.head_dim : D, d_v = kPad ? a.head_dim_v : D;
@@ -72,11 +86,9 @@ void sink_dkdv_kernel(const SinkBwdArgs a) {
     }
   }
 
-  // steps: (q-head of the group, 32 queries), the part's a contiguous run of them, which the waves take in turn
-  const int first = n0 - shift > 0 ? (n0 - shift) / 32 : 0;      // (no query before it sees a key of the block)
-  const int per_head = (si.seqlen_q + 31) / 32 - first;
-  const int steps = per_head > 0 ? per_head * group : 0;
-  const int t0 = (int)((int64_t)steps * part / a.sink_parts), t1 = (int)((int64_t)steps * (part + 1) / a.sink_parts);
+  // the piece's steps, which the waves take in turn
+  const int first = work.first, per_head = work.per_head;
+  const int t0 = part * a.sink_steps, t1 = t0 + a.sink_steps < work.steps ? t0 + a.sink_steps : work.steps;
 
   f32x16 dk[DB], dv[DB];
 #pragma unroll
@@ -192,10 +204,10 @@ void sink_dkdv_kernel(const SinkBwdArgs a) {
   const f32x4* in = reinterpret_cast<const f32x4*>(smem_raw);
 #pragma unroll
   for (int e = tid; e < SM::SUM_BYTES / 16; e += 256)
-    if (DC == D || e / 256 % (D / 32) < DB) out[e] = in[e] + in[e + SM::SUM_BYTES / 16];
+    if ((e & 31) < keys - n0 && (DC == D || e / 256 % (D / 32) < DB)) out[e] = in[e] + in[e + SM::SUM_BYTES / 16];      // (only keys that are there)
 }
 
-// Adds up the parts: four columns of a key's dK or dV per thread.
+// Adds up the pieces: four columns of a key's dK or dV per thread.
 template <typename T, int D>
 static __global__ __launch_bounds__(256) void sink_sum_kernel(const SinkBwdArgs a) {
   constexpr int SUMS = SinkSmem<D>::SUM_BYTES / 16, PER = SUMS / 256;      // pieces of a key block, workgroups for them
@@ -206,10 +218,11 @@ static __global__ __launch_bounds__(256) void sink_sum_kernel(const SinkBwdArgs 
   const int lane = e % 64, g = e / 64 % 4, db = e / 256 % (D / 32), which = e / (SUMS / 2);
   const int key = block * 32 + (lane & 31), col = 32 * db + 8 * g + 4 * (lane >> 5);
   if (key >= si.seqlen_k || key >= a.sinks || col >= (which ? a.head_dim_v : a.head_dim)) return;
+  const int pieces = SinkSteps(a, si, block * 32).pieces(a);
   const f32x4* p = reinterpret_cast<const f32x4*>(a.sink_ws) + ((int64_t)pair * blocks + block) * a.sink_parts * SUMS + e;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = 0; i < a.sink_parts; ++i) acc += p[(int64_t)i * SUMS];
+#pragma unroll 8
+  for (int i = 0; i < pieces; ++i) acc += p[(int64_t)i * SUMS];
   const Strides3& st = which ? a.sdv : a.sdk;
   const float f = which ? 1.0f : a.sm_scale;
   vec<T, 4> t4;
@@ -220,22 +233,30 @@ static __global__ __launch_bounds__(256) void sink_sum_kernel(const SinkBwdArgs 
 }
 
 // ---- launchers ------------------------------------------------------------------------------------------------
+// a.half_tiles, a.splits and the scratch pointers are the caller's
 template <typename T, int D, int kPad>
 hipError_t launch_fwd_sinks(const SinkFwdArgs& a, hipStream_t stream) {
   const int half = a.half_tiles, BM = half ? 128 : FwdTile<T, D, true>::BM;
   SinkFwdArgs b = a;
   b.num_m_tiles = (a.seq.max_seqlen_q + BM - 1) / BM;
-  const TileWork w = tile_work(nseq_of(a.seq, a.batch) * a.hq, q_head_group(a.hq, a.hk), b.num_m_tiles);
+  const TileWork w = tile_work(nseq_of(a.seq, a.batch) * a.hq, q_head_group(a.hq, a.hk), b.num_m_tiles * (a.splits > 1 ? a.splits : 1));
   b.num_zh = w.num_zh; b.zh_per_xcd = w.zh_per_xcd; b.zh_group = w.zh_group; b.items_per_xcd = w.items_per_xcd;
   const dim3 grid((unsigned)(kNumXcd * tile_workers(w.items_per_xcd, a.num_cu, half ? half : 1)));
-  if (half) return launch_fwd_variant<T, D, true, false, false, kPad, false, false, FwdHalfTile<D>, false, true>(b, grid, stream);
-  return launch_fwd_variant<T, D, true, false, false, kPad, false, false, FwdTile<T, D, true>, false, true>(b, grid, stream);
+  using Half = FwdHalfTile<D>;
+  using Whole = FwdTile<T, D, true>;
+  if (a.splits > 1) {
+    b.part_group = 1; b.part_block = BM; b.part_rows = BM; b.row_blocks = b.num_m_tiles;
+    if (half) return launch_fwd_variant<T, D, true, false, false, kPad, true, false, Half, false, true>(b, grid, stream);
+    return launch_fwd_variant<T, D, true, false, false, kPad, true, false, Whole, false, true>(b, grid, stream);
+  }
+  if (half) return launch_fwd_variant<T, D, true, false, false, kPad, false, false, Half, false, true>(b, grid, stream);
+  return launch_fwd_variant<T, D, true, false, false, kPad, false, false, Whole, false, true>(b, grid, stream);
 }
 
 // dK and dV of the window's keys, and over them those of the sinks
 template <typename T, int D, int kPad>
 hipError_t launch_dkdv_sinks(const SinkBwdArgs& a, hipStream_t stream) {
-  hipError_t e = launch_dkdv_form<T, D, kPad, true, false, false, false, false, kBiasAny, true>(a, stream);
+  hipError_t e = a.wide ? hipSuccess : launch_dkdv_form<T, D, kPad, true, false, false, false, false, kBiasAny, true>(a, stream);
   const int pairs = bwd_nseq(a) * a.hk, blocks = (a.sinks + 31) / 32;
   if (e != hipSuccess || blocks == 0 || pairs == 0 || a.seq.max_seqlen_k <= 0) return e;
   e = launch_with_lds<sink_dkdv_kernel<T, D, kPad>>(dim3((unsigned)(pairs * blocks * a.sink_parts)), 256, SinkSmem<D>::BYTES, stream, a);

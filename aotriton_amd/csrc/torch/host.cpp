@@ -516,7 +516,8 @@ std::tuple<Tensor, Tensor> sink_forward_kernel(const Tensor& q_in, const Tensor&
   if (o.stride(-1) != 1) o = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
   Tensor lse = at::empty({packed ? q.size(1) : q.size(0) * q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
   TORCH_CHECK(view2(lse, &p.L) && view4(o, &p.Out), "outputs");
-  check_rc(fa_attn_fwd_sinks(&p, FA_FWD_PARAMS_VERSION, w, n, current_stream(), nullptr), false);
+  Scratch scratch;
+  check_rc(fa_attn_fwd_sinks(&p, FA_FWD_PARAMS_VERSION, w, n, current_stream(), nullptr, &scratch.c), false);
   return {std::move(o), std::move(lse)};
 }
 

@@ -282,13 +282,14 @@ FA_API int fa_attn_bwd(const fa_bwd_params* params, int32_t params_version,
  * (more queries than keys) gives 0 and a logsumexp of +inf, and no gradient.  params->causal_type is FA_CAUSAL_NONE: the two
  * numbers are the mask.  FA_ERROR_INVALID_VALUE: window < 1, sinks < 0, another causal_type; FA_ERROR_NOT_SUPPORTED: a bias, dropout,
  * encoded_softmax, other element types, head dims or alignment, sinks > FA_MAX_SINKS; all before anything is launched.
- * The backward takes scratch memory for fp32 sums of the sinks' gradients (all queries add to them): from `alloc`, as
- * fa_attn_fwd_alloc describes it, or without one from the library's workspace; FA_ERROR_OUT_OF_MEMORY where there is none (stream
- * capture without an allocator, the limit), with nothing launched.  It needs params->D, has no single-launch backend and no
+ * Both take scratch memory from `alloc`, as fa_attn_fwd_alloc describes it, or without one from the library's workspace.  The forward
+ * splits the keys of calls with few rows over workgroups, and without scratch does not.  The backward adds up fp32 sums of the sinks'
+ * gradients, which all queries contribute to; FA_ERROR_OUT_OF_MEMORY where there is no scratch (stream capture without an allocator, the
+ * limit), with nothing launched.  It needs params->D, has no single-launch backend and no
  * atomics: results do not change from call to call.  No counterpart in the reference. */
 #define FA_MAX_SINKS 1024
 FA_API int fa_attn_fwd_sinks(const fa_fwd_params* params, int32_t params_version, int32_t window, int32_t sinks,
-                             void* hip_stream, const fa_options* options);
+                             void* hip_stream, const fa_options* options, fa_allocator* alloc);
 FA_API int fa_attn_bwd_sinks(const fa_bwd_params* params, int32_t params_version, int32_t window, int32_t sinks,
                              void* hip_stream, const fa_options* options, fa_allocator* alloc);
 

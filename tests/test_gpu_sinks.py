@@ -120,7 +120,7 @@ def test_rows_behind_the_last_sequence_stay():
     c.Max_seqlen_q = c.Max_seqlen_k = 90
     c.varlen_type = 1
     c.Sm_scale = 0.125
-    assert lib.fa_attn_fwd_sinks(ctypes.byref(c), 3, 30, 4, torch.cuda.current_stream().cuda_stream, None) == 0
+    assert lib.fa_attn_fwd_sinks(ctypes.byref(c), 3, 30, 4, torch.cuda.current_stream().cuda_stream, None, None) == 0
     torch.cuda.synchronize()
     # (the logsumexp of packed sequences is (heads, tokens up to the last offset))
     flat = lse.flatten()

@@ -46,7 +46,7 @@ def _fwd(D=64, dtype=torch.bfloat16, Sq=100, Sk=100, **change):
 
 
 def _run_fwd(p, window=10, sinks=4, version=3, options=None):
-    return _lib().lib.fa_attn_fwd_sinks(ctypes.byref(p), version, window, sinks, None, options)
+    return _lib().lib.fa_attn_fwd_sinks(ctypes.byref(p), version, window, sinks, None, options, None)
 
 
 ACCEPTED = (0, NO_GPU)      # (the device is asked after the arguments: none here)
