@@ -1388,10 +1388,10 @@ SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, int32_t window, int32_
   double least = 0;
   const int64_t seqs = s.num_seqlens != 0 ? std::abs(s.num_seqlens) : s.batch;
   for (int half = 0; half < 2; ++half) {
-    const int bm = half ? 128 : 256, per_cu = half ? 2 : 1;
+    const int shift = fa::sink_head_shift(s.hq, s.hk, half ? 4 : 8), bm = (half ? 128 : 256) >> shift, per_cu = half ? 2 : 1;
     const double item = s.d > 64 ? (half ? 6.5 : 6.3) : (half ? 4.5 : 4.35), step = s.d > 64 ? (half ? 1.8 : 1.74) : (half ? 1.2 : 1.12);
     const int64_t keys = std::min<int64_t>(s.max_sk, (int64_t)window + bm) + std::min<int64_t>(sinks, 64), tiles = (keys + 63) / 64;
-    const int64_t items = sink_tiles(s, s.hq, false, tokens, bm), stored = seqs * s.hq * ((s.max_sq + bm - 1) / bm) * bm;
+    const int64_t items = sink_tiles(s, s.hq >> shift, false, tokens, bm), stored = seqs * s.hq * ((s.max_sq + bm - 1) / bm) * bm;
     for (int splits = 1; splits <= 8 && (splits == 1 || (s.num_seqlens == 0 && splits * 2 <= tiles)); ++splits) {
       const int64_t o_bytes = splits > 1 ? stored * splits * s.d * 4 : 0, bytes = splits > 1 ? o_bytes + stored * splits * 8 : 0;
       const double t = rounds_time(items * splits, (int64_t)per_cu * num_cu, item + step * ((tiles + splits - 1) / splits)) +
@@ -1411,10 +1411,12 @@ SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, int32_t window, int32_
 struct SinkBwdRoute { bool wide_dq, wide_dkdv; };
 SinkBwdRoute sink_bwd_route(const Shape& s, int64_t tokens_q, int64_t tokens_k, int32_t window, int num_cu) {
   if (s.d != 128) return SinkBwdRoute{false, false};
-  auto time = [&](bool keys, int tile, int step, double item, double cost) {
+  const int shift = fa::sink_head_shift(s.hq, s.hk, 4);
+  auto time = [&](bool keys, int rows, int step, double item, double cost) {
+    const int tile = keys ? rows : rows >> shift;
     const int64_t span = std::min<int64_t>(keys ? s.max_sq : s.max_sk, (int64_t)window - 1 + tile);
     const double steps = (keys ? s.hq / s.hk : 1) * (double)(span / step + 1) + (keys ? 0 : 1);
-    return rounds_time(sink_tiles(s, keys ? s.hk : s.hq, keys, keys ? tokens_k : tokens_q, tile), num_cu, item + cost * steps);
+    return rounds_time(sink_tiles(s, keys ? s.hk : s.hq >> shift, keys, keys ? tokens_k : tokens_q, tile), num_cu, item + cost * steps);
   };
   return SinkBwdRoute{time(false, 256, 32, 5, 1.42) < 0.95 * time(false, 128, 64, 5, 1.7),
                       time(true, 256, 32, 7, 1.8) < time(true, 128, 64, 9, 1.95)};

@@ -208,6 +208,7 @@ struct BwdArgs {
 // (Blocks of their own, and not members of the ones above: the kernels without sinks keep their argument layout and so their code.)
 struct SinkFwdArgs : FwdArgs {
   int32_t window, sinks;
+  int32_t head_shift;    // a tile holds fewer rows of 2^head_shift heads (sink_head_shift)
 };
 struct SinkBwdArgs : BwdArgs {
   int32_t window, sinks;
@@ -215,8 +216,20 @@ struct SinkBwdArgs : BwdArgs {
   // (fa_sinks.h)
   int32_t sink_parts, sink_steps;
   int32_t wide;          // the window's part of dK and dV is another launch's (64 keys per wave)
+  int32_t head_shift;    // as in SinkFwdArgs, of the dQ kernel
   float* sink_ws;
 };
+
+// Query heads that share a K/V head take the waves of one workgroup, each with the same rows: as many heads as divide
+// the group and there are waves for.  A tile of R rows visits window + R keys, and R is so much smaller, with the same K
+// and V for all waves.  (us, the waves' rows from one head -> from four, bf16 D128: Hq 32 Hk 8 S8192 window 1024 forward
+// 215 -> 183, dQ 291 -> 251; 16 packed sequences of up to 6000, Hq 16 Hk 4, window 512 forward 245 -> 213, dQ 397 -> 315;
+// S32768 window 4096 forward 2117 -> 2040.)
+inline int32_t sink_head_shift(int32_t hq, int32_t hk, int32_t waves) {
+  int32_t n = 0;
+  while ((2 << n) <= waves && hq / hk % (2 << n) == 0) ++n;
+  return n;
+}
 
 template <bool kSinks> using FwdArgsOf = std::conditional_t<kSinks, SinkFwdArgs, FwdArgs>;
 template <bool kSinks> using BwdArgsOf = std::conditional_t<kSinks, SinkBwdArgs, BwdArgs>;

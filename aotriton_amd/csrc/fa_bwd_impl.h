@@ -899,14 +899,13 @@ __device__ __forceinline__ void dkdv_item(const BwdArgsOf<kSinks>& a, const int 
 // the split backward has no preprocess launch, the dK/dV kernel runs after this one and reads it.
 template <typename T, int D, int NW, int BN, bool kWindowed, bool kBias, bool kDropout, bool kInlineDelta, int kPad,
           bool kStoreDelta = false, bool kSinks = false>
-__device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h, const int mt, const int z,
+__device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h0, const int mt, const int z,
                                         char* smem_raw) {
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
   using q4_t = typename Tr::q4_t;
   using SM = DqSmem<D, BN>;
   constexpr int NT = NW * 64;
-  constexpr int BM = NW * 32;
   constexpr int DC = kPad ? kPad : D;            // columns computed; those past a tensor's head dim are zero
   constexpr int KS = DC / 16, MB = BN / 32, DB = DC / 32, TS = BN / 16;
   constexpr int CH = (BN * D / 8) / NT;          // 16-byte chunks per thread, per tensor
@@ -914,6 +913,11 @@ __device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h,
 
   const int tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63, c = lane & 31, hi = lane >> 5;
+  // as in fwd_item: BM rows of a head, the wave's place among those that share one
+  int shift = 0;
+  if constexpr (kSinks) shift = a.head_shift;
+  const int BM = NW * 32 >> shift, rw = wave >> shift;
+  const int h = kSinks ? h0 + (__builtin_amdgcn_readfirstlane(wave) & ((1 << shift) - 1)) : h0;
   // columns of Q/K/dQ/dK and of V/Out/dOut/dV: <= D, multiples of 8; constants unless a head dim is rounded up
   const int d_qk = kPad ? a.head_dim : D, d_v = kPad ? a.head_dim_v : D;
 
@@ -930,7 +934,7 @@ __device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h,
   const BlockRanges br = block_ranges(kWindowed, w.left, w.right, q0, si.seqlen_q, si.seqlen_k, BM, BN);
 
   const int hk = h / (a.hq / a.hk);
-  const int row = q0 + wave * 32 + c;
+  const int row = q0 + rw * 32 + c;
   const bool row_ok = row < si.seqlen_q;
   const int row_c = row_ok ? row : si.seqlen_q - 1;
 
@@ -968,7 +972,7 @@ __device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h,
                      (reinterpret_cast<uintptr_t>(a.db) & 15) == 0;
     const op_t zero8 = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int rr = 0; rr < 32; ++rr) {
-      const int m = q0 + wave * 32 + rr;
+      const int m = q0 + rw * 32 + rr;
       if (m >= si.seqlen_q) break;
       T* rowp = dbase + (int64_t)m * a.sdb_m;
       if (vec) {
@@ -1041,7 +1045,7 @@ __device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h,
     d_row = cross_sum(acc);
     if (kStoreDelta) {
       // (through a descriptor instead of a branch: lanes with hi set and rows past the sequence write nothing)
-      const int first = q0 + wave * 32, rows = si.seqlen_q - first;
+      const int first = q0 + rw * 32, rows = si.seqlen_q - first;
       const auto rs = wave_rsrc(a.delta + lse_offset(si, h, a.hq) + first, rows < 0 ? 0 : rows < 32 ? rows * 4 : 128);
       __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, d_row), rs, hi ? kVoffOutOfRange : c * 4, 0, 0);
     }
@@ -1130,7 +1134,7 @@ __device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h,
   static_assert(!kDirect || RPI % 8 == 0, "the swizzle must repeat every two pieces");
   op_t kch[kDirect ? 1 : CH], vch[kDirect ? 1 : CH];
   const int r0 = tid / LPR, cc0 = tid % LPR;
-  const int wave_u = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave_u = __builtin_amdgcn_readfirstlane(tid >> 6), rw_u = wave_u >> shift;
   int f_stage = 0;                               // stage the running fetch fills
   int k_voff_d[2] = {0, 0}, v_voff_d[2] = {0, 0};
   if (kDirect) {
@@ -1237,7 +1241,7 @@ __device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h,
     if (kBias && tile_co) {
 #pragma unroll
       for (int i = 0; i < BNI; ++i) {
-        int m = q0 + wave * 32 + brow + BRPI * i;
+        int m = q0 + rw * 32 + brow + BRPI * i;
         m = m < si.seqlen_q ? m : si.seqlen_q - 1;
         if constexpr (kStoreDelta) bco[i] = load_row_piece<T, false>(bias_head + (int64_t)m * a.sb_m, j * BN + bch * 8, 0);
         else bco[i] = *reinterpret_cast<const op_t*>(bias_head + (int64_t)m * a.sb_m + j * BN + bch * 8);
@@ -1375,7 +1379,7 @@ __device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h,
         dp[E / 16][E % 16] -= off;
         ds_el(E);
       }
-      const int first = q0 + wave_u * 32, rows = si.seqlen_q - first;
+      const int first = q0 + rw_u * 32, rows = si.seqlen_q - first;
       const auto rs = wave_rsrc(a.delta + lse_offset(si, h, a.hq) + first, rows < 0 ? 0 : rows < 32 ? rows * 4 : 128);
       __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, d_row + off), rs, hi ? kVoffOutOfRange : c * 4, 0, 0);
     }
@@ -1405,7 +1409,7 @@ __device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h,
       // the wave's dB tile leaves as whole 16-byte pieces of its rows
 #pragma unroll
       for (int i = 0; i < BNI; ++i) {
-        const int m = q0 + wave * 32 + brow + BRPI * i;
+        const int m = q0 + rw * 32 + brow + BRPI * i;
         const op_t x = *reinterpret_cast<const op_t*>(bw + (brow + BRPI * i) * SM::BIAS_ROW + bch * 16);
         if constexpr (kStoreDelta) {
           if (m < si.seqlen_q) __builtin_memcpy(db_head + (int64_t)m * a.sdb_m + j * BN + bch * 8, &x, 16);
@@ -1429,7 +1433,7 @@ __device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h,
     bool one_tile = false;      // all keys that the wave's rows see lie in the first tile
     if constexpr (kSinks) {
       if (front > 0) j = 0;
-      const int last = q0 + wave_u * 32 + 31 < si.seqlen_q ? q0 + wave_u * 32 + 31 : si.seqlen_q - 1;
+      const int last = q0 + rw_u * 32 + 31 < si.seqlen_q ? q0 + rw_u * 32 + 31 : si.seqlen_q - 1;
       one_tile = si.seqlen_k <= BN || last + w.right < BN;
     }
     auto step = [&](auto masked_tag, auto fast_tag) __attribute__((always_inline)) {
@@ -1557,10 +1561,10 @@ void bwd_dq_kernel(const BwdArgsOf<kSinks> a) {
   const int xcd = blockIdx.x % kNumXcd, p = blockIdx.x / kNumXcd, workers = gridDim.x / kNumXcd;
   if constexpr (kSinks) {
     EvenWalk even;
-    int pos = even.template init<NW * 64>(reinterpret_cast<int*>(smem_raw + DqSmem<D, BN>::BYTES), a.seq, a.num_zh / a.hq, a.num_m_tiles, a.hk, a.hq / a.hk,
-                                          NW * 32, false, xcd, threadIdx.x) + p;
+    int pos = even.template init<NW * 64>(reinterpret_cast<int*>(smem_raw + DqSmem<D, BN>::BYTES), a.seq, a.num_zh / a.hq, a.num_m_tiles, a.hk,
+                                          a.hq / a.hk >> a.head_shift, NW * 32 >> a.head_shift, false, xcd, threadIdx.x) + p;
     for (int z, h, mt; even.at(pos, z, h, mt); pos += workers) {
-      dq_item<T, D, NW, BN, kWindowed, kBias, kDropout, true, kPad, true, kSinks>(a, h, mt, z, smem_raw);
+      dq_item<T, D, NW, BN, kWindowed, kBias, kDropout, true, kPad, true, kSinks>(a, h << a.head_shift, mt, z, smem_raw);
       __syncthreads();     // the next item reuses the LDS stages
     }
     return;
@@ -1721,7 +1725,14 @@ hipError_t launch_dq_variant(const BwdArgsOf<kSinks>& a0, hipStream_t stream) {
   constexpr int NW = Tile::NW, BN = kDqBN<T, D, W, B>, BM = NW * 32;
   BwdArgsOf<kSinks> a = a0;
   a.num_m_tiles = (a.seq.max_seqlen_q + BM - 1) / BM;
+  int items = 0;
+  if constexpr (kSinks) {
+    a.head_shift = sink_head_shift(a.hq, a.hk, NW);
+    a.num_m_tiles = (a.seq.max_seqlen_q + (BM >> a.head_shift) - 1) / (BM >> a.head_shift);
+    items = tile_work(bwd_nseq(a) * (a.hq >> a.head_shift), 1, a.num_m_tiles).items_per_xcd;
+  }
   set_work(a, tile_work(bwd_nseq(a) * a.hq, q_head_group(a.hq, a.hk), a.num_m_tiles));
+  if constexpr (kSinks) a.items_per_xcd = items;
   dim3 grid((unsigned)(kNumXcd * bwd_workers(D, B, a.items_per_xcd, a.num_cu, kTwoWaves<D, B> ? 2 : 1)));
   return launch_with_lds<bwd_dq_kernel<T, D, NW, BN, W, B, P, kPad, kSinks>>(grid, NW * 64, DqSmem<D, BN>::BYTES + (kSinks ? kLevelBytes : 0), stream, a);
 }

@@ -472,8 +472,8 @@ struct WideDqSmem {
 };
 
 template <typename T, bool kWindowed, int kPad, bool kSinks = false>
-__device__ __forceinline__ void dq_wide_item(const BwdArgsOf<kSinks>& a, const int h, const int mt, const int z, char* smem_raw) {
-  constexpr int D = 128, BM = kWideBN, BN = kWideBM, QB = 2;
+__device__ __forceinline__ void dq_wide_item(const BwdArgsOf<kSinks>& a, const int h0, const int mt, const int z, char* smem_raw) {
+  constexpr int D = 128, BN = kWideBM, QB = 2;
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
   using q4_t = typename Tr::q4_t;
@@ -489,6 +489,11 @@ __device__ __forceinline__ void dq_wide_item(const BwdArgsOf<kSinks>& a, const i
   const int d_qk = kPad ? a.head_dim : D, d_v = kPad ? a.head_dim_v : D;
 
   const SeqInfo si = uniform(get_seq(a.seq, z));
+  // as in fwd_item: BM rows of a head
+  int shift = 0;
+  if constexpr (kSinks) shift = a.head_shift;
+  const int BM = kWideBN >> shift;
+  const int h = kSinks ? h0 + (wave & ((1 << shift) - 1)) : h0;
   const int q0 = mt * BM;
   if (q0 >= si.seqlen_q) return;
 
@@ -498,7 +503,7 @@ __device__ __forceinline__ void dq_wide_item(const BwdArgsOf<kSinks>& a, const i
   w.left = w.left > (1 << 30) ? (1 << 30) : (w.left < -(1 << 30) ? -(1 << 30) : w.left);
   w.right = w.right > (1 << 30) ? (1 << 30) : (w.right < -(1 << 30) ? -(1 << 30) : w.right);
   const BlockRanges br = block_ranges(kWindowed, w.left, w.right, q0, si.seqlen_q, si.seqlen_k, BM, BN);
-  const int qw = q0 + 64 * wave;
+  const int qw = q0 + 64 * (wave >> shift);
   const BlockRanges wr = block_ranges(kWindowed, w.left, w.right, qw, si.seqlen_q, si.seqlen_k, 64, BN);
   // kSinks, as in dq_item: tiles before the window's first, in which only sinks are visible
   int sinks = 0;
@@ -825,10 +830,10 @@ void bwd_dq_wide_kernel(const BwdArgsOf<kSinks> a) {
   const int xcd = blockIdx.x % kNumXcd, p = blockIdx.x / kNumXcd, workers = gridDim.x / kNumXcd;
   if constexpr (kSinks) {
     EvenWalk even;
-    int pos = even.template init<256>(reinterpret_cast<int*>(smem_raw + WideDqSmem::BYTES), a.seq, a.num_zh / a.hq, a.num_m_tiles, a.hk, a.hq / a.hk, kWideBN,
-                                      false, xcd, threadIdx.x) + p;
+    int pos = even.template init<256>(reinterpret_cast<int*>(smem_raw + WideDqSmem::BYTES), a.seq, a.num_zh / a.hq, a.num_m_tiles, a.hk, a.hq / a.hk >> a.head_shift,
+                                      kWideBN >> a.head_shift, false, xcd, threadIdx.x) + p;
     for (int z, h, mt; even.at(pos, z, h, mt); pos += workers) {
-      dq_wide_item<T, kWindowed, kPad, kSinks>(a, h, mt, z, smem_raw);
+      dq_wide_item<T, kWindowed, kPad, kSinks>(a, h << a.head_shift, mt, z, smem_raw);
       __syncthreads();
     }
     return;
@@ -869,7 +874,14 @@ template <typename T, bool W, int kPad, bool kSinks = false>
 hipError_t launch_dq_wide(const BwdArgsOf<kSinks>& a0, hipStream_t stream) {
   BwdArgsOf<kSinks> a = a0;
   a.num_m_tiles = (a.seq.max_seqlen_q + kWideBN - 1) / kWideBN;
+  int items = 0;
+  if constexpr (kSinks) {
+    a.head_shift = sink_head_shift(a.hq, a.hk, 4);
+    a.num_m_tiles = (a.seq.max_seqlen_q + (kWideBN >> a.head_shift) - 1) / (kWideBN >> a.head_shift);
+    items = tile_work(bwd_nseq(a) * (a.hq >> a.head_shift), 1, a.num_m_tiles).items_per_xcd;
+  }
   set_work(a, tile_work(bwd_nseq(a) * a.hq, a.walk_group, a.num_m_tiles));
+  if constexpr (kSinks) a.items_per_xcd = items;
   dim3 grid((unsigned)(kNumXcd * bwd_workers(128, false, a.items_per_xcd, a.num_cu, 1)));
   return launch_with_lds<bwd_dq_wide_kernel<T, W, kPad, kSinks>>(grid, 256, WideDqSmem::BYTES + kLevelBytes, stream, a);
 }

@@ -45,14 +45,13 @@ struct FwdSmem {
 // the `front` ones that only the first keys are visible in, and those of the window, as one run of tiles with a jump in it.
 template <typename T, int D, int NW, int BN, bool kWindowed, bool kBias, bool kDropout, int kPad, bool kSplit, bool kKeyBias,
           bool kAnyRow, bool kSinks>
-__device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z, const int h, const int mt, const int split,
+__device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z, const int h0, const int mt, const int split,
                                          char* smem_raw) {
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
   using q4_t = typename Tr::q4_t;
   using SM = FwdSmem<D, BN, NW>;
   constexpr int NT = NW * 64;
-  constexpr int BM = NW * 32;
   constexpr int DC = kPad ? kPad : D;   // columns computed; those past a tensor's head dim are zero
   constexpr int KS = DC / 16;   // k-steps of S^T = K Q^T
   constexpr int MB = BN / 32;   // 32-key blocks per tile
@@ -68,6 +67,11 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   const int tid = threadIdx.x;
   const int wave = tid >> 6;
   const int lane = tid & 63, c = lane & 31, hi = lane >> 5;
+  // BM rows of a head; `rw` is the wave's place among those that share a head (SinkFwdArgs::head_shift)
+  int shift = 0;
+  if constexpr (kSinks) shift = a.head_shift;
+  const int BM = NW * 32 >> shift, rw = wave >> shift;
+  const int h = kSinks ? h0 + (__builtin_amdgcn_readfirstlane(wave) & ((1 << shift) - 1)) : h0;
   // columns of Q/K and of V/Out: <= D, multiples of 8; constants unless a head dim is rounded up
   const int d_qk = kPad ? a.head_dim : D, d_v = kPad ? a.head_dim_v : D;
 
@@ -106,7 +110,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   }
 
   const int hk = h / (a.hq / a.hk);                       // fwd_kernel.py:360
-  const int row = q0 + wave * 32 + c;                     // this lane's query row
+  const int row = q0 + rw * 32 + c;                     // this lane's query row
   const bool row_ok = row < si.seqlen_q;
   const int row_c = row_ok ? row : si.seqlen_q - 1;
 
@@ -114,7 +118,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
             (int64_t)(si.q_start + row_c) * a.so.s;
   float* lse_ptr = a.lse ? a.lse + lse_offset(si, h, a.hq) : nullptr;
 
-  const int64_t part_row = kSplit ? (((int64_t)z * a.hq + h) * a.num_m_tiles + mt) * (int64_t)(a.splits * BM) + split * BM + wave * 32 + c : 0;
+  const int64_t part_row = kSplit ? (((int64_t)z * a.hq + h) * a.num_m_tiles + mt) * (int64_t)(a.splits * BM) + split * BM + rw * 32 + c : 0;
   if (kSplit && (kSinks ? tiles <= 0 : br.lo > br.hi)) {
     if (row_ok && hi == 0) {
       a.part_ml[part_row * 2] = kNegBig;
@@ -149,8 +153,8 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   // and a register spilled next to one of them was stored while no lane was enabled (the loop
   // leaves exec at zero and the spill landed before exec is restored), so that the fourth Q piece
   // of a D = 64 bias + dropout build was fetched from wherever the slot's old content pointed.
-  const int wave_u = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wrows = si.seqlen_q - q0 - wave_u * 32 < 32 ? si.seqlen_q - q0 - wave_u * 32 : 32;   // may be <= 0
+  const int wave_u = __builtin_amdgcn_readfirstlane(tid >> 6), rw_u = wave_u >> shift;
+  const int wrows = si.seqlen_q - q0 - rw_u * 32 < 32 ? si.seqlen_q - q0 - rw_u * 32 : 32;   // may be <= 0
   const int rq = lane / LPRQ, cq = lane % LPRQ;
   const T* kbase = reinterpret_cast<const T*>(a.k) + (int64_t)si.batch_index * a.sk.z +
                    (int64_t)hk * a.sk.h + (int64_t)si.k_start * a.sk.s;
@@ -245,7 +249,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   op_t qreg[KS];
   {
     const T* qw = reinterpret_cast<const T*>(a.q) + (int64_t)si.batch_index * a.sq.z + (int64_t)h * a.sq.h +
-                  (int64_t)(si.q_start + q0 + wave_u * 32) * a.sq.s;
+                  (int64_t)(si.q_start + q0 + rw_u * 32) * a.sq.s;
     const auto qrs = wave_rsrc(qw, wrows > 0 ? ((wrows - 1) * (int)a.sq.s + d_qk) * 2 : 0);
     const int qvoff = cq * 8 < d_qk ? rq * (int)a.sq.s * 2 + cq * 16 : kVoffOutOfRange;
     op_t qin[32 / RPQ];
@@ -295,7 +299,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   // see nothing in the trailing K tiles and only take part in staging and barriers
   int wave_hi = br.hi;
   if (kWindowed) {
-    const int64_t wl = (int64_t)(q0 + wave * 32 + 31 < si.seqlen_q ? q0 + wave * 32 + 31 : si.seqlen_q - 1);
+    const int64_t wl = (int64_t)(q0 + rw * 32 + 31 < si.seqlen_q ? q0 + rw * 32 + 31 : si.seqlen_q - 1);
     int64_t cmax = wl + w.right;
     if (cmax > si.seqlen_k - 1) cmax = si.seqlen_k - 1;
     wave_hi = cmax < 0 ? -1 : (int)(cmax / BN);
@@ -307,7 +311,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   // A K tile needs no mask in this wave when every key of it is visible to every (valid) row of
   // the wave: the tile ends inside the sequence, at or before the first row's right bound, and
   // starts at or after the last row's left bound.
-  const int w_rmin = q0 + wave * 32;
+  const int w_rmin = q0 + rw * 32;
   const int w_rmax = w_rmin + 31 < si.seqlen_q ? w_rmin + 31 : si.seqlen_q - 1;
   auto wave_sees_all = [&](int j) -> bool {
     const int n_first = j * BN, n_last = j * BN + BN - 1;
@@ -349,7 +353,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   constexpr int BNI = 32 / BRPI;          // accesses per chunk
   const int brow = lane / BLPR, bch = lane % BLPR;
   const int b_row = kBias ? (int)a.sb_m * 2 : 0;
-  const int b_first = q0 + wave_u * 32 < si.seqlen_q ? q0 + wave_u * 32 : si.seqlen_q - 1;
+  const int b_first = q0 + rw_u * 32 < si.seqlen_q ? q0 + rw_u * 32 : si.seqlen_q - 1;
   const char* bias_tile = reinterpret_cast<const char*>(a.bias) +
                           2 * ((int64_t)si.batch_index * a.sb_z + (int64_t)h * a.sb_h + (int64_t)b_first * a.sb_m);
   const bool bias_co = kBias && a.sb_n == 1 &&
@@ -360,7 +364,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
   auto bias_put = [&](int i, op_t x) { *reinterpret_cast<op_t*>(rowbuf + (brow + BRPI * i) * SM::ROW_STR + bch * 16) = x; };
   auto bias_piece = [&](auto end_tag, int j, int i) {
     const T* bh = reinterpret_cast<const T*>(a.bias) + (int64_t)si.batch_index * a.sb_z + (int64_t)h * a.sb_h;
-    int m = q0 + wave * 32 + brow + BRPI * i;
+    int m = q0 + rw * 32 + brow + BRPI * i;
     m = m < si.seqlen_q ? m : si.seqlen_q - 1;
     return load_row_piece<T, decltype(end_tag)::value>(bh + (int64_t)m * a.sb_m, j * BN + bch * 8, si.seqlen_k);
   };
@@ -727,7 +731,7 @@ __device__ __forceinline__ void fwd_item(const FwdArgsOf<kSinks>& a, const int z
     }
   {
     T* ow = reinterpret_cast<T*>(a.out) + (int64_t)si.batch_index * a.so.z + (int64_t)h * a.so.h +
-            (int64_t)(si.q_start + q0 + wave_u * 32) * a.so.s;
+            (int64_t)(si.q_start + q0 + rw_u * 32) * a.so.s;
     const auto ors = wave_rsrc(ow, wrows > 0 ? ((wrows - 1) * (int)a.so.s + d_v) * 2 : 0);
     const int ovoff = cq * 8 < d_v ? rq * (int)a.so.s * 2 + cq * 16 : kVoffOutOfRange;
 #pragma unroll
@@ -782,9 +786,10 @@ void fwd_kernel(const FwdArgsOf<kSinks> a) {
   const int zh_lo = xcd * a.zh_per_xcd;
   if constexpr (kSinks) {
     EvenWalk even;
-    int pos = even.template init<NW * 64>(reinterpret_cast<int*>(smem_raw + kSmem), a.seq, nseq, a.num_m_tiles, a.hk, ratio, kRows, false, xcd, threadIdx.x, kSplit ? a.splits : 1) + p;
+    int pos = even.template init<NW * 64>(reinterpret_cast<int*>(smem_raw + kSmem), a.seq, nseq, a.num_m_tiles, a.hk, ratio >> a.head_shift,
+                                          kRows >> a.head_shift, false, xcd, threadIdx.x, kSplit ? a.splits : 1) + p;
     for (int z, h, mt, split; even.at(pos, z, h, mt, split); pos += workers) {
-      fwd_item<T, D, NW, BN, kWindowed, kBias, kDropout, kPad, kSplit, kKeyBias, kAnyRow, kSinks>(a, z, h, mt, split, smem_raw);
+      fwd_item<T, D, NW, BN, kWindowed, kBias, kDropout, kPad, kSplit, kKeyBias, kAnyRow, kSinks>(a, z, h << a.head_shift, mt, split, smem_raw);
       __syncthreads();      // (the table's reads and the next item's areas)
     }
     return;

@@ -236,11 +236,14 @@ static __global__ __launch_bounds__(256) void sink_sum_kernel(const SinkBwdArgs 
 // a.half_tiles, a.splits and the scratch pointers are the caller's
 template <typename T, int D, int kPad>
 hipError_t launch_fwd_sinks(const SinkFwdArgs& a, hipStream_t stream) {
-  const int half = a.half_tiles, BM = half ? 128 : FwdTile<T, D, true>::BM;
+  const int half = a.half_tiles, waves = half ? 4 : 8;
+  static_assert(FwdTile<T, D, true>::BM == 256, "eight waves");
   SinkFwdArgs b = a;
+  b.head_shift = sink_head_shift(a.hq, a.hk, waves);
+  const int BM = waves * 32 >> b.head_shift, nseq = nseq_of(a.seq, a.batch);
   b.num_m_tiles = (a.seq.max_seqlen_q + BM - 1) / BM;
-  const TileWork w = tile_work(nseq_of(a.seq, a.batch) * a.hq, q_head_group(a.hq, a.hk), b.num_m_tiles * (a.splits > 1 ? a.splits : 1));
-  b.num_zh = w.num_zh; b.zh_per_xcd = w.zh_per_xcd; b.zh_group = w.zh_group; b.items_per_xcd = w.items_per_xcd;
+  b.num_zh = nseq * a.hq;
+  const TileWork w = tile_work(nseq * (a.hq >> b.head_shift), 1, b.num_m_tiles * (a.splits > 1 ? a.splits : 1));
   const dim3 grid((unsigned)(kNumXcd * tile_workers(w.items_per_xcd, a.num_cu, half ? half : 1)));
   using Half = FwdHalfTile<D>;
   using Whole = FwdTile<T, D, true>;
