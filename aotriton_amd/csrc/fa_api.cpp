@@ -1495,25 +1495,35 @@ int fa_attn_bwd_sinks(const fa_bwd_params* p, int32_t params_version, int32_t wi
   a.window = window_of(window);
   a.sinks = std::min(sinks, s.max_sk);
 
-  // Pieces of the sinks' sums: one round of workgroups (two on a CU at 64 columns, one at 128), of eight steps at least.
+  // The sinks' dK and dV: a piece for every workgroup that the chip takes at once (two on a CU at 64 columns, one at 128), of
+  // eight steps at least; of packed sequences a list, unless the longest is no more than half a piece of it.
   const int64_t seqs = s.num_seqlens != 0 ? std::abs(s.num_seqlens) : s.batch, blocks = (a.sinks + 31) / 32;
   const int64_t items = seqs * s.hk * blocks, longest = (int64_t)(s.hq / s.hk) * ((s.max_sq + 31) / 32);
-  const int64_t steps = s.num_seqlens > 0 ? (int64_t)s.hq * ((int64_t)p->Q.sizes[2] / 32 + seqs) : seqs * s.hk * longest;
+  const int64_t steps = s.num_seqlens > 0 ? (int64_t)s.hq * ((int64_t)p->Q.sizes[2] / 32 + seqs) * blocks : items * longest;
   const int64_t chip = (int64_t)(s.d == 64 ? 2 : 1) * dev->num_cu;
-  a.sink_steps = (int32_t)std::max<int64_t>(8, (steps * blocks + chip - 1) / chip);
-  a.sink_parts = (int32_t)std::max<int64_t>(1, (longest + a.sink_steps - 1) / a.sink_steps);
-  const size_t bytes = (size_t)items * a.sink_parts * 2 * 32 * s.d * sizeof(float);
+  int64_t sums = 0;      // fp32 sums of a block of 32 keys
+  a.sink_parts = 1;
+  a.sink_steps = (int32_t)longest;
+  if (s.num_seqlens != 0 && longest > std::max<int64_t>(8, steps / chip / 2) && (seqs > fa::kEvenCap ? items * longest : steps) < (1 << 30)) {
+    a.sink_pieces = (int32_t)std::min(chip, (steps + 7) / 8);
+    sums = 2 * (int64_t)a.sink_pieces;
+  } else if (s.num_seqlens == 0 && longest > 8) {
+    a.sink_steps = (int32_t)std::max<int64_t>(8, (steps + chip - 1) / chip);
+    a.sink_parts = (int32_t)((longest + a.sink_steps - 1) / a.sink_steps);
+    sums = a.sink_parts > 1 ? items * a.sink_parts : 0;
+  }
+  const size_t bytes = (size_t)sums * 2 * 32 * s.d * sizeof(float);
   bool held = false;
   if (bytes > 0) {
-    void* sums = nullptr;
+    void* ws = nullptr;
     if (alloc != nullptr) {
-      sums = alloc->alloc(alloc, (uint64_t)bytes);
+      ws = alloc->alloc(alloc, (uint64_t)bytes);
     } else if (!stream_is_capturing(stream) && (int64_t)bytes <= ws_limit_bytes(device_index(dev))) {
-      held = ws_acquire(device_index(dev), bytes, stream, &sums) == hipSuccess;
-      if (!held) sums = nullptr;
+      held = ws_acquire(device_index(dev), bytes, stream, &ws) == hipSuccess;
+      if (!held) ws = nullptr;
     }
-    if (sums == nullptr) return FA_ERROR_OUT_OF_MEMORY;
-    a.sink_ws = static_cast<float*>(sums);
+    if (ws == nullptr) return FA_ERROR_OUT_OF_MEMORY;
+    a.sink_ws = static_cast<float*>(ws);
   }
   fa_lazy_tensor2* lazy = const_cast<fa_lazy_tensor2*>(&p->D);
   fa_tensor2 delta = p->D.eager;
@@ -1527,7 +1537,7 @@ int fa_attn_bwd_sinks(const fa_bwd_params* p, int32_t params_version, int32_t wi
       rc = FA_ERROR_INVALID_VALUE;
   }
   a.delta = static_cast<float*>(delta.ptr);
-  FA_LOG(4, "attn_bwd_sinks: D=%d window=%d sinks=%d nseq=%d parts=%d", s.d, a.window, a.sinks, s.num_seqlens, a.sink_parts);
+  FA_LOG(4, "attn_bwd_sinks: D=%d window=%d sinks=%d nseq=%d pieces=%d parts=%d", s.d, a.window, a.sinks, s.num_seqlens, a.sink_pieces, a.sink_parts);
   const SinkBwdRoute route = sink_bwd_route(s, (int64_t)p->Q.sizes[2], (int64_t)p->K.sizes[2], a.window, dev->num_cu);
   a.wide = route.wide_dkdv ? 1 : 0;
   a.walk_group = 2;

@@ -8,6 +8,7 @@
 namespace fa {
 
 constexpr int kNumXcd = 8;   // MI355X: 8 XCDs x 32 CUs, one L2 each
+constexpr int kEvenCap = 1023;   // sequences whose tiles a workgroup lists (EvenWalk)
 
 // The 1-D work list of a kernel over the tiles of (batch element or sequence, head) pairs: each XCD owns a
 // contiguous range of pairs and walks them `zh_group` at a time.  Launchers and fa_query_*_config form it here.
@@ -212,12 +213,12 @@ struct SinkFwdArgs : FwdArgs {
 };
 struct SinkBwdArgs : BwdArgs {
   int32_t window, sinks;
-  // dK and dV of the first keys come from fp32 sums over pieces of sink_steps steps, at most sink_parts of them per sequence and K/V head
-  // (fa_sinks.h)
-  int32_t sink_parts, sink_steps;
+  // Work on the first keys' dK and dV (fa_sinks.h): in sink_pieces equal pieces of a list of all its steps, or, where that is 0,
+  // sink_parts pieces of sink_steps steps for every block of 32 keys of a sequence.
+  int32_t sink_pieces, sink_parts, sink_steps;
   int32_t wide;          // the window's part of dK and dV is another launch's (64 keys per wave)
   int32_t head_shift;    // as in SinkFwdArgs, of the dQ kernel
-  float* sink_ws;
+  float* sink_ws;        // fp32 sums of the pieces of blocks that are several (of a list: two per piece)
 };
 
 // Query heads that share a K/V head take the waves of one workgroup, each with the same rows: as many heads as divide

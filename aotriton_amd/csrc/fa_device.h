@@ -510,7 +510,7 @@ struct LevelWalk {
 // sequences of 266-6000 tokens and 4 K/V heads, window 512: forward 329 -> 269 us, dQ 524 -> 406), and the tiles that its workers have in hand
 // are neighbours, whose windows overlap.  `table`: tiles in front of each sequence, in LDS; packed sequences beyond kEvenCap, and dense
 // batches, count num_tiles for every sequence (a tile behind a sequence's end is an empty item).
-constexpr int kEvenCap = kLevelBytes / 4 - 1;
+static_assert(kEvenCap + 1 <= kLevelBytes / 4, "the table fits");
 struct EvenWalk {
   const int* table;                // null: num_tiles per sequence
   int nseq, num_tiles, ratio, hi;

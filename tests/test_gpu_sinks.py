@@ -47,11 +47,11 @@ def _inputs(B, Hq, Hk, Sq, Sk, D, dtype, seed=0, Dv=None, scale=1.0):
             rn(B, Sq, Hq, Dv).transpose(1, 2))
 
 
-def _check(q, k, v, do, window, sinks, scale, out, lse, grads, what=''):
+def _check(q, k, v, do, window, sinks, scale, out, lse, grads, what='', device='cpu'):
     """one sequence, (heads, rows, head dim)"""
     dt = q.dtype
-    q, k, v, do = (t.detach().cpu() for t in (q, k, v, do))
-    seen = longctx.sink_mask(q.shape[1], k.shape[1], window, sinks)
+    q, k, v, do = (t.detach().to(device) for t in (q, k, v, do))
+    seen = longctx.sink_mask(q.shape[1], k.shape[1], window, sinks, device=device)
     want, want_lse, p = longctx.attention(q, k, v, seen, scale)
     size = torch.matmul(p, v.double().abs().repeat_interleave(q.shape[0] // k.shape[0], 0))
     e = score_error(q, k, scale)
@@ -281,3 +281,50 @@ def test_the_library_takes_its_workspace_without_an_allocator():
         assert lib.fa_attn_bwd_sinks(ctypes.byref(c), 6, 50, 4, stream, None, None) == 2      # no memory, nothing launched
     finally:
         lib.fa_set_bwd_workspace_limit(-1)
+
+
+@pytest.mark.parametrize('Hq,Hk,S,D,dtype', [
+    (4, 1, 417, 128, torch.bfloat16), (8, 1, 290, 64, torch.float16), (6, 2, 333, 128, torch.float16), (12, 2, 200, 64, torch.bfloat16),
+    (16, 2, 97, 128, torch.bfloat16), (7, 1, 130, 96, torch.float16), (8, 2, 33, 80, torch.bfloat16), (2, 1, 1000, 128, torch.bfloat16)])
+def test_heads_of_a_group(Hq, Hk, S, D, dtype):
+    """groups that take a workgroup's waves whole, in part, and not at all"""
+    q, k, v, do = _inputs(2, Hq, Hk, S, S + 40, D, dtype, seed=S)
+    out, grads = _step(q, k, v, do, 90, 5)
+    _, lse = _raw(q, k, v, 90, 5, 1 / math.sqrt(D))
+    for b in range(2):
+        _check(q[b], k[b], v[b], do[b], 90, 5, 1 / math.sqrt(D), out[b], lse.view(2, Hq, S)[b], [g[b] for g in grads], f'sequence {b} ')
+
+
+@pytest.mark.parametrize('Hq,Hk,S,window,D,dtype', [
+    (32, 8, 4099, 1100, 128, torch.bfloat16), (32, 8, 4099, 1100, 96, torch.float16), (32, 8, 4099, 1100, 104, torch.bfloat16),
+    (16, 16, 4100, 1030, 128, torch.float16), (32, 8, 4099, 1100, 64, torch.bfloat16)])
+def test_long_sequences(Hq, Hk, S, window, D, dtype):
+    """the kernels of long sequences (64 rows per wave above 64 columns); the oracle takes the first and the last group"""
+    q, k, v, do = _inputs(1, Hq, Hk, S, S, D, dtype, seed=D)
+    out, grads = _step(q, k, v, do, window, 40)
+    _, lse = _raw(q, k, v, window, 40, 1 / math.sqrt(D))
+    g = Hq // Hk
+    for hk in (0, Hk - 1):
+        hq, kv = slice(hk * g, hk * g + g), slice(hk, hk + 1)
+        _check(q[0, hq], k[0, kv], v[0, kv], do[0, hq], window, 40, 1 / math.sqrt(D), out[0, hq], lse.view(Hq, S)[hq],
+               [grads[0][0, hq], grads[1][0, kv], grads[2][0, kv]], f'group {hk} ', device=DEV)
+
+
+@pytest.mark.parametrize('lens,Hq,Hk,D,sinks', [
+    ([3, 1, 1000, 2] * 7 + [2900] + [1] * 60, 4, 1, 128, 70),          # one long one among many, three blocks of sinks
+    ([1 + i * i % 37 for i in range(1100)] + [700], 2, 1, 64, 3),      # more sequences than a table holds
+    ([5 + i % 11 for i in range(1100)], 2, 2, 128, 4),
+    ([2500, 0, 0, 0, 1, 0], 8, 2, 128, 33)])
+def test_sequences_of_very_different_lengths(lens, Hq, Hk, D, sinks):
+    window, n = 50, sum(lens)
+    q, k, v, do = _inputs(1, Hq, Hk, n, n, D, torch.bfloat16, seed=len(lens))
+    offs = [0]
+    for x in lens:
+        offs.append(offs[-1] + x)
+    cu = torch.tensor(offs, dtype=torch.int32, device=DEV)
+    out, grads = _step(q, k, v, do, window, sinks, cu_seqlens_q=cu, cu_seqlens_k=cu, max_seqlen_q=max(lens), max_seqlen_k=max(lens))
+    assert all(torch.isfinite(t).all() for t in (out, *grads))
+    for i in sorted({*range(0, len(lens), max(1, len(lens) // 24)), lens.index(max(lens)), len(lens) - 1}):
+        at = slice(offs[i], offs[i + 1])
+        _check(q[0][:, at], k[0][:, at], v[0][:, at], do[0][:, at], window, sinks, 1 / math.sqrt(D), out[0][:, at], None,
+               [t[0][:, at] for t in grads], f'sequence {i} ', device=DEV)
