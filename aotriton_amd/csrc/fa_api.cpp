@@ -1378,10 +1378,12 @@ int64_t sink_tiles(const Shape& s, int heads, bool keys, int64_t tokens, int row
   return heads * (s.num_seqlens > 0 ? tokens / rows + seqs / 2 + 1 : seqs * (((keys ? s.max_sk : s.max_sq) + rows - 1) / rows));
 }
 
-// Forward: tiles of 256 rows or of 128, two workgroups per CU, and the parts that a tile's keys are split into where the tiles do not fill
-// the chip.  The costs are about those of fwd_small_tiles and fwd_plan (an item, 64 keys of it; a second launch and the parts' sums at 4 TB/s).
-// (us, 256 rows / 128 rows / split in two / in four: B1 Hq 32 Hk 8 D128 S32768 window 4096 2023 / 2249, S8192 1024 197 / 194, 256 100 / 83; 256 queries
-// of 4096 keys window 1024 43 / 38 / 32 / 31, 64 of 8192 window 4096 108 / 110 / 65 / 40; B4 H16 D64 512 of 4601 window 2048 58 / 46 / 43 / 51.)
+// Forward: tiles of 256 rows (of one head or of several, sink_head_shift) or of 128, two workgroups per CU, and the parts that a tile's
+// keys are split into where the tiles do not fill the chip.  Costs: an item, 64 keys of it (`alone` on a CU, or two there); a second
+// launch and the parts' sums.  (us, 256 rows / 128 / 256 split in two / 128 split in two: B1 Hq 32 Hk 8 D128 S32768 window 4096 1897 / 2149,
+// S8192 1024 161 / 168, 256 76 / 69; 256 queries of 4096 keys window 1024 36 / 34 / 34 / 30 (in four 34 / 30), 64 of 8192 window 4096
+// 109 / 107 / 66 / 64 (in four 43 / 40, in eight 34); D64 B4 H16 512 of 4601 window 2048 57 / 46 / 45 / 43, S8192 1024 70 / 64,
+// B2 Hq 16 Hk 4 S1000 window 300 23 / 16.)
 struct SinkFwdPlan { int half_tiles, splits; int64_t o_bytes, bytes; };
 SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, int32_t window, int32_t sinks, int num_cu) {
   SinkFwdPlan best{0, 1, 0, 0};
@@ -1389,14 +1391,17 @@ SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, int32_t window, int32_
   const int64_t seqs = s.num_seqlens != 0 ? std::abs(s.num_seqlens) : s.batch;
   for (int half = 0; half < 2; ++half) {
     const int shift = fa::sink_head_shift(s.hq, s.hk, half ? 4 : 8), bm = (half ? 128 : 256) >> shift, per_cu = half ? 2 : 1;
-    const double item = s.d > 64 ? (half ? 6.5 : 6.3) : (half ? 4.5 : 4.35), step = s.d > 64 ? (half ? 1.8 : 1.74) : (half ? 1.2 : 1.12);
-    const int64_t keys = std::min<int64_t>(s.max_sk, (int64_t)window + bm) + std::min<int64_t>(sinks, 64), tiles = (keys + 63) / 64;
+    const int tile = s.d == 64 && !half ? 128 : 64;
+    const int64_t keys = std::min<int64_t>(s.max_sk, (int64_t)window + bm) + std::min<int64_t>(sinks, 64), tiles = (keys + tile - 1) / tile;
     const int64_t items = sink_tiles(s, s.hq >> shift, false, tokens, bm), stored = seqs * s.hq * ((s.max_sq + bm - 1) / bm) * bm;
     for (int splits = 1; splits <= 8 && (splits == 1 || (s.num_seqlens == 0 && splits * 2 <= tiles)); ++splits) {
       const int64_t o_bytes = splits > 1 ? stored * splits * s.d * 4 : 0, bytes = splits > 1 ? o_bytes + stored * splits * 8 : 0;
-      const double t = rounds_time(items * splits, (int64_t)per_cu * num_cu, item + step * ((tiles + splits - 1) / splits)) +
-                       (splits > 1 ? 5 + 2.0 * bytes / 4e6 : 0.0);
-      if ((half == 0 && splits == 1) || t < 0.97 * least) {
+      const bool alone = items * splits <= num_cu;
+      const double item = s.d > 64 ? (half ? 6.5 : 6.3) : (half ? 5.0 : 7.0);
+      const double step = s.d > 64 ? (half ? (alone ? 1.55 : 1.85) : 1.74) : (half ? (alone ? 1.15 : 1.5) : 1.3);
+      const double t = rounds_time(items * splits, (int64_t)per_cu * num_cu, item + step * (tile / 64) * ((tiles + splits - 1) / splits)) +
+                       (splits > 1 ? 5 + 1.6 * bytes / 4e6 : 0.0);
+      if ((half == 0 && splits == 1) || t < 0.99 * least) {
         least = t;
         best = SinkFwdPlan{half ? 2 : 0, splits, o_bytes, bytes};
       }
@@ -1405,21 +1410,46 @@ SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, int32_t window, int32_
   return best;
 }
 
-// Backward: the kernels with 64 rows per wave (head dims above 64)?  Costs as in bwd_route.  (us of the whole backward, 128 rows / 256: bf16
-// Hq 32 Hk 8 S8192 D128 window 256 297 / 299, 512 389 / 372, 1024 613 / 541, 2048 928 / 845; B4 Hq 16 Hk 4 S1024 window 256 112 / 156,
-// only dQ wide 109; B1 Hq 8 Hk 2 S4096 window 512 122 / 199.)
+// Time of the tiles of a backward kernel: `rows` rows, of `heads` heads, `group` of them a position of the walk apart in each K/V head
+// (dQ), or keys whose queries in `group` heads are visited (dK/dV).  Dense: what the busiest workgroup of an XCD has (EvenWalk; tiles at the
+// start, or of keys at the end, of a sequence are shorter); packed: an average, and half an item for its end.
+double sink_bwd_time(const Shape& s, bool keys, int64_t tokens, int heads, int group, int rows, int step, int32_t window, int num_cu, double item,
+                     double cost) {
+  const int64_t span = (int64_t)window - 1 + rows, shift = (int64_t)s.max_sk - s.max_sq;
+  const int steps_of = keys ? group : 1, extra = keys ? 0 : 1;
+  auto of_tile = [&](int64_t t) {
+    const int64_t seen = keys ? s.max_sk - t * rows : (t + 1) * rows + shift;
+    const int64_t n = std::max<int64_t>(0, std::min({span, seen, (int64_t)(keys ? s.max_sq : s.max_sk)}));
+    return item + cost * (steps_of * (double)(n / step + 1) + extra);
+  };
+  if (s.num_seqlens == 0) {
+    const int64_t tiles = ((keys ? s.max_sk : s.max_sq) + rows - 1) / rows, share = (s.batch * heads * tiles + 7) / 8;
+    const int workers = std::max(1, std::min(num_cu / 8, 64)), in_a_row = keys ? 1 : group;
+    if (share <= 8 * workers && tiles > 0) {
+      double load[64] = {}, most = 0;
+      for (int64_t i = 0; i < share; ++i) most = std::max(most, load[i % workers] += of_tile(i / in_a_row % tiles));
+      return most;
+    }
+  }
+  const double rounds = (double)sink_tiles(s, heads, keys, tokens, rows) / num_cu;
+  return std::max(1.0, rounds + 0.5) * (item + cost * (steps_of * (double)(std::min<int64_t>(keys ? s.max_sq : s.max_sk, span) / step + 1) + extra));
+}
+
+// Backward: the kernels with 64 rows per wave (head dims above 64)?  (us of the whole backward, neither / dQ / dK and dV / both: bf16 D128
+// Hq 32 Hk 8 S8192 window 256 325 / 277 / 312 / 267, 1024 589 / 521 / 573 / 505, 2048 932 / 847 / 885 / 797; S4099 window 1100 340 / 295 / 414 / 374;
+// B4 Hq 16 Hk 4 S1024 window 256 110 / 99 / 157 / 146; B1 Hq 8 Hk 2 S4096 window 512 121 / 124 / 184 / 189; packed, 4 of up to 8000 tokens, H8,
+// window 1024 359 / 327 / 342 / 310, 16 of up to 6000, Hq 16 Hk 4, 512 874 / 757 / 929 / 804.)
 struct SinkBwdRoute { bool wide_dq, wide_dkdv; };
 SinkBwdRoute sink_bwd_route(const Shape& s, int64_t tokens_q, int64_t tokens_k, int32_t window, int num_cu) {
   if (s.d != 128) return SinkBwdRoute{false, false};
-  const int shift = fa::sink_head_shift(s.hq, s.hk, 4);
-  auto time = [&](bool keys, int rows, int step, double item, double cost) {
-    const int tile = keys ? rows : rows >> shift;
-    const int64_t span = std::min<int64_t>(keys ? s.max_sq : s.max_sk, (int64_t)window - 1 + tile);
-    const double steps = (keys ? s.hq / s.hk : 1) * (double)(span / step + 1) + (keys ? 0 : 1);
-    return rounds_time(sink_tiles(s, keys ? s.hk : s.hq >> shift, keys, keys ? tokens_k : tokens_q, tile), num_cu, item + cost * steps);
+  const int shift = fa::sink_head_shift(s.hq, s.hk, 4), group = s.hq / s.hk;
+  auto dq = [&](int rows, int step, double item, double cost) {
+    return sink_bwd_time(s, false, tokens_q, s.hq >> shift, group >> shift, rows >> shift, step, window, num_cu, item, cost);
   };
-  return SinkBwdRoute{time(false, 256, 32, 5, 1.42) < 0.95 * time(false, 128, 64, 5, 1.7),
-                      time(true, 256, 32, 7, 1.8) < time(true, 128, 64, 9, 1.95)};
+  auto dkdv = [&](int rows, int step, double item, double cost) {
+    return sink_bwd_time(s, true, tokens_k, s.hk, group, rows, step, window, num_cu, item, cost);
+  };
+  return SinkBwdRoute{dq(256, 32, 5, 1.42) < 0.97 * dq(128, 64, 5, 1.7), dkdv(256, 32, 7, 1.8) < dkdv(128, 64, 9, 1.95)};
 }
 
 }  // namespace
