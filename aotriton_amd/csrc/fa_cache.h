@@ -454,10 +454,10 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
     } else {
       const int pq = (r0 + r) / group, ph = hk * group + (r0 + r) % group;
       if (at < d_v) {
-        const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+        const float inv = 1.0f / lsum;
         q4_t t4;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) t4[x] = Tr::cvt(lsum > 0.f ? acc[x] * inv : 0.f);
+        for (int x = 0; x < 4; ++x) t4[x] = Tr::cvt(lsum == 0.f ? 0.f : acc[x] * inv);      // (a NaN stays one)
         *reinterpret_cast<q4_t*>(reinterpret_cast<T*>(a.out) + (int64_t)z * a.so.z + (int64_t)ph * a.so.h + (int64_t)pq * a.so.s + at) = t4;
       }
       if (a.lse && at == 0) a.lse[((int64_t)z * a.hq + ph) * a.tokens + pq] = lse_of(m, sc, lsum);
@@ -756,7 +756,7 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
     }
     return;
   }
-  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  const float inv = 1.0f / l;
   T* op = reinterpret_cast<T*>(a.out) + (int64_t)z * a.so.z + (int64_t)h * a.so.h + (int64_t)token * a.so.s;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -764,7 +764,7 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
     for (int g = 0; g < 4; ++g) {
       q4_t t4;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) t4[x] = Tr::cvt(l > 0.f ? o[db][4 * g + x] * inv : 0.f);
+      for (int x = 0; x < 4; ++x) t4[x] = Tr::cvt(l == 0.f ? 0.f : o[db][4 * g + x] * inv);
       const int at = 32 * db + 8 * g + 4 * hi;
       if (!kPad || at < d_v) *reinterpret_cast<q4_t*>(op + at) = t4;
     }
@@ -861,7 +861,7 @@ static __global__ __launch_bounds__(256) void tree_sum_kernel(const TreeArgs a) 
   if (!ok) return;
   const int token = pr / group, h = hk * group + pr % group;
   if (col < c.head_dim_v) {
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
     vec<T, 4> t;
 #pragma unroll
     for (int j = 0; j < 4; ++j) t[j] = Traits<T>::cvt(acc[j] * inv);

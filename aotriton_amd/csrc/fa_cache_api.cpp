@@ -70,6 +70,13 @@ int check_int_rows(const fa_tensor2& t, uint64_t rows) {
 
 // Rows of a tensor that is written have to lie apart.
 bool rows_apart(const fa_tensor2& t) { return t.sizes[0] <= 1 || t.strides[0] >= t.sizes[1]; }
+// (an expanded cache has one row for many)
+bool written_apart(const fa_tensor4& t) {
+  for (int i = 0; i < 3; ++i)
+    if (t.sizes[i] > 1 && t.strides[i] < t.sizes[3]) return false;
+  return true;
+}
+bool written_apart(const fa_cache& c) { return written_apart(c.K) && written_apart(c.V); }
 
 fa::Strides3 strides3(const fa_tensor4& t) {
   return fa::Strides3{(int64_t)t.strides[0], (int64_t)t.strides[1], (int64_t)t.strides[2]};
@@ -222,6 +229,7 @@ int fa_cache_append(const fa_tensor4* k, const fa_tensor4* v, const fa_cache* ca
   fa::AppendArgs a{};
   int e = check_cache(cache, &a.cache);
   if (e != FA_SUCCESS) return e;
+  if (!written_apart(*cache)) return FA_ERROR_NOT_SUPPORTED;
   const fa::CacheArgs& c = a.cache;
   if ((e = check_rows(*k, cache->K.dtype)) != FA_SUCCESS || (e = check_rows(*v, cache->K.dtype)) != FA_SUCCESS) return e;
   for (const fa_tensor4* t : {k, v})
@@ -244,6 +252,7 @@ int fa_cache_copy_pages(const fa_tensor4* k_cache, const fa_tensor4* v_cache, co
   fa::CopyArgs a{};
   int e = check_pages(*k_cache, *v_cache, &a.cache);
   if (e != FA_SUCCESS) return e;
+  if (!written_apart(*k_cache) || !written_apart(*v_cache)) return FA_ERROR_NOT_SUPPORTED;
   const uint64_t n = source->sizes[0];
   if (n > kMaxCount) return FA_ERROR_INVALID_VALUE;
   if ((e = check_ints(*source, n)) != FA_SUCCESS || (e = check_ints(*target, n)) != FA_SUCCESS) return e;
@@ -274,7 +283,7 @@ int fa_cache_fork(const fa_cache* cache, const fa_tensor1* uses, const fa_tensor
   if ((e = check_ints(*uses, (uint64_t)c.pages)) != FA_SUCCESS) return e;
   for (const fa_tensor1* t : {source, target, spare})
     if ((e = check_ints(*t, n)) != FA_SUCCESS) return e;
-  if (!rows_apart(cache->table)) return FA_ERROR_NOT_SUPPORTED;
+  if (!rows_apart(cache->table) || !written_apart(*cache)) return FA_ERROR_NOT_SUPPORTED;
   a.table_out = static_cast<int32_t*>(cache->table.ptr);
   a.lengths_out = static_cast<int32_t*>(cache->lengths.ptr);
   a.uses = static_cast<int32_t*>(uses->ptr);
@@ -293,6 +302,7 @@ int fa_cache_keep_path(const fa_cache* cache, const fa_tensor2* path, const fa_t
   int e = check_cache(cache, &a.cache);
   if (e != FA_SUCCESS) return e;
   const fa::CacheArgs& c = a.cache;
+  if (!written_apart(*cache)) return FA_ERROR_NOT_SUPPORTED;
   if ((e = check_int_rows(*path, (uint64_t)c.sequences)) != FA_SUCCESS) return e;
   if ((e = check_ints(*counts, (uint64_t)c.sequences)) != FA_SUCCESS || (e = check_ints(*new_lengths, (uint64_t)c.sequences)) != FA_SUCCESS) return e;
   // (workgroups of one sequence read its length while another one writes the new one)

@@ -103,6 +103,37 @@ def test_many_parts_of_a_long_cache():
     _check(q, k, v, table, n, None, 0, 0, 0.125, out, lse)
 
 
+@pytest.mark.parametrize('tokens,Hq,D,window', [(1, 8, 64, 0), (5, 16, 128, 0), (24, 32, 64, 0), (40, 64, 64, 0), (24, 32, 128, 1500)])
+def test_equal_pieces_of_many_sequences(tokens, Hq, D, window):
+    """more than 64 sequences, of very different lengths, cut into equal pieces: few rows, tiles of 128 and of 256"""
+    rng = random.Random(tokens)
+    lens = [rng.choice([0, 3, 60, 500, 1100, 1300]) for _ in range(69)] + [2900, 1, 1299]
+    k, v, table, n = _pool(lens, tokens, 8, D, 64, torch.bfloat16, seed=30)
+    q = torch.randn(len(lens), tokens, Hq, D, generator=torch.Generator().manual_seed(31)).bfloat16().transpose(1, 2)
+    parents = torch.tensor([_tree(rng, tokens) for _ in lens], dtype=torch.int32)
+    scale = 1 / math.sqrt(D)
+    out, lse = _run(q, k, v, table, n, parents, window, 3 if window else 0, scale, 2900)
+    pick = [0, 1, 2, 30, 62, 63, 64, 65, 69, 70, 71]
+    _check(q[pick], k, v, table[pick], n[pick], parents[pick], window, 3 if window else 0, scale, out[pick], lse[pick])
+    alone, alone_lse = _run(q, k, v, table, n, parents, window, 3 if window else 0, scale, 0)      # hardly split
+    far = (alone.float() - out.float()).abs().amax((1, 2, 3))
+    most = torch.where(torch.isfinite(v), v, 0.0).abs().max().item()
+    assert (far <= 2 * 2.1 * 2.0 ** -8 * most).all()      # (two of out_bound's: 2.01 half steps of |V|, and what the scores are off by)
+
+
+@pytest.mark.parametrize('tokens,Hq', [(1, 2), (20, 8)])
+def test_a_visible_nan_stays(tokens, Hq):
+    k, v, table, n = _pool([300, 40], tokens, 2, 64, 16, torch.float16, seed=32)
+    k[table[0, 3], 0, 5] = float('nan')
+    v[table[1, 1], 1, 2] = float('nan')
+    q = torch.randn(2, Hq, tokens, 64, generator=torch.Generator().manual_seed(33)).half()
+    for top in (None, 0):
+        out, _ = _run(q, k, v, table, n, None, 0, 0, 0.125, top)
+        half = Hq // 2
+        assert out[0, :half].isnan().all() and out[1, half:].isnan().all()
+        assert torch.isfinite(out[0, half:]).all() and torch.isfinite(out[1, :half]).all()
+
+
 @pytest.mark.parametrize('window', [0, 20])
 def test_tokens_that_are_not_there(window):
     lens, tokens = [70, 33, 0], 21

@@ -221,6 +221,16 @@ def test_page_refusals():
     assert lib.fa_cache_keep_path(ref(c), ref(path), ref(t1(3)), ref(t1(3)), None) == INVALID      # onto the lengths themselves
     assert lib.fa_cache_keep_path(ref(c), ref(path), ref(t1(4)), ref(new), None) == INVALID
     assert lib.fa_cache_keep_path(ref(c), ref(_fill(L.fa_tensor2(), (2, 4), torch.int32)), ref(t1(3)), ref(new), None) == INVALID
+    for which, dim in (('K', 0), ('V', 1), ('K', 2)):      # a cache that is expanded is read, not written
+        wide = _cache()
+        getattr(wide, which).strides[dim] = 0
+        assert lib.fa_cache_append(ref(k), ref(v), ref(wide), None, None) == NOT_SUPPORTED
+        assert lib.fa_cache_copy_pages(ref(wide.K), ref(wide.V), ref(t1(4)), ref(t1(4)), None) == NOT_SUPPORTED
+        assert lib.fa_cache_keep_path(ref(wide), ref(path), ref(t1(3)), ref(new), None) == NOT_SUPPORTED
+        assert fork(cache=wide) == NOT_SUPPORTED
+        tree = _tree()
+        tree.cache = wide
+        assert lib.fa_tree_attn(ref(tree), None, None) in ACCEPTED
     table = _fill(L.fa_tensor2(), (3, 5), torch.int32)
     assert lib.fa_cache_free(ref(table), ref(t1(9)), ref(t1(2)), ref(t1(2)), ref(t1(2)), None) in ACCEPTED
     assert lib.fa_cache_free(ref(table), ref(t1(9)), ref(t1(2)), ref(t1(1)), ref(t1(2)), None) == INVALID
