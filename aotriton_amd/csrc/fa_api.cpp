@@ -1384,9 +1384,9 @@ int64_t sink_tiles(const Shape& s, int heads, bool keys, int64_t tokens, int row
 // S8192 1024 161 / 168, 256 76 / 69; 256 queries of 4096 keys window 1024 36 / 34 / 34 / 30 (in four 34 / 30), 64 of 8192 window 4096
 // 109 / 107 / 66 / 64 (in four 43 / 40, in eight 34); D64 B4 H16 512 of 4601 window 2048 57 / 46 / 45 / 43, S8192 1024 70 / 64,
 // B2 Hq 16 Hk 4 S1000 window 300 23 / 16.)
-struct SinkFwdPlan { int half_tiles, splits; int64_t o_bytes, bytes; };
-SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, int32_t window, int32_t sinks, int num_cu) {
-  SinkFwdPlan best{0, 1, 0, 0};
+struct SinkFwdPlan { int half_tiles, splits; int64_t o_bytes, bytes; bool wide; };
+SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, float scale, int32_t window, int32_t sinks, int num_cu) {
+  SinkFwdPlan best{0, 1, 0, 0, false};
   double least = 0;
   const int64_t seqs = s.num_seqlens != 0 ? std::abs(s.num_seqlens) : s.batch;
   for (int half = 0; half < 2; ++half) {
@@ -1403,9 +1403,16 @@ SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, int32_t window, int32_
                        (splits > 1 ? 5 + 1.6 * bytes / 4e6 : 0.0);
       if ((half == 0 && splits == 1) || t < 0.99 * least) {
         least = t;
-        best = SinkFwdPlan{half ? 2 : 0, splits, o_bytes, bytes};
+        best = SinkFwdPlan{half ? 2 : 0, splits, o_bytes, bytes, false};
       }
     }
+  }
+  // 64 rows per wave: more at an item's ends and for masked tiles, less for the others.  (us, 256 rows of 32 per wave -> 64, Hq 32 Hk 8 D128:
+  // S8192 window 512 102 -> 114, 1024 156 -> 162, 2048 271 -> 263, S32768 window 4096 2010 -> 1930; H32 S6000 window 3000 258 -> 260.)
+  if (s.d == 128 && scale > 0.f) {
+    const int shift = fa::sink_head_shift(s.hq, s.hk, 4), bm = 256 >> shift;
+    const int64_t keys = std::min<int64_t>(s.max_sk, (int64_t)window + bm) + std::min<int64_t>(sinks, 64), tiles = (keys + 63) / 64;
+    if (rounds_time(sink_tiles(s, s.hq >> shift, false, tokens, bm), num_cu, 9.5 + 1.62 * tiles) < 0.99 * least) best = SinkFwdPlan{0, 1, 0, 0, true};
   }
   return best;
 }
@@ -1475,11 +1482,12 @@ int fa_attn_fwd_sinks(const fa_fwd_params* p, int32_t params_version, int32_t wi
   a.num_cu = dev->num_cu;
   a.window = window_of(window);
   a.sinks = sinks;
-  bool held = false;
+  bool held = false, wide = false;
   a.splits = 1;
   if (s.max_sq > 0 && s.max_sk > 0 && s.batch > 0) {
-    const SinkFwdPlan plan = sink_fwd_plan(s, (int64_t)p->Q.sizes[2], a.window, sinks, dev->num_cu);
+    const SinkFwdPlan plan = sink_fwd_plan(s, (int64_t)p->Q.sizes[2], a.sm_scale, a.window, sinks, dev->num_cu);
     a.half_tiles = plan.half_tiles;
+    wide = plan.wide;
     if (plan.splits > 1) {
       void* scratch = nullptr;
       if (alloc != nullptr) {
@@ -1495,8 +1503,8 @@ int fa_attn_fwd_sinks(const fa_fwd_params* p, int32_t params_version, int32_t wi
       }
     }
   }
-  FA_LOG(4, "attn_fwd_sinks: D=%d window=%d sinks=%d nseq=%d half_tiles=%d splits=%d", s.d, a.window, sinks, s.num_seqlens, a.half_tiles, a.splits);
-  const hipError_t err = fa::run_sinks_fwd(p->Q.dtype, s.d, a, stream);
+  FA_LOG(4, "attn_fwd_sinks: D=%d window=%d sinks=%d nseq=%d half_tiles=%d splits=%d wide=%d", s.d, a.window, sinks, s.num_seqlens, a.half_tiles, a.splits, (int)wide);
+  const hipError_t err = wide ? fa::run_sinks_fwd_wide(p->Q.dtype, a, stream) : fa::run_sinks_fwd(p->Q.dtype, s.d, a, stream);
   if (held) ws_release(device_index(dev), stream);
   return (int)err;
 }

@@ -34,9 +34,9 @@ struct WideFwdSmem {
 
 // Tile mt (256 rows of head h of sequence z) against all its visible key tiles, with kSplit against part `split` of them: the
 // fp32 sums and the row statistics of the part then go to scratch memory, where combine_rows_kernel picks them up.
-template <typename T, bool kWindowed, int kPad, bool kSplit>
-__device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, const int h, const int mt, const int split, char* smem_raw) {
-  constexpr int D = 128, BM = 256, BN = 64, QB = 2;
+template <typename T, bool kWindowed, int kPad, bool kSplit, bool kSinks = false>
+__device__ __forceinline__ void fwd_wide_item(const FwdArgsOf<kSinks>& a, const int z, const int h0, const int mt, const int split, char* smem_raw) {
+  constexpr int D = 128, BN = 64, QB = 2;
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
   using q4_t = typename Tr::q4_t;
@@ -52,11 +52,18 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
   const int d_qk = kPad ? a.head_dim : D, d_v = kPad ? a.head_dim_v : D;
 
   const SeqInfo si = uniform(get_seq(a.seq, z));
+  // kSinks, as in fwd_item: BM rows of a head
+  static_assert(!kSinks || (kWindowed && !kSplit), "a window with sinks, whole");
+  int shift = 0;
+  if constexpr (kSinks) shift = a.head_shift;
+  const int BM = 256 >> shift;
+  const int h = kSinks ? h0 + (wave & ((1 << shift) - 1)) : h0;
   const int q0 = mt * BM;
   if (q0 >= si.seqlen_q) return;
 
   Window w{0, 0};
-  if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right, si.seqlen_q, si.seqlen_k);
+  if constexpr (kSinks) w = aligned_window(a.window, si.seqlen_q, si.seqlen_k);
+  else if (kWindowed) w = parse_window(a.mask.causal_type, a.mask.window_left, a.mask.window_right, si.seqlen_q, si.seqlen_k);
   w.left = w.left > (1 << 30) ? (1 << 30) : (w.left < -(1 << 30) ? -(1 << 30) : w.left);
   w.right = w.right > (1 << 30) ? (1 << 30) : (w.right < -(1 << 30) ? -(1 << 30) : w.right);
   BlockRanges br = block_ranges(kWindowed, w.left, w.right, q0, si.seqlen_q, si.seqlen_k, BM, BN);
@@ -65,8 +72,14 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
     br.lo += split * per;
     if (br.lo + per - 1 < br.hi) br.hi = br.lo + per - 1;
   }
-  const int qw = q0 + 64 * wave;
+  const int qw = q0 + 64 * (wave >> shift);
   const BlockRanges wr = block_ranges(kWindowed, w.left, w.right, qw, si.seqlen_q, si.seqlen_k, 64, BN);
+
+  // and tiles before the window's first, in which only sinks are visible
+  int sinks = 0;
+  if constexpr (kSinks) sinks = a.sinks;
+  const int front = kSinks ? (sinks < br.lo * BN ? (sinks + BN - 1) / BN : br.lo) : 0;
+  const int fetch_lo = front > 0 ? 0 : br.lo;
 
   const int hk = h / (a.hq / a.hk);
   const int row0 = qw + c;                       // this lane's queries: row0 and row0 + 32
@@ -112,9 +125,10 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
   const int k_voff = gch * 8 < d_qk ? r0 * (int)a.sk.s * 2 + gch * 16 : kVoffOutOfRange;
   const int v_voff = gch * 8 < d_v ? r0 * (int)a.sv.s * 2 + gch * 16 : kVoffOutOfRange;
   const int k_row = (int)a.sk.s * 2, v_row = (int)a.sv.s * 2;
-  const T* kb = reinterpret_cast<const T*>(a.k) + (int64_t)si.batch_index * a.sk.z + (int64_t)hk * a.sk.h + ((int64_t)si.k_start + (int64_t)br.lo * BN) * a.sk.s;
-  const T* vb = reinterpret_cast<const T*>(a.v) + (int64_t)si.batch_index * a.sv.z + (int64_t)hk * a.sv.h + ((int64_t)si.k_start + (int64_t)br.lo * BN) * a.sv.s;
-  int f_tiles = br.hi - br.lo + 1, f_rows = si.seqlen_k - br.lo * BN;
+  const T* kb = reinterpret_cast<const T*>(a.k) + (int64_t)si.batch_index * a.sk.z + (int64_t)hk * a.sk.h + ((int64_t)si.k_start + (int64_t)fetch_lo * BN) * a.sk.s;
+  const T* vb = reinterpret_cast<const T*>(a.v) + (int64_t)si.batch_index * a.sv.z + (int64_t)hk * a.sv.h + ((int64_t)si.k_start + (int64_t)fetch_lo * BN) * a.sv.s;
+  int f_tiles = br.hi - br.lo + 1 + front, f_rows = si.seqlen_k - fetch_lo * BN;
+  int front_left = front;
   u32x4_t k_rs, v_rs;
   auto fetch_begin = [&]() __attribute__((always_inline)) {
     const int rows = f_tiles > 0 ? min(f_rows, BN) : 0;
@@ -122,6 +136,11 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
     v_rs = wave_rsrc_words(vb, rows_extent(rows, v_row, d_v * 2));
     kb += (int64_t)BN * a.sk.s; vb += (int64_t)BN * a.sv.s;
     f_rows -= BN; --f_tiles;
+    if constexpr (kSinks)
+      if (--front_left == 0) {
+        kb += (int64_t)(br.lo - front) * BN * a.sk.s; vb += (int64_t)(br.lo - front) * BN * a.sv.s;
+        f_rows -= (br.lo - front) * BN;
+      }
   };
   auto fetch_piece = [&](int stage, int i) __attribute__((always_inline)) {
     const int half = i & 1, lds = smem0 + stage + i / 2 * SM::TILE_BYTES + wave * 4 * ROWB + half * 32 * ROWB;
@@ -169,6 +188,7 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
   int m_lo[QB];
   unsigned m_rng[QB];
   bool m_none[QB];
+  int m_sink[QB];
 #pragma unroll
   for (int b = 0; b < QB; ++b) {
     const int row = row0 + 32 * b;
@@ -180,6 +200,7 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
     m_none[b] = hi_ < lo;
     m_rng[b] = m_none[b] ? 0u : (unsigned)(hi_ - lo);
     m_lo[b] = lo;
+    m_sink[b] = sinks < hi_ + 1 ? sinks : hi_ + 1;
   }
 
   float m_i[QB] = {kNegBig, kNegBig}, l_i[QB] = {0.f, 0.f}, l_even[QB] = {0.f, 0.f}, msc[QB] = {0.f, 0.f};      // reference maximum (raw scores), partial row sum, maximum * sc
@@ -235,7 +256,8 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
         const unsigned d = mask_at(b, n0 + 32 * (u - U0));
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const bool vis = d + (unsigned)(8 * (i / 4) + i % 4) <= m_rng[b];
+          bool vis = d + (unsigned)(8 * (i / 4) + i % 4) <= m_rng[b];
+          if constexpr (kSinks) vis = vis || n0 + 32 * (u - U0) + 4 * hi + 8 * (i / 4) + i % 4 < m_sink[b];
           s[u][b][i] = vis ? s[u][b][i] : -__builtin_inff();
           mx = fmaxf(mx, s[u][b][i]);
         }
@@ -331,7 +353,8 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
       const int b = E / 16, i = E % 16;
       float x = __builtin_fmaf(s[U][b][i], sc, -msc[b]);
       if (masked) {
-        const bool vis = d[b] + (unsigned)(8 * (i / 4) + i % 4) <= m_rng[b];
+        bool vis = d[b] + (unsigned)(8 * (i / 4) + i % 4) <= m_rng[b];
+        if constexpr (kSinks) vis = vis || n0 + 4 * hi + 8 * (i / 4) + i % 4 < m_sink[b];
         x = vis ? x : -__builtin_inff();
       }
       s[U][b][i] = x;
@@ -415,20 +438,23 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
   // masked, skipped; all waves take every barrier
   const int lo = max(wr.lo, br.lo), hi_t = min(wr.hi, br.hi);
   const bool none = wr.lo > wr.hi || lo > hi_t;
-  const int j_lo = none ? br.hi + 1 : lo, j_end = none ? br.hi + 1 : hi_t + 1;
+  // (kSinks: tile j < br.lo is the one of `front` that stands there; a wave whose rows see a sink starts with it and computes what it would skip)
+  auto at = [&](int j) __attribute__((always_inline)) { return kSinks && j < br.lo ? j + front - br.lo : j; };
+  const int first = kSinks ? br.lo - front : br.lo;
+  const int j_lo = none ? br.hi + 1 : kSinks && at(first) * BN < sinks ? first : lo, j_end = none ? br.hi + 1 : hi_t + 1;
   const bool full = wr.fb_lo <= wr.fb_hi;
   const int f_lo = full ? min(max(wr.fb_lo, j_lo), j_end) : j_end, f_end = full ? min(max(wr.fb_hi + 1, f_lo), j_end) : j_end;
   auto skip = [&]() __attribute__((always_inline)) {
     meet();
     fetch_all(st_nxt);
   };
-  int j = br.lo;
+  int j = first;
   for (; j < j_lo; ++j) skip();
   if (j < j_end) {
     const int cur = st_cur;
     plain_s(even{}, cur);
     plain_s(odd{}, cur);
-    full_step(even{}, two{}, j * BN);
+    full_step(even{}, two{}, at(j) * BN);
     v_to(cur);
     meet();
     fetch_all(st_nxt);
@@ -436,7 +462,7 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
     second_unit();
     ++j;
     // (left of a window rows see their first keys here: full steps, so that each settles its reference on all of them)
-    for (; j < f_lo; ++j) { have_ref = have_ref && !full; tile(std::true_type{}, j); }
+    for (; j < f_lo; ++j) { have_ref = have_ref && !full; tile(std::true_type{}, at(j)); }
     for (; j < f_end; ++j) tile(std::false_type{}, j);
     for (; j < j_end; ++j) tile(std::true_type{}, j);
     asm volatile("s_nop 1");
@@ -490,11 +516,21 @@ __device__ __forceinline__ void fwd_wide_item(const FwdArgs& a, const int z, con
   }
 }
 
-template <typename T, bool kWindowed, int kPad, bool kSplit>
+template <typename T, bool kWindowed, int kPad, bool kSplit, bool kSinks = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256))) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void fwd_wide_kernel(const FwdArgs a) {
+void fwd_wide_kernel(const FwdArgsOf<kSinks> a) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   const int xcd = blockIdx.x % kNumXcd, p = blockIdx.x / kNumXcd, workers = gridDim.x / kNumXcd;
+  if constexpr (kSinks) {
+    EvenWalk even;
+    int pos = even.template init<256>(reinterpret_cast<int*>(smem_raw + WideFwdSmem::BYTES), a.seq, a.num_zh / a.hq, a.num_m_tiles, a.hk,
+                                      a.hq / a.hk >> a.head_shift, 256 >> a.head_shift, false, xcd, threadIdx.x) + p;
+    for (int z, h, mt; even.at(pos, z, h, mt); pos += workers) {
+      fwd_wide_item<T, kWindowed, kPad, kSplit, kSinks>(a, z, h << a.head_shift, mt, 0, smem_raw);
+      __syncthreads();
+    }
+    return;
+  }
   const int per_group = a.zh_group * a.num_m_tiles;
   const int ratio = a.hq / a.hk, nseq = a.num_zh / a.hq;
   const bool ragged = a.seq.num_seqlens != 0 && a.zh_per_xcd <= kLevelCap && a.num_m_tiles <= 0xffff;
@@ -522,21 +558,23 @@ void fwd_wide_kernel(const FwdArgs a) {
     }
     int z, h;
     split_zh(zh, nseq, ratio, z, h);
-    fwd_wide_item<T, kWindowed, kPad, kSplit>(a, z, h, mt, split, smem_raw);
+    fwd_wide_item<T, kWindowed, kPad, kSplit, kSinks>(a, z, h, mt, split, smem_raw);
     __syncthreads();
   }
 }
 
-template <typename T, bool W, int kPad, bool kSplit>
-hipError_t launch_fwd_wide(const FwdArgs& a, dim3 grid, hipStream_t stream) {
-  auto kern = fwd_wide_kernel<T, W, kPad, kSplit>;
+template <typename T, bool W, int kPad, bool kSplit, bool kSinks = false>
+hipError_t launch_fwd_wide(const FwdArgsOf<kSinks>& a, dim3 grid, hipStream_t stream) {
+  auto kern = fwd_wide_kernel<T, W, kPad, kSplit, kSinks>;
   constexpr int smem = WideFwdSmem::BYTES + kLevelBytes;
   static std::atomic<uint64_t> lds_set{0};
   hipError_t e = allow_large_lds(reinterpret_cast<const void*>(kern), smem, lds_set);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, grid, dim3(256), smem, stream, a);
   e = hipGetLastError();
-  if (kSplit && e == hipSuccess) e = launch_combine_rows<T, 128>(a, a.num_zh, stream);
+  if constexpr (kSplit) {
+    if (e == hipSuccess) e = launch_combine_rows<T, 128>(a, a.num_zh, stream);
+  }
   return e;
 }
 
@@ -555,6 +593,17 @@ hipError_t launch_fwd_wide_any(const FwdArgs& a, bool windowed, hipStream_t stre
     return windowed ? launch_fwd_wide<T, true, kPad, true>(b, grid, stream) : launch_fwd_wide<T, false, kPad, true>(b, grid, stream);
   }
   return windowed ? launch_fwd_wide<T, true, kPad, false>(b, grid, stream) : launch_fwd_wide<T, false, kPad, false>(b, grid, stream);
+}
+
+template <typename T, int kPad>
+hipError_t launch_fwd_wide_sinks(const SinkFwdArgs& a, hipStream_t stream) {
+  SinkFwdArgs b = a;
+  b.head_shift = sink_head_shift(a.hq, a.hk, 4);
+  const int BM = 256 >> b.head_shift, nseq = nseq_of(a.seq, a.batch);
+  b.num_m_tiles = (a.seq.max_seqlen_q + BM - 1) / BM;
+  b.num_zh = nseq * a.hq;
+  const dim3 grid((unsigned)(kNumXcd * tile_workers(tile_work(nseq * (a.hq >> b.head_shift), 1, b.num_m_tiles).items_per_xcd, a.num_cu, 1)));
+  return grid.x == 0 ? hipSuccess : launch_fwd_wide<T, true, kPad, false, true>(b, grid, stream);
 }
 
 }  // namespace fa

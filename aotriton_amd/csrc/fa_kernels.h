@@ -113,18 +113,19 @@ FA_DECL_SINKS(run_sinks_fwd, SinkFwdArgs)
 FA_DECL_SINKS(run_sinks_dkdv, SinkBwdArgs)
 FA_DECL_SINKS(run_sinks_dq, SinkBwdArgs)
 #undef FA_DECL_SINKS
-// the same with 64 rows per wave, head dims above 64 (fa_bwd_wide.h; of dK/dV the window's part)
-#define FA_DECL_SINKS(name)                                                                   \
-  hipError_t name##_d128(int, const SinkBwdArgs&, hipStream_t);                               \
-  hipError_t name##_d128_padded(int, const SinkBwdArgs&, hipStream_t);                        \
-  hipError_t name##_d128_cols96(int, const SinkBwdArgs&, hipStream_t);                        \
-  inline hipError_t name(int dtype, const SinkBwdArgs& a, hipStream_t s) {                    \
+// the same with 64 rows per wave, head dims above 64 (fa_fwd_wide.h, fa_bwd_wide.h; of dK/dV the window's part)
+#define FA_DECL_SINKS(name, Args)                                                             \
+  hipError_t name##_d128(int, const Args&, hipStream_t);                                      \
+  hipError_t name##_d128_padded(int, const Args&, hipStream_t);                               \
+  hipError_t name##_d128_cols96(int, const Args&, hipStream_t);                               \
+  inline hipError_t name(int dtype, const Args& a, hipStream_t s) {                           \
     if (a.head_dim == 128 && a.head_dim_v == 128) return name##_d128(dtype, a, s);            \
     const bool upto96 = a.head_dim <= 96 && a.head_dim_v <= 96;                               \
     return (upto96 ? name##_d128_cols96 : name##_d128_padded)(dtype, a, s);                   \
   }
-FA_DECL_SINKS(run_sinks_dkdv_wide)
-FA_DECL_SINKS(run_sinks_dq_wide)
+FA_DECL_SINKS(run_sinks_fwd_wide, SinkFwdArgs)
+FA_DECL_SINKS(run_sinks_dkdv_wide, SinkBwdArgs)
+FA_DECL_SINKS(run_sinks_dq_wide, SinkBwdArgs)
 #undef FA_DECL_SINKS
 
 // Vector-ALU kernels (no MFMA): every type at every compiled head dim; they serve tensors whose

@@ -298,7 +298,8 @@ def test_heads_of_a_group(Hq, Hk, S, D, dtype):
 @pytest.mark.parametrize('Hq,Hk,S,window,D,dtype', [
     (32, 8, 4099, 1100, 128, torch.bfloat16), (32, 8, 4099, 1100, 96, torch.float16), (32, 8, 4099, 1100, 104, torch.bfloat16),
     (16, 16, 4100, 1030, 128, torch.float16), (32, 8, 4099, 1100, 64, torch.bfloat16),
-    (32, 8, 8190, 1030, 128, torch.bfloat16), (32, 8, 8190, 1030, 104, torch.float16), (32, 32, 6000, 2900, 96, torch.bfloat16)])
+    (32, 8, 8190, 1030, 128, torch.bfloat16), (32, 8, 8190, 1030, 104, torch.float16), (32, 32, 6000, 2900, 96, torch.bfloat16),
+    (16, 4, 8190, 4100, 128, torch.float16), (16, 2, 8190, 4100, 104, torch.bfloat16), (12, 4, 8190, 4100, 96, torch.bfloat16)])
 def test_long_sequences(Hq, Hk, S, window, D, dtype):
     """the kernels of long sequences (64 rows per wave above 64 columns); the oracle takes the first and the last group"""
     q, k, v, do = _inputs(1, Hq, Hk, S, S, D, dtype, seed=D)
