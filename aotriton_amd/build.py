@@ -49,6 +49,8 @@ EXTRA = {
     'fa_bwd_pair_d256.hip': ['-Wno-inline-asm'],
     'fa_bwd_dqs.hip': ['-Wno-inline-asm'],
     'fa_fwd_d256.hip': ['-Wno-inline-asm'],
+    'fa_tree_d64.hip': ['-Wno-inline-asm'],
+    'fa_tree_d128.hip': ['-Wno-inline-asm'],
     'fa_bwd_dq_d128.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form'],
     # (the same kernels with sinks)
     'fa_sinks_dkdv_d128.hip': ['-mllvm', '-amdgpu-sched-strategy=max-ilp'],

@@ -2,6 +2,7 @@
 #pragma once
 #include "fa_cache_args.h"
 #include "fa_device.h"
+#include "fa_wide.h"
 
 namespace fa {
 
@@ -61,18 +62,32 @@ __device__ __forceinline__ TreeNode tree_nodes(const TreeArgs& a, int z, int len
   return n;
 }
 
-// A sequence's pages: `at` is scalar, and the table is read through the scalar cache (a kernel does not write it).
-struct PageTable {
-  const __attribute__((address_space(4))) int32_t* row;
-  int32_t columns, pages, shift;
-  __device__ __forceinline__ PageTable(const CacheArgs& c, int z)
-      : row((const __attribute__((address_space(4))) int32_t*)(c.table + (int64_t)z * c.table_row)), columns(c.columns), pages(c.pages), shift(c.page_shift) {}
-  __device__ __forceinline__ int page_of(int slot) const {      // negative: not there
-    const int col = slot >> shift;
-    if (col < 0 || col >= columns) return -1;
-    const int p = row[col];
+// Pages of a run of 16-slot stretches, entry by entry in order: 64 of them are looked up at once, a lane each, and the 64 behind them
+// are on their way.  (One at a time through the scalar cache every look-up waited for the one before: PAGES.)
+template <typename SlotOf>      // the slot of an entry, -1 behind the last
+struct PageRun {
+  const int32_t* row;
+  int32_t columns, pages, shift, lane;
+  SlotOf slot_of;
+  int now, next, first;          // this lane's pages (-1: not there); the first entry of `now`
+  __device__ __forceinline__ int look(int entry) const {
+    const int slot = slot_of(entry), col = slot >> shift;
+    int p = -1;
+    if (slot >= 0 && col < columns) p = row[col];
     return p < pages ? p : -1;
   }
+  __device__ __forceinline__ PageRun(const CacheArgs& c, int z, int lane_, SlotOf f)
+      : row(c.table + (int64_t)z * c.table_row), columns(c.columns), pages(c.pages), shift(c.page_shift), lane(lane_), slot_of(f), first(0) {
+    now = look(lane);
+    next = look(lane + 64);
+  }
+  __device__ __forceinline__ void to(int entry) {      // 0, or at most 64 after the last
+    if (entry - first < 64) return;
+    now = next;
+    first += 64;
+    next = look(first + 64 + lane);
+  }
+  __device__ __forceinline__ int at(int entry) const { return __builtin_amdgcn_readlane(now, entry - first); }      // negative: not there
 };
 
 // The blocks of slots that a sequence's rows may see: those that hold sinks, then those of the window (without one: all).
@@ -278,7 +293,11 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
     }
   }
 
-  const PageTable pages(c, z);
+  auto slot_of_half = [&](int e) {
+    const int i = from + wave + 4 * (e >> 1);
+    return i < b1 ? range.block_of(i) * 32 + 16 * (e & 1) : -1;
+  };
+  PageRun<decltype(slot_of_half)> pages(c, z, lane, slot_of_half);
   const T* kbase = reinterpret_cast<const T*>(c.k) + (int64_t)hk * c.sk.h;
   const T* vbase = reinterpret_cast<const T*>(c.v) + (int64_t)hk * c.sv.h;
   const int slot_mask = (1 << c.page_shift) - 1;
@@ -286,11 +305,10 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
   const bool k_col = !kPad || vc0 * 8 < d_qk, v_col = !kPad || vc0 * 8 < d_v;
   // pages have 16 slots or more, so a block lies in two pages at most, 16 slots in one
   struct Halves { int p0, p1; };
-  auto halves_of = [&](int b) {
-    Halves x;
-    x.p0 = pages.page_of(b * 32);
-    x.p1 = pages.page_of(b * 32 + 16);
-    return x;
+  auto halves_of = [&](int i) {
+    const int e = (i - from - wave) >> 1;
+    pages.to(e);
+    return Halves{pages.at(e), pages.at(e + 1)};
   };
   // K and V travel as whole rows, 16 bytes per lane and consecutive lanes along a row, and change to the operands' layouts in the wave's
   // LDS area, one after the other.  (K loaded as the operand that it is, 16 bytes of 32 rows per access, takes its cache lines a quarter at
@@ -335,10 +353,10 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
   int i = from + wave;
   Halves now{-1, -1}, next{-1, -1};
   if (i < b1) {
-    now = halves_of(range.block_of(i));
+    now = halves_of(i);
     load_k(range.block_of(i), now);
     load_v(range.block_of(i), now);
-    if (i + 4 < b1) next = halves_of(range.block_of(i + 4));
+    if (i + 4 < b1) next = halves_of(i + 4);
   }
   for (; i < b1; i += 4) {
     const int n0 = range.block_of(i) * 32;
@@ -368,7 +386,7 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
     if (i + 4 < b1) {
       now = next;
       load_v(range.block_of(i + 4), now);
-      if (i + 8 < b1) next = halves_of(range.block_of(i + 8));
+      if (i + 8 < b1) next = halves_of(i + 8);
     }
 
     if (prescale)
@@ -482,11 +500,13 @@ void tree_rows_kernel(const TreeArgs a) {
 // 32 rows each, as in fwd_item (the same layouts, double buffer and one barrier per tile).  Bound by HBM up to about
 // 128 rows, by what the waves issue beyond: 192 rows (48 tokens, Hq 32 Hk 8 D128, B8 up to 16384 slots) take six of eight waves,
 // 72 us for 159 MB and 29 GFLOP.
-template <int D>
+// Tiles go from memory into LDS without registers.  With one workgroup on a CU (256 rows) two of them are on their way: a tile is worked
+// on in less time than memory takes to answer.
+template <int D, int NW>
 struct TreeTileSmem {
-  static constexpr int KSTR = D + 8, VSTR = D + 32;
-  static constexpr int K_ELEMS = 64 * KSTR, V_ELEMS = 64 * VSTR;
-  static constexpr int BYTES = 2 * (K_ELEMS + V_ELEMS) * 2;
+  static constexpr int ROWB = Swz<D>::ROWB, TILE_BYTES = 64 * ROWB, STAGE_BYTES = 2 * TILE_BYTES;      // K, V (swizzled)
+  static constexpr int STAGES = NW == 8 ? 3 : 2;
+  static constexpr int BYTES = STAGES * STAGE_BYTES;
 };
 
 template <typename T, int D, int NW, bool kPad>
@@ -495,10 +515,10 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
   using q4_t = typename Tr::q4_t;
-  using SM = TreeTileSmem<D>;
-  constexpr int KS = D / 16, DB = D / 32, KSTR = SM::KSTR, VSTR = SM::VSTR;
+  using SM = TreeTileSmem<D, NW>;
+  constexpr int KS = D / 16, DB = D / 32, ROWB = SM::ROWB, AHEAD = SM::STAGES - 1;
   constexpr int LPR = D / 8, RW = 64 / LPR, RPI = NW * RW, CH = 64 / RPI;      // lanes per row; rows per wave's access, per workgroup's; accesses
-  static_assert(16 % RW == 0 && (RPI % 16 == 0), "a wave's access lies in 16 slots");
+  static_assert(16 % RW == 0 && (RPI % 16 == 0), "a wave's access lies in 16 slots, its swizzle in all of them");
 
   const CacheArgs& c = a.cache;
   const int group = a.hq / c.heads;
@@ -532,18 +552,26 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
     }
   }
 
-  const PageTable table(c, z);
+  auto slot_of = [&](int t) { return range.block_of(t) * 64; };
+  auto slot_of_quarter = [&](int e) {
+    const int t = t0 + (e >> 2);
+    return t < t1 ? slot_of(t) + 16 * (e & 3) : -1;
+  };
+  PageRun<decltype(slot_of_quarter)> table(c, z, lane, slot_of_quarter);
   const T* kbase = reinterpret_cast<const T*>(c.k) + (int64_t)hk * c.sk.h;
   const T* vbase = reinterpret_cast<const T*>(c.v) + (int64_t)hk * c.sv.h;
   const int slot_mask = (1 << c.page_shift) - 1;
-  const int rl = lane / LPR, cl = lane % LPR;      // the lane's row within a wave's access, and its piece
-  const bool k_col = !kPad || cl * 8 < d_qk, v_col = !kPad || cl * 8 < d_v;
-  const int64_t k_off = rl * c.sk.s + cl * 8, v_off = rl * c.sv.s + cl * 8;
+  const int rl = lane / LPR, cl = lane % LPR;      // the lane's row within a wave's access, and where its piece goes
+  const int ch = cl ^ Swz<D>::f(wave * RW + rl);
+  const int k_voff = !kPad || ch * 8 < d_qk ? rl * (int)c.sk.s * 2 + ch * 16 : kVoffOutOfRange;
+  const int v_voff = !kPad || ch * 8 < d_v ? rl * (int)c.sv.s * 2 + ch * 16 : kVoffOutOfRange;
   struct Quarters { int p[4]; };      // pages of a tile's 16-slot quarters
-  auto pages_of = [&](int n0) {
+  auto pages_of = [&](int t) {
+    const int e = (t - t0) * 4;
+    table.to(e);
     Quarters x;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) x.p[g] = table.page_of(n0 + 16 * g);
+    for (int g = 0; g < 4; ++g) x.p[g] = table.at(e + g);
     return x;
   };
   // access i of this wave: rows row_of(i) .. + RW - 1 of the tile
@@ -552,36 +580,34 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
     const int g = row_of(i) / 16;
     return g == 0 ? x.p[0] : g == 1 ? x.p[1] : g == 2 ? x.p[2] : x.p[3];
   };
-  op_t kreg[CH], vreg[CH];
-  auto load_tile = [&](int n0, const Quarters& x) __attribute__((always_inline)) {
+  auto holes_of = [&](const Quarters& x) {      // a bit for each quarter that has no page
+    return (x.p[0] < 0 ? 1 : 0) | (x.p[1] < 0 ? 2 : 0) | (x.p[2] < 0 ? 4 : 0) | (x.p[3] < 0 ? 8 : 0);
+  };
+  const int smem0 = lds_offset(smem_raw);
+  auto fetch = [&](int stage, int n0, const Quarters& x) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int p = page_at(x, i), slot = (n0 + row_of(i)) & slot_mask;
-      const int64_t page = p < 0 ? 0 : p;      // (not there: page 0 stands aside for it)
-      kreg[i] = op_t{};
-      vreg[i] = op_t{};
-      if (k_col) kreg[i] = *reinterpret_cast<const op_t*>(kbase + page * c.sk.z + slot * c.sk.s + k_off);
-      if (v_col) vreg[i] = *reinterpret_cast<const op_t*>(vbase + page * c.sv.z + slot * c.sv.s + v_off);
+      const int p = page_at(x, i), slot = (n0 + row_of(i)) & slot_mask, lds = smem0 + stage + row_of(i) * ROWB;
+      const int64_t page = p < 0 ? 0 : p;      // (not there: a descriptor of nothing, which reads as zero)
+      load_to_lds1(wave_rsrc_words(kbase + page * c.sk.z + slot * c.sk.s, p < 0 ? 0 : ((RW - 1) * (int)c.sk.s + d_qk) * 2), k_voff, lds);
+      load_to_lds1(wave_rsrc_words(vbase + page * c.sv.z + slot * c.sv.s, p < 0 ? 0 : ((RW - 1) * (int)c.sv.s + d_v) * 2), v_voff, lds + SM::TILE_BYTES);
     }
   };
-  T* const Ks = reinterpret_cast<T*>(smem_raw);
-  T* const Vs = Ks + 2 * SM::K_ELEMS;
-  auto is_edge = [&](int n0, const Quarters& x) {
-    return !range.whole(seq, n0, 64) || (x.p[0] | x.p[1] | x.p[2] | x.p[3]) < 0;
-  };
-  auto store_tile = [&](int stage, int n0, const Quarters& x) __attribute__((always_inline)) {
-    if (is_edge(n0, x)) {
-      // (V of slots that no row sees is 0, as above)
+  auto is_edge = [&](int n0, int holes) { return !range.whole(seq, n0, 64) || holes != 0; };
+  // The tile at n0 has landed, as far as this wave brought it (`more`: the one behind it is on its way): V of slots that no row sees
+  // becomes 0, as above.
+  auto landed = [&](int stage, int n0, int holes, bool more) __attribute__((always_inline)) {
+    if (AHEAD == 2 && more) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * CH) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (is_edge(n0, holes)) {
 #pragma unroll
       for (int i = 0; i < CH; ++i)
-        if (!range.seen(seq, there, n0 + row_of(i) + rl) || page_at(x, i) < 0) vreg[i] = op_t{};
-    }
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      *reinterpret_cast<op_t*>(Ks + stage * SM::K_ELEMS + (row_of(i) + rl) * KSTR + cl * 8) = kreg[i];
-      *reinterpret_cast<op_t*>(Vs + stage * SM::V_ELEMS + (row_of(i) + rl) * VSTR + cl * 8) = vreg[i];
+        if (!range.seen(seq, there, n0 + row_of(i) + rl))
+          *reinterpret_cast<op_t*>(smem_raw + stage + SM::TILE_BYTES + (row_of(i) + rl) * ROWB + cl * 16) = op_t{};
     }
   };
+  // (no wait for what is on its way)
+  auto meet = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
   f32x16 o[DB];
 #pragma unroll
@@ -592,16 +618,15 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
   const float qk_scale = a.sm_scale * kLog2e;
   const float sc = score_scale(a.sm_scale, false);
   const bool prescale = !(qk_scale > 0.f);
-  const int v_lane = (4 * hi + (lane & 15) / 4) * VSTR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);      // see lds_read_tr8
+  const int row_a = Swz<D>::row_base(lane), tr_a0 = Swz<D>::tr_base(lane, 0), tr_a1 = Swz<D>::tr_base(lane, 1);
 
-  auto slot_of = [&](int t) { return range.block_of(t) * 64; };
   // S^T = K Q^T with the operands read two k-steps ahead of their MFMAs; V's first operands are in flight while the softmax runs; the
   // exponentials are taken against the maximum that the rows have already, and a tile whose row sums tell that it does not do
   // goes through the full step: all as in fwd_item.
   f32x16 s[2];
   op_t va[2][DB];
   auto qk = [&](int stage) __attribute__((always_inline)) {
-    const T* ks = Ks + stage * SM::K_ELEMS + col * KSTR + 8 * hi;
+    const char* ks = smem_raw + stage;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -612,23 +637,23 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb) ka[k][mb] = *reinterpret_cast<const op_t*>(ks + mb * 32 * KSTR + 16 * k);
+      for (int mb = 0; mb < 2; ++mb) ka[k][mb] = swz_read_row<T, D>(ks, row_a, k, mb);
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       if (k + kAhead < KS)
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb)
-          ka[(k + kAhead) % (kAhead + 1)][mb] = *reinterpret_cast<const op_t*>(ks + mb * 32 * KSTR + 16 * (k + kAhead));
+          ka[(k + kAhead) % (kAhead + 1)][mb] = swz_read_row<T, D>(ks, row_a, k + kAhead, mb);
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb) s[mb] = Tr::mfma(ka[k % (kAhead + 1)][mb], qreg[k], s[mb]);
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
   };
-  auto prepare = [&](int stage, int n0, const Quarters& x, bool edge) __attribute__((always_inline)) {
-    const T* vs = Vs + stage * SM::V_ELEMS + v_lane;
+  auto prepare = [&](int stage, int n0, int holes, bool edge) __attribute__((always_inline)) {
+    const char* vs = smem_raw + stage + SM::TILE_BYTES;
 #pragma unroll
-    for (int db = 0; db < DB; ++db) va[0][db] = lds_read_tr8<T>(vs + db * 32, VSTR);
+    for (int db = 0; db < DB; ++db) va[0][db] = swz_read_tr<T, D>(vs, tr_a0, tr_a1, 0, db);
     if (prescale) {
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb)
@@ -640,13 +665,13 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
       for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const bool seen = row.sees(seq, n0 + 32 * mb + 8 * (e / 4) + 4 * hi + (e % 4)) && x.p[2 * mb + e / 8] >= 0;
+          const bool seen = row.sees(seq, n0 + 32 * mb + 8 * (e / 4) + 4 * hi + (e % 4)) && (holes >> (2 * mb + e / 8) & 1) == 0;
           s[mb][e] = seen ? s[mb][e] : -__builtin_inff();
         }
     }
   };
   auto finish = [&](int stage) __attribute__((always_inline)) {
-    const T* vs = Vs + stage * SM::V_ELEMS + v_lane;
+    const char* vs = smem_raw + stage + SM::TILE_BYTES;
     op_t pb[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) pb[k] = pack8<T>(s[k / 2], k % 2);
@@ -656,7 +681,7 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
     for (int k = 0; k < 4; ++k) {
       if (k + 1 < 4)
 #pragma unroll
-        for (int db = 0; db < DB; ++db) va[(k + 1) & 1][db] = lds_read_tr8<T>(vs + (k + 1) * 16 * VSTR + db * 32, VSTR);
+        for (int db = 0; db < DB; ++db) va[(k + 1) & 1][db] = swz_read_tr<T, D>(vs, tr_a0, tr_a1, k + 1, db);
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] = Tr::mfma(va[k & 1][db], pb[k], o[db]);
       __builtin_amdgcn_sched_barrier(0);
@@ -665,8 +690,8 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
   };
   bool have_ref = false;      // every row of the wave has a usable maximum
   float msc = 0.f;            // m_i * sc
-  auto fast_step = [&](int stage, int n0, const Quarters& x, bool edge) __attribute__((always_inline)) {
-    prepare(stage, n0, x, edge);
+  auto fast_step = [&](int stage, int n0, int holes, bool edge) __attribute__((always_inline)) {
+    prepare(stage, n0, holes, edge);
     float rs = 0.f;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
@@ -680,8 +705,8 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
     finish(stage);
     return true;
   };
-  auto full_step = [&](int stage, int n0, const Quarters& x, bool edge) __attribute__((always_inline)) {
-    prepare(stage, n0, x, edge);
+  auto full_step = [&](int stage, int n0, int holes, bool edge) __attribute__((always_inline)) {
+    prepare(stage, n0, holes, edge);
     float mx = s[0][0];
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
@@ -714,32 +739,45 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
     finish(stage);
   };
 
-  Quarters now{}, next{};      // pages of the tile that is worked on; of the next one to be asked for
+  // stages and holes of the tile that is worked on and of those behind it; the pages of the tile to be asked for next
+  int st[SM::STAGES], holes[AHEAD + 1];
+  Quarters next{};
+#pragma unroll
+  for (int i = 0; i < SM::STAGES; ++i) st[i] = i * SM::STAGE_BYTES;
+  auto ask = [&](int i, int t) __attribute__((always_inline)) {      // for tile t, i behind the one that is worked on
+    holes[i] = 0;
+    if (t >= t1) return;
+    fetch(st[i], slot_of(t), next);
+    holes[i] = holes_of(next);
+    if (t + 1 < t1) next = pages_of(t + 1);
+  };
   if (t0 < t1) {
-    now = pages_of(slot_of(t0));
-    load_tile(slot_of(t0), now);
-    if (t0 + 1 < t1) next = pages_of(slot_of(t0 + 1));
-    store_tile(0, slot_of(t0), now);
+    next = pages_of(t0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) ask(i, t0 + i);
+    landed(st[0], slot_of(t0), holes[0], t0 + 1 < t1);
   }
-  __syncthreads();
+  meet();
   for (int t = t0; t < t1; ++t) {
-    const int stage = (t - t0) & 1, n0 = slot_of(t);
-    const Quarters was = now;
-    if (t + 1 < t1) {
-      now = next;
-      load_tile(slot_of(t + 1), now);
-      if (t + 2 < t1) next = pages_of(slot_of(t + 2));
-    }
+    const int n0 = slot_of(t);
+    ask(AHEAD, t + AHEAD);
     if (active) {
-      const bool edge = is_edge(n0, was);
-      qk(stage);
-      if (!(have_ref && fast_step(stage, n0, was, edge))) {
-        if (have_ref) qk(stage);      // (the scores are spent)
-        full_step(stage, n0, was, edge);
+      const bool edge = is_edge(n0, holes[0]);
+      qk(st[0]);
+      if (!(have_ref && fast_step(st[0], n0, holes[0], edge))) {
+        if (have_ref) qk(st[0]);      // (the scores are spent)
+        full_step(st[0], n0, holes[0], edge);
       }
     }
-    if (t + 1 < t1) store_tile(stage ^ 1, slot_of(t + 1), now);
-    __syncthreads();
+    if (t + 1 < t1) landed(st[1], slot_of(t + 1), holes[1], t + 2 < t1);
+    meet();
+    const int done = st[0];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      st[i] = st[i + 1];
+      holes[i] = holes[i + 1];
+    }
+    st[AHEAD] = done;
   }
 
   if (!active) return;
@@ -776,7 +814,7 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
 template <typename T, int D, int NW, bool kPad>
 __global__ __attribute__((amdgpu_flat_work_group_size(NW * 64, NW * 64))) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void tree_tile_kernel(const TreeArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  extern __shared__ __attribute__((aligned(kSwzAlign))) char smem_raw[];
   tree_work(a, threadIdx.x & 63, [&](int z, int hk, int rb, int from, int to, bool whole, int piece) __attribute__((always_inline)) {
     tree_tile_item<T, D, NW, kPad>(a, z, hk, rb, from, to, whole, piece, smem_raw);
   });
@@ -907,8 +945,8 @@ hipError_t launch_tree(const TreeArgs& a, hipStream_t stream) {
   hipError_t e = hipErrorNotSupported;
   if (a.row_rows == 32) e = launch_tree_kernel<tree_rows_kernel<T, D, kPad>>(a, 256, TreeSmem<D>::BYTES, stream);
   if constexpr (D <= 128) {
-    if (a.row_rows == 128) e = launch_tree_kernel<tree_tile_kernel<T, D, 4, kPad>>(a, 256, TreeTileSmem<D>::BYTES, stream);
-    if (a.row_rows == 256) e = launch_tree_kernel<tree_tile_kernel<T, D, 8, kPad>>(a, 512, TreeTileSmem<D>::BYTES, stream);
+    if (a.row_rows == 128) e = launch_tree_kernel<tree_tile_kernel<T, D, 4, kPad>>(a, 256, TreeTileSmem<D, 4>::BYTES, stream);
+    if (a.row_rows == 256) e = launch_tree_kernel<tree_tile_kernel<T, D, 8, kPad>>(a, 512, TreeTileSmem<D, 8>::BYTES, stream);
   }
   return e != hipSuccess || a.part_o == nullptr ? e : launch_tree_sum<T, D>(a, stream);
 }
