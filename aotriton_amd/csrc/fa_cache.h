@@ -63,7 +63,7 @@ __device__ __forceinline__ TreeNode tree_nodes(const TreeArgs& a, int z, int len
 }
 
 // Pages of a run of 16-slot stretches, entry by entry in order: 64 of them are looked up at once, a lane each, and the 64 behind them
-// are on their way.  (One at a time through the scalar cache every look-up waited for the one before: PAGES.)
+// are on their way.  (One at a time through the scalar cache every look-up waited for the one before: B32 4900 slots, 48 tokens 225 us instead of 205.)
 template <typename SlotOf>      // the slot of an entry, -1 behind the last
 struct PageRun {
   const int32_t* row;
@@ -227,10 +227,14 @@ struct TreeRow {
     m_sink = alive && a.window > 0 ? a.sinks : 0;
     if (!alive) kin = 0;
   }
-  __device__ __forceinline__ bool sees(const TreeSeq& seq, int n) const {
-    const int j = n - seq.length;
-    return j < 0 ? (n >= m_lo || n < m_sink) : j < 64 && (kin >> (j & 63) & 1) != 0;
+  // Bit b: the row sees slot n0 + b.  (A test of its own for each slot: 48 tokens, B8 up to 16384 slots 76 us instead of 67, 64 tokens Hq 64
+  // D64 80 instead of 64.)
+  __device__ __forceinline__ uint64_t sees(const TreeSeq& seq, int n0) const {
+    const int d = seq.length - n0;
+    const uint64_t drafted = d >= 64 || d <= -64 ? 0 : d >= 0 ? kin << d : kin >> -d;
+    return (below(d) & (~below(m_lo - n0) | below(m_sink - n0))) | drafted;
   }
+  static __device__ __forceinline__ uint64_t below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
 };
 
 // ---- few rows: 32 packed (token, q-head) rows of one K/V head x one piece of the keys per workgroup -----------------------
@@ -393,11 +397,10 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] *= qk_scale;
     if (edge) {
+      const uint32_t there_now = (was.p0 < 0 ? 0 : 0xffffu) | (was.p1 < 0 ? 0 : 0xffff0000u);
+      const uint32_t seen = ((uint32_t)row.sees(seq, n0) & there_now) >> 4 * hi;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const bool seen = row.sees(seq, n0 + 8 * (e / 4) + 4 * hi + (e % 4)) && (e < 8 ? was.p0 : was.p1) >= 0;
-        s[e] = seen ? s[e] : -__builtin_inff();
-      }
+      for (int e = 0; e < 16; ++e) s[e] = (seen >> (8 * (e / 4) + e % 4) & 1) != 0 ? s[e] : -__builtin_inff();
     }
 
     float mx = s[0];
@@ -661,13 +664,14 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
         for (int e = 0; e < 16; ++e) s[mb][e] *= qk_scale;
     }
     if (edge) {
+      const uint64_t all = row.sees(seq, n0);
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
+      for (int mb = 0; mb < 2; ++mb) {
+        const uint32_t there_now = (holes >> 2 * mb & 1 ? 0 : 0xffffu) | (holes >> 2 * mb & 2 ? 0 : 0xffff0000u);
+        const uint32_t seen = ((uint32_t)(all >> 32 * mb) & there_now) >> 4 * hi;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const bool seen = row.sees(seq, n0 + 32 * mb + 8 * (e / 4) + 4 * hi + (e % 4)) && (holes >> (2 * mb + e / 8) & 1) == 0;
-          s[mb][e] = seen ? s[mb][e] : -__builtin_inff();
-        }
+        for (int e = 0; e < 16; ++e) s[mb][e] = (seen >> (8 * (e / 4) + e % 4) & 1) != 0 ? s[mb][e] : -__builtin_inff();
+      }
     }
   };
   auto finish = [&](int stage) __attribute__((always_inline)) {
