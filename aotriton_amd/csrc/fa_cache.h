@@ -88,6 +88,7 @@ struct PageRun {
     next = look(first + 64 + lane);
   }
   __device__ __forceinline__ int at(int entry) const { return __builtin_amdgcn_readlane(now, entry - first); }      // negative: not there
+  __device__ __forceinline__ int holes(int entry) const { return (int)(__builtin_amdgcn_ballot_w64(now < 0) >> (entry - first)); }      // a bit for each
 };
 
 // The blocks of slots that a sequence's rows may see: those that hold sinks, then those of the window (without one: all).
@@ -564,36 +565,26 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
   const T* kbase = reinterpret_cast<const T*>(c.k) + (int64_t)hk * c.sk.h;
   const T* vbase = reinterpret_cast<const T*>(c.v) + (int64_t)hk * c.sv.h;
   const int slot_mask = (1 << c.page_shift) - 1;
+  // strides in 32 bits (check_pages): products of two scalar instructions instead of six
+  const uint32_t k_page = (uint32_t)c.sk.z, v_page = (uint32_t)c.sv.z, k_slot = (uint32_t)c.sk.s, v_slot = (uint32_t)c.sv.s;
+  const int k_bytes = ((RW - 1) * (int)c.sk.s + d_qk) * 2, v_bytes = ((RW - 1) * (int)c.sv.s + d_v) * 2;
   const int rl = lane / LPR, cl = lane % LPR;      // the lane's row within a wave's access, and where its piece goes
   const int ch = cl ^ Swz<D>::f(wave * RW + rl);
   const int k_voff = !kPad || ch * 8 < d_qk ? rl * (int)c.sk.s * 2 + ch * 16 : kVoffOutOfRange;
   const int v_voff = !kPad || ch * 8 < d_v ? rl * (int)c.sv.s * 2 + ch * 16 : kVoffOutOfRange;
-  struct Quarters { int p[4]; };      // pages of a tile's 16-slot quarters
-  auto pages_of = [&](int t) {
-    const int e = (t - t0) * 4;
-    table.to(e);
-    Quarters x;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) x.p[g] = table.at(e + g);
-    return x;
-  };
   // access i of this wave: rows row_of(i) .. + RW - 1 of the tile
   auto row_of = [&](int i) { return wave * RW + i * RPI; };
-  auto page_at = [&](const Quarters& x, int i) {
-    const int g = row_of(i) / 16;
-    return g == 0 ? x.p[0] : g == 1 ? x.p[1] : g == 2 ? x.p[2] : x.p[3];
-  };
-  auto holes_of = [&](const Quarters& x) {      // a bit for each quarter that has no page
-    return (x.p[0] < 0 ? 1 : 0) | (x.p[1] < 0 ? 2 : 0) | (x.p[2] < 0 ? 4 : 0) | (x.p[3] < 0 ? 8 : 0);
-  };
   const int smem0 = lds_offset(smem_raw);
-  auto fetch = [&](int stage, int n0, const Quarters& x) __attribute__((always_inline)) {
+  // (a page that is not there: a descriptor of nothing, which reads as zero)
+  auto fetch = [&](int stage, int t) __attribute__((always_inline)) {
+    const int e = (t - t0) * 4, n0 = slot_of(t);
+    table.to(e);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int p = page_at(x, i), slot = (n0 + row_of(i)) & slot_mask, lds = smem0 + stage + row_of(i) * ROWB;
-      const int64_t page = p < 0 ? 0 : p;      // (not there: a descriptor of nothing, which reads as zero)
-      load_to_lds1(wave_rsrc_words(kbase + page * c.sk.z + slot * c.sk.s, p < 0 ? 0 : ((RW - 1) * (int)c.sk.s + d_qk) * 2), k_voff, lds);
-      load_to_lds1(wave_rsrc_words(vbase + page * c.sv.z + slot * c.sv.s, p < 0 ? 0 : ((RW - 1) * (int)c.sv.s + d_v) * 2), v_voff, lds + SM::TILE_BYTES);
+      const int p = table.at(e + row_of(i) / 16), slot = (n0 + row_of(i)) & slot_mask, lds = smem0 + stage + row_of(i) * ROWB;
+      const uint32_t page = p < 0 ? 0 : p;
+      load_to_lds1(wave_rsrc_words(kbase + ((uint64_t)page * k_page + (uint64_t)(uint32_t)slot * k_slot), p < 0 ? 0 : k_bytes), k_voff, lds);
+      load_to_lds1(wave_rsrc_words(vbase + ((uint64_t)page * v_page + (uint64_t)(uint32_t)slot * v_slot), p < 0 ? 0 : v_bytes), v_voff, lds + SM::TILE_BYTES);
     }
   };
   auto is_edge = [&](int n0, int holes) { return !range.whole(seq, n0, 64) || holes != 0; };
@@ -743,20 +734,17 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
     finish(stage);
   };
 
-  // stages and holes of the tile that is worked on and of those behind it; the pages of the tile to be asked for next
+  // stages and holes of the tile that is worked on and of those behind it
   int st[SM::STAGES], holes[AHEAD + 1];
-  Quarters next{};
 #pragma unroll
   for (int i = 0; i < SM::STAGES; ++i) st[i] = i * SM::STAGE_BYTES;
   auto ask = [&](int i, int t) __attribute__((always_inline)) {      // for tile t, i behind the one that is worked on
     holes[i] = 0;
     if (t >= t1) return;
-    fetch(st[i], slot_of(t), next);
-    holes[i] = holes_of(next);
-    if (t + 1 < t1) next = pages_of(t + 1);
+    fetch(st[i], t);
+    holes[i] = table.holes((t - t0) * 4) & 15;
   };
   if (t0 < t1) {
-    next = pages_of(t0);
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) ask(i, t0 + i);
     landed(st[0], slot_of(t0), holes[0], t0 + 1 < t1);

@@ -89,6 +89,9 @@ int check_pages(const fa_tensor4& k, const fa_tensor4& v, fa::CacheArgs* out) {
   if ((e = check_rows(k, k.dtype)) != FA_SUCCESS || (e = check_rows(v, k.dtype)) != FA_SUCCESS) return e;
   for (int i = 0; i < 3; ++i)
     if (k.sizes[i] != v.sizes[i] || k.sizes[i] == 0) return FA_ERROR_INVALID_VALUE;
+  // (kernels multiply with the strides of pages and rows in 32 bits)
+  for (const fa_tensor4* t : {&k, &v})
+    if (t->sizes[0] > 1 && (int64_t)t->strides[0] > 0x7fffffff) return FA_ERROR_NOT_SUPPORTED;
   const uint64_t page = k.sizes[2];
   if (page < 16 || page > (1 << 20) || (page & (page - 1)) != 0) return FA_ERROR_NOT_SUPPORTED;
   fa::CacheArgs& c = *out;

@@ -178,7 +178,7 @@ def test_tree_refusals():
         change(p)
         assert run(p) == INVALID
     for change in (lambda p: setattr(p.cache.K, 'ptr', 4104), lambda p: p.cache.K.strides.__setitem__(3, 2), lambda p: p.cache.V.strides.__setitem__(2, 60),
-                   lambda p: p.cache.V.strides.__setitem__(0, 2 ** 64 - 64), lambda p: p.cache.table.strides.__setitem__(1, 2),
+                   lambda p: p.cache.V.strides.__setitem__(0, 2 ** 64 - 64), lambda p: p.cache.K.strides.__setitem__(0, 2 ** 31), lambda p: p.cache.table.strides.__setitem__(1, 2),
                    lambda p: p.cache.lengths.strides.__setitem__(0, 2), lambda p: p.Q.strides.__setitem__(1, 100), lambda p: p.L.strides.__setitem__(0, 9)):
         p = _tree()
         change(p)
