@@ -28,7 +28,11 @@ struct TreeNode {
 __device__ __forceinline__ uint64_t shfl64(uint64_t x, int lane) {
   return (uint64_t)(uint32_t)__shfl((int)(uint32_t)(x >> 32), lane) << 32 | (uint32_t)__shfl((int)(uint32_t)x, lane);
 }
-__device__ __forceinline__ TreeNode tree_nodes(const TreeArgs& a, int z, int length, int lane, uint64_t& there) {
+// (the parents are asked for early, and looked at while the first keys are on their way)
+__device__ __forceinline__ int tree_parent(const TreeArgs& a, int z, int lane) {
+  return a.parents != nullptr && lane < a.tokens ? a.parents[(int64_t)z * a.parents_row + lane] : -2;
+}
+__device__ __forceinline__ TreeNode tree_nodes(const TreeArgs& a, int up, int length, int lane, uint64_t& there) {
   TreeNode n;
   const bool token = lane < a.tokens;
   if (a.parents == nullptr) {
@@ -36,8 +40,6 @@ __device__ __forceinline__ TreeNode tree_nodes(const TreeArgs& a, int z, int len
     n.depth = lane;
     there = a.tokens < 64 ? (1ull << a.tokens) - 1 : ~0ull;
   } else {
-    int up = -2;
-    if (token) up = a.parents[(int64_t)z * a.parents_row + lane];
     const bool ok = up >= -1 && up < lane;
     if (!ok) up = -1;
     n.kin = 1ull << lane;
@@ -276,16 +278,18 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
   const int lane = tid & 63, col = lane & 31, hi = lane >> 5;
   const int d_qk = kPad ? c.head_dim : D, d_v = kPad ? c.head_dim_v : D;
 
-  uint64_t there;
-  const TreeNode node = tree_nodes(a, z, seq.length, lane, there);
-  if (seq.end == 0) there = 0;
+  const int up = tree_parent(a, z, lane);
+  const int b1 = to < range.blocks ? to : range.blocks;
+  auto slot_of_half = [&](int e) {
+    const int i = from + wave + 4 * (e >> 1);
+    return i < b1 ? range.block_of(i) * 32 + 16 * (e & 1) : -1;
+  };
+  PageRun<decltype(slot_of_half)> pages(c, z, lane, slot_of_half);
 
-  // this lane's packed row: its drafted token, and what it sees
+  // this lane's packed row: its drafted token
   const bool row_ok = col < nrows;
   const int pr = r0 + (row_ok ? col : nrows - 1);
   const int token = pr / group, h = hk * group + pr % group;
-  const TreeRow row(a, seq, node, there, token);
-  const int b1 = to < range.blocks ? to : range.blocks;
 
   // ---- Q rows as the B operand (column = packed row), straight from global memory ----------------
   op_t qreg[KS];
@@ -298,11 +302,6 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
     }
   }
 
-  auto slot_of_half = [&](int e) {
-    const int i = from + wave + 4 * (e >> 1);
-    return i < b1 ? range.block_of(i) * 32 + 16 * (e & 1) : -1;
-  };
-  PageRun<decltype(slot_of_half)> pages(c, z, lane, slot_of_half);
   const T* kbase = reinterpret_cast<const T*>(c.k) + (int64_t)hk * c.sk.h;
   const T* vbase = reinterpret_cast<const T*>(c.v) + (int64_t)hk * c.sv.h;
   const int slot_mask = (1 << c.page_shift) - 1;
@@ -363,6 +362,10 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
     load_v(range.block_of(i), now);
     if (i + 4 < b1) next = halves_of(i + 4);
   }
+  uint64_t there;
+  const TreeNode node = tree_nodes(a, up, seq.length, lane, there);
+  if (seq.end == 0) there = 0;
+  const TreeRow row(a, seq, node, there, token);
   for (; i < b1; i += 4) {
     const int n0 = range.block_of(i) * 32;
     const bool edge = !range.whole(seq, n0, 32) || now.p0 < 0 || now.p1 < 0;
@@ -533,9 +536,14 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, col = lane & 31, hi = lane >> 5;
   const int d_qk = kPad ? c.head_dim : D, d_v = kPad ? c.head_dim_v : D;
-  uint64_t there;
-  const TreeNode node = tree_nodes(a, z, seq.length, lane, there);
-  if (seq.end == 0) there = 0;
+  const int up = tree_parent(a, z, lane);
+  const int t0 = from, t1 = to < range.blocks ? to : range.blocks;
+  auto slot_of = [&](int t) { return range.block_of(t) * 64; };
+  auto slot_of_quarter = [&](int e) {
+    const int t = t0 + (e >> 2);
+    return t < t1 ? slot_of(t) + 16 * (e & 3) : -1;
+  };
+  PageRun<decltype(slot_of_quarter)> table(c, z, lane, slot_of_quarter);
 
   // this lane's packed row (waves past the last row only stage)
   const int first_row = rb * a.row_rows + wave * 32;
@@ -543,9 +551,6 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
   const bool row_ok = first_row + col < rows;
   const int pr = row_ok ? first_row + col : rows - 1;
   const int token = pr / group, h = hk * group + pr % group;
-  const TreeRow row(a, seq, node, there, token);
-  const int t0 = from, t1 = to < range.blocks ? to : range.blocks;
-
   op_t qreg[KS];
   {
     const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)z * a.sq.z + (int64_t)h * a.sq.h + (int64_t)token * a.sq.s + 8 * hi;
@@ -556,12 +561,6 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
     }
   }
 
-  auto slot_of = [&](int t) { return range.block_of(t) * 64; };
-  auto slot_of_quarter = [&](int e) {
-    const int t = t0 + (e >> 2);
-    return t < t1 ? slot_of(t) + 16 * (e & 3) : -1;
-  };
-  PageRun<decltype(slot_of_quarter)> table(c, z, lane, slot_of_quarter);
   const T* kbase = reinterpret_cast<const T*>(c.k) + (int64_t)hk * c.sk.h;
   const T* vbase = reinterpret_cast<const T*>(c.v) + (int64_t)hk * c.sv.h;
   const int slot_mask = (1 << c.page_shift) - 1;
@@ -587,6 +586,23 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
       load_to_lds1(wave_rsrc_words(vbase + ((uint64_t)page * v_page + (uint64_t)(uint32_t)slot * v_slot), p < 0 ? 0 : v_bytes), v_voff, lds + SM::TILE_BYTES);
     }
   };
+  // stages and holes of the tile that is worked on and of those behind it
+  int st[SM::STAGES], holes[AHEAD + 1];
+#pragma unroll
+  for (int i = 0; i < SM::STAGES; ++i) st[i] = i * SM::STAGE_BYTES;
+  auto ask = [&](int i, int t) __attribute__((always_inline)) {      // for tile t, i behind the one that is worked on
+    holes[i] = 0;
+    if (t >= t1) return;
+    fetch(st[i], t);
+    holes[i] = table.holes((t - t0) * 4) & 15;
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) ask(i, t0 + i);
+
+  uint64_t there;
+  const TreeNode node = tree_nodes(a, up, seq.length, lane, there);
+  if (seq.end == 0) there = 0;
+  const TreeRow row(a, seq, node, there, token);
   auto is_edge = [&](int n0, int holes) { return !range.whole(seq, n0, 64) || holes != 0; };
   // The tile at n0 has landed, as far as this wave brought it (`more`: the one behind it is on its way): V of slots that no row sees
   // becomes 0, as above.
@@ -734,21 +750,7 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
     finish(stage);
   };
 
-  // stages and holes of the tile that is worked on and of those behind it
-  int st[SM::STAGES], holes[AHEAD + 1];
-#pragma unroll
-  for (int i = 0; i < SM::STAGES; ++i) st[i] = i * SM::STAGE_BYTES;
-  auto ask = [&](int i, int t) __attribute__((always_inline)) {      // for tile t, i behind the one that is worked on
-    holes[i] = 0;
-    if (t >= t1) return;
-    fetch(st[i], t);
-    holes[i] = table.holes((t - t0) * 4) & 15;
-  };
-  if (t0 < t1) {
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) ask(i, t0 + i);
-    landed(st[0], slot_of(t0), holes[0], t0 + 1 < t1);
-  }
+  if (t0 < t1) landed(st[0], slot_of(t0), holes[0], t0 + 1 < t1);
   meet();
   for (int t = t0; t < t1; ++t) {
     const int n0 = slot_of(t);

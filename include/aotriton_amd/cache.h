@@ -4,7 +4,7 @@
  * the reference.
  *
  * A cache is two tensors (pages, heads, slots of a page, head dim) of fp16 or bf16: any strides with a unit last one, made of aligned
- * 16-byte pieces (head dims, up to 256, and strides multiples of 8, 16-byte aligned bases), so that (pages, slots, heads, head dim) storage
+ * 16-byte pieces (head dims, up to 256, and strides multiples of 8, 16-byte aligned bases, pages less than 2^31 elements apart), so that (pages, slots, heads, head dim) storage
  * is as good; the slots of a page are a power of two from 16 up.  A sequence is a row of the page table, int32 with -1 where
  * there is no page, and a length: slot n of the sequence is slot n % slots of the page in column n / slots.  All indices are read on the
  * device, and none is trusted: pages outside the cache, sequences outside the table, slots outside a row of the table are not
