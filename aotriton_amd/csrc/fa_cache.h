@@ -243,7 +243,7 @@ struct TreeRow {
 // ---- few rows: 32 packed (token, q-head) rows of one K/V head x one piece of the keys per workgroup -----------------------
 // As fwd_rows_kernel: the waves take blocks of 32 slots in turn, each with an online softmax of its own; they meet in LDS, the parts
 // in tree_sum_kernel.  K and V are read once per 32 rows, and what bounds it is HBM (B64 up to 8192 slots, Hq 32 Hk 8 D128, one token:
-// 654 MB in 129 us, 5.1 TB/s), for short sequences the chain from the length over the page table to the rows (B1 4096 slots 8.8 us,
+// 654 MB in 129 us, 5.1 TB/s), for short sequences the chain from the length over the page table to the rows (B1 4096 slots 8.1 us,
 // 17 MB).  The blocks of an item are those that hold sinks, then those of the window (without one: all).
 template <int D>
 struct TreeSmem {
@@ -504,9 +504,8 @@ void tree_rows_kernel(const TreeArgs a) {
 // ---- many rows: 32 * NW packed rows of one K/V head x one piece of the keys per workgroup ---------------------------------------
 // With 64 drafted tokens and grouped heads a K/V head has hundreds of packed rows.  The kernel above would read its K and V once per 32 of
 // them (from L2) and feed one MFMA operand with each piece; here a tile of 64 slots is staged in LDS once for all waves, which own
-// 32 rows each, as in fwd_item (the same layouts, double buffer and one barrier per tile).  Bound by HBM up to about
-// 128 rows, by what the waves issue beyond: 192 rows (48 tokens, Hq 32 Hk 8 D128, B8 up to 16384 slots) take six of eight waves,
-// 72 us for 159 MB and 29 GFLOP.
+// 32 rows each, as in fwd_item (swizzled rows, one barrier per tile).  Bound by HBM up to about 128 rows, by what the waves issue beyond: 192 rows (48 tokens, Hq 32 Hk 8 D128, B8 up to 16384 slots) take six of eight waves,
+// 57 us for 159 MB and 29 GFLOP.
 // Tiles go from memory into LDS without registers.  With one workgroup on a CU (256 rows) two of them are on their way: a tile is worked
 // on in less time than memory takes to answer.
 template <int D, int NW>
