@@ -134,28 +134,33 @@ TreePlan tree_plan(fa::TreeArgs* a, int64_t max_length, int num_cu) {
   TreePlan p{};
   const int d = fa::compiled_columns(a->cache);
   const int64_t rows = (int64_t)a->tokens * (a->hq / a->cache.heads), sequences = a->cache.sequences;
-  a->row_rows = rows <= 64 || d > 128 ? 32 : rows <= 128 ? 128 : 256;
-  a->row_blocks = (int)((rows + a->row_rows - 1) / a->row_rows);
-  a->part_rows = (int)std::min<int64_t>(rows, a->row_rows);
-  a->block_shift = a->row_rows == 32 ? 5 : 6;
-  a->least = a->row_rows == 32 ? 8 : 2;
   // (the blocks that a sequence of that length has, at the most)
-  const int64_t size = 1 << a->block_shift;
-  auto blocks_of = [&](int64_t length) {
+  auto blocks_of = [&](int64_t length, int64_t size) {
     int64_t slots = length + a->tokens;
     if (a->window > 0) slots = std::min<int64_t>(slots, (int64_t)a->window + a->tokens + std::min<int64_t>(a->sinks, length) + 3 * size);
     return std::max<int64_t>(1, (slots + size - 1) / size);
   };
+  // 32 rows per workgroup where it has few blocks of 32 slots to do, tiles where it has many.  (us, 32 rows / 128 / 256, D128 Hq 32 Hk 8 unless
+  // said: one token, B1 4096 slots 11.5 / 12.7, B8 up to 2048 14.5 / 16.8, B64 up to 8192 129 / 129, D64 75 / 72; 4 tokens, B16 up to 8192
+  // 37 / 35, 16 tokens 46 / 40 / 42, B4 800 slots 15.3 / 16.8 / 17; 32 tokens, B1 4096 slots 21 / 26 / 22, B8 up to 6000 40 / 31 / 31; 48 tokens, B8 700
+  // slots 34 / 29 / 27, 4900 80 / 62 / 54; 64 tokens, B1 4000 slots 25 / 29 / 32.)
+  const int64_t work = blocks_of(max_length, 32) * sequences * a->cache.heads * ((rows + 31) / 32) / (2 * num_cu);
+  a->row_rows = d > 128 || work <= (rows <= 64 ? 32 : 16) ? 32 : rows <= 128 ? 128 : 256;
+  a->row_blocks = (int)((rows + a->row_rows - 1) / a->row_rows);
+  a->part_rows = (int)std::min<int64_t>(rows, a->row_rows);
+  a->block_shift = a->row_rows == 32 ? 5 : 6;
+  a->least = a->row_rows == 32 ? 8 : 2;
+  const int64_t size = 1 << a->block_shift;
   // One round of workgroups: two on a CU, one with tiles of 256 rows or more than 128 columns.
   const int64_t heads = (int64_t)a->cache.heads * a->row_blocks, chip = (int64_t)(d > 128 || a->row_rows == 256 ? 1 : 2) * num_cu;
-  const int64_t blocks = blocks_of(max_length), most = blocks_of((int64_t)a->cache.columns << a->cache.page_shift);
+  const int64_t blocks = blocks_of(max_length, size), most = blocks_of((int64_t)a->cache.columns << a->cache.page_shift, size);
   const int64_t row_bytes = d * 4 + 8;
   int64_t per = std::max<int64_t>(a->least, (blocks * sequences * heads + chip - 1) / chip), stored = 0;
-  const int64_t short_piece = a->row_rows == 32 ? 32 : 16;
   // Short pieces: a workgroup has one, of one sequence, so that nothing waits for the lengths of the others or for an item before.
-  // Long ones: equal pieces of all keys, whatever the lengths.  (us, the one / the other, D128 unless said, Hq 32 Hk 8: B1 4096 slots 11.7 / 13.3,
-  // B8 up to 2048 14.9 / 18.2, B32 Hq 16 Hk 2 D64 7 tokens window 1024 15.4 / 22.3; B64 up to 8192 145 / 132, D64 87 / 79, B8 48 tokens up to
-  // 16384 94 / 75; level B16 8 tokens up to 8192.)
+  // Long ones: equal pieces of all keys, whatever the lengths: a piece may hold the ends of two sequences, 12 us more with tiles.  (us,
+  // the one / the other, D128 unless said, Hq 32 Hk 8: B1 4096 slots 11.7 / 13.3, B8 up to 2048 14.9 / 18.2, B32 Hq 16 Hk 2 D64 7 tokens window 1024
+  // 15.4 / 22.3, B8 48 tokens 4900 54 / 66; B64 up to 8192 145 / 132, D64 87 / 79, B8 48 tokens up to 16384 117 / 63.)
+  const int64_t short_piece = a->row_rows == 32 ? 32 : 24;
   if (per <= short_piece) {
     per = std::max(per, (most * sequences * heads * a->part_rows * row_bytes + kMostScratch - 1) / kMostScratch);
     a->part_blocks = (int)per;
