@@ -93,6 +93,25 @@ def test_tree_attention(lens, Hq, Hk, tokens, D, page, window, sinks, dtype, tre
     for top in (max(lens), 0, None):      # split for the lengths, hardly, and for the table's
         out, lse = _run(q, k, v, table, n, parents, window, sinks, scale, top)
         _check(q, k, v, table, n, parents, window, sinks, scale, out, lse)
+    # a table for far more: what is planned for long caches has to do for these
+    wide = torch.full((len(lens), (1 << 22) // page), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    out, lse = _run(q, k, v, wide, n, parents, window, sinks, scale)
+    _check(q, k, v, table, n, parents, window, sinks, scale, out, lse)
+
+
+@pytest.mark.parametrize('lens,Hq,Hk,tokens,D,page,window,sinks', [
+    ([1000, 900], 64, 8, 64, 64, 16, 0, 0), ([1000, 63], 64, 8, 60, 128, 128, 500, 70), ([700, 650, 0, 5] * 4, 16, 8, 48, 64, 32, 0, 0),
+    ([700, 128, 64, 1] * 4, 24, 8, 40, 120, 16, 600, 9)])
+def test_tiles_of_short_caches(lens, Hq, Hk, tokens, D, page, window, sinks):
+    k, v, table, n = _pool(lens, tokens, Hk, D, page, torch.float16, seed=40)
+    table[0, 3] = -1
+    rng = random.Random(41)
+    parents = torch.tensor([_tree(rng, tokens, holes=0.1) for _ in lens], dtype=torch.int32)
+    q = torch.randn(len(lens), tokens, Hq, D, generator=torch.Generator().manual_seed(42)).half().transpose(1, 2)
+    out, lse = _run(q, k, v, table, n, parents, window, sinks, 1 / math.sqrt(D))
+    pick = list(range(min(len(lens), 4)))
+    _check(q[pick], k, v, table[pick], n[pick], parents[pick], window, sinks, 1 / math.sqrt(D), out[pick], lse[pick])
 
 
 def test_many_parts_of_a_long_cache():
@@ -151,8 +170,11 @@ def test_tokens_that_are_not_there(window):
                 k[table[z, s // 16], :, s % 16] = float('inf')
                 v[table[z, s // 16], :, s % 16] = float('nan')
     q = torch.randn(3, 4, tokens, 64, generator=torch.Generator().manual_seed(6)).half()
-    out, lse = _run(q, k, v, table, n, parents, window, 2 if window else 0, 0.125)
-    _check(q, k, v, table, n, parents, window, 2 if window else 0, 0.125, out, lse)
+    wide = torch.full((3, 1 << 18), -1, dtype=torch.int32)      # (of 16 slots: planned for a long cache)
+    wide[:, :table.shape[1]] = table
+    for t in (wide, table):
+        out, lse = _run(q, k, v, t, n, parents, window, 2 if window else 0, 0.125)
+        _check(q, k, v, table, n, parents, window, 2 if window else 0, 0.125, out, lse)
     assert (out[2] == 0).all() and torch.isinf(lse[2]).all()
 
 
@@ -172,6 +194,10 @@ def test_bad_lengths_and_pages():
     for window, sinks in ((0, 0), (50, 20)):
         out, lse = _run(q, k, v, table, n, parents, window, sinks, 0.125)
         _check(q, k, v, table, n, parents, window, sinks, 0.125, out, lse)
+        many = [0, 1, 2, 3] * 64                             # (enough of them for tiles)
+        far, far_lse = _run(q[many], k, v, table[many], n[many], parents[many], window, sinks, 0.125)
+        _check(q[:4], k, v, table, n, parents, window, sinks, 0.125, far[:4], far_lse[:4])
+        assert all(torch.equal(far[i:i + 4], far[:4]) for i in range(0, 256, 4))
     assert (out[0] == 0).all()
 
 
