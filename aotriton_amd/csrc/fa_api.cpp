@@ -1588,6 +1588,28 @@ int fa_attn_bwd_sinks(const fa_bwd_params* p, int32_t params_version, int32_t wi
   return rc;
 }
 
+int fa_zero_tails(const fa_tensor4* tensors, const fa_tensor1* cu_seqlens, int32_t count, void* hip_stream) {
+  if (count < 0 || count > FA_MAX_TAILS || (count > 0 && (tensors == nullptr || cu_seqlens == nullptr))) return FA_ERROR_INVALID_VALUE;
+  fa::TailArgs a{};
+  int n = 0;
+  for (int i = 0; i < count; ++i) {
+    const fa_tensor4& t = tensors[i];
+    const fa_tensor1& c = cu_seqlens[i];
+    if (!is_16bit(t.dtype) || t.sizes[0] != 1 || t.sizes[1] > INT32_MAX || t.sizes[2] > INT32_MAX || c.dtype != FA_DTYPE_INT32 || c.sizes[0] < 1 || c.ptr == nullptr)
+      return FA_ERROR_INVALID_VALUE;
+    if (t.sizes[1] == 0 || t.sizes[2] == 0) continue;
+    if (t.sizes[3] == 0 || t.sizes[3] % 8 != 0 || t.strides[3] != 1 || (reinterpret_cast<uintptr_t>(t.ptr) & 15) != 0) return FA_ERROR_NOT_SUPPORTED;
+    for (int d = 1; d < 3; ++d)
+      if (t.sizes[d] > 1 && ((int64_t)t.strides[d] <= 0 || t.strides[d] % 8 != 0)) return FA_ERROR_NOT_SUPPORTED;
+    if (c.sizes[0] > 1 && c.strides[0] != 1) return FA_ERROR_NOT_SUPPORTED;
+    if (t.ptr == nullptr) return FA_ERROR_INVALID_VALUE;
+    a.t[n++] = {static_cast<uint16_t*>(t.ptr), static_cast<const int32_t*>(c.ptr) + c.sizes[0] - 1, (int64_t)t.strides[1], (int64_t)t.strides[2],
+                (int32_t)t.sizes[1], (int32_t)t.sizes[2], (int32_t)(t.sizes[3] / 8)};
+  }
+  const int e = fa_check_gpu(hip_stream);
+  return e != FA_SUCCESS ? e : (int)fa::run_zero_tails(a, n, static_cast<hipStream_t>(hip_stream));
+}
+
 // kernel_slot < 0: the whole backward of the chosen backend; otherwise only that
 // kernel (0 delta, 1 dK/dV, 2 dQ, 3 fused; 4-6 the three kernels of the backward that keeps dS).
 // own_delta: the split backend with delta in the library's own per-device array (params->D is

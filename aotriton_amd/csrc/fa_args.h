@@ -235,6 +235,16 @@ inline int32_t sink_head_shift(int32_t hq, int32_t hk, int32_t waves) {
 template <bool kSinks> using FwdArgsOf = std::conditional_t<kSinks, SinkFwdArgs, FwdArgs>;
 template <bool kSinks> using BwdArgsOf = std::conditional_t<kSinks, SinkBwdArgs, BwdArgs>;
 
+// Rows of packed tensors behind the last sequence, which ends at *end.
+struct TailArgs {
+  struct Tensor {
+    uint16_t* ptr;
+    const int32_t* end;
+    int64_t head, row;      // strides
+    int32_t heads, tokens, pieces;
+  } t[4];
+};
+
 // Copy between a rank-4 tensor of any strides and head dim (unit last stride) and its packed
 // image: contiguous (n0, n1, n2, dp) with dp the head dim rounded up to a multiple of 8, zeros in
 // the excess columns.

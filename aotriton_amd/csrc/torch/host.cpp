@@ -518,6 +518,7 @@ std::tuple<Tensor, Tensor> sink_forward_kernel(const Tensor& q_in, const Tensor&
   TORCH_CHECK(view2(lse, &p.L) && view4(o, &p.Out), "outputs");
   Scratch scratch;
   check_rc(fa_attn_fwd_sinks(&p, FA_FWD_PARAMS_VERSION, w, n, current_stream(), nullptr, &scratch.c), false);
+  if (packed) check_rc(fa_zero_tails(&p.Out, &p.cu_seqlens_q, 1, current_stream()), false);
   return {std::move(o), std::move(lse)};
 }
 
@@ -542,6 +543,11 @@ std::tuple<Tensor, Tensor, Tensor> sink_backward_kernel(const Tensor& dout_in, c
   p.D = delta.c;
   Scratch scratch;
   check_rc(fa_attn_bwd_sinks(&p, FA_BWD_PARAMS_VERSION, w, n, current_stream(), nullptr, &scratch.c), false);
+  if (vl.cu_q.defined()) {
+    const fa_tensor4 grads[3] = {p.DQ, p.DK, p.DV};
+    const fa_tensor1 ends[3] = {p.cu_seqlens_q, p.cu_seqlens_k, p.cu_seqlens_k};
+    check_rc(fa_zero_tails(grads, ends, 3, current_stream()), false);
+  }
   return {std::move(dq), std::move(dk), std::move(dv)};
 }
 

@@ -293,6 +293,12 @@ FA_API int fa_attn_fwd_sinks(const fa_fwd_params* params, int32_t params_version
 FA_API int fa_attn_bwd_sinks(const fa_bwd_params* params, int32_t params_version, int32_t window, int32_t sinks,
                              void* hip_stream, const fa_options* options, fa_allocator* alloc);
 
+/* Zeros behind the last sequence of up to four packed 16-bit tensors (1, heads, tokens, head dim) of aligned 16-byte pieces: the rows from
+ * tensor i's last offset on, cu_seqlens[i] an int32 vector on the device.  The attention calls leave these rows alone; a caller that
+ * hands out new tensors clears them here, without reading the offset back. */
+#define FA_MAX_TAILS 4
+FA_API int fa_zero_tails(const fa_tensor4* tensors, const fa_tensor1* cu_seqlens, int32_t count, void* hip_stream);
+
 /* The positional v2 API: v2::flash::attn_fwd, attn_fwd_compact_varlen, attn_bwd, attn_bwd_fused,
  * attn_bwd_compact_varlen.  These are not in the reference tree (0.14 keeps only the v3 params
  * entry points); their signatures are those of AOTriton 0.11's include/aotriton/v2/flash.h:31-141

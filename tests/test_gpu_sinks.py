@@ -330,3 +330,24 @@ def test_sequences_of_very_different_lengths(lens, Hq, Hk, D, sinks):
         at = slice(offs[i], offs[i + 1])
         _check(q[0][:, at], k[0][:, at], v[0][:, at], do[0][:, at], window, sinks, 1 / math.sqrt(D), out[0][:, at], None,
                [t[0][:, at] for t in grads], f'sequence {i} ', device=DEV)
+
+
+@pytest.mark.parametrize('tail_q,tail_k,Hq,Hk,D,layout', [(5, 0, 4, 2, 64, 'tokens first'), (0, 300, 2, 2, 128, 'heads first'), (700, 1, 8, 1, 96, 'tokens first'),
+                                                        (0, 0, 2, 1, 64, 'heads first')])
+def test_tokens_behind_the_last_sequence_get_zeros(tail_q, tail_k, Hq, Hk, D, layout):
+    lens = [130, 1, 77]
+    n = sum(lens)
+    q, _, _, do = _inputs(1, Hq, Hk, n + tail_q, 1, D, torch.float16, seed=50)
+    _, k, v, _ = _inputs(1, Hq, Hk, 1, n + tail_k, D, torch.float16, seed=51)
+    if layout == 'heads first':
+        q, k, v, do = (t.contiguous() for t in (q, k, v, do))
+    for t, tail in ((q, tail_q), (do, tail_q), (k, tail_k), (v, tail_k)):
+        t[:, :, t.shape[2] - tail:] = float('nan')
+    rubbish = [torch.full((1, Hq, n + 700, 128), float('nan'), dtype=torch.float16, device=DEV) for _ in range(8)]
+    del rubbish      # what new tensors are made of
+    cu = torch.tensor([0, 130, 131, n], dtype=torch.int32, device=DEV)
+    out, grads = _step(q, k, v, do, 40, 3, cu_seqlens_q=cu, cu_seqlens_k=cu, max_seqlen_q=130, max_seqlen_k=130)
+    for t in (out, *grads):
+        assert torch.isfinite(t).all() and (t[:, :, n:] == 0).all()
+    at = slice(0, 130)
+    _check(q[0][:, at], k[0][:, at], v[0][:, at], do[0][:, at], 40, 3, 1 / math.sqrt(D), out[0][:, at], None, [t[0][:, at] for t in grads])

@@ -237,6 +237,25 @@ def test_page_refusals():
     assert lib.fa_cache_free(ref(over.table), ref(t1(9)), ref(t1(2)), ref(t1(2)), ref(t1(2)), None) == NOT_SUPPORTED
 
 
+def test_tail_refusals():
+    if torch.cuda.is_available():
+        pytest.skip('arguments stand for no memory')
+    L = _lib()
+
+    def run(count=2, sizes=(1, 4, 100, 64), dtype=torch.bfloat16, ptr=4096, strides=None, cu=torch.int32, cu_ptr=4096, n=3):
+        t, c = (L.fa_tensor4 * 2)(), (L.fa_tensor1 * 2)()
+        for i in range(2):
+            _fill(t[i], sizes, dtype, ptr, strides)
+            _fill(c[i], (n,), cu, cu_ptr)
+        return L.lib.fa_zero_tails(t, c, count, None)
+    assert run() in ACCEPTED and run(count=0) in ACCEPTED and run(sizes=(1, 4, 0, 64), ptr=0) in ACCEPTED
+    for bad in (dict(count=5), dict(count=-1), dict(sizes=(2, 4, 100, 64)), dict(dtype=torch.float32), dict(ptr=0), dict(cu=torch.int64), dict(cu_ptr=0), dict(n=0)):
+        assert run(**bad) == INVALID
+    for bad in (dict(sizes=(1, 4, 100, 60)), dict(ptr=4104), dict(strides=(1, 6400, 0, 1)), dict(strides=(1, 6404, 64, 1)), dict(strides=(1, 6400, 64, 2))):
+        assert run(**bad) == NOT_SUPPORTED
+    assert L.lib.fa_zero_tails(None, None, 1, None) == INVALID
+
+
 # ---- the oracle -----------------------------------------------------------------------------------------------------
 
 def test_mask_of_window_and_sinks():
