@@ -250,7 +250,8 @@ int fa_cache_append(const fa_tensor4* k, const fa_tensor4* v, const fa_cache* ca
   a.new_k = k->ptr; a.new_v = v->ptr;
   a.snk = strides3(*k); a.snv = strides3(*v);
   a.tokens = (int32_t)k->sizes[2];
-  if (!fits((double)c.sequences * a.tokens * c.heads * ((c.head_dim + c.head_dim_v) / 8) / 256 + 1)) return FA_ERROR_NOT_SUPPORTED;
+  const double pieces = (double)a.tokens * c.heads * ((c.head_dim + c.head_dim_v) / 8);
+  if (!fits(pieces) || !fits(c.sequences * (pieces / 256 + 1))) return FA_ERROR_NOT_SUPPORTED;
   if ((e = fa_check_gpu(hip_stream)) != FA_SUCCESS) return e;
   return (int)fa::run_cache_append(a, static_cast<hipStream_t>(hip_stream));
 }

@@ -45,7 +45,7 @@ struct AppendArgs {
   const void* new_k; const void* new_v;      // (sequences, heads, tokens, columns)
   Strides3 snk, snv;
   const int32_t* counts;                     // rows of each sequence; null: all
-  int32_t tokens;
+  int32_t tokens, chunks;                    // chunks: workgroups of a sequence (the launcher's)
 };
 
 struct CopyArgs {

@@ -2,8 +2,8 @@
 //
 // All of it moves bytes: 16 bytes per lane, consecutive lanes along a row.  What bounds the bulk copy is HBM (2048 pages of 64 slots,
 // 8 heads, D128, bf16: 1.07 GB in 218 us, 4.9 TB/s); the others move a few MB and are bound by their launch and two dependent round trips
-// to memory, the page table, then the rows (32 sequences, 24 rows each: append and a path of 6 of them 5.0-5.8 us each; 8 forks and
-// 8 frees of 63 pages 3.7 us each).
+// to memory, the page table, then the rows (32 sequences, 24 rows each: append 3.6 us, a path of 6 of them 6.7; 8 forks 3.9, 8 frees of
+// 63 pages 2.7 us; a caller in Python takes longer to ask for them).
 #include "fa_cache.h"
 #include "fa_kernels.h"
 
@@ -25,17 +25,16 @@ __device__ __forceinline__ uint16_t* row_of(void* base, const Strides3& s, int p
 }
 
 // ---- append: row t of sequence z to slot lengths[z] + t ----------------------------------------------------------
-// A thread per piece.
+// A thread per piece, a.chunks workgroups per sequence (one list of all pieces divides 64-bit numbers).
 __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
   const CacheArgs& c = a.cache;
-  const int per_k = c.head_dim / 8, per_v = c.head_dim_v / 8, per = per_k + per_v;
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int ch = (int)(e % per), h = (int)(e / per % c.heads);
-  const int64_t zt = e / per / c.heads;
-  const int t = (int)(zt % a.tokens), z = (int)(zt / a.tokens);
-  if (z >= c.sequences) return;
-  if (a.counts != nullptr && t >= a.counts[z]) return;
-  const int n = c.lengths[z];
+  const uint32_t per_k = c.head_dim / 8, per = per_k + c.head_dim_v / 8;
+  const int z = blockIdx.x / a.chunks;
+  const int n = c.lengths[z], count = a.counts != nullptr ? a.counts[z] : a.tokens;
+  const uint32_t e = blockIdx.x % a.chunks * 256 + threadIdx.x, th = e / per;
+  const int t = th / (uint32_t)c.heads, h = th % (uint32_t)c.heads;
+  const uint32_t ch = e % per;
+  if (t >= a.tokens || t >= count) return;
   int page;
   if (n < 0 || !page_at(c, z, (int64_t)n + t, page)) return;
   const int slot = slot_in_page(c, (int64_t)n + t);
@@ -140,22 +139,33 @@ __global__ __launch_bounds__(64) void keep_path_kernel(const KeepArgs a) {
   void* base = v ? c.v : c.k;
   const Strides3& st = v ? c.sv : c.sk;
   const int32_t* path = a.path + (int64_t)z * a.path_row;
+  if (c.columns == 0) return;
+  const int32_t* row = c.table + (int64_t)z * c.table_row;
+  // (a look-up without a branch: all of a step's are on their way together, and in front of its stores, which the compiler must not
+  // pass with loads)
+  auto look = [&](int64_t slot, int& page) {
+    const int64_t at = slot >> c.page_shift;
+    const bool ok = at >= 0 && at < c.columns;
+    page = row[ok ? at : 0];
+    return ok && page >= 0 && page < c.pages;
+  };
   for (int i0 = 0; i0 < count; i0 += kKeepRows) {
     piece_t x[kKeepRows];
+    int from[kKeepRows], page[kKeepRows], to[kKeepRows];
     bool live[kKeepRows];
 #pragma unroll
-    for (int k = 0; k < kKeepRows; ++k) {
-      const int i = i0 + k, from = i < count ? path[i] : -1;
-      int page;
-      live[k] = from > i && page_at(c, z, (int64_t)length + from, page);      // (from == i: it is there already)
-      if (live[k]) x[k] = *reinterpret_cast<const piece_t*>(row_of(base, st, page, h, slot_in_page(c, (int64_t)length + from)) + col);
-    }
+    for (int k = 0; k < kKeepRows; ++k) from[k] = path[i0 + k < count ? i0 + k : i0];
 #pragma unroll
     for (int k = 0; k < kKeepRows; ++k) {
-      int page;
-      const int64_t slot = (int64_t)length + i0 + k;
-      if (live[k] && page_at(c, z, slot, page)) *reinterpret_cast<piece_t*>(row_of(base, st, page, h, slot_in_page(c, slot)) + col) = x[k];
+      const bool there = look((int64_t)length + from[k], page[k]), room = look((int64_t)length + i0 + k, to[k]);
+      live[k] = i0 + k < count && from[k] > i0 + k && there && room;      // (from == i: it is there already)
     }
+#pragma unroll
+    for (int k = 0; k < kKeepRows; ++k)
+      if (live[k]) x[k] = *reinterpret_cast<const piece_t*>(row_of(base, st, page[k], h, slot_in_page(c, (int64_t)length + from[k])) + col);
+#pragma unroll
+    for (int k = 0; k < kKeepRows; ++k)
+      if (live[k]) *reinterpret_cast<piece_t*>(row_of(base, st, to[k], h, slot_in_page(c, (int64_t)length + i0 + k)) + col) = x[k];
   }
 }
 
@@ -173,10 +183,11 @@ unsigned blocks_of(int64_t n, int per) { return (unsigned)((n + per - 1) / per);
 
 }  // namespace
 
-hipError_t run_cache_append(const AppendArgs& a, hipStream_t s) {
-  const int64_t n = (int64_t)a.cache.sequences * a.tokens * a.cache.heads * ((a.cache.head_dim + a.cache.head_dim_v) / 8);
-  if (n == 0) return hipSuccess;
-  hipLaunchKernelGGL(append_kernel, dim3(blocks_of(n, 256)), dim3(256), 0, s, a);
+hipError_t run_cache_append(const AppendArgs& a0, hipStream_t s) {
+  AppendArgs a = a0;
+  a.chunks = (int)blocks_of((int64_t)a.tokens * a.cache.heads * ((a.cache.head_dim + a.cache.head_dim_v) / 8), 256);
+  if (a.cache.sequences == 0 || a.chunks == 0) return hipSuccess;
+  hipLaunchKernelGGL(append_kernel, dim3((unsigned)(a.cache.sequences * a.chunks)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
