@@ -1447,6 +1447,11 @@ double sink_bwd_time(const Shape& s, bool keys, int64_t tokens, int heads, int g
 // B4 Hq 16 Hk 4 S1024 window 256 110 / 99 / 157 / 146; B1 Hq 8 Hk 2 S4096 window 512 121 / 124 / 184 / 189; packed, 4 of up to 8000 tokens, H8,
 // window 1024 359 / 327 / 342 / 310, 16 of up to 6000, Hq 16 Hk 4, 512 874 / 757 / 929 / 804.)
 struct SinkBwdRoute { bool wide_dq, wide_dkdv; };
+// Up to this window dQ's kernel with 32 rows per wave takes delta from P and dP (SinkBwdArgs::exact_delta): the fewer keys a row has, the more
+// the rounding of its output weighs.  (dQ off from 64 bits by so many times what fp32 arithmetic is, 4 sinks, S3000 D64 fp16: window 16 1.54 -> 1.42,
+// 32 1.49 -> 1.42, 48 1.47, 300 1.45; at D128 1.53 -> 1.42 at 16.  The backward in us: window 32, H16 S8192 D64 85 -> 99, B4 H8 S1000 D128 56 -> 64,
+// Hq 32 Hk 8 S8192 D128, which would take 64 rows per wave, 198 -> 278.)
+constexpr int32_t kShortWindow = 40;
 SinkBwdRoute sink_bwd_route(const Shape& s, int64_t tokens_q, int64_t tokens_k, int32_t window, int num_cu) {
   if (s.d != 128) return SinkBwdRoute{false, false};
   const int shift = fa::sink_head_shift(s.hq, s.hk, 4), group = s.hq / s.hk;
@@ -1456,7 +1461,7 @@ SinkBwdRoute sink_bwd_route(const Shape& s, int64_t tokens_q, int64_t tokens_k, 
   auto dkdv = [&](int rows, int step, double item, double cost) {
     return sink_bwd_time(s, true, tokens_k, s.hk, group, rows, step, window, num_cu, item, cost);
   };
-  return SinkBwdRoute{dq(256, 32, 5, 1.42) < 0.97 * dq(128, 64, 5, 1.7), dkdv(256, 32, 7, 1.8) < dkdv(128, 64, 9, 1.95)};
+  return SinkBwdRoute{window > kShortWindow && dq(256, 32, 5, 1.42) < 0.97 * dq(128, 64, 5, 1.7), dkdv(256, 32, 7, 1.8) < dkdv(128, 64, 9, 1.95)};
 }
 
 }  // namespace
@@ -1578,6 +1583,7 @@ int fa_attn_bwd_sinks(const fa_bwd_params* p, int32_t params_version, int32_t wi
   FA_LOG(4, "attn_bwd_sinks: D=%d window=%d sinks=%d nseq=%d pieces=%d parts=%d", s.d, a.window, a.sinks, s.num_seqlens, a.sink_pieces, a.sink_parts);
   const SinkBwdRoute route = sink_bwd_route(s, (int64_t)p->Q.sizes[2], (int64_t)p->K.sizes[2], a.window, dev->num_cu);
   a.wide = route.wide_dkdv ? 1 : 0;
+  a.exact_delta = a.window <= kShortWindow ? 1 : 0;
   a.walk_group = 2;
   // (dQ in front: it writes delta, which the others read)
   if (rc == FA_SUCCESS) rc = (int)(route.wide_dq ? fa::run_sinks_dq_wide(p->Q.dtype, a, stream) : fa::run_sinks_dq(p->Q.dtype, s.d, a, stream));

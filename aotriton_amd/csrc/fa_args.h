@@ -218,6 +218,7 @@ struct SinkBwdArgs : BwdArgs {
   int32_t sink_pieces, sink_parts, sink_steps;
   int32_t wide;          // the window's part of dK and dV is another launch's (64 keys per wave)
   int32_t head_shift;    // as in SinkFwdArgs, of the dQ kernel
+  int32_t exact_delta;   // dQ's kernel (32 rows per wave) forms delta from P and dP, not from the rounded output
   float* sink_ws;        // fp32 sums of the pieces of blocks that are several (of a list: two per piece)
 };
 

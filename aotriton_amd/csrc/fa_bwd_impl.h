@@ -1419,6 +1419,57 @@ __device__ __forceinline__ void dq_item(const BwdArgsOf<kSinks>& a, const int h0
     direct_landed();
   };
 
+  // Short windows (SinkBwdArgs::exact_delta): the rows' sums of dS over all their tiles first, which put delta right as above.
+  // (window 16, 4 sinks, S3000 D64 fp16: dQ 1.54 times as far from 64 bits as fp32 arithmetic without, 1.42 with.)
+  if constexpr (kSinks) {
+    if (a.exact_delta) {
+      fetch_begin(true);
+#pragma unroll
+      for (int i = 0; i < FETCH_PIECES; ++i) fetch_piece(i);
+      direct_landed();
+      __syncthreads();
+      float off = 0.f;
+      for (int j = front > 0 ? 0 : br.lo, at = 0; j <= br.hi; ++at) {
+        const char* Kb = smem_raw + (at & 1) * SM::STAGE_BYTES;
+        f_stage = (at & 1) ^ 1;
+        fetch_begin(j < br.hi);
+#pragma unroll
+        for (int i = 0; i < FETCH_PIECES; ++i) fetch_piece(i);
+        const unsigned m_d = m_none ? 0x40000000u : (unsigned)(j * BN + 4 * hi - m_lo);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          f32x16 s, dp = negd16;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) s = Tr::mfma(swz_read_row<T, D>(Kb, row_a, k, mb), qreg[k], s);
+#pragma unroll
+          for (int k = 0; k < KS; ++k) dp = Tr::mfma(swz_read_row<T, D>(Kb + SM::TILE_BYTES, row_a, k, mb), doreg[k], dp);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int e = 32 * mb + 8 * (i / 4) + i % 4;
+            const bool vis = m_d + (unsigned)e <= m_rng || j * BN + 4 * hi + e < m_sink;
+            off += fast_exp2(vis ? __builtin_fmaf(s[i], qk_scale, -l_row) : -__builtin_inff()) * dp[i];
+          }
+        }
+        direct_landed();
+        __syncthreads();
+        if (++j == front) j = br.lo;
+      }
+      d_row += cross_sum(off);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) negd16[i] = -d_row;
+      const int first = q0 + rw_u * 32, rows = si.seqlen_q - first;
+      const auto rs = wave_rsrc(a.delta + lse_offset(si, h, a.hq) + first, rows < 0 ? 0 : rows < 32 ? rows * 4 : 128);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, d_row), rs, hi ? kVoffOutOfRange : c * 4, 0, 0);
+      // the tiles once more, from the first
+      kt = kbase + (front > 0 ? 0 : (int64_t)br.lo * BN * a.sk.s);
+      vt = vbase + (front > 0 ? 0 : (int64_t)br.lo * BN * a.sv.s);
+      rows_left = si.seqlen_k - (front > 0 ? 0 : br.lo * BN);
+      front_left = front;
+      f_stage = 0;
+    }
+  }
   fetch_begin(true);
 #pragma unroll
   for (int i = 0; i < FETCH_PIECES; ++i) fetch_piece(i);
