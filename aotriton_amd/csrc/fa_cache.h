@@ -243,7 +243,7 @@ struct TreeRow {
 // ---- few rows: 32 packed (token, q-head) rows of one K/V head x one piece of the keys per workgroup -----------------------
 // As fwd_rows_kernel: the waves take blocks of 32 slots in turn, each with an online softmax of its own; they meet in LDS, the parts
 // in tree_sum_kernel.  K and V are read once per 32 rows, and what bounds it is HBM (B64 up to 8192 slots, Hq 32 Hk 8 D128, one token:
-// 654 MB in 129 us, 5.1 TB/s), for short sequences the chain from the length over the page table to the rows (B1 4096 slots 8.1 us,
+// 654 MB in 129 us, in tiles 126), for short sequences the chain from the length over the page table to the rows (B1 4096 slots 8.1 us,
 // 17 MB).  The blocks of an item are those that hold sinks, then those of the window (without one: all).
 template <int D>
 struct TreeSmem {
