@@ -438,8 +438,10 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
   }
 
   // ---- the four waves' partial results meet in LDS --------------------------------------------
-  // (a token that is not there is masked in edge blocks only; it ends without a sum, and what it summed is not looked at)
+  // (a token that is not there is masked in edge blocks only; it ends without a sum, and what it summed is not looked at.  Nor is its
+  // maximum, which a query that may hold anything can make inf: differences of those would be NaN)
   const float l = row.alive ? cross_sum(l_i) : 0.f;
+  if (!row.alive) m_i = kNegBig;
   __syncthreads();      // the V areas become the O areas
   float* ml = reinterpret_cast<float*>(smem_raw + SM::ML_OFF);
   float* ow = reinterpret_cast<float*>(smem_raw + wave * SM::O_BYTES);

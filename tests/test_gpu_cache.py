@@ -178,6 +178,28 @@ def test_tokens_that_are_not_there(window):
     assert (out[2] == 0).all() and torch.isinf(lse[2]).all()
 
 
+@pytest.mark.parametrize('lens,tokens,Hq,Hk,D', [([700, 140, 40], 5, 4, 2, 64), ([900, 300], 12, 8, 2, 128), ([600, 200], 40, 16, 2, 64), ([300, 5], 4, 2, 2, 256)])
+def test_queries_of_tokens_that_are_not_there(lens, tokens, Hq, Hk, D):
+    """they may be anything: scores that overflow to inf or are NaN, in slots that every other token sees whole"""
+    k, v, table, n = _pool(lens, tokens, Hk, D, 16, torch.bfloat16, seed=70)
+    rng = random.Random(71)
+    rows = [_tree(rng, tokens, holes=0.3) for _ in lens]
+    rows[0][1], rows[0][2] = -2, -1
+    gone = torch.tensor([[longctx.chain(r, t) is None for t in range(tokens)] for r in rows])
+    parents = torch.tensor(rows, dtype=torch.int32)
+    clean = torch.randn(len(lens), Hq, tokens, D, generator=torch.Generator().manual_seed(72)).bfloat16()
+    clean[gone[:, None].expand(-1, Hq, -1)] = 0
+    for value, columns in ((3e38, 1), (3e38, D), (math.inf, 1), (-math.inf, 1), (math.inf, D), (math.nan, D)):
+        q = clean.clone()
+        q[..., :columns][gone[:, None, :].expand(-1, Hq, -1)] = value
+        for top in (None, max(lens), 0):
+            out, lse = _run(q, k, v, table, n, parents, 0, 0, 1 / math.sqrt(D), top)
+            _check(clean, k, v, table, n, parents, 0, 0, 1 / math.sqrt(D), out, lse)
+            many = list(range(len(lens))) * 48                 # (equal pieces)
+            far, far_lse = _run(q[many], k, v, table[many], n[many], parents[many], 0, 0, 1 / math.sqrt(D), top)
+            _check(clean, k, v, table, n, parents, 0, 0, 1 / math.sqrt(D), far[-len(lens):], far_lse[-len(lens):])
+
+
 def test_bad_lengths_and_pages():
     """a negative length, lengths past the table, entries that are no pages: what they stand for is not there"""
     lens, tokens, page = [100, 200, 60, 150], 3, 16
