@@ -511,8 +511,8 @@ std::tuple<Tensor, Tensor> sink_forward_kernel(const Tensor& q_in, const Tensor&
   fa_fwd_params p{};
   fill_common(p, q, k, v, Tensor(), sm_scale, 0.0, Mask{}, vl);
   const bool packed = vl.cu_q.defined();
-  // in the memory order of the queries
-  Tensor o = q.size(3) == v.size(3) ? at::empty_like(q) : at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
+  // in the memory order of the queries as they came: the traced call, which knows of no copies, says so
+  Tensor o = q.size(3) == v.size(3) ? at::empty_like(q_in) : at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
   if (o.stride(-1) != 1) o = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
   Tensor lse = at::empty({packed ? q.size(1) : q.size(0) * q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
   TORCH_CHECK(view2(lse, &p.L) && view4(o, &p.Out), "outputs");
@@ -536,7 +536,7 @@ std::tuple<Tensor, Tensor, Tensor> sink_backward_kernel(const Tensor& dout_in, c
   fa_bwd_params p{};
   fill_common(p, q, k, v, Tensor(), sm_scale, 0.0, Mask{}, vl);
   const auto like = [](const Tensor& t) { Tensor g = at::empty_like(t); return g.stride(-1) == 1 ? g : at::empty(t.sizes(), t.options()); };
-  Tensor dq = like(q), dk = like(k), dv = like(v);
+  Tensor dq = like(q_in), dk = like(k_in), dv = like(v_in);      // (as they came, see above)
   TORCH_CHECK(view4(out, &p.Out) && view4(dout, &p.DO) && view2(lse, &p.L) && view4(dq, &p.DQ) && view4(dk, &p.DK) && view4(dv, &p.DV),
               "the last stride of tensors must be 1");
   LazyDelta delta(lse.sizes(), lse.device());

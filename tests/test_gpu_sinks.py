@@ -364,3 +364,55 @@ def test_short_windows_take_delta_from_the_tiles(Hq, Hk, S, D, window, sinks):
     want = longctx.attention_grads(q[0], k[0], v[0], do[0], seen, 1 / math.sqrt(D))[0]
     off = ((grads[0][0].double() - want).norm() / want.norm()).item()
     assert off < 1.04 * 0.600 * 2.0 ** -11, off * 2 ** 11
+
+
+def _odd(t, n=67):
+    """the same values in (batch, tokens, heads, n) storage: rows that are no 16-byte pieces"""
+    x = t.transpose(1, 2)
+    return torch.empty(*x.shape[:3], n, dtype=t.dtype, device=t.device)[..., 1:1 + t.shape[3]].copy_(x).transpose(1, 2)
+
+
+@pytest.mark.parametrize('which', ['q', 'k', 'v', 'all', 'offset'])
+def test_layouts_of_results(which):
+    """what the traced call says of its results' storage is what they have"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from aotriton_amd import torch_ops  # noqa: F401  (the fakes)
+    q, k, v, do = _inputs(2, 4, 2, 130, 130, 64, torch.bfloat16, seed=80)
+    if which == 'offset':
+        q, k, v = (torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.transpose(1, 2).shape).copy_(t.transpose(1, 2)).transpose(1, 2) for t in (q, k, v))
+    else:
+        q, k, v = (_odd(t) if which in (name, 'all') else t for name, t in (('q', q), ('k', k), ('v', v)))
+    fwd, bwd = torch.ops.aotriton_amd.sink_attention_forward, torch.ops.aotriton_amd.sink_attention_backward
+    out, lse = fwd(q, k, v, None, None, 0, 0, 33, 4, 0.125)
+    grads = bwd(do, q, k, v, out, lse, None, None, 0, 0, 33, 4, 0.125)
+    with FakeTensorMode() as mode:
+        f = [mode.from_tensor(t) for t in (do, q, k, v, out, lse)]
+        said = [*fwd(*f[1:4], None, None, 0, 0, 33, 4, 0.125), *bwd(*f, None, None, 0, 0, 33, 4, 0.125)]
+    for got, want in zip((out, lse, *grads), said):
+        assert got.shape == want.shape and got.stride() == want.stride()
+
+
+@pytest.mark.parametrize('packed', [False, True])
+def test_compiled_steps_on_any_storage(packed):
+    from aotriton_amd import torch_ops
+    B = 1 if packed else 2
+    q, k, v, do = _inputs(B, 4, 2, 130, 130, 64, torch.bfloat16, seed=81)
+    extra = {}
+    if packed:
+        cu = torch.tensor([0, 70, 71, 130], dtype=torch.int32, device=DEV)
+        extra = dict(cu_seqlens_q=cu, cu_seqlens_k=cu, max_seqlen_q=70, max_seqlen_k=70)
+
+    def step(q, k, v):
+        out = torch_ops.sink_attention(q, k, v, 33, 4, **extra)
+        return out.transpose(1, 2).reshape(B, 130, 256)      # (a view, if the result is stored as the query is)
+    weight = do.transpose(1, 2).reshape(B, 130, 256)
+    want = None
+    for odd in (False, True):
+        leaves = [(_odd(t) if odd else t).detach().requires_grad_(True) for t in (q, k, v)]
+        torch._dynamo.reset()
+        compiled = torch.compile(step, backend='aot_eager', fullgraph=True)
+        for f in (step, compiled):
+            out = f(*leaves)
+            got = (out.detach(), *torch.autograd.grad(out, leaves, weight))
+            want = got if want is None else want
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
