@@ -167,11 +167,11 @@ struct TreeList {
   }
 };
 
-// First row of the sums of a sequence in one of its pieces.  Pieces of the list and their sequences ascend together, so that
-// piece + sequence names the pair.
-__device__ __forceinline__ int64_t tree_sums(const TreeArgs& a, int hk, int rb, int piece, int z) {
+// First row of the sums of a sequence in one of its pieces.  A piece of the list has two places: for the one sequence that
+// began in front of it, and for the one that begins in it and goes on behind.
+__device__ __forceinline__ int64_t tree_sums(const TreeArgs& a, int hk, int rb, int piece, int z, bool begins) {
   const int64_t block = hk * a.row_blocks + rb;
-  return (a.workers > 0 ? block * (a.workers + a.cache.sequences) + piece + z : (block * a.cache.sequences + z) * a.parts + piece) * a.part_rows;
+  return (a.workers > 0 ? (block * a.workers + piece) * 2 + (begins ? 1 : 0) : (block * a.cache.sequences + z) * a.parts + piece) * a.part_rows;
 }
 
 // A workgroup's items: f(sequence, head, block of rows, first block, end, whether these are all of the sequence's, piece).
@@ -205,9 +205,10 @@ __device__ __forceinline__ void tree_work(const TreeArgs& a, int lane, F f) {
       first = (int)(at - list.start);
       take = size - first < end - at ? size - first : (int)(end - at);
     } else {
-      if (piece > 0 && piece >= (size + a.part_blocks - 1) / a.part_blocks) return;
+      // (the last piece has what is left, also of a sequence that is longer than planned)
       first = piece * a.part_blocks;
-      take = size - first < a.part_blocks ? size - first : a.part_blocks;
+      if (piece > 0 && first >= size) return;
+      take = piece + 1 == a.parts || size - first < a.part_blocks ? size - first : a.part_blocks;
     }
     f(z, hk, rb, first, first + take, take == size, piece);
     at += take;
@@ -473,7 +474,7 @@ __device__ __forceinline__ void tree_rows_item(const TreeArgs& a, const int z, c
       acc += f * *reinterpret_cast<const f32x4*>(smem_raw + v * SM::O_BYTES + (r * OSTR + at) * 4);
     }
     if (!whole) {
-      const int64_t sums = tree_sums(a, hk, rb, piece, z) + r;
+      const int64_t sums = tree_sums(a, hk, rb, piece, z, from == 0) + r;
       *reinterpret_cast<f32x4*>(a.part_o + sums * D + at) = acc;
       if (at == 0) {
         a.part_ml[sums * 2] = m;
@@ -779,7 +780,7 @@ __device__ __forceinline__ void tree_tile_item(const TreeArgs& a, const int z, c
   const float l = row.alive ? cross_sum(l_i) : 0.f;
   if (!row_ok) return;
   if (!whole) {
-    const int64_t sums = tree_sums(a, hk, rb, piece, z) + wave * 32 + col;
+    const int64_t sums = tree_sums(a, hk, rb, piece, z, from == 0) + wave * 32 + col;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -837,13 +838,16 @@ static __global__ __launch_bounds__(256) void tree_sum_kernel(const TreeArgs a) 
     parts = (int)((list.start + size - 1) / list.per) - p0 + 1;
   } else {
     parts = (size + a.part_blocks - 1) / a.part_blocks;
+    parts = parts < a.parts ? parts : a.parts;
   }
   if (parts <= 1) return;                              // (the whole workgroup: its results are there already)
   const int lane_row = threadIdx.x / TPR / kSlots, slot = threadIdx.x / TPR % kSlots, col = threadIdx.x % TPR * 4;
   const int r = blockIdx.x % chunks * ROWS + lane_row, pr = rb * a.row_rows + r;
   const bool ok = r < a.part_rows && pr < a.tokens * group;
   const float sc = score_scale(a.sm_scale, false);
-  const int64_t at = tree_sums(a, hk, rb, p0, z) + (ok ? r : 0);
+  const int64_t at = tree_sums(a, hk, rb, p0, z, true) + (ok ? r : 0);
+  // (tree_sums of piece i behind that of the first: of a list 0, 1, 3, 5, ...)
+  auto place = [&](int i) { return (int64_t)(a.workers > 0 && i > 0 ? 2 * i - 1 : i) * a.part_rows; };
   const float* po = a.part_o + at * D + col;
   const float* pm = a.part_ml + at * 2;
   float m = kNegBig, l = 0.f;
@@ -854,8 +858,8 @@ static __global__ __launch_bounds__(256) void tree_sum_kernel(const TreeArgs a) 
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
       const int i = i0 + k * kSlots < parts ? i0 + k * kSlots : i0;
-      ml[k] = *reinterpret_cast<const vec<float, 2>*>(pm + (int64_t)i * a.part_rows * 2);
-      x[k] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(po + (int64_t)i * a.part_rows * D));
+      ml[k] = *reinterpret_cast<const vec<float, 2>*>(pm + place(i) * 2);
+      x[k] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(po + place(i) * D));
     }
     float top = m;
 #pragma unroll

@@ -129,7 +129,6 @@ bool fits(double workgroups) { return workgroups < 2147483648.0; }
 
 // Rows per workgroup, how the keys are cut, and the scratch for the sums of sequences that lie in several pieces.
 struct TreePlan { int64_t o_bytes, bytes; };
-constexpr int64_t kMostScratch = 256 << 20;
 TreePlan tree_plan(fa::TreeArgs* a, int64_t max_length, int num_cu) {
   TreePlan p{};
   const int d = fa::compiled_columns(a->cache);
@@ -151,27 +150,28 @@ TreePlan tree_plan(fa::TreeArgs* a, int64_t max_length, int num_cu) {
   a->block_shift = a->row_rows == 32 ? 5 : 6;
   a->least = a->row_rows == 32 ? 8 : 2;
   const int64_t size = 1 << a->block_shift;
-  // One round of workgroups: two on a CU, one with tiles of 256 rows or more than 128 columns.
+  // One round of workgroups: two on a CU, one with tiles of 256 rows or more than 128 columns.  What else the table has room for plays no
+  // part.  (us, cut for a table of 131072 slots / for max_length, D128 Hq 32 Hk 8: B64 512 slots, one token, 391 / 24, B8 4096 slots, 64 tokens,
+  // 122 / 57.)
   const int64_t heads = (int64_t)a->cache.heads * a->row_blocks, chip = (int64_t)(d > 128 || a->row_rows == 256 ? 1 : 2) * num_cu;
-  const int64_t blocks = blocks_of(max_length, size), most = blocks_of((int64_t)a->cache.columns << a->cache.page_shift, size);
-  const int64_t row_bytes = d * 4 + 8;
-  int64_t per = std::max<int64_t>(a->least, (blocks * sequences * heads + chip - 1) / chip), stored = 0;
+  const int64_t blocks = blocks_of(max_length, size);
+  const int64_t per = std::max<int64_t>(a->least, (blocks * sequences * heads + chip - 1) / chip);
+  int64_t stored = 0;      // (at most two places for a workgroup of the round, whatever the table and the sequences are)
   // Short pieces: a workgroup has one, of one sequence, so that nothing waits for the lengths of the others or for an item before.
   // Long ones: equal pieces of all keys, whatever the lengths: a piece may hold the ends of two sequences, 12 us more with tiles.  (us,
   // the one / the other, D128 unless said, Hq 32 Hk 8: B1 4096 slots 11.7 / 13.3, B8 up to 2048 14.9 / 18.2, B32 Hq 16 Hk 2 D64 7 tokens window 1024
   // 15.4 / 22.3, B8 48 tokens 4900 54 / 66; B64 up to 8192 145 / 132, D64 87 / 79, B8 48 tokens up to 16384 117 / 63.)
   const int64_t short_piece = a->row_rows == 32 ? 32 : 24;
   if (per <= short_piece) {
-    per = std::max(per, (most * sequences * heads * a->part_rows * row_bytes + kMostScratch - 1) / kMostScratch);
     a->part_blocks = (int)per;
-    a->parts = (int)((most + per - 1) / per);
+    a->parts = (int)((blocks + per - 1) / per);
     if (a->parts > 1) stored = heads * sequences * a->parts * a->part_rows;
   } else if (chip / heads > 1) {
     a->workers = (int)(chip / heads);
-    stored = heads * (a->workers + sequences) * a->part_rows;
+    stored = heads * a->workers * 2 * a->part_rows;
   }
   p.o_bytes = stored * d * 4;
-  p.bytes = stored * row_bytes;
+  p.bytes = stored * (d * 4 + 8);
   return p;
 }
 
@@ -226,7 +226,6 @@ int fa_tree_attn(const fa_tree_params* p, void* hip_stream, fa_allocator* alloc)
   if (a.part_o == nullptr) {      // every sequence is one piece
     a.workers = 0;
     a.parts = 1;
-    a.part_blocks = 1 << 29;
   }
   if (!fits(((double)c.heads * (a.workers > 0 ? a.workers : (double)c.sequences * a.parts) + 8) * a.row_blocks) || !fits((double)c.sequences * c.heads * a.row_blocks * 256)) return FA_ERROR_NOT_SUPPORTED;
   return (int)fa::run_tree(dtype, a, static_cast<hipStream_t>(hip_stream));

@@ -1,5 +1,6 @@
 """The cache of pages and the attention of drafted tokens over it, against the 64-bit oracle: lengths around blocks, pages and parts, trees
 with tokens that are not there, windows with sinks, holes in the page table, slots that hold anything.  Bounds: tests/_longctx.py."""
+import ctypes
 import math
 import random
 
@@ -138,6 +139,64 @@ def test_equal_pieces_of_many_sequences(tokens, Hq, D, window):
     far = (alone.float() - out.float()).abs().amax((1, 2, 3))
     most = torch.where(torch.isfinite(v), v, 0.0).abs().max().item()
     assert (far <= 2 * 2.1 * 2.0 ** -8 * most).all()      # (two of out_bound's: 2.01 half steps of |V|, and what the scores are off by)
+
+
+def _scratch(q, k, v, table, n, max_length):
+    """fa_tree_attn through the C ABI: its result, and the bytes of scratch that it asks for"""
+    from aotriton_amd._lib import fa_tree_params, lib
+    from test_gpu_sinks import _view
+    held, asked = [], []
+
+    def alloc(_, size):
+        asked.append(size)
+        held.append(torch.empty(size, dtype=torch.uint8, device=DEV))
+        return held[-1].data_ptr()
+
+    class Allocator(ctypes.Structure):
+        _fields_ = [('cookie', ctypes.c_void_p), ('alloc', ctypes.CFUNCTYPE(ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64))]
+    a = Allocator()
+    a.alloc = Allocator._fields_[1][1](alloc)
+    p = fa_tree_params()
+    out = torch.empty_like(q)
+    for view, t in ((p.Q, q), (p.Out, out), (p.cache.K, k), (p.cache.V, v), (p.cache.table, table), (p.cache.lengths, n)):
+        _view(view, t)
+    p.Sm_scale, p.max_length = 0.125, max_length
+    assert lib.fa_tree_attn(ctypes.byref(p), torch.cuda.current_stream().cuda_stream, ctypes.byref(a)) == 0
+    torch.cuda.synchronize()
+    return out, sum(asked)
+
+
+@pytest.mark.parametrize('B,tokens,length,columns', [(8, 64, 4096, 2048), (1, 1, 2048, 4096), (8, 1, 300, 8192)])
+def test_scratch_follows_the_lengths(B, tokens, length, columns):
+    """a table for much longer sequences changes neither how the keys are cut nor the scratch"""
+    page, Hq, Hk, D = 64, 32, 8, 128
+    need = -(-(length + tokens) // page)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k, v = (torch.randn(need * 2, Hk, page, D, device=DEV, generator=g).bfloat16() for _ in range(2))
+    table = torch.full((B, columns), -1, dtype=torch.int32, device=DEV)
+    table[:, :need] = torch.randint(0, need * 2, (B, need), device=DEV, generator=g, dtype=torch.int32)
+    n = torch.full((B,), length, dtype=torch.int32, device=DEV)
+    q = torch.randn(B, Hq, tokens, D, device=DEV, generator=g).bfloat16()
+    out, narrow = _scratch(q, k, v, table[:, :need].contiguous(), n, length)
+    far, wide = _scratch(q, k, v, table, n, length)
+    assert torch.equal(out, far)
+    assert narrow == wide
+
+
+def test_scratch_of_many_sequences():
+    """the sums of sequences that lie in several pieces are of a number that the chip sets, not the sequences"""
+    page, tokens, Hq, Hk, D, length = 64, 64, 8, 2, 64, 2000
+    need = -(-(length + tokens) // page)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    k, v = (torch.randn(need, Hk, page, D, device=DEV, generator=g).half() for _ in range(2))
+    asked = []
+    for B in (300, 600):
+        table = torch.arange(need, dtype=torch.int32, device=DEV).expand(B, need).contiguous()
+        n = torch.full((B,), length, dtype=torch.int32, device=DEV)
+        q = torch.randn(B, Hq, tokens, D, device=DEV, generator=g).half()
+        out, size = _scratch(q, k, v, table, n, length)
+        asked.append(size)
+    assert asked[0] == asked[1] <= 128 << 20
 
 
 @pytest.mark.parametrize('tokens,Hq', [(1, 2), (20, 8)])
