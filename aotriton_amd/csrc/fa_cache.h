@@ -11,7 +11,8 @@ struct TreeSeq {
   int32_t length, end;           // filled slots; slots with the drafted tokens, as far as the table goes (0: the sequence is not there)
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int z) {
-  const int n = a.cache.lengths[z];
+  // (positions, which are up to 63 more, stay below 2^31; the table, and with it what such a sequence sees, ends at 2^29)
+  const int raw = a.cache.lengths[z], n = raw < 0x7fffffff - kTreeTokens ? raw : 0x7fffffff - kTreeTokens;
   const int64_t room = (int64_t)a.cache.columns << a.cache.page_shift, end = (int64_t)n + a.tokens;
   TreeSeq s;
   s.length = n;
@@ -107,7 +108,8 @@ struct TreeBlocks {
     first = win_lo >> shift;
     sinks = a.window > 0 ? a.sinks : 0;
     front = sinks < first << shift ? (sinks + (1 << shift) - 1) >> shift : first;
-    blocks = last >= first ? front + last - first + 1 : 0;
+    // (a window that starts behind the table leaves the sinks)
+    blocks = last >= first ? front + last - first + 1 : front < last + 1 ? front : last + 1;
   }
   __device__ __forceinline__ int block_of(int i) const { return i < front ? i : first + i - front; }
   // every row sees all of these slots, as far as their pages are there

@@ -282,6 +282,27 @@ def test_bad_lengths_and_pages():
     assert (out[0] == 0).all()
 
 
+@pytest.mark.parametrize('past', [1, 10, 100, 2 ** 31 - 1])
+@pytest.mark.parametrize('tokens,Hq', [(1, 4), (3, 4), (40, 16)])
+def test_a_window_behind_the_table(past, tokens, Hq):
+    """of a sequence that is longer than its row of the table the sinks are still there"""
+    page, columns, window, sinks = 16, 6, 10, 20
+    room = page * columns
+    k, v, table, _ = _pool([room], 0, 2, 64, page, torch.bfloat16, seed=73, columns=columns)
+    table = table.expand(3, columns).clone()
+    table[1, 1] = -1
+    n = torch.tensor([min(room + past, 2 ** 31 - 1), min(room + past, 2 ** 31 - 2), room], dtype=torch.int64).int()
+    q = torch.randn(3, Hq, tokens, 64, generator=torch.Generator().manual_seed(74)).bfloat16()
+    # (the oracle goes through all slots: a length that the window leaves the table behind by)
+    same = torch.tensor([min(room + past, 3 * room), min(room + past, 3 * room), room], dtype=torch.int32)
+    for w, s in ((window, sinks), (1, 1), (window, 5000), (1, 0)):
+        out, lse = _run(q, k, v, table, n, None, w, s, 0.125)
+        _check(q, k, v, table, same, None, w, s, 0.125, out, lse)
+        many = [0, 1, 2] * 80
+        far, far_lse = _run(q[many], k, v, table[many], n[many], None, w, s, 0.125)
+        _check(q, k, v, table, same, None, w, s, 0.125, far[-3:], far_lse[-3:])
+
+
 def test_released_pages_under_a_window():
     """pages between the sinks and the window go back to the pool and are somebody else's"""
     from aotriton_amd import cache
