@@ -94,12 +94,12 @@ __global__ __launch_bounds__(256) void fork_kernel(const ForkArgs a) {
   if (b >= a.chunks) {
     const int col = (b - a.chunks) * 256 + threadIdx.x;
     if (col >= c.columns) return;
+    // (a partial page that is not there has no copy, and leaves the spare one alone)
     int page = -1;
-    if (col < full) {
+    if (col < full || (col == full && tail > 0)) {
       page = c.table[(int64_t)from * c.table_row + col];
       if (page < 0 || page >= c.pages) page = -1;
-    } else if (col == full && tail > 0 && spare_ok) {
-      page = spare;
+      else if (col == full) page = spare_ok ? spare : -1;
     }
     if (page >= 0) atomicAdd(a.uses + page, 1);      // (whole numbers: the order does not matter)
     a.table_out[(int64_t)to * c.table_row + col] = page;

@@ -447,6 +447,38 @@ def test_fork_and_free():
     assert torch.equal(dt.cpu(), table) and torch.equal(du.cpu(), uses)
 
 
+def test_a_fork_of_rows_that_are_not_there():
+    """the partial page of the source is no page: the spare one stays free"""
+    from aotriton_amd import cache
+    page = 16
+    k, v, table, n = _pool([40, 24, 20, 7, 5], 0, 2, 64, page, torch.float16, seed=75, extra=8, columns=4)
+    table = torch.cat([table, torch.tensor([[0, 1, 2, 3]] * 5, dtype=torch.int32)])
+    n = torch.cat([n, torch.full((5,), 9, dtype=torch.int32)])
+    table[0, 2], table[1, 1], table[2, 1] = -1, k.shape[0], -(2 ** 31)
+    used = set(table[:5].flatten().tolist())
+    spare = [p for p in range(k.shape[0]) if p not in used][:5]
+    uses = torch.zeros(k.shape[0], dtype=torch.int32)
+    dk, dv, dt, dn, du = (t.to(DEV) for t in (k, v, table, n, uses))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    cache.fork(dk, dv, dt, dn, du, ints([0, 1, 2, 3, 4]), ints([5, 6, 7, 8, 9]), ints(spare))
+    want, want_n = table.clone(), n.clone()
+    for a, b in ((0, 5), (1, 6), (2, 7), (3, 8), (4, 9)):
+        full = int(n[a]) // page
+        want[b] = -1
+        want[b, :full] = table[a, :full]
+        want_n[b] = n[a]
+        for p in table[a, :full].tolist():
+            uses[p] += 1
+    for a, b, rows in ((3, 8, 7), (4, 9, 5)):
+        want[b, 0] = spare[a]
+        uses[spare[a]] += 1
+        k[spare[a], :, :rows], v[spare[a], :, :rows] = k[table[a, 0], :, :rows].clone(), v[table[a, 0], :, :rows].clone()
+    assert torch.equal(dt.cpu(), want)
+    assert torch.equal(dn.cpu(), want_n) and torch.equal(du.cpu(), uses)
+    _equal(dk, k)
+    _equal(dv, v)
+
+
 @pytest.mark.parametrize('window,sinks', [(0, 0), (90, 4)])
 def test_a_prompt_then_drafted_tokens(window, sinks):
     """The operators together: a prompt goes through attention with sinks into the cache, the sequence is forked, trees are drafted,
