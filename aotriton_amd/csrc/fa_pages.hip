@@ -88,7 +88,8 @@ __global__ __launch_bounds__(256) void fork_kernel(const ForkArgs a) {
   const int per_fork = a.chunks + a.table_chunks, i = blockIdx.x / per_fork, b = blockIdx.x % per_fork;
   const int from = a.source[i], to = a.target[i];
   if (from < 0 || from >= c.sequences || to < 0 || to >= c.sequences || from == to) return;
-  const int length = c.lengths[from] > 0 ? c.lengths[from] : 0;
+  const int length = c.lengths[from];
+  if (length < 0) return;      // (a sequence that is not there has no forks)
   const int full = length >> c.page_shift, tail = slot_in_page(c, length), spare = a.spare[i];
   const bool spare_ok = spare >= 0 && spare < c.pages;
   if (b >= a.chunks) {

@@ -479,6 +479,19 @@ def test_a_fork_of_rows_that_are_not_there():
     _equal(dv, v)
 
 
+def test_a_sequence_that_is_not_there_has_no_fork():
+    from aotriton_amd import cache
+    k, v, table, n = _pool([40, 24, 20, 7], 0, 2, 64, 16, torch.float16, seed=76, extra=3)
+    n[0], n[1] = -1, -(2 ** 31)
+    uses = torch.zeros(k.shape[0], dtype=torch.int32)
+    dk, dv, dt, dn, du = (t.to(DEV) for t in (k, v, table, n, uses))
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    cache.fork(dk, dv, dt, dn, du, ints(0, 1), ints(2, 3), ints(8, 9))
+    assert torch.equal(dt.cpu(), table) and torch.equal(dn.cpu(), n) and torch.equal(du.cpu(), uses)
+    _equal(dk, k)
+    _equal(dv, v)
+
+
 @pytest.mark.parametrize('window,sinks', [(0, 0), (90, 4)])
 def test_a_prompt_then_drafted_tokens(window, sinks):
     """The operators together: a prompt goes through attention with sinks into the cache, the sequence is forked, trees are drafted,
