@@ -14,7 +14,8 @@ A step of speculative decoding, with nothing that waits for the device:
 Which pages belong to whom is the caller's: page_table, and ``uses``, the number of table entries that name a page (a page without
 one is free).  fork and free keep both up to date.  Indices are read on the device and none is trusted: a page outside the
 cache, a sequence outside the table, a slot outside a row of the table, a negative length stand for nothing, which is not read and not
-written.  All functions run on torch's current stream and can be captured into a HIP graph.  Shapes, types, strides and devices
+written.  All functions run on torch's current stream and can be captured into a HIP graph.  None has a gradient: where autograd
+would record one (NotImplementedError), call them under torch.no_grad().  Shapes, types, strides and devices
 are checked on the host: ValueError, or RuntimeError with the library's hipError_t.
 """
 import math

@@ -7,6 +7,7 @@
 #include <limits>
 #include <optional>
 #include <tuple>
+#include <type_traits>
 #include <vector>
 
 #include "aotriton_amd/cache.h"
@@ -166,6 +167,49 @@ std::tuple<Tensor, Tensor> tree_autograd(const Tensor& query, const Tensor& k, c
   return op.call(query, k, v, table, lengths, parents, max_length, window, sinks, sm_scale);
 }
 
+// The ops that write, kWritten the places of what they write to: no derivatives either, and the version counters of those tensors move,
+// so that a backward that has kept one of them says so.
+constexpr char kAppend[] = "aotriton_amd::cache_append", kCopy[] = "aotriton_amd::cache_copy_pages", kFork[] = "aotriton_amd::cache_fork",
+               kKeep[] = "aotriton_amd::cache_keep_path", kFree[] = "aotriton_amd::cache_free";
+template <const char* kName, auto kKernel, size_t... kWritten> struct Writer;
+template <const char* kName, typename R, typename... A, R (*kKernel)(A...), size_t... kWritten>
+struct Writer<kName, kKernel, kWritten...> {
+  static const c10::TypedOperatorHandle<R(A...)>& op() {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(kName, "").template typed<R(A...)>();
+    return op;
+  }
+  static R autograd(c10::DispatchKeySet keys, A... a) {
+    const auto refuse = [](const auto& t) {
+      if constexpr (std::is_same_v<std::decay_t<decltype(t)>, Tensor>) {
+        refuse_tangents({&t});
+        TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t.requires_grad()), kName, " has no gradient; call it under torch.no_grad()");
+      }
+    };
+    (refuse(a), ...);
+    return op().redispatch(keys & c10::after_autograd_keyset, a...);
+  }
+  static R inplace(c10::DispatchKeySet keys, A... a) {
+    const auto all = std::forward_as_tuple(a...);
+    // (a tensor of inference mode has no counter)
+    const auto written = [](const Tensor& t) {
+      if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+    };
+    if constexpr (std::is_void_v<R>) {
+      op().redispatch(keys & c10::after_ADInplaceOrView_keyset, a...);
+      (written(std::get<kWritten>(all)), ...);
+    } else {
+      R r = op().redispatch(keys & c10::after_ADInplaceOrView_keyset, a...);
+      (written(std::get<kWritten>(all)), ...);
+      return r;
+    }
+  }
+};
+using Append = Writer<kAppend, &append_kernel, 2, 3>;
+using Copy = Writer<kCopy, &copy_kernel, 0, 1>;
+using Fork = Writer<kFork, &fork_kernel, 0, 1, 2, 3, 4>;
+using Keep = Writer<kKeep, &keep_kernel, 0, 1>;
+using Free = Writer<kFree, &free_kernel, 0, 1>;
+
 TORCH_LIBRARY_FRAGMENT(aotriton_amd, m) {
   const std::vector<at::Tag> compliant{at::Tag::pt2_compliant_tag};
   m.def("tree_attention(Tensor query, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor lengths, Tensor? parents, SymInt max_length, "
@@ -187,6 +231,18 @@ TORCH_LIBRARY_IMPL(aotriton_amd, CUDA, m) {
 }
 TORCH_LIBRARY_IMPL(aotriton_amd, Autograd, m) {
   m.impl("tree_attention", &tree_autograd);
+  m.impl("cache_append", &Append::autograd);
+  m.impl("cache_copy_pages", &Copy::autograd);
+  m.impl("cache_fork", &Fork::autograd);
+  m.impl("cache_keep_path", &Keep::autograd);
+  m.impl("cache_free", &Free::autograd);
+}
+TORCH_LIBRARY_IMPL(aotriton_amd, ADInplaceOrView, m) {
+  m.impl("cache_append", &Append::inplace);
+  m.impl("cache_copy_pages", &Copy::inplace);
+  m.impl("cache_fork", &Fork::inplace);
+  m.impl("cache_keep_path", &Keep::inplace);
+  m.impl("cache_free", &Free::inplace);
 }
 
 }  // namespace

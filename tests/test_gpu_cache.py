@@ -606,3 +606,60 @@ def test_two_streams_and_schemas():
         torch.library.opcheck(getattr(torch.ops.aotriton_amd, op), args, test_utils=('test_schema', 'test_faketensor'))
     with pytest.raises(NotImplementedError, match='no gradient'):
         cache.tree_attention(q.requires_grad_(True), k, v, table, n)
+
+
+def test_writes_are_seen_by_autograd():
+    from aotriton_amd import cache
+    k, v, table, n = (t.to(DEV) for t in _pool([20, 5], 4, 2, 64, 16, torch.float16, seed=82))
+    new = torch.randn(2, 2, 4, 64, device=DEV).half()
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    uses = torch.ones(k.shape[0], dtype=torch.int32, device=DEV)
+    calls = [(lambda: cache.append(new, new, k, v, table, n), (k, v)),
+             (lambda: cache.copy_pages(k, v, ints(0), ints(1)), (k, v)),
+             (lambda: cache.keep_path(k, v, table, n, ints(0, 1, 2, 3).view(2, 2), ints(1, 2)), (k, v)),
+             (lambda: cache.fork(k, v, table, n, uses, ints(0), ints(1), ints(3)), (k, v, table, n, uses)),
+             (lambda: cache.free(table, uses, ints(0), ints(0), ints(1)), (table, uses))]
+    for call, written in calls:
+        before = [t._version for t in written]
+        call()
+        assert [t._version for t in written] == [x + 1 for x in before]
+    for quiet in (torch.no_grad, torch.inference_mode):
+        with quiet():
+            before = k._version
+            calls[0][0]()
+            assert k._version == before + 1
+    with torch.inference_mode():
+        mine = [t.clone() for t in (k, v)]
+    cache.append(new, new, *mine, table, n)
+    _equal(mine[0], k)
+    # a backward that needs a cache as it was says so
+    w = torch.ones_like(k, requires_grad=True)
+    y = (w * k).sum()
+    calls[0][0]()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward()
+
+
+@pytest.mark.parametrize('window', [0, 30])
+def test_compiled_serving_step(window):
+    from aotriton_amd import cache
+    k, v, table, n = (t.to(DEV) for t in _pool([300, 45], 16, 2, 64, 16, torch.bfloat16, seed=83))
+    g = torch.Generator().manual_seed(84)
+    q, nk, nv = (torch.randn(2, 8, h, 64, generator=g).bfloat16().to(DEV).transpose(1, 2) for h in (4, 2, 2))
+    parents = torch.tensor([_tree(random.Random(z), 8) for z in range(2)], dtype=torch.int32, device=DEV)
+    path = torch.tensor([[0, 2, 3, 6], [1, 2, 4, 7]], dtype=torch.int32, device=DEV)
+    counts = torch.tensor([4, 2], dtype=torch.int32, device=DEV)
+
+    def step(k, v, n):
+        cache.append(nk, nv, k, v, table, n)
+        out, lse = cache.tree_attention(q, k, v, table, n, parents, max_length=320, window=window, sinks=2 if window else 0, return_lse=True)
+        return out.transpose(1, 2).reshape(2, 8, 256), lse, cache.keep_path(k, v, table, n, path, counts)
+    torch._dynamo.reset()
+    compiled = torch.compile(step, backend='aot_eager', fullgraph=True)
+    ek, ev, en, cn = k.clone(), v.clone(), n, n
+    for _ in range(2):
+        *want, en = step(ek, ev, en)
+        *got, cn = compiled(k, v, cn)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(cn, en)
+        _equal(k, ek)
+        _equal(v, ev)

@@ -310,3 +310,19 @@ def test_host_checks_of_the_ops():
     out, lse = cache.tree_attention(meta(3, 4, 5, 64), meta(9, 2, 16, 64), meta(9, 2, 16, 64), meta(3, 4, dtype=torch.int32),
                                     meta(3, dtype=torch.int32), return_lse=True)
     assert out.shape == (3, 4, 5, 64) and lse.shape == (3, 4, 5)
+
+
+def test_writes_to_a_cache_have_no_gradient():
+    """where autograd would record one they say so, before any kernel"""
+    from aotriton_amd import cache
+    x = lambda grad=False: torch.zeros(3, 2, 16, 64, requires_grad=grad)
+    ints = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    calls = [lambda *t: cache.append(*t, ints(3, 1), ints(3)), lambda k, v, *_: cache.copy_pages(k, v, ints(1), ints(1)),
+             lambda k, v, *_: cache.keep_path(k, v, ints(3, 1), ints(3), ints(3, 1), ints(3)),
+             lambda k, v, *_: cache.fork(k, v, ints(3, 1), ints(3), ints(3), ints(1), ints(1), ints(1))]
+    for call in calls:
+        for i in range(4 if call is calls[0] else 2):
+            with pytest.raises(NotImplementedError, match='no gradient'):
+                call(*(x(j == i) for j in range(4)))
+            with torch.no_grad(), pytest.raises(NotImplementedError, match='CPU'):      # (there is no kernel for this device)
+                call(*(x(j == i) for j in range(4)))
