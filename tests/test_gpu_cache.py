@@ -115,6 +115,22 @@ def test_tiles_of_short_caches(lens, Hq, Hk, tokens, D, page, window, sinks):
     _check(q[pick], k, v, table[pick], n[pick], parents[pick], window, sinks, 1 / math.sqrt(D), out[pick], lse[pick])
 
 
+@pytest.mark.parametrize('lens,times,Hq,Hk,tokens,D,Dv,window,sinks', [
+    ([1000, 63, 0], 1, 8, 2, 64, 256, 256, 0, 0), ([700, 129], 1, 16, 2, 40, 200, 136, 0, 0), ([600, 333], 1, 6, 1, 33, 136, 256, 100, 9),
+    ([900, 5], 40, 8, 8, 64, 256, 256, 0, 0), ([1500, 0, 64], 30, 16, 4, 20, 192, 192, 300, 40), ([130, 1], 1, 32, 1, 2, 64, 160, 0, 0)])
+def test_wide_heads_of_many_rows(lens, times, Hq, Hk, tokens, D, Dv, window, sinks):
+    """head dims above 128: several blocks of 32 packed rows, in one piece and in several, in equal pieces of many sequences"""
+    k, v, table, n = _pool(lens, tokens, Hk, D, 32, torch.bfloat16, seed=50, Dv=Dv)
+    many = list(range(len(lens))) * times
+    rng = random.Random(51)
+    parents = torch.tensor([_tree(rng, tokens, holes=0.1) for _ in many], dtype=torch.int32)
+    q = torch.randn(len(many), tokens, Hq, D, generator=torch.Generator().manual_seed(52)).bfloat16().transpose(1, 2)
+    pick = sorted({0, 1, len(many) - 1})
+    for top in (None, max(lens), 0):
+        out, lse = _run(q, k, v, table[many], n[many], parents, window, sinks, 1 / math.sqrt(D), top)
+        _check(q[pick], k, v, table[many][pick], n[many][pick], parents[pick], window, sinks, 1 / math.sqrt(D), out[pick], lse[pick])
+
+
 def test_many_parts_of_a_long_cache():
     lens = [9000]
     k, v, table, n = _pool(lens, 1, 1, 64, 64, torch.bfloat16, seed=3)
