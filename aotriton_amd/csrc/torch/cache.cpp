@@ -4,7 +4,6 @@
 #include <c10/core/DeviceGuard.h>
 #include <torch/library.h>
 
-#include <limits>
 #include <optional>
 #include <tuple>
 #include <type_traits>
@@ -51,24 +50,13 @@ fa_cache cache_of(const Tensor& k, const Tensor& v, const Tensor& table, const T
   return c;
 }
 
-int32_t number(int64_t x, const char* what) {
-  TORCH_CHECK_VALUE(x >= 0 && x <= std::numeric_limits<int32_t>::max(), what, " must be a number of 31 bits, not ", x);
-  return (int32_t)x;
-}
-
-Tensor aligned(const Tensor& t) {
-  bool ok = t.stride(-1) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
-  for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.size(i) <= 1 || t.stride(i) % 8 == 0;
-  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
-}
-
 std::tuple<Tensor, Tensor> tree_kernel(const Tensor& query, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths,
                                        const std::optional<Tensor>& parents, int64_t max_length, int64_t window, int64_t sinks, double sm_scale) {
   const c10::DeviceGuard guard(k.device());
   fa_tree_params p{};
   p.cache = cache_of(k, v, table, lengths);
   TORCH_CHECK_VALUE(query.dim() == 4, "expected a (sequences, heads, tokens, head_dim) query");
-  const Tensor q = aligned(query);
+  const Tensor q = pieces(query);
   rows4(q, k, &p.Q, "the query");
   const Tensor out = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
   const Tensor lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
@@ -79,9 +67,9 @@ std::tuple<Tensor, Tensor> tree_kernel(const Tensor& query, const Tensor& k, con
     int_rows(*parents, q.size(0), k, &p.parents, "parents");
   }
   p.Sm_scale = (float)sm_scale;
-  p.max_length = number(max_length, "max_length");
-  p.window = number(window, "window");
-  p.sinks = number(sinks, "sinks");
+  p.max_length = as_int32(max_length, "max_length");
+  p.window = as_int32(window, "window");
+  p.sinks = as_int32(sinks, "sinks");
   Scratch scratch;
   check_rc(fa_tree_attn(&p, current_stream(), &scratch.c), false);
   return {out, lse};
@@ -92,7 +80,7 @@ void append_kernel(const Tensor& key, const Tensor& value, const Tensor& k, cons
   const c10::DeviceGuard guard(k.device());
   const fa_cache c = cache_of(k, v, table, lengths);
   TORCH_CHECK_VALUE(key.dim() == 4 && value.dim() == 4, "expected (sequences, heads, tokens, head_dim) rows");
-  const Tensor nk = aligned(key), nv = aligned(value);
+  const Tensor nk = pieces(key), nv = pieces(value);
   fa_tensor4 kv{}, vv{};
   rows4(nk, k, &kv, "the new keys");
   rows4(nv, k, &vv, "the new values");

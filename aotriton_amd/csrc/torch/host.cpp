@@ -470,18 +470,6 @@ const c10::TypedOperatorHandle<SinkBwdSig>& sink_backward_op() {
   return op;
 }
 
-// The kernels move rows in aligned 16-byte pieces; a tensor whose rows are not made of them is copied.
-Tensor pieces(const Tensor& t) {
-  bool ok = t.stride(-1) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
-  for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.size(i) <= 1 || t.stride(i) % 8 == 0;
-  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
-}
-
-int32_t as_int32(int64_t x, const char* what) {
-  TORCH_CHECK_VALUE(x >= 0 && x <= std::numeric_limits<int32_t>::max(), what, " must be a number of 31 bits, not ", x);
-  return (int32_t)x;
-}
-
 Varlen sink_varlen(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& cu_q, const std::optional<Tensor>& cu_k,
                    int64_t max_q, int64_t max_k) {
   TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "expected (batch, heads, seq, head_dim) tensors");

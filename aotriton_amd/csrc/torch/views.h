@@ -6,6 +6,8 @@
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <limits>
+
 #include "aotriton_amd/flash.h"
 
 namespace fa_host {
@@ -66,6 +68,18 @@ inline fa_tensor0 scalar_at(const Tensor& block, int i) {
   v.ptr = static_cast<uint64_t*>(block.data_ptr()) + i;
   v.dtype = FA_DTYPE_UINT64;
   return v;
+}
+
+// The kernels move rows in aligned 16-byte pieces; a tensor whose rows are not made of them is copied.
+inline Tensor pieces(const Tensor& t) {
+  bool ok = t.stride(-1) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
+  for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.size(i) <= 1 || t.stride(i) % 8 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+inline int32_t as_int32(int64_t x, const char* what) {
+  TORCH_CHECK_VALUE(x >= 0 && x <= std::numeric_limits<int32_t>::max(), what, " must be a number of 31 bits, not ", x);
+  return (int32_t)x;
 }
 
 inline void* current_stream() { return c10::hip::getCurrentHIPStream().stream(); }
