@@ -92,6 +92,7 @@ __global__ __launch_bounds__(256) void fork_kernel(const ForkArgs a) {
   if (length < 0) return;      // (a sequence that is not there has no forks)
   const int full = length >> c.page_shift, tail = slot_in_page(c, length), spare = a.spare[i];
   const bool spare_ok = spare >= 0 && spare < c.pages;
+  if (b == 0 && threadIdx.x == 0) a.lengths_out[to] = length;
   if (b >= a.chunks) {
     const int col = (b - a.chunks) * 256 + threadIdx.x;
     if (col >= c.columns) return;
@@ -104,7 +105,6 @@ __global__ __launch_bounds__(256) void fork_kernel(const ForkArgs a) {
     }
     if (page >= 0) atomicAdd(a.uses + page, 1);      // (whole numbers: the order does not matter)
     a.table_out[(int64_t)to * c.table_row + col] = page;
-    if (col == 0) a.lengths_out[to] = length;
     return;
   }
   int page;

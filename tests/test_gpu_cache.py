@@ -508,6 +508,15 @@ def test_a_sequence_that_is_not_there_has_no_fork():
     _equal(dv, v)
 
 
+def test_a_fork_without_columns():
+    from aotriton_amd import cache
+    k, v, _, _ = (t.to(DEV) for t in _pool([40], 0, 2, 64, 16, torch.float16, seed=77))
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    lengths, uses = ints(0, 7, 9), torch.zeros(k.shape[0], dtype=torch.int32, device=DEV)
+    cache.fork(k, v, torch.empty(3, 0, dtype=torch.int32, device=DEV), lengths, uses, ints(1), ints(0), ints(2))
+    assert lengths.tolist() == [7, 7, 9] and (uses == 0).all()
+
+
 @pytest.mark.parametrize('window,sinks', [(0, 0), (90, 4)])
 def test_a_prompt_then_drafted_tokens(window, sinks):
     """The operators together: a prompt goes through attention with sinks into the cache, the sequence is forked, trees are drafted,
