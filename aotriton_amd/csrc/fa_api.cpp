@@ -1380,10 +1380,11 @@ int64_t sink_tiles(const Shape& s, int heads, bool keys, int64_t tokens, int row
 
 // Forward: tiles of 256 rows (of one head or of several, sink_head_shift) or of 128, two workgroups per CU, and the parts that a tile's
 // keys are split into where the tiles do not fill the chip.  Costs: an item, 64 keys of it (`alone` on a CU, or two there); a second
-// launch and the parts' sums.  (us, 256 rows / 128 / 256 split in two / 128 split in two: B1 Hq 32 Hk 8 D128 S32768 window 4096 1897 / 2149,
-// S8192 1024 161 / 168, 256 76 / 69; 256 queries of 4096 keys window 1024 36 / 34 / 34 / 30 (in four 34 / 30), 64 of 8192 window 4096
-// 109 / 107 / 66 / 64 (in four 43 / 40, in eight 34); D64 B4 H16 512 of 4601 window 2048 57 / 46 / 45 / 43, S8192 1024 70 / 64,
-// B2 Hq 16 Hk 4 S1000 window 300 23 / 16.)
+// launch and the parts' sums.  (us, 256 rows / 128 / 256 split in two / 128 split in two, the calls one behind the other in a graph: B1 Hq 32 Hk 8 D128
+// S32768 window 4096 1974 / 2204, S8192 1024 155 / 166, 512 97 / 98, 256 73 / 66; 256 queries of 4096 keys window 1024 36 / 33 / 32 / 29 (in four
+// 32 / 27), 64 of 8192 window 4096 107 / 106 / 65 / 64 (in four 43 / 40, in eight 30); D64 fp16 B4 H16 512 of 4601 window 2048
+// 53 / 43 / 42 / 41, Hq 32 Hk 8 S8192 1024 112 / 108, B2 Hq 16 Hk 4 S1000 window 300 20 / 14.  The sides of a pair were timed in turn on one card;
+// where every call is waited for the card takes up to a quarter longer, on both sides.)
 struct SinkFwdPlan { int half_tiles, splits; int64_t o_bytes, bytes; bool wide; };
 SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, float scale, int32_t window, int32_t sinks, int num_cu) {
   SinkFwdPlan best{0, 1, 0, 0, false};
@@ -1408,7 +1409,7 @@ SinkFwdPlan sink_fwd_plan(const Shape& s, int64_t tokens, float scale, int32_t w
     }
   }
   // 64 rows per wave: more at an item's ends and for masked tiles, less for the others.  (us, 256 rows of 32 per wave -> 64, Hq 32 Hk 8 D128:
-  // S8192 window 512 102 -> 114, 1024 156 -> 162, 2048 271 -> 263, S32768 window 4096 2010 -> 1930; H32 S6000 window 3000 258 -> 260.)
+  // S8192 window 512 97 -> 114, 1024 155 -> 162, 2048 263 -> 256, S32768 window 4096 1974 -> 1881; H32 S6000 window 3000 252 -> 256.)
   if (s.d == 128 && scale > 0.f) {
     const int shift = fa::sink_head_shift(s.hq, s.hk, 4), bm = 256 >> shift;
     const int64_t keys = std::min<int64_t>(s.max_sk, (int64_t)window + bm) + std::min<int64_t>(sinks, 64), tiles = (keys + 63) / 64;
@@ -1443,14 +1444,16 @@ double sink_bwd_time(const Shape& s, bool keys, int64_t tokens, int heads, int g
 }
 
 // Backward: the kernels with 64 rows per wave (head dims above 64)?  (us of the whole backward, neither / dQ / dK and dV / both: bf16 D128
-// Hq 32 Hk 8 S8192 window 256 325 / 277 / 312 / 267, 1024 589 / 521 / 573 / 505, 2048 932 / 847 / 885 / 797; S4099 window 1100 340 / 295 / 414 / 374;
-// B4 Hq 16 Hk 4 S1024 window 256 110 / 99 / 157 / 146; B1 Hq 8 Hk 2 S4096 window 512 121 / 124 / 184 / 189; packed, 4 of up to 8000 tokens, H8,
-// window 1024 359 / 327 / 342 / 310, 16 of up to 6000, Hq 16 Hk 4, 512 874 / 757 / 929 / 804.)
+// Hq 32 Hk 8 S8192 window 256 311 / 258 / 308 / 256, 1024 596 / 516 / 577 / 496, 2048 959 / 862 / 905 / 812; S4099 window 1100 339 / 298 / 414 / 375;
+// B4 Hq 16 Hk 4 S1024 window 256 112 / 97 / 157 / 143; B1 Hq 8 Hk 2 S4096 window 512 121 / 122 / 183 / 185; packed, 4 of up to 8000 tokens, H8,
+// window 1024 350 / 311 / 334 / 293, 16 of up to 6000 (29849 in all), Hq 16 Hk 4, 512 759 / 627 / 749 / 616.)
 struct SinkBwdRoute { bool wide_dq, wide_dkdv; };
 // Up to this window dQ's kernel with 32 rows per wave takes delta from P and dP (SinkBwdArgs::exact_delta): the fewer keys a row has, the more
 // the rounding of its output weighs.  (dQ off from 64 bits by so many times what fp32 arithmetic is, 4 sinks, S3000 D64 fp16: window 16 1.54 -> 1.42,
-// 32 1.49 -> 1.42, 48 1.47, 300 1.45; at D128 1.53 -> 1.42 at 16.  The backward in us: window 32, H16 S8192 D64 85 -> 99, B4 H8 S1000 D128 56 -> 64,
-// Hq 32 Hk 8 S8192 D128, which would take 64 rows per wave, 198 -> 278.)
+// 32 1.49 -> 1.42, 48 1.47, 300 1.45; at D128 1.53 -> 1.42 at 16.  The backward in us: window 32, H16 S8192 D64 83 -> 97, B4 H8 S1000 D128 54 -> 63,
+// Hq 32 Hk 8 S8192 D128, which would take 64 rows per wave, 192 -> 279.)  The line is where the factor without it is 1.48, half way between that of
+// the shortest windows and 1.42: beyond it there is less to be had than the long windows' 1.45 leave.  A call at the line is up to 45 %
+// slower than one behind it, in exchange for that.
 constexpr int32_t kShortWindow = 40;
 SinkBwdRoute sink_bwd_route(const Shape& s, int64_t tokens_q, int64_t tokens_k, int32_t window, int num_cu) {
   if (s.d != 128) return SinkBwdRoute{false, false};

@@ -2,7 +2,7 @@
 //
 // All of it moves bytes: 16 bytes per lane, consecutive lanes along a row.  What bounds the bulk copy is HBM (2048 pages of 64 slots,
 // 8 heads, D128, bf16: 1.07 GB in 218 us, 4.9 TB/s); the others move a few MB and are bound by their launch and two dependent round trips
-// to memory, the page table, then the rows (32 sequences, 24 rows each: append 3.6 us, a path of 6 of them 6.7; 8 forks 3.9, 8 frees of
+// to memory, the page table, then the rows (32 sequences, 24 rows each: append 3.6 us, a path of 6 of them 6.0-6.4; 16 forks 4.0, 16 frees of
 // 63 pages 2.7 us; a caller in Python takes longer to ask for them).
 #include "fa_cache.h"
 #include "fa_kernels.h"
