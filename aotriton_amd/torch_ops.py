@@ -111,7 +111,7 @@ def sink_attention(query, key, value, window, sinks=0, scale=None, cu_seqlens_q=
     before the first key yields zeros and no gradient.
 
     Packed sequences: (1, H, tokens, E) tensors with the sequences' offsets in cu_seqlens_q / cu_seqlens_k (int32 tensors on the device,
-    sequences + 1 values) and their greatest lengths in max_seqlen_q / max_seqlen_k; positions and sinks count from each
+    sequences + 1 values) and their greatest lengths, 1 at least, in max_seqlen_q / max_seqlen_k; positions and sinks count from each
     sequence's start, and tokens behind the last offset belong to no sequence: their rows of the result and of the gradients are 0.
 
     Works under HIP graph capture and torch.compile; results do not change from call to call.  There is no dropout and no bias.

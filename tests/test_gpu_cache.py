@@ -215,6 +215,21 @@ def test_scratch_of_many_sequences():
     assert asked[0] == asked[1] <= 128 << 20
 
 
+@pytest.mark.parametrize('lens,times,tokens,Hq,D,top,window', [
+    ([3000, 500, 0], 1, 1, 8, 64, 700, 0), ([3000, 500, 0], 1, 6, 8, 128, 700, 0), ([2500, 64], 12, 40, 16, 128, 900, 0), ([2500, 64], 20, 24, 8, 64, 600, 0),
+    ([1200, 3], 2, 4, 8, 256, 300, 0), ([1500, 3], 1, 2, 8, 64, 900, 800)])
+def test_sequences_longer_than_planned(lens, times, tokens, Hq, D, top, window):
+    """the last piece of a sequence has what is left of it"""
+    k, v, table, n = _pool(lens, tokens, 2, D, 16, torch.float16, seed=85)
+    many = list(range(len(lens))) * times
+    rng = random.Random(86)
+    parents = torch.tensor([_tree(rng, tokens) for _ in many], dtype=torch.int32)
+    q = torch.randn(len(many), tokens, Hq, D, generator=torch.Generator().manual_seed(87)).half().transpose(1, 2)
+    out, lse = _run(q, k, v, table[many], n[many], parents, window, 3 if window else 0, 1 / math.sqrt(D), top)
+    pick = sorted({0, 1, len(many) - 2, len(many) - 1})
+    _check(q[pick], k, v, table[many][pick], n[many][pick], parents[pick], window, 3 if window else 0, 1 / math.sqrt(D), out[pick], lse[pick])
+
+
 @pytest.mark.parametrize('tokens,Hq', [(1, 2), (20, 8)])
 def test_a_visible_nan_stays(tokens, Hq):
     k, v, table, n = _pool([300, 40], tokens, 2, 64, 16, torch.float16, seed=32)

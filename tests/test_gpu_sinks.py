@@ -201,6 +201,16 @@ def test_nothing_to_do(Sq, Sk):
         assert g.shape == t.shape and (g == 0).all()
 
 
+def test_no_sequence_and_no_token():
+    q, k, v, do = _inputs(0, 4, 2, 30, 40, 64, torch.bfloat16)
+    out, grads = _step(q, k, v, do, 3, 1)
+    assert out.shape == q.shape and [g.shape for g in grads] == [t.shape for t in (q, k, v)]
+    q, k, v, do = _inputs(1, 4, 2, 5, 7, 64, torch.bfloat16)      # tokens that belong to no sequence
+    cu = torch.zeros(3, dtype=torch.int32, device=DEV)
+    out, grads = _step(q, k, v, do, 3, 1, cu_seqlens_q=cu, cu_seqlens_k=cu, max_seqlen_q=1, max_seqlen_k=1)
+    assert all((t == 0).all() for t in (out, *grads))
+
+
 def test_results_do_not_change_and_other_streams():
     q, k, v, do = _inputs(2, 8, 2, 777, 777, 128, torch.bfloat16, seed=10)
     want = _step(q, k, v, do, 100, 4)
