@@ -82,9 +82,9 @@ def copy_pages(k_cache, v_cache, source, target):
 
 def fork(k_cache, v_cache, page_table, lengths, uses, source, target, spare):
     """Makes sequence target[i] a fork of sequence source[i] (int32 vectors): it shares the full pages and gets a copy of the
-    last, partial one in page spare[i], which has to be free (and is not looked at where the last page is full or is not there).  page_table, lengths and
-    uses are updated; what the target's row named before is overwritten, not freed; a source that is not there has no fork.  No target may be named twice or be a source of
-    the same call."""
+    last, partial one in page spare[i], which has to be free (and is not looked at where the last page is full or is not there).
+    page_table, lengths and uses are updated; what the target's row named before is overwritten, not freed; a source that is not
+    there has no fork.  No target may be named twice or be a source of the same call."""
     _ops.cache_fork(k_cache, v_cache, page_table, lengths, uses, source, target, spare)
 
 

@@ -33,8 +33,9 @@ struct TreeArgs {
   int32_t window, sinks;         // window 0: none
   // Work, in blocks of 1 << block_shift slots for row_rows packed rows of a head.  workers > 0: the blocks of all sequences, one after the
   // other, are cut into that many equal pieces of at least `least` blocks, one for a workgroup.  Otherwise every sequence is cut into
-  // pieces of part_blocks blocks, at most `parts`, the last of which has what is left.  The rows' sums over a sequence that lies in several pieces go to part_o (null: none does)
-  // as (head, block of rows, tree_sums' place, row of the block, compiled columns) and, maximum and row sum, to part_ml.
+  // pieces of part_blocks blocks, at most `parts`, the last of which has what is left.  The rows' sums over a sequence that lies in several
+  // pieces go to part_o (null: none does) as (head, block of rows, tree_sums' place, row of the block, compiled columns) and, maximum and
+  // row sum, to part_ml.
   int32_t workers, least, parts, part_blocks, block_shift;
   int32_t row_blocks, row_rows, part_rows;      // part_rows: stored per block of rows
   float* part_o; float* part_ml;

@@ -58,9 +58,9 @@ FA_API int fa_cache_append(const fa_tensor4* k, const fa_tensor4* v, const fa_ca
 FA_API int fa_cache_copy_pages(const fa_tensor4* k_cache, const fa_tensor4* v_cache, const fa_tensor1* source, const fa_tensor1* target, void* hip_stream);
 
 /* Sequence target[i] becomes sequence source[i]: it shares its full pages, whose uses[] go up by one, and gets the rows of the last, partial
- * one in page spare[i] (not looked at where the length is a multiple of the slots or that page is not there), whose count goes up as well; the rest of its
- * table is -1.  A source that is not there (a negative length) has no fork.  The target's table is overwritten, not freed (fa_cache_free).  No target may be named twice or be a source of the
- * same call. */
+ * one in page spare[i] (not looked at where the length is a multiple of the slots or that page is not there), whose count goes up
+ * as well; the rest of its table is -1.  A source that is not there (a negative length) has no fork.  The target's table is overwritten, not
+ * freed (fa_cache_free).  No target may be named twice or be a source of the same call. */
 FA_API int fa_cache_fork(const fa_cache* cache, const fa_tensor1* uses, const fa_tensor1* source, const fa_tensor1* target,
                          const fa_tensor1* spare, void* hip_stream);
 
