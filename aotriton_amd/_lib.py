@@ -101,6 +101,26 @@ class fa_tree_params(ctypes.Structure):
                 ('Sm_scale', ctypes.c_float), ('max_length', ctypes.c_int32), ('window', ctypes.c_int32), ('sinks', ctypes.c_int32)]
 
 
+class fa_reserve_params(ctypes.Structure):
+    _fields_ = [(n, fa_tensor2 if n == 'table' else fa_tensor1) for n in ('table', 'uses', 'lengths', 'counts', 'starts', 'slot_map', 'missing')] + [
+        ('slots', ctypes.c_int32)]
+
+
+class fa_latent_fwd_params(ctypes.Structure):
+    _fields_ = [(n, fa_tensor4) for n in ('Q', 'K', 'V', 'S', 'Out')] + [
+        ('L', fa_tensor2), ('cu_seqlens_q', fa_tensor1), ('cu_seqlens_k', fa_tensor1), ('max_seqlen_q', ctypes.c_int32),
+        ('max_seqlen_k', ctypes.c_int32), ('Sm_scale', ctypes.c_float), ('causal', ctypes.c_int32)]
+
+
+class fa_latent_bwd_params(ctypes.Structure):
+    _fields_ = [('fwd', fa_latent_fwd_params)] + [(n, fa_tensor4) for n in ('DO', 'DQ', 'DK', 'DV', 'DS')]
+
+
+class fa_latent_cache_params(ctypes.Structure):
+    _fields_ = [('Q', fa_tensor4), ('Out', fa_tensor4), ('L', fa_tensor2), ('latent', fa_tensor4), ('table', fa_tensor2),
+                ('lengths', fa_tensor1), ('starts', fa_tensor1), ('Sm_scale', ctypes.c_float), ('max_length', ctypes.c_int32)]
+
+
 # every symbol that include/aotriton_amd/*.h declare: name -> (restype, argtypes)
 P = ctypes.POINTER
 SYMBOLS = {
@@ -122,6 +142,11 @@ SYMBOLS = {
     'fa_cache_fork': (ctypes.c_int, [P(fa_cache)] + [P(fa_tensor1)] * 4 + [ctypes.c_void_p]),
     'fa_cache_keep_path': (ctypes.c_int, [P(fa_cache), P(fa_tensor2), P(fa_tensor1), P(fa_tensor1), ctypes.c_void_p]),
     'fa_cache_free': (ctypes.c_int, [P(fa_tensor2)] + [P(fa_tensor1)] * 4 + [ctypes.c_void_p]),
+    'fa_cache_reserve': (ctypes.c_int, [P(fa_reserve_params), ctypes.c_void_p, ctypes.c_void_p]),
+    'fa_cache_append_packed': (ctypes.c_int, [P(fa_tensor4)] * 4 + [P(fa_tensor1), ctypes.c_void_p]),
+    'fa_latent_fwd': (ctypes.c_int, [P(fa_latent_fwd_params), ctypes.c_void_p, ctypes.c_void_p]),
+    'fa_latent_bwd': (ctypes.c_int, [P(fa_latent_bwd_params), ctypes.c_void_p, ctypes.c_void_p]),
+    'fa_latent_cache_attn': (ctypes.c_int, [P(fa_latent_cache_params), ctypes.c_void_p, ctypes.c_void_p]),
     'fa_v2_attn_fwd': (ctypes.c_int, [P(fa_tensor4)] * 4 + [ctypes.c_float, P(fa_tensor2), P(fa_tensor4), ctypes.c_float,
                                       P(fa_tensor0), P(fa_tensor0), ctypes.c_int64, P(fa_tensor0), P(fa_tensor0),
                                       P(fa_tensor4), ctypes.c_int32, P(fa_tensor0), ctypes.c_void_p]),

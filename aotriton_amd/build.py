@@ -18,8 +18,8 @@ CSRC = os.path.join(HERE, 'csrc')
 ROOT = os.path.dirname(HERE)
 OBJ = os.path.join(CSRC, 'obj')
 LIB = os.path.join(HERE, 'libaotriton_amd.so')
-HOST_SRC = [os.path.join(CSRC, 'torch', f) for f in ('host.cpp', 'cache.cpp')]
-HOST_HEADERS = [os.path.join(CSRC, 'torch', 'views.h')] + [os.path.join(ROOT, 'include', 'aotriton_amd', f) for f in ('flash.h', 'cache.h')]
+HOST_SRC = [os.path.join(CSRC, 'torch', f) for f in ('host.cpp', 'cache.cpp', 'latent.cpp')]
+HOST_HEADERS = [os.path.join(CSRC, 'torch', 'views.h')] + [os.path.join(ROOT, 'include', 'aotriton_amd', f) for f in ('flash.h', 'cache.h', 'latent.h')]
 HOST_LIB = os.path.join(HERE, '_torch_host.so')
 HOST_STAMP = os.path.join(OBJ, '_torch_host.torch')      # the torch version it was built for
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
@@ -51,6 +51,12 @@ EXTRA = {
     'fa_fwd_d256.hip': ['-Wno-inline-asm'],
     'fa_tree_d64.hip': ['-Wno-inline-asm'],
     'fa_tree_d128.hip': ['-Wno-inline-asm'],
+    'fa_latent_d64.hip': ['-Wno-inline-asm'],
+    'fa_latent_d128.hip': ['-Wno-inline-asm'],
+    'fa_latent_cache_d256.hip': ['-Wno-inline-asm'],
+    'fa_latent_cache_d512.hip': ['-Wno-inline-asm'],
+    # (scores in vector registers, results as asm operands in accumulation registers)
+    'fa_latent_cache_full_d512.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', '-Wno-inline-asm'],
     'fa_bwd_dq_d128.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form'],
     # (the same kernels with sinks)
     'fa_sinks_dkdv_d128.hip': ['-mllvm', '-amdgpu-sched-strategy=max-ilp'],

@@ -4,6 +4,7 @@
 
 #include "aotriton_amd/cache.h"
 #include "fa_cache_args.h"
+#include "fa_checks.h"
 #include "fa_kernels.h"
 
 namespace fa {
@@ -35,58 +36,13 @@ hipError_t run_tree(int dtype, const TreeArgs& a, hipStream_t s) {
 
 namespace {
 
-constexpr int64_t kMaxRowStride = 1 << 21;      // elements, as in the other entry points
-constexpr uint64_t kMaxCount = 0x7fffffff;
-
-bool empty(const fa_tensor4& t) { return t.sizes[0] == 0 || t.sizes[1] == 0 || t.sizes[2] == 0; }
-
-// rows of aligned 16-byte pieces, no negative stride
-int check_rows(const fa_tensor4& t, int dtype) {
-  if (t.dtype != dtype || (t.ptr == nullptr && !empty(t))) return FA_ERROR_INVALID_VALUE;
-  for (int i = 0; i < 4; ++i)
-    if (t.sizes[i] > kMaxCount) return FA_ERROR_INVALID_VALUE;
-  if (t.sizes[3] == 0 || t.sizes[3] > 256 || t.sizes[3] % 8 != 0 || (t.strides[3] != 1 && t.sizes[3] > 1)) return FA_ERROR_NOT_SUPPORTED;
-  if ((reinterpret_cast<uintptr_t>(t.ptr) & 15u) != 0) return FA_ERROR_NOT_SUPPORTED;
-  for (int i = 0; i < 3; ++i)
-    if (t.sizes[i] > 1 && ((int64_t)t.strides[i] < 0 || t.strides[i] % 8 != 0)) return FA_ERROR_NOT_SUPPORTED;
-  if (t.sizes[2] > 1 && (int64_t)t.strides[2] > kMaxRowStride) return FA_ERROR_NOT_SUPPORTED;
-  return FA_SUCCESS;
-}
-
-// int32 values next to each other, `n` of them
-int check_ints(const fa_tensor1& t, uint64_t n) {
-  if (t.dtype != FA_DTYPE_INT32 || t.sizes[0] != n || (t.ptr == nullptr && n > 0)) return FA_ERROR_INVALID_VALUE;
-  if (n > 1 && t.strides[0] != 1) return FA_ERROR_NOT_SUPPORTED;
-  return FA_SUCCESS;
-}
-
-// int32 rows with adjacent columns
-int check_int_rows(const fa_tensor2& t, uint64_t rows) {
-  if (t.dtype != FA_DTYPE_INT32 || t.sizes[0] != rows || t.sizes[1] > kMaxCount) return FA_ERROR_INVALID_VALUE;
-  if (t.ptr == nullptr && t.sizes[0] * t.sizes[1] > 0) return FA_ERROR_INVALID_VALUE;
-  if ((t.sizes[1] > 1 && t.strides[1] != 1) || (t.sizes[0] > 1 && (int64_t)t.strides[0] < 0)) return FA_ERROR_NOT_SUPPORTED;
-  return FA_SUCCESS;
-}
-
-// Rows of a tensor that is written have to lie apart.
-bool rows_apart(const fa_tensor2& t) { return t.sizes[0] <= 1 || t.strides[0] >= t.sizes[1]; }
-// (an expanded cache has one row for many)
-bool written_apart(const fa_tensor4& t) {
-  for (int i = 0; i < 3; ++i)
-    if (t.sizes[i] > 1 && t.strides[i] < t.sizes[3]) return false;
-  return true;
-}
-bool written_apart(const fa_cache& c) { return written_apart(c.K) && written_apart(c.V); }
-
-fa::Strides3 strides3(const fa_tensor4& t) {
-  return fa::Strides3{(int64_t)t.strides[0], (int64_t)t.strides[1], (int64_t)t.strides[2]};
-}
+using namespace fa::checks;
 
 // K and V of a cache
-int check_pages(const fa_tensor4& k, const fa_tensor4& v, fa::CacheArgs* out) {
+int check_pages(const fa_tensor4& k, const fa_tensor4& v, fa::CacheArgs* out, uint64_t columns) {
   int e = FA_SUCCESS;
   if (k.dtype != FA_DTYPE_FLOAT16 && k.dtype != FA_DTYPE_BFLOAT16) return FA_ERROR_INVALID_VALUE;
-  if ((e = check_rows(k, k.dtype)) != FA_SUCCESS || (e = check_rows(v, k.dtype)) != FA_SUCCESS) return e;
+  if ((e = check_rows(k, k.dtype, columns)) != FA_SUCCESS || (e = check_rows(v, k.dtype, columns)) != FA_SUCCESS) return e;
   for (int i = 0; i < 3; ++i)
     if (k.sizes[i] != v.sizes[i] || k.sizes[i] == 0) return FA_ERROR_INVALID_VALUE;
   // (kernels multiply with the strides of pages and rows in 32 bits)
@@ -106,9 +62,9 @@ int check_pages(const fa_tensor4& k, const fa_tensor4& v, fa::CacheArgs* out) {
   return FA_SUCCESS;
 }
 
-int check_cache(const fa_cache* p, fa::CacheArgs* out) {
+int check_cache(const fa_cache* p, fa::CacheArgs* out, uint64_t columns = kRowColumns) {
   if (p == nullptr) return FA_ERROR_INVALID_VALUE;
-  int e = check_pages(p->K, p->V, out);
+  int e = check_pages(p->K, p->V, out, columns);
   if (e != FA_SUCCESS) return e;
   fa::CacheArgs& c = *out;
   if (p->lengths.sizes[0] > kMaxCount) return FA_ERROR_INVALID_VALUE;
@@ -123,9 +79,6 @@ int check_cache(const fa_cache* p, fa::CacheArgs* out) {
   c.columns = (int32_t)p->table.sizes[1];
   return FA_SUCCESS;
 }
-
-// a launch's workgroups have to fit 31 bits
-bool fits(double workgroups) { return workgroups < 2147483648.0; }
 
 // Rows per workgroup, how the keys are cut, and the scratch for the sums of sequences that lie in several pieces.
 struct TreePlan { int64_t o_bytes, bytes; };
@@ -182,11 +135,11 @@ extern "C" {
 int fa_tree_attn(const fa_tree_params* p, void* hip_stream, fa_allocator* alloc) {
   if (p == nullptr) return FA_ERROR_INVALID_VALUE;
   fa::TreeArgs a{};
-  int e = check_cache(&p->cache, &a.cache);
+  int e = check_cache(&p->cache, &a.cache, kTreeColumns);
   if (e != FA_SUCCESS) return e;
   const fa::CacheArgs& c = a.cache;
   const int dtype = p->cache.K.dtype;
-  if ((e = check_rows(p->Q, dtype)) != FA_SUCCESS || (e = check_rows(p->Out, dtype)) != FA_SUCCESS) return e;
+  if ((e = check_rows(p->Q, dtype, kTreeColumns)) != FA_SUCCESS || (e = check_rows(p->Out, dtype, kTreeColumns)) != FA_SUCCESS) return e;
   const uint64_t tokens = p->Q.sizes[2], hq = p->Q.sizes[1];
   if (p->Q.sizes[0] != (uint64_t)c.sequences || p->Q.sizes[3] != (uint64_t)c.head_dim || hq == 0 || hq % (uint64_t)c.heads != 0) return FA_ERROR_INVALID_VALUE;
   for (int i = 0; i < 3; ++i)
@@ -238,7 +191,7 @@ int fa_cache_append(const fa_tensor4* k, const fa_tensor4* v, const fa_cache* ca
   if (e != FA_SUCCESS) return e;
   if (!written_apart(*cache)) return FA_ERROR_NOT_SUPPORTED;
   const fa::CacheArgs& c = a.cache;
-  if ((e = check_rows(*k, cache->K.dtype)) != FA_SUCCESS || (e = check_rows(*v, cache->K.dtype)) != FA_SUCCESS) return e;
+  if ((e = check_rows(*k, cache->K.dtype, kRowColumns)) != FA_SUCCESS || (e = check_rows(*v, cache->K.dtype, kRowColumns)) != FA_SUCCESS) return e;
   for (const fa_tensor4* t : {k, v})
     if (t->sizes[0] != (uint64_t)c.sequences || t->sizes[1] != (uint64_t)c.heads || t->sizes[2] != k->sizes[2]) return FA_ERROR_INVALID_VALUE;
   if (k->sizes[3] != (uint64_t)c.head_dim || v->sizes[3] != (uint64_t)c.head_dim_v) return FA_ERROR_INVALID_VALUE;
@@ -258,7 +211,7 @@ int fa_cache_append(const fa_tensor4* k, const fa_tensor4* v, const fa_cache* ca
 int fa_cache_copy_pages(const fa_tensor4* k_cache, const fa_tensor4* v_cache, const fa_tensor1* source, const fa_tensor1* target, void* hip_stream) {
   if (k_cache == nullptr || v_cache == nullptr || source == nullptr || target == nullptr) return FA_ERROR_INVALID_VALUE;
   fa::CopyArgs a{};
-  int e = check_pages(*k_cache, *v_cache, &a.cache);
+  int e = check_pages(*k_cache, *v_cache, &a.cache, kRowColumns);
   if (e != FA_SUCCESS) return e;
   if (!written_apart(*k_cache) || !written_apart(*v_cache)) return FA_ERROR_NOT_SUPPORTED;
   const uint64_t n = source->sizes[0];
@@ -348,6 +301,76 @@ int fa_cache_free(const fa_tensor2* table, const fa_tensor1* uses, const fa_tens
   if (!fits((double)n * (a.columns / 256 + 1))) return FA_ERROR_NOT_SUPPORTED;
   if ((e = fa_check_gpu(hip_stream)) != FA_SUCCESS) return e;
   return (int)fa::run_cache_free(a, (int)n, static_cast<hipStream_t>(hip_stream));
+}
+
+int fa_cache_append_packed(const fa_tensor4* k, const fa_tensor4* v, const fa_tensor4* k_cache, const fa_tensor4* v_cache, const fa_tensor1* slot_map, void* hip_stream) {
+  if (k == nullptr || k_cache == nullptr || slot_map == nullptr || (v == nullptr) != (v_cache == nullptr)) return FA_ERROR_INVALID_VALUE;
+  fa::PackedAppendArgs a{};
+  int e = check_pages(*k_cache, v_cache != nullptr ? *v_cache : *k_cache, &a.cache, kRowColumns);
+  if (e != FA_SUCCESS) return e;
+  if (!written_apart(*k_cache) || (v_cache != nullptr && !written_apart(*v_cache))) return FA_ERROR_NOT_SUPPORTED;
+  const fa_tensor4* rows[2] = {k, v};
+  const fa_tensor4* caches[2] = {k_cache, v_cache};
+  for (int i = 0; i < (v != nullptr ? 2 : 1); ++i) {
+    const fa_tensor4 &t = *rows[i], &c = *caches[i];
+    if ((e = check_rows(t, c.dtype, kRowColumns)) != FA_SUCCESS) return e;
+    if (t.sizes[0] != 1 || t.sizes[1] != k->sizes[1] || t.sizes[2] != c.sizes[1] || t.sizes[3] != c.sizes[3]) return FA_ERROR_INVALID_VALUE;
+  }
+  const fa_tensor1& m = *slot_map;
+  if (m.dtype != FA_DTYPE_INT64 || m.sizes[0] != k->sizes[1] || (m.ptr == nullptr && m.sizes[0] > 0)) return FA_ERROR_INVALID_VALUE;
+  if (m.sizes[0] > 1 && m.strides[0] != 1) return FA_ERROR_NOT_SUPPORTED;
+  if (v == nullptr) a.cache.head_dim_v = 0;
+  a.new_k = k->ptr;
+  a.snk = fa::Strides3{(int64_t)k->strides[1], (int64_t)k->strides[2], 0};
+  if (v != nullptr) {
+    a.new_v = v->ptr;
+    a.snv = fa::Strides3{(int64_t)v->strides[1], (int64_t)v->strides[2], 0};
+  }
+  a.slots = static_cast<const int64_t*>(m.ptr);
+  a.tokens = (int32_t)k->sizes[1];
+  // (pieces are counted in 32 bits, those of the last workgroup past the end as well)
+  if (!fits((double)a.tokens * a.cache.heads * ((a.cache.head_dim + a.cache.head_dim_v) / 8) + 256)) return FA_ERROR_NOT_SUPPORTED;
+  if ((e = fa_check_gpu(hip_stream)) != FA_SUCCESS) return e;
+  return (int)fa::run_cache_append_packed(a, static_cast<hipStream_t>(hip_stream));
+}
+
+int fa_cache_reserve(const fa_reserve_params* p, void* hip_stream, fa_allocator* alloc) {
+  if (p == nullptr || alloc == nullptr) return FA_ERROR_INVALID_VALUE;
+  fa::ReserveArgs a{};
+  const uint64_t n = p->lengths.sizes[0], pages = p->uses.sizes[0], tokens = p->slot_map.sizes[0];
+  if (n >= kMaxCount || pages > kMaxCount || tokens > kMaxCount) return FA_ERROR_INVALID_VALUE;
+  int e = check_int_rows(p->table, n);
+  if (e != FA_SUCCESS) return e;
+  if (!rows_apart(p->table)) return FA_ERROR_NOT_SUPPORTED;
+  if ((e = check_ints(p->uses, pages)) != FA_SUCCESS || (e = check_ints(p->lengths, n)) != FA_SUCCESS || (e = check_ints(p->counts, n)) != FA_SUCCESS ||
+      (e = check_ints(p->starts, n + 1)) != FA_SUCCESS || (e = check_ints(p->missing, 1)) != FA_SUCCESS) return e;
+  if (p->slot_map.dtype != FA_DTYPE_INT64 || (p->slot_map.ptr == nullptr && tokens > 0)) return FA_ERROR_INVALID_VALUE;
+  if (tokens > 1 && p->slot_map.strides[0] != 1) return FA_ERROR_NOT_SUPPORTED;
+  if (p->slots < 16 || p->slots > (1 << 20) || (p->slots & (p->slots - 1)) != 0) return FA_ERROR_NOT_SUPPORTED;
+  a.table = static_cast<int32_t*>(p->table.ptr);
+  a.table_row = (int64_t)p->table.strides[0];
+  a.uses = static_cast<int32_t*>(p->uses.ptr);
+  a.lengths = static_cast<const int32_t*>(p->lengths.ptr);
+  a.counts = static_cast<const int32_t*>(p->counts.ptr);
+  a.sequences = (int32_t)n;
+  a.columns = (int32_t)p->table.sizes[1];
+  a.pages = (int32_t)pages;
+  a.page_shift = __builtin_ctz((unsigned)p->slots);
+  a.tokens = (int32_t)tokens;
+  a.starts = static_cast<int32_t*>(p->starts.ptr);
+  a.slots = static_cast<int64_t*>(p->slot_map.ptr);
+  a.missing = static_cast<int32_t*>(p->missing.ptr);
+  a.words = (int32_t)((pages + 63) / 64);
+  for (a.run_shift = 4; (a.words + (1 << a.run_shift) - 1) >> a.run_shift > fa::kReserveRuns;) ++a.run_shift;
+  a.runs = (a.words + (1 << a.run_shift) - 1) >> a.run_shift;
+  if (!fits((double)n + a.runs + 1)) return FA_ERROR_NOT_SUPPORTED;
+  if ((e = fa_check_gpu(hip_stream)) != FA_SUCCESS) return e;
+  void* scratch = alloc->alloc(alloc, (uint64_t)a.words * 8 + ((uint64_t)a.runs + n + 2) * 4);
+  if (scratch == nullptr) return FA_ERROR_OUT_OF_MEMORY;
+  a.free_bits = static_cast<uint64_t*>(scratch);
+  a.run_free = reinterpret_cast<int32_t*>(a.free_bits + a.words);
+  a.wanted = a.run_free + a.runs;
+  return (int)fa::run_cache_reserve(a, static_cast<hipStream_t>(hip_stream));
 }
 
 }  // extern "C"

@@ -80,6 +80,29 @@ struct FreeArgs {
   int32_t chunks;                            // workgroups per sequence (launcher)
 };
 
+struct PackedAppendArgs {
+  CacheArgs cache;                           // (without a table; head_dim_v 0: there is no V)
+  const void* new_k; const void* new_v;      // (tokens, heads, columns): z of the strides is the token's
+  Strides3 snk, snv;
+  const int64_t* slots;                      // page times slots of a page, plus the slot in it
+  int32_t tokens;
+};
+
+struct ReserveArgs {
+  int32_t* table; int64_t table_row;
+  int32_t* uses;
+  const int32_t* lengths; const int32_t* counts;
+  int32_t sequences, columns, pages, page_shift, tokens;
+  int32_t* starts;               // (sequences + 1)
+  int64_t* slots;                // (tokens)
+  int32_t* missing;
+  // Scratch: a bit for every page, 64 to a word, set where the page is free; the free pages of each run of 1 << run_shift words; the pages
+  // that each sequence asks for.
+  uint64_t* free_bits; int32_t* run_free; int32_t* wanted;
+  int32_t words, run_shift, runs;
+};
+constexpr int kReserveRuns = 2048;           // at most
+
 // dtype: kDtypeF16 or kDtypeBF16; the others move 16-bit columns whatever they stand for.  Scratch of TreeArgs is the caller's.
 hipError_t run_tree(int dtype, const TreeArgs& a, hipStream_t s);
 hipError_t run_cache_append(const AppendArgs& a, hipStream_t s);
@@ -87,5 +110,7 @@ hipError_t run_cache_copy(const CopyArgs& a, int count, hipStream_t s);
 hipError_t run_cache_fork(const ForkArgs& a, int count, hipStream_t s);
 hipError_t run_cache_keep(const KeepArgs& a, hipStream_t s);
 hipError_t run_cache_free(const FreeArgs& a, int count, hipStream_t s);
+hipError_t run_cache_append_packed(const PackedAppendArgs& a, hipStream_t s);
+hipError_t run_cache_reserve(const ReserveArgs& a, hipStream_t s);
 
 }  // namespace fa

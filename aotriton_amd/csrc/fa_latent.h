@@ -1,0 +1,490 @@
+// Attention whose keys are part per head, part shared by all heads, forward and backward: gfx950, MFMA 32x32x16.
+//
+//   S = scale (Qe K^T + Qr C^T),  P = softmax(S),  O = P V
+//   dV = P^T dO,  dS = P (dO V^T - rowsum(dO O)),  dQ = scale [dS K | dS C],  dK = scale dS^T Qe,  dC = scale sum over heads of dS^T Qr
+//
+// The shared part is never copied per head: its tile stands next to that of K in LDS, and a key is the two of them.  K and V (64 or 128
+// compiled columns) and C (64) may have fewer columns each; what is past them reads as zero.
+//
+// Layouts and products as in fa_fwd_impl.h: a wave owns 32 rows (dK/dV: keys), a lane one of them; tiles come straight into swizzled LDS
+// (fa_device.h: Swz), the next one while this one is worked on, and serve row reads and transposing reads alike.
+#pragma once
+#include "fa_device.h"
+#include "fa_latent_args.h"
+#include "fa_latent_parts.h"
+#include "fa_wide.h"
+
+namespace fa {
+
+constexpr int kLatentShared = 64;      // compiled columns of the shared part
+
+// A tile's 64 rows as they come into LDS: 16 rows a wave, 1 KB an access.  A lane's byte offsets of its accesses; the columns start at
+// `col0` of the row, and there are `cols` of them.
+template <int D> struct TileRows {
+  static constexpr int LPR = D / 8, RPL = 64 / LPR, N = 16 / RPL;      // lanes of a row, rows of an access, accesses
+  int voff[N];
+  __device__ __forceinline__ TileRows(int lane, int row_bytes, int col0, int cols) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int row = i * RPL + lane / LPR, ch = (lane % LPR) ^ Swz<D>::f(row);
+      voff[i] = ch * 8 < cols ? row * row_bytes + (col0 + ch * 8) * 2 : kVoffOutOfRange;
+    }
+  }
+  __device__ __forceinline__ void fetch(u32x4_t rsrc, int lds) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) load_to_lds1(rsrc, voff[i], lds + i * 1024);
+  }
+};
+
+// Rows of a wave as MFMA operands in registers, row lane % 32: columns [col0, col0 + cols) of the first `rows` rows, zeros elsewhere.
+template <typename T, int N>
+__device__ __forceinline__ void load_operands(typename Traits<T>::op_t* x, const void* base, int row_bytes, int rows, int lane, int col0, int cols) {
+  using op_t = typename Traits<T>::op_t;
+  const auto rs = wave_rsrc(base, rows_extent(rows, row_bytes, (col0 + cols) * 2));
+  const int c = lane & 31, hi = lane >> 5;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int col = 16 * k + 8 * hi;
+    x[k] = __builtin_bit_cast(op_t, __builtin_amdgcn_raw_buffer_load_b128(rs, col < cols && c < rows ? c * row_bytes + (col0 + col) * 2 : kVoffOutOfRange, 0, 0));
+  }
+}
+
+// A transposed accumulator (columns x 32 rows) times `f` to row lane % 32 of a tensor, columns [0, cols).
+template <typename T, int NB>
+__device__ __forceinline__ void store_rows(const f32x16* x, float f, T* row, int cols, int hi) {
+  using q4_t = typename Traits<T>::q4_t;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * b + 8 * g + 4 * hi;
+      q4_t y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(x[b][4 * g + r] * f);
+      if (col < cols) *reinterpret_cast<q4_t*>(row + col) = y;
+    }
+}
+
+__device__ __forceinline__ void latent_meet() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int EC> struct LatentSmem {
+  static constexpr int TILE = 64 * EC * 2, SHARED = 64 * kLatentShared * 2;
+  static constexpr int C_OFF = TILE, V_OFF = TILE + SHARED;
+  static constexpr int STAGE = 2 * TILE + SHARED;      // K, C, V (dK/dV: Q, its shared part, dO)
+  static constexpr int STATS = 2 * 64 * 4;
+  static constexpr int BYTES = 2 * STAGE, BWD_BYTES = 2 * (STAGE + STATS);
+};
+
+// (the offsets of packed sequences are held inside the tensors, and lengths inside the greatest: what lies past them is not there)
+__device__ __forceinline__ SeqInfo latent_seq(const LatentArgs& a, int z) {
+  SeqInfo r{a.seq.max_seqlen_q, a.seq.max_seqlen_k, 0, 0, z, a.rows_q};
+  if (a.seq.num_seqlens != 0) {
+    auto hold = [](int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; };
+    r.q_start = hold(a.seq.cu_q[z], 0, a.rows_q);
+    r.k_start = hold(a.seq.cu_k[z], 0, a.rows_k);
+    r.seqlen_q = hold(hold(a.seq.cu_q[z + 1], 0, a.rows_q) - r.q_start, 0, a.seq.max_seqlen_q);
+    r.seqlen_k = hold(hold(a.seq.cu_k[z + 1], 0, a.rows_k) - r.k_start, 0, a.seq.max_seqlen_k);
+    r.batch_index = 0;
+  }
+  return uniform(r);
+}
+
+// (sequence, head, tile) of a workgroup: the tiles of a kind one behind the other, the heads of all sequences side by side, so that an
+// XCD keeps its heads where their number is a multiple of 8.  Causal tiles have the more keys the later they stand: those first.
+__device__ __forceinline__ void latent_item(const LatentArgs& a, int id, int nseq, int tiles, bool backwards, int& z, int& h, int& t) {
+  const int pairs = nseq * a.heads, zh = id % pairs;
+  t = id / pairs;
+  if (backwards) t = tiles - 1 - t;
+  h = zh % a.heads;
+  z = zh / a.heads;
+}
+
+template <typename T> __device__ __forceinline__ T* row_at(const void* base, const Strides3& s, const SeqInfo& si, int h, int64_t row) {
+  return const_cast<T*>(reinterpret_cast<const T*>(base)) + (int64_t)si.batch_index * s.z + (int64_t)h * s.h + row * s.s;
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------
+template <typename T, int EC>
+__global__ __launch_bounds__(256, 2) void latent_fwd_kernel(const LatentArgs a, int nseq, int tiles) {
+  using Tr = Traits<T>;
+  using op_t = typename Tr::op_t;
+  using SM = LatentSmem<EC>;
+  constexpr int KE = EC / 16, KR = kLatentShared / 16, DB = EC / 32;
+  extern __shared__ __attribute__((aligned(kSwzAlign))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int z, h, mt;
+  const int part = blockIdx.x / (nseq * a.heads) % a.parts;
+  latent_item(a, blockIdx.x % (nseq * a.heads) + blockIdx.x / (nseq * a.heads * a.parts) * (nseq * a.heads), nseq, tiles, a.causal != 0, z, h, mt);
+  const SeqInfo si = latent_seq(a, z);
+  const int q0 = mt * 128;
+  if (q0 >= si.seqlen_q) return;
+  const int shift = si.seqlen_k - si.seqlen_q;
+  const int w0 = q0 + wave * 32, row = w0 + c, rows = si.seqlen_q - w0;
+  // key tiles of the workgroup, of the part, of the wave
+  auto last_key = [&](int r) { return a.causal ? (r < si.seqlen_q ? r : si.seqlen_q - 1) + shift : si.seqlen_k - 1; };
+  auto tiles_of = [&](int r) { const int n = last_key(r) + 1; return n > 0 ? (n + 63) / 64 : 0; };
+  const int all = tiles_of(q0 + 127), per = (all + a.parts - 1) / a.parts;
+  const int j0 = part * per, j1 = j0 + per < all ? j0 + per : all, wave_end = tiles_of(w0 + 31);
+  const int see = last_key(row);
+
+  const int smem0 = lds_offset(smem);
+  const int k_row = (int)a.sk.s * 2, v_row = (int)a.sv.s * 2, c_row = (int)a.c_s * 2;
+  const TileRows<EC> kt(lane, k_row, 0, a.e), vt(lane, v_row, 0, a.ev);
+  const TileRows<kLatentShared> ct(lane, c_row, 0, a.r);
+  auto fetch = [&](int stage, int j) __attribute__((always_inline)) {
+    const int n = j * 64 + wave * 16, left = si.seqlen_k - n < 16 ? si.seqlen_k - n : 16;
+    const int64_t at = si.k_start + n;
+    const int lds = smem0 + stage * SM::STAGE + wave * 16 * 2 * EC;
+    kt.fetch(wave_rsrc_words(row_at<T>(a.k, a.sk, si, h, at), rows_extent(left, k_row, a.e * 2)), lds);
+    vt.fetch(wave_rsrc_words(row_at<T>(a.v, a.sv, si, h, at), rows_extent(left, v_row, a.ev * 2)), lds + SM::V_OFF);
+    ct.fetch(wave_rsrc_words(row_at<T>(a.c, Strides3{a.c_z, 0, a.c_s}, si, 0, at), rows_extent(left, c_row, a.r * 2)),
+             smem0 + stage * SM::STAGE + SM::C_OFF + wave * 16 * 2 * kLatentShared);
+  };
+  if (j0 < j1) fetch(0, j0);
+
+  op_t q[KE + KR];
+  {
+    const T* qp = row_at<T>(a.q, a.sq, si, h, (int64_t)si.q_start + w0);
+    load_operands<T, KE>(q, qp, (int)a.sq.s * 2, rows, lane, 0, a.e);
+    load_operands<T, KR>(q + KE, qp, (int)a.sq.s * 2, rows, lane, a.e, a.r);
+  }
+  f32x16 o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+  RowSoftmax sm(a.sm_scale);
+  const int row_e = Swz<EC>::row_base(lane), row_r = Swz<kLatentShared>::row_base(lane);
+  const int tr0 = Swz<EC>::tr_base(lane, 0), tr1 = Swz<EC>::tr_base(lane, 1);
+
+  for (int j = j0; j < j1; ++j) {
+    latent_meet();
+    const int stage = (j - j0) & 1;
+    if (j + 1 < j1) fetch(stage ^ 1, j + 1);
+    if (j >= wave_end) continue;
+    const char* K = smem + stage * SM::STAGE;
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KE; ++k) s[b] = Tr::mfma(swz_read_row<T, EC>(K, row_e, k, b), q[k], s[b]);
+#pragma unroll
+      for (int k = 0; k < KR; ++k) s[b] = Tr::mfma(swz_read_row<T, kLatentShared>(K + SM::C_OFF, row_r, k, b), q[KE + k], s[b]);
+    }
+    const int n0 = j * 64;
+    const bool masked = n0 + 64 > si.seqlen_k || (a.causal && n0 + 63 > w0 + shift);
+    sm.step(s, masked, see - n0 - 4 * hi, [&](float f) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] *= f;
+    });
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const op_t p = pack8<T>(s[t / 2], t % 2);
+#pragma unroll
+      for (int b = 0; b < DB; ++b) o[b] = Tr::mfma(swz_read_tr<T, EC>(K + SM::V_OFF, tr0, tr1, t, b), p, o[b]);
+    }
+  }
+  if (a.parts > 1) {
+    store_part<DB>(a.part_o, a.part_ml, (((int64_t)(z * a.heads + h) * tiles + mt) * 4 + wave) * a.parts + part, o, sm, lane);
+    return;
+  }
+  if (row >= si.seqlen_q) return;
+  const float l = cross_sum(sm.l);
+  store_rows<T, DB>(o, l == 0.f ? 0.f : 1.0f / l, row_at<T>(a.out, a.so, si, h, (int64_t)si.q_start + row), a.ev, hi);
+  if (a.lse != nullptr && hi == 0) a.lse[lse_offset(si, h, a.heads) + row] = sm.lse(l);
+}
+
+// the parts' sums of 32 rows and 32 columns put together
+template <typename T, int EC>
+__global__ __launch_bounds__(256) void latent_fwd_sum_kernel(const LatentArgs a, int nseq, int tiles) {
+  constexpr int DB = EC / 32;
+  const int db = blockIdx.x % DB, slab = blockIdx.x / DB, wave = slab % 4, mt = slab / 4 % tiles, zh = slab / 4 / tiles;
+  const int h = zh % a.heads, z = zh / a.heads;
+  const SeqInfo si = latent_seq(a, z);
+  const int lane = threadIdx.x & 63, hi = lane >> 5, row = mt * 128 + wave * 32 + (lane & 31);
+  if (row >= si.seqlen_q) return;
+  float lse;
+  const vec<float, 4> x = sum_parts<DB>(a.part_o, a.part_ml, (int64_t)slab * a.parts, a.parts, a.sm_scale, db, threadIdx.x, lse);
+  const int col = 32 * db + 8 * (threadIdx.x >> 6) + 4 * hi;
+  typename Traits<T>::q4_t y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(x[r]);
+  if (col < a.ev) *reinterpret_cast<typename Traits<T>::q4_t*>(row_at<T>(a.out, a.so, si, h, (int64_t)si.q_start + row) + col) = y;
+  if (a.lse != nullptr && db == 0 && threadIdx.x < 32) a.lse[lse_offset(si, h, a.heads) + row] = lse;
+}
+
+// ---- dQ ------------------------------------------------------------------------------------------------------------
+// Rows as in the forward; also delta, which needs the rows of O and dO that are here anyway.
+template <typename T, int EC>
+__global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a, int nseq, int tiles) {
+  using Tr = Traits<T>;
+  using op_t = typename Tr::op_t;
+  using SM = LatentSmem<EC>;
+  constexpr int KE = EC / 16, KR = kLatentShared / 16, DB = EC / 32, RB = kLatentShared / 32;
+  extern __shared__ __attribute__((aligned(kSwzAlign))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int z, h, mt;
+  latent_item(a, blockIdx.x, nseq, tiles, a.causal != 0, z, h, mt);
+  const SeqInfo si = latent_seq(a, z);
+  const int q0 = mt * 128;
+  if (q0 >= si.seqlen_q) return;
+  const int shift = si.seqlen_k - si.seqlen_q;
+  const int w0 = q0 + wave * 32, row = w0 + c, rows = si.seqlen_q - w0;
+  auto last_key = [&](int r) { return a.causal ? (r < si.seqlen_q ? r : si.seqlen_q - 1) + shift : si.seqlen_k - 1; };
+  auto tiles_of = [&](int r) { const int n = last_key(r) + 1; return n > 0 ? (n + 63) / 64 : 0; };
+  const int j1 = tiles_of(q0 + 127), wave_end = tiles_of(w0 + 31), see = last_key(row);
+
+  const int smem0 = lds_offset(smem);
+  const int k_row = (int)a.sk.s * 2, v_row = (int)a.sv.s * 2, c_row = (int)a.c_s * 2;
+  const TileRows<EC> kt(lane, k_row, 0, a.e), vt(lane, v_row, 0, a.ev);
+  const TileRows<kLatentShared> ct(lane, c_row, 0, a.r);
+  auto fetch = [&](int stage, int j) __attribute__((always_inline)) {
+    const int n = j * 64 + wave * 16, left = si.seqlen_k - n < 16 ? si.seqlen_k - n : 16;
+    const int64_t at = si.k_start + n;
+    const int lds = smem0 + stage * SM::STAGE + wave * 16 * 2 * EC;
+    kt.fetch(wave_rsrc_words(row_at<T>(a.k, a.sk, si, h, at), rows_extent(left, k_row, a.e * 2)), lds);
+    vt.fetch(wave_rsrc_words(row_at<T>(a.v, a.sv, si, h, at), rows_extent(left, v_row, a.ev * 2)), lds + SM::V_OFF);
+    ct.fetch(wave_rsrc_words(row_at<T>(a.c, Strides3{a.c_z, 0, a.c_s}, si, 0, at), rows_extent(left, c_row, a.r * 2)),
+             smem0 + stage * SM::STAGE + SM::C_OFF + wave * 16 * 2 * kLatentShared);
+  };
+  if (j1 > 0) fetch(0, 0);
+
+  op_t q[KE + KR], dout[KE];
+  {
+    const T* qp = row_at<T>(a.q, a.sq, si, h, (int64_t)si.q_start + w0);
+    load_operands<T, KE>(q, qp, (int)a.sq.s * 2, rows, lane, 0, a.e);
+    load_operands<T, KR>(q + KE, qp, (int)a.sq.s * 2, rows, lane, a.e, a.r);
+    load_operands<T, KE>(dout, row_at<T>(a.dout, a.sdo, si, h, (int64_t)si.q_start + w0), (int)a.sdo.s * 2, rows, lane, 0, a.ev);
+  }
+  float delta = 0.f, lse = __builtin_inff();
+  {
+    op_t out[KE];
+    load_operands<T, KE>(out, row_at<T>(a.out, a.so, si, h, (int64_t)si.q_start + w0), (int)a.so.s * 2, rows, lane, 0, a.ev);
+#pragma unroll
+    for (int k = 0; k < KE; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta += (float)out[k][i] * (float)dout[k][i];
+    delta = cross_sum(delta);
+    if (row < si.seqlen_q) {
+      const int64_t at = lse_offset(si, h, a.heads) + row;
+      lse = a.lse[at] * kLog2e;
+      if (hi == 0) { a.stat_lse[at] = lse; a.stat_delta[at] = delta; }
+    }
+  }
+  f32x16 dq[DB + RB];
+#pragma unroll
+  for (int b = 0; b < DB + RB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dq[b][i] = 0.f;
+  const float qs = a.sm_scale * kLog2e;
+  const int row_e = Swz<EC>::row_base(lane), row_r = Swz<kLatentShared>::row_base(lane);
+  const int tr0 = Swz<EC>::tr_base(lane, 0), tr1 = Swz<EC>::tr_base(lane, 1);
+  const int rr0 = Swz<kLatentShared>::tr_base(lane, 0), rr1 = Swz<kLatentShared>::tr_base(lane, 1);
+
+  for (int j = 0; j < j1; ++j) {
+    latent_meet();
+    const int stage = j & 1;
+    if (j + 1 < j1) fetch(stage ^ 1, j + 1);
+    if (j >= wave_end) continue;
+    const char* K = smem + stage * SM::STAGE;
+    const int n0 = j * 64;
+    const bool masked = n0 + 64 > si.seqlen_k || (a.causal && n0 + 63 > w0 + shift);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16 s, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KE; ++k) s = Tr::mfma(swz_read_row<T, EC>(K, row_e, k, b), q[k], s);
+#pragma unroll
+      for (int k = 0; k < KR; ++k) s = Tr::mfma(swz_read_row<T, kLatentShared>(K + SM::C_OFF, row_r, k, b), q[KE + k], s);
+#pragma unroll
+      for (int k = 0; k < KE; ++k) dp = Tr::mfma(swz_read_row<T, EC>(K + SM::V_OFF, row_e, k, b), dout[k], dp);
+      const int limit = see - n0 - 32 * b - 4 * hi;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float p = fast_exp2(__builtin_fmaf(s[i], qs, -lse));
+        if (masked && 8 * (i / 4) + i % 4 > limit) p = 0.f;
+        s[i] = p * (dp[i] - delta);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const op_t ds = pack8<T>(s, t);
+#pragma unroll
+        for (int x = 0; x < DB; ++x) dq[x] = Tr::mfma(swz_read_tr<T, EC>(K, tr0, tr1, 2 * b + t, x), ds, dq[x]);
+#pragma unroll
+        for (int x = 0; x < RB; ++x) dq[DB + x] = Tr::mfma(swz_read_tr<T, kLatentShared>(K + SM::C_OFF, rr0, rr1, 2 * b + t, x), ds, dq[DB + x]);
+      }
+    }
+  }
+  if (row >= si.seqlen_q) return;
+  T* to = row_at<T>(a.dq, a.sdq, si, h, (int64_t)si.q_start + row);
+  store_rows<T, DB>(dq, a.sm_scale, to, a.e, hi);
+  store_rows<T, RB>(dq + DB, a.sm_scale, to + a.e, a.r, hi);
+}
+
+// ---- dK, dV and every head's part of dC -----------------------------------------------------------------------------
+// A wave owns 32 keys, a lane one of them, with K, C and V as operands in registers; tiles of 64 queries pass.
+template <typename T, int EC>
+__global__ __launch_bounds__(256, EC == 64 ? 2 : 1) void latent_dkdv_kernel(const LatentBwdArgs a, int nseq, int tiles) {
+  using Tr = Traits<T>;
+  using op_t = typename Tr::op_t;
+  using SM = LatentSmem<EC>;
+  constexpr int KE = EC / 16, KR = kLatentShared / 16, DB = EC / 32, RB = kLatentShared / 32;
+  extern __shared__ __attribute__((aligned(kSwzAlign))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int z, h, nt;
+  latent_item(a, blockIdx.x, nseq, tiles, false, z, h, nt);
+  const SeqInfo si = latent_seq(a, z);
+  if (nt * 128 >= si.seqlen_k) return;
+  const int shift = si.seqlen_k - si.seqlen_q;
+  const int w0 = nt * 128 + wave * 32, key = w0 + c, keys = si.seqlen_k - w0;
+  // the first query that sees a key
+  auto first_query = [&](int n) { return a.causal && n - shift > 0 ? n - shift : 0; };
+  const int j0 = first_query(nt * 128) / 64, j1 = (si.seqlen_q + 63) / 64;
+
+  const int smem0 = lds_offset(smem);
+  const int q_row = (int)a.sq.s * 2, do_row = (int)a.sdo.s * 2;
+  const TileRows<EC> qt(lane, q_row, 0, a.e), dt(lane, do_row, 0, a.ev);
+  const TileRows<kLatentShared> rt(lane, q_row, a.e, a.r);
+  const float* stats = (wave & 1 ? a.stat_delta : a.stat_lse) + lse_offset(si, h, a.heads);
+  auto fetch = [&](int stage, int j) __attribute__((always_inline)) {
+    const int m = j * 64 + wave * 16, left = si.seqlen_q - m < 16 ? si.seqlen_q - m : 16;
+    const int64_t at = si.q_start + m;
+    const int base = smem0 + stage * (SM::STAGE + SM::STATS), lds = base + wave * 16 * 2 * EC;
+    const auto q_rs = wave_rsrc_words(row_at<T>(a.q, a.sq, si, h, at), rows_extent(left, q_row, (a.e + a.r) * 2));
+    qt.fetch(q_rs, lds);
+    rt.fetch(q_rs, base + SM::C_OFF + wave * 16 * 2 * kLatentShared);
+    dt.fetch(wave_rsrc_words(row_at<T>(a.dout, a.sdo, si, h, at), rows_extent(left, do_row, a.ev * 2)), lds + SM::V_OFF);
+    // (of a row past the sequence Q, dO and both statistics are 0: nothing comes of it)
+    if (wave < 2) {
+      const int n = si.seqlen_q - j * 64 < 64 ? si.seqlen_q - j * 64 : 64;
+      load_word_to_lds(wave_rsrc_words(stats + j * 64, n > 0 ? n * 4 : 0), lane * 4, base + SM::STAGE + wave * 256);
+    }
+  };
+  if (j0 < j1) fetch(0, j0);
+
+  op_t k[KE + KR], v[KE];
+  load_operands<T, KE>(k, row_at<T>(a.k, a.sk, si, h, (int64_t)si.k_start + w0), (int)a.sk.s * 2, keys, lane, 0, a.e);
+  load_operands<T, KR>(k + KE, row_at<T>(a.c, Strides3{a.c_z, 0, a.c_s}, si, 0, (int64_t)si.k_start + w0), (int)a.c_s * 2, keys, lane, 0, a.r);
+  load_operands<T, KE>(v, row_at<T>(a.v, a.sv, si, h, (int64_t)si.k_start + w0), (int)a.sv.s * 2, keys, lane, 0, a.ev);
+  f32x16 dk[DB + RB], dv[DB];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+#pragma unroll
+    for (int b = 0; b < DB + RB; ++b) dk[b][i] = 0.f;
+#pragma unroll
+    for (int b = 0; b < DB; ++b) dv[b][i] = 0.f;
+  }
+  const float qs = a.sm_scale * kLog2e;
+  const int row_e = Swz<EC>::row_base(lane), row_r = Swz<kLatentShared>::row_base(lane);
+  const int tr0 = Swz<EC>::tr_base(lane, 0), tr1 = Swz<EC>::tr_base(lane, 1);
+  const int rr0 = Swz<kLatentShared>::tr_base(lane, 0), rr1 = Swz<kLatentShared>::tr_base(lane, 1);
+
+  for (int j = j0; j < j1; ++j) {
+    latent_meet();
+    const int stage = (j - j0) & 1;
+    if (j + 1 < j1) fetch(stage ^ 1, j + 1);
+    const char* Q = smem + stage * (SM::STAGE + SM::STATS);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int m0 = j * 64 + 32 * b;
+      if (m0 + 31 < first_query(w0)) continue;      // none of its queries sees a key of the wave
+      const bool masked = a.causal && m0 < w0 + 31 - shift;
+      f32x16 s, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+      for (int x = 0; x < KE; ++x) s = Tr::mfma(swz_read_row<T, EC>(Q, row_e, x, b), k[x], s);
+#pragma unroll
+      for (int x = 0; x < KR; ++x) s = Tr::mfma(swz_read_row<T, kLatentShared>(Q + SM::C_OFF, row_r, x, b), k[KE + x], s);
+#pragma unroll
+      for (int x = 0; x < KE; ++x) dp = Tr::mfma(swz_read_row<T, EC>(Q + SM::V_OFF, row_e, x, b), v[x], dp);
+      const int from = key - shift - m0 - 4 * hi;      // the lane's key is seen from this row of the block on
+      const float* st = reinterpret_cast<const float*>(Q + SM::STAGE) + 32 * b + 4 * hi;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 8 * g), delta = *reinterpret_cast<const f32x4*>(st + 64 + 8 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = 4 * g + r;
+          float p = fast_exp2(__builtin_fmaf(s[i], qs, -lse[r]));
+          if (masked && 8 * g + r < from) p = 0.f;
+          dp[i] = p * (dp[i] - delta[r]);
+          s[i] = p;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const op_t p = pack8<T>(s, t), ds = pack8<T>(dp, t);
+#pragma unroll
+        for (int x = 0; x < DB; ++x) dv[x] = Tr::mfma(swz_read_tr<T, EC>(Q + SM::V_OFF, tr0, tr1, 2 * b + t, x), p, dv[x]);
+#pragma unroll
+        for (int x = 0; x < DB; ++x) dk[x] = Tr::mfma(swz_read_tr<T, EC>(Q, tr0, tr1, 2 * b + t, x), ds, dk[x]);
+#pragma unroll
+        for (int x = 0; x < RB; ++x) dk[DB + x] = Tr::mfma(swz_read_tr<T, kLatentShared>(Q + SM::C_OFF, rr0, rr1, 2 * b + t, x), ds, dk[DB + x]);
+      }
+    }
+  }
+  if (key >= si.seqlen_k) return;
+  store_rows<T, DB>(dk, a.sm_scale, row_at<T>(a.dk, a.sdk, si, h, (int64_t)si.k_start + key), a.e, hi);
+  store_rows<T, DB>(dv, 1.0f, row_at<T>(a.dv, a.sdv, si, h, (int64_t)si.k_start + key), a.ev, hi);
+  float* to = a.part_c + (((int64_t)si.batch_index * a.heads + h) * a.part_rows + si.k_start + key) * kLatentShared + 4 * hi;
+#pragma unroll
+  for (int x = 0; x < RB; ++x)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4*>(to + 32 * x + 8 * g) = f32x4{dk[DB + x][4 * g], dk[DB + x][4 * g + 1], dk[DB + x][4 * g + 2], dk[DB + x][4 * g + 3]};
+}
+
+// dC: the heads' parts added in their order, four columns a lane
+template <typename T>
+__global__ __launch_bounds__(256) void latent_dc_kernel(const LatentBwdArgs a, int64_t keys, const int32_t* end) {
+  const int64_t at = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+  const int64_t b = at / keys, n = at % keys;
+  const int col = threadIdx.x % 16 * 4;
+  if (b >= a.batch || (end != nullptr && n >= *end) || col >= a.r) return;
+  const float* from = a.part_c + (b * a.heads * a.part_rows + n) * kLatentShared + col;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int h = 0; h < a.heads; ++h) sum += *reinterpret_cast<const f32x4*>(from + (int64_t)h * a.part_rows * kLatentShared);
+  typename Traits<T>::q4_t y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(sum[r] * a.sm_scale);
+  *reinterpret_cast<typename Traits<T>::q4_t*>(reinterpret_cast<T*>(a.dc) + b * a.dc_z + n * a.dc_s + col) = y;
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------
+template <typename T, int EC> hipError_t launch_latent_fwd(const LatentArgs& a, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  const int nseq = nseq_of(a.seq, a.batch), tiles = (a.seq.max_seqlen_q + 127) / 128;
+  if (nseq == 0 || tiles == 0) return hipSuccess;
+  hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_fwd_kernel<T, EC>), LatentSmem<EC>::BYTES, done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((latent_fwd_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles * a.parts)), dim3(256), LatentSmem<EC>::BYTES, s, a, nseq, tiles);
+  if (a.parts > 1)
+    hipLaunchKernelGGL((latent_fwd_sum_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles * 4 * (EC / 32))), dim3(256), 0, s, a, nseq, tiles);
+  return hipGetLastError();
+}
+
+template <typename T, int EC> hipError_t launch_latent_bwd(const LatentBwdArgs& a, hipStream_t s) {
+  static std::atomic<uint64_t> done_q{0}, done_k{0};
+  const int nseq = nseq_of(a.seq, a.batch), q_tiles = (a.seq.max_seqlen_q + 127) / 128, k_tiles = (a.seq.max_seqlen_k + 127) / 128;
+  hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_dq_kernel<T, EC>), LatentSmem<EC>::BYTES, done_q);
+  if (e == hipSuccess) e = allow_large_lds(reinterpret_cast<const void*>(&latent_dkdv_kernel<T, EC>), LatentSmem<EC>::BWD_BYTES, done_k);
+  if (e != hipSuccess || nseq == 0) return e;
+  if (q_tiles > 0) hipLaunchKernelGGL((latent_dq_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * q_tiles)), dim3(256), LatentSmem<EC>::BYTES, s, a, nseq, q_tiles);
+  if (k_tiles > 0) {
+    hipLaunchKernelGGL((latent_dkdv_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * k_tiles)), dim3(256), LatentSmem<EC>::BWD_BYTES, s, a, nseq, k_tiles);
+    const int32_t* end = a.seq.num_seqlens != 0 ? a.seq.cu_k + nseq : nullptr;
+    hipLaunchKernelGGL((latent_dc_kernel<T>), dim3((unsigned)((a.batch * a.part_rows + 15) / 16)), dim3(256), 0, s, a, a.part_rows, end);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace fa

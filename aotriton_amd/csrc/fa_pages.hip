@@ -180,6 +180,191 @@ __global__ __launch_bounds__(256) void free_pages_kernel(const FreeArgs a) {
   if (page >= 0 && page < a.pages) atomicSub(a.uses + page, 1);
 }
 
+// ---- append_packed: row t to the slot that is named for it -----------------------------------------------------------------
+// A thread per piece; a token's pieces lie next to each other.
+__global__ __launch_bounds__(256) void append_packed_kernel(const PackedAppendArgs a) {
+  const CacheArgs& c = a.cache;
+  const uint32_t per_k = c.head_dim / 8 * c.heads, per = per_k + c.head_dim_v / 8 * c.heads;
+  const uint32_t e = blockIdx.x * 256 + threadIdx.x;
+  const int t = (int)(e / per);
+  if (t >= a.tokens) return;
+  const int64_t slot = a.slots[t], page = slot >> c.page_shift;
+  if (slot < 0 || page >= c.pages) return;
+  uint32_t x = e % per;
+  const bool v = x >= per_k;
+  if (v) x -= per_k;
+  const uint32_t pieces = (v ? c.head_dim_v : c.head_dim) / 8, h = x / pieces;
+  const int col = (int)(x % pieces) * 8;
+  const Strides3& from = v ? a.snv : a.snk;
+  const uint16_t* src = reinterpret_cast<const uint16_t*>(v ? a.new_v : a.new_k) + (int64_t)t * from.z + (int64_t)h * from.h;
+  uint16_t* dst = row_of(v ? c.v : c.k, v ? c.sv : c.sk, (int)page, h, slot_in_page(c, slot));
+  *reinterpret_cast<piece_t*>(dst + col) = *reinterpret_cast<const piece_t*>(src + col);
+}
+
+// ---- reserve: pages for the rows that a batch adds, and where each goes ----------------------------------------------------
+// The k-th column that needs a page, in the order of sequences and columns, gets the k-th free page.  Two launches: the first notes which
+// pages are free and counts what each sequence asks for; the second gives each sequence its pages from there, so that nothing it reads is
+// what another workgroup writes.  Bound by dependent round trips to memory.
+struct Reserve {
+  int32_t start, count;          // first row of the sequence in the batch, rows
+  int32_t first, last;           // columns that they touch, as far as the table goes
+};
+// Sum of the values in front of place z of n, and of all.  All threads of the workgroup call it; `sums` has room for a word per wave.
+template <typename Value>
+__device__ __forceinline__ void sum_before(int n, int z, Value value, int64_t* sums, int64_t& before, int64_t& all) {
+  int64_t b = 0, s = 0;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int64_t x = value(i);
+    s += x;
+    b += i < z ? x : 0;
+  }
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) { b += __shfl_xor(b, i); s += __shfl_xor(s, i); }
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) { sums[wave] = b; sums[4 + wave] = s; }
+  __syncthreads();
+  before = sums[0] + sums[1] + sums[2] + sums[3];
+  all = sums[4] + sums[5] + sums[6] + sums[7];
+  __syncthreads();
+}
+__device__ __forceinline__ int rows_asked(const ReserveArgs& a, int z) { return a.lengths[z] < 0 || a.counts[z] < 0 ? 0 : a.counts[z]; }
+__device__ __forceinline__ Reserve reserve_of(const ReserveArgs& a, int z, int64_t start) {
+  Reserve r;
+  const int length = a.lengths[z], asked = rows_asked(a, z);
+  r.start = (int)(start < a.tokens ? start : a.tokens);
+  r.count = asked < a.tokens - r.start ? asked : a.tokens - r.start;
+  const int64_t first = (int64_t)length >> a.page_shift, last = ((int64_t)length + r.count + (1 << a.page_shift) - 1) >> a.page_shift;
+  r.first = (int)(r.count > 0 && first < a.columns ? first : 0);
+  r.last = (int)(r.count > 0 && first < a.columns ? (last < a.columns ? last : a.columns) : 0);
+  return r;
+}
+__device__ __forceinline__ bool no_page(const ReserveArgs& a, int entry) { return entry < 0 || entry >= a.pages; }
+
+// workgroups below a.runs: a run of pages each; the others: a sequence each
+__global__ __launch_bounds__(256) void reserve_count_kernel(const ReserveArgs a) {
+  __shared__ int64_t sums[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if ((int)blockIdx.x < a.runs) {
+    int n = 0;
+    const int w0 = (int)blockIdx.x << a.run_shift, w1 = w0 + (1 << a.run_shift) < a.words ? w0 + (1 << a.run_shift) : a.words;
+    for (int w = w0 + wave; w < w1; w += 4) {
+      const int64_t page = (int64_t)w * 64 + lane;
+      const uint64_t bits = __builtin_amdgcn_ballot_w64(page < a.pages && a.uses[page < a.pages ? page : 0] == 0);
+      if (lane == 0) a.free_bits[w] = bits;
+      n += __builtin_popcountll(bits);
+    }
+    if (lane == 0) sums[wave] = n;
+    __syncthreads();
+    if (tid == 0) a.run_free[blockIdx.x] = (int)(sums[0] + sums[1] + sums[2] + sums[3]);
+    return;
+  }
+  const int z = blockIdx.x - a.runs;
+  int64_t before, all;
+  sum_before(a.sequences, z, [&](int i) { return (int64_t)rows_asked(a, i); }, sums, before, all);
+  if (z >= a.sequences) {      // (of no sequence: the end)
+    if (tid == 0) a.starts[a.sequences] = (int)(all < a.tokens ? all : a.tokens);
+    return;
+  }
+  const Reserve r = reserve_of(a, z, before);
+  int n = 0;
+  for (int c = r.first + tid; c < r.last; c += 256) n += no_page(a, a.table[(int64_t)z * a.table_row + c]) ? 1 : 0;
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) n += __shfl_xor(n, i);
+  if (lane == 0) sums[wave] = n;
+  __syncthreads();
+  if (tid == 0) {
+    a.starts[z] = r.start;
+    a.wanted[z] = (int)(sums[0] + sums[1] + sums[2] + sums[3]);
+  }
+}
+
+// Free page number k: the run by its sums in LDS, the word in the run, the bit in the word.
+__device__ __forceinline__ int free_page(const ReserveArgs& a, const int32_t* run_sum, int k) {
+  int lo = 0, n = a.runs;        // the last run with no more than k free pages in front of it
+  while (n > 1) {
+    const int half = n / 2;
+    if (run_sum[lo + half] <= k) lo += half;
+    n -= half;
+  }
+  k -= run_sum[lo];
+  int w = lo << a.run_shift;
+  for (;; ++w) {
+    const int c = __builtin_popcountll(a.free_bits[w]);
+    if (k < c) break;
+    k -= c;
+  }
+  uint64_t bits = a.free_bits[w];
+  int at = 0;
+#pragma unroll
+  for (int half = 32; half >= 1; half /= 2) {
+    const uint64_t low = bits & ((1ull << half) - 1);
+    const int c = __builtin_popcountll(low);
+    if (k >= c) { k -= c; at += half; bits >>= half; }
+    else bits = low;
+  }
+  return w * 64 + at;
+}
+
+__global__ __launch_bounds__(256) void reserve_kernel(const ReserveArgs a) {
+  __shared__ int64_t sums[8];
+  __shared__ int32_t run_sum[kReserveRuns + 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, z = blockIdx.x;
+  // free pages in front of each run
+  int base = 0;
+  for (int i0 = 0; i0 < a.runs; i0 += 256) {
+    const int n = i0 + tid < a.runs ? a.run_free[i0 + tid] : 0;
+    int s = n;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) { const int y = __shfl_up(s, i); s += lane >= i ? y : 0; }
+    if (lane == 63) sums[wave] = s;
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) s += (int)sums[w];
+    }
+    if (i0 + tid < a.runs) run_sum[i0 + tid] = base + s - n;
+    base += (int)(sums[0] + sums[1] + sums[2] + sums[3]);
+    __syncthreads();
+  }
+  const int free = base;
+  int64_t rank, all;
+  sum_before(a.sequences, z, [&](int i) { return (int64_t)a.wanted[i]; }, sums, rank, all);
+  if (z == 0 && tid == 0) *a.missing = (int)(all > free ? all - free : 0);
+  // rows of no sequence
+  for (int64_t i = (int64_t)a.starts[a.sequences] + blockIdx.x * 256 + tid; i < a.tokens; i += (int64_t)gridDim.x * 256) a.slots[i] = -1;
+  if (z >= a.sequences) return;
+  const Reserve r = reserve_of(a, z, a.starts[z]);
+  int32_t* row = a.table + (int64_t)z * a.table_row;
+  if (a.wanted[z] > 0)
+    for (int c0 = r.first; c0 < r.last; c0 += 256) {
+      const int c = c0 + tid;
+      const bool want = c < r.last && no_page(a, row[c]);
+      const uint64_t ask = __builtin_amdgcn_ballot_w64(want);
+      if (lane == 0) sums[wave] = __builtin_popcountll(ask);
+      __syncthreads();
+      int64_t k = rank + __builtin_popcountll(ask & ((1ull << lane) - 1));
+      for (int w = 0; w < 4; ++w) {
+        if (w < wave) k += sums[w];
+        rank += sums[w];
+      }
+      if (want && k < free) {
+        const int page = free_page(a, run_sum, (int)k);
+        row[c] = page;
+        a.uses[page] = 1;
+      }
+      __syncthreads();
+    }
+  const int length = a.lengths[z];
+  for (int i = tid; i < r.count; i += 256) {
+    const int64_t slot = (int64_t)length + i, c = slot >> a.page_shift;
+    int64_t at = -1;
+    if (c < a.columns) {
+      const int page = row[c];
+      if (!no_page(a, page)) at = ((int64_t)page << a.page_shift) + (slot & ((1 << a.page_shift) - 1));
+    }
+    a.slots[(int64_t)r.start + i] = at;
+  }
+}
+
 unsigned blocks_of(int64_t n, int per) { return (unsigned)((n + per - 1) / per); }
 
 }  // namespace
@@ -224,6 +409,19 @@ hipError_t run_cache_free(const FreeArgs& a0, int count, hipStream_t s) {
   a.chunks = (int)blocks_of(a.columns, 256);
   if (count == 0 || a.columns == 0) return hipSuccess;
   hipLaunchKernelGGL(free_pages_kernel, dim3((unsigned)(count * a.chunks)), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t run_cache_append_packed(const PackedAppendArgs& a, hipStream_t s) {
+  const int64_t pieces = (int64_t)a.tokens * a.cache.heads * ((a.cache.head_dim + a.cache.head_dim_v) / 8);
+  if (pieces == 0) return hipSuccess;
+  hipLaunchKernelGGL(append_packed_kernel, dim3(blocks_of(pieces, 256)), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t run_cache_reserve(const ReserveArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL(reserve_count_kernel, dim3((unsigned)(a.runs + a.sequences + 1)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(reserve_kernel, dim3((unsigned)(a.sequences > 0 ? a.sequences : 1)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

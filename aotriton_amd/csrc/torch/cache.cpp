@@ -140,6 +140,47 @@ void free_kernel(const Tensor& table, const Tensor& uses, const Tensor& sequence
   check_rc(fa_cache_free(&t, &u, &s, &a, &b, current_stream()), false);
 }
 
+std::tuple<Tensor, Tensor, Tensor> reserve_kernel(const Tensor& table, const Tensor& uses, const Tensor& lengths, const Tensor& counts,
+                                                  int64_t tokens, int64_t slots) {
+  const c10::DeviceGuard guard(table.device());
+  TORCH_CHECK_VALUE(table.dim() == 2 && uses.dim() == 1, "a table of rows, and vectors");
+  fa_reserve_params p{};
+  const int64_t n = table.size(0);
+  int_rows(table, n, table, &p.table, "the page table");
+  ints(uses, uses.size(0), table, &p.uses, "uses");
+  ints(lengths, n, table, &p.lengths, "lengths");
+  ints(counts, n, table, &p.counts, "counts");
+  p.slots = as_int32(slots, "slots");
+  const Tensor starts = at::empty({n + 1}, lengths.options()), missing = at::empty({1}, lengths.options());
+  const Tensor map = at::empty({as_int32(tokens, "tokens")}, lengths.options().dtype(at::kLong));
+  ints(starts, n + 1, table, &p.starts, "starts");
+  ints(missing, 1, table, &p.missing, "missing");
+  p.slot_map = fa_tensor1{map.data_ptr(), {(uint64_t)tokens}, {1}, FA_DTYPE_INT64};
+  Scratch scratch;
+  check_rc(fa_cache_reserve(&p, current_stream(), &scratch.c), false);
+  return {starts, map, missing};
+}
+
+void append_packed_kernel(const Tensor& key, const std::optional<Tensor>& value, const Tensor& k, const std::optional<Tensor>& v, const Tensor& slot_map) {
+  const c10::DeviceGuard guard(k.device());
+  const bool both = value.has_value() && value->defined();
+  TORCH_CHECK_VALUE(both == (v.has_value() && v->defined()), "values come with a cache of values, or neither");
+  TORCH_CHECK_VALUE(key.dim() == 3 && (!both || value->dim() == 3), "expected (rows, heads, head_dim) rows");
+  TORCH_CHECK_VALUE(slot_map.dim() == 1 && slot_map.size(0) == key.size(0) && slot_map.scalar_type() == at::kLong && slot_map.device() == k.device() &&
+                        (slot_map.size(0) <= 1 || slot_map.stride(0) == 1),
+                    "the slot map is a contiguous int64 tensor of a value for each row, on the device of the cache");
+  fa_tensor4 kv{}, vv{}, kc{}, vc{};
+  rows4(k, k, &kc, "the cache of keys");
+  const Tensor nk = pieces(key).unsqueeze(0), nv = both ? pieces(*value).unsqueeze(0) : Tensor();
+  rows4(nk, k, &kv, "the new keys");
+  if (both) {
+    rows4(*v, k, &vc, "the cache of values");
+    rows4(nv, k, &vv, "the new values");
+  }
+  const fa_tensor1 m{slot_map.data_ptr(), {(uint64_t)slot_map.size(0)}, {1}, FA_DTYPE_INT64};
+  check_rc(fa_cache_append_packed(&kv, both ? &vv : nullptr, &kc, both ? &vc : nullptr, &m, current_stream()), false);
+}
+
 // (no derivatives: caches are inference state.  A call that would have to record one says so)
 std::tuple<Tensor, Tensor> tree_autograd(const Tensor& query, const Tensor& k, const Tensor& v, const Tensor& table,
                                          const Tensor& lengths, const std::optional<Tensor>& parents, c10::SymInt max_length, c10::SymInt window,
@@ -158,20 +199,24 @@ std::tuple<Tensor, Tensor> tree_autograd(const Tensor& query, const Tensor& k, c
 // The ops that write, kWritten the places of what they write to: no derivatives either, and the version counters of those tensors move,
 // so that a backward that has kept one of them says so.
 constexpr char kAppend[] = "aotriton_amd::cache_append", kCopy[] = "aotriton_amd::cache_copy_pages", kFork[] = "aotriton_amd::cache_fork",
-               kKeep[] = "aotriton_amd::cache_keep_path", kFree[] = "aotriton_amd::cache_free";
-template <const char* kName, auto kKernel, size_t... kWritten> struct Writer;
-template <const char* kName, typename R, typename... A, R (*kKernel)(A...), size_t... kWritten>
-struct Writer<kName, kKernel, kWritten...> {
+               kKeep[] = "aotriton_amd::cache_keep_path", kFree[] = "aotriton_amd::cache_free", kReserve[] = "aotriton_amd::cache_reserve",
+               kAppendPacked[] = "aotriton_amd::cache_append_packed";
+template <const char* kName, typename Signature, size_t... kWritten> struct Writer;
+template <const char* kName, typename R, typename... A, size_t... kWritten>
+struct Writer<kName, R(A...), kWritten...> {
   static const c10::TypedOperatorHandle<R(A...)>& op() {
     static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(kName, "").template typed<R(A...)>();
     return op;
   }
   static R autograd(c10::DispatchKeySet keys, A... a) {
-    const auto refuse = [](const auto& t) {
-      if constexpr (std::is_same_v<std::decay_t<decltype(t)>, Tensor>) {
-        refuse_tangents({&t});
-        TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t.requires_grad()), kName, " has no gradient; call it under torch.no_grad()");
-      }
+    const auto refuse_one = [](const Tensor& t) {
+      refuse_tangents({&t});
+      TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t.requires_grad()), kName, " has no gradient; call it under torch.no_grad()");
+    };
+    const auto refuse = [&](const auto& t) {
+      if constexpr (std::is_same_v<std::decay_t<decltype(t)>, Tensor>) refuse_one(t);
+      if constexpr (std::is_same_v<std::decay_t<decltype(t)>, std::optional<Tensor>>)
+        if (t.has_value() && t->defined()) refuse_one(*t);
     };
     (refuse(a), ...);
     return op().redispatch(keys & c10::after_autograd_keyset, a...);
@@ -179,8 +224,8 @@ struct Writer<kName, kKernel, kWritten...> {
   static R inplace(c10::DispatchKeySet keys, A... a) {
     const auto all = std::forward_as_tuple(a...);
     // (a tensor of inference mode has no counter)
-    const auto written = [](const Tensor& t) {
-      if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+    const auto written = [](const std::optional<Tensor>& t) {
+      if (t.has_value() && t->defined() && !t->is_inference()) torch::autograd::impl::bump_version(*t);
     };
     if constexpr (std::is_void_v<R>) {
       op().redispatch(keys & c10::after_ADInplaceOrView_keyset, a...);
@@ -192,11 +237,13 @@ struct Writer<kName, kKernel, kWritten...> {
     }
   }
 };
-using Append = Writer<kAppend, &append_kernel, 2, 3>;
-using Copy = Writer<kCopy, &copy_kernel, 0, 1>;
-using Fork = Writer<kFork, &fork_kernel, 0, 1, 2, 3, 4>;
-using Keep = Writer<kKeep, &keep_kernel, 0, 1>;
-using Free = Writer<kFree, &free_kernel, 0, 1>;
+using Append = Writer<kAppend, decltype(append_kernel), 2, 3>;
+using Copy = Writer<kCopy, decltype(copy_kernel), 0, 1>;
+using Fork = Writer<kFork, decltype(fork_kernel), 0, 1, 2, 3, 4>;
+using Keep = Writer<kKeep, decltype(keep_kernel), 0, 1>;
+using Free = Writer<kFree, decltype(free_kernel), 0, 1>;
+using Reserve = Writer<kReserve, std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, c10::SymInt, c10::SymInt), 0, 1>;
+using AppendPacked = Writer<kAppendPacked, decltype(append_packed_kernel), 2, 3>;
 
 TORCH_LIBRARY_FRAGMENT(aotriton_amd, m) {
   const std::vector<at::Tag> compliant{at::Tag::pt2_compliant_tag};
@@ -207,6 +254,8 @@ TORCH_LIBRARY_FRAGMENT(aotriton_amd, m) {
   m.def("cache_fork(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) page_table, Tensor(d!) lengths, Tensor(e!) uses, Tensor source, "
         "Tensor target, Tensor spare) -> ()", compliant);
   m.def("cache_keep_path(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table, Tensor lengths, Tensor path, Tensor counts) -> Tensor", compliant);
+  m.def("cache_reserve(Tensor(a!) page_table, Tensor(b!) uses, Tensor lengths, Tensor counts, SymInt tokens, SymInt slots) -> (Tensor, Tensor, Tensor)", compliant);
+  m.def("cache_append_packed(Tensor key, Tensor? value, Tensor(a!) k_cache, Tensor(b!)? v_cache, Tensor slot_map) -> ()", compliant);
   m.def("cache_free(Tensor(a!) page_table, Tensor(b!) uses, Tensor sequences, Tensor first, Tensor last) -> ()", compliant);
 }
 TORCH_LIBRARY_IMPL(aotriton_amd, CUDA, m) {
@@ -216,6 +265,8 @@ TORCH_LIBRARY_IMPL(aotriton_amd, CUDA, m) {
   m.impl("cache_fork", &fork_kernel);
   m.impl("cache_keep_path", &keep_kernel);
   m.impl("cache_free", &free_kernel);
+  m.impl("cache_reserve", &reserve_kernel);
+  m.impl("cache_append_packed", &append_packed_kernel);
 }
 TORCH_LIBRARY_IMPL(aotriton_amd, Autograd, m) {
   m.impl("tree_attention", &tree_autograd);
@@ -224,6 +275,8 @@ TORCH_LIBRARY_IMPL(aotriton_amd, Autograd, m) {
   m.impl("cache_fork", &Fork::autograd);
   m.impl("cache_keep_path", &Keep::autograd);
   m.impl("cache_free", &Free::autograd);
+  m.impl("cache_reserve", &Reserve::autograd);
+  m.impl("cache_append_packed", &AppendPacked::autograd);
 }
 TORCH_LIBRARY_IMPL(aotriton_amd, ADInplaceOrView, m) {
   m.impl("cache_append", &Append::inplace);
@@ -231,6 +284,8 @@ TORCH_LIBRARY_IMPL(aotriton_amd, ADInplaceOrView, m) {
   m.impl("cache_fork", &Fork::inplace);
   m.impl("cache_keep_path", &Keep::inplace);
   m.impl("cache_free", &Free::inplace);
+  m.impl("cache_reserve", &Reserve::inplace);
+  m.impl("cache_append_packed", &AppendPacked::inplace);
 }
 
 }  // namespace

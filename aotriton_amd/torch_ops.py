@@ -15,7 +15,12 @@ so that code using them can be traced by torch.compile / AOTAutograd.
         -> Out, logsumexp; a sliding window and first tokens that stay visible (sink_attention below)
     sink_attention_backward(dout, q, k, v, out, lse, cu_seqlens_q, ..., sm_scale)
         -> dQ, dK, dV
-    tree_attention, cache_append, cache_copy_pages, cache_fork, cache_keep_path, cache_free
+    latent_attention_forward(query, key, value, shared_key, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, is_causal, sm_scale)
+        -> Out, logsumexp; keys that are part per head, part shared (latent_attention below)
+    latent_attention_backward(dout, query, key, value, shared_key, out, lse, cu_seqlens_q, ..., sm_scale)
+        -> gradients of the four
+    tree_attention, latent_cache_attention, cache_append, cache_append_packed, cache_reserve, cache_copy_pages, cache_fork, cache_keep_path,
+    cache_free
         the cache of pages (cache.py)
     philox_state(like, increment)
         -> seed and offset (uint64[1] tensors on like's device) of the device's default generator, whose
@@ -47,7 +52,7 @@ from .sdpa import prepare
 _torch_host = _host.load()      # registers the ops
 
 __all__ = ['flash_attention_forward', 'flash_attention_backward', 'philox_state', 'scaled_dot_product_attention',
-           'sink_attention']
+           'sink_attention', 'latent_attention']
 
 
 philox_state = torch.ops.aotriton_amd.philox_state
@@ -124,6 +129,49 @@ def sink_attention(query, key, value, window, sinks=0, scale=None, cu_seqlens_q=
         raise ValueError('packed sequences need max_seqlen_q and max_seqlen_k')
     o, _ = torch.ops.aotriton_amd.sink_attention_forward(query, key, value, cu_seqlens_q, cu_seqlens_k, max_seqlen_q or 0,
                                                          max_seqlen_k or 0, window, sinks, sm_scale)
+    return o
+
+
+@torch.library.register_fake('aotriton_amd::latent_attention_forward')
+def _(query, key, value, shared_key, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, is_causal, sm_scale):
+    out = torch.empty((query.shape[0], query.shape[1], query.shape[2], value.shape[3]), device=query.device, dtype=query.dtype)
+    return out, torch.empty((query.shape[0] * query.shape[1], query.shape[2]), device=query.device, dtype=torch.float32)
+
+
+@torch.library.register_fake('aotriton_amd::latent_attention_backward')
+def _(dout, query, key, value, shared_key, out, lse, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, is_causal, sm_scale):
+    def like(t):
+        g = torch.empty_like(t)
+        return g if g.stride(-1) == 1 else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+    return like(query), like(key), like(value), like(shared_key)
+
+
+def latent_attention(query, key, value, shared_key, is_causal=True, scale=None, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=None,
+                     max_seqlen_k=None):
+    """Attention whose keys are part per head and part shared by all heads, forward and backward: latent attention in its expanded form, in
+    which a projection makes every head's ``key`` and ``value`` from one latent vector a token, and the rotary part of the key is one vector
+    for all heads.
+
+    query (B, H, Sq, E + R), key (B, H, Sk, E), value (B, H, Sk, Ev), shared_key (B, Sk, R): fp16 or bf16 CUDA tensors of any storage, E and Ev
+    multiples of 8 up to 128, R up to 64.  The score of a query and a key is ``scale`` (1 / sqrt(E + R)) times query[..., :E] . key + query[..., E:] .
+    shared_key.  With ``is_causal`` the queries stand at the last keys: query i sees keys up to i + Sk - Sq; one that sees none yields zeros
+    and no gradient.  The gradient of shared_key is the sum over the heads, added up in fp32.  Keys and values that a query does not see
+    have to be finite all the same where they belong to its sequence.
+
+    Packed sequences: (1, H, tokens, ...) tensors with the sequences' offsets in cu_seqlens_q / cu_seqlens_k (int32 tensors on the device,
+    sequences + 1 values) and their greatest lengths in max_seqlen_q / max_seqlen_k; tokens behind the last offset belong to no sequence:
+    their rows of the result and of the gradients are 0, and may hold anything.
+
+    Works under HIP graph capture and torch.compile; results do not change from call to call.  There is no dropout and no bias.  The same
+    attention of new tokens over a cache of the latent vectors: aotriton_amd.cache.latent_attention.
+    """
+    sm_scale = 1.0 / math.sqrt(query.shape[-1]) if scale is None else float(scale)
+    if (cu_seqlens_q is None) != (cu_seqlens_k is None):
+        raise ValueError('cu_seqlens come for queries and keys or for neither')
+    if cu_seqlens_q is not None and (max_seqlen_q is None or max_seqlen_k is None):
+        raise ValueError('packed sequences need max_seqlen_q and max_seqlen_k')
+    o, _ = torch.ops.aotriton_amd.latent_attention_forward(query, key, value, shared_key, cu_seqlens_q, cu_seqlens_k, max_seqlen_q or 0,
+                                                           max_seqlen_k or 0, is_causal, sm_scale)
     return o
 
 

@@ -4,8 +4,8 @@
  * the reference.
  *
  * A cache is two tensors (pages, heads, slots of a page, head dim) of fp16 or bf16: any strides with a unit last one, made of aligned
- * 16-byte pieces (head dims, up to 256, and strides multiples of 8, 16-byte aligned bases, pages less than 2^31 elements apart), so that (pages, slots, heads, head dim) storage
- * is as good; the slots of a page are a power of two from 16 up.  A sequence is a row of the page table, int32 with -1 where
+ * 16-byte pieces (head dims, up to 256, where rows only move 576, and strides multiples of 8, 16-byte aligned bases, pages less than 2^31 elements apart), so that (pages, slots, heads, head dim) storage
+ * is as good, and so are two ranges of columns of one tensor (a cache of latent rows, latent.h); the slots of a page are a power of two from 16 up.  A sequence is a row of the page table, int32 with -1 where
  * there is no page, and a length: slot n of the sequence is slot n % slots of the page in column n / slots.  All indices are read on the
  * device, and none is trusted: pages outside the cache, sequences outside the table, slots outside a row of the table are not
  * read and not written (what would have stood there is not there); a negative length is a sequence that is not there.
@@ -53,6 +53,29 @@ FA_API int fa_tree_attn(const fa_tree_params* params, void* hip_stream, fa_alloc
 /* Rows t < counts[z] (null: all) of k (sequences, Hk, tokens, D) and v into slots lengths[z] + t.  Lengths stay as they are.  Two
  * sequences that share the page written to race. */
 FA_API int fa_cache_append(const fa_tensor4* k, const fa_tensor4* v, const fa_cache* cache, const fa_tensor1* counts, void* hip_stream);
+
+/* A batch of sequences adds rows, which are packed: sequence z adds counts[z] of them (a negative count, or length, is none), rows
+ * [starts[z], starts[z + 1]) of the batch, and none past the batch's rows, which are as many as slot_map has.  Every column of the page table that
+ * they touch and that has no page gets a free one (uses[] 0), in the order of sequences and columns the free pages in theirs, and its uses[]
+ * become 1.  slot_map[starts[z] + t] is where slot lengths[z] + t lies: its page times `slots`, plus the slot in the page; -1 where there is
+ * no page, for rows of no sequence, and for slots outside the table.  missing[0]: columns for which there was no free page.  Lengths stay as they
+ * are.  Takes scratch memory from alloc: a bit for every page, a word for every sequence. */
+typedef struct fa_reserve_params {
+  fa_tensor2 table;     /* int32 (sequences, columns) */
+  fa_tensor1 uses;      /* int32 (pages) */
+  fa_tensor1 lengths;   /* int32 (sequences) */
+  fa_tensor1 counts;    /* int32 (sequences) */
+  fa_tensor1 starts;    /* out, int32 (sequences + 1) */
+  fa_tensor1 slot_map;  /* out, int64 (rows of the batch) */
+  fa_tensor1 missing;   /* out, int32 (1) */
+  int32_t slots;        /* of a page: a power of two from 16 up */
+} fa_reserve_params;
+FA_API int fa_cache_reserve(const fa_reserve_params* params, void* hip_stream, fa_allocator* alloc);
+
+/* Row t of k (1, rows, Hk, D) and v into slot slot_map[t] (int64: page times slots of a page, plus the slot in it); one outside the cache
+ * is not written.  v and v_cache may both be null.  No slot may be named twice. */
+FA_API int fa_cache_append_packed(const fa_tensor4* k, const fa_tensor4* v, const fa_tensor4* k_cache, const fa_tensor4* v_cache,
+                                  const fa_tensor1* slot_map, void* hip_stream);
 
 /* Page target[i] becomes a copy of page source[i].  No target may be named twice or be a source of the same call. */
 FA_API int fa_cache_copy_pages(const fa_tensor4* k_cache, const fa_tensor4* v_cache, const fa_tensor1* source, const fa_tensor1* target, void* hip_stream);

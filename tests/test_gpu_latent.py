@@ -1,0 +1,285 @@
+"""Attention over keys that are part per head, part shared by all heads, forward and backward, against the 64-bit oracle: lengths around the
+tiles' edges, one row to many, queries without a key, keys cut into parts, packed sequences, columns that are rounded up, strides, streams,
+graphs.  The bounds are those of tests/_longctx.py; the shared part's gradient has those of its heads together, and of their fp32 sum."""
+import math
+
+import pytest
+import torch
+
+from _longctx import assert_within, grad_bounds, lse_bound, out_bound, score_error
+from oracle import latent
+
+pytestmark = pytest.mark.gpu
+
+DEV = 'cuda'
+BF, HF = torch.bfloat16, torch.float16
+
+CASES = [
+    # B, H, Sq, Sk, E, R, Ev, causal, dtype
+    (1, 1, 1, 1, 128, 64, 128, True, BF),
+    (1, 2, 1, 65, 64, 32, 64, True, HF),
+    (2, 3, 64, 64, 128, 64, 128, True, HF),
+    (1, 2, 127, 127, 128, 64, 128, True, BF),
+    (1, 2, 129, 129, 64, 64, 64, True, BF),
+    (2, 4, 331, 331, 64, 32, 64, True, HF),
+    (1, 3, 257, 257, 128, 64, 128, False, BF),
+    (1, 2, 200, 333, 128, 64, 128, True, HF),       # a chunk behind earlier keys
+    (1, 2, 33, 700, 64, 64, 64, False, BF),
+    (1, 2, 300, 170, 128, 64, 128, True, BF),       # queries before the first key
+    (1, 2, 200, 3, 64, 8, 64, True, HF),
+    (1, 2, 150, 150, 40, 24, 56, True, BF),         # columns that are rounded up
+    (1, 2, 150, 150, 8, 8, 8, True, HF),
+    (1, 2, 150, 150, 96, 32, 96, True, HF),
+    (1, 2, 140, 140, 72, 16, 128, True, BF),
+    (1, 2, 140, 140, 128, 40, 32, True, BF),
+    (1, 1, 700, 700, 128, 64, 128, True, HF),
+    (3, 5, 100, 100, 64, 32, 128, True, BF),
+]
+
+
+def _inputs(B, H, Sq, Sk, E, R, Ev, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=g).to(dtype).to(DEV)
+    kv = rn(B, Sk, H, E + Ev).transpose(1, 2)       # as a projection leaves them
+    return rn(B, Sq, H, E + R).transpose(1, 2), kv[..., :E], kv[..., E:], rn(B, Sk, R), rn(B, Sq, H, Ev).transpose(1, 2)
+
+
+def _check(q, k, v, c, do, causal, scale, out, lse, grads, what=''):
+    """one sequence, (heads, rows, columns); the shared part (rows, R)"""
+    q, k, v, c, do = (t.detach().cpu() for t in (q, k, v, c, do))
+    seen = latent.mask(q.shape[1], k.shape[1], causal)
+    kk = latent.keys(k, c)
+    want, want_lse, p = latent.attention(q, k, v, c, causal, scale)
+    size = torch.matmul(p, v.double().abs())
+    e = score_error(q, kk, scale)
+    assert_within(what + 'out', out, want, out_bound(q.dtype, want, size, v.double().abs().sum(1, keepdim=True), e))
+    if lse is not None:
+        assert_within(what + 'lse', lse, want_lse, lse_bound(torch.where(want_lse.isinf(), 0.0, want_lse), e))
+    if grads is None:
+        return
+    dq, dk, dv, dc = latent.attention_grads(q, k, v, c, do, causal, scale)
+    bq, bk, bv, u, tiny = grad_bounds(q.dtype, q, kk, v, do, seen, scale, want, size, p)
+    E, H = k.shape[2], q.shape[0]
+    # A probability below the smallest number is 0 to the hardware (tests/_longctx.py: smallest): dS = P (dP - delta) is then off by that number
+    # times |dP - delta|, which is 20 to 40 here, and the bounds count it once (scale 3: dK 5.3e-37 for 4.4e-37 where dP - delta is 30).
+    lost = tiny * abs(scale) * torch.where(seen, (torch.matmul(do.double(), v.double().transpose(1, 2)) - (do.double() * want).sum(-1, keepdim=True)).abs(), 0.0)
+    bq = bq + torch.matmul(lost, kk.double().abs())
+    bk = bk + torch.matmul(lost.transpose(1, 2), q.double().abs())
+    for name, got, w, b in (('dq', grads[0], dq, bq), ('dk', grads[1], dk, bk[..., :E]), ('dv', grads[2], dv, bv),
+                            ('dshared', grads[3], dc, (1 + H * 2.0 ** -23) * bk[..., E:].sum(0))):
+        assert_within(what + name, got, w, b + u * w.abs() + tiny)
+
+
+def _step(q, k, v, c, do, causal=True, scale=None, **packed):
+    from aotriton_amd import torch_ops
+    q, k, v, c = (t.detach().requires_grad_(True) for t in (q, k, v, c))
+    out = torch_ops.latent_attention(q, k, v, c, is_causal=causal, scale=scale, **packed)
+    return out.detach(), torch.autograd.grad(out, (q, k, v, c), do)
+
+
+def _raw(q, k, v, c, causal, scale):
+    return torch.ops.aotriton_amd.latent_attention_forward(q, k, v, c, None, None, 0, 0, causal, scale)
+
+
+@pytest.mark.parametrize('B,H,Sq,Sk,E,R,Ev,causal,dtype', CASES)
+def test_against_the_oracle(B, H, Sq, Sk, E, R, Ev, causal, dtype):
+    q, k, v, c, do = _inputs(B, H, Sq, Sk, E, R, Ev, dtype, seed=Sq + E)
+    out, grads = _step(q, k, v, c, do, causal)
+    _, lse = _raw(q, k, v, c, causal, 1 / math.sqrt(E + R))
+    for b in range(B):
+        _check(q[b], k[b], v[b], c[b], do[b], causal, 1 / math.sqrt(E + R), out[b], lse.view(B, H, Sq)[b], [g[b] for g in grads], f'sequence {b} ')
+
+
+@pytest.mark.parametrize('B,H,Sq,Sk,E,R,Ev,causal,dtype', [
+    (1, 1, 1, 4000, 128, 64, 128, True, BF), (1, 2, 130, 3000, 128, 64, 128, True, HF), (2, 1, 5, 2049, 64, 32, 64, False, HF),
+    (1, 3, 17, 1100, 40, 8, 24, True, BF), (1, 1, 2000, 1900, 64, 64, 64, True, BF)])
+def test_keys_cut_into_parts(B, H, Sq, Sk, E, R, Ev, causal, dtype):
+    q, k, v, c, do = _inputs(B, H, Sq, Sk, E, R, Ev, dtype, seed=3)
+    scale = 0.1
+    out, lse = _raw(q, k, v, c, causal, scale)
+    for b in range(B):
+        _check(q[b], k[b], v[b], c[b], do[b], causal, scale, out[b], lse.view(B, H, Sq)[b], None)
+
+
+@pytest.mark.parametrize('dtype', [HF, BF])
+@pytest.mark.parametrize('E,R,Ev', [(64, 32, 64), (128, 64, 128), (72, 64, 40)])
+@pytest.mark.parametrize('causal', [True, False])
+def test_packed_sequences(E, R, Ev, causal, dtype):
+    lens_q, lens_k = [1, 300, 0, 77, 513, 5, 40], [1, 300, 7, 200, 513, 2, 0]
+    H, tq, tk, pad = 3, sum(lens_q), sum(lens_k), 3
+    q, _, _, _, do = _inputs(1, H, tq + pad, 1, E, R, Ev, dtype, seed=1)
+    _, k, v, c, _ = _inputs(1, H, 1, tk + pad, E, R, Ev, dtype, seed=2)
+    for t in (q, do):
+        t[:, :, tq:] = float('nan')                  # rows of no sequence may hold anything
+    for t in (k, v):
+        t[:, :, tk:] = float('inf')
+    c[:, tk:] = float('nan')
+    offs = lambda lens: [sum(lens[:i]) for i in range(len(lens) + 1)]
+    cq, ck = offs(lens_q), offs(lens_k)
+    cu = lambda o: torch.tensor(o, dtype=torch.int32, device=DEV)
+    out, grads = _step(q, k, v, c, do, causal, cu_seqlens_q=cu(cq), cu_seqlens_k=cu(ck), max_seqlen_q=max(lens_q), max_seqlen_k=max(lens_k))
+    for i in range(len(lens_q)):
+        sq, sk = slice(cq[i], cq[i + 1]), slice(ck[i], ck[i + 1])
+        _check(q[0][:, sq], k[0][:, sk], v[0][:, sk], c[0][sk], do[0][:, sq], causal, 1 / math.sqrt(E + R), out[0][:, sq], None,
+               [grads[0][0][:, sq], grads[1][0][:, sk], grads[2][0][:, sk], grads[3][0][sk]], f'sequence {i} ')
+    assert (out[:, :, tq:] == 0).all() and (grads[0][:, :, tq:] == 0).all()
+    assert all((g[:, :, tk:] == 0).all() for g in grads[1:3]) and (grads[3][:, tk:] == 0).all()
+
+
+def test_offsets_outside_the_tensors():
+    """what they name past the rows is not there, and neither are rows past the greatest length"""
+    q, k, v, c, do = _inputs(1, 2, 200, 200, 64, 32, 64, BF, seed=4)
+    cu = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    want, _ = _step(q, k, v, c, do, cu_seqlens_q=cu(0, 90, 200), cu_seqlens_k=cu(0, 90, 200), max_seqlen_q=110, max_seqlen_k=110)
+    out, _ = _step(q, k, v, c, do, cu_seqlens_q=cu(-5, 90, 10 ** 9), cu_seqlens_k=cu(-9, 90, 2 ** 31 - 1), max_seqlen_q=110, max_seqlen_k=110)
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize('Sq,Sk', [(0, 0), (0, 5), (5, 0)])
+def test_nothing_to_do(Sq, Sk):
+    q, k, v, c, do = _inputs(1, 2, Sq, Sk, 64, 32, 64, BF)
+    out, grads = _step(q, k, v, c, do)
+    assert out.shape == (1, 2, Sq, 64) and (out == 0).all()
+    for g, t in zip(grads, (q, k, v, c)):
+        assert g.shape == t.shape and (g == 0).all()
+    q, k, v, c, do = _inputs(0, 2, 30, 40, 64, 32, 64, BF)
+    out, grads = _step(q, k, v, c, do)
+    assert out.shape == (0, 2, 30, 64) and [g.shape for g in grads] == [t.shape for t in (q, k, v, c)]
+
+
+@pytest.mark.parametrize('scale', [0.0, -0.1, 3.0, 1e-3])
+def test_scales(scale):
+    q, k, v, c, do = _inputs(1, 2, 150, 150, 128, 64, 128, BF, seed=5)
+    out, grads = _step(q, k, v, c, do, scale=scale)
+    _check(q[0], k[0], v[0], c[0], do[0], True, scale, out[0], None, [g[0] for g in grads])
+
+
+@pytest.mark.parametrize('order', [1, -1])
+def test_the_largest_scores_come_first_or_last(order):
+    """the running maximum moves at every tile, or never; scores far past the range of exp"""
+    q, k, v, c, do = _inputs(1, 2, 300, 300, 64, 32, 64, BF, seed=6)
+    size = torch.linspace(0.1, 30, 300, device=DEV)
+    size = size if order > 0 else size.flip(0)
+    k, c = (k * size[:, None]).to(BF), (c * size[:, None]).to(BF)
+    out, grads = _step(q, k, v, c, do, scale=0.3)
+    _check(q[0], k[0], v[0], c[0], do[0], True, 0.3, out[0], None, [g[0] for g in grads])
+
+
+def test_strides_alignment_and_shared_storage():
+    q, k, v, c, do = _inputs(2, 3, 130, 130, 64, 32, 64, HF, seed=7)
+    want, wgrads = _step(q, k, v, c, do)
+    odd = lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape).copy_(t)             # an unaligned base
+    wide = lambda t: torch.zeros(*t.shape[:-1], t.shape[-1] + 4, dtype=t.dtype, device=DEV)[..., 4:].copy_(t)     # rows no multiple of 16 bytes apart
+    for f in (odd, wide, lambda t: t.contiguous()):
+        out, grads = _step(f(q), f(k), f(v), f(c), f(do))
+        assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(grads, wgrads))
+    # one key and value for all heads, seen through an expanded view
+    k1, v1 = k[:, :1].expand(-1, 3, -1, -1), v[:, :1].expand(-1, 3, -1, -1)
+    out, grads = _step(q, k1, v1, c, do)
+    full, fgrads = _step(q, k1.contiguous(), v1.contiguous(), c, do)
+    assert torch.equal(out, full) and all(torch.equal(a, b) for a, b in zip(grads, fgrads))
+
+
+def test_gradient_of_a_broadcast_key():
+    """leaves that the call sees expanded get the sum of their uses"""
+    from aotriton_amd import torch_ops
+    q, k, v, c, do = _inputs(2, 3, 90, 90, 64, 32, 64, BF, seed=8)
+    c1 = c[:1].detach().requires_grad_(True)
+    out = torch_ops.latent_attention(q, k, v, c1.expand(2, -1, -1))
+    (got,) = torch.autograd.grad(out, c1, do)
+    _, grads = _step(q, k, v, c[:1].expand(2, -1, -1), do)
+    assert torch.equal(got, grads[3].sum(0, keepdim=True).to(BF))
+
+
+def test_results_do_not_change_and_other_streams():
+    x = _inputs(2, 5, 777, 777, 128, 64, 128, BF, seed=10)
+    want = _step(*x)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(4):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(_step(*x))
+    torch.cuda.synchronize()
+    for out, grads in got:
+        assert torch.equal(out, want[0]) and all(torch.equal(a, b) for a, b in zip(grads, want[1]))
+
+
+@pytest.mark.parametrize('packed', [False, True])
+def test_captured_step(packed):
+    """forward and backward in a graph, replayed on new values with eager work between the replays"""
+    sets = [_inputs(1, 4, 400, 400, 64, 32, 64, HF, seed=20 + i) for i in range(3)]
+    kw = {}
+    if packed:
+        cu = torch.tensor([0, 130, 390], dtype=torch.int32, device=DEV)
+        kw = dict(cu_seqlens_q=cu, cu_seqlens_k=cu, max_seqlen_q=300, max_seqlen_k=300)
+    static = [t.clone() for t in sets[0]]
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        _step(*static, **kw)
+    torch.cuda.current_stream().wait_stream(warm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, grads = _step(*static, **kw)
+    for values in sets + sets[:1]:
+        for s, x in zip(static, values):
+            s.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _step(*values, **kw)
+        assert torch.equal(out, want[0])
+        assert all(torch.equal(a, b) for a, b in zip(grads, want[1]))
+
+
+def test_compiled_and_traced():
+    from aotriton_amd import torch_ops
+    q, k, v, c, do = _inputs(1, 2, 100, 100, 64, 32, 64, BF, seed=11)
+    args = (q, k, v, c, None, None, 0, 0, True, 0.125)
+    torch.library.opcheck(torch.ops.aotriton_amd.latent_attention_forward, args, test_utils=('test_schema', 'test_faketensor'))
+    out, lse = _raw(q, k, v, c, True, 0.125)
+    torch.library.opcheck(torch.ops.aotriton_amd.latent_attention_backward, (do, q, k, v, c, out, lse) + args[4:],
+                          test_utils=('test_schema', 'test_faketensor'))
+
+    def step(q, k, v, c):
+        return torch_ops.latent_attention(q, k, v, c).transpose(1, 2).flatten(2)
+    torch._dynamo.reset()
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, c)]
+    a, b = step(*leaves), torch.compile(step, backend='aot_eager', fullgraph=True)(*leaves)
+    assert torch.equal(a, b)
+    up = torch.randn_like(a)
+    assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(a, leaves, up), torch.autograd.grad(b, leaves, up)))
+
+
+def test_second_derivatives_are_refused():
+    from aotriton_amd import torch_ops
+    q, k, v, c, do = _inputs(1, 1, 20, 20, 64, 32, 64, BF)
+    q = q.detach().requires_grad_(True)
+    (dq,) = torch.autograd.grad(torch_ops.latent_attention(q, k, v, c), q, do, create_graph=True)
+    with pytest.raises(RuntimeError, match='second derivatives'):
+        dq.sum().backward()
+
+
+def test_gradients_against_differences():
+    """along a direction, in steps that the types' half steps leave visible: (f(x + h d) - f(x - h d)) / 2 h.  The outputs are rounded by a
+    half step u each: the difference of the sums is off by u |out| |do| / h, and by h^2 / 6 times a third derivative, which for scores of
+    this size is below the first"""
+    from aotriton_amd import torch_ops
+    x = _inputs(1, 2, 70, 70, 64, 32, 64, HF, seed=12)
+    do = x[4].float()
+    _, grads = _step(*x)
+    f = lambda t: (torch_ops.latent_attention(*t).float() * do).sum().double()
+    g = torch.Generator().manual_seed(13)
+    for i in range(4):
+        d = torch.randn(x[i].shape, generator=g).to(DEV)
+        h = 2.0 ** -4
+        up, down = (x[i].float() + h * d).half(), (x[i].float() - h * d).half()
+        step = (up.float() - down.float()).double()          # what was added in fact
+        a, b = (list(x[:4]) for _ in range(2))
+        a[i], b[i] = up, down
+        got = float(f(a) - f(b))
+        want = float((grads[i].double() * step).sum())
+        outs = torch_ops.latent_attention(*x[:4]).double()
+        # (each of n outputs is rounded apart from the others: their sum by a few times the root of the sum of squares)
+        off = 6 * 2.0 ** -11 * float((outs.abs() * do.double().abs()).norm()) + 0.02 * float((grads[i].double() * step).norm()) + 0.01 * abs(want)
+        assert abs(got - want) < off, (i, got, want, off)
