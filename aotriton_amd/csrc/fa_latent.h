@@ -149,6 +149,8 @@ __global__ __launch_bounds__(256, 2) void latent_fwd_kernel(const LatentArgs a, 
     load_operands<T, KE>(q, qp, (int)a.sq.s * 2, rows, lane, 0, a.e);
     load_operands<T, KR>(q + KE, qp, (int)a.sq.s * 2, rows, lane, a.e, a.r);
   }
+  // (Q has to be there before the loop: left to the first use in it the compiler waits there, in every round, for all that is on its way)
+  arrived(q);
   f32x16 o[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -242,9 +244,12 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
 
   const int smem0 = lds_offset(smem);
   const int k_row = (int)a.sk.s * 2, v_row = (int)a.sv.s * 2, c_row = (int)a.c_s * 2;
-  const TileRows<EC> kt(lane, k_row, 0, a.e), vt(lane, v_row, 0, a.ev);
-  const TileRows<kLatentShared> ct(lane, c_row, 0, a.r);
+  // (what depends on the lane alone is formed anew for every tile: held, it would be spilled, and a reload waits for the tile on its way)
+  auto own_lane = [&]() __attribute__((always_inline)) { int l = threadIdx.x; asm volatile("" : "+v"(l)); return l & 63; };
   auto fetch = [&](int stage, int j) __attribute__((always_inline)) {
+    const int l = own_lane();
+    const TileRows<EC> kt(l, k_row, 0, a.e), vt(l, v_row, 0, a.ev);
+    const TileRows<kLatentShared> ct(l, c_row, 0, a.r);
     const int n = j * 64 + wave * 16, left = si.seqlen_k - n < 16 ? si.seqlen_k - n : 16;
     const int64_t at = si.k_start + n;
     const int lds = smem0 + stage * SM::STAGE + wave * 16 * 2 * EC;
@@ -277,15 +282,14 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
       if (hi == 0) { a.stat_lse[at] = lse; a.stat_delta[at] = delta; }
     }
   }
+  arrived(q);
+  arrived(dout);
   f32x16 dq[DB + RB];
 #pragma unroll
   for (int b = 0; b < DB + RB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dq[b][i] = 0.f;
   const float qs = a.sm_scale * kLog2e;
-  const int row_e = Swz<EC>::row_base(lane), row_r = Swz<kLatentShared>::row_base(lane);
-  const int tr0 = Swz<EC>::tr_base(lane, 0), tr1 = Swz<EC>::tr_base(lane, 1);
-  const int rr0 = Swz<kLatentShared>::tr_base(lane, 0), rr1 = Swz<kLatentShared>::tr_base(lane, 1);
 
   for (int j = 0; j < j1; ++j) {
     latent_meet();
@@ -297,6 +301,8 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
     const bool masked = n0 + 64 > si.seqlen_k || (a.causal && n0 + 63 > w0 + shift);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+      const int l = own_lane();
+      const int row_e = Swz<EC>::row_base(l), row_r = Swz<kLatentShared>::row_base(l);
       f32x16 s, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
@@ -313,6 +319,8 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
         if (masked && 8 * (i / 4) + i % 4 > limit) p = 0.f;
         s[i] = p * (dp[i] - delta);
       }
+      const int m = own_lane();
+      const int tr0 = Swz<EC>::tr_base(m, 0), tr1 = Swz<EC>::tr_base(m, 1), rr0 = Swz<kLatentShared>::tr_base(m, 0), rr1 = Swz<kLatentShared>::tr_base(m, 1);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const op_t ds = pack8<T>(s, t);
@@ -375,6 +383,8 @@ __global__ __launch_bounds__(256, EC == 64 ? 2 : 1) void latent_dkdv_kernel(cons
   load_operands<T, KE>(k, row_at<T>(a.k, a.sk, si, h, (int64_t)si.k_start + w0), (int)a.sk.s * 2, keys, lane, 0, a.e);
   load_operands<T, KR>(k + KE, row_at<T>(a.c, Strides3{a.c_z, 0, a.c_s}, si, 0, (int64_t)si.k_start + w0), (int)a.c_s * 2, keys, lane, 0, a.r);
   load_operands<T, KE>(v, row_at<T>(a.v, a.sv, si, h, (int64_t)si.k_start + w0), (int)a.sv.s * 2, keys, lane, 0, a.ev);
+  arrived(k);
+  arrived(v);
   f32x16 dk[DB + RB], dv[DB];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {

@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
   const int smem0 = lds_offset(smem);
   // What depends on the lane alone is formed where it is needed: held through the loop over tiles, which Q and O leave little room, it would be
   // spilled, and a reload waits for the tiles that are on their way.
-  auto own_lane = [&]() __attribute__((always_inline)) { int l = threadIdx.x & 63; asm volatile("" : "+v"(l)); return l; };
+  auto own_lane = [&]() __attribute__((always_inline)) { int l = threadIdx.x; asm volatile("" : "+v"(l)); return l & 63; };
   const int x_row = (int)ca.sk.s * 2;
   constexpr int LPR = EA / 8, RPL = 64 / LPR;      // lanes of a row, rows of an access
   while (u < u_end) {
@@ -200,7 +200,6 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     };
     // (tiles are fetched two ahead; their pages are looked up 32 tiles at a time)
     int holes = fetch(j0), holes1 = 0, holes2 = 0;
-    if (n_tiles > 1) holes1 = fetch(j0 + 1);
 
     op_t q[KE + KR];
     {
@@ -214,6 +213,9 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
         q[k] = __builtin_bit_cast(op_t, __builtin_amdgcn_raw_buffer_load_b128(rs, col < e ? at + col * 2 : kVoffOutOfRange, 0, 0));
       }
     }
+    // (Q has to be there before the loop: left to the first use in it the compiler waits there, in every round, for all that is on its way)
+    arrived(q);
+    if (n_tiles > 1) holes1 = fetch(j0 + 1);
     f32x16 o[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b) {
@@ -324,12 +326,13 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
   }
 }
 
-// The pieces of a block put together: a workgroup per 32 rows and 32 columns.  A block that one worker had is written already.
+// The pieces of a block put together: a workgroup per 32 rows and `wide` blocks of 32 columns.  A block that one worker had is written already.
+// Bound by round trips to memory for few rows (hence eight pieces at a time: 33 of them one after the other took 22 us), by the pieces' bytes for many.
 template <typename T, int EA, int RW>
-__global__ __launch_bounds__(256) void latent_cache_sum_kernel(const LatentCacheArgs a) {
+__global__ __launch_bounds__(256) void latent_cache_sum_kernel(const LatentCacheArgs a, int wide) {
   __shared__ __attribute__((aligned(8))) char words[64];
   constexpr int DB = EA / 32;
-  const int db = blockIdx.x % DB, rw = blockIdx.x / DB % RW, vb = blockIdx.x / DB / RW;
+  const int per = DB / wide, db0 = blockIdx.x % per * wide, rw = blockIdx.x / per % RW, vb = blockIdx.x / per / RW;
   // (blocks numbered with a gap or two: those of sequence z start at its first row's number divided by the rows of a block, plus z)
   auto base_of = [&](int z, const LatentSeq& s) { return (int)((int64_t)s.start * a.hq / a.block_rows) + z; };
   const LatentCut cut = latent_find(a, words, [&](const LatentCut&, int z, int64_t, const LatentSeq& s) {
@@ -340,28 +343,52 @@ __global__ __launch_bounds__(256) void latent_cache_sum_kernel(const LatentCache
   const LatentSeq s = latent_cache_seq(a, cut.z);
   const int block = vb - base_of(cut.z, s);
   const int64_t u0 = cut.first + (int64_t)block * s.tiles, u1 = u0 + s.tiles;
-  const int64_t w0 = u0 / cut.per, w1 = (u1 - 1) / cut.per;
+  const int w0 = (int)(u0 / cut.per), w1 = (int)((u1 - 1) / cut.per);
   if (w0 == w1) return;
-  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, row = block * a.block_rows + rw * 32 + (lane & 31);
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, c = lane & 31, row = block * a.block_rows + rw * 32 + c;
   if (row >= s.tokens * a.hq) return;
-  auto at = [&](int64_t w) { return (w * 2 + (w == w0 && u0 != w0 * cut.per ? 1 : 0)) * RW + rw; };
+  const int first_place = u0 != w0 * cut.per ? 1 : 0;
+  auto at = [&](int w) { return ((int64_t)w * 2 + (w == w0 ? first_place : 0)) * RW + rw; };
   const float sc = score_scale(a.sm_scale, false);
-  float m = kNegBig, l = 0.f;
-  for (int64_t w = w0; w <= w1; ++w) m = fmaxf(m, a.part_ml[at(w) * 64 + (lane & 31)]);
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t w = w0; w <= w1; ++w) {
-    const float f = fast_exp2((a.part_ml[at(w) * 64 + (lane & 31)] - m) * sc);
-    l += f * a.part_ml[at(w) * 64 + 32 + (lane & 31)];
-    x += f * *reinterpret_cast<const f32x4*>(a.part_o + at(w) * (DB * 1024) + db * 1024 + tid * 4);
-  }
-  const float f = l == 0.f ? 0.f : 1.0f / l;
-  const int token = row / a.hq, head = row - token * a.hq, col = 32 * db + 8 * (tid >> 6) + 4 * hi;
-  typename Traits<T>::q4_t y;
+  const int token = row / a.hq, head = row - token * a.hq;
+  T* out = reinterpret_cast<T*>(a.out) + (int64_t)(s.start + token) * a.o_row + (int64_t)head * a.o_head;
+  for (int db = db0; db < db0 + wide; ++db) {
+    float m = kNegBig, l = 0.f;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    constexpr int N = 8;
+    for (int w = w0; w <= w1; w += N) {
+      float pm[N], pl[N];
+      f32x4 px[N];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(x[r] * f);
-  if (col < a.cache.head_dim_v)
-    *reinterpret_cast<typename Traits<T>::q4_t*>(reinterpret_cast<T*>(a.out) + (int64_t)(s.start + token) * a.o_row + (int64_t)head * a.o_head + col) = y;
-  if (a.lse != nullptr && db == 0 && tid < 32) a.lse[(int64_t)(s.start + token) * a.hq + head] = l == 0.f ? __builtin_inff() : __builtin_fmaf(m, sc, fast_log2(l)) * kLn2;
+      for (int i = 0; i < N; ++i) {
+        const int64_t p = at(w + i < w1 ? w + i : w1);
+        pm[i] = a.part_ml[p * 64 + c];
+        pl[i] = a.part_ml[p * 64 + 32 + c];
+        px[i] = *reinterpret_cast<const f32x4*>(a.part_o + p * (DB * 1024) + db * 1024 + tid * 4);
+      }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < N; ++i) top = fmaxf(top, pm[i]);
+      const float f = fast_exp2((m - top) * sc);
+      m = top;
+      l *= f;
+      x *= f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float g = w + i <= w1 ? fast_exp2((pm[i] - top) * sc) : 0.f;
+        l += g * pl[i];
+        if (w + i <= w1) x += g * px[i];
+      }
+    }
+    const float f = l == 0.f ? 0.f : 1.0f / l;
+    const int col = 32 * db + 8 * (tid >> 6) + 4 * hi;
+    typename Traits<T>::q4_t y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(x[r] * f);
+    if (col < a.cache.head_dim_v) *reinterpret_cast<typename Traits<T>::q4_t*>(out + col) = y;
+    if (a.lse != nullptr && db == 0 && tid < 32)
+      a.lse[(int64_t)(s.start + token) * a.hq + head] = l == 0.f ? __builtin_inff() : __builtin_fmaf(m, sc, fast_log2(l)) * kLn2;
+  }
 }
 
 template <typename T, int EA, int RW> hipError_t launch_latent_cache_rows(const LatentCacheArgs& a, hipStream_t s) {
@@ -371,7 +398,9 @@ template <typename T, int EA, int RW> hipError_t launch_latent_cache_rows(const 
   hipLaunchKernelGGL((latent_cache_kernel<T, EA, RW>), dim3((unsigned)a.workers), dim3(256), LatentCacheSmem<EA>::BYTES, s, a);
   if (a.part_o != nullptr && a.cache.sequences > 0) {
     const int64_t blocks = (int64_t)a.rows * a.hq / a.block_rows + a.cache.sequences;
-    hipLaunchKernelGGL((latent_cache_sum_kernel<T, EA, RW>), dim3((unsigned)(blocks * RW * (EA / 32))), dim3(256), 0, s, a);
+    int wide = 1;      // (two rounds of workgroups, or nearly)
+    while (wide < EA / 32 && blocks * RW * (EA / 32) / wide > 4096) wide *= 2;
+    hipLaunchKernelGGL((latent_cache_sum_kernel<T, EA, RW>), dim3((unsigned)(blocks * RW * (EA / 32 / wide))), dim3(256), 0, s, a, wide);
   }
   return hipGetLastError();
 }

@@ -10,6 +10,12 @@ __device__ __forceinline__ void load_word_to_lds(u32x4_t rsrc, int voff, int lds
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(lds), "v"(voff), "s"(rsrc) : "m0");
 }
 
+// What was loaded is in its registers from here on.
+template <typename V, int N> __device__ __forceinline__ void arrived(V (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
+}
+
 // Maximum and sum of a lane's row; the sum is over the lane's half of the keys until cross_sum.
 // The maximum is a reference: it moves, and O with it, only where a score passes it by more than 2^kSlack (P is then up to 2^kSlack, which
 // both types hold without losing a bit; sums are fp32).  O lies in accumulation registers, where a product costs three
