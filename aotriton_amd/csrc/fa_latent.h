@@ -178,7 +178,14 @@ __global__ __launch_bounds__(256, 2) void latent_fwd_kernel(const LatentArgs a, 
     }
     const int n0 = j * 64;
     const bool masked = n0 + 64 > si.seqlen_k || (a.causal && n0 + 63 > w0 + shift);
-    sm.step(s, masked, see - n0 - 4 * hi, [&](float f) __attribute__((always_inline)) {
+    if (masked) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * b + 8 * (i / 4) + i % 4 > see - n0 - 4 * hi) s[b][i] = sm.hidden();
+    }
+    sm.step(s, [&](float f) __attribute__((always_inline)) {
 #pragma unroll
       for (int b = 0; b < DB; ++b)
 #pragma unroll

@@ -186,9 +186,10 @@ int fa_latent_cache_attn(const fa_latent_cache_params* p, void* hip_stream, fa_a
   a.o_row = (int64_t)p->Out.strides[1]; a.o_head = (int64_t)p->Out.strides[2];
   a.rows = (int32_t)rows; a.hq = (int32_t)hq;
   a.sm_scale = p->Sm_scale;
-  // slots are counted in 32 bits, and a wave reaches its 32 rows of Q with 32-bit offsets; (rows, heads) pairs of a sequence are 31 bits
-  if ((p->table.sizes[1] << c.page_shift) > 1ull << 29 || hq > 65536) return FA_ERROR_NOT_SUPPORTED;
-  if ((double)a.q_row * 32 + (double)a.q_head * (double)hq + kLatent >= (double)(1 << 29) || (double)rows * (double)hq >= (double)(1 << 30)) return FA_ERROR_NOT_SUPPORTED;
+  // slots are counted in 32 bits, and a block's 128 rows of Q and Out are reached with 32-bit offsets; (rows, heads) pairs of a sequence are 31 bits
+  if ((p->table.sizes[1] << c.page_shift) > 1ull << 29 || hq > 65536 || (double)rows * (double)hq >= (double)(1 << 30)) return FA_ERROR_NOT_SUPPORTED;
+  auto near = [&](int64_t row, int64_t head) { return (double)row * (double)(128 / hq + 1) + (double)head * (double)hq + kLatent < (double)(1 << 29); };
+  if (!near(a.q_row, a.q_head) || !near(rows > 1 ? a.o_row : 0, hq > 1 ? a.o_head : 0)) return FA_ERROR_NOT_SUPPORTED;
   if ((e = fa_check_gpu(hip_stream)) != FA_SUCCESS) return e;
   if (rows == 0) return FA_SUCCESS;
 
@@ -201,13 +202,15 @@ int fa_latent_cache_attn(const fa_latent_cache_params* p, void* hip_stream, fa_a
   if (!fits((double)blocks * 4 * 16)) return FA_ERROR_NOT_SUPPORTED;
   const int64_t room = (int64_t)c.columns << c.page_shift;
   const int64_t tiles = (std::min<int64_t>(p->max_length, room) + (int64_t)rows + 31) / 32 + 1;
+  a.blocks = (int32_t)blocks;
   a.least = 4;
   a.workers = (int32_t)std::max<int64_t>(1, std::min<int64_t>(num_cu, blocks * ((tiles + a.least - 1) / a.least)));
   const int64_t places = 2 * (int64_t)a.workers * (a.block_rows / 32), o_bytes = places * 32 * d * 4;
-  void* scratch = alloc != nullptr && a.workers > 1 ? alloc->alloc(alloc, (uint64_t)(o_bytes + places * 64 * 4)) : nullptr;
+  void* scratch = alloc != nullptr && a.workers > 1 ? alloc->alloc(alloc, (uint64_t)(o_bytes + places * 64 * 4 + blocks * (int64_t)sizeof(fa::LatentHead))) : nullptr;
   if (scratch != nullptr) {
     a.part_o = static_cast<float*>(scratch);
     a.part_ml = reinterpret_cast<float*>(static_cast<char*>(scratch) + o_bytes);
+    a.heads = reinterpret_cast<fa::LatentHead*>(a.part_ml + places * 64);
   } else if (a.workers > 1) {
     return FA_ERROR_OUT_OF_MEMORY;
   }

@@ -36,6 +36,10 @@ struct LatentBwdArgs : LatentArgs {
   int64_t part_rows;             // keys of a (batch, head) slab of part_c
 };
 
+// A block of rows that lies in several pieces: the first of them (two times its worker, plus its place there), how many (0: the block is one
+// piece), first row of the sequence, number in it, rows of it.
+struct LatentHead { int32_t piece, pieces, start, block, rows; };
+
 // Attention over a cache of latent rows (CacheArgs: K is the cache, of one head; head_dim_v of its columns are the values).
 struct LatentCacheArgs {
   const void* q; void* out; float* lse;
@@ -49,6 +53,8 @@ struct LatentCacheArgs {
   // part_o, two places for every worker.
   int32_t block_rows, workers, least;
   float* part_o; float* part_ml;
+  LatentHead* heads;             // of the blocks, `blocks` of them (fa_latent_cache.h: latent_block)
+  int32_t blocks;
 };
 
 // compiled columns of K and V (64 or 128; of the shared part 64)

@@ -20,7 +20,7 @@ constexpr int kLatentTail = 64;
 template <int EA> struct LatentCacheSmem {
   static constexpr int A = 32 * EA * 2, STAGE = A + 32 * kLatentTail * 2, STAGES = 4;
   static constexpr int LIST = STAGES * STAGE;           // words of latent_find
-  static constexpr int BYTES = LIST + 64;
+  static constexpr int BYTES = LIST + 128;
 };
 
 // A sequence as the list of work has it: `blocks` blocks of rows, `tiles` tiles each (one at least, for rows that see nothing).
@@ -42,14 +42,18 @@ __device__ __forceinline__ LatentSeq latent_cache_seq(const LatentCacheArgs& a, 
   return s;
 }
 
+// Number of a sequence's first block, with a gap or two: that of its first row, divided by the rows of a block, and one more for every sequence in
+// front.  LatentCacheArgs::blocks bounds them.
+__device__ __forceinline__ int latent_block(const LatentCacheArgs& a, int z, int start) { return (int)((int64_t)start * a.hq / a.block_rows) + z; }
+
 // The cut of the list: its length, that of a piece, and of the sequence looked for its number and where it starts in the list.  `mine(z, first
 // unit, sequence)` says which one that is.  All 256 threads call this.
-struct LatentCut { int64_t per, total, first; int z; };
+struct LatentCut { int64_t per, total, first; int z; LatentSeq seq; };
 template <typename Mine>
 __device__ __forceinline__ LatentCut latent_find(const LatentCacheArgs& a, char* words, Mine mine) {
   int64_t* sums = reinterpret_cast<int64_t*>(words);      // of the four waves; then the answer
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.cache.sequences;
-  LatentCut cut{0, 0, 0, -1};
+  LatentCut cut{0, 0, 0, -1, {}};
   int64_t base = 0;
   LatentSeq s;
   int64_t before = 0;
@@ -88,12 +92,14 @@ __device__ __forceinline__ LatentCut latent_find(const LatentCacheArgs& a, char*
     if (z < n && s.units() > 0 && mine(cut, z, before, s)) {
       sums[4] = before;
       sums[5] = z;
+      *reinterpret_cast<LatentSeq*>(sums + 6) = s;
     }
     if (n > 256) __syncthreads();
   }
   __syncthreads();
   cut.first = sums[4];
   cut.z = (int)sums[5];
+  cut.seq = *reinterpret_cast<const LatentSeq*>(sums + 6);
   return cut;
 }
 
@@ -106,7 +112,8 @@ template <int DB> __device__ __forceinline__ void settle(f32x16 (&o)[DB]) {
   for (int b = 0; b < DB; ++b) asm volatile("" : "+a"(o[b]));
 }
 
-template <typename T, int EA, int RW>
+// kCut: rows have fewer than EA columns; those past them are zero.
+template <typename T, int EA, int RW, bool kCut>
 __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheArgs a) {
   using Tr = Traits<T>;
   using op_t = typename Tr::op_t;
@@ -142,6 +149,12 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
   });
   int64_t u = worker * cut.per;
   const int64_t u_end = u + cut.per < cut.total ? u + cut.per : cut.total;
+  // (for the kernel that puts the pieces together: a block's head is written by the worker that begins it, and where blocks are numbered with a
+  // gap by the one that begins the block in front, or the first)
+  auto put_heads = [&](int from, int to) {
+    for (int i = (from < 0 ? 0 : from) + (int)threadIdx.x; i < to && i < a.blocks; i += 256) a.heads[i] = LatentHead{0, 0, 0, 0, 0};
+  };
+  if (a.heads != nullptr && cut.total == 0 && worker == 0) put_heads(0, a.blocks);
   if (u >= u_end) return;
   int z = __builtin_amdgcn_readfirstlane(cut.z);
   int64_t first = cut.first;
@@ -149,11 +162,12 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
   const int smem0 = lds_offset(smem);
   // What depends on the lane alone is formed where it is needed: held through the loop over tiles, which Q and O leave little room, it would be
   // spilled, and a reload waits for the tiles that are on their way.
-  auto own_lane = [&]() __attribute__((always_inline)) { int l = threadIdx.x; asm volatile("" : "+v"(l)); return l & 63; };
+  auto own_lane = [&]() __attribute__((always_inline)) { int l = threadIdx.x; if constexpr (kFull) asm volatile("" : "+v"(l)); return l & 63; };
   const int x_row = (int)ca.sk.s * 2;
   constexpr int LPR = EA / 8, RPL = 64 / LPR;      // lanes of a row, rows of an access
-  while (u < u_end) {
-    LatentSeq s = latent_cache_seq(a, z);
+  LatentSeq s = cut.seq;
+  for (bool again = false; u < u_end; again = true) {
+    if (again) s = latent_cache_seq(a, z);
     s.start = __builtin_amdgcn_readfirstlane(s.start); s.tokens = __builtin_amdgcn_readfirstlane(s.tokens);
     s.length = __builtin_amdgcn_readfirstlane(s.length); s.end = __builtin_amdgcn_readfirstlane(s.end);
     s.tiles = __builtin_amdgcn_readfirstlane(s.tiles); s.blocks = __builtin_amdgcn_readfirstlane(s.blocks);
@@ -162,7 +176,9 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
       ++z;
       continue;
     }
-    const int block = (int)((u - first) / s.tiles), j0 = (int)((u - first) % s.tiles);
+    // (a division of 64 bits takes a microsecond)
+    const int64_t rel = u - first;
+    const int block = rel >> 32 == 0 ? (int)((uint32_t)rel / (uint32_t)s.tiles) : (int)(rel / s.tiles), j0 = (int)(rel - (int64_t)block * s.tiles);
     const int n_tiles = (int)(u_end - u < s.tiles - j0 ? u_end - u : s.tiles - j0);
     const int rows = s.tokens * a.hq, w0 = block * a.block_rows + rw * 32, w_last = w0 + 31 < rows ? w0 + 31 : rows - 1;
     const bool row_ok = w0 + c < rows;
@@ -170,52 +186,104 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     // the last slot that the row sees, that the wave's first and last rows see
     auto sees = [&](int t) { const int n = s.length + t; return n < s.end ? n : s.end - 1; };
     const int see = sees(token);
-    const int see_least = __builtin_amdgcn_readfirstlane(sees(w0 / a.hq)), see_most = __builtin_amdgcn_readfirstlane(sees(w_last / a.hq));
+    const int see_least = __builtin_amdgcn_readfirstlane(sees(w0 / a.hq));
+    const int see_most = __builtin_amdgcn_readfirstlane(sees(w_last / a.hq));
     const int j1 = j0 + n_tiles, wave_end = w0 < rows ? see_most / 32 + 1 : 0;
 
     auto slot_of = [&](int entry) { const int n = (j0 + entry / 2) * 32 + entry % 2 * 16; return entry < 2 * n_tiles && n < s.end ? n : -1; };
     PageRun<decltype(slot_of)> pages(ca, z, lane, slot_of);
     const char* xbase = reinterpret_cast<const char*>(ca.k);
-    auto fetch = [&](int j) __attribute__((always_inline)) {      // returns which of the tile's halves have no page
+    auto stage_of = [&](int j) { return smem0 + ((j - j0) & (SM::STAGES - 1)) * SM::STAGE; };
+    constexpr int kLoads = 8 / RPL + 1, kPieces = 4 / RPL + 1;      // of a tile, and the pairs they come in
+    u32x4_t f_rs;
+    int f_lds;
+    auto fetch_begin = [&](int j) __attribute__((always_inline)) {      // returns which of the tile's halves have no page
       pages.to((j - j0) * 2);
       const int n = j * 32 + wave * 8, left = s.end - n < 8 ? s.end - n : 8;
       const int p = pages.at((j - j0) * 2 + wave / 2);
       const char* from = xbase + ((int64_t)(p < 0 ? 0 : p) * ca.sk.z + (int64_t)(n & ((1 << ca.page_shift) - 1)) * ca.sk.s) * 2;
-      const u32x4_t rs = wave_rsrc_words(from, p < 0 ? 0 : rows_extent(left, x_row, e * 2));
-      const int lds = smem0 + ((j - j0) & (SM::STAGES - 1)) * SM::STAGE, lds_a = lds + wave * 8 * EA * 2;
-      const int l = own_lane(), lrow = l / LPR, lch = l % LPR;
-#pragma unroll
-      for (int i = 0; i < 8 / RPL; i += 2) {
-        int voff[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int ch = lch ^ Swz<EA>::f((i + t) * RPL + lrow + 8 * (wave & 1));
-          voff[t] = ch * 8 < e ? lrow * x_row + ch * 16 : kVoffOutOfRange;
-        }
-        load_to_lds(rs, voff[0], i * RPL * x_row, lds_a + i * 1024, voff[1], (i + 1) * RPL * x_row, lds_a + (i + 1) * 1024);
-      }
-      const int ch = (l % 8) ^ Swz<kLatentTail>::f(8 * (wave & 1) + l / 8);      // (a wave's eight rows are the first or second of 16)
-      load_to_lds1(rs, EA + ch * 8 < e ? l / 8 * x_row + (EA + ch * 8) * 2 : kVoffOutOfRange, lds + SM::A + wave * 1024);
+      f_rs = wave_rsrc_words(from, p < 0 ? 0 : rows_extent(left, x_row, e * 2));      // (a page that is not there: zeros, no traffic)
+      f_lds = stage_of(j);
       return pages.holes((j - j0) * 2) & 3;
     };
-    // (tiles are fetched two ahead; their pages are looked up 32 tiles at a time)
-    int holes = fetch(j0), holes1 = 0, holes2 = 0;
-
-    op_t q[KE + KR];
-    {
-      const int t0 = w0 < rows ? w0 / a.hq : 0, t1 = w_last / a.hq;
-      const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(s.start + t0) * a.q_row;
-      const auto rs = wave_rsrc(qp, w0 < rows ? (int)(((t1 - t0) * a.q_row + (a.hq - 1) * a.q_head + e) * 2) : 0);
-      const int at = row_ok ? (int)(((token - t0) * a.q_row + head * a.q_head) * 2) : kVoffOutOfRange;
+    auto fetch_piece = [&](int i) __attribute__((always_inline)) {
+      const int l = own_lane();
+      if (i < kPieces - 1) {
+        // a lane's piece of its row: the lane's number, swizzled by the row's
+        const int lrow = l / LPR, base = (l % LPR) ^ Swz<EA>::f(lrow + 8 * (wave & 1)), lds = f_lds + wave * 8 * EA * 2;
+        static_assert(RPL == 1 || RPL == 2, "f of a row is that of its access and that of its place in it");
+        int voff[2];
 #pragma unroll
-      for (int k = 0; k < KE + KR; ++k) {
-        const int col = 16 * k + 8 * hi;
-        q[k] = __builtin_bit_cast(op_t, __builtin_amdgcn_raw_buffer_load_b128(rs, col < e ? at + col * 2 : kVoffOutOfRange, 0, 0));
+        for (int t = 0; t < 2; ++t) voff[t] = lrow * x_row + ((base ^ Swz<EA>::f((2 * i + t) * RPL)) << 4);
+        if (kCut) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if ((base ^ Swz<EA>::f((2 * i + t) * RPL)) * 8 >= e) voff[t] = kVoffOutOfRange;
+        }
+        load_to_lds(f_rs, voff[0], 2 * i * RPL * x_row, lds + 2 * i * 1024, voff[1], (2 * i + 1) * RPL * x_row, lds + (2 * i + 1) * 1024);
+      } else {
+        const int ch = (l % 8) ^ Swz<kLatentTail>::f(8 * (wave & 1) + l / 8);      // (a wave's eight rows are the first or second of 16)
+        load_to_lds1(f_rs, EA + ch * 8 < e ? l / 8 * x_row + (EA + ch * 8) * 2 : kVoffOutOfRange, f_lds + SM::A + wave * 1024);
+      }
+    };
+    auto fetch = [&](int j) __attribute__((always_inline)) {
+      const int holes = fetch_begin(j);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) fetch_piece(i);
+      return holes;
+    };
+    auto k_read = [&](int X, int at_e, int at_r, int k) __attribute__((always_inline)) {
+      return k < KE ? lds_read<op_t>((at_e ^ ((k & 7) << 5)) + X + (k >> 3) * 256) : lds_read<op_t>((at_r ^ ((k - KE) << 5)) + X + SM::A);
+    };
+    // Q passes through the last RW stages as tiles of 32 rows, as the latent rows do: whole rows of memory, each once (as a lane's row in pieces
+    // straight into registers it took 11 us for 128 rows).
+    {
+      const int r0 = block * a.block_rows, tb = r0 / a.hq, t_end = (r0 + a.block_rows - 1 < rows ? r0 + a.block_rows - 1 : rows - 1) / a.hq;
+      const u32x4_t rs = wave_rsrc_words(reinterpret_cast<const T*>(a.q) + (int64_t)(s.start + tb) * a.q_row,
+                                         (int)(((t_end - tb) * a.q_row + (a.hq - 1) * a.q_head + e) * 2));
+      const int q_row = (int)a.q_row * 2, q_head = (int)a.q_head * 2;
+#pragma unroll
+      for (int g = 0; g < RW; ++g) {
+        const int R = r0 + g * 32 + wave * 8, lds = smem0 + (SM::STAGES - RW + g) * SM::STAGE, lds_a = lds + wave * 8 * EA * 2;
+        const int l = own_lane(), lrow = l / LPR, base = (l % LPR) ^ Swz<EA>::f(lrow + 8 * (wave & 1)), tail_ch = (l % 8) ^ Swz<kLatentTail>::f(8 * (wave & 1) + l / 8);
+        int t = __builtin_amdgcn_readfirstlane(R / a.hq), h = R - t * a.hq, off[8], tail = kVoffOutOfRange;
+        t -= tb;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          off[i] = R + i < rows ? t * q_row + h * q_head : -1;
+          if (l / 8 == i && off[i] >= 0 && EA + tail_ch * 8 < e) tail = off[i] + (EA + tail_ch * 8) * 2;
+          if (++h == a.hq) { h = 0; ++t; }
+        }
+#pragma unroll
+        for (int i = 0; i < 8 / RPL; i += 2) {
+          int voff[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int at = RPL == 1 ? off[i + k] : lrow ? off[(i + k) * RPL + RPL - 1] : off[(i + k) * RPL], ch = base ^ Swz<EA>::f((i + k) * RPL);
+            voff[k] = at >= 0 && (!kCut || ch * 8 < e) ? at + (ch << 4) : kVoffOutOfRange;
+          }
+          load_to_lds(rs, voff[0], 0, lds_a + i * 1024, voff[1], 0, lds_a + (i + 1) * 1024);
+        }
+        load_to_lds1(rs, tail, lds + SM::A + wave * 1024);
       }
     }
-    // (Q has to be there before the loop: left to the first use in it the compiler waits there, in every round, for all that is on its way)
+    // (pages are looked up 32 tiles at a time; as many tiles as Q leaves room for are on their way with it)
+    int holes = 0, holes1 = 0, holes2 = 0;      // of this tile, the next, the one behind it
+    if (RW <= 3) holes = fetch(j0);
+    if (RW <= 2) holes1 = fetch(j0 + 1);
+    if (RW <= 1) holes2 = fetch(j0 + 2);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((SM::STAGES - RW) * kLoads) : "memory");
+    op_t q[KE + KR];
+    {
+      const int X = smem0 + (SM::STAGES - RW + rw) * SM::STAGE, at_e = Swz<EA>::row_base(own_lane()), at_r = Swz<kLatentTail>::row_base(own_lane());
+#pragma unroll
+      for (int k = 0; k < KE + KR; ++k) q[k] = k_read(X, at_e, at_r, k);
+    }
     arrived(q);
-    if (n_tiles > 1) holes1 = fetch(j0 + 1);
+    if (RW > 1) asm volatile("s_barrier" ::: "memory");      // (all waves have their rows)
+    if (RW > 3) holes = fetch(j0);
+    if (RW > 2) holes1 = fetch(j0 + 1);
+    if (RW > 1) holes2 = fetch(j0 + 2);
     f32x16 o[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b) {
@@ -224,74 +292,147 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     }
     RowSoftmax sm(a.sm_scale);
 
-    for (int j = j0; j < j1; ++j, holes = holes1, holes1 = holes2) {
-      constexpr int kLoads = 8 / RPL + 1;      // of a tile
-      if (j + 1 < j1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kLoads) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (j + 2 < j1) holes2 = fetch(j + 2);
-      if (j >= wave_end) continue;
-      // (a few operands at a time are on their way: left to itself the compiler keeps dozens)
-      const int X = smem0 + ((j - j0) & (SM::STAGES - 1)) * SM::STAGE;
-      const int at_e = Swz<EA>::row_base(own_lane()), at_r = Swz<kLatentTail>::row_base(own_lane());
-      auto k_read = [&](int k) __attribute__((always_inline)) {
-        return k < KE ? lds_read<op_t>((at_e ^ ((k & 7) << 5)) + X + (k >> 3) * 256) : lds_read<op_t>((at_r ^ ((k - KE) << 5)) + X + SM::A);
-      };
-      constexpr int kRing = 5;
-      f32x16 x[1];
-      op_t xa[kRing];
+    constexpr int kRing = 5;      // operands on their way: left to itself the compiler keeps dozens
+    f32x16 x[1];
+    op_t p[2], p_next[2], ring[kRing];
+    // x = S of tile j, with the pieces of the tile that is being fetched behind its MFMAs
+    auto scores = [&](int j, auto fetching) __attribute__((always_inline)) {
+      const int X = stage_of(j), at_e = Swz<EA>::row_base(own_lane()), at_r = Swz<kLatentTail>::row_base(own_lane());
+      auto read = [&](int k) __attribute__((always_inline)) { return k_read(X, at_e, at_r, k); };
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[0][i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < kRing - 1; ++k) xa[k] = k_read(k);
+      for (int k = 0; k < kRing - 1; ++k) ring[k] = read(k);
 #pragma unroll
       for (int k = 0; k < KE + KR; ++k) {
-        if (k + kRing - 1 < KE + KR) xa[(k + kRing - 1) % kRing] = k_read(k + kRing - 1);
-        x[0] = Tr::mfma(xa[k % kRing], q[k], x[0]);
+        if (k + kRing - 1 < KE + KR) ring[(k + kRing - 1) % kRing] = read(k + kRing - 1);
+        x[0] = Tr::mfma(ring[k % kRing], q[k], k == 0 ? f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f} : x[0]);
+        if (decltype(fetching)::value && k % 3 == 2 && k / 3 < kPieces) fetch_piece(k / 3);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (holes != 0) {
+    };
+    // scores that a lane's row does not see of tile j (x[i] is key 8 (i / 4) + 4 hi + i % 4), where there may be some
+    auto hide = [&](int j, int hol, float to) __attribute__((always_inline)) {
+      if (hol == 0 && j * 32 + 31 <= see_least) return;
+      const int n = see - j * 32 - 4 * hi, limit[2] = {hol & 1 ? -1 : n, hol & 2 ? -1 : n};
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (holes >> (i / 8) & 1) x[0][i] = -__builtin_inff();
-      }
-      sm.step(x, j * 32 + 31 > see_least, see - j * 32 - 4 * hi, [&](float f) __attribute__((always_inline)) {
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i / 4) + i % 4 > limit[i / 8]) x[0][i] = to;
+    };
+    // P of tile j from x, with the rows' maxima as they are after it
+    auto full_step = [&](int j, int hol, auto rescale) __attribute__((always_inline)) {
+      hide(j, hol, sm.hidden());
+      sm.step(x, rescale);
 #pragma unroll
-        for (int b = 0; b < DB; ++b) {
-          if constexpr (kFull) asm volatile("s_nop 15\n\ts_nop 7" : "+a"(o[b]));
-          f32x16 t = o[b];
-          t *= f;
-          if constexpr (kFull) asm volatile("" : "+v"(t));
-          o[b] = t;
-          if constexpr (kFull) asm volatile("s_nop 3" : "+a"(o[b]));
-        }
-      });
-      op_t p[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) p[t] = pack8<T>(x[0], t);
-      if constexpr (kFull) asm volatile("s_nop 1" : "+v"(p[0]), "+v"(p[1]));
+      for (int t = 0; t < 2; ++t) p_next[t] = pack8<T>(x[0], t);
+    };
+    // O += X(j)^T P(j)^T, and P of tile j + 1 from x behind its MFMAs, against the maxima that the rows have (an element's three parts behind
+    // different ones, as in fa_fwd_wide.h); returns whether they will do
+    auto values = [&](int j, int hol) __attribute__((always_inline)) {
+      constexpr int N = 2 * DB, kLag = 2;
       // (the group's first block of columns: of its number the lower two bits are swizzled)
       const int first_block = cg * DB, block_xor = (first_block & 3) << 6, block_off = (first_block >> 2) * 256;
       const int at_0 = (Swz<EA>::tr_base(own_lane(), 0) ^ block_xor) + block_off, at_1 = (Swz<EA>::tr_base(own_lane(), 1) ^ block_xor) + block_off;
-      auto v_read = [&](int i) __attribute__((always_inline)) {
+      const int X = stage_of(j);
+      auto read = [&](int i) __attribute__((always_inline)) {
         const int b = i % DB, off = X + i / DB * 16 * Swz<EA>::ROWB + (b >> 2) * 256;
         const auto lo = __builtin_bit_cast(typename Tr::q4_t, lds_read_tr_at((at_0 ^ ((b & 3) << 6)) + off));
         const auto up = __builtin_bit_cast(typename Tr::q4_t, lds_read_tr_at((at_1 ^ ((b & 3) << 6)) + off));
         return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
       };
+      hide(j + 1, hol, -__builtin_inff());
+      const float msc = sm.m * sm.sc;
+      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < kRing - 1; ++i) xa[i] = v_read(i);
+      for (int i = 0; i < kRing - 1 && i < N; ++i) ring[i] = read(i);
 #pragma unroll
-      for (int i = 0; i < 2 * DB; ++i) {
-        if (i + kRing - 1 < 2 * DB) xa[(i + kRing - 1) % kRing] = v_read(i + kRing - 1);
-        if constexpr (kFull) mfma_acc<T>(o[i % DB], xa[i % kRing], p[i / DB]);
-        else o[i % DB] = Tr::mfma(xa[i % kRing], p[i / DB], o[i % DB]);
+      for (int i = 0; i < N; ++i) {
+        if (i + kRing - 1 < N) ring[(i + kRing - 1) % kRing] = read(i + kRing - 1);
+        if constexpr (kFull) mfma_acc<T>(o[i % DB], ring[i % kRing], p[i / DB]);
+        else o[i % DB] = Tr::mfma(ring[i % kRing], p[i / DB], o[i % DB]);
+#pragma unroll
+        for (int E = first_of(i, 16 + kLag, N); E < first_of(i + 1, 16 + kLag, N); ++E) {
+          if (E < 16) {
+            x[0][E] = __builtin_fmaf(x[0][E], sm.sc, -msc);
+          }
+          if (E >= kLag / 2 && E < 16 + kLag / 2) x[0][E - kLag / 2] = fast_exp2(x[0][E - kLag / 2]);
+          if (E >= kLag) {
+            const int e2 = E - kLag;
+            sum += x[0][e2];
+            if (e2 & 1) {
+              const typename Tr::p2_t p2 = Tr::cvt2(x[0][e2 - 1], x[0][e2]);
+              p_next[e2 / 8][e2 % 8 - 1] = p2[0];
+              p_next[e2 / 8][e2 % 8] = p2[1];
+            }
+          }
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
+      // (also catches inf and NaN)
+      if ((sm.prescale && hol != 3) || __builtin_amdgcn_ballot_w64(!(sum < 4096.f)) != 0) return false;
+      sm.l += sum;
+      return true;
+    };
+    using yes = std::true_type;
+    using no = std::false_type;
+    const int jw = j1 < wave_end ? j1 : wave_end;      // the wave's tiles end here
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(2 * kLoads) : "memory");
+    if (j0 < jw) {
+      scores(j0, no{});
+      full_step(j0, holes, [](float) {});
     }
+    // In a round: S of the next tile, then the values of this one with the exponentials of the next behind them.  Tiles are fetched three
+    // ahead, into the stage of the one before this; those behind the last are empty.
+    for (int j = j0; j < j1; ++j) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) p[t] = p_next[t];
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kLoads) : "memory");
+      const int holes3 = fetch_begin(j + 3);
+      if (j + 1 < jw) {
+        scores(j + 1, yes{});
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) fetch_piece(i);
+      }
+      if (j < jw && !values(j, j + 1 < jw ? holes1 : 3)) {
+        scores(j + 1, no{});
+        full_step(j + 1, holes1, [&](float f) __attribute__((always_inline)) {
+#pragma unroll
+          for (int b = 0; b < DB; ++b) {
+            if constexpr (kFull) asm volatile("s_nop 15\n\ts_nop 7" : "+a"(o[b]));
+            f32x16 t = o[b];
+            t *= f;
+            if constexpr (kFull) asm volatile("" : "+v"(t));
+            o[b] = t;
+            if constexpr (kFull) asm volatile("s_nop 3" : "+a"(o[b]));
+          }
+        });
+      }
+      holes1 = holes2;
+      holes2 = holes3;
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (all waves have left the stages)
     if constexpr (kFull) settle(o);
     // (the row once more, as above)
     const int tail_lane = own_lane(), up = tail_lane >> 5, out_row = w0 + (tail_lane & 31);
     const float sum = cross_sum(sm.l);
+    if (a.heads != nullptr && j0 == 0) {
+      const int at = latent_block(a, z, s.start) + block;
+      if (at < a.blocks && threadIdx.x == 0) {
+        a.heads[at] = n_tiles < s.tiles ? LatentHead{(int)(worker * 2 + (u == worker * cut.per ? 0 : 1)), (int)((u + s.tiles - 1) / cut.per - worker) + 1, s.start, block, rows}
+                                        : LatentHead{0, 0, 0, 0, 0};
+      }
+      if (u == 0) put_heads(0, at);
+      if (block == s.blocks - 1) {
+        int next = a.blocks;
+        for (int y = z + 1; y < ca.sequences; ++y) {
+          const LatentSeq t = latent_cache_seq(a, y);
+          if (t.blocks > 0) {
+            next = latent_block(a, y, t.start);
+            break;
+          }
+        }
+        put_heads(at + 1, next);
+      }
+    }
     if (n_tiles < s.tiles) {      // a piece: the first of the worker, or its last
       const int place = u == worker * cut.per ? 0 : 1;
       const int64_t at = (worker * 2 + place) * RW + rw;
@@ -303,26 +444,36 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
         __builtin_amdgcn_sched_barrier(0);
       }
       if (cg == 0) a.part_ml[at * 64 + tail_lane] = tail_lane < 32 ? sm.m : sum;
-    } else if (out_row < rows) {
+    } else {
+      // O passes through the wave's stage, so that rows go out whole (as a lane's row in pieces of 8 bytes: 19 us for 128 rows)
+      constexpr int W = DB * 32, ROW = W * 2 + 16, LPO = W / 8, RPO = 64 / LPO;
+      static_assert(32 * ROW <= SM::STAGE, "the rows fit");
+      const int r = out_row < rows ? out_row : rows - 1, t = r / a.hq, h = r - t * a.hq, t0 = __builtin_amdgcn_readfirstlane(t);
       const float f = sum == 0.f ? 0.f : 1.0f / sum;
-      const int t = out_row / a.hq, h = out_row - t * a.hq;
-      T* to = reinterpret_cast<T*>(a.out) + (int64_t)(s.start + t) * a.o_row + (int64_t)h * a.o_head;
+      const int place = smem0 + wave * SM::STAGE;
 #pragma unroll
       for (int b = 0; b < DB; ++b) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int col = 32 * (cg * DB + b) + 8 * g + 4 * up;
           typename Tr::q4_t y;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[r] = Tr::cvt(o[b][4 * g + r] * f);
-          if (col < ev) *reinterpret_cast<typename Tr::q4_t*>(to + col) = y;
+          for (int i = 0; i < 4; ++i) y[i] = Tr::cvt(o[b][4 * g + i] * f);
+          lds_write(place + (tail_lane & 31) * ROW + (32 * b + 8 * g + 4 * up) * 2, y);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (a.lse != nullptr && up == 0 && cg == 0) a.lse[(int64_t)(s.start + t) * a.hq + h] = sm.lse(sum);
+      if (a.lse != nullptr && up == 0 && cg == 0 && out_row < rows) a.lse[(int64_t)(s.start + t) * a.hq + h] = sm.lse(sum);
+      const int off = (int)((t - t0) * a.o_row + h * a.o_head), lpo = tail_lane % LPO, col = cg * W + lpo * 8;
+      T* to = reinterpret_cast<T*>(a.out) + (int64_t)(s.start + t0) * a.o_row + col;
+#pragma unroll
+      for (int i = 0; i < 32 / RPO; ++i) {
+        const int r1 = i * RPO + tail_lane / LPO, at = RPO == 1 ? __builtin_amdgcn_readlane(off, i) : __shfl(off, r1);
+        const u32x4_t y = lds_read<u32x4_t>(place + r1 * ROW + lpo * 16);
+        if (w0 + r1 < rows && col < ev) *reinterpret_cast<u32x4_t*>(to + at) = y;
+      }
     }
     u += n_tiles;
-    __syncthreads();      // (the next segment's first tile takes the place of one that may still be read)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (what comes next takes the rows' place)
   }
 }
 
@@ -330,28 +481,18 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
 // Bound by round trips to memory for few rows (hence eight pieces at a time: 33 of them one after the other took 22 us), by the pieces' bytes for many.
 template <typename T, int EA, int RW>
 __global__ __launch_bounds__(256) void latent_cache_sum_kernel(const LatentCacheArgs a, int wide) {
-  __shared__ __attribute__((aligned(8))) char words[64];
   constexpr int DB = EA / 32;
-  const int per = DB / wide, db0 = blockIdx.x % per * wide, rw = blockIdx.x / per % RW, vb = blockIdx.x / per / RW;
-  // (blocks numbered with a gap or two: those of sequence z start at its first row's number divided by the rows of a block, plus z)
-  auto base_of = [&](int z, const LatentSeq& s) { return (int)((int64_t)s.start * a.hq / a.block_rows) + z; };
-  const LatentCut cut = latent_find(a, words, [&](const LatentCut&, int z, int64_t, const LatentSeq& s) {
-    const int base = base_of(z, s);
-    return base <= vb && vb < base + s.blocks;
-  });
-  if (cut.z < 0) return;
-  const LatentSeq s = latent_cache_seq(a, cut.z);
-  const int block = vb - base_of(cut.z, s);
-  const int64_t u0 = cut.first + (int64_t)block * s.tiles, u1 = u0 + s.tiles;
-  const int w0 = (int)(u0 / cut.per), w1 = (int)((u1 - 1) / cut.per);
-  if (w0 == w1) return;
-  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, c = lane & 31, row = block * a.block_rows + rw * 32 + c;
-  if (row >= s.tokens * a.hq) return;
-  const int first_place = u0 != w0 * cut.per ? 1 : 0;
-  auto at = [&](int w) { return ((int64_t)w * 2 + (w == w0 ? first_place : 0)) * RW + rw; };
+  const int per = DB / wide, db0 = blockIdx.x % per * wide, rw = blockIdx.x / per % RW;
+  const LatentHead head_of = a.heads[blockIdx.x / per / RW];
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, c = lane & 31, row = head_of.block * a.block_rows + rw * 32 + c;
+  const int w0 = head_of.piece / 2, w1 = w0 + head_of.pieces - 1;
+  // (offsets of sequences that do not ascend leave heads that nobody wrote)
+  if (head_of.pieces <= 0 || w0 < 0 || w1 < w0 || w1 >= a.workers || head_of.block < 0 || row < 0 || row >= head_of.rows) return;
+  if (head_of.start < 0 || (int64_t)head_of.start * a.hq + row >= (int64_t)a.rows * a.hq) return;
+  auto at = [&](int w) { return (int64_t)(w == w0 ? head_of.piece : w * 2) * RW + rw; };
   const float sc = score_scale(a.sm_scale, false);
   const int token = row / a.hq, head = row - token * a.hq;
-  T* out = reinterpret_cast<T*>(a.out) + (int64_t)(s.start + token) * a.o_row + (int64_t)head * a.o_head;
+  T* out = reinterpret_cast<T*>(a.out) + (int64_t)(head_of.start + token) * a.o_row + (int64_t)head * a.o_head;
   for (int db = db0; db < db0 + wide; ++db) {
     float m = kNegBig, l = 0.f;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
@@ -387,20 +528,24 @@ __global__ __launch_bounds__(256) void latent_cache_sum_kernel(const LatentCache
     for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(x[r] * f);
     if (col < a.cache.head_dim_v) *reinterpret_cast<typename Traits<T>::q4_t*>(out + col) = y;
     if (a.lse != nullptr && db == 0 && tid < 32)
-      a.lse[(int64_t)(s.start + token) * a.hq + head] = l == 0.f ? __builtin_inff() : __builtin_fmaf(m, sc, fast_log2(l)) * kLn2;
+      a.lse[(int64_t)(head_of.start + token) * a.hq + head] = l == 0.f ? __builtin_inff() : __builtin_fmaf(m, sc, fast_log2(l)) * kLn2;
   }
 }
 
-template <typename T, int EA, int RW> hipError_t launch_latent_cache_rows(const LatentCacheArgs& a, hipStream_t s) {
+template <typename T, int EA, int RW, bool kCut> hipError_t launch_latent_cache_main(const LatentCacheArgs& a, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
-  const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_cache_kernel<T, EA, RW>), LatentCacheSmem<EA>::BYTES, done);
+  const hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_cache_kernel<T, EA, RW, kCut>), LatentCacheSmem<EA>::BYTES, done);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((latent_cache_kernel<T, EA, RW>), dim3((unsigned)a.workers), dim3(256), LatentCacheSmem<EA>::BYTES, s, a);
+  hipLaunchKernelGGL((latent_cache_kernel<T, EA, RW, kCut>), dim3((unsigned)a.workers), dim3(256), LatentCacheSmem<EA>::BYTES, s, a);
+  return hipGetLastError();
+}
+template <typename T, int EA, int RW> hipError_t launch_latent_cache_rows(const LatentCacheArgs& a, hipStream_t s) {
+  const hipError_t e = (a.cache.head_dim < EA ? launch_latent_cache_main<T, EA, RW, true> : launch_latent_cache_main<T, EA, RW, false>)(a, s);
+  if (e != hipSuccess) return e;
   if (a.part_o != nullptr && a.cache.sequences > 0) {
-    const int64_t blocks = (int64_t)a.rows * a.hq / a.block_rows + a.cache.sequences;
     int wide = 1;      // (two rounds of workgroups, or nearly)
-    while (wide < EA / 32 && blocks * RW * (EA / 32) / wide > 4096) wide *= 2;
-    hipLaunchKernelGGL((latent_cache_sum_kernel<T, EA, RW>), dim3((unsigned)(blocks * RW * (EA / 32 / wide))), dim3(256), 0, s, a, wide);
+    while (wide < EA / 32 && (int64_t)a.blocks * RW * (EA / 32) / wide > 4096) wide *= 2;
+    hipLaunchKernelGGL((latent_cache_sum_kernel<T, EA, RW>), dim3((unsigned)(a.blocks * RW * (EA / 32 / wide))), dim3(256), 0, s, a, wide);
   }
   return hipGetLastError();
 }

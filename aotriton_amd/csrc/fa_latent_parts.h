@@ -26,20 +26,17 @@ struct RowSoftmax {
   bool prescale;
   __device__ __forceinline__ RowSoftmax(float sm_scale) : m(kNegBig), l(0.f), sc(score_scale(sm_scale, false)), scale(sm_scale * kLog2e), prescale(!(sm_scale * kLog2e > 0.f)) {}
 
-  // s: scores of NB x 32 keys, to be P; key 32 b + 8 (i / 4) + i % 4 of this lane's half is seen up to `limit`.  `rescale` takes O times a factor.
+  // s: scores of NB x 32 keys, to be P, as the MFMAs leave them but for hidden() in the place of those that the row does not see.  `rescale` takes O
+  // times a factor.
+  __device__ __forceinline__ float hidden() const { return prescale && scale < 0.f ? __builtin_inff() : -__builtin_inff(); }
   template <int NB, typename Rescale>
-  __device__ __forceinline__ void step(f32x16 (&s)[NB], bool masked, int limit, Rescale rescale) {
+  __device__ __forceinline__ void step(f32x16 (&s)[NB], Rescale rescale) {
     if (prescale) {
+      // (a scale of 0: what is hidden stays so)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] *= scale;
-    }
-    if (masked) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = 32 * b + 8 * (i / 4) + i % 4 <= limit ? s[b][i] : -__builtin_inff();
+        for (int i = 0; i < 16; ++i) s[b][i] = scale == 0.f && s[b][i] == hidden() ? s[b][i] : s[b][i] * scale;
     }
     float top = s[0][0];
 #pragma unroll
@@ -50,8 +47,8 @@ struct RowSoftmax {
     if (__builtin_amdgcn_ballot_w64((top - m) * sc > kSlack) != 0) {
       const float to = fmaxf(m, top), alpha = fast_exp2((m - to) * sc);
       m = to;
+      if (__builtin_amdgcn_ballot_w64(l != 0.f) != 0) rescale(alpha);      // (before a row's first sum O is 0)
       l *= alpha;
-      rescale(alpha);
     }
     const float msc = m * sc;
     float sum[2] = {0.f, 0.f};
