@@ -292,12 +292,17 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     }
     RowSoftmax sm(a.sm_scale);
 
-    constexpr int kRing = 5;      // operands on their way: left to itself the compiler keeps dozens
+    constexpr int kRing = 8;      // operands on their way: left to itself the compiler keeps dozens
     f32x16 x[1];
     op_t p[2], p_next[2], ring[kRing];
+    // (lane constants of the operands' addresses; the group's first block of columns: of its number the lower two bits are swizzled)
+    const int first_block = cg * DB, block_xor = (first_block & 3) << 6, block_off = (first_block >> 2) * 256;
+    int at_e = Swz<EA>::row_base(lane), at_r = Swz<kLatentTail>::row_base(lane);
+    int at_0 = (Swz<EA>::tr_base(lane, 0) ^ block_xor) + block_off, at_1 = (Swz<EA>::tr_base(lane, 1) ^ block_xor) + block_off;
+    if constexpr (kFull) asm volatile("" : "+v"(at_e), "+v"(at_r), "+v"(at_0), "+v"(at_1));
     // x = S of tile j, with the pieces of the tile that is being fetched behind its MFMAs
     auto scores = [&](int j, auto fetching) __attribute__((always_inline)) {
-      const int X = stage_of(j), at_e = Swz<EA>::row_base(own_lane()), at_r = Swz<kLatentTail>::row_base(own_lane());
+      const int X = stage_of(j);
       auto read = [&](int k) __attribute__((always_inline)) { return k_read(X, at_e, at_r, k); };
 #pragma unroll
       for (int k = 0; k < kRing - 1; ++k) ring[k] = read(k);
@@ -328,9 +333,6 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     // different ones, as in fa_fwd_wide.h); returns whether they will do
     auto values = [&](int j, int hol) __attribute__((always_inline)) {
       constexpr int N = 2 * DB, kLag = 2;
-      // (the group's first block of columns: of its number the lower two bits are swizzled)
-      const int first_block = cg * DB, block_xor = (first_block & 3) << 6, block_off = (first_block >> 2) * 256;
-      const int at_0 = (Swz<EA>::tr_base(own_lane(), 0) ^ block_xor) + block_off, at_1 = (Swz<EA>::tr_base(own_lane(), 1) ^ block_xor) + block_off;
       const int X = stage_of(j);
       auto read = [&](int i) __attribute__((always_inline)) {
         const int b = i % DB, off = X + i / DB * 16 * Swz<EA>::ROWB + (b >> 2) * 256;
