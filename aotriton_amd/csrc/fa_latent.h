@@ -17,6 +17,7 @@
 namespace fa {
 
 constexpr int kLatentShared = 64;      // compiled columns of the shared part
+constexpr int kLatentFewTiles = 4;     // tiles of 64 keys up to which dQ sums delta itself
 
 // A tile's 64 rows as they come into LDS: 16 rows a wave, 1 KB an access.  A lane's byte offsets of its accesses; the columns start at
 // `col0` of the row, and there are `cols` of them.
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(256) void latent_fwd_sum_kernel(const LatentArgs a,
 }
 
 // ---- dQ ------------------------------------------------------------------------------------------------------------
-// Rows as in the forward; also delta, which needs the rows of O and dO that are here anyway.
+// Rows as in the forward; also delta.
 template <typename T, int EC>
 __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a, int nseq, int tiles) {
   using Tr = Traits<T>;
@@ -274,58 +275,80 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
     load_operands<T, KR>(q + KE, qp, (int)a.sq.s * 2, rows, lane, a.e, a.r);
     load_operands<T, KE>(dout, row_at<T>(a.dout, a.sdo, si, h, (int64_t)si.q_start + w0), (int)a.sdo.s * 2, rows, lane, 0, a.ev);
   }
+  // delta of few keys is summed from P and dP in a pass of its own, else from O: of O's rounding as much is left as the keys that weigh in
+  // have not averaged out, and with few of them it is the largest error of the gradients (two thirds of dQ's products once more, for rows
+  // whose tiles are few).
+  const bool few = j1 <= kLatentFewTiles;
   float delta = 0.f, lse = __builtin_inff();
-  {
+  if (row < si.seqlen_q) lse = a.lse[lse_offset(si, h, a.heads) + row] * kLog2e;
+  if (!few) {
     op_t out[KE];
     load_operands<T, KE>(out, row_at<T>(a.out, a.so, si, h, (int64_t)si.q_start + w0), (int)a.so.s * 2, rows, lane, 0, a.ev);
 #pragma unroll
     for (int k = 0; k < KE; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta += (float)out[k][i] * (float)dout[k][i];
-    delta = cross_sum(delta);
-    if (row < si.seqlen_q) {
-      const int64_t at = lse_offset(si, h, a.heads) + row;
-      lse = a.lse[at] * kLog2e;
-      if (hi == 0) { a.stat_lse[at] = lse; a.stat_delta[at] = delta; }
-    }
   }
   arrived(q);
   arrived(dout);
+  const float qs = a.sm_scale * kLog2e;
+  // P and dP of 32 keys of tile j
+  auto products = [&](const char* K, int j, int b, f32x16& p, f32x16& dp) __attribute__((always_inline)) {
+    const int l = own_lane(), n0 = j * 64;
+    const bool masked = n0 + 64 > si.seqlen_k || (a.causal && n0 + 63 > w0 + shift);
+    const int row_e = Swz<EC>::row_base(l), row_r = Swz<kLatentShared>::row_base(l);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = dp[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KE; ++k) p = Tr::mfma(swz_read_row<T, EC>(K, row_e, k, b), q[k], p);
+#pragma unroll
+    for (int k = 0; k < KR; ++k) p = Tr::mfma(swz_read_row<T, kLatentShared>(K + SM::C_OFF, row_r, k, b), q[KE + k], p);
+#pragma unroll
+    for (int k = 0; k < KE; ++k) dp = Tr::mfma(swz_read_row<T, EC>(K + SM::V_OFF, row_e, k, b), dout[k], dp);
+    const int limit = see - n0 - 32 * b - 4 * hi;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p[i] = fast_exp2(__builtin_fmaf(p[i], qs, -lse));
+      if (masked && 8 * (i / 4) + i % 4 > limit) p[i] = 0.f;
+    }
+  };
+  int stage = 0;      // of the tile that comes next
+  if (few) {
+    for (int j = 0; j < j1; ++j, stage ^= 1) {
+      latent_meet();
+      fetch(stage ^ 1, j + 1 < j1 ? j + 1 : 0);
+      if (j >= wave_end) continue;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        f32x16 p, dp;
+        products(smem + stage * SM::STAGE, j, b, p, dp);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) delta = __builtin_fmaf(p[i], dp[i], delta);
+      }
+    }
+  }
+  delta = cross_sum(delta);
+  if (row < si.seqlen_q && hi == 0) {
+    const int64_t at = lse_offset(si, h, a.heads) + row;
+    a.stat_lse[at] = lse;
+    a.stat_delta[at] = delta;
+  }
   f32x16 dq[DB + RB];
 #pragma unroll
   for (int b = 0; b < DB + RB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dq[b][i] = 0.f;
-  const float qs = a.sm_scale * kLog2e;
-
-  for (int j = 0; j < j1; ++j) {
+  for (int j = 0; j < j1; ++j, stage ^= 1) {
     latent_meet();
-    const int stage = j & 1;
     if (j + 1 < j1) fetch(stage ^ 1, j + 1);
     if (j >= wave_end) continue;
     const char* K = smem + stage * SM::STAGE;
-    const int n0 = j * 64;
-    const bool masked = n0 + 64 > si.seqlen_k || (a.causal && n0 + 63 > w0 + shift);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const int l = own_lane();
-      const int row_e = Swz<EC>::row_base(l), row_r = Swz<kLatentShared>::row_base(l);
       f32x16 s, dp;
+      products(K, j, b, s, dp);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KE; ++k) s = Tr::mfma(swz_read_row<T, EC>(K, row_e, k, b), q[k], s);
-#pragma unroll
-      for (int k = 0; k < KR; ++k) s = Tr::mfma(swz_read_row<T, kLatentShared>(K + SM::C_OFF, row_r, k, b), q[KE + k], s);
-#pragma unroll
-      for (int k = 0; k < KE; ++k) dp = Tr::mfma(swz_read_row<T, EC>(K + SM::V_OFF, row_e, k, b), dout[k], dp);
-      const int limit = see - n0 - 32 * b - 4 * hi;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float p = fast_exp2(__builtin_fmaf(s[i], qs, -lse));
-        if (masked && 8 * (i / 4) + i % 4 > limit) p = 0.f;
-        s[i] = p * (dp[i] - delta);
-      }
+      for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
       const int m = own_lane();
       const int tr0 = Swz<EC>::tr_base(m, 0), tr1 = Swz<EC>::tr_base(m, 1), rr0 = Swz<kLatentShared>::tr_base(m, 0), rr1 = Swz<kLatentShared>::tr_base(m, 1);
 #pragma unroll

@@ -90,6 +90,25 @@ def test_against_the_oracle(B, H, Sq, Sk, E, R, Ev, causal, dtype):
         _check(q[b], k[b], v[b], c[b], do[b], causal, 1 / math.sqrt(E + R), out[b], lse.view(B, H, Sq)[b], [g[b] for g in grads], f'sequence {b} ')
 
 
+@pytest.mark.parametrize('dtype', [HF, BF])
+def test_gradients_of_a_single_key(dtype):
+    """P is 1 and dS = P (dP - delta) nothing, whatever O's rounding: what is left is P's error.  The logarithm of the sum, below 8 here, is rounded
+    three times on its way, 3 2^-24 8, and the exponential and the product add less than as much again: dS is under 2^-18 |dP|.  (Delta from O
+    in 16 bits is off by up to 2^-12 of its terms, 2^-8 for bf16.)  Half the smallest number that the type holds comes on top."""
+    B, H, E, R, Ev = 3, 4, 128, 64, 128
+    q, k, v, c, do = _inputs(B, H, 1, 1, E, R, Ev, dtype, seed=8)
+    out, (dq, dk, _, dc) = _step(q, k, v, c, do, scale=0.05)
+    assert torch.equal(out, v)
+    assert (torch.matmul(q.float(), torch.cat([k, c[:, None].expand(-1, H, -1, -1)], -1).float().transpose(2, 3)) * 0.05 * 1.5).abs().max() < 8
+    dp = (do.double() * v.double()).abs().sum(-1, keepdim=True)
+    least = 2.0 ** -25 if dtype == HF else 0.0
+    bound = 2.0 ** -18 * 0.05 * dp
+    assert (dq[..., :E].double().abs() <= bound * k.double().abs() + least).all()
+    assert (dq[..., E:].double().abs() <= bound * c[:, None].double().abs() + least).all()
+    assert (dk.double().abs() <= bound * q[..., :E].double().abs() + least).all()
+    assert (dc.double().abs() <= (bound * q[..., E:].double().abs()).sum(1) + least).all()
+
+
 @pytest.mark.parametrize('B,H,Sq,Sk,E,R,Ev,causal,dtype', [
     (1, 1, 1, 4000, 128, 64, 128, True, BF), (1, 2, 130, 3000, 128, 64, 128, True, HF), (2, 1, 5, 2049, 64, 32, 64, False, HF),
     (1, 3, 17, 1100, 40, 8, 24, True, BF), (1, 1, 2000, 1900, 64, 64, 64, True, BF)])
