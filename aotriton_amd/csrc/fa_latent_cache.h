@@ -197,15 +197,23 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     constexpr int kLoads = 8 / RPL + 1, kPieces = 4 / RPL + 1;      // of a tile, and the pairs they come in
     u32x4_t f_rs;
     int f_lds;
-    auto fetch_begin = [&](int j) __attribute__((always_inline)) {      // returns which of the tile's halves have no page
-      pages.to((j - j0) * 2);
-      const int n = j * 32 + wave * 8, left = s.end - n < 8 ? s.end - n : 8;
-      const int p = pages.at((j - j0) * 2 + wave / 2);
-      const char* from = xbase + ((int64_t)(p < 0 ? 0 : p) * ca.sk.z + (int64_t)(n & ((1 << ca.page_shift) - 1)) * ca.sk.s) * 2;
-      f_rs = wave_rsrc_words(from, p < 0 ? 0 : rows_extent(left, x_row, e * 2));      // (a page that is not there: zeros, no traffic)
+    // What a tile's fetch needs, in steps that stand behind different MFMAs; fetch_holes says which of its halves have no page.
+    int f_page, f_left, f_entry;
+    const char* f_from;
+    auto fetch_page = [&](int j) __attribute__((always_inline)) {
+      f_entry = (j - j0) * 2;
+      f_page = pages.at(f_entry + wave / 2);
       f_lds = stage_of(j);
-      return pages.holes((j - j0) * 2) & 3;
     };
+    auto fetch_rows = [&](int j) __attribute__((always_inline)) {
+      const int n = j * 32 + wave * 8;
+      f_left = s.end - n < 8 ? s.end - n : 8;
+      f_from = xbase + (int64_t)(n & ((1 << ca.page_shift) - 1)) * ca.sk.s * 2;
+    };
+    auto fetch_rsrc = [&]() __attribute__((always_inline)) {      // (a page that is not there: zeros, no traffic)
+      f_rs = wave_rsrc_words(f_from + (int64_t)(f_page < 0 ? 0 : f_page) * ca.sk.z * 2, f_page < 0 ? 0 : rows_extent(f_left, x_row, e * 2));
+    };
+    auto fetch_holes = [&]() __attribute__((always_inline)) { return pages.holes(f_entry) & 3; };
     auto fetch_piece = [&](int i) __attribute__((always_inline)) {
       const int l = own_lane();
       if (i < kPieces - 1) {
@@ -227,10 +235,13 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
       }
     };
     auto fetch = [&](int j) __attribute__((always_inline)) {
-      const int holes = fetch_begin(j);
+      pages.to((j - j0) * 2);
+      fetch_page(j);
+      fetch_rows(j);
+      fetch_rsrc();
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) fetch_piece(i);
-      return holes;
+      return fetch_holes();
     };
     auto k_read = [&](int X, int at_e, int at_r, int k) __attribute__((always_inline)) {
       return k < KE ? lds_read<op_t>((at_e ^ ((k & 7) << 5)) + X + (k >> 3) * 256) : lds_read<op_t>((at_r ^ ((k - KE) << 5)) + X + SM::A);
@@ -292,25 +303,57 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     }
     RowSoftmax sm(a.sm_scale);
 
-    constexpr int kRing = 8;      // operands on their way: left to itself the compiler keeps dozens
+    constexpr int kRing = 8, kS = KE + KR, kV = 2 * DB;      // operands on their way: left to itself the compiler keeps dozens
     f32x16 x[1];
     op_t p[2], p_next[2], ring[kRing];
-    // (lane constants of the operands' addresses; the group's first block of columns: of its number the lower two bits are swizzled)
-    const int first_block = cg * DB, block_xor = (first_block & 3) << 6, block_off = (first_block >> 2) * 256;
-    int at_e = Swz<EA>::row_base(lane), at_r = Swz<kLatentTail>::row_base(lane);
-    int at_0 = (Swz<EA>::tr_base(lane, 0) ^ block_xor) + block_off, at_1 = (Swz<EA>::tr_base(lane, 1) ^ block_xor) + block_off;
-    if constexpr (kFull) asm volatile("" : "+v"(at_e), "+v"(at_r), "+v"(at_0), "+v"(at_1));
-    // x = S of tile j, with the pieces of the tile that is being fetched behind its MFMAs
-    auto scores = [&](int j, auto fetching) __attribute__((always_inline)) {
-      const int X = stage_of(j);
-      auto read = [&](int k) __attribute__((always_inline)) { return k_read(X, at_e, at_r, k); };
+    // Addresses of the operands in the tiles of S and of the values, which move from stage to stage (formed for every read they cost an
+    // instruction each, where the compiler does not see that an offset would do; of the number of the group's first block of columns the lower
+    // two bits are swizzled).
+    int at_e[8], at_r[KR], at_v[8];
+    {
+      const int first_block = cg * DB, block_xor = (first_block & 3) << 6, block_off = (first_block >> 2) * 256;
 #pragma unroll
-      for (int k = 0; k < kRing - 1; ++k) ring[k] = read(k);
+      for (int i = 0; i < 8; ++i) {
+        at_e[i] = smem0 + (Swz<EA>::row_base(lane) ^ (i << 5));
+        at_v[i] = smem0 + (Swz<EA>::tr_base(lane, i >> 2) ^ block_xor ^ ((i & 3) << 6)) + block_off;
+      }
 #pragma unroll
-      for (int k = 0; k < KE + KR; ++k) {
-        if (k + kRing - 1 < KE + KR) ring[(k + kRing - 1) % kRing] = read(k + kRing - 1);
+      for (int i = 0; i < KR; ++i) at_r[i] = smem0 + SM::A + (Swz<kLatentTail>::row_base(lane) ^ (i << 5));
+      arrived(at_e);
+      arrived(at_r);
+      arrived(at_v);
+    }
+    auto onward = [&](auto& at, int j) __attribute__((always_inline)) {      // from the stage of tile j to that of j + 1
+      const int by = ((j - j0) & (SM::STAGES - 1)) == SM::STAGES - 1 ? -(SM::STAGES - 1) * SM::STAGE : SM::STAGE;
+#pragma unroll
+      for (auto& x : at) x += by;
+      arrived(at);
+    };
+    auto read_s = [&](int k) __attribute__((always_inline)) { return k < KE ? lds_read<op_t>(at_e[k & 7] + (k >> 3) * 256) : lds_read<op_t>(at_r[k - KE]); };
+    auto read_v = [&](int i) __attribute__((always_inline)) {
+      const int b = i % DB, off = i / DB * 16 * Swz<EA>::ROWB + (b >> 2) * 256;
+      const auto lo = __builtin_bit_cast(typename Tr::q4_t, lds_read_tr_at(at_v[b & 3] + off));
+      const auto up = __builtin_bit_cast(typename Tr::q4_t, lds_read_tr_at(at_v[4 + (b & 3)] + off));
+      return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    // x = S of a tile.  Behind its MFMAs: tile `next` is fetched, and the first operands of the values that come next are read.
+    auto scores = [&](int next, int& holes_next, auto goes_on) __attribute__((always_inline)) {
+      constexpr bool on = decltype(goes_on)::value;
+#pragma unroll
+      for (int k = 0; k < kRing - 1; ++k) ring[k] = read_s(k);
+#pragma unroll
+      for (int k = 0; k < kS; ++k) {
+        constexpr int kAhead = kRing - 1;
+        if (k + kAhead < kS) ring[(k + kAhead) % kRing] = read_s(k + kAhead);
+        else if (on && k + kAhead - kS < kV) ring[(k + kAhead) % kRing] = read_v(k + kAhead - kS);
         x[0] = Tr::mfma(ring[k % kRing], q[k], k == 0 ? f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f} : x[0]);
-        if (decltype(fetching)::value && k % 3 == 2 && k / 3 < kPieces) fetch_piece(k / 3);
+        if (on) {
+          if (k == 0) fetch_page(next);
+          if (k == 1) fetch_rows(next);
+          if (k == 2) fetch_rsrc();
+          if (k == 3) holes_next = fetch_holes();
+          if (k % 3 == 1 && k > 3 && k / 3 - 1 < kPieces) fetch_piece(k / 3 - 1);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -330,40 +373,29 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
       for (int t = 0; t < 2; ++t) p_next[t] = pack8<T>(x[0], t);
     };
     // O += X(j)^T P(j)^T, and P of tile j + 1 from x behind its MFMAs, against the maxima that the rows have (an element's three parts behind
-    // different ones, as in fa_fwd_wide.h); returns whether they will do
+    // different ones, as in fa_fwd_wide.h); returns whether they will do.  The first operands are there or on their way.
     auto values = [&](int j, int hol) __attribute__((always_inline)) {
-      constexpr int N = 2 * DB, kLag = 2;
-      const int X = stage_of(j);
-      auto read = [&](int i) __attribute__((always_inline)) {
-        const int b = i % DB, off = X + i / DB * 16 * Swz<EA>::ROWB + (b >> 2) * 256;
-        const auto lo = __builtin_bit_cast(typename Tr::q4_t, lds_read_tr_at((at_0 ^ ((b & 3) << 6)) + off));
-        const auto up = __builtin_bit_cast(typename Tr::q4_t, lds_read_tr_at((at_1 ^ ((b & 3) << 6)) + off));
-        return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
-      };
+      constexpr int kLag = 2, kFrom = kV > 8 ? 2 : 0;      // (S comes out of its last MFMA meanwhile)
       hide(j + 1, hol, -__builtin_inff());
       const float msc = sm.m * sm.sc;
       float sum = 0.f;
+      uint32_t words[8];
 #pragma unroll
-      for (int i = 0; i < kRing - 1 && i < N; ++i) ring[i] = read(i);
+      for (int i = 0; i < kV; ++i) {
+        if (i + kRing - 1 < kV) ring[(kS + i + kRing - 1) % kRing] = read_v(i + kRing - 1);
+        if constexpr (kFull) mfma_acc<T>(o[i % DB], ring[(kS + i) % kRing], p[i / DB]);
+        else o[i % DB] = Tr::mfma(ring[(kS + i) % kRing], p[i / DB], o[i % DB]);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i + kRing - 1 < N) ring[(i + kRing - 1) % kRing] = read(i + kRing - 1);
-        if constexpr (kFull) mfma_acc<T>(o[i % DB], ring[i % kRing], p[i / DB]);
-        else o[i % DB] = Tr::mfma(ring[i % kRing], p[i / DB], o[i % DB]);
-#pragma unroll
-        for (int E = first_of(i, 16 + kLag, N); E < first_of(i + 1, 16 + kLag, N); ++E) {
-          if (E < 16) {
-            x[0][E] = __builtin_fmaf(x[0][E], sm.sc, -msc);
-          }
+        for (int E = i < kFrom ? 0 : first_of(i - kFrom, 16 + kLag, kV - kFrom); E < (i < kFrom ? 0 : first_of(i + 1 - kFrom, 16 + kLag, kV - kFrom)); ++E) {
+          if (E < 16) x[0][E] = __builtin_fmaf(x[0][E], sm.sc, -msc);
           if (E >= kLag / 2 && E < 16 + kLag / 2) x[0][E - kLag / 2] = fast_exp2(x[0][E - kLag / 2]);
           if (E >= kLag) {
             const int e2 = E - kLag;
             sum += x[0][e2];
-            if (e2 & 1) {
-              const typename Tr::p2_t p2 = Tr::cvt2(x[0][e2 - 1], x[0][e2]);
-              p_next[e2 / 8][e2 % 8 - 1] = p2[0];
-              p_next[e2 / 8][e2 % 8] = p2[1];
-            }
+            if (e2 & 1) words[e2 / 2] = __builtin_bit_cast(uint32_t, Tr::cvt2(x[0][e2 - 1], x[0][e2]));
+            // (here and not behind the last MFMA, where the compiler would have them)
+            asm volatile("" : "+v"(sum));
+            if (e2 & 1) asm volatile("" : "+v"(words[e2 / 2]));
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -371,6 +403,8 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
       // (also catches inf and NaN)
       if ((sm.prescale && hol != 3) || __builtin_amdgcn_ballot_w64(!(sum < 4096.f)) != 0) return false;
       sm.l += sum;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) p_next[t] = __builtin_bit_cast(op_t, u32x4_t{words[4 * t], words[4 * t + 1], words[4 * t + 2], words[4 * t + 3]});
       return true;
     };
     using yes = std::true_type;
@@ -378,7 +412,7 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     const int jw = j1 < wave_end ? j1 : wave_end;      // the wave's tiles end here
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(2 * kLoads) : "memory");
     if (j0 < jw) {
-      scores(j0, no{});
+      scores(0, holes, no{});
       full_step(j0, holes, [](float) {});
     }
     // In a round: S of the next tile, then the values of this one with the exponentials of the next behind them.  Tiles are fetched three
@@ -387,15 +421,21 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
 #pragma unroll
       for (int t = 0; t < 2; ++t) p[t] = p_next[t];
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kLoads) : "memory");
-      const int holes3 = fetch_begin(j + 3);
+      pages.to((j + 3 - j0) * 2);
+      int holes3 = 0;
       if (j + 1 < jw) {
-        scores(j + 1, yes{});
+        onward(at_e, j);
+        onward(at_r, j);
+        scores(j + 3, holes3, yes{});
       } else {
+        holes3 = fetch(j + 3);
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) fetch_piece(i);
+        for (int i = 0; i < kRing - 1 && i < kV; ++i) ring[(kS + i) % kRing] = read_v(i);
       }
-      if (j < jw && !values(j, j + 1 < jw ? holes1 : 3)) {
-        scores(j + 1, no{});
+      const bool done = j >= jw || values(j, j + 1 < jw ? holes1 : 3);
+      onward(at_v, j);
+      if (!done) {
+        scores(0, holes3, no{});
         full_step(j + 1, holes1, [&](float f) __attribute__((always_inline)) {
 #pragma unroll
           for (int b = 0; b < DB; ++b) {
