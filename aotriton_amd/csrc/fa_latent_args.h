@@ -52,6 +52,8 @@ struct LatentCacheArgs {
   // `workers` equal pieces of at least `least`, one for a workgroup; the sums of a block that lies in several pieces go to
   // part_o, two places for every worker.
   int32_t block_rows, workers, least;
+  int32_t margin;                // fa_latent_cache.h: LatentSeq::units
+  int32_t group, step;           // blocks that 32 tokens make (one at least), tiles that a group's tokens make
   float* part_o; float* part_ml;
   LatentHead* heads;             // of the blocks, `blocks` of them (fa_latent_cache.h: latent_block)
   int32_t blocks;

@@ -20,14 +20,60 @@ constexpr int kLatentTail = 64;
 template <int EA> struct LatentCacheSmem {
   static constexpr int A = 32 * EA * 2, STAGE = A + 32 * kLatentTail * 2, STAGES = 4;
   static constexpr int LIST = STAGES * STAGE;           // words of latent_find
-  static constexpr int BYTES = LIST + 128;
+  static constexpr int BYTES = EA == 256 ? 2 * LIST : LIST + 128 + 8192;      // (with 128 rows of Q)
+  // Q of RW x 32 rows: in how many parts of its columns it comes, with how many tiles of the cache in front of it.  (Where it lies on the list, that
+  // has been read.)
+  template <int RW> struct Q {
+    static constexpr int HALVES = EA == 512 && RW == 4 ? 2 : 1, COLUMNS = EA / HALVES, FIRST = EA == 256 || RW == 1 ? 3 : 2;
+    __host__ __device__ static constexpr int at(int half, int group) {
+      const int size = 32 * COLUMNS * 2 + (half == HALVES - 1 ? 32 * kLatentTail * 2 : 0);
+      return (EA == 256 ? LIST : FIRST * STAGE) + group * size;
+    }
+    static_assert(EA == 256 || 2 * STAGE + 4 * 32 * (COLUMNS + kLatentTail) * 2 <= BYTES || RW < 4, "Q fits");
+  };
 };
 
-// A sequence as the list of work has it: `blocks` blocks of rows, `tiles` tiles each (one at least, for rows that see nothing).
+// a / b of numbers that are not negative (a division of 64 bits takes a microsecond)
+__device__ __forceinline__ int64_t latent_div(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b; }
+
+// A sequence as the list of work has it: `blocks` blocks of rows, of tiles as many as their last row sees, or some more: the blocks of a group
+// (LatentCacheArgs::group) have the same number, `step` more than the group in front, up to all `tiles`.
 struct LatentSeq {
   int32_t start, tokens, length, end;      // first row of Q, tokens, filled slots, slots with the new ones as far as the table goes
-  int32_t blocks, tiles;
-  __device__ __forceinline__ int64_t units() const { return (int64_t)blocks * tiles; }
+  int32_t blocks, tiles, filled;           // (filled: tiles in front of the first new slot)
+  __device__ __forceinline__ int tiles_of_group(const LatentCacheArgs& a, int g) const {
+    const int64_t n = filled + (int64_t)a.step * (g + 1);
+    return n < tiles ? (int)n : tiles;
+  }
+  __device__ __forceinline__ int tiles_of(const LatentCacheArgs& a, int block) const { return tiles_of_group(a, block / a.group); }
+  // groups that have not all tiles, as far as there are blocks
+  __device__ __forceinline__ int short_groups(const LatentCacheArgs& a) const {
+    const int n = tiles > filled ? (tiles - filled - 1) / a.step : 0, all = (blocks + a.group - 1) / a.group;
+    return n < all ? n : all;
+  }
+  // The list counts a block's tiles and LatentCacheArgs::margin on either side of them, for what beginning and ending it takes.
+  __device__ __forceinline__ int64_t units(const LatentCacheArgs& a) const {
+    const int64_t n = short_groups(a), over = n * a.group - blocks;      // (the last group may be short of blocks)
+    const int64_t u = a.group * (n * filled + a.step * (n * (n + 1) / 2)), last = over > 0 ? filled + a.step * n : tiles;
+    return u - over * last + (int64_t)blocks * (2 * a.margin);
+  }
+  // the block with unit `rel` of the sequence, and the unit's number in it
+  __device__ __forceinline__ int block_of(const LatentCacheArgs& a, int64_t rel, int& unit) const {
+    const int n = short_groups(a);
+    for (int g = 0; g < n; ++g) {
+      const int t = filled + a.step * (g + 1) + 2 * a.margin, have = blocks - g * a.group < a.group ? blocks - g * a.group : a.group;
+      if (rel < (int64_t)have * t) {
+        const int b = (int)((uint32_t)rel / (uint32_t)t);
+        unit = (int)rel - b * t;
+        return g * a.group + b;
+      }
+      rel -= (int64_t)have * t;
+    }
+    const int t = tiles + 2 * a.margin;
+    const int64_t b = latent_div(rel, t);
+    unit = (int)(rel - b * t);
+    return n * a.group + (int)b;
+  }
 };
 __device__ __forceinline__ LatentSeq latent_cache_seq(const LatentCacheArgs& a, int z) {
   auto hold = [](int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; };
@@ -37,14 +83,15 @@ __device__ __forceinline__ LatentSeq latent_cache_seq(const LatentCacheArgs& a, 
   s.length = a.cache.lengths[z];
   const int64_t room = (int64_t)a.cache.columns << a.cache.page_shift, end = (int64_t)s.length + s.tokens;
   s.end = s.length < 0 ? 0 : (int)(end < room ? end : room);
-  s.blocks = (int)(((int64_t)s.tokens * a.hq + a.block_rows - 1) / a.block_rows);
+  s.blocks = (int)latent_div((int64_t)s.tokens * a.hq + a.block_rows - 1, a.block_rows);
   s.tiles = s.end > 32 ? (s.end + 31) / 32 : 1;
+  s.filled = s.length <= 0 ? 0 : s.length < s.end ? (s.length + 31) / 32 : s.tiles;
   return s;
 }
 
 // Number of a sequence's first block, with a gap or two: that of its first row, divided by the rows of a block, and one more for every sequence in
 // front.  LatentCacheArgs::blocks bounds them.
-__device__ __forceinline__ int latent_block(const LatentCacheArgs& a, int z, int start) { return (int)((int64_t)start * a.hq / a.block_rows) + z; }
+__device__ __forceinline__ int latent_block(const LatentCacheArgs& a, int z, int start) { return (int)latent_div((int64_t)start * a.hq, a.block_rows) + z; }
 
 // The cut of the list: its length, that of a piece, and of the sequence looked for its number and where it starts in the list.  `mine(z, first
 // unit, sequence)` says which one that is.  All 256 threads call this.
@@ -62,7 +109,7 @@ __device__ __forceinline__ LatentCut latent_find(const LatentCacheArgs& a, char*
     int64_t u = 0;
     if (z < n) {
       s = latent_cache_seq(a, z);
-      u = s.units();
+      u = s.units(a);
     }
     int64_t sum = u;
 #pragma unroll
@@ -81,7 +128,7 @@ __device__ __forceinline__ LatentCut latent_find(const LatentCacheArgs& a, char*
   };
   for (int z0 = 0; z0 < n; z0 += 256) chunk(z0);
   cut.total = base;
-  const int64_t even = (base + a.workers - 1) / a.workers;
+  const int64_t even = latent_div(base + a.workers - 1, a.workers);
   cut.per = even > a.least ? even : a.least;
   if (tid == 0) sums[5] = -1;
   __syncthreads();
@@ -89,7 +136,7 @@ __device__ __forceinline__ LatentCut latent_find(const LatentCacheArgs& a, char*
   for (int z0 = 0; z0 < n; z0 += 256) {
     if (n > 256) chunk(z0);
     const int z = z0 + tid;
-    if (z < n && s.units() > 0 && mine(cut, z, before, s)) {
+    if (z < n && s.blocks > 0 && mine(cut, z, before, s)) {
       sums[4] = before;
       sums[5] = z;
       *reinterpret_cast<LatentSeq*>(sums + 6) = s;
@@ -100,6 +147,7 @@ __device__ __forceinline__ LatentCut latent_find(const LatentCacheArgs& a, char*
   cut.first = sums[4];
   cut.z = (int)sums[5];
   cut.seq = *reinterpret_cast<const LatentSeq*>(sums + 6);
+  __syncthreads();      // (Q may come to lie on the words)
   return cut;
 }
 
@@ -123,31 +171,30 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
   // to place the two, spills a thousand bytes.
   constexpr bool kFull = DB == 16;
   extern __shared__ __attribute__((aligned(kSwzAlign))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hi = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % RW, cg = wave / RW;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW, cg = wave / RW;
   const CacheArgs& ca = a.cache;
   const int e = ca.head_dim, ev = ca.head_dim_v;
 
+  const int n_seq = ca.sequences, starts_first = n_seq > 0 ? a.starts[0] : a.rows, starts_last = n_seq > 0 ? a.starts[n_seq] : 0;
+  // (workgroups go round the XCDs: those of neighbouring pieces, which read the same Q, stand on one)
+  const int xcd = blockIdx.x % 8, each = a.workers / 8, more = a.workers % 8;
+  const int64_t worker = xcd * each + (xcd < more ? xcd : more) + (int)blockIdx.x / 8;
+  const LatentCut cut = latent_find(a, smem + SM::LIST, [&](const LatentCut& t, int, int64_t first, const LatentSeq& s) {
+    return first <= worker * t.per && worker * t.per < first + s.units(a);
+  });
   // rows of no sequence
   {
-    const int n = ca.sequences;
-    const int first = n > 0 ? a.starts[0] : a.rows, last = n > 0 ? a.starts[n] : 0;
-    const int gap = first < 0 ? 0 : first > a.rows ? a.rows : first, end = last < gap ? gap : last;
+    const int gap = starts_first < 0 ? 0 : starts_first > a.rows ? a.rows : starts_first, end = starts_last < gap ? gap : starts_last;
     for (int i = blockIdx.x; i < gap + (a.rows - end); i += gridDim.x) {
       const int row = i < gap ? i : end + i - gap;
-      for (int x = tid; x < a.hq * (ev / 8); x += 256) {
+      for (int x = threadIdx.x; x < a.hq * (ev / 8); x += 256) {
         const int h = x / (ev / 8), col = x % (ev / 8) * 8;
         *reinterpret_cast<u32x4_t*>(reinterpret_cast<T*>(a.out) + (int64_t)row * a.o_row + (int64_t)h * a.o_head + col) = u32x4_t{0, 0, 0, 0};
         if (a.lse != nullptr && col == 0) a.lse[(int64_t)row * a.hq + h] = __builtin_inff();
       }
     }
-    if (n == 0) return;
   }
-  const int64_t worker = blockIdx.x;
-  const LatentCut cut = latent_find(a, smem + SM::LIST, [&](const LatentCut& t, int, int64_t first, const LatentSeq& s) {
-    return first <= worker * t.per && worker * t.per < first + s.units();
-  });
-  int64_t u = worker * cut.per;
+  const int64_t u = worker * cut.per;
   const int64_t u_end = u + cut.per < cut.total ? u + cut.per : cut.total;
   // (for the kernel that puts the pieces together: a block's head is written by the worker that begins it, and where blocks are numbered with a
   // gap by the one that begins the block in front, or the first)
@@ -157,7 +204,6 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
   if (a.heads != nullptr && cut.total == 0 && worker == 0) put_heads(0, a.blocks);
   if (u >= u_end) return;
   int z = __builtin_amdgcn_readfirstlane(cut.z);
-  int64_t first = cut.first;
 
   const int smem0 = lds_offset(smem);
   // What depends on the lane alone is formed where it is needed: held through the loop over tiles, which Q and O leave little room, it would be
@@ -166,20 +212,37 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
   const int x_row = (int)ca.sk.s * 2;
   constexpr int LPR = EA / 8, RPL = 64 / LPR;      // lanes of a row, rows of an access
   LatentSeq s = cut.seq;
-  for (bool again = false; u < u_end; again = true) {
+  int block = 0;
+  int64_t at_unit = u;      // where the block begins
+  for (bool again = false; at_unit < u_end; again = true) {
     if (again) s = latent_cache_seq(a, z);
     s.start = __builtin_amdgcn_readfirstlane(s.start); s.tokens = __builtin_amdgcn_readfirstlane(s.tokens);
     s.length = __builtin_amdgcn_readfirstlane(s.length); s.end = __builtin_amdgcn_readfirstlane(s.end);
     s.tiles = __builtin_amdgcn_readfirstlane(s.tiles); s.blocks = __builtin_amdgcn_readfirstlane(s.blocks);
-    if (u - first >= s.units()) {      // (the next one that has rows)
-      first += s.units();
+    s.filled = __builtin_amdgcn_readfirstlane(s.filled);
+    if (!again) {
+      int unit;
+      block = __builtin_amdgcn_readfirstlane(s.block_of(a, u - cut.first, unit));
+      at_unit = u - __builtin_amdgcn_readfirstlane(unit);
+    }
+    if (block >= s.blocks) {      // (the next one that has rows)
+      block = 0;
       ++z;
       continue;
     }
-    // (a division of 64 bits takes a microsecond)
-    const int64_t rel = u - first;
-    const int block = rel >> 32 == 0 ? (int)((uint32_t)rel / (uint32_t)s.tiles) : (int)(rel / s.tiles), j0 = (int)(rel - (int64_t)block * s.tiles);
-    const int n_tiles = (int)(u_end - u < s.tiles - j0 ? u_end - u : s.tiles - j0);
+    const int lane = own_lane(), c = lane & 31, hi = lane >> 5;
+    const int block_tiles = __builtin_amdgcn_readfirstlane(s.tiles_of(a, block));
+    // (a cut beside the tiles leaves the block to one side of it)
+    auto tile_of = [&](int64_t x) {
+      const int64_t n = x - at_unit - a.margin;
+      return __builtin_amdgcn_readfirstlane(n < 0 ? 0 : n < block_tiles ? (int)n : block_tiles);
+    };
+    const int j0 = tile_of(u), n_tiles = tile_of(u_end) - j0;
+    if (n_tiles <= 0) {
+      at_unit += block_tiles + 2 * a.margin;
+      ++block;
+      continue;
+    }
     const int rows = s.tokens * a.hq, w0 = block * a.block_rows + rw * 32, w_last = w0 + 31 < rows ? w0 + 31 : rows - 1;
     const bool row_ok = w0 + c < rows;
     const int row = row_ok ? w0 + c : rows - 1, token = row / a.hq, head = row - token * a.hq;
@@ -203,7 +266,7 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     auto fetch_page = [&](int j) __attribute__((always_inline)) {
       f_entry = (j - j0) * 2;
       f_page = pages.at(f_entry + wave / 2);
-      f_lds = stage_of(j);
+      f_lds = __builtin_amdgcn_readfirstlane(stage_of(j));
     };
     auto fetch_rows = [&](int j) __attribute__((always_inline)) {
       const int n = j * 32 + wave * 8;
@@ -243,58 +306,77 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
       for (int i = 0; i < kPieces; ++i) fetch_piece(i);
       return fetch_holes();
     };
-    auto k_read = [&](int X, int at_e, int at_r, int k) __attribute__((always_inline)) {
-      return k < KE ? lds_read<op_t>((at_e ^ ((k & 7) << 5)) + X + (k >> 3) * 256) : lds_read<op_t>((at_r ^ ((k - KE) << 5)) + X + SM::A);
-    };
-    // Q passes through the last RW stages as tiles of 32 rows, as the latent rows do: whole rows of memory, each once (as a lane's row in pieces
-    // straight into registers it took 11 us for 128 rows).
-    {
+    // Q passes through LDS as tiles of 32 rows, as the latent rows do: whole rows of memory, each once (as a lane's row in pieces straight into
+    // registers it took 11 us for 128 rows).  It lies behind the first kFirst stages, whose tiles are on their way with it; where it does not fit
+    // there, it comes in two halves of its columns.
+    auto fetch_q = [&](auto half) __attribute__((always_inline)) {
+      constexpr int H = decltype(half)::value, at_col = H * SM::template Q<RW>::COLUMNS, QC = SM::template Q<RW>::COLUMNS, QL = QC / 8, QR = 64 / QL;
+      constexpr bool ends = H == SM::template Q<RW>::HALVES - 1;
       const int r0 = block * a.block_rows, tb = r0 / a.hq, t_end = (r0 + a.block_rows - 1 < rows ? r0 + a.block_rows - 1 : rows - 1) / a.hq;
       const u32x4_t rs = wave_rsrc_words(reinterpret_cast<const T*>(a.q) + (int64_t)(s.start + tb) * a.q_row,
                                          (int)(((t_end - tb) * a.q_row + (a.hq - 1) * a.q_head + e) * 2));
       const int q_row = (int)a.q_row * 2, q_head = (int)a.q_head * 2;
 #pragma unroll
       for (int g = 0; g < RW; ++g) {
-        const int R = r0 + g * 32 + wave * 8, lds = smem0 + (SM::STAGES - RW + g) * SM::STAGE, lds_a = lds + wave * 8 * EA * 2;
-        const int l = own_lane(), lrow = l / LPR, base = (l % LPR) ^ Swz<EA>::f(lrow + 8 * (wave & 1)), tail_ch = (l % 8) ^ Swz<kLatentTail>::f(8 * (wave & 1) + l / 8);
+        const int R = r0 + g * 32 + wave * 8, lds = smem0 + SM::template Q<RW>::at(H, g), lds_a = lds + wave * 8 * QC * 2;
+        const int l = own_lane(), lrow = l / QL, base = (l % QL) ^ Swz<QC>::f(lrow + 8 * (wave & 1)), tail_ch = (l % 8) ^ Swz<kLatentTail>::f(8 * (wave & 1) + l / 8);
         int t = __builtin_amdgcn_readfirstlane(R / a.hq), h = R - t * a.hq, off[8], tail = kVoffOutOfRange;
         t -= tb;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           off[i] = R + i < rows ? t * q_row + h * q_head : -1;
           if (l / 8 == i && off[i] >= 0 && EA + tail_ch * 8 < e) tail = off[i] + (EA + tail_ch * 8) * 2;
-          if (++h == a.hq) { h = 0; ++t; }
+          const bool wraps = h + 1 == a.hq;
+          h = wraps ? 0 : h + 1;
+          t += wraps ? 1 : 0;
         }
+        static_assert(QR == 1 || QR == 2, "f of a row is that of its access and that of its place in it");
 #pragma unroll
-        for (int i = 0; i < 8 / RPL; i += 2) {
+        for (int i = 0; i < 8 / QR; i += 2) {
           int voff[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const int at = RPL == 1 ? off[i + k] : lrow ? off[(i + k) * RPL + RPL - 1] : off[(i + k) * RPL], ch = base ^ Swz<EA>::f((i + k) * RPL);
-            voff[k] = at >= 0 && (!kCut || ch * 8 < e) ? at + (ch << 4) : kVoffOutOfRange;
+            const int at = QR == 1 ? off[i + k] : lrow ? off[(i + k) * QR + QR - 1] : off[(i + k) * QR], ch = base ^ Swz<QC>::f((i + k) * QR);
+            voff[k] = at >= 0 && (!kCut || at_col + ch * 8 < e) ? at + at_col * 2 + (ch << 4) : kVoffOutOfRange;
           }
           load_to_lds(rs, voff[0], 0, lds_a + i * 1024, voff[1], 0, lds_a + (i + 1) * 1024);
         }
-        load_to_lds1(rs, tail, lds + SM::A + wave * 1024);
+        if (ends) load_to_lds1(rs, tail, lds + 32 * QC * 2 + wave * 1024);
       }
-    }
-    // (pages are looked up 32 tiles at a time; as many tiles as Q leaves room for are on their way with it)
-    int holes = 0, holes1 = 0, holes2 = 0;      // of this tile, the next, the one behind it
-    if (RW <= 3) holes = fetch(j0);
-    if (RW <= 2) holes1 = fetch(j0 + 1);
-    if (RW <= 1) holes2 = fetch(j0 + 2);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((SM::STAGES - RW) * kLoads) : "memory");
+    };
     op_t q[KE + KR];
-    {
-      const int X = smem0 + (SM::STAGES - RW + rw) * SM::STAGE, at_e = Swz<EA>::row_base(own_lane()), at_r = Swz<kLatentTail>::row_base(own_lane());
+    auto take_q = [&](auto half) __attribute__((always_inline)) {
+      constexpr int H = decltype(half)::value, QC = SM::template Q<RW>::COLUMNS, N = QC / 16;
+      const int X = smem0 + SM::template Q<RW>::at(H, rw), q_e = Swz<QC>::row_base(own_lane()), q_r = Swz<kLatentTail>::row_base(own_lane());
 #pragma unroll
-      for (int k = 0; k < KE + KR; ++k) q[k] = k_read(X, at_e, at_r, k);
+      for (int k = 0; k < N; ++k) q[H * N + k] = lds_read<op_t>((q_e ^ ((k & 7) << 5)) + X + (k >> 3) * 256);
+      if (H == SM::template Q<RW>::HALVES - 1) {
+#pragma unroll
+        for (int k = 0; k < KR; ++k) q[KE + k] = lds_read<op_t>((q_r ^ (k << 5)) + X + 32 * QC * 2);
+      }
+    };
+    using zero = std::integral_constant<int, 0>;
+    using one = std::integral_constant<int, 1>;
+    // (pages are looked up 32 tiles at a time, and where the compiler waits for them it waits for Q too)
+    constexpr int kFirst = SM::template Q<RW>::FIRST;
+    int holes = 0, holes1 = 0, holes2 = 0;      // of this tile, the next, the one behind it
+    fetch_q(zero{});
+    holes = fetch(j0);
+    holes1 = fetch(j0 + 1);
+    if (kFirst > 2) holes2 = fetch(j0 + 2);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kFirst * kLoads) : "memory");
+    take_q(zero{});
+    if constexpr (SM::template Q<RW>::HALVES == 2) {
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      fetch_q(one{});
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      take_q(one{});
     }
     arrived(q);
-    if (RW > 1) asm volatile("s_barrier" ::: "memory");      // (all waves have their rows)
-    if (RW > 3) holes = fetch(j0);
-    if (RW > 2) holes1 = fetch(j0 + 1);
-    if (RW > 1) holes2 = fetch(j0 + 2);
+    if (kFirst < SM::STAGES - 1) {
+      asm volatile("s_barrier" ::: "memory");      // (all waves have their rows)
+      holes2 = fetch(j0 + 2);
+    }
     f32x16 o[DB];
 #pragma unroll
     for (int b = 0; b < DB; ++b) {
@@ -459,10 +541,10 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     if (a.heads != nullptr && j0 == 0) {
       const int at = latent_block(a, z, s.start) + block;
       if (at < a.blocks && threadIdx.x == 0) {
-        a.heads[at] = n_tiles < s.tiles ? LatentHead{(int)(worker * 2 + (u == worker * cut.per ? 0 : 1)), (int)((u + s.tiles - 1) / cut.per - worker) + 1, s.start, block, rows}
+        a.heads[at] = n_tiles < block_tiles ? LatentHead{(int)worker * 2 + 1, (int)latent_div(at_unit + a.margin + block_tiles - 1 - u, cut.per) + 1, s.start, block, rows}
                                         : LatentHead{0, 0, 0, 0, 0};
       }
-      if (u == 0) put_heads(0, at);
+      if (at_unit == 0) put_heads(0, at);
       if (block == s.blocks - 1) {
         int next = a.blocks;
         for (int y = z + 1; y < ca.sequences; ++y) {
@@ -475,17 +557,19 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
         put_heads(at + 1, next);
       }
     }
-    if (n_tiles < s.tiles) {      // a piece: the first of the worker, or its last
-      const int place = u == worker * cut.per ? 0 : 1;
-      const int64_t at = (worker * 2 + place) * RW + rw;
-      float* to = a.part_o + at * (EA / 32 * 1024) + cg * DB * 1024 + tail_lane * 4;
-#pragma unroll
-      for (int b = 0; b < DB; ++b) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4*>(to + (4 * b + g) * 256) = f32x4{o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
-        __builtin_amdgcn_sched_barrier(0);
+    if (n_tiles < block_tiles) {      // a piece, the first of the worker or its last
+      if (w0 < rows) {
+        const int place = j0 > 0 ? 0 : 1;
+        const int64_t at = (worker * 2 + place) * RW + rw;
+        float* to = a.part_o + at * (EA / 32 * 1024) + cg * DB * 1024 + tail_lane * 4;
+  #pragma unroll
+        for (int b = 0; b < DB; ++b) {
+  #pragma unroll
+          for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4*>(to + (4 * b + g) * 256) = f32x4{o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (cg == 0) a.part_ml[at * 64 + tail_lane] = tail_lane < 32 ? sm.m : sum;
       }
-      if (cg == 0) a.part_ml[at * 64 + tail_lane] = tail_lane < 32 ? sm.m : sum;
     } else {
       // O passes through the wave's stage, so that rows go out whole (as a lane's row in pieces of 8 bytes: 19 us for 128 rows)
       constexpr int W = DB * 32, ROW = W * 2 + 16, LPO = W / 8, RPO = 64 / LPO;
@@ -514,7 +598,8 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
         if (w0 + r1 < rows && col < ev) *reinterpret_cast<u32x4_t*>(to + at) = y;
       }
     }
-    u += n_tiles;
+    at_unit += block_tiles + 2 * a.margin;
+    ++block;
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (what comes next takes the rows' place)
   }
 }
