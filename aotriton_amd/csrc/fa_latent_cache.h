@@ -605,7 +605,7 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
 }
 
 // The pieces of a block put together: a workgroup per 32 rows and `wide` blocks of 32 columns.  A block that one worker had is written already.
-// Bound by round trips to memory for few rows (hence eight pieces at a time: 33 of them one after the other took 22 us), by the pieces' bytes for many.
+// Bound by round trips to memory for few rows (hence 16 loads at a time: 33 pieces one after the other took 22 us), by the pieces' bytes for many.
 template <typename T, int EA, int RW>
 __global__ __launch_bounds__(256) void latent_cache_sum_kernel(const LatentCacheArgs a, int wide) {
   constexpr int DB = EA / 32;
@@ -620,19 +620,23 @@ __global__ __launch_bounds__(256) void latent_cache_sum_kernel(const LatentCache
   const float sc = score_scale(a.sm_scale, false);
   const int token = row / a.hq, head = row - token * a.hq;
   T* out = reinterpret_cast<T*>(a.out) + (int64_t)(head_of.start + token) * a.o_row + (int64_t)head * a.o_head;
-  for (int db = db0; db < db0 + wide; ++db) {
+  // N pieces of W blocks of columns at a time
+  auto columns = [&](auto n, auto w, int db) __attribute__((always_inline)) {
+    constexpr int N = decltype(n)::value, W = decltype(w)::value;
     float m = kNegBig, l = 0.f;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    constexpr int N = 8;
+    f32x4 x[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int w = w0; w <= w1; w += N) {
       float pm[N], pl[N];
-      f32x4 px[N];
+      f32x4 px[N][W];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int64_t p = at(w + i < w1 ? w + i : w1);
         pm[i] = a.part_ml[p * 64 + c];
         pl[i] = a.part_ml[p * 64 + 32 + c];
-        px[i] = *reinterpret_cast<const f32x4*>(a.part_o + p * (DB * 1024) + db * 1024 + tid * 4);
+#pragma unroll
+        for (int k = 0; k < W; ++k) px[i][k] = *reinterpret_cast<const f32x4*>(a.part_o + p * (DB * 1024) + (db + k) * 1024 + tid * 4);
       }
       float top = m;
 #pragma unroll
@@ -640,23 +644,36 @@ __global__ __launch_bounds__(256) void latent_cache_sum_kernel(const LatentCache
       const float f = fast_exp2((m - top) * sc);
       m = top;
       l *= f;
-      x *= f;
+#pragma unroll
+      for (int k = 0; k < W; ++k) x[k] *= f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float g = w + i <= w1 ? fast_exp2((pm[i] - top) * sc) : 0.f;
+        if (w + i > w1) continue;
+        const float g = fast_exp2((pm[i] - top) * sc);
         l += g * pl[i];
-        if (w + i <= w1) x += g * px[i];
+#pragma unroll
+        for (int k = 0; k < W; ++k) x[k] += g * px[i][k];
       }
     }
     const float f = l == 0.f ? 0.f : 1.0f / l;
-    const int col = 32 * db + 8 * (tid >> 6) + 4 * hi;
-    typename Traits<T>::q4_t y;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(x[r] * f);
-    if (col < a.cache.head_dim_v) *reinterpret_cast<typename Traits<T>::q4_t*>(out + col) = y;
+    for (int k = 0; k < W; ++k) {
+      const int col = 32 * (db + k) + 8 * (tid >> 6) + 4 * hi;
+      typename Traits<T>::q4_t y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(x[k][r] * f);
+      if (col < a.cache.head_dim_v) *reinterpret_cast<typename Traits<T>::q4_t*>(out + col) = y;
+    }
     if (a.lse != nullptr && db == 0 && tid < 32)
       a.lse[(int64_t)(head_of.start + token) * a.hq + head] = l == 0.f ? __builtin_inff() : __builtin_fmaf(m, sc, fast_log2(l)) * kLn2;
-  }
+  };
+  using std::integral_constant;
+  int db = db0;
+  if (head_of.pieces <= 4)
+    for (; db + 4 <= db0 + wide; db += 4) columns(integral_constant<int, 4>{}, integral_constant<int, 4>{}, db);
+  if (head_of.pieces <= 8)
+    for (; db + 2 <= db0 + wide; db += 2) columns(integral_constant<int, 8>{}, integral_constant<int, 2>{}, db);
+  for (; db < db0 + wide; ++db) columns(integral_constant<int, 16>{}, integral_constant<int, 1>{}, db);
 }
 
 template <typename T, int EA, int RW, bool kCut> hipError_t launch_latent_cache_main(const LatentCacheArgs& a, hipStream_t s) {
