@@ -53,6 +53,8 @@ EXTRA = {
     'fa_tree_d128.hip': ['-Wno-inline-asm'],
     'fa_latent_d64.hip': ['-Wno-inline-asm'],
     'fa_latent_d128.hip': ['-Wno-inline-asm'],
+    'fa_latent_keys_d64.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', '-Wno-inline-asm'],
+    'fa_latent_keys_d128.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form', '-Wno-inline-asm'],
     'fa_latent_cache_d256.hip': ['-Wno-inline-asm'],
     'fa_latent_cache_d512.hip': ['-Wno-inline-asm'],
     # (scores in vector registers, results as asm operands in accumulation registers)

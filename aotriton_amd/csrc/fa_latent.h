@@ -1,4 +1,4 @@
-// Attention whose keys are part per head, part shared by all heads, forward and backward: gfx950, MFMA 32x32x16.
+// Attention whose keys are part per head, part shared by all heads, forward and dQ (dK, dV and dC: fa_latent_keys.h): gfx950, MFMA 32x32x16.
 //
 //   S = scale (Qe K^T + Qr C^T),  P = softmax(S),  O = P V
 //   dV = P^T dO,  dS = P (dO V^T - rowsum(dO O)),  dQ = scale [dS K | dS C],  dK = scale dS^T Qe,  dC = scale sum over heads of dS^T Qr
@@ -37,33 +37,50 @@ template <int D> struct TileRows {
   }
 };
 
-// Rows of a wave as MFMA operands in registers, row lane % 32: columns [col0, col0 + cols) of the first `rows` rows, zeros elsewhere.
-template <typename T, int N>
-__device__ __forceinline__ void load_operands(typename Traits<T>::op_t* x, const void* base, int row_bytes, int rows, int lane, int col0, int cols) {
-  using op_t = typename Traits<T>::op_t;
-  const auto rs = wave_rsrc(base, rows_extent(rows, row_bytes, (col0 + cols) * 2));
-  const int c = lane & 31, hi = lane >> 5;
+// A wave's 32 rows on their way into `lds`, as TileRows has them: columns [col0, col0 + cols) of the first `rows` rows, zeros elsewhere.  From there they
+// go into registers, and results back the same way: whole rows of memory, which a lane's row in pieces of 8 or 16 bytes leaves to the caches
+// (a block of dK/dV spent 35 us on that, as much as on twelve of its tiles).
+template <int D>
+__device__ __forceinline__ void fetch_rows(const void* base, int row_bytes, int rows, int lane, int col0, int cols, int lds) {
+  const TileRows<D> t(lane, row_bytes, col0, cols);
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int col = 16 * k + 8 * hi;
-    x[k] = __builtin_bit_cast(op_t, __builtin_amdgcn_raw_buffer_load_b128(rs, col < cols && c < rows ? c * row_bytes + (col0 + col) * 2 : kVoffOutOfRange, 0, 0));
-  }
+  for (int i = 0; i < 2; ++i)
+    t.fetch(wave_rsrc_words(reinterpret_cast<const char*>(base) + (int64_t)(16 * i) * row_bytes, rows_extent(rows - 16 * i < 16 ? rows - 16 * i : 16, row_bytes, (col0 + cols) * 2)),
+            lds + i * 16 * 2 * D);
+}
+// as MFMA operands, row lane % 32
+template <typename T, int D>
+__device__ __forceinline__ void take_rows(typename Traits<T>::op_t* x, int lane, int lds) {
+  const int at = Swz<D>::row_base(lane);
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) x[k] = lds_read<typename Traits<T>::op_t>((at ^ (k << 5)) + lds);
 }
 
-// A transposed accumulator (columns x 32 rows) times `f` to row lane % 32 of a tensor, columns [0, cols).
+// A transposed accumulator (columns x 32 rows) times `f` to the first `rows` rows of a tensor, columns [0, cols), through the wave's piece of LDS (RowsOut bytes).
+template <typename T, int NB> constexpr int kRowsOut = 32 * (NB * 32 * (int)sizeof(T) + 16);
 template <typename T, int NB>
-__device__ __forceinline__ void store_rows(const f32x16* x, float f, T* row, int cols, int hi) {
-  using q4_t = typename Traits<T>::q4_t;
+__device__ __forceinline__ void store_rows(const f32x16* x, float f, T* to, int64_t stride, int rows, int cols, int lane, int lds) {
+  constexpr int ROW = NB * 32 * (int)sizeof(T) + 16, LPR = NB * 32 * (int)sizeof(T) / 16, RPL = 64 / LPR, PER = 16 / (int)sizeof(T);
+  const int c = lane & 31, hi = lane >> 5;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int col = 32 * b + 8 * g + 4 * hi;
-      q4_t y;
+      vec<T, 4> y;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(x[b][4 * g + r] * f);
-      if (col < cols) *reinterpret_cast<q4_t*>(row + col) = y;
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (sizeof(T) == 4) y[r] = x[b][4 * g + r] * f;
+        else y[r] = Traits<T>::cvt(x[b][4 * g + r] * f);
+      }
+      lds_write(lds + c * ROW + (32 * b + 8 * g + 4 * hi) * (int)sizeof(T), y);
     }
+  const int ch = lane % LPR;
+#pragma unroll
+  for (int i = 0; i < 32 / RPL; ++i) {
+    const int r = i * RPL + lane / LPR;
+    const u32x4_t y = lds_read<u32x4_t>(lds + r * ROW + ch * 16);
+    if (r < rows && ch * PER < cols) *reinterpret_cast<u32x4_t*>(to + r * stride + ch * PER) = y;
+  }
 }
 
 __device__ __forceinline__ void latent_meet() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -73,7 +90,9 @@ template <int EC> struct LatentSmem {
   static constexpr int C_OFF = TILE, V_OFF = TILE + SHARED;
   static constexpr int STAGE = 2 * TILE + SHARED;      // K, C, V (dK/dV: Q, its shared part, dO)
   static constexpr int STATS = 2 * 64 * 4;
-  static constexpr int BYTES = 2 * STAGE, BWD_BYTES = 2 * (STAGE + STATS);
+  static constexpr int BYTES = 2 * STAGE, BWD_STAGE = STAGE + STATS, BWD_BYTES = 3 * BWD_STAGE;
+  // a wave's own rows before and after the loop over tiles: two tensors of EC columns, then one of the shared part
+  static constexpr int WAVE = STAGE / 2, WAVE_V = 32 * EC * 2, WAVE_C = 2 * WAVE_V;
 };
 
 // (the offsets of packed sequences are held inside the tensors, and lengths inside the greatest: what lies past them is not there)
@@ -142,16 +161,20 @@ __global__ __launch_bounds__(256, 2) void latent_fwd_kernel(const LatentArgs a, 
     ct.fetch(wave_rsrc_words(row_at<T>(a.c, Strides3{a.c_z, 0, a.c_s}, si, 0, at), rows_extent(left, c_row, a.r * 2)),
              smem0 + stage * SM::STAGE + SM::C_OFF + wave * 16 * 2 * kLatentShared);
   };
-  if (j0 < j1) fetch(0, j0);
-
   op_t q[KE + KR];
   {
     const T* qp = row_at<T>(a.q, a.sq, si, h, (int64_t)si.q_start + w0);
-    load_operands<T, KE>(q, qp, (int)a.sq.s * 2, rows, lane, 0, a.e);
-    load_operands<T, KR>(q + KE, qp, (int)a.sq.s * 2, rows, lane, a.e, a.r);
+    const int own = smem0 + wave * SM::WAVE;
+    fetch_rows<EC>(qp, (int)a.sq.s * 2, rows, lane, 0, a.e, own);
+    fetch_rows<kLatentShared>(qp, (int)a.sq.s * 2, rows, lane, a.e, a.r, own + SM::WAVE_C);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    take_rows<T, EC>(q, lane, own);
+    take_rows<T, kLatentShared>(q + KE, lane, own + SM::WAVE_C);
   }
   // (Q has to be there before the loop: left to the first use in it the compiler waits there, in every round, for all that is on its way)
   arrived(q);
+  latent_meet();
+  if (j0 < j1) fetch(0, j0);
   f32x16 o[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -203,10 +226,10 @@ __global__ __launch_bounds__(256, 2) void latent_fwd_kernel(const LatentArgs a, 
     store_part<DB>(a.part_o, a.part_ml, (((int64_t)(z * a.heads + h) * tiles + mt) * 4 + wave) * a.parts + part, o, sm, lane);
     return;
   }
-  if (row >= si.seqlen_q) return;
   const float l = cross_sum(sm.l);
-  store_rows<T, DB>(o, l == 0.f ? 0.f : 1.0f / l, row_at<T>(a.out, a.so, si, h, (int64_t)si.q_start + row), a.ev, hi);
-  if (a.lse != nullptr && hi == 0) a.lse[lse_offset(si, h, a.heads) + row] = sm.lse(l);
+  if (a.lse != nullptr && hi == 0 && row < si.seqlen_q) a.lse[lse_offset(si, h, a.heads) + row] = sm.lse(l);
+  latent_meet();
+  store_rows<T, DB>(o, l == 0.f ? 0.f : 1.0f / l, row_at<T>(a.out, a.so, si, h, (int64_t)si.q_start + w0), a.so.s, rows, a.ev, lane, smem0 + wave * SM::WAVE);
 }
 
 // the parts' sums of 32 rows and 32 columns put together
@@ -266,15 +289,22 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
     ct.fetch(wave_rsrc_words(row_at<T>(a.c, Strides3{a.c_z, 0, a.c_s}, si, 0, at), rows_extent(left, c_row, a.r * 2)),
              smem0 + stage * SM::STAGE + SM::C_OFF + wave * 16 * 2 * kLatentShared);
   };
-  if (j1 > 0) fetch(0, 0);
-
   op_t q[KE + KR], dout[KE];
+  const int own = smem0 + wave * SM::WAVE;
   {
     const T* qp = row_at<T>(a.q, a.sq, si, h, (int64_t)si.q_start + w0);
-    load_operands<T, KE>(q, qp, (int)a.sq.s * 2, rows, lane, 0, a.e);
-    load_operands<T, KR>(q + KE, qp, (int)a.sq.s * 2, rows, lane, a.e, a.r);
-    load_operands<T, KE>(dout, row_at<T>(a.dout, a.sdo, si, h, (int64_t)si.q_start + w0), (int)a.sdo.s * 2, rows, lane, 0, a.ev);
+    fetch_rows<EC>(qp, (int)a.sq.s * 2, rows, lane, 0, a.e, own);
+    fetch_rows<EC>(row_at<T>(a.dout, a.sdo, si, h, (int64_t)si.q_start + w0), (int)a.sdo.s * 2, rows, lane, 0, a.ev, own + SM::WAVE_V);
+    fetch_rows<kLatentShared>(qp, (int)a.sq.s * 2, rows, lane, a.e, a.r, own + SM::WAVE_C);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    take_rows<T, EC>(q, lane, own);
+    take_rows<T, EC>(dout, lane, own + SM::WAVE_V);
+    take_rows<T, kLatentShared>(q + KE, lane, own + SM::WAVE_C);
   }
+  arrived(q);
+  arrived(dout);
+  latent_meet();
+  if (j1 > 0) fetch(0, 0);
   // delta of few keys is summed from P and dP in a pass of its own, else from O: of O's rounding as much is left as the keys that weigh in
   // have not averaged out, and with few of them it is the largest error of the gradients (two thirds of dQ's products once more, for rows
   // whose tiles are few).
@@ -283,14 +313,15 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
   if (row < si.seqlen_q) lse = a.lse[lse_offset(si, h, a.heads) + row] * kLog2e;
   if (!few) {
     op_t out[KE];
-    load_operands<T, KE>(out, row_at<T>(a.out, a.so, si, h, (int64_t)si.q_start + w0), (int)a.so.s * 2, rows, lane, 0, a.ev);
+    const int place = smem0 + SM::STAGE + wave * SM::WAVE_V;      // (in the other stage)
+    fetch_rows<EC>(row_at<T>(a.out, a.so, si, h, (int64_t)si.q_start + w0), (int)a.so.s * 2, rows, lane, 0, a.ev, place);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    take_rows<T, EC>(out, lane, place);
 #pragma unroll
     for (int k = 0; k < KE; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta += (float)out[k][i] * (float)dout[k][i];
   }
-  arrived(q);
-  arrived(dout);
   const float qs = a.sm_scale * kLog2e;
   // P and dP of 32 keys of tile j
   auto products = [&](const char* K, int j, int b, f32x16& p, f32x16& dp) __attribute__((always_inline)) {
@@ -361,142 +392,11 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
       }
     }
   }
-  if (row >= si.seqlen_q) return;
-  T* to = row_at<T>(a.dq, a.sdq, si, h, (int64_t)si.q_start + row);
-  store_rows<T, DB>(dq, a.sm_scale, to, a.e, hi);
-  store_rows<T, RB>(dq + DB, a.sm_scale, to + a.e, a.r, hi);
-}
-
-// ---- dK, dV and every head's part of dC -----------------------------------------------------------------------------
-// A wave owns 32 keys, a lane one of them, with K, C and V as operands in registers; tiles of 64 queries pass.
-template <typename T, int EC>
-__global__ __launch_bounds__(256, EC == 64 ? 2 : 1) void latent_dkdv_kernel(const LatentBwdArgs a, int nseq, int tiles) {
-  using Tr = Traits<T>;
-  using op_t = typename Tr::op_t;
-  using SM = LatentSmem<EC>;
-  constexpr int KE = EC / 16, KR = kLatentShared / 16, DB = EC / 32, RB = kLatentShared / 32;
-  extern __shared__ __attribute__((aligned(kSwzAlign))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hi = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int z, h, nt;
-  latent_item(a, blockIdx.x, nseq, tiles, false, z, h, nt);
-  const SeqInfo si = latent_seq(a, z);
-  if (nt * 128 >= si.seqlen_k) return;
-  const int shift = si.seqlen_k - si.seqlen_q;
-  const int w0 = nt * 128 + wave * 32, key = w0 + c, keys = si.seqlen_k - w0;
-  // the first query that sees a key
-  auto first_query = [&](int n) { return a.causal && n - shift > 0 ? n - shift : 0; };
-  const int j0 = first_query(nt * 128) / 64, j1 = (si.seqlen_q + 63) / 64;
-
-  const int smem0 = lds_offset(smem);
-  const int q_row = (int)a.sq.s * 2, do_row = (int)a.sdo.s * 2;
-  const TileRows<EC> qt(lane, q_row, 0, a.e), dt(lane, do_row, 0, a.ev);
-  const TileRows<kLatentShared> rt(lane, q_row, a.e, a.r);
-  const float* stats = (wave & 1 ? a.stat_delta : a.stat_lse) + lse_offset(si, h, a.heads);
-  auto fetch = [&](int stage, int j) __attribute__((always_inline)) {
-    const int m = j * 64 + wave * 16, left = si.seqlen_q - m < 16 ? si.seqlen_q - m : 16;
-    const int64_t at = si.q_start + m;
-    const int base = smem0 + stage * (SM::STAGE + SM::STATS), lds = base + wave * 16 * 2 * EC;
-    const auto q_rs = wave_rsrc_words(row_at<T>(a.q, a.sq, si, h, at), rows_extent(left, q_row, (a.e + a.r) * 2));
-    qt.fetch(q_rs, lds);
-    rt.fetch(q_rs, base + SM::C_OFF + wave * 16 * 2 * kLatentShared);
-    dt.fetch(wave_rsrc_words(row_at<T>(a.dout, a.sdo, si, h, at), rows_extent(left, do_row, a.ev * 2)), lds + SM::V_OFF);
-    // (of a row past the sequence Q, dO and both statistics are 0: nothing comes of it)
-    if (wave < 2) {
-      const int n = si.seqlen_q - j * 64 < 64 ? si.seqlen_q - j * 64 : 64;
-      load_word_to_lds(wave_rsrc_words(stats + j * 64, n > 0 ? n * 4 : 0), lane * 4, base + SM::STAGE + wave * 256);
-    }
-  };
-  if (j0 < j1) fetch(0, j0);
-
-  op_t k[KE + KR], v[KE];
-  load_operands<T, KE>(k, row_at<T>(a.k, a.sk, si, h, (int64_t)si.k_start + w0), (int)a.sk.s * 2, keys, lane, 0, a.e);
-  load_operands<T, KR>(k + KE, row_at<T>(a.c, Strides3{a.c_z, 0, a.c_s}, si, 0, (int64_t)si.k_start + w0), (int)a.c_s * 2, keys, lane, 0, a.r);
-  load_operands<T, KE>(v, row_at<T>(a.v, a.sv, si, h, (int64_t)si.k_start + w0), (int)a.sv.s * 2, keys, lane, 0, a.ev);
-  arrived(k);
-  arrived(v);
-  f32x16 dk[DB + RB], dv[DB];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-#pragma unroll
-    for (int b = 0; b < DB + RB; ++b) dk[b][i] = 0.f;
-#pragma unroll
-    for (int b = 0; b < DB; ++b) dv[b][i] = 0.f;
-  }
-  const float qs = a.sm_scale * kLog2e;
-  const int row_e = Swz<EC>::row_base(lane), row_r = Swz<kLatentShared>::row_base(lane);
-  const int tr0 = Swz<EC>::tr_base(lane, 0), tr1 = Swz<EC>::tr_base(lane, 1);
-  const int rr0 = Swz<kLatentShared>::tr_base(lane, 0), rr1 = Swz<kLatentShared>::tr_base(lane, 1);
-
-  for (int j = j0; j < j1; ++j) {
-    latent_meet();
-    const int stage = (j - j0) & 1;
-    if (j + 1 < j1) fetch(stage ^ 1, j + 1);
-    const char* Q = smem + stage * (SM::STAGE + SM::STATS);
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int m0 = j * 64 + 32 * b;
-      if (m0 + 31 < first_query(w0)) continue;      // none of its queries sees a key of the wave
-      const bool masked = a.causal && m0 < w0 + 31 - shift;
-      f32x16 s, dp;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-#pragma unroll
-      for (int x = 0; x < KE; ++x) s = Tr::mfma(swz_read_row<T, EC>(Q, row_e, x, b), k[x], s);
-#pragma unroll
-      for (int x = 0; x < KR; ++x) s = Tr::mfma(swz_read_row<T, kLatentShared>(Q + SM::C_OFF, row_r, x, b), k[KE + x], s);
-#pragma unroll
-      for (int x = 0; x < KE; ++x) dp = Tr::mfma(swz_read_row<T, EC>(Q + SM::V_OFF, row_e, x, b), v[x], dp);
-      const int from = key - shift - m0 - 4 * hi;      // the lane's key is seen from this row of the block on
-      const float* st = reinterpret_cast<const float*>(Q + SM::STAGE) + 32 * b + 4 * hi;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 8 * g), delta = *reinterpret_cast<const f32x4*>(st + 64 + 8 * g);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 4 * g + r;
-          float p = fast_exp2(__builtin_fmaf(s[i], qs, -lse[r]));
-          if (masked && 8 * g + r < from) p = 0.f;
-          dp[i] = p * (dp[i] - delta[r]);
-          s[i] = p;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const op_t p = pack8<T>(s, t), ds = pack8<T>(dp, t);
-#pragma unroll
-        for (int x = 0; x < DB; ++x) dv[x] = Tr::mfma(swz_read_tr<T, EC>(Q + SM::V_OFF, tr0, tr1, 2 * b + t, x), p, dv[x]);
-#pragma unroll
-        for (int x = 0; x < DB; ++x) dk[x] = Tr::mfma(swz_read_tr<T, EC>(Q, tr0, tr1, 2 * b + t, x), ds, dk[x]);
-#pragma unroll
-        for (int x = 0; x < RB; ++x) dk[DB + x] = Tr::mfma(swz_read_tr<T, kLatentShared>(Q + SM::C_OFF, rr0, rr1, 2 * b + t, x), ds, dk[DB + x]);
-      }
-    }
-  }
-  if (key >= si.seqlen_k) return;
-  store_rows<T, DB>(dk, a.sm_scale, row_at<T>(a.dk, a.sdk, si, h, (int64_t)si.k_start + key), a.e, hi);
-  store_rows<T, DB>(dv, 1.0f, row_at<T>(a.dv, a.sdv, si, h, (int64_t)si.k_start + key), a.ev, hi);
-  float* to = a.part_c + (((int64_t)si.batch_index * a.heads + h) * a.part_rows + si.k_start + key) * kLatentShared + 4 * hi;
-#pragma unroll
-  for (int x = 0; x < RB; ++x)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4*>(to + 32 * x + 8 * g) = f32x4{dk[DB + x][4 * g], dk[DB + x][4 * g + 1], dk[DB + x][4 * g + 2], dk[DB + x][4 * g + 3]};
-}
-
-// dC: the heads' parts added in their order, four columns a lane
-template <typename T>
-__global__ __launch_bounds__(256) void latent_dc_kernel(const LatentBwdArgs a, int64_t keys, const int32_t* end) {
-  const int64_t at = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-  const int64_t b = at / keys, n = at % keys;
-  const int col = threadIdx.x % 16 * 4;
-  if (b >= a.batch || (end != nullptr && n >= *end) || col >= a.r) return;
-  const float* from = a.part_c + (b * a.heads * a.part_rows + n) * kLatentShared + col;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int h = 0; h < a.heads; ++h) sum += *reinterpret_cast<const f32x4*>(from + (int64_t)h * a.part_rows * kLatentShared);
-  typename Traits<T>::q4_t y;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(sum[r] * a.sm_scale);
-  *reinterpret_cast<typename Traits<T>::q4_t*>(reinterpret_cast<T*>(a.dc) + b * a.dc_z + n * a.dc_s + col) = y;
+  latent_meet();
+  T* to = row_at<T>(a.dq, a.sdq, si, h, (int64_t)si.q_start + w0);
+  const int out_lane = own_lane();
+  store_rows<T, DB>(dq, a.sm_scale, to, a.sdq.s, rows, a.e, out_lane, own);
+  store_rows<T, RB>(dq + DB, a.sm_scale, to + a.e, a.sdq.s, rows, a.r, out_lane, own + kRowsOut<T, DB>);
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------
@@ -512,18 +412,13 @@ template <typename T, int EC> hipError_t launch_latent_fwd(const LatentArgs& a, 
   return hipGetLastError();
 }
 
-template <typename T, int EC> hipError_t launch_latent_bwd(const LatentBwdArgs& a, hipStream_t s) {
-  static std::atomic<uint64_t> done_q{0}, done_k{0};
-  const int nseq = nseq_of(a.seq, a.batch), q_tiles = (a.seq.max_seqlen_q + 127) / 128, k_tiles = (a.seq.max_seqlen_k + 127) / 128;
-  hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_dq_kernel<T, EC>), LatentSmem<EC>::BYTES, done_q);
-  if (e == hipSuccess) e = allow_large_lds(reinterpret_cast<const void*>(&latent_dkdv_kernel<T, EC>), LatentSmem<EC>::BWD_BYTES, done_k);
-  if (e != hipSuccess || nseq == 0) return e;
-  if (q_tiles > 0) hipLaunchKernelGGL((latent_dq_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * q_tiles)), dim3(256), LatentSmem<EC>::BYTES, s, a, nseq, q_tiles);
-  if (k_tiles > 0) {
-    hipLaunchKernelGGL((latent_dkdv_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * k_tiles)), dim3(256), LatentSmem<EC>::BWD_BYTES, s, a, nseq, k_tiles);
-    const int32_t* end = a.seq.num_seqlens != 0 ? a.seq.cu_k + nseq : nullptr;
-    hipLaunchKernelGGL((latent_dc_kernel<T>), dim3((unsigned)((a.batch * a.part_rows + 15) / 16)), dim3(256), 0, s, a, a.part_rows, end);
-  }
+template <typename T, int EC> hipError_t launch_latent_dq(const LatentBwdArgs& a, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  const int nseq = nseq_of(a.seq, a.batch), tiles = (a.seq.max_seqlen_q + 127) / 128;
+  if (nseq == 0 || tiles == 0) return hipSuccess;
+  hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_dq_kernel<T, EC>), LatentSmem<EC>::BYTES, done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((latent_dq_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles)), dim3(256), LatentSmem<EC>::BYTES, s, a, nseq, tiles);
   return hipGetLastError();
 }
 

@@ -64,6 +64,8 @@ hipError_t run_latent_fwd_d64(int dtype, const LatentArgs& a, hipStream_t s);
 hipError_t run_latent_fwd_d128(int dtype, const LatentArgs& a, hipStream_t s);
 hipError_t run_latent_bwd_d64(int dtype, const LatentBwdArgs& a, hipStream_t s);
 hipError_t run_latent_bwd_d128(int dtype, const LatentBwdArgs& a, hipStream_t s);
+hipError_t run_latent_keys_d64(int dtype, const LatentBwdArgs& a, hipStream_t s);      // dK, dV and dC, behind dQ
+hipError_t run_latent_keys_d128(int dtype, const LatentBwdArgs& a, hipStream_t s);
 // compiled columns in front of the last 64 (256 or 512)
 hipError_t run_latent_cache_d256(int dtype, const LatentCacheArgs& a, hipStream_t s);
 hipError_t run_latent_cache_d512(int dtype, const LatentCacheArgs& a, hipStream_t s);

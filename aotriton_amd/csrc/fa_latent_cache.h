@@ -151,15 +151,6 @@ __device__ __forceinline__ LatentCut latent_find(const LatentCacheArgs& a, char*
   return cut;
 }
 
-// Behind the last MFMA onto the accumulators, which the compiler does not see (fa_wide.h): 16 passes and what the register file takes.
-template <int DB> __device__ __forceinline__ void settle(f32x16 (&o)[DB]) {
-#pragma unroll
-  for (int b = 0; b < DB; ++b) asm volatile("" : "+a"(o[b]));
-  asm volatile("s_nop 15\n\ts_nop 15");
-#pragma unroll
-  for (int b = 0; b < DB; ++b) asm volatile("" : "+a"(o[b]));
-}
-
 // kCut: rows have fewer than EA columns; those past them are zero.
 template <typename T, int EA, int RW, bool kCut>
 __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheArgs a) {

@@ -1,0 +1,232 @@
+// dK, dV and dC of attention whose keys are part per head, part shared by all heads (fa_latent.h): gfx950, MFMA 32x32x16.
+#pragma once
+#include "fa_latent.h"
+
+namespace fa {
+
+// ---- dK, dV and every head's part of dC -----------------------------------------------------------------------------
+// A wave owns 32 keys, a lane one of them, with K, C and V as operands in registers; tiles of 64 queries pass, 32 of them at a time: in a round the
+// MFMAs of S and dP of the next 32 stand over the exponentials of these, then those of dV, dK and dC follow.  The wave is the only one on its
+// SIMD (dK, dV and dC take 160 accumulators), so that what is not behind an MFMA costs its time.
+template <typename T, int EC>
+__global__ __launch_bounds__(256, 1) void latent_dkdv_kernel(const LatentBwdArgs a, int nseq, int tiles) {
+  using Tr = Traits<T>;
+  using op_t = typename Tr::op_t;
+  using SM = LatentSmem<EC>;
+  constexpr int KE = EC / 16, KR = kLatentShared / 16, DB = EC / 32, RB = kLatentShared / 32;
+  extern __shared__ __attribute__((aligned(kSwzAlign))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int z, h, nt;
+  latent_item(a, blockIdx.x, nseq, tiles, false, z, h, nt);
+  const SeqInfo si = latent_seq(a, z);
+  if (nt * 128 >= si.seqlen_k) return;
+  const int shift = si.seqlen_k - si.seqlen_q;
+  const int w0 = nt * 128 + wave * 32, key = w0 + c, keys = si.seqlen_k - w0;
+  // the first query that sees a key
+  auto first_query = [&](int n) { return a.causal && n - shift > 0 ? n - shift : 0; };
+  const int j0 = first_query(nt * 128) / 64, j1 = (si.seqlen_q + 63) / 64;
+
+  const int smem0 = lds_offset(smem);
+  const int q_row = (int)a.sq.s * 2, do_row = (int)a.sdo.s * 2;
+  const TileRows<EC> qt(lane, q_row, 0, a.e), dt(lane, do_row, 0, a.ev);
+  const TileRows<kLatentShared> rt(lane, q_row, a.e, a.r);
+  const float* stats = (wave & 1 ? a.stat_delta : a.stat_lse) + lse_offset(si, h, a.heads);
+  auto fetch = [&](int stage, int j) __attribute__((always_inline)) {
+    const int m = j * 64 + wave * 16, left = si.seqlen_q - m < 16 ? si.seqlen_q - m : 16;
+    const int64_t at = si.q_start + m;
+    const int base = smem0 + stage * SM::BWD_STAGE, lds = base + wave * 16 * 2 * EC;
+    const auto q_rs = wave_rsrc_words(row_at<T>(a.q, a.sq, si, h, at), rows_extent(left, q_row, (a.e + a.r) * 2));
+    qt.fetch(q_rs, lds);
+    rt.fetch(q_rs, base + SM::C_OFF + wave * 16 * 2 * kLatentShared);
+    dt.fetch(wave_rsrc_words(row_at<T>(a.dout, a.sdo, si, h, at), rows_extent(left, do_row, a.ev * 2)), lds + SM::V_OFF);
+    // (of a row past the sequence Q, dO and both statistics are 0: nothing comes of it)
+    if (wave < 2) {
+      const int n = si.seqlen_q - j * 64 < 64 ? si.seqlen_q - j * 64 : 64;
+      load_word_to_lds(wave_rsrc_words(stats + j * 64, n > 0 ? n * 4 : 0), lane * 4, base + SM::STAGE + wave * 256);
+    }
+  };
+  op_t k[KE + KR], v[KE];
+  const int own = smem0 + wave * SM::WAVE;
+  fetch_rows<EC>(row_at<T>(a.k, a.sk, si, h, (int64_t)si.k_start + w0), (int)a.sk.s * 2, keys, lane, 0, a.e, own);
+  fetch_rows<EC>(row_at<T>(a.v, a.sv, si, h, (int64_t)si.k_start + w0), (int)a.sv.s * 2, keys, lane, 0, a.ev, own + SM::WAVE_V);
+  fetch_rows<kLatentShared>(row_at<T>(a.c, Strides3{a.c_z, 0, a.c_s}, si, 0, (int64_t)si.k_start + w0), (int)a.c_s * 2, keys, lane, 0, a.r, own + SM::WAVE_C);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  take_rows<T, EC>(k, lane, own);
+  take_rows<T, EC>(v, lane, own + SM::WAVE_V);
+  take_rows<T, kLatentShared>(k + KE, lane, own + SM::WAVE_C);
+  arrived(k);
+  arrived(v);
+  latent_meet();
+  if (j0 < j1) fetch(0, j0);
+  // (accumulators are written as asm, fa_wide.h, so that S and dP lie in vector registers, where the exponentials are)
+  f32x16 dk[DB + RB], dv[DB];
+#pragma unroll
+  for (int b = 0; b < DB + RB; ++b) acc_zero<T>(dk[b]);
+#pragma unroll
+  for (int b = 0; b < DB; ++b) acc_zero<T>(dv[b]);
+  const float qs = a.sm_scale * kLog2e, qs_or_1 = qs == 0.f ? 1.f : qs;
+  constexpr int kS = KE + KR, kA = kS + KE, kB = 2 * (2 * DB + RB), kRing = 6;      // MFMAs of S, of both; of the products with P and dS; operands on their way
+  // addresses of the operands in the stages of S and of the products (fa_latent_cache.h)
+  int at_e[8], at_r[KR], at_t[8], at_c[4], at_stats = smem0 + SM::STAGE + 16 * hi;
+  static_assert(KE <= 8 && DB <= 4, "a tile's row is one period of the swizzle");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    at_e[i] = smem0 + (Swz<EC>::row_base(lane) ^ (i % KE << 5));
+    at_t[i] = smem0 + (Swz<EC>::tr_base(lane, i >> 2) ^ ((i & 3) % DB << 6));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    at_r[i] = smem0 + SM::C_OFF + (Swz<kLatentShared>::row_base(lane) ^ (i << 5));
+    at_c[i] = smem0 + SM::C_OFF + (Swz<kLatentShared>::tr_base(lane, i >> 1) ^ ((i & 1) << 6));
+  }
+  auto onward = [&](auto& at, int by) __attribute__((always_inline)) {
+#pragma unroll
+    for (auto& x : at) x += by;
+    arrived(at);
+  };
+  op_t ring[kRing];
+  f32x16 s[2], dp[2];
+  // operand n of the products of S and dP of half b of a tile: Q, the shared part of Q, dO
+  auto read_a = [&](int b, int n) __attribute__((always_inline)) {
+    if (n < KE) return lds_read<op_t>(at_e[n] + b * 32 * Swz<EC>::ROWB);
+    if (n < kS) return lds_read<op_t>(at_r[n - KE] + b * 32 * Swz<kLatentShared>::ROWB);
+    return lds_read<op_t>(at_e[n - kS] + SM::V_OFF + b * 32 * Swz<EC>::ROWB);
+  };
+  // of dV, dK and dC, 16 queries after the other
+  auto read_b = [&](int b, int n) __attribute__((always_inline)) {
+    const int t = 2 * b + n / (kB / 2), x = n % (kB / 2);
+    int lo, hi2;
+    if (x < 2 * DB) {
+      const int off = t * 16 * Swz<EC>::ROWB + (x < DB ? SM::V_OFF : 0);
+      lo = at_t[x % DB] + off;
+      hi2 = at_t[4 + x % DB] + off;
+    } else {
+      lo = at_c[x - 2 * DB] + t * 16 * Swz<kLatentShared>::ROWB;
+      hi2 = at_c[2 + x - 2 * DB] + t * 16 * Swz<kLatentShared>::ROWB;
+    }
+    return __builtin_shufflevector(__builtin_bit_cast(typename Tr::q4_t, lds_read_tr_at(lo)), __builtin_bit_cast(typename Tr::q4_t, lds_read_tr_at(hi2)), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  op_t p_op[2], ds_op[2];
+  f32x4 st_lse, st_delta;
+  // P and dS of the 32 queries in s[b] and dp[b], element e of the lane's 16
+  auto element = [&](int b, int e) __attribute__((always_inline)) {
+    if (e % 4 == 0) {
+      const int st = at_stats + 128 * b + 32 * (e / 4);
+      st_lse = lds_read<f32x4>(st);
+      st_delta = lds_read<f32x4>(st + 256);
+    }
+    const float p = fast_exp2(__builtin_fmaf(s[b][e], qs_or_1, -st_lse[e % 4]));
+    s[b][e] = p;
+    dp[b][e] = p * (dp[b][e] - st_delta[e % 4]);
+    if (e % 8 == 7) {
+      p_op[e / 8] = pack8<T>(s[b], e / 8);
+      ds_op[e / 8] = pack8<T>(dp[b], e / 8);
+    }
+  };
+  // Half b of the queries from m0 on: of those that do not see the lane's key, S is what P of 0 comes from.
+  auto hide = [&](auto half, int m0) __attribute__((always_inline)) {
+    constexpr int b = decltype(half)::value;
+    if (!(a.causal && m0 < w0 + 31 - shift) && qs != 0.f) return;
+    const int from = a.causal ? key - shift - m0 - 4 * hi : 0;      // the lane's key is seen from this row of the half on
+    const float never = qs < 0.f ? __builtin_inff() : -__builtin_inff();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[b][e] = 8 * (e / 4) + e % 4 < from ? never : qs == 0.f ? 0.f : s[b][e];
+  };
+  // S and dP of half b of a tile, with P and dS of the half in front behind their MFMAs
+  auto front = [&](auto half, auto behind) __attribute__((always_inline)) {
+    constexpr int b = decltype(half)::value;
+#pragma unroll
+    for (int n = 0; n < kRing - 1; ++n) ring[n] = read_a(b, n);
+#pragma unroll
+    for (int n = 0; n < kA; ++n) {
+      if (n + kRing - 1 < kA) ring[(n + kRing - 1) % kRing] = read_a(b, n + kRing - 1);
+      const f32x16 none = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (n < kS) s[b] = Tr::mfma(ring[n % kRing], k[n], n == 0 ? none : s[b]);
+      else dp[b] = Tr::mfma(ring[n % kRing], v[n - kS], n == kS ? none : dp[b]);
+      if constexpr (decltype(behind)::value) {
+#pragma unroll
+        for (int e = first_of(n, 16, kA); e < first_of(n + 1, 16, kA); ++e) element(1 - b, e);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto back = [&](auto half) __attribute__((always_inline)) {
+    constexpr int b = decltype(half)::value;
+#pragma unroll
+    for (int n = 0; n < kRing - 1; ++n) ring[n] = read_b(b, n);
+#pragma unroll
+    for (int n = 0; n < kB; ++n) {
+      if (n + kRing - 1 < kB) ring[(n + kRing - 1) % kRing] = read_b(b, n + kRing - 1);
+      const int t = n / (kB / 2), x = n % (kB / 2);
+      if (x < DB) mfma_acc<T>(dv[x], ring[n % kRing], p_op[t]);
+      else mfma_acc<T>(dk[x - DB], ring[n % kRing], ds_op[t]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  using zero = std::integral_constant<int, 0>;
+  using one = std::integral_constant<int, 1>;
+  using yes = std::true_type;
+  using no = std::false_type;
+  // Tiles lie in three stages: the next one's S is formed while this one's products still read theirs.  (Behind the last half S of what a stage held
+  // is formed, for nothing, rather than a way around it taken, for which the accumulators would be moved.)
+  if (j0 < j1) {
+    latent_meet();
+    if (j0 + 1 < j1) fetch(1, j0 + 1);
+    front(zero{}, no{});
+  }
+  for (int j = j0, stage = 0; j < j1; ++j) {
+    hide(zero{}, 64 * j);
+    front(one{}, yes{});
+    back(zero{});
+    const int by = stage == 2 ? -2 * SM::BWD_STAGE : SM::BWD_STAGE;
+    onward(at_e, by);
+    onward(at_r, by);
+    if (j + 1 < j1) latent_meet();
+    if (j + 2 < j1) fetch(stage == 0 ? 2 : stage - 1, j + 2);
+    hide(one{}, 64 * j + 32);
+    front(zero{}, yes{});
+    back(one{});
+    onward(at_t, by);
+    onward(at_c, by);
+    at_stats += by;
+    stage = stage == 2 ? 0 : stage + 1;
+  }
+  latent_meet();
+  settle(dk);
+  settle(dv);
+  store_rows<T, DB>(dk, a.sm_scale, row_at<T>(a.dk, a.sdk, si, h, (int64_t)si.k_start + w0), a.sdk.s, keys, a.e, lane, own);
+  store_rows<T, DB>(dv, 1.0f, row_at<T>(a.dv, a.sdv, si, h, (int64_t)si.k_start + w0), a.sdv.s, keys, a.ev, lane, own + kRowsOut<T, DB>);
+  store_rows<float, RB>(dk + DB, 1.0f, a.part_c + (((int64_t)si.batch_index * a.heads + h) * a.part_rows + si.k_start + w0) * kLatentShared, kLatentShared, keys,
+                        kLatentShared, lane, own);
+}
+
+// dC: the heads' parts added in their order, four columns a lane
+template <typename T>
+__global__ __launch_bounds__(256) void latent_dc_kernel(const LatentBwdArgs a, int64_t keys, const int32_t* end) {
+  const int64_t at = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+  const int64_t b = at / keys, n = at % keys;
+  const int col = threadIdx.x % 16 * 4;
+  if (b >= a.batch || (end != nullptr && n >= *end) || col >= a.r) return;
+  const float* from = a.part_c + (b * a.heads * a.part_rows + n) * kLatentShared + col;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int h = 0; h < a.heads; ++h) sum += *reinterpret_cast<const f32x4*>(from + (int64_t)h * a.part_rows * kLatentShared);
+  typename Traits<T>::q4_t y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = Traits<T>::cvt(sum[r] * a.sm_scale);
+  *reinterpret_cast<typename Traits<T>::q4_t*>(reinterpret_cast<T*>(a.dc) + b * a.dc_z + n * a.dc_s + col) = y;
+}
+
+template <typename T, int EC> hipError_t launch_latent_keys(const LatentBwdArgs& a, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  const int nseq = nseq_of(a.seq, a.batch), tiles = (a.seq.max_seqlen_k + 127) / 128;
+  if (nseq == 0 || tiles == 0) return hipSuccess;
+  hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_dkdv_kernel<T, EC>), LatentSmem<EC>::BWD_BYTES, done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((latent_dkdv_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles)), dim3(256), LatentSmem<EC>::BWD_BYTES, s, a, nseq, tiles);
+  const int32_t* end = a.seq.num_seqlens != 0 ? a.seq.cu_k + nseq : nullptr;
+  hipLaunchKernelGGL((latent_dc_kernel<T>), dim3((unsigned)((a.batch * a.part_rows + 15) / 16)), dim3(256), 0, s, a, a.part_rows, end);
+  return hipGetLastError();
+}
+
+}  // namespace fa

@@ -16,6 +16,15 @@ template <typename V, int N> __device__ __forceinline__ void arrived(V (&x)[N]) 
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 
+// Behind the last MFMA onto the accumulators, which the compiler does not see (fa_wide.h): 16 passes and what the register file takes.
+template <int DB> __device__ __forceinline__ void settle(f32x16 (&o)[DB]) {
+#pragma unroll
+  for (int b = 0; b < DB; ++b) asm volatile("" : "+a"(o[b]));
+  asm volatile("s_nop 15\n\ts_nop 15");
+#pragma unroll
+  for (int b = 0; b < DB; ++b) asm volatile("" : "+a"(o[b]));
+}
+
 // Maximum and sum of a lane's row; the sum is over the lane's half of the keys until cross_sum.
 // The maximum is a reference: it moves, and O with it, only where a score passes it by more than 2^kSlack (P is then up to 2^kSlack, which
 // both types hold without losing a bit; sums are fp32).  O lies in accumulation registers, where a product costs three
