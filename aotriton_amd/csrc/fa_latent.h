@@ -9,6 +9,7 @@
 // Layouts and products as in fa_fwd_impl.h: a wave owns 32 rows (dK/dV: keys), a lane one of them; tiles come straight into swizzled LDS
 // (fa_device.h: Swz), the next one while this one is worked on, and serve row reads and transposing reads alike.
 #pragma once
+#include <algorithm>
 #include "fa_device.h"
 #include "fa_latent_args.h"
 #include "fa_latent_parts.h"
@@ -109,11 +110,12 @@ __device__ __forceinline__ SeqInfo latent_seq(const LatentArgs& a, int z) {
   return uniform(r);
 }
 
-// (sequence, head, tile) of a workgroup: the tiles of a kind one behind the other, the heads of all sequences side by side, so that an
-// XCD keeps its heads where their number is a multiple of 8.  Causal tiles have the more keys the later they stand: those first.
+// (sequence, head, tile) of a workgroup.  LatentArgs::group heads (of all sequences side by side, the last ones the rest) stand side by side, their
+// tiles of a kind one behind the other.  Causal tiles have the more keys the later they stand: those first.
 __device__ __forceinline__ void latent_item(const LatentArgs& a, int id, int nseq, int tiles, bool backwards, int& z, int& h, int& t) {
-  const int pairs = nseq * a.heads, zh = id % pairs;
-  t = id / pairs;
+  const int pairs = nseq * a.heads, front = id / (a.group * tiles) * a.group, have = pairs - front < a.group ? pairs - front : a.group;
+  const int rest = id - front * tiles, zh = front + rest % have;
+  t = rest / have;
   if (backwards) t = tiles - 1 - t;
   h = zh % a.heads;
   z = zh / a.heads;
@@ -322,7 +324,7 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta += (float)out[k][i] * (float)dout[k][i];
   }
-  const float qs = a.sm_scale * kLog2e;
+  const float qs = a.sm_scale * kLog2e, qs_or_1 = qs == 0.f ? 1.f : qs;
   // P and dP of 32 keys of tile j
   auto products = [&](const char* K, int j, int b, f32x16& p, f32x16& dp) __attribute__((always_inline)) {
     const int l = own_lane(), n0 = j * 64;
@@ -336,12 +338,14 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
     for (int k = 0; k < KR; ++k) p = Tr::mfma(swz_read_row<T, kLatentShared>(K + SM::C_OFF, row_r, k, b), q[KE + k], p);
 #pragma unroll
     for (int k = 0; k < KE; ++k) dp = Tr::mfma(swz_read_row<T, EC>(K + SM::V_OFF, row_e, k, b), dout[k], dp);
-    const int limit = see - n0 - 32 * b - 4 * hi;
+    if (masked || qs == 0.f) {      // (of what a row does not see S is what P of 0 comes from)
+      const int limit = see - n0 - 32 * b - 4 * hi;
+      const float never = qs < 0.f ? __builtin_inff() : -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      p[i] = fast_exp2(__builtin_fmaf(p[i], qs, -lse));
-      if (masked && 8 * (i / 4) + i % 4 > limit) p[i] = 0.f;
+      for (int i = 0; i < 16; ++i) p[i] = 8 * (i / 4) + i % 4 > limit ? never : qs == 0.f ? 0.f : p[i];
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = fast_exp2(__builtin_fmaf(p[i], qs_or_1, -lse));
   };
   int stage = 0;      // of the tile that comes next
   if (few) {
@@ -399,11 +403,21 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
   store_rows<T, RB>(dq + DB, a.sm_scale, to + a.e, a.sdq.s, rows, a.r, out_lane, own + kRowsOut<T, DB>);
 }
 
+// Heads whose tiles are worked on side by side: as many as have two workgroups for a CU, a multiple of 8 (an XCD keeps its heads).  Those that run at a
+// time then share what passes by in L2: the step of 12 packed sequences of 200 to 4000 tokens with 16 heads takes 1830 us, with all heads side by
+// side 2010, with one an XCD 1900; three long sequences, the last of which ends by itself, 1490 for 1410; equal lengths the same.
+inline int latent_group(int pairs, int tiles) {
+  const int n = (512 / std::max(tiles, 1) + 7) / 8 * 8;
+  return std::min(std::max(n, 8), pairs);
+}
+
 // ---- launches ------------------------------------------------------------------------------------------------------
-template <typename T, int EC> hipError_t launch_latent_fwd(const LatentArgs& a, hipStream_t s) {
+template <typename T, int EC> hipError_t launch_latent_fwd(const LatentArgs& args, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
-  const int nseq = nseq_of(a.seq, a.batch), tiles = (a.seq.max_seqlen_q + 127) / 128;
+  const int nseq = nseq_of(args.seq, args.batch), tiles = (args.seq.max_seqlen_q + 127) / 128;
   if (nseq == 0 || tiles == 0) return hipSuccess;
+  LatentArgs a = args;
+  a.group = a.parts > 1 ? nseq * a.heads : latent_group(nseq * a.heads, tiles);
   hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_fwd_kernel<T, EC>), LatentSmem<EC>::BYTES, done);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((latent_fwd_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles * a.parts)), dim3(256), LatentSmem<EC>::BYTES, s, a, nseq, tiles);
@@ -412,10 +426,12 @@ template <typename T, int EC> hipError_t launch_latent_fwd(const LatentArgs& a, 
   return hipGetLastError();
 }
 
-template <typename T, int EC> hipError_t launch_latent_dq(const LatentBwdArgs& a, hipStream_t s) {
+template <typename T, int EC> hipError_t launch_latent_dq(const LatentBwdArgs& args, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
-  const int nseq = nseq_of(a.seq, a.batch), tiles = (a.seq.max_seqlen_q + 127) / 128;
+  const int nseq = nseq_of(args.seq, args.batch), tiles = (args.seq.max_seqlen_q + 127) / 128;
   if (nseq == 0 || tiles == 0) return hipSuccess;
+  LatentBwdArgs a = args;
+  a.group = latent_group(nseq * a.heads, tiles);
   hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_dq_kernel<T, EC>), LatentSmem<EC>::BYTES, done);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((latent_dq_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles)), dim3(256), LatentSmem<EC>::BYTES, s, a, nseq, tiles);

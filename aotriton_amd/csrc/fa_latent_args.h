@@ -19,6 +19,7 @@ struct LatentArgs {
   int32_t causal;                // query i sees keys up to i + Sk - Sq
   SeqArgs seq;
   int32_t rows_q, rows_k;        // of the tensors: packed offsets are held inside them
+  int32_t group;                 // fa_latent.h: latent_item
   // The keys of a tile cut into `parts` (> 1), for calls with few queries: the parts' sums, laid out as latent_part says.
   int32_t parts;
   float* part_o; float* part_ml;

@@ -217,10 +217,12 @@ __global__ __launch_bounds__(256) void latent_dc_kernel(const LatentBwdArgs a, i
   *reinterpret_cast<typename Traits<T>::q4_t*>(reinterpret_cast<T*>(a.dc) + b * a.dc_z + n * a.dc_s + col) = y;
 }
 
-template <typename T, int EC> hipError_t launch_latent_keys(const LatentBwdArgs& a, hipStream_t s) {
+template <typename T, int EC> hipError_t launch_latent_keys(const LatentBwdArgs& args, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
-  const int nseq = nseq_of(a.seq, a.batch), tiles = (a.seq.max_seqlen_k + 127) / 128;
+  const int nseq = nseq_of(args.seq, args.batch), tiles = (args.seq.max_seqlen_k + 127) / 128;
   if (nseq == 0 || tiles == 0) return hipSuccess;
+  LatentBwdArgs a = args;
+  a.group = latent_group(nseq * a.heads, tiles);
   hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_dkdv_kernel<T, EC>), LatentSmem<EC>::BWD_BYTES, done);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((latent_dkdv_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles)), dim3(256), LatentSmem<EC>::BWD_BYTES, s, a, nseq, tiles);
