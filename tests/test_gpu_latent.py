@@ -145,6 +145,16 @@ def test_packed_sequences(E, R, Ev, causal, dtype):
     assert all((g[:, :, tk:] == 0).all() for g in grads[1:3]) and (grads[3][:, tk:] == 0).all()
 
 
+def test_more_heads_than_stand_side_by_side():
+    """a greatest length beyond every sequence leaves all tiles but the first ones empty and the heads in several groups: the same results"""
+    lens, H = [70, 300, 129], 5
+    q, k, v, c, do = _inputs(1, H, sum(lens), sum(lens), 128, 64, 128, HF, seed=6)
+    cu = torch.tensor([0, 70, 370, 499], dtype=torch.int32, device=DEV)
+    want, grads = _step(q, k, v, c, do, cu_seqlens_q=cu, cu_seqlens_k=cu, max_seqlen_q=300, max_seqlen_k=300)
+    out, more = _step(q, k, v, c, do, cu_seqlens_q=cu, cu_seqlens_k=cu, max_seqlen_q=8192, max_seqlen_k=8192)
+    assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(more, grads))
+
+
 def test_offsets_outside_the_tensors():
     """what they name past the rows is not there, and neither are rows past the greatest length"""
     q, k, v, c, do = _inputs(1, 2, 200, 200, 64, 32, 64, BF, seed=4)

@@ -103,6 +103,21 @@ def test_many_sequences(Hq, most):
     _check(q, cache, table, n, starts, 128, 0.1, out, lse)
 
 
+@pytest.mark.parametrize('Hq', [1, 3, 20, 32, 128])
+@pytest.mark.parametrize('seed', [0, 1, 2])
+def test_cuts_of_prompts_and_decoding(Hq, seed):
+    """the list of work is cut anywhere: blocks of a prompt's rows that see one tile more from group to group, single tokens, sequences of a tile and
+    less, one that takes most of the list; more rows of a block than a sequence has"""
+    rng = random.Random(100 * seed + Hq)
+    most = max(2, 1200 // Hq)
+    lens = [rng.choice([0, rng.randint(1, 70), rng.randint(100, 900)]) for _ in range(6)] + [2500]
+    counts = [rng.choice([1, 1, rng.randint(2, most), most]) for _ in range(6)] + [rng.choice([1, 40])]
+    cache, table, n, starts = _pool(lens, counts, 576, rng.choice([16, 64]), HF, seed=seed)
+    q = torch.randn(sum(counts), Hq, 576, generator=torch.Generator().manual_seed(seed)).half()
+    out, lse = _run(q, cache, table, n, starts, 512, 0.05)
+    _check(q, cache, table, n, starts, 512, 0.05, out, lse)
+
+
 def test_rows_of_no_sequence():
     cache, table, n, starts = _pool([40, 70], [3, 2], 136, 16, HF, seed=4)
     q = torch.randn(11, 6, 136, generator=torch.Generator().manual_seed(5)).half()
