@@ -234,6 +234,8 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
       ++block;
       continue;
     }
+    auto slot_of = [&](int entry) { const int n = (j0 + entry / 2) * 32 + entry % 2 * 16; return entry < 2 * n_tiles && n < s.end ? n : -1; };
+    PageRun<decltype(slot_of)> pages(ca, z, lane, slot_of);
     const int rows = s.tokens * a.hq, w0 = block * a.block_rows + rw * 32, w_last = w0 + 31 < rows ? w0 + 31 : rows - 1;
     const bool row_ok = w0 + c < rows;
     const int row = row_ok ? w0 + c : rows - 1, token = row / a.hq, head = row - token * a.hq;
@@ -244,8 +246,6 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     const int see_most = __builtin_amdgcn_readfirstlane(sees(w_last / a.hq));
     const int j1 = j0 + n_tiles, wave_end = w0 < rows ? see_most / 32 + 1 : 0;
 
-    auto slot_of = [&](int entry) { const int n = (j0 + entry / 2) * 32 + entry % 2 * 16; return entry < 2 * n_tiles && n < s.end ? n : -1; };
-    PageRun<decltype(slot_of)> pages(ca, z, lane, slot_of);
     const char* xbase = reinterpret_cast<const char*>(ca.k);
     auto stage_of = [&](int j) { return smem0 + ((j - j0) & (SM::STAGES - 1)) * SM::STAGE; };
     constexpr int kLoads = 8 / RPL + 1, kPieces = 4 / RPL + 1;      // of a tile, and the pairs they come in
@@ -300,39 +300,35 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     // Q passes through LDS as tiles of 32 rows, as the latent rows do: whole rows of memory, each once (as a lane's row in pieces straight into
     // registers it took 11 us for 128 rows).  It lies behind the first kFirst stages, whose tiles are on their way with it; where it does not fit
     // there, it comes in two halves of its columns.
+    // (lane l has the place of row l % 8 of the wave's eight of the l / 8-th 32)
+    const int r0 = block * a.block_rows, tb = r0 / a.hq, r_lane = r0 + lane / 8 * 32 + wave * 8 + lane % 8, t_lane = r_lane / a.hq;
+    const int q_off = r_lane < rows && lane < 8 * RW ? (t_lane - tb) * ((int)a.q_row * 2) + (r_lane - t_lane * a.hq) * ((int)a.q_head * 2) : -1;
+    const int t_end = (r0 + a.block_rows - 1 < rows ? r0 + a.block_rows - 1 : rows - 1) / a.hq;
+    const u32x4_t q_rs = wave_rsrc_words(reinterpret_cast<const T*>(a.q) + (int64_t)(s.start + tb) * a.q_row,
+                                         (int)(((t_end - tb) * a.q_row + (a.hq - 1) * a.q_head + e) * 2));
     auto fetch_q = [&](auto half) __attribute__((always_inline)) {
       constexpr int H = decltype(half)::value, at_col = H * SM::template Q<RW>::COLUMNS, QC = SM::template Q<RW>::COLUMNS, QL = QC / 8, QR = 64 / QL;
       constexpr bool ends = H == SM::template Q<RW>::HALVES - 1;
-      const int r0 = block * a.block_rows, tb = r0 / a.hq, t_end = (r0 + a.block_rows - 1 < rows ? r0 + a.block_rows - 1 : rows - 1) / a.hq;
-      const u32x4_t rs = wave_rsrc_words(reinterpret_cast<const T*>(a.q) + (int64_t)(s.start + tb) * a.q_row,
-                                         (int)(((t_end - tb) * a.q_row + (a.hq - 1) * a.q_head + e) * 2));
-      const int q_row = (int)a.q_row * 2, q_head = (int)a.q_head * 2;
+      static_assert(QR == 1 || QR == 2, "f of a row is that of its access and that of its place in it");
+      const int l = own_lane(), lrow = l / QL, base = (l % QL) ^ Swz<QC>::f(lrow + 8 * (wave & 1)), tail_ch = (l % 8) ^ Swz<kLatentTail>::f(8 * (wave & 1) + l / 8);
 #pragma unroll
       for (int g = 0; g < RW; ++g) {
-        const int R = r0 + g * 32 + wave * 8, lds = smem0 + SM::template Q<RW>::at(H, g), lds_a = lds + wave * 8 * QC * 2;
-        const int l = own_lane(), lrow = l / QL, base = (l % QL) ^ Swz<QC>::f(lrow + 8 * (wave & 1)), tail_ch = (l % 8) ^ Swz<kLatentTail>::f(8 * (wave & 1) + l / 8);
-        int t = __builtin_amdgcn_readfirstlane(R / a.hq), h = R - t * a.hq, off[8], tail = kVoffOutOfRange;
-        t -= tb;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          off[i] = R + i < rows ? t * q_row + h * q_head : -1;
-          if (l / 8 == i && off[i] >= 0 && EA + tail_ch * 8 < e) tail = off[i] + (EA + tail_ch * 8) * 2;
-          const bool wraps = h + 1 == a.hq;
-          h = wraps ? 0 : h + 1;
-          t += wraps ? 1 : 0;
-        }
-        static_assert(QR == 1 || QR == 2, "f of a row is that of its access and that of its place in it");
+        const int lds = smem0 + SM::template Q<RW>::at(H, g), lds_a = lds + wave * 8 * QC * 2;
+        auto off = [&](int i) { return __builtin_amdgcn_readlane(q_off, 8 * g + i); };
 #pragma unroll
         for (int i = 0; i < 8 / QR; i += 2) {
           int voff[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const int at = QR == 1 ? off[i + k] : lrow ? off[(i + k) * QR + QR - 1] : off[(i + k) * QR], ch = base ^ Swz<QC>::f((i + k) * QR);
+            const int at = QR == 1 ? off(i + k) : lrow ? off((i + k) * QR + QR - 1) : off((i + k) * QR), ch = base ^ Swz<QC>::f((i + k) * QR);
             voff[k] = at >= 0 && (!kCut || at_col + ch * 8 < e) ? at + at_col * 2 + (ch << 4) : kVoffOutOfRange;
           }
-          load_to_lds(rs, voff[0], 0, lds_a + i * 1024, voff[1], 0, lds_a + (i + 1) * 1024);
+          load_to_lds(q_rs, voff[0], 0, lds_a + i * 1024, voff[1], 0, lds_a + (i + 1) * 1024);
         }
-        if (ends) load_to_lds1(rs, tail, lds + 32 * QC * 2 + wave * 1024);
+        if (ends) {
+          const int at = __shfl(q_off, 8 * g + l / 8);
+          load_to_lds1(q_rs, at >= 0 && EA + tail_ch * 8 < e ? at + (EA + tail_ch * 8) * 2 : kVoffOutOfRange, lds + 32 * QC * 2 + wave * 1024);
+        }
       }
     };
     op_t q[KE + KR];
