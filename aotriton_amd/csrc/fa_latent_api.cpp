@@ -205,8 +205,10 @@ int fa_latent_cache_attn(const fa_latent_cache_params* p, void* hip_stream, fa_a
   a.blocks = (int32_t)blocks;
   a.least = 4;
   a.margin = 4;
-  a.group = std::max<int32_t>(1, (int32_t)(32 * (int64_t)a.hq / a.block_rows));
-  a.step = a.group > 1 ? 1 : (a.block_rows + 32 * a.hq - 1) / (32 * a.hq);
+  a.block_shift = a.block_rows == 32 ? 5 : a.block_rows == 64 ? 6 : 7;
+  a.group_shift = a.step_shift = 0;
+  while ((2ull << a.group_shift) * a.block_rows <= 32 * hq) ++a.group_shift;
+  while ((32ull * hq << a.step_shift) < (uint64_t)a.block_rows) ++a.step_shift;
   a.workers = (int32_t)std::max<int64_t>(1, std::min<int64_t>(num_cu, blocks * ((tiles + a.least - 1) / a.least)));
   const int64_t places = 2 * (int64_t)a.workers * (a.block_rows / 32), o_bytes = places * 32 * d * 4;
   void* scratch = alloc != nullptr && a.workers > 1 ? alloc->alloc(alloc, (uint64_t)(o_bytes + places * 64 * 4 + blocks * (int64_t)sizeof(fa::LatentHead))) : nullptr;

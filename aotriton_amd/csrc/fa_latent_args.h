@@ -54,7 +54,8 @@ struct LatentCacheArgs {
   // part_o, two places for every worker.
   int32_t block_rows, workers, least;
   int32_t margin;                // fa_latent_cache.h: LatentSeq::units
-  int32_t group, step;           // blocks that 32 tokens make (one at least), tiles that a group's tokens make
+  int32_t block_shift;           // block_rows as a power of two; so, rounded, blocks that 32 tokens make (one at least), and tiles that a group's tokens make
+  int32_t group_shift, step_shift;
   float* part_o; float* part_ml;
   LatentHead* heads;             // of the blocks, `blocks` of them (fa_latent_cache.h: latent_block)
   int32_t blocks;

@@ -37,42 +37,42 @@ template <int EA> struct LatentCacheSmem {
 __device__ __forceinline__ int64_t latent_div(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b; }
 
 // A sequence as the list of work has it: `blocks` blocks of rows, of tiles as many as their last row sees, or some more: the blocks of a group
-// (LatentCacheArgs::group) have the same number, `step` more than the group in front, up to all `tiles`.
+// (LatentCacheArgs::group_shift) have the same number, a step more than the group in front, up to all `tiles`.
 struct LatentSeq {
   int32_t start, tokens, length, end;      // first row of Q, tokens, filled slots, slots with the new ones as far as the table goes
   int32_t blocks, tiles, filled;           // (filled: tiles in front of the first new slot)
   __device__ __forceinline__ int tiles_of_group(const LatentCacheArgs& a, int g) const {
-    const int64_t n = filled + (int64_t)a.step * (g + 1);
+    const int64_t n = filled + ((int64_t)(g + 1) << a.step_shift);
     return n < tiles ? (int)n : tiles;
   }
-  __device__ __forceinline__ int tiles_of(const LatentCacheArgs& a, int block) const { return tiles_of_group(a, block / a.group); }
+  __device__ __forceinline__ int tiles_of(const LatentCacheArgs& a, int block) const { return tiles_of_group(a, block >> a.group_shift); }
   // groups that have not all tiles, as far as there are blocks
   __device__ __forceinline__ int short_groups(const LatentCacheArgs& a) const {
-    const int n = tiles > filled ? (tiles - filled - 1) / a.step : 0, all = (blocks + a.group - 1) / a.group;
+    const int n = tiles > filled ? (tiles - filled - 1) >> a.step_shift : 0, all = (blocks + (1 << a.group_shift) - 1) >> a.group_shift;
     return n < all ? n : all;
   }
   // The list counts a block's tiles and LatentCacheArgs::margin on either side of them, for what beginning and ending it takes.
   __device__ __forceinline__ int64_t units(const LatentCacheArgs& a) const {
-    const int64_t n = short_groups(a), over = n * a.group - blocks;      // (the last group may be short of blocks)
-    const int64_t u = a.group * (n * filled + a.step * (n * (n + 1) / 2)), last = over > 0 ? filled + a.step * n : tiles;
+    const int64_t n = short_groups(a), over = (n << a.group_shift) - blocks;      // (the last group may be short of blocks)
+    const int64_t u = (n * filled + ((n * (n + 1) / 2) << a.step_shift)) << a.group_shift, last = over > 0 ? filled + (n << a.step_shift) : tiles;
     return u - over * last + (int64_t)blocks * (2 * a.margin);
   }
   // the block with unit `rel` of the sequence, and the unit's number in it
   __device__ __forceinline__ int block_of(const LatentCacheArgs& a, int64_t rel, int& unit) const {
     const int n = short_groups(a);
     for (int g = 0; g < n; ++g) {
-      const int t = filled + a.step * (g + 1) + 2 * a.margin, have = blocks - g * a.group < a.group ? blocks - g * a.group : a.group;
+      const int group = 1 << a.group_shift, t = filled + ((g + 1) << a.step_shift) + 2 * a.margin, have = blocks - g * group < group ? blocks - g * group : group;
       if (rel < (int64_t)have * t) {
         const int b = (int)((uint32_t)rel / (uint32_t)t);
         unit = (int)rel - b * t;
-        return g * a.group + b;
+        return g * group + b;
       }
       rel -= (int64_t)have * t;
     }
     const int t = tiles + 2 * a.margin;
     const int64_t b = latent_div(rel, t);
     unit = (int)(rel - b * t);
-    return n * a.group + (int)b;
+    return (n << a.group_shift) + (int)b;
   }
 };
 __device__ __forceinline__ LatentSeq latent_cache_seq(const LatentCacheArgs& a, int z) {
@@ -83,7 +83,7 @@ __device__ __forceinline__ LatentSeq latent_cache_seq(const LatentCacheArgs& a, 
   s.length = a.cache.lengths[z];
   const int64_t room = (int64_t)a.cache.columns << a.cache.page_shift, end = (int64_t)s.length + s.tokens;
   s.end = s.length < 0 ? 0 : (int)(end < room ? end : room);
-  s.blocks = (int)latent_div((int64_t)s.tokens * a.hq + a.block_rows - 1, a.block_rows);
+  s.blocks = (s.tokens * a.hq + a.block_rows - 1) >> a.block_shift;
   s.tiles = s.end > 32 ? (s.end + 31) / 32 : 1;
   s.filled = s.length <= 0 ? 0 : s.length < s.end ? (s.length + 31) / 32 : s.tiles;
   return s;
@@ -91,7 +91,7 @@ __device__ __forceinline__ LatentSeq latent_cache_seq(const LatentCacheArgs& a, 
 
 // Number of a sequence's first block, with a gap or two: that of its first row, divided by the rows of a block, and one more for every sequence in
 // front.  LatentCacheArgs::blocks bounds them.
-__device__ __forceinline__ int latent_block(const LatentCacheArgs& a, int z, int start) { return (int)latent_div((int64_t)start * a.hq, a.block_rows) + z; }
+__device__ __forceinline__ int latent_block(const LatentCacheArgs& a, int z, int start) { return (start * a.hq >> a.block_shift) + z; }
 
 // The cut of the list: its length, that of a piece, and of the sequence looked for its number and where it starts in the list.  `mine(z, first
 // unit, sequence)` says which one that is.  All 256 threads call this.
