@@ -194,17 +194,21 @@ int fa_latent_cache_attn(const fa_latent_cache_params* p, void* hip_stream, fa_a
   if (rows == 0) return FA_SUCCESS;
 
   const int num_cu = fa_get_multiprocessor_count(hip_stream), d = c.head_dim <= 320 && c.head_dim_v <= 256 ? 256 : 512;
-  // Rows of a workgroup by those that a sequence has on average.
+  // Rows of a workgroup.  32 where a sequence has no more on average, or where blocks of 128, which take longer to begin and to end, would leave a CU
+  // a few tiles of 32 slots.  64 sequences of 4096 slots, 576 columns: 32 heads 90 us with blocks of 32 and of 128, 40 heads 124 and 94, 128 heads 211
+  // and 114; 16 sequences (8 tiles a CU) with 64 heads 45 and 43; 8 sequences (4 tiles) 32 and 35, with 128 heads 44 and 46; 2 sequences 25 and 29.
+  // 64 rows only up to 256 columns of values (64 sequences, 64 heads, 320 columns: 75, 58, 59 us for 32, 64, 128 rows); above they took 111.
   const int64_t mean = n > 0 ? (int64_t)(rows * hq / n) : 0;
-  a.block_rows = mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
+  const int64_t room = (int64_t)c.columns << c.page_shift;
+  const int64_t tiles = (std::min<int64_t>(p->max_length, room) + (int64_t)rows + 31) / 32 + 1;
+  const bool much = (int64_t)n * ((mean + 127) / 128) * tiles >= 6 * (int64_t)num_cu;
+  a.block_rows = mean <= 32 || !much ? 32 : mean <= 64 && d == 256 ? 64 : 128;
   // One workgroup on a CU, one round of them.
   const int64_t blocks = (int64_t)rows * (int64_t)hq / a.block_rows + (int64_t)n;
   if (!fits((double)blocks * 4 * 16)) return FA_ERROR_NOT_SUPPORTED;
-  const int64_t room = (int64_t)c.columns << c.page_shift;
-  const int64_t tiles = (std::min<int64_t>(p->max_length, room) + (int64_t)rows + 31) / 32 + 1;
   a.blocks = (int32_t)blocks;
   a.least = 4;
-  a.margin = 4;
+  a.margin = 5;
   a.block_shift = a.block_rows == 32 ? 5 : a.block_rows == 64 ? 6 : 7;
   a.group_shift = a.step_shift = 0;
   while ((2ull << a.group_shift) * a.block_rows <= 32 * hq) ++a.group_shift;
