@@ -12,7 +12,7 @@
 // Bound by the matrix pipe, and by what the card's power leaves of its rate: two waves on a SIMD keep it busy 60 % of the time.  16 heads of 8192
 // causal tokens, E = Ev = 128, R = 64, bf16: forward 346-360 us (970 TFLOP/s; a product of 8192^3 reaches 1160-1190), dQ 570-580 (950), dK, dV and dC
 // 690.  dQ and dK/dV each form S and dP, 25 % of the backward's products, rather than dQ in pieces from the other's blocks: no atomics, results that
-// do not change.  (dQ with 64 rows of Q, C and dO as operands has no register left over; with one more held value it spills.)
+// do not change.
 #pragma once
 #include <algorithm>
 #include "fa_device.h"
