@@ -391,13 +391,25 @@ __global__ __launch_bounds__(256, 2) void latent_dq_kernel(const LatentBwdArgs a
       for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
       const int m = own_lane();
       const int tr0 = Swz<EC>::tr_base(m, 0), tr1 = Swz<EC>::tr_base(m, 1), rr0 = Swz<kLatentShared>::tr_base(m, 0), rr1 = Swz<kLatentShared>::tr_base(m, 1);
+      op_t ds[2];
+      auto add = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const op_t ds = pack8<T>(s, t);
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int x = 0; x < DB; ++x) dq[x] = Tr::mfma(swz_read_tr<T, EC>(K, tr0, tr1, 2 * b + t, x), ds, dq[x]);
+          for (int x = 0; x < DB; ++x) dq[x] = Tr::mfma(swz_read_tr<T, EC>(K, tr0, tr1, 2 * b + t, x), ds[t], dq[x]);
 #pragma unroll
-        for (int x = 0; x < RB; ++x) dq[DB + x] = Tr::mfma(swz_read_tr<T, kLatentShared>(K + SM::C_OFF, rr0, rr1, 2 * b + t, x), ds, dq[DB + x]);
+          for (int x = 0; x < RB; ++x) dq[DB + x] = Tr::mfma(swz_read_tr<T, kLatentShared>(K + SM::C_OFF, rr0, rr1, 2 * b + t, x), ds[t], dq[DB + x]);
+        }
+      };
+#pragma unroll
+      for (int t = 0; t < 2; ++t) ds[t] = pack8<T>(s, t);
+      add();
+      if (j1 == 1) {      // (what dS lost in 16 bits, where few keys do not average it out: fa_latent_keys.h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] -= (float)ds[i / 8][i % 8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) ds[t] = pack8<T>(s, t);
+        add();
       }
     }
   }
