@@ -109,6 +109,33 @@ def test_gradients_of_a_single_key(dtype):
     assert (dc.double().abs() <= (bound * q[..., E:].double().abs()).sum(1) + least).all()
 
 
+@pytest.mark.parametrize('dtype', [HF, BF])
+@pytest.mark.parametrize('n', [2, 4, 21, 64])
+def test_gradients_of_one_tile(n, dtype):
+    """P and dS go through the products as two numbers of 16 bits each, off by u^2, and delta is the sum of P dP: what the gradients are off by is their
+    own rounding, u, and what fp32 sums (fdot) and scores (e) leave."""
+    B, H, E, R, Ev, scale = 2, 3, 128, 64, 128, 0.02
+    q, k, v, c, do = _inputs(B, H, n, n, E, R, Ev, dtype, seed=n)
+    _, grads = _step(q, k, v, c, do, scale=scale)
+    for b in range(B):
+        Q, K, V, C, DO = (t[b].cpu() for t in (q, k, v, c, do))
+        kk = latent.keys(K, C)
+        _, _, p = latent.attention(Q, K, V, C, True, scale)
+        want = latent.attention_grads(Q, K, V, C, DO, True, scale)
+        e, u, fdot = score_error(Q, kk, scale), torch.finfo(dtype).eps / 2, (E + R + 8) * 2.0 ** -24
+        dp, dp_off = torch.matmul(DO.double(), V.double().transpose(1, 2)), fdot * torch.matmul(DO.double().abs(), V.double().abs().transpose(1, 2))
+        share = 1.1 * u * u + 2 * e + (2 * n + 8) * 2.0 ** -24
+        delta = (p * dp).sum(-1, keepdim=True)
+        delta_off = (p * (share * dp.abs() + dp_off)).sum(-1, keepdim=True)
+        off = share * (p * (dp - delta)).abs() + 1.01 * p * (dp_off + delta_off)
+        least = 2.0 ** -24 if dtype == HF else 0.0      # (fp16's least number, for what is left of dS and P, and for the results)
+        off, p_off = off + least, share * p + least
+        bk = scale * torch.matmul(off.transpose(1, 2), Q.double().abs())
+        for name, got, w, bound in (('dq', grads[0][b], want[0], scale * torch.matmul(off, kk.double().abs())), ('dk', grads[1][b], want[1], bk[..., :E]),
+                                    ('dv', grads[2][b], want[2], torch.matmul(p_off.transpose(1, 2), DO.double().abs())), ('dshared', grads[3][b], want[3], bk[..., E:].sum(0))):
+            assert_within(name, got, w, bound + u * w.abs() + least)
+
+
 @pytest.mark.parametrize('B,H,Sq,Sk,E,R,Ev,causal,dtype', [
     (1, 1, 1, 4000, 128, 64, 128, True, BF), (1, 2, 130, 3000, 128, 64, 128, True, HF), (2, 1, 5, 2049, 64, 32, 64, False, HF),
     (1, 3, 17, 1100, 40, 8, 24, True, BF), (1, 1, 2000, 1900, 64, 64, 64, True, BF)])
