@@ -432,7 +432,7 @@ inline int latent_group(int pairs, int tiles) {
 template <typename T, int EC> hipError_t launch_latent_fwd(const LatentArgs& args, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   const int nseq = nseq_of(args.seq, args.batch), tiles = (args.seq.max_seqlen_q + 127) / 128;
-  if (nseq == 0 || tiles == 0) return hipSuccess;
+  if (nseq * args.heads == 0 || tiles == 0) return hipSuccess;
   LatentArgs a = args;
   a.group = a.parts > 1 ? nseq * a.heads : latent_group(nseq * a.heads, tiles);
   hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_fwd_kernel<T, EC>), LatentSmem<EC>::BYTES, done);
@@ -446,7 +446,7 @@ template <typename T, int EC> hipError_t launch_latent_fwd(const LatentArgs& arg
 template <typename T, int EC> hipError_t launch_latent_dq(const LatentBwdArgs& args, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   const int nseq = nseq_of(args.seq, args.batch), tiles = (args.seq.max_seqlen_q + 127) / 128;
-  if (nseq == 0 || tiles == 0) return hipSuccess;
+  if (nseq * args.heads == 0 || tiles == 0) return hipSuccess;
   LatentBwdArgs a = args;
   a.group = latent_group(nseq * a.heads, tiles);
   hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_dq_kernel<T, EC>), LatentSmem<EC>::BYTES, done);

@@ -137,10 +137,13 @@ int fa_latent_bwd(const fa_latent_bwd_params* p, void* hip_stream, fa_allocator*
   if (!fits((double)a.batch * a.rows_k / 16 + 1)) return FA_ERROR_NOT_SUPPORTED;
   if ((e = fa_check_gpu(hip_stream)) != FA_SUCCESS) return e;
   const int64_t stats = (int64_t)a.batch * a.heads * a.rows_q, shared = (int64_t)a.batch * a.heads * a.rows_k * kShared;
-  if (stats + shared == 0) return FA_SUCCESS;
+  if (stats + (int64_t)a.batch * a.rows_k == 0) return FA_SUCCESS;
   const int64_t stat_bytes = (stats * 2 * 4 + 255) / 256 * 256;
-  void* scratch = alloc != nullptr ? alloc->alloc(alloc, (uint64_t)(stat_bytes + shared * 4)) : nullptr;
-  if (scratch == nullptr) return FA_ERROR_OUT_OF_MEMORY;
+  void* scratch = nullptr;      // (without heads DS is 0)
+  if (a.heads > 0) {
+    scratch = alloc != nullptr ? alloc->alloc(alloc, (uint64_t)(stat_bytes + shared * 4)) : nullptr;
+    if (scratch == nullptr) return FA_ERROR_OUT_OF_MEMORY;
+  }
   a.stat_lse = static_cast<float*>(scratch);
   a.stat_delta = a.stat_lse + stats;
   a.part_c = reinterpret_cast<float*>(static_cast<char*>(scratch) + stat_bytes);

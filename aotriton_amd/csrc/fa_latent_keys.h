@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256, 1) void latent_dkdv_kernel(const LatentBwdArgs
     qt.fetch(q_rs, lds);
     rt.fetch(q_rs, base + SM::C_OFF + wave * 16 * 2 * kLatentShared);
     dt.fetch(wave_rsrc_words(row_at<T>(a.dout, a.sdo, si, h, at), rows_extent(left, do_row, a.ev * 2)), lds + SM::V_OFF);
-    // (of a row past the sequence Q, dO and both statistics are 0: nothing comes of it)
+    // (of a row past the sequence both statistics are 0)
     if (wave < 2) {
       const int n = si.seqlen_q - j * 64 < 64 ? si.seqlen_q - j * 64 : 64;
       load_word_to_lds(wave_rsrc_words(stats + j * 64, n > 0 ? n * 4 : 0), lane * 4, base + SM::STAGE + wave * 256);
@@ -126,14 +126,15 @@ __global__ __launch_bounds__(256, 1) void latent_dkdv_kernel(const LatentBwdArgs
       ds_op[e / 8] = pack8<T>(dp[b], e / 8);
     }
   };
-  // Half b of the queries from m0 on: of those that do not see the lane's key, S is what P of 0 comes from.
+  // Half b of the queries from m0 on: of those that do not see the lane's key, and those behind the sequence (rows that share memory, as those of the
+  // gradient of a sum, do not read as zeros there), S is what P of 0 comes from.
   auto hide = [&](auto half, int m0) __attribute__((always_inline)) {
     constexpr int b = decltype(half)::value;
-    if (!(a.causal && m0 < w0 + 31 - shift) && qs != 0.f) return;
-    const int from = a.causal ? key - shift - m0 - 4 * hi : 0;      // the lane's key is seen from this row of the half on
+    if (!(a.causal && m0 < w0 + 31 - shift) && m0 + 32 <= si.seqlen_q && qs != 0.f) return;
+    const int from = a.causal ? key - shift - m0 - 4 * hi : 0, to = si.seqlen_q - m0 - 4 * hi;      // rows of the half that see the lane's key
     const float never = qs < 0.f ? __builtin_inff() : -__builtin_inff();
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[b][e] = 8 * (e / 4) + e % 4 < from ? never : qs == 0.f ? 0.f : s[b][e];
+    for (int e = 0; e < 16; ++e) s[b][e] = 8 * (e / 4) + e % 4 < from || 8 * (e / 4) + e % 4 >= to ? never : qs == 0.f ? 0.f : s[b][e];
   };
   // S and dP of half b of a tile, with P and dS of the half in front behind their MFMAs
   auto front = [&](auto half, auto behind) __attribute__((always_inline)) {
@@ -251,7 +252,8 @@ template <typename T, int EC> hipError_t launch_latent_keys(const LatentBwdArgs&
   a.group = latent_group(nseq * a.heads, tiles);
   hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_dkdv_kernel<T, EC>), LatentSmem<EC>::BWD_BYTES, done);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((latent_dkdv_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles)), dim3(256), LatentSmem<EC>::BWD_BYTES, s, a, nseq, tiles);
+  if (a.heads > 0)
+    hipLaunchKernelGGL((latent_dkdv_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles)), dim3(256), LatentSmem<EC>::BWD_BYTES, s, a, nseq, tiles);
   const int32_t* end = a.seq.num_seqlens != 0 ? a.seq.cu_k + nseq : nullptr;
   hipLaunchKernelGGL((latent_dc_kernel<T>), dim3((unsigned)((a.batch * a.part_rows + 15) / 16)), dim3(256), 0, s, a, a.part_rows, end);
   return hipGetLastError();

@@ -203,6 +203,24 @@ def test_nothing_to_do(Sq, Sk):
     assert out.shape == (0, 2, 30, 64) and [g.shape for g in grads] == [t.shape for t in (q, k, v, c)]
 
 
+def test_no_heads():
+    q, k, v, c, do = _inputs(2, 0, 30, 40, 64, 32, 64, BF)
+    out, grads = _step(q, k, v, c, do)
+    assert out.shape == (2, 0, 30, 64) and [g.shape for g in grads] == [t.shape for t in (q, k, v, c)] and (grads[3] == 0).all()
+
+
+@pytest.mark.parametrize('Sq', [1, 70, 128])
+def test_rows_that_share_memory(Sq):
+    """the gradient of a sum over rows, the same query for all of them, a single row whose stride says nothing: nothing of them lies behind the last row"""
+    q, k, v, c, do = _inputs(2, 3, Sq, 100, 64, 32, 64, HF, seed=12)
+    one = lambda t: t[:, :, :1].expand(-1, -1, Sq, -1)
+    flat = lambda t: t.as_strided(t.shape, (t.stride(0), t.stride(1), 0, 1)) if Sq == 1 else one(t)
+    for qq, dd in ((q, one(do)), (one(q), do), (flat(q), flat(do))):
+        want, wgrads = _step(qq.contiguous(), k, v, c, dd.contiguous())
+        out, grads = _step(qq, k, v, c, dd)
+        assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(grads, wgrads))
+
+
 @pytest.mark.parametrize('scale', [0.0, -0.1, 3.0, 1e-3])
 def test_scales(scale):
     q, k, v, c, do = _inputs(1, 2, 150, 150, 128, 64, 128, BF, seed=5)
