@@ -205,8 +205,8 @@ __global__ __launch_bounds__(256) void append_packed_kernel(const PackedAppendAr
 // ---- reserve: pages for the rows that a batch adds, and where each goes ----------------------------------------------------
 // The k-th column that needs a page, in the order of sequences and columns, gets the k-th free page.  Two launches: the first notes which
 // pages are free and counts what each sequence asks for; the second gives each sequence its pages from there, so that nothing it reads is
-// what another workgroup writes.  Bound by dependent round trips to memory: 200 sequences and 16384 pages 3.8 + 5.9 us, 500 with prompts of up to
-// 6000 tokens and 400000 pages 4.8 + 13.3.
+// what another workgroup writes.  Bound by dependent round trips to memory: 200 sequences and 16384 pages 3.8 + 6 us, 500 with prompts of up to
+// 6000 tokens and 400000 pages 4.8 + 10.4 (one workgroup with all of it in LDS: 15.6 for the former).
 struct Reserve {
   int32_t start, count;          // first row of the sequence in the batch, rows
   int32_t first, last;           // columns that they touch, as far as the table goes
@@ -323,19 +323,29 @@ __global__ __launch_bounds__(256) void reserve_kernel(const ReserveArgs a) {
   __shared__ int64_t sums[8];
   __shared__ int32_t run_sum[kReserveRuns + 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, z = blockIdx.x;
+  // (what is read from memory whatever comes of it, in front of the first wait)
+  const bool is = z < a.sequences;
+  const int end = a.starts[a.sequences], length = is ? a.lengths[z] : 0, wanted = is ? a.wanted[z] : 0;
+  const Reserve r = is ? reserve_of(a, z, a.starts[z]) : Reserve{0, 0, 0, 0};
+  int32_t* row = a.table + (int64_t)z * a.table_row;
+  int own = r.first + tid < r.last ? row[r.first + tid] : 0, in_run[kReserveRuns / 256];
+#pragma unroll
+  for (int i = 0; i < kReserveRuns / 256; ++i) in_run[i] = i * 256 + tid < a.runs ? a.run_free[i * 256 + tid] : 0;
   // free pages in front of each run
   int base = 0;
-  for (int i0 = 0; i0 < a.runs; i0 += 256) {
-    const int n = i0 + tid < a.runs ? a.run_free[i0 + tid] : 0;
+#pragma unroll
+  for (int i = 0; i < kReserveRuns / 256; ++i) {
+    if (i * 256 >= a.runs) break;
+    const int n = in_run[i];
     int s = n;
 #pragma unroll
-    for (int i = 1; i < 64; i *= 2) { const int y = __shfl_up(s, i); s += lane >= i ? y : 0; }
+    for (int d = 1; d < 64; d *= 2) { const int y = __shfl_up(s, d); s += lane >= d ? y : 0; }
     if (lane == 63) sums[wave] = s;
     __syncthreads();
     for (int w = 0; w < 4; ++w) {
       if (w < wave) s += (int)sums[w];
     }
-    if (i0 + tid < a.runs) run_sum[i0 + tid] = base + s - n;
+    if (i * 256 + tid < a.runs) run_sum[i * 256 + tid] = base + s - n;
     base += (int)(sums[0] + sums[1] + sums[2] + sums[3]);
     __syncthreads();
   }
@@ -344,14 +354,13 @@ __global__ __launch_bounds__(256) void reserve_kernel(const ReserveArgs a) {
   sum_before(a.sequences, z, [&](int i) { return (int64_t)a.wanted[i]; }, sums, rank, all);
   if (z == 0 && tid == 0) *a.missing = (int)(all > free ? all - free : 0);
   // rows of no sequence
-  for (int64_t i = (int64_t)a.starts[a.sequences] + blockIdx.x * 256 + tid; i < a.tokens; i += (int64_t)gridDim.x * 256) a.slots[i] = -1;
-  if (z >= a.sequences) return;
-  const Reserve r = reserve_of(a, z, a.starts[z]);
-  int32_t* row = a.table + (int64_t)z * a.table_row;
-  if (a.wanted[z] > 0)
+  for (int64_t i = (int64_t)end + blockIdx.x * 256 + tid; i < a.tokens; i += (int64_t)gridDim.x * 256) a.slots[i] = -1;
+  if (!is) return;
+  if (wanted > 0)
     for (int c0 = r.first; c0 < r.last; c0 += 256) {
-      const int c = c0 + tid;
-      const bool want = c < r.last && no_page(a, row[c]);
+      const int c = c0 + tid, entry = own;
+      own = c + 256 < r.last ? row[c + 256] : 0;
+      const bool want = c < r.last && no_page(a, entry);
       const uint64_t ask = __builtin_amdgcn_ballot_w64(want);
       if (lane == 0) sums[wave] = __builtin_popcountll(ask);
       __syncthreads();
@@ -367,7 +376,6 @@ __global__ __launch_bounds__(256) void reserve_kernel(const ReserveArgs a) {
       }
       __syncthreads();
     }
-  const int length = a.lengths[z];
   // (eight look-ups on their way: one after the other 6000 rows took 6 us)
   constexpr int N = 8;
   for (int i0 = tid; i0 < r.count; i0 += 256 * N) {
