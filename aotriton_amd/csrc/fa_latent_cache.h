@@ -57,14 +57,20 @@ struct LatentSeq {
     const int n = tiles > filled ? (tiles - filled - 1) >> a.step_shift : 0, all = (blocks + (1 << a.group_shift) - 1) >> a.group_shift;
     return n < all ? n : all;
   }
-  // The list counts a block's tiles and LatentCacheArgs::margin on either side of them, for what beginning and ending it takes.
+  // The list counts a block's tiles and LatentCacheArgs::margin on either side of them, for what beginning and ending it takes; blocks alone where
+  // they stay whole.
   __device__ __forceinline__ int64_t units(const LatentCacheArgs& a) const {
+    if (a.margin < 0) return blocks;
     const int64_t n = short_groups(a), over = (n << a.group_shift) - blocks;      // (the last group may be short of blocks)
     const int64_t u = (n * filled + ((n * (n + 1) / 2) << a.step_shift)) << a.group_shift, last = over > 0 ? filled + (n << a.step_shift) : tiles;
     return u - over * last + (int64_t)blocks * (2 * a.margin);
   }
   // the block with unit `rel` of the sequence, and the unit's number in it
   __device__ __forceinline__ int block_of(const LatentCacheArgs& a, int64_t rel, int& unit) const {
+    if (a.margin < 0) {
+      unit = 0;
+      return (int)rel;
+    }
     const int n = short_groups(a);
     for (int g = 0; g < n; ++g) {
       const int group = 1 << a.group_shift, t = filled + ((g + 1) << a.step_shift) + 2 * a.margin, have = blocks - g * group < group ? blocks - g * group : group;
@@ -230,13 +236,14 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     const int lane = own_lane(), c = lane & 31, hi = lane >> 5;
     const int block_tiles = __builtin_amdgcn_readfirstlane(s.tiles_of(a, block));
     // (a cut beside the tiles leaves the block to one side of it)
+    const int span = a.margin < 0 ? 1 : block_tiles + 2 * a.margin;
     auto tile_of = [&](int64_t x) {
-      const int64_t n = x - at_unit - a.margin;
+      const int64_t n = a.margin < 0 ? (x > at_unit ? block_tiles : 0) : x - at_unit - a.margin;
       return __builtin_amdgcn_readfirstlane(n < 0 ? 0 : n < block_tiles ? (int)n : block_tiles);
     };
     const int j0 = tile_of(u), n_tiles = tile_of(u_end) - j0;
     if (n_tiles <= 0) {
-      at_unit += block_tiles + 2 * a.margin;
+      at_unit += span;
       ++block;
       continue;
     }
@@ -591,7 +598,7 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
         if (w0 + r1 < rows && col < ev) *reinterpret_cast<u32x4_t*>(to + at) = y;
       }
     }
-    at_unit += block_tiles + 2 * a.margin;
+    at_unit += span;
     ++block;
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (what comes next takes the rows' place)
   }
