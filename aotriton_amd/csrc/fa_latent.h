@@ -96,7 +96,7 @@ template <int EC> struct LatentSmem {
   static constexpr int C_OFF = TILE, V_OFF = TILE + SHARED;
   static constexpr int STAGE = 2 * TILE + SHARED;      // K, C, V (dK/dV: Q, its shared part, dO)
   static constexpr int STATS = 2 * 64 * 4;
-  static constexpr int BYTES = 2 * STAGE, BWD_STAGE = STAGE + STATS, BWD_BYTES = 3 * BWD_STAGE;
+  static constexpr int BYTES = 2 * STAGE, BWD_STAGE = STAGE + STATS, BWD_BYTES = 3 * BWD_STAGE, DQ_BYTES = 3 * STAGE;
   // a wave's own rows before and after the loop over tiles: two tensors of EC columns, then one of the shared part
   static constexpr int WAVE = STAGE / 2, WAVE_V = 32 * EC * 2, WAVE_C = 2 * WAVE_V;
 };

@@ -82,12 +82,17 @@ int check_fwd(const fa_latent_fwd_params* p, bool lse_needed, fa::LatentArgs* ou
 
 int compiled(const fa::LatentArgs& a) { return a.e <= 64 && a.ev <= 64 ? 64 : 128; }
 
+// Tiles of 128 queries of all heads; of packed sequences about as many.
+int64_t query_tiles(const fa::LatentArgs& a) {
+  const int64_t nseq = sequences(a);
+  return a.heads * (a.seq.num_seqlens > 0 ? a.rows_q / 128 + (nseq + 1) / 2 : nseq * ((a.rows_q + 127) / 128));
+}
+
 // Parts that the keys are cut into: where the tiles of 128 queries do not fill the chip, as many as do, of eight tiles of keys at least.
 // (4 heads, 128 queries, 8192 keys: uncut 181 us, in 4 parts 54, in 16, the rule's, 30; 16 heads, 128 queries, 4096 keys: 95, 33, in 8 25, in 16 28;
 // 16 heads, 1024 queries, 4096 keys: 102, in 4, the rule's, 53, in 8 65.)
 int latent_parts(const fa::LatentArgs& a, int num_cu) {
-  const int64_t nseq = sequences(a);
-  const int64_t tiles = a.heads * (a.seq.num_seqlens > 0 ? a.rows_q / 128 + (nseq + 1) / 2 : nseq * ((a.rows_q + 127) / 128));
+  const int64_t tiles = query_tiles(a);
   const int64_t chip = 2 * (int64_t)num_cu, keys = (a.seq.max_seqlen_k + 63) / 64;
   if (tiles == 0) return 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>({chip / tiles, keys / 8, 16}));
@@ -147,6 +152,9 @@ int fa_latent_bwd(const fa_latent_bwd_params* p, void* hip_stream, fa_allocator*
   a.stat_lse = static_cast<float*>(scratch);
   a.stat_delta = a.stat_lse + stats;
   a.part_c = reinterpret_cast<float*>(static_cast<char*>(scratch) + stat_bytes);
+  // (steps of 1 to 16 heads, E = Ev = 128, R = 64: 128 tiles 361 us with two waves on a SIMD, 311 alone, 256 tiles 399 and 350, 512 480 and 443, 752 878 and
+  // 881, 2800 1655 and 1705)
+  a.alone = query_tiles(a) <= 2 * (int64_t)fa_get_multiprocessor_count(hip_stream);
   return (int)(compiled(a) == 64 ? fa::run_latent_bwd_d64 : fa::run_latent_bwd_d128)(f.Q.dtype, a, static_cast<hipStream_t>(hip_stream));
 }
 

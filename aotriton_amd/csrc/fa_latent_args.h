@@ -35,6 +35,7 @@ struct LatentBwdArgs : LatentArgs {
   // Every head's sum for the shared part, fp32 (sequence or batch and head, key, 64 columns): summed over the heads by a launch of its own.
   float* part_c;
   int64_t part_rows;             // keys of a (batch, head) slab of part_c
+  bool alone;                    // dQ in its form for few workgroups (fa_latent_keys.h)
 };
 
 // A block of rows that lies in several pieces: the first of them (two times its worker, plus its place there), how many (0: the block is one
@@ -66,6 +67,8 @@ hipError_t run_latent_fwd_d64(int dtype, const LatentArgs& a, hipStream_t s);
 hipError_t run_latent_fwd_d128(int dtype, const LatentArgs& a, hipStream_t s);
 hipError_t run_latent_bwd_d64(int dtype, const LatentBwdArgs& a, hipStream_t s);
 hipError_t run_latent_bwd_d128(int dtype, const LatentBwdArgs& a, hipStream_t s);
+hipError_t run_latent_dq_alone_d64(int dtype, const LatentBwdArgs& a, hipStream_t s);
+hipError_t run_latent_dq_alone_d128(int dtype, const LatentBwdArgs& a, hipStream_t s);
 hipError_t run_latent_keys_d64(int dtype, const LatentBwdArgs& a, hipStream_t s);      // dK, dV and dC, behind dQ
 hipError_t run_latent_keys_d128(int dtype, const LatentBwdArgs& a, hipStream_t s);
 // compiled columns in front of the last 64 (256 or 512)

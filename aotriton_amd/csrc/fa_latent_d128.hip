@@ -7,7 +7,7 @@ hipError_t run_latent_fwd_d128(int dtype, const LatentArgs& a, hipStream_t s) {
   return dtype == kDtypeBF16 ? launch_latent_fwd<bf16_t, 128>(a, s) : launch_latent_fwd<f16_t, 128>(a, s);
 }
 hipError_t run_latent_bwd_d128(int dtype, const LatentBwdArgs& a, hipStream_t s) {
-  const hipError_t e = dtype == kDtypeBF16 ? launch_latent_dq<bf16_t, 128>(a, s) : launch_latent_dq<f16_t, 128>(a, s);
+  const hipError_t e = a.alone ? run_latent_dq_alone_d128(dtype, a, s) : dtype == kDtypeBF16 ? launch_latent_dq<bf16_t, 128>(a, s) : launch_latent_dq<f16_t, 128>(a, s);
   return e != hipSuccess ? e : run_latent_keys_d128(dtype, a, s);
 }
 }  // namespace fa

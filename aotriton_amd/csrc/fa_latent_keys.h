@@ -228,6 +228,231 @@ __global__ __launch_bounds__(256, 1) void latent_dkdv_kernel(const LatentBwdArgs
                         kLatentShared, lane, own);
 }
 
+// ---- dQ where a CU has no more than two workgroups --------------------------------------------------------------------
+// As dK/dV above, with a wave's 32 rows in registers and tiles of 64 keys passing: one wave on a SIMD gets through a tile sooner than one of two, which
+// is what counts where few workgroups are all there is.  delta as in latent_dq_kernel.
+template <typename T, int EC>
+__global__ __launch_bounds__(256, 1) void latent_dq_alone_kernel(const LatentBwdArgs a, int nseq, int tiles) {
+  using Tr = Traits<T>;
+  using op_t = typename Tr::op_t;
+  using SM = LatentSmem<EC>;
+  constexpr int KE = EC / 16, KR = kLatentShared / 16, DB = EC / 32, RB = kLatentShared / 32;
+  extern __shared__ __attribute__((aligned(kSwzAlign))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int z, h, mt;
+  latent_item(a, blockIdx.x, nseq, tiles, a.causal != 0, z, h, mt);
+  const SeqInfo si = latent_seq(a, z);
+  const int q0 = mt * 128;
+  if (q0 >= si.seqlen_q) return;
+  const int shift = si.seqlen_k - si.seqlen_q;
+  const int w0 = q0 + wave * 32, row = w0 + c, rows = si.seqlen_q - w0;
+  auto last_key = [&](int r) { return a.causal ? (r < si.seqlen_q ? r : si.seqlen_q - 1) + shift : si.seqlen_k - 1; };
+  auto tiles_of = [&](int r) { const int n = last_key(r) + 1; return n > 0 ? (n + 63) / 64 : 0; };
+  const int j1 = tiles_of(q0 + 127), see = last_key(row);
+  const int see_least = __builtin_amdgcn_readfirstlane(last_key(w0));      // of the wave's rows
+
+  const int smem0 = lds_offset(smem);
+  const int k_row = (int)a.sk.s * 2, v_row = (int)a.sv.s * 2, c_row = (int)a.c_s * 2;
+  const TileRows<EC> kt(lane, k_row, 0, a.e), vt(lane, v_row, 0, a.ev);
+  const TileRows<kLatentShared> ct(lane, c_row, 0, a.r);
+  auto fetch = [&](int stage, int j) __attribute__((always_inline)) {
+    const int n = j * 64 + wave * 16, left = si.seqlen_k - n < 16 ? si.seqlen_k - n : 16;
+    const int64_t at = si.k_start + n;
+    const int lds = smem0 + stage * SM::STAGE + wave * 16 * 2 * EC;
+    kt.fetch(wave_rsrc_words(row_at<T>(a.k, a.sk, si, h, at), rows_extent(left, k_row, a.e * 2)), lds);
+    vt.fetch(wave_rsrc_words(row_at<T>(a.v, a.sv, si, h, at), rows_extent(left, v_row, a.ev * 2)), lds + SM::V_OFF);
+    ct.fetch(wave_rsrc_words(row_at<T>(a.c, Strides3{a.c_z, 0, a.c_s}, si, 0, at), rows_extent(left, c_row, a.r * 2)),
+             smem0 + stage * SM::STAGE + SM::C_OFF + wave * 16 * 2 * kLatentShared);
+  };
+  op_t q[KE + KR], dout[KE];
+  const int own = smem0 + wave * SM::WAVE;
+  {
+    const T* qp = row_at<T>(a.q, a.sq, si, h, (int64_t)si.q_start + w0);
+    fetch_rows<EC>(qp, (int)a.sq.s * 2, rows, lane, 0, a.e, own);
+    fetch_rows<EC>(row_at<T>(a.dout, a.sdo, si, h, (int64_t)si.q_start + w0), (int)a.sdo.s * 2, rows, lane, 0, a.ev, own + SM::WAVE_V);
+    fetch_rows<kLatentShared>(qp, (int)a.sq.s * 2, rows, lane, a.e, a.r, own + SM::WAVE_C);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    take_rows<T, EC>(q, lane, own);
+    take_rows<T, EC>(dout, lane, own + SM::WAVE_V);
+    take_rows<T, kLatentShared>(q + KE, lane, own + SM::WAVE_C);
+  }
+  arrived(q);
+  arrived(dout);
+  latent_meet();
+  if (j1 > 0) fetch(0, 0);
+  const bool few = j1 <= kLatentFewTiles;
+  float delta = 0.f, lse = __builtin_inff();
+  if (row < si.seqlen_q) lse = a.lse[lse_offset(si, h, a.heads) + row] * kLog2e;
+  if (!few) {
+    op_t out[KE];
+    const int place = smem0 + SM::STAGE + wave * SM::WAVE_V;      // (in the next stage)
+    fetch_rows<EC>(row_at<T>(a.out, a.so, si, h, (int64_t)si.q_start + w0), (int)a.so.s * 2, rows, lane, 0, a.ev, place);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    take_rows<T, EC>(out, lane, place);
+#pragma unroll
+    for (int k = 0; k < KE; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta += (float)out[k][i] * (float)dout[k][i];
+  }
+  const float qs = a.sm_scale * kLog2e, qs_or_1 = qs == 0.f ? 1.f : qs;
+  constexpr int kS = KE + KR, kA = kS + KE, kB = 2 * (DB + RB), kRing = 6;      // MFMAs of S, of both; of the product with dS; operands on their way
+  // addresses of the operands in the stages of S and of the product (fa_latent_cache.h)
+  int at_e[8], at_r[KR], at_t[8], at_c[4];
+  static_assert(KE <= 8 && DB <= 4, "a tile's row is one period of the swizzle");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    at_e[i] = smem0 + (Swz<EC>::row_base(lane) ^ (i % KE << 5));
+    at_t[i] = smem0 + (Swz<EC>::tr_base(lane, i >> 2) ^ ((i & 3) % DB << 6));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    at_r[i] = smem0 + SM::C_OFF + (Swz<kLatentShared>::row_base(lane) ^ (i << 5));
+    at_c[i] = smem0 + SM::C_OFF + (Swz<kLatentShared>::tr_base(lane, i >> 1) ^ ((i & 1) << 6));
+  }
+  auto onward = [&](auto& at, int by) __attribute__((always_inline)) {
+#pragma unroll
+    for (auto& x : at) x += by;
+    arrived(at);
+  };
+  op_t ring[kRing], ds_op[2];
+  f32x16 s[2], dp[2];
+  // operand n of the products of S and dP of half b of a tile: K, the shared part, V
+  auto read_a = [&](int b, int n) __attribute__((always_inline)) {
+    if (n < KE) return lds_read<op_t>(at_e[n] + b * 32 * Swz<EC>::ROWB);
+    if (n < kS) return lds_read<op_t>(at_r[n - KE] + b * 32 * Swz<kLatentShared>::ROWB);
+    return lds_read<op_t>(at_e[n - kS] + SM::V_OFF + b * 32 * Swz<EC>::ROWB);
+  };
+  // of dQ, 16 keys after the other
+  auto read_b = [&](int b, int n) __attribute__((always_inline)) {
+    const int t = 2 * b + n / (kB / 2), x = n % (kB / 2);
+    const int off = t * 16 * (x < DB ? Swz<EC>::ROWB : Swz<kLatentShared>::ROWB);
+    const int lo = (x < DB ? at_t[x % DB] : at_c[x - DB]) + off, up = (x < DB ? at_t[4 + x % DB] : at_c[2 + x - DB]) + off;
+    return __builtin_shufflevector(__builtin_bit_cast(typename Tr::q4_t, lds_read_tr_at(lo)), __builtin_bit_cast(typename Tr::q4_t, lds_read_tr_at(up)), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  // Half b of the keys from n0 on: of those that a row does not see, S is what P of 0 comes from.
+  auto hide = [&](auto half, int n0) __attribute__((always_inline)) {
+    constexpr int b = decltype(half)::value;
+    if (n0 + 31 <= see_least && qs != 0.f) return;
+    const int limit = see - n0 - 4 * hi;
+    const float never = qs < 0.f ? __builtin_inff() : -__builtin_inff();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[b][e] = 8 * (e / 4) + e % 4 > limit ? never : qs == 0.f ? 0.f : s[b][e];
+  };
+  // P and dS of element e of the lane's 16 in s[b] and dp[b]
+  auto element = [&](int b, int e) __attribute__((always_inline)) {
+    s[b][e] = fast_exp2(__builtin_fmaf(s[b][e], qs_or_1, -lse)) * (dp[b][e] - delta);
+    if (e % 8 == 7) ds_op[e / 8] = pack8<T>(s[b], e / 8);
+  };
+  // S and dP of half b of a tile, with dS of the half in front behind their MFMAs
+  auto front = [&](auto half, auto behind) __attribute__((always_inline)) {
+    constexpr int b = decltype(half)::value;
+#pragma unroll
+    for (int n = 0; n < kRing - 1; ++n) ring[n] = read_a(b, n);
+#pragma unroll
+    for (int n = 0; n < kA; ++n) {
+      if (n + kRing - 1 < kA) ring[(n + kRing - 1) % kRing] = read_a(b, n + kRing - 1);
+      const f32x16 none = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (n < kS) s[b] = Tr::mfma(ring[n % kRing], q[n], n == 0 ? none : s[b]);
+      else dp[b] = Tr::mfma(ring[n % kRing], dout[n - kS], n == kS ? none : dp[b]);
+      if constexpr (decltype(behind)::value) {
+#pragma unroll
+        for (int e = first_of(n, 16, kA); e < first_of(n + 1, 16, kA); ++e) element(1 - b, e);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  using zero = std::integral_constant<int, 0>;
+  using one = std::integral_constant<int, 1>;
+  using yes = std::true_type;
+  using no = std::false_type;
+  int stage = 0;      // of the tile that comes next
+  auto step_of = [&]() { return stage == 2 ? -2 * SM::STAGE : SM::STAGE; };
+  if (few) {
+    for (int j = 0; j < j1; ++j) {
+      latent_meet();
+      fetch(stage == 2 ? 0 : stage + 1, j + 1 < j1 ? j + 1 : 0);
+      front(zero{}, no{});
+      front(one{}, no{});
+      hide(zero{}, 64 * j);
+      hide(one{}, 64 * j + 32);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) delta = __builtin_fmaf(fast_exp2(__builtin_fmaf(s[b][e], qs_or_1, -lse)), dp[b][e], delta);
+      onward(at_e, step_of());
+      onward(at_r, step_of());
+      onward(at_t, step_of());
+      onward(at_c, step_of());
+      stage = stage == 2 ? 0 : stage + 1;
+    }
+  }
+  delta = cross_sum(delta);
+  if (row < si.seqlen_q && hi == 0) {
+    const int64_t at = lse_offset(si, h, a.heads) + row;
+    a.stat_lse[at] = lse;
+    a.stat_delta[at] = delta;
+  }
+  // (accumulators are written as asm, fa_wide.h, so that S and dP lie in vector registers, where the exponentials are)
+  f32x16 dq[DB + RB];
+#pragma unroll
+  for (int b = 0; b < DB + RB; ++b) acc_zero<T>(dq[b]);
+  auto back = [&](auto half) __attribute__((always_inline)) {
+    constexpr int b = decltype(half)::value;
+#pragma unroll
+    for (int n = 0; n < kRing - 1; ++n) ring[n] = read_b(b, n);
+#pragma unroll
+    for (int n = 0; n < kB; ++n) {
+      if (n + kRing - 1 < kB) ring[(n + kRing - 1) % kRing] = read_b(b, n + kRing - 1);
+      mfma_acc<T>(dq[n % (kB / 2)], ring[n % kRing], ds_op[n / (kB / 2)]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // (what dS lost in 16 bits, where few keys do not average it out: latent_dkdv_kernel)
+  const bool twice = j1 == 1;
+  auto rest = [&](auto half) __attribute__((always_inline)) {
+    constexpr int b = decltype(half)::value;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[b][e] -= (float)ds_op[e / 8][e % 8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) ds_op[t] = pack8<T>(s[b], t);
+  };
+  if (j1 > 0) {
+    latent_meet();
+    if (j1 > 1) fetch(stage == 2 ? 0 : stage + 1, 1);
+    front(zero{}, no{});
+  }
+  for (int j = 0; j < j1; ++j) {
+    hide(zero{}, 64 * j);
+    front(one{}, yes{});
+    back(zero{});
+    if (twice) {
+      rest(zero{});
+      back(zero{});
+    }
+    const int by = step_of();
+    onward(at_e, by);
+    onward(at_r, by);
+    if (j + 1 < j1) latent_meet();
+    if (j + 2 < j1) fetch(stage == 0 ? 2 : stage - 1, j + 2);
+    hide(one{}, 64 * j + 32);
+    front(zero{}, yes{});
+    back(one{});
+    if (twice) {
+      rest(one{});
+      back(one{});
+    }
+    onward(at_t, by);
+    onward(at_c, by);
+    stage = stage == 2 ? 0 : stage + 1;
+  }
+  latent_meet();
+  settle(dq);
+  T* to = row_at<T>(a.dq, a.sdq, si, h, (int64_t)si.q_start + w0);
+  store_rows<T, DB>(dq, a.sm_scale, to, a.sdq.s, rows, a.e, lane, own);
+  store_rows<T, RB>(dq + DB, a.sm_scale, to + a.e, a.sdq.s, rows, a.r, lane, own + kRowsOut<T, DB>);
+}
+
 // dC: the heads' parts added in their order, four columns a lane
 template <typename T>
 __global__ __launch_bounds__(256) void latent_dc_kernel(const LatentBwdArgs a, int64_t keys, const int32_t* end) {
@@ -256,6 +481,18 @@ template <typename T, int EC> hipError_t launch_latent_keys(const LatentBwdArgs&
     hipLaunchKernelGGL((latent_dkdv_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles)), dim3(256), LatentSmem<EC>::BWD_BYTES, s, a, nseq, tiles);
   const int32_t* end = a.seq.num_seqlens != 0 ? a.seq.cu_k + nseq : nullptr;
   hipLaunchKernelGGL((latent_dc_kernel<T>), dim3((unsigned)((a.batch * a.part_rows + 15) / 16)), dim3(256), 0, s, a, a.part_rows, end);
+  return hipGetLastError();
+}
+
+template <typename T, int EC> hipError_t launch_latent_dq_alone(const LatentBwdArgs& args, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  const int nseq = nseq_of(args.seq, args.batch), tiles = (args.seq.max_seqlen_q + 127) / 128;
+  if (nseq * args.heads == 0 || tiles == 0) return hipSuccess;
+  LatentBwdArgs a = args;
+  a.group = latent_group(nseq * a.heads, tiles);
+  hipError_t e = allow_large_lds(reinterpret_cast<const void*>(&latent_dq_alone_kernel<T, EC>), LatentSmem<EC>::DQ_BYTES, done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((latent_dq_alone_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles)), dim3(256), LatentSmem<EC>::DQ_BYTES, s, a, nseq, tiles);
   return hipGetLastError();
 }
 

@@ -6,4 +6,7 @@ namespace fa {
 hipError_t run_latent_keys_d64(int dtype, const LatentBwdArgs& a, hipStream_t s) {
   return dtype == kDtypeBF16 ? launch_latent_keys<bf16_t, 64>(a, s) : launch_latent_keys<f16_t, 64>(a, s);
 }
+hipError_t run_latent_dq_alone_d64(int dtype, const LatentBwdArgs& a, hipStream_t s) {
+  return dtype == kDtypeBF16 ? launch_latent_dq_alone<bf16_t, 64>(a, s) : launch_latent_dq_alone<f16_t, 64>(a, s);
+}
 }  // namespace fa

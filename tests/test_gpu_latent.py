@@ -182,6 +182,20 @@ def test_more_heads_than_stand_side_by_side():
     assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(more, grads))
 
 
+@pytest.mark.parametrize('dtype', [HF, BF])
+@pytest.mark.parametrize('E,R,Ev,causal', [(64, 32, 64, True), (128, 64, 128, True), (72, 64, 40, False)])
+def test_many_workgroups(E, R, Ev, causal, dtype):
+    """more tiles of queries than two for a CU, of which a few heads are looked at: rows with few keys, and past those whose delta comes from P"""
+    B, H, Sq, Sk = 12, 24, 330, 333
+    q, k, v, c, do = _inputs(B, H, Sq, Sk, E, R, Ev, dtype, seed=E)
+    out, grads = _step(q, k, v, c, do, causal)
+    for b, h in ((0, 0), (5, 23), (11, 7)):
+        one = [t[b, h:h + 1] for t in (q, k, v)]
+        alone, g1 = _step(*(t[None] for t in one), c[b:b + 1], do[b:b + 1, h:h + 1], causal)
+        _check(*one, c[b], do[b, h:h + 1], causal, 1 / math.sqrt(E + R), out[b, h:h + 1], None, [grads[0][b, h:h + 1], grads[1][b, h:h + 1], grads[2][b, h:h + 1], g1[3][0]])
+        assert_within('out', out[b, h:h + 1], alone[0], torch.zeros(()))
+
+
 def test_offsets_outside_the_tensors():
     """what they name past the rows is not there, and neither are rows past the greatest length"""
     q, k, v, c, do = _inputs(1, 2, 200, 200, 64, 32, 64, BF, seed=4)
