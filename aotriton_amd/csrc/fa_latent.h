@@ -1,4 +1,4 @@
-// Attention whose keys are part per head, part shared by all heads, forward and dQ (dK, dV and dC: fa_latent_keys.h): gfx950, MFMA 32x32x16.
+// Attention whose keys are part per head, part shared by all heads, forward and dQ (dK, dV and dC, and dQ of few workgroups: fa_latent_keys.h): gfx950, MFMA 32x32x16.
 //
 //   S = scale (Qe K^T + Qr C^T),  P = softmax(S),  O = P V
 //   dV = P^T dO,  dS = P (dO V^T - rowsum(dO O)),  dQ = scale [dS K | dS C],  dK = scale dS^T Qe,  dC = scale sum over heads of dS^T Qr

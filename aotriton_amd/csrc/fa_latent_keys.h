@@ -1,4 +1,4 @@
-// dK, dV and dC of attention whose keys are part per head, part shared by all heads (fa_latent.h): gfx950, MFMA 32x32x16.
+// dK, dV and dC of attention whose keys are part per head, part shared by all heads (fa_latent.h), and dQ of few workgroups: gfx950, MFMA 32x32x16.
 #pragma once
 #include "fa_latent.h"
 
