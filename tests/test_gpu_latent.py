@@ -371,3 +371,68 @@ def test_gradients_against_differences():
         # (each of n outputs is rounded apart from the others: their sum by a few times the root of the sum of squares)
         off = 6 * 2.0 ** -11 * float((outs.abs() * do.double().abs()).norm()) + 0.02 * float((grads[i].double() * step).norm()) + 0.01 * abs(want)
         assert abs(got - want) < off, (i, got, want, off)
+
+
+# ---- dQ with two waves on a SIMD: calls with more than two workgroups for a CU -----------------------------------------------
+
+def _many(heads, tiles):
+    """query tiles of 128 over all heads, which choose the kernel"""
+    assert heads * tiles > 2 * torch.cuda.get_device_properties(0).multi_processor_count
+
+
+def _offsets(lens, first=0):
+    return torch.tensor([first + sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize('dtype', [HF, BF])
+@pytest.mark.parametrize('E,R,Ev,causal,scale', [(128, 64, 128, True, None), (64, 32, 64, True, -0.1), (72, 64, 40, False, None), (128, 64, 128, False, 0.0), (128, 64, 128, True, 1.0)])
+def test_packed_gradients_of_many_workgroups(E, R, Ev, causal, scale, dtype):
+    """sequences without queries or keys, of one tile and of several, rows before the first key; the shared part's gradient over all heads"""
+    lens_q, lens_k = [1, 300, 0, 77, 257, 5, 40, 64, 150], [1, 300, 7, 200, 257, 2, 0, 64, 90]
+    H, tq, tk, pad = 64, sum(lens_q), sum(lens_k), 3
+    _many(H, tq // 128 + (len(lens_q) + 1) // 2)
+    q, _, _, _, do = _inputs(1, H, tq + pad, 1, E, R, Ev, dtype, seed=31)
+    _, k, v, c, _ = _inputs(1, H, 1, tk + pad, E, R, Ev, dtype, seed=32)
+    for t in (q, do):
+        t[:, :, tq:] = float('nan')
+    for t in (k, v):
+        t[:, :, tk:] = float('inf')
+    c[:, tk:] = float('nan')
+    cq, ck = _offsets(lens_q), _offsets(lens_k)
+    out, grads = _step(q, k, v, c, do, causal, scale, cu_seqlens_q=cq, cu_seqlens_k=ck, max_seqlen_q=max(lens_q), max_seqlen_k=max(lens_k))
+    s = 1 / math.sqrt(E + R) if scale is None else scale
+    for i in range(len(lens_q)):
+        a, b = slice(int(cq[i]), int(cq[i + 1])), slice(int(ck[i]), int(ck[i + 1]))
+        _check(q[0][:, a], k[0][:, b], v[0][:, b], c[0][b], do[0][:, a], causal, s, out[0][:, a], None,
+               [grads[0][0][:, a], grads[1][0][:, b], grads[2][0][:, b], grads[3][0][b]], f'sequence {i} ')
+    assert (grads[0][:, :, tq:] == 0).all() and all((g[:, :, tk:] == 0).all() for g in grads[1:3]) and (grads[3][:, tk:] == 0).all()
+
+
+@pytest.mark.parametrize('dtype', [HF, BF])
+@pytest.mark.parametrize('B,H,Sq,Sk,E,R,Ev,causal,scale', [
+    (12, 48, 40, 40, 128, 64, 128, True, None),        # one tile of keys: what dS loses in 16 bits goes through the product as well
+    (18, 30, 100, 64, 64, 32, 64, False, -0.2),
+    (9, 64, 90, 30, 64, 64, 64, True, None),           # queries before the first key
+    (5, 60, 140, 100, 128, 40, 72, True, 0.0),
+    (6, 50, 200, 290, 128, 64, 128, True, 2.0)])       # delta from O
+def test_gradients_of_many_workgroups(B, H, Sq, Sk, E, R, Ev, causal, scale, dtype):
+    """every head of a few batches, and with them the shared part's gradient"""
+    _many(B * H, (Sq + 127) // 128)
+    q, k, v, c, do = _inputs(B, H, Sq, Sk, E, R, Ev, dtype, seed=Sq + 1)
+    out, grads = _step(q, k, v, c, do, causal, scale)
+    for b in (0, B - 1):
+        _check(q[b], k[b], v[b], c[b], do[b], causal, 1 / math.sqrt(E + R) if scale is None else scale, out[b], None, [g[b] for g in grads], f'sequence {b} ')
+
+
+@pytest.mark.parametrize('Sq,Sk', [(70, 100), (1, 60), (128, 300)])
+def test_rows_that_share_memory_of_many_workgroups(Sq, Sk):
+    B, H = 11, 50
+    _many(B * H, 1)
+    q, k, v, c, do = _inputs(B, H, Sq, Sk, 64, 32, 64, HF, seed=33)
+    one = lambda t: t[:, :, :1].expand(-1, -1, t.shape[2], -1)
+    heads = lambda t: t[:, :1].expand(-1, H, -1, -1)
+    for qq, kk, vv, dd in ((q, k, v, one(do)), (one(q), k, v, do), (q, heads(k), heads(v), one(do))):
+        want, wgrads = _step(qq.contiguous(), kk.contiguous(), vv.contiguous(), c, dd.contiguous())
+        out, grads = _step(qq, kk, vv, c, dd)
+        assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(grads, wgrads))
+    _check(q[3], k[3], v[3], c[3], do[3, :, :1].expand(-1, Sq, -1), True, 1 / math.sqrt(96), *(lambda o, g: (o[3], None, [x[3] for x in g]))(*_step(q, k, v, c, one(do))))
