@@ -54,7 +54,7 @@ struct LatentCacheArgs {
   // `workers` equal pieces of at least `least`, one for a workgroup; the sums of a block that lies in several pieces go to
   // part_o, two places for every worker.
   int32_t block_rows, workers, least;
-  int32_t margin;                // tiles that a block's beginning and its end take each (fa_latent_cache.h: LatentSeq::units); negative: blocks stay whole
+  int32_t margin;                // tiles that a block's beginning and its end take each (fa_latent_list.h: LatentSeq::units); negative: blocks stay whole
   int32_t block_shift;           // block_rows as a power of two; so, rounded, blocks that 32 tokens make (one at least), and tiles that a group's tokens make
   int32_t group_shift, step_shift;
   float* part_o; float* part_ml;

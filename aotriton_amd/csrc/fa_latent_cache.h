@@ -17,6 +17,7 @@
 #pragma once
 #include "fa_cache.h"
 #include "fa_latent_args.h"
+#include "fa_latent_list.h"
 #include "fa_latent_parts.h"
 
 namespace fa {
@@ -39,66 +40,10 @@ template <int EA> struct LatentCacheSmem {
   };
 };
 
-// a / b of numbers that are not negative (a division of 64 bits takes a microsecond)
-__device__ __forceinline__ int64_t latent_div(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b; }
-
-// A sequence as the list of work has it: `blocks` blocks of rows, of tiles as many as their last row sees, or some more: the blocks of a group
-// (LatentCacheArgs::group_shift) have the same number, a step more than the group in front, up to all `tiles`.
-struct LatentSeq {
-  int32_t start, tokens, length, end;      // first row of Q, tokens, filled slots, slots with the new ones as far as the table goes
-  int32_t blocks, tiles, filled;           // (filled: tiles in front of the first new slot)
-  __device__ __forceinline__ int tiles_of_group(const LatentCacheArgs& a, int g) const {
-    const int64_t n = filled + ((int64_t)(g + 1) << a.step_shift);
-    return n < tiles ? (int)n : tiles;
-  }
-  __device__ __forceinline__ int tiles_of(const LatentCacheArgs& a, int block) const { return tiles_of_group(a, block >> a.group_shift); }
-  // groups that have not all tiles, as far as there are blocks
-  __device__ __forceinline__ int short_groups(const LatentCacheArgs& a) const {
-    const int n = tiles > filled ? (tiles - filled - 1) >> a.step_shift : 0, all = (blocks + (1 << a.group_shift) - 1) >> a.group_shift;
-    return n < all ? n : all;
-  }
-  // The list counts a block's tiles and LatentCacheArgs::margin on either side of them, for what beginning and ending it takes; blocks alone where
-  // they stay whole.
-  __device__ __forceinline__ int64_t units(const LatentCacheArgs& a) const {
-    if (a.margin < 0) return blocks;
-    const int64_t n = short_groups(a), over = (n << a.group_shift) - blocks;      // (the last group may be short of blocks)
-    const int64_t u = (n * filled + ((n * (n + 1) / 2) << a.step_shift)) << a.group_shift, last = over > 0 ? filled + (n << a.step_shift) : tiles;
-    return u - over * last + (int64_t)blocks * (2 * a.margin);
-  }
-  // the block with unit `rel` of the sequence, and the unit's number in it
-  __device__ __forceinline__ int block_of(const LatentCacheArgs& a, int64_t rel, int& unit) const {
-    if (a.margin < 0) {
-      unit = 0;
-      return (int)rel;
-    }
-    const int n = short_groups(a);
-    for (int g = 0; g < n; ++g) {
-      const int group = 1 << a.group_shift, t = filled + ((g + 1) << a.step_shift) + 2 * a.margin, have = blocks - g * group < group ? blocks - g * group : group;
-      if (rel < (int64_t)have * t) {
-        const int b = (int)((uint32_t)rel / (uint32_t)t);
-        unit = (int)rel - b * t;
-        return g * group + b;
-      }
-      rel -= (int64_t)have * t;
-    }
-    const int t = tiles + 2 * a.margin;
-    const int64_t b = latent_div(rel, t);
-    unit = (int)(rel - b * t);
-    return (n << a.group_shift) + (int)b;
-  }
-};
 __device__ __forceinline__ LatentSeq latent_cache_seq(const LatentCacheArgs& a, int z) {
   auto hold = [](int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; };
-  LatentSeq s;
-  s.start = hold(a.starts[z], 0, a.rows);
-  s.tokens = hold(hold(a.starts[z + 1], 0, a.rows) - s.start, 0, a.rows);
-  s.length = a.cache.lengths[z];
-  const int64_t room = (int64_t)a.cache.columns << a.cache.page_shift, end = (int64_t)s.length + s.tokens;
-  s.end = s.length < 0 ? 0 : (int)(end < room ? end : room);
-  s.blocks = (s.tokens * a.hq + a.block_rows - 1) >> a.block_shift;
-  s.tiles = s.end > 32 ? (s.end + 31) / 32 : 1;
-  s.filled = s.length <= 0 ? 0 : s.length < s.end ? (s.length + 31) / 32 : s.tiles;
-  return s;
+  const int start = hold(a.starts[z], 0, a.rows);
+  return latent_seq_of(a, start, hold(hold(a.starts[z + 1], 0, a.rows) - start, 0, a.rows), a.cache.lengths[z], (int64_t)a.cache.columns << a.cache.page_shift);
 }
 
 // Number of a sequence's first block, with a gap or two: that of its first row, divided by the rows of a block, and one more for every sequence in
