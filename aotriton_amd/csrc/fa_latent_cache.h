@@ -198,10 +198,9 @@ __global__ __launch_bounds__(256, 1) void latent_cache_kernel(const LatentCacheA
     const bool row_ok = w0 + c < rows;
     const int row = row_ok ? w0 + c : rows - 1, token = row / a.hq, head = row - token * a.hq;
     // the last slot that the row sees, that the wave's first and last rows see
-    auto sees = [&](int t) { const int n = s.length + t; return n < s.end ? n : s.end - 1; };
-    const int see = sees(token);
-    const int see_least = __builtin_amdgcn_readfirstlane(sees(w0 / a.hq));
-    const int see_most = __builtin_amdgcn_readfirstlane(sees(w_last / a.hq));
+    const int see = s.last_slot(token);
+    const int see_least = __builtin_amdgcn_readfirstlane(s.last_slot(w0 / a.hq));
+    const int see_most = __builtin_amdgcn_readfirstlane(s.last_slot(w_last / a.hq));
     const int j1 = j0 + n_tiles, wave_end = w0 < rows ? see_most / 32 + 1 : 0;
 
     const char* xbase = reinterpret_cast<const char*>(ca.k);

@@ -15,13 +15,15 @@ FA_LIST int64_t latent_div(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ?
 // A sequence as the list of work has it: `blocks` blocks of rows, of tiles as many as their last row sees, or some more: the blocks of a group
 // (LatentCacheArgs::group_shift) have the same number, a step more than the group in front, up to all `tiles`.
 struct LatentSeq {
-  int32_t start, tokens, length, end;      // first row of Q, tokens, filled slots, slots with the new ones as far as the table goes
+  int32_t start, tokens, length, end;      // first row of Q, tokens, filled slots (-1: not there), slots with the new ones as far as the table goes
   int32_t blocks, tiles, filled;           // (filled: tiles in front of the first new slot)
   template <typename Args> FA_LIST int tiles_of_group(const Args& a, int g) const {
     const int64_t n = filled + ((int64_t)(g + 1) << a.step_shift);
     return n < tiles ? (int)n : tiles;
   }
   template <typename Args> FA_LIST int tiles_of(const Args& a, int block) const { return tiles_of_group(a, block >> a.group_shift); }
+  // the last slot that token t sees (no sum of the two: a length may be the largest number there is)
+  FA_LIST int last_slot(int t) const { return t < end - length ? length + t : end - 1; }
   // groups that have not all tiles, as far as there are blocks
   template <typename Args> FA_LIST int short_groups(const Args& a) const {
     const int n = tiles > filled ? (tiles - filled - 1) >> a.step_shift : 0, all = (blocks + (1 << a.group_shift) - 1) >> a.group_shift;
@@ -63,7 +65,7 @@ template <typename Args> FA_LIST LatentSeq latent_seq_of(const Args& a, int32_t 
   LatentSeq s;
   s.start = start;
   s.tokens = tokens;
-  s.length = length;
+  s.length = length < 0 ? -1 : length;
   const int64_t end = (int64_t)s.length + s.tokens;
   s.end = s.length < 0 ? 0 : (int)(end < room ? end : room);
   s.blocks = (s.tokens * a.hq + a.block_rows - 1) >> a.block_shift;

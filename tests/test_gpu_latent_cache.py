@@ -513,3 +513,27 @@ def test_forks_of_a_latent_cache():
     ops.append(rows[:1].expand(2, -1, -1, -1)[..., :512], rows[:1].expand(2, -1, -1, -1)[..., 512:], k, v, table, n)
     out = ops.latent_attention(q, cache, table, n, ints(0, 1, 2), 512, 0.05)
     assert torch.equal(out[0], out[1])
+
+
+@pytest.mark.parametrize('Hq', [1, 16, 128])
+@pytest.mark.parametrize('E,Ev,room', [(320, 256, 0), (320, 256, 1 << 18), (576, 512, 0), (576, 512, 1 << 18)])
+def test_lengths_at_the_end_of_their_type(E, Ev, room, Hq):
+    """past the table what the table has is seen, by all of a sequence's tokens, however far past it the length is: the results of a length that the
+    table just holds"""
+    lens, counts = [300, 90, 40], [2, 5, 1]
+    cache, table, n, starts = _pool(lens, counts, E, 16, BF, seed=21)
+    cache = torch.where(torch.isfinite(cache), cache, 0.25)
+    narrow, table = table, _wide(table, 16, room)
+    holds = table.shape[1] * 16
+    q = torch.randn(8, Hq, E, generator=torch.Generator().manual_seed(22)).to(BF)
+    n[1] = holds
+    out, lse = _run(q, cache, table, n, starts, Ev, 0.1, 400)
+    _check(q, cache, narrow, torch.clamp(n, max=narrow.shape[1] * 16), starts, Ev, 0.1, out, lse)
+    for far in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 4, 2 ** 31 - 6, 2 ** 30):
+        n[1] = far
+        out2, lse2 = _run(q, cache, table, n, starts, Ev, 0.1, 400)
+        assert torch.equal(out2, out) and torch.equal(lse2, lse), far
+    for none in (-1, -2, -2 ** 31, -2 ** 31 + 3):
+        n[1] = none
+        out2, lse2 = _run(q, cache, table, n, starts, Ev, 0.1, 400)
+        assert (out2[2:7] == 0).all() and torch.isposinf(lse2[2:7]).all()

@@ -18,6 +18,7 @@ extern "C" int64_t units(const Call* c) { return seq(*c).units(c->a); }
 extern "C" int block_of(const Call* c, int64_t rel, int* unit) { return seq(*c).block_of(c->a, rel, *unit); }
 extern "C" int tiles_of(const Call* c, int block) { return seq(*c).tiles_of(c->a, block); }
 extern "C" int blocks(const Call* c) { return seq(*c).blocks; }
+extern "C" int last_slot(const Call* c, int t) { return seq(*c).last_slot(t); }
 '''
 
 
@@ -92,3 +93,13 @@ def test_the_largest_sequences(lib, hq, rows, tokens, length):
         for unit in (0, 1, t // 2, t - 1):
             assert _block(lib, c, first + unit) == (b, unit)
     assert first + t == lib.units(p)
+
+
+@pytest.mark.parametrize('room', [0, 16, 1 << 29])
+@pytest.mark.parametrize('length', [-2 ** 31, -2 ** 31 + 3, -1, 0, 1, 15, 16, 100, (1 << 29) - 2, 1 << 29, 2 ** 31 - 1000, 2 ** 31 - 2, 2 ** 31 - 1])
+def test_the_last_slot_that_a_token_sees(lib, length, room):
+    """no further than the table goes, wherever the length stands; none of a sequence that is not there"""
+    tokens = 1 << 20
+    c = _call(16, 32, 5, tokens, length, room)
+    for t in (0, 1, 2, 3, 14, 15, 16, 999, 1000, tokens - 1):
+        assert lib.last_slot(ctypes.byref(c), t) == (min(length + t, room - 1) if length >= 0 else -1)
