@@ -130,6 +130,13 @@ template <typename T> __device__ __forceinline__ T* row_at(const void* base, con
   return const_cast<T*>(reinterpret_cast<const T*>(base)) + (int64_t)si.batch_index * s.z + (int64_t)h * s.h + row * s.s;
 }
 
+// Number of the slab of a sequence's rows from 32 `block` on.  Packed sequences have theirs one behind the other, each from q_start / 32 + z on: that
+// is past those of the sequence in front, ceil(n / 32) of them, and a head has no more than rows / 32 + sequences.  (As many for every sequence as the
+// longest has would be 850 MB where one of 2048 tokens stands beside 199 of 4 with one head; so they are 19.)
+__device__ __forceinline__ int64_t latent_slab(const LatentArgs& a, const SeqInfo& si, int z, int h, int block) {
+  return ((int64_t)si.batch_index * a.heads + h) * a.slabs + si.q_start / 32 + (a.seq.num_seqlens != 0 ? z : 0) + block;
+}
+
 // ---- forward -------------------------------------------------------------------------------------------------------
 template <typename T, int EC>
 __global__ __launch_bounds__(256, 2) void latent_fwd_kernel(const LatentArgs a, int nseq, int tiles) {
@@ -230,7 +237,7 @@ __global__ __launch_bounds__(256, 2) void latent_fwd_kernel(const LatentArgs a, 
     }
   }
   if (a.parts > 1) {
-    store_part<DB>(a.part_o, a.part_ml, (((int64_t)(z * a.heads + h) * tiles + mt) * 4 + wave) * a.parts + part, o, sm, lane);
+    if (rows > 0) store_part<DB>(a.part_o, a.part_ml, latent_slab(a, si, z, h, mt * 4 + wave) * a.parts + part, o, sm, lane);
     return;
   }
   const float l = cross_sum(sm.l);
@@ -243,13 +250,13 @@ __global__ __launch_bounds__(256, 2) void latent_fwd_kernel(const LatentArgs a, 
 template <typename T, int EC>
 __global__ __launch_bounds__(256) void latent_fwd_sum_kernel(const LatentArgs a, int nseq, int tiles) {
   constexpr int DB = EC / 32;
-  const int db = blockIdx.x % DB, slab = blockIdx.x / DB, wave = slab % 4, mt = slab / 4 % tiles, zh = slab / 4 / tiles;
+  const int db = blockIdx.x % DB, item = blockIdx.x / DB, wave = item % 4, mt = item / 4 % tiles, zh = item / 4 / tiles;
   const int h = zh % a.heads, z = zh / a.heads;
   const SeqInfo si = latent_seq(a, z);
   const int lane = threadIdx.x & 63, hi = lane >> 5, row = mt * 128 + wave * 32 + (lane & 31);
   if (row >= si.seqlen_q) return;
   float lse;
-  const vec<float, 4> x = sum_parts<DB>(a.part_o, a.part_ml, (int64_t)slab * a.parts, a.parts, a.sm_scale, db, threadIdx.x, lse);
+  const vec<float, 4> x = sum_parts<DB>(a.part_o, a.part_ml, latent_slab(a, si, z, h, mt * 4 + wave) * a.parts, a.parts, a.sm_scale, db, threadIdx.x, lse);
   const int col = 32 * db + 8 * (threadIdx.x >> 6) + 4 * hi;
   typename Traits<T>::q4_t y;
 #pragma unroll

@@ -110,7 +110,8 @@ int fa_latent_fwd(const fa_latent_fwd_params* p, void* hip_stream, fa_allocator*
   if ((e = fa_check_gpu(hip_stream)) != FA_SUCCESS) return e;
   const int d = compiled(a), parts = alloc != nullptr ? latent_parts(a, fa_get_multiprocessor_count(hip_stream)) : 1;
   if (parts > 1) {
-    const int64_t slabs = sequences(a) * a.heads * ((a.seq.max_seqlen_q + 127) / 128) * 4 * parts;
+    a.slabs = a.rows_q / 32 + (int32_t)(a.seq.num_seqlens != 0 ? a.seq.num_seqlens : 1);
+    const int64_t slabs = (int64_t)a.batch * a.heads * a.slabs * parts;
     const int64_t o_bytes = slabs * 32 * d * 4;
     void* scratch = alloc->alloc(alloc, (uint64_t)(o_bytes + slabs * 64 * 4));
     if (scratch != nullptr) {

@@ -20,8 +20,9 @@ struct LatentArgs {
   SeqArgs seq;
   int32_t rows_q, rows_k;        // of the tensors: packed offsets are held inside them
   int32_t group;                 // fa_latent.h: latent_item
-  // The keys of a tile cut into `parts` (> 1), for calls with few queries: the parts' sums, laid out as latent_part says.
-  int32_t parts;
+  // The keys of a tile cut into `parts` (> 1), for calls with few queries: the parts' sums, side by side for every slab of 32 rows.  A batch's
+  // head has `slabs` of them (fa_latent.h: latent_slab).
+  int32_t parts, slabs;
   float* part_o; float* part_ml;
 };
 

@@ -436,3 +436,42 @@ def test_rows_that_share_memory_of_many_workgroups(Sq, Sk):
         out, grads = _step(qq, kk, vv, c, dd)
         assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(grads, wgrads))
     _check(q[3], k[3], v[3], c[3], do[3, :, :1].expand(-1, Sq, -1), True, 1 / math.sqrt(96), *(lambda o, g: (o[3], None, [x[3] for x in g]))(*_step(q, k, v, c, one(do))))
+
+
+# ---- packed sequences whose keys are cut into parts -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize('dtype', [HF, BF])
+@pytest.mark.parametrize('E,R,Ev,causal,top', [(128, 64, 128, True, 2100), (64, 32, 64, False, 2100), (40, 8, 24, True, 9000)])
+def test_packed_keys_cut_into_parts(E, R, Ev, causal, top, dtype):
+    """few rows, long and short keys, none; a greatest length beyond them all cuts the keys more finely"""
+    lens_q, lens_k, H, pad = [130, 1, 0, 64, 7, 33], [2100, 1500, 40, 0, 1030, 3], 2, 5
+    tq, tk = sum(lens_q), sum(lens_k)
+    q, _, _, _, do = _inputs(1, H, tq + pad, 1, E, R, Ev, dtype, seed=41)
+    _, k, v, c, _ = _inputs(1, H, 1, tk + pad, E, R, Ev, dtype, seed=42)
+    q[:, :, tq:] = float('nan')
+    k[:, :, tk:] = float('inf')
+    cq, ck = _offsets(lens_q), _offsets(lens_k)
+    scale = 0.1
+    out, lse = torch.ops.aotriton_amd.latent_attention_forward(q, k, v, c, cq, ck, max(lens_q), top, causal, scale)
+    for i in range(len(lens_q)):
+        a, b = slice(int(cq[i]), int(cq[i + 1])), slice(int(ck[i]), int(ck[i + 1]))
+        _check(q[0][:, a], k[0][:, b], v[0][:, b], c[0][b], do[0][:, a], causal, scale, out[0][:, a], lse[:, a], None, f'sequence {i} ')
+    assert (out[:, :, tq:] == 0).all()
+
+
+def test_scratch_of_a_ragged_batch():
+    """one long sequence and many short ones: scratch goes by the rows, a slab of 32 of them and two words a row for every part (16 at most), and no
+    sequence has more than one slab that is not full"""
+    lens, E = [2048] + [4] * 199, 128
+    q, k, v, c, do = _inputs(1, 1, sum(lens), sum(lens), E, 64, E, BF, seed=43)
+    cu = _offsets(lens)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out, lse = torch.ops.aotriton_amd.latent_attention_forward(q, k, v, c, cu, cu, 2048, 2048, True, 0.05)
+    used = torch.cuda.max_memory_allocated() - before
+    slabs = sum(lens) // 32 + len(lens)
+    assert used <= out.numel() * 2 + lse.numel() * 4 + 16 * slabs * (32 * E * 4 + 256) + (8 << 20)
+    for i in (0, 1, 100, 199):
+        a = slice(int(cu[i]), int(cu[i + 1]))
+        _check(q[0][:, a], k[0][:, a], v[0][:, a], c[0][a], do[0][:, a], True, 0.05, out[0][:, a], lse[:, a], None, f'sequence {i} ')
