@@ -132,6 +132,7 @@ SYMBOLS = {
                                             ctypes.c_void_p]),
     'fa_attn_bwd': (ctypes.c_int, [P(fa_bwd_params), ctypes.c_int32, ctypes.c_void_p, P(fa_options)]),
     'fa_zero_tails': (ctypes.c_int, [P(fa_tensor4), P(fa_tensor1), ctypes.c_int32, ctypes.c_void_p]),
+    'fa_zero_gaps': (ctypes.c_int, [P(fa_tensor4), P(fa_tensor1), P(ctypes.c_int32), ctypes.c_int32, ctypes.c_void_p]),
     'fa_attn_fwd_sinks': (ctypes.c_int, [P(fa_fwd_params), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
                                          P(fa_options), ctypes.c_void_p]),
     'fa_attn_bwd_sinks': (ctypes.c_int, [P(fa_bwd_params), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,

@@ -1467,6 +1467,30 @@ SinkBwdRoute sink_bwd_route(const Shape& s, int64_t tokens_q, int64_t tokens_k, 
   return SinkBwdRoute{window > kShortWindow && dq(256, 32, 5, 1.42) < 0.97 * dq(128, 64, 5, 1.7), dkdv(256, 32, 7, 1.8) < dkdv(128, 64, 9, 1.95)};
 }
 
+// the tensors of fa_zero_tails and fa_zero_gaps (`longest`: null for the former), those without rows left out
+int tail_args(const fa_tensor4* tensors, const fa_tensor1* cu_seqlens, const int32_t* longest, int32_t count, fa::TailArgs* out, int* out_count) {
+  if (count < 0 || count > FA_MAX_TAILS || (count > 0 && (tensors == nullptr || cu_seqlens == nullptr))) return FA_ERROR_INVALID_VALUE;
+  fa::TailArgs& a = *out;
+  int& n = *out_count;
+  for (int i = 0; i < count; ++i) {
+    const fa_tensor4& t = tensors[i];
+    const fa_tensor1& c = cu_seqlens[i];
+    if (!is_16bit(t.dtype) || t.sizes[0] != 1 || t.sizes[1] > INT32_MAX || t.sizes[2] > INT32_MAX || c.dtype != FA_DTYPE_INT32 || c.sizes[0] < 1 || c.ptr == nullptr)
+      return FA_ERROR_INVALID_VALUE;
+    if (longest != nullptr && (longest[i] < 0 || c.sizes[0] > INT32_MAX)) return FA_ERROR_INVALID_VALUE;
+    if (t.sizes[1] == 0 || t.sizes[2] == 0) continue;
+    if (t.sizes[3] == 0 || t.sizes[3] % 8 != 0 || t.strides[3] != 1 || (reinterpret_cast<uintptr_t>(t.ptr) & 15) != 0) return FA_ERROR_NOT_SUPPORTED;
+    for (int d = 1; d < 3; ++d)
+      if (t.sizes[d] > 1 && ((int64_t)t.strides[d] <= 0 || t.strides[d] % 8 != 0)) return FA_ERROR_NOT_SUPPORTED;
+    if (c.sizes[0] > 1 && c.strides[0] != 1) return FA_ERROR_NOT_SUPPORTED;
+    if (t.ptr == nullptr) return FA_ERROR_INVALID_VALUE;
+    a.t[n++] = {static_cast<uint16_t*>(t.ptr), static_cast<const int32_t*>(c.ptr) + c.sizes[0] - 1, (int64_t)t.strides[1], (int64_t)t.strides[2],
+                (int32_t)t.sizes[1], (int32_t)t.sizes[2], (int32_t)(t.sizes[3] / 8),
+                longest != nullptr ? (int32_t)c.sizes[0] - 1 : 0, longest != nullptr ? longest[i] : 0};
+  }
+  return FA_SUCCESS;
+}
+
 }  // namespace
 
 int fa_attn_fwd_sinks(const fa_fwd_params* p, int32_t params_version, int32_t window, int32_t sinks, void* hip_stream,
@@ -1598,25 +1622,18 @@ int fa_attn_bwd_sinks(const fa_bwd_params* p, int32_t params_version, int32_t wi
 }
 
 int fa_zero_tails(const fa_tensor4* tensors, const fa_tensor1* cu_seqlens, int32_t count, void* hip_stream) {
-  if (count < 0 || count > FA_MAX_TAILS || (count > 0 && (tensors == nullptr || cu_seqlens == nullptr))) return FA_ERROR_INVALID_VALUE;
   fa::TailArgs a{};
-  int n = 0;
-  for (int i = 0; i < count; ++i) {
-    const fa_tensor4& t = tensors[i];
-    const fa_tensor1& c = cu_seqlens[i];
-    if (!is_16bit(t.dtype) || t.sizes[0] != 1 || t.sizes[1] > INT32_MAX || t.sizes[2] > INT32_MAX || c.dtype != FA_DTYPE_INT32 || c.sizes[0] < 1 || c.ptr == nullptr)
-      return FA_ERROR_INVALID_VALUE;
-    if (t.sizes[1] == 0 || t.sizes[2] == 0) continue;
-    if (t.sizes[3] == 0 || t.sizes[3] % 8 != 0 || t.strides[3] != 1 || (reinterpret_cast<uintptr_t>(t.ptr) & 15) != 0) return FA_ERROR_NOT_SUPPORTED;
-    for (int d = 1; d < 3; ++d)
-      if (t.sizes[d] > 1 && ((int64_t)t.strides[d] <= 0 || t.strides[d] % 8 != 0)) return FA_ERROR_NOT_SUPPORTED;
-    if (c.sizes[0] > 1 && c.strides[0] != 1) return FA_ERROR_NOT_SUPPORTED;
-    if (t.ptr == nullptr) return FA_ERROR_INVALID_VALUE;
-    a.t[n++] = {static_cast<uint16_t*>(t.ptr), static_cast<const int32_t*>(c.ptr) + c.sizes[0] - 1, (int64_t)t.strides[1], (int64_t)t.strides[2],
-                (int32_t)t.sizes[1], (int32_t)t.sizes[2], (int32_t)(t.sizes[3] / 8)};
-  }
-  const int e = fa_check_gpu(hip_stream);
+  int n = 0, e = tail_args(tensors, cu_seqlens, nullptr, count, &a, &n);
+  if (e == FA_SUCCESS) e = fa_check_gpu(hip_stream);
   return e != FA_SUCCESS ? e : (int)fa::run_zero_tails(a, n, static_cast<hipStream_t>(hip_stream));
+}
+
+int fa_zero_gaps(const fa_tensor4* tensors, const fa_tensor1* cu_seqlens, const int32_t* max_seqlens, int32_t count, void* hip_stream) {
+  if (count > 0 && max_seqlens == nullptr) return FA_ERROR_INVALID_VALUE;
+  fa::TailArgs a{};
+  int n = 0, e = tail_args(tensors, cu_seqlens, max_seqlens, count, &a, &n);
+  if (e == FA_SUCCESS) e = fa_check_gpu(hip_stream);
+  return e != FA_SUCCESS ? e : (int)fa::run_zero_gaps(a, n, static_cast<hipStream_t>(hip_stream));
 }
 
 // kernel_slot < 0: the whole backward of the chosen backend; otherwise only that

@@ -243,6 +243,7 @@ struct TailArgs {
     const int32_t* end;
     int64_t head, row;      // strides
     int32_t heads, tokens, pieces;
+    int32_t sequences, longest;      // of the gaps: offsets in front of `end`, rows that a sequence has at most
   } t[4];
 };
 

@@ -101,7 +101,8 @@ template <int EC> struct LatentSmem {
   static constexpr int WAVE = STAGE / 2, WAVE_V = 32 * EC * 2, WAVE_C = 2 * WAVE_V;
 };
 
-// (the offsets of packed sequences are held inside the tensors, and lengths inside the greatest: what lies past them is not there)
+// (The offsets of packed sequences are held inside the tensors, and lengths inside the greatest: what lies past them is not there, and no kernel reads or
+// writes it.)
 __device__ __forceinline__ SeqInfo latent_seq(const LatentArgs& a, int z) {
   SeqInfo r{a.seq.max_seqlen_q, a.seq.max_seqlen_k, 0, 0, z, a.rows_q};
   if (a.seq.num_seqlens != 0) {

@@ -453,13 +453,26 @@ __global__ __launch_bounds__(256, 1) void latent_dq_alone_kernel(const LatentBwd
   store_rows<T, RB>(dq + DB, a.sm_scale, to + a.e, a.sdq.s, rows, a.r, lane, own + kRowsOut<T, DB>);
 }
 
-// dC: the heads' parts added in their order, four columns a lane
+// Whether a sequence has row n of packed keys, as latent_seq holds them: the last one that starts no later, if it goes so far.
+__device__ __forceinline__ bool latent_has_key(const LatentArgs& a, int n) {
+  auto hold = [&](int x) { return x < 0 ? 0 : x < a.rows_k ? x : a.rows_k; };
+  int z = 0;
+  for (int left = a.seq.num_seqlens; left > 1;) {
+    const int half = left / 2;
+    if (hold(a.seq.cu_k[z + half]) <= n) z += half;
+    left -= half;
+  }
+  const int start = hold(a.seq.cu_k[z]), end = hold(a.seq.cu_k[z + 1]);
+  return n >= start && n < end && n - start < a.seq.max_seqlen_k;
+}
+
+// dC: the heads' parts added in their order, four columns a lane; packed rows of no sequence, which have no parts, stay as they are
 template <typename T>
-__global__ __launch_bounds__(256) void latent_dc_kernel(const LatentBwdArgs a, int64_t keys, const int32_t* end) {
+__global__ __launch_bounds__(256) void latent_dc_kernel(const LatentBwdArgs a, int64_t keys) {
   const int64_t at = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
   const int64_t b = at / keys, n = at % keys;
   const int col = threadIdx.x % 16 * 4;
-  if (b >= a.batch || (end != nullptr && n >= *end) || col >= a.r) return;
+  if (b >= a.batch || col >= a.r || (a.seq.num_seqlens != 0 && !latent_has_key(a, (int)n))) return;
   const float* from = a.part_c + (b * a.heads * a.part_rows + n) * kLatentShared + col;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   for (int h = 0; h < a.heads; ++h) sum += *reinterpret_cast<const f32x4*>(from + (int64_t)h * a.part_rows * kLatentShared);
@@ -479,8 +492,7 @@ template <typename T, int EC> hipError_t launch_latent_keys(const LatentBwdArgs&
   if (e != hipSuccess) return e;
   if (a.heads > 0)
     hipLaunchKernelGGL((latent_dkdv_kernel<T, EC>), dim3((unsigned)(nseq * a.heads * tiles)), dim3(256), LatentSmem<EC>::BWD_BYTES, s, a, nseq, tiles);
-  const int32_t* end = a.seq.num_seqlens != 0 ? a.seq.cu_k + nseq : nullptr;
-  hipLaunchKernelGGL((latent_dc_kernel<T>), dim3((unsigned)((a.batch * a.part_rows + 15) / 16)), dim3(256), 0, s, a, a.part_rows, end);
+  hipLaunchKernelGGL((latent_dc_kernel<T>), dim3((unsigned)((a.batch * a.part_rows + 15) / 16)), dim3(256), 0, s, a, a.part_rows);
   return hipGetLastError();
 }
 

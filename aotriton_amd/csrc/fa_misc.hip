@@ -112,6 +112,45 @@ hipError_t run_zero_tails(const TailArgs& a, int count, hipStream_t s) {
   return hipGetLastError();
 }
 
+// fa_zero_gaps: a column of workgroups per tensor, all of them for the rows at both ends; a wave looks at 64 sequences and clears what it finds.  (No
+// more than the tails take where there is nothing between: 4.7 us for the four gradients of 12 sequences.)
+__global__ __launch_bounds__(256) void zero_gaps_kernel(const TailArgs a) {
+  const TailArgs::Tensor& t = a.t[blockIdx.y];
+  const int32_t* offsets = t.end - t.sequences;
+  auto hold = [&](int x) { return x < 0 ? 0 : x < t.tokens ? x : t.tokens; };
+  auto clear = [&](int64_t i, int64_t rows, int64_t row) {
+    const int64_t piece = i % t.pieces, head = i / t.pieces / rows;
+    *reinterpret_cast<u32x4_t*>(t.ptr + head * t.head + row * t.row + piece * 8) = u32x4_t{0, 0, 0, 0};
+  };
+  const int first = hold(offsets[0]), last = hold(*t.end), tail = last > first ? last : first;
+  const int64_t ends = first + (t.tokens - tail);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < ends * t.heads * t.pieces; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / t.pieces % ends;
+    clear(i, ends, row < first ? row : tail + row - first);
+  }
+  const int lane = threadIdx.x & 63, wave = blockIdx.x * 4 + (threadIdx.x >> 6);
+  for (int64_t z0 = (int64_t)wave * 64; z0 < t.sequences; z0 += (int64_t)gridDim.x * 256) {
+    int from = 0, to = 0;
+    if (z0 + lane < t.sequences) {
+      from = hold(offsets[z0 + lane]);
+      to = hold(offsets[z0 + lane + 1]);
+      if (to - from > t.longest) from += t.longest;
+      else from = to;
+    }
+    for (uint64_t left = __builtin_amdgcn_ballot_w64(from < to); left != 0; left &= left - 1) {
+      const int which = __builtin_ctzll(left), r0 = __shfl(from, which);
+      const int64_t rows = __shfl(to, which) - r0;
+      for (int64_t i = lane; i < rows * t.heads * t.pieces; i += 64) clear(i, rows, r0 + i / t.pieces % rows);
+    }
+  }
+}
+
+hipError_t run_zero_gaps(const TailArgs& a, int count, hipStream_t s) {
+  if (count == 0) return hipSuccess;
+  hipLaunchKernelGGL(zero_gaps_kernel, dim3(64, count), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
 // A few words of the host (Philox seeds, the offsets of packed sequences) to device memory: they
 // travel in the kernel's argument block, so nothing is pinned, copied through a staging buffer or
 // waited for (a copy from pageable memory takes 20-30 us and synchronises).

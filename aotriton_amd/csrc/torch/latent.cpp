@@ -83,7 +83,7 @@ std::tuple<Tensor, Tensor> forward_kernel(const Tensor& q, const Tensor& k, cons
   TORCH_CHECK(view4(out, &in.p.Out) && view2(lse, &in.p.L), "outputs");
   Scratch scratch;
   check_rc(fa_latent_fwd(&in.p, current_stream(), &scratch.c), false);
-  if (in.packed) check_rc(fa_zero_tails(&in.p.Out, &in.p.cu_seqlens_q, 1, current_stream()), false);
+  if (in.packed) check_rc(fa_zero_gaps(&in.p.Out, &in.p.cu_seqlens_q, &in.p.max_seqlen_q, 1, current_stream()), false);
   return {out, lse};
 }
 
@@ -107,7 +107,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> backward_kernel(const Tensor& dout_in
   if (in.packed) {
     const fa_tensor4 grads[4] = {p.DQ, p.DK, p.DV, p.DS};
     const fa_tensor1 ends[4] = {p.fwd.cu_seqlens_q, p.fwd.cu_seqlens_k, p.fwd.cu_seqlens_k, p.fwd.cu_seqlens_k};
-    check_rc(fa_zero_tails(grads, ends, 4, current_stream()), false);
+    const int32_t longest[4] = {p.fwd.max_seqlen_q, p.fwd.max_seqlen_k, p.fwd.max_seqlen_k, p.fwd.max_seqlen_k};
+    check_rc(fa_zero_gaps(grads, ends, longest, 4, current_stream()), false);
   }
   return {dq, dk, dv, ds};
 }

@@ -159,8 +159,9 @@ def latent_attention(query, key, value, shared_key, is_causal=True, scale=None, 
     have to be finite all the same where they belong to its sequence.
 
     Packed sequences: (1, H, tokens, ...) tensors with the sequences' offsets in cu_seqlens_q / cu_seqlens_k (int32 tensors on the device,
-    sequences + 1 values) and their greatest lengths in max_seqlen_q / max_seqlen_k; tokens behind the last offset belong to no sequence:
-    their rows of the result and of the gradients are 0, and may hold anything.
+    sequences + 1 values, ascending) and their greatest lengths in max_seqlen_q / max_seqlen_k, which a longer one is cut to.  Tokens in front of the
+    first offset, past the greatest length and behind the last offset belong to no sequence: their rows of the result and of the gradients are 0,
+    and may hold anything.
 
     Works under HIP graph capture and torch.compile; results do not change from call to call.  There is no dropout and no bias.  The same
     attention of new tokens over a cache of the latent vectors: aotriton_amd.cache.latent_attention.

@@ -298,6 +298,9 @@ FA_API int fa_attn_bwd_sinks(const fa_bwd_params* params, int32_t params_version
  * hands out new tensors clears them here, without reading the offset back. */
 #define FA_MAX_TAILS 4
 FA_API int fa_zero_tails(const fa_tensor4* tensors, const fa_tensor1* cu_seqlens, int32_t count, void* hip_stream);
+/* The same for every row that no sequence has where sequences are held to a greatest length (latent.h): also those in front of the first offset, and
+ * those of a sequence past its first max_seqlens[i] rows (host values, one for each tensor).  Offsets ascend. */
+FA_API int fa_zero_gaps(const fa_tensor4* tensors, const fa_tensor1* cu_seqlens, const int32_t* max_seqlens, int32_t count, void* hip_stream);
 
 /* The positional v2 API: v2::flash::attn_fwd, attn_fwd_compact_varlen, attn_bwd, attn_bwd_fused,
  * attn_bwd_compact_varlen.  These are not in the reference tree (0.14 keeps only the v3 params

@@ -22,9 +22,9 @@ extern "C" {
 /* The expanded form.  Head h scores query i against key j with
  *   Sm_scale (Q[h, i, :E] . K[h, j] + Q[h, i, E:] . S[j]);
  * with `causal` query i sees keys up to i + Sk - Sq, without it all.  E and Ev up to 128, R up to 64.  A query that sees no key gives 0 and
- * a logsumexp of +inf, and has no gradient.  Packed sequences: batch 1, offsets in cu_seqlens_q and cu_seqlens_k (int32, sequences + 1 values on
- * the device), greatest lengths in max_seqlen_q and max_seqlen_k; rows behind the last sequence are neither read nor written
- * (fa_zero_tails). */
+ * a logsumexp of +inf, and has no gradient.  Packed sequences: batch 1, ascending offsets in cu_seqlens_q and cu_seqlens_k (int32, sequences + 1
+ * values on the device), held inside the tensors, and greatest lengths in max_seqlen_q and max_seqlen_k, which a longer sequence is cut to.  Rows that no
+ * sequence has (in front of the first offset, past the greatest length, behind the last offset) are neither read nor written (fa_zero_gaps). */
 typedef struct fa_latent_fwd_params {
   fa_tensor4 Q;              /* (batch, heads, Sq, E + R) */
   fa_tensor4 K;              /* (batch, heads, Sk, E) */

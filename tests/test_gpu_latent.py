@@ -475,3 +475,86 @@ def test_scratch_of_a_ragged_batch():
     for i in (0, 1, 100, 199):
         a = slice(int(cu[i]), int(cu[i + 1]))
         _check(q[0][:, a], k[0][:, a], v[0][:, a], c[0][a], do[0][:, a], True, 0.05, out[0][:, a], lse[:, a], None, f'sequence {i} ')
+
+
+# ---- rows of no sequence ------------------------------------------------------------------------------------------------------
+
+def _poison():
+    """memory that the next calls are given holds NaN"""
+    made = [torch.full((n,), float('nan'), device=DEV) for n in (1 << 12, 1 << 16, 1 << 18, 1 << 20, 1 << 22) for _ in range(6)]
+    torch.cuda.synchronize()
+    del made
+
+
+@pytest.mark.parametrize('dtype', [HF, BF])
+@pytest.mark.parametrize('H', [3, 80])
+@pytest.mark.parametrize('causal', [True, False])
+def test_rows_in_front_and_past_the_greatest_length(causal, H, dtype):
+    """offsets that do not begin at 0, sequences longer than the greatest length: what no sequence has is not there, may hold anything, and gets zeros"""
+    cu_q, cu_k, top_q, top_k, E, R, Ev = [5, 60, 60, 200, 203], [9, 80, 100, 250, 251], 100, 120, 64, 32, 64
+    q, _, _, _, do = _inputs(1, H, 230, 1, E, R, Ev, dtype, seed=51)
+    _, k, v, c, _ = _inputs(1, H, 1, 260, E, R, Ev, dtype, seed=52)
+    has = lambda cu, top: [slice(cu[i], cu[i] + min(cu[i + 1] - cu[i], top)) for i in range(len(cu) - 1)]
+    rows_q, rows_k = has(cu_q, top_q), has(cu_k, top_k)
+    off = lambda n, rows: torch.tensor([not any(r.start <= i < r.stop for r in rows) for i in range(n)], device=DEV)
+    off_q, off_k = off(230, rows_q), off(260, rows_k)
+    for t in (q, do):
+        t[:, :, off_q] = float('nan')
+    for t in (k, v):
+        t[:, :, off_k] = float('inf')
+    c[:, off_k] = float('nan')
+    cu = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    _poison()
+    out, grads = _step(q, k, v, c, do, causal, cu_seqlens_q=cu(cu_q), cu_seqlens_k=cu(cu_k), max_seqlen_q=top_q, max_seqlen_k=top_k)
+    for i, (a, b) in enumerate(zip(rows_q, rows_k)):
+        _check(q[0][:, a], k[0][:, b], v[0][:, b], c[0][b], do[0][:, a], causal, 1 / math.sqrt(E + R), out[0][:, a], None,
+               [grads[0][0][:, a], grads[1][0][:, b], grads[2][0][:, b], grads[3][0][b]], f'sequence {i} ')
+    assert (out[:, :, off_q] == 0).all() and (grads[0][:, :, off_q] == 0).all()
+    assert all((g[:, :, off_k] == 0).all() for g in grads[1:3]) and (grads[3][:, off_k] == 0).all()
+
+
+@pytest.mark.parametrize('top_q,top_k', [(0, 0), (0, 9), (9, 0)])
+def test_greatest_lengths_of_nothing(top_q, top_k):
+    q, k, v, c, do = _inputs(1, 2, 40, 50, 64, 32, 64, BF, seed=53)
+    cu = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    _poison()
+    out, grads = _step(q, k, v, c, do, cu_seqlens_q=cu(0, 30, 40), cu_seqlens_k=cu(0, 20, 50), max_seqlen_q=top_q, max_seqlen_k=top_k)
+    assert all((t == 0).all() for t in (out, *grads))
+
+
+def test_offsets_that_end_outside_or_descend():
+    """in front of the tensors, behind them, falling: inside the tensors whatever comes of it, and rows that a sequence has are right"""
+    q, k, v, c, do = _inputs(1, 2, 200, 200, 64, 32, 64, BF, seed=54)
+    cu = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    want, wgrads = _step(q, k, v, c, do, cu_seqlens_q=cu(0, 90, 200), cu_seqlens_k=cu(0, 90, 200), max_seqlen_q=110, max_seqlen_k=110)
+    out, grads = _step(q, k, v, c, do, cu_seqlens_q=cu(-5, 90, 10 ** 9), cu_seqlens_k=cu(-9, 90, 2 ** 31 - 1), max_seqlen_q=110, max_seqlen_k=110)
+    assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(grads, wgrads))
+    out, grads = _step(q, k, v, c, do, cu_seqlens_q=cu(300, 250), cu_seqlens_k=cu(300, 250), max_seqlen_q=110, max_seqlen_k=110)
+    assert all((t == 0).all() for t in (out, *grads))
+    for odd in (cu(150, 90, 200), cu(10 ** 9, -5, 2 ** 31 - 1, -2 ** 31)):
+        _step(q, k, v, c, do, cu_seqlens_q=odd, cu_seqlens_k=odd, max_seqlen_q=110, max_seqlen_k=110)
+
+
+def test_captured_rows_of_no_sequence():
+    """offsets that change between the replays of a graph"""
+    cu = torch.tensor([0, 60, 200], dtype=torch.int32, device=DEV)
+    x = _inputs(1, 3, 230, 230, 64, 32, 64, HF, seed=55)
+    kw = dict(cu_seqlens_q=cu, cu_seqlens_k=cu, max_seqlen_q=100, max_seqlen_k=100)
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        _step(*x, **kw)
+    torch.cuda.current_stream().wait_stream(warm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, grads = _step(*x, **kw)
+    for offsets in ([0, 60, 200], [7, 60, 90], [0, 0, 230], [100, 230, 230], [0, 60, 200]):
+        cu.copy_(torch.tensor(offsets, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _step(*x, **kw)
+        assert torch.equal(out, want[0]) and all(torch.equal(a, b) for a, b in zip(grads, want[1]))
+        covered = torch.zeros(230, dtype=torch.bool, device=DEV)
+        for a, b in zip(offsets, offsets[1:]):
+            covered[a:min(b, a + 100)] = True
+        assert (out[:, :, ~covered] == 0).all() and all((g[:, :, ~covered] == 0).all() for g in grads[:3]) and (grads[3][:, ~covered] == 0).all()

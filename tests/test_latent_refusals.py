@@ -216,6 +216,25 @@ def test_host_checks_of_the_ops():
     cache.append_packed(meta(7, 1, 576), None, meta(9, 1, 16, 576), None, meta(7, dtype=torch.int64))
 
 
+def test_gap_refusals():
+    """what fa_zero_gaps takes: as fa_zero_tails, and a greatest length for every tensor"""
+    L = _lib()
+
+    def run(count=2, sizes=(1, 4, 100, 64), dtype=torch.bfloat16, ptr=4096, strides=None, n=4, cu=torch.int32, cu_ptr=4096, longest=(50, 0)):
+        t, c = (L.fa_tensor4 * 2)(), (L.fa_tensor1 * 2)()
+        for i in range(2):
+            _fill(t[i], sizes, dtype, ptr, strides)
+            _fill(c[i], (n,), cu, cu_ptr)
+        return L.lib.fa_zero_gaps(t, c, longest and (ctypes.c_int32 * 2)(*longest), count, None)
+    assert run() in ACCEPTED and run(count=0) in ACCEPTED and run(sizes=(1, 4, 0, 64), ptr=0) in ACCEPTED and run(n=1) in ACCEPTED and run(count=0, longest=None) in ACCEPTED
+    for bad in (dict(count=5), dict(count=-1), dict(sizes=(2, 4, 100, 64)), dict(dtype=torch.float32), dict(ptr=0), dict(cu=torch.int64), dict(cu_ptr=0), dict(n=0), dict(n=2 ** 31),
+                dict(longest=None), dict(longest=(5, -1))):
+        assert run(**bad) == INVALID
+    for bad in (dict(sizes=(1, 4, 100, 60)), dict(ptr=4104), dict(strides=(1, 6400, 0, 1)), dict(strides=(1, 6404, 64, 1)), dict(strides=(1, 6400, 64, 2))):
+        assert run(**bad) == NOT_SUPPORTED
+    assert L.lib.fa_zero_gaps(None, None, None, 1, None) == INVALID
+
+
 def test_writes_to_a_cache_have_no_gradient():
     from aotriton_amd import cache
     x = lambda grad=False: torch.zeros(3, 2, 16, 64, requires_grad=grad)
