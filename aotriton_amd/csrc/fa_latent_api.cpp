@@ -211,7 +211,8 @@ int fa_latent_cache_attn(const fa_latent_cache_params* p, void* hip_stream, fa_a
   // Rows of a workgroup.  32 where a sequence has no more on average, or where blocks of 128, which take longer to begin and to end, would leave a CU
   // a few tiles of 32 slots.  64 sequences of 4096 slots, 576 columns: 32 heads 90 us with blocks of 32 and of 128, 40 heads 124 and 94, 128 heads 211
   // and 114; 16 sequences (8 tiles a CU) with 64 heads 45 and 43; 8 sequences (4 tiles) 32 and 35, with 128 heads 44 and 46; 2 sequences 25 and 29.
-  // 64 rows only up to 256 columns of values (64 sequences, 64 heads, 320 columns: 75, 58, 59 us for 32, 64, 128 rows); above they took 111.
+  // 64 rows only up to 256 columns of values (64 sequences, 64 heads, 320 columns: 75, 58, 59 us for 32, 64, 128 rows); above, 40 heads took 111 with them.
+  // (Sequences without a new token count, too: 64 with 128 heads take 111 us in a table of 64 rows, 204 to 215 in one of 256.)
   const int64_t mean = n > 0 ? (int64_t)(rows * hq / n) : 0;
   const int64_t room = (int64_t)c.columns << c.page_shift;
   const int64_t most = std::max<int64_t>(1, (int64_t)rows - (int64_t)n + 1);      // new tokens of a sequence, if all have some

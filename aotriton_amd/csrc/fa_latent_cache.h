@@ -12,7 +12,7 @@
 // Work is a list of blocks of rows times tiles of slots, cut into one piece for a CU wherever the cut falls; the sums of a block that lies in
 // several pieces are put together by a launch of its own (with one workgroup for a sequence, 64 sequences with 128 heads would take four times
 // as long).  576 columns, values of 512: a tile of 128 rows takes 3600 cycles, 2180 of them MFMAs (the products alone 2700, with the
-// exponentials 3100); 64 sequences with 128 heads 84 us, of which 68 here and 16 for the pieces (86 MiB of fp32 sums, written and read); 16 heads
+// exponentials 3100); 64 sequences with 128 heads 78 to 84 us, of which 63 to 68 here and 16 for the pieces (86 MiB of fp32 sums, written and read); 16 heads
 // over up to 16384 slots 79 us, 4.2 TB/s.
 #pragma once
 #include "fa_cache.h"
